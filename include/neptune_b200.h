@@ -287,6 +287,92 @@ int nb200_attention(const void* q, const void* k, const void* v, void* o, float*
                     int64_t batch, int64_t heads, int64_t seq, int64_t head_dim,
                     int causal, float scale, void* stream);
 
+/* The same attention with shared key/value heads, strided tensors and per-batch lengths, and its
+ * backward pass. q, o are [batch, heads, seq, head_dim], k, v [batch, kv_heads, seq, head_dim] with
+ * heads a multiple of kv_heads (query head h reads key/value head h / (heads / kv_heads)); the last
+ * dimension is contiguous, the others have element strides. Every base is 16-byte aligned and every
+ * stride of a dimension longer than one is a positive multiple of 8 elements (else NB200_ERR_ARG).
+ * seq_lens (nullable, device memory): tokens of each batch element, read as clamped to [0, seq];
+ * queries and keys at or past it are masked whatever they hold: their rows of o and of the gradients
+ * are zero, their lse is -inf. lse is contiguous [batch, heads, seq]. head_dim must be 128. */
+typedef struct {
+    int64_t batch, heads, kv_heads, seq, head_dim;
+    const int32_t* seq_lens;
+    int32_t causal;
+    float scale;
+} nb200_attn_args;
+typedef struct {
+    int64_t batch, head, seq; /* elements */
+} nb200_attn_strides;
+
+/* strides: of q, k, v, o. lse nullable. */
+int nb200_attention_fwd(const nb200_attn_args* args, const nb200_attn_strides* strides,
+                        const void* q, const void* k, const void* v, void* o, float* lse, void* stream);
+
+/* Gradients of the forward pass's o with respect to q, k, v, given o, lse and grad_o: with
+ * P = exp(scale q k^T - lse) recomputed, dv = P^T grad_o, dS = P * (grad_o v^T - rowsum(grad_o * o)),
+ * dq = scale dS k, dk = scale dS^T q; dk and dv of a shared head sum over its query heads. P and dS
+ * are rounded to bf16 for the products, whose sums are fp32. The result does not depend on
+ * scheduling. strides: of q, k, v, o, grad_o, dq, dk, dv. work: device memory, 16-byte aligned, of
+ * nb200_attention_bwd_work_bytes(args) bytes. */
+int64_t nb200_attention_bwd_work_bytes(const nb200_attn_args* args);
+int nb200_attention_bwd(const nb200_attn_args* args, const nb200_attn_strides* strides,
+                        const void* q, const void* k, const void* v, const void* o, const float* lse,
+                        const void* grad_o, void* dq, void* dk, void* dv, void* work, int64_t work_bytes,
+                        void* stream);
+
+/* ------------------------------------------------------------------ norms around a block
+ * y = residual + scale a(gate) z with z = post_weight * x rsqrt(mean x^2 + eps) (z = x without a
+ * post weight), and h = pre_weight * y rsqrt(mean y^2 + eps) (not computed without a pre weight).
+ * x and residual are [rows, width] with unit column stride; gate (nullable) holds one row per
+ * rows_per_gate consecutive rows; weights are contiguous [width]; everything is of one dtype. y, h and
+ * every gradient are contiguous. All of it is computed in fp32 and rounded once, h from the
+ * unrounded y. rstd is fp32 [rows, 2]: the two reciprocal norms (1 where a weight is absent).
+ * width <= 16384 (else NB200_ERR_CAPACITY); rows a multiple of rows_per_gate. No counterpart in the
+ * reference, whose RMSNorm is forward only (neptune_codegen/emitters.py:549-627). */
+typedef enum { NB200_GATE_NONE = 0, NB200_GATE_TANH = 1, NB200_GATE_SIGMOID = 2 } nb200_gate_act;
+typedef struct {
+    const void *x, *residual, *gate, *post_weight, *pre_weight;
+    int64_t rows, width;
+    int64_t stride_x, stride_residual, stride_gate;     /* elements between rows */
+    int64_t stride_grad_y, stride_grad_h;               /* of the backward pass's inputs */
+    int64_t rows_per_gate;
+    int32_t gate_act;
+    double scale, eps;
+} nb200_norm_args;
+int nb200_gated_norm(const nb200_norm_args* args, int dtype, void* y, void* h, float* rstd, void* stream);
+
+/* Gradients given rstd of the forward pass, grad_y and grad_h (each nullable: zero). dx and dresidual
+ * are required; dgate (one row per gate row), dpost and dpre are nullable. work: device memory,
+ * 16-byte aligned, of nb200_gated_norm_bwd_work_bytes(args) bytes: fp32 column sums per chunk of
+ * rows, added in a fixed order. */
+int64_t nb200_gated_norm_bwd_work_bytes(const nb200_norm_args* args);
+int nb200_gated_norm_bwd(const nb200_norm_args* args, int dtype, const float* rstd, const void* grad_y,
+                         const void* grad_h, void* dx, void* dresidual, void* dgate, void* dpost, void* dpre,
+                         void* work, int64_t work_bytes, void* stream);
+
+/* ------------------------------------------------------------------ distillation loss
+ * Per row: p_j = exp(teacher_j / T - Z) over the kept entries, Z = logsumexp of their teacher_j / T
+ * (teacher_lse null) or teacher_lse[row]; q = softmax(x / T); loss = sum_j p_j (log p_j - log q at
+ * index_j); stats = {logsumexp(x / T), Z, sum_j p_j}. An index outside [0, vocab) marks an entry
+ * that is not kept; a row without kept entries has loss 0 and gradient 0. x is [rows, vocab] and
+ * teacher, index [rows, top], unit column stride; top <= 256 (else NB200_ERR_CAPACITY). loss and
+ * teacher_lse are fp32 [rows], stats fp32 [rows, 3], contiguous. Built on the reference's logsumexp
+ * skeleton (neptune_codegen/library.py:19); the reference has no loss and no gradient. */
+typedef struct {
+    const void *x, *teacher, *index;
+    int64_t rows, vocab, top;
+    int64_t stride_x, stride_teacher, stride_index;     /* elements between rows */
+    int32_t dtype, teacher_dtype, index_dtype;
+    double temperature;
+} nb200_distill_args;
+int nb200_distill_loss(const nb200_distill_args* args, const float* teacher_lse, float* loss, float* stats,
+                       void* stream);
+
+/* dx[r, c] = grad[r * stride_grad] / T * (stats mass * q_c - sum of p_j with index_j == c), contiguous, in x's dtype. */
+int nb200_distill_loss_bwd(const nb200_distill_args* args, const float* grad, int64_t stride_grad,
+                           const float* stats, void* dx, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

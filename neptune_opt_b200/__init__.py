@@ -11,12 +11,20 @@ include/neptune_b200.h; there is no Triton and no CPU fallback.
 Explicit operator library (as neptune_opt's one-function-per-skeleton surface): `logsumexp(x)`,
 `stable_l2(x)`, ... plus the fused readouts `softmax(x)`, `log_softmax(x)`, `l2_normalize(x)`,
 `rms_norm(x, gamma, eps)`, `segment_sum/segment_mean(data, segments, ...)` and `attention(q, k, v)`.
+
+Training operators, differentiable through autograd and as explicit forward/backward calls:
+`attention(q, k, v, seq_lens=...)` / `attention_backward`, `gated_residual_norm(x, residual, gate,
+...)` / `gated_residual_norm_backward` (the norms around a block with its gate and residual scale)
+and `distill_loss(logits, teacher_logits, teacher_index, ...)` / `distill_loss_backward`.
 """
 from __future__ import annotations
 
 from neptune_opt_b200 import autotune  # noqa: F401
 from neptune_opt_b200._lib import BackendUnavailable, LIB_PATH, launch_count, load  # noqa: F401
-from neptune_opt_b200.attention import attention_op, run_attention  # noqa: F401
+from neptune_opt_b200.attention import attention_backward, attention_op, run_attention  # noqa: F401
+from neptune_opt_b200.block_norm import (gated_residual_norm, gated_residual_norm_backward,  # noqa: F401
+                                         run_gated_residual_norm)
+from neptune_opt_b200.distill import distill_loss, distill_loss_backward, run_distill_loss  # noqa: F401
 from neptune_opt_b200.skeletons import (SKELETONS, all_registered, op_parameters, param_defaults,  # noqa: F401
                                         supported)
 from neptune_opt_b200.template import (MAX_SPLIT_PARTS, launch_reduction, run, run_l2_normalize,  # noqa: F401
@@ -67,9 +75,11 @@ def rms_norm(x, gamma, eps: float = 1e-6, plan: str = "serial"):
     return run_rms_norm(x, gamma, eps=eps, plan=plan)
 
 
-def attention(q, k, v, *, causal: bool = False, scale=None, return_lse: bool = False):
-    """softmax(scale * q k^T [+ causal mask]) v over bf16 [batch, heads, seq, 128] tensors."""
-    return run_attention(q, k, v, causal=causal, scale=scale, return_lse=return_lse)
+def attention(q, k, v, *, causal: bool = False, scale=None, return_lse: bool = False, seq_lens=None):
+    """softmax(scale * q k^T [+ masks]) v over bf16 [batch, heads, seq, 128] tensors; k and v may have
+    fewer heads (shared by consecutive query heads), seq_lens [batch] int32 masks each sequence's tail.
+    Differentiable in q, k and v."""
+    return run_attention(q, k, v, causal=causal, scale=scale, return_lse=return_lse, seq_lens=seq_lens)
 
 
 def segment_sum(data, segments, *, offsets=False, initial=None, unsafe=False):
@@ -82,7 +92,8 @@ def segment_mean(data, segments, *, offsets=False, initial=None, unsafe=False):
 
 __all__ = [
     "MAX_SPLIT_PARTS", "SKELETONS", "BackendUnavailable", "all_registered", "as_cuda_op", "as_segment_op",
-    "attention", "attention_op", "run_attention",
+    "attention", "attention_backward", "attention_op", "run_attention", "distill_loss", "distill_loss_backward",
+    "run_distill_loss", "gated_residual_norm", "gated_residual_norm_backward", "run_gated_residual_norm",
     "as_state_op", "as_triton_op", "autotune", "check_segment_status", "cuda_op_name", "l2_normalize",
     "launch_count", "log_softmax", "op_handle", "op_parameters", "param_defaults", "rms_norm", "run",
     "run_l2_normalize", "run_rms_norm", "run_rms_norm_host", "run_segment_pool", "run_softmax", "run_softmax_lse",

@@ -41,10 +41,39 @@ class NB200State(ctypes.Structure):
                 ("status", ctypes.c_int32)]
 
 
+class NB200AttnArgs(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_int64), ("heads", ctypes.c_int64), ("kv_heads", ctypes.c_int64),
+                ("seq", ctypes.c_int64), ("head_dim", ctypes.c_int64), ("seq_lens", ctypes.c_void_p),
+                ("causal", ctypes.c_int32), ("scale", ctypes.c_float)]
+
+
+class NB200AttnStrides(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_int64), ("head", ctypes.c_int64), ("seq", ctypes.c_int64)]
+
+
+class NB200NormArgs(ctypes.Structure):
+    _fields_ = [("x", ctypes.c_void_p), ("residual", ctypes.c_void_p), ("gate", ctypes.c_void_p),
+                ("post_weight", ctypes.c_void_p), ("pre_weight", ctypes.c_void_p), ("rows", ctypes.c_int64),
+                ("width", ctypes.c_int64), ("stride_x", ctypes.c_int64), ("stride_residual", ctypes.c_int64),
+                ("stride_gate", ctypes.c_int64), ("stride_grad_y", ctypes.c_int64),
+                ("stride_grad_h", ctypes.c_int64), ("rows_per_gate", ctypes.c_int64),
+                ("gate_act", ctypes.c_int32), ("scale", ctypes.c_double), ("eps", ctypes.c_double)]
+
+
+class NB200DistillArgs(ctypes.Structure):
+    _fields_ = [("x", ctypes.c_void_p), ("teacher", ctypes.c_void_p), ("index", ctypes.c_void_p),
+                ("rows", ctypes.c_int64), ("vocab", ctypes.c_int64), ("top", ctypes.c_int64),
+                ("stride_x", ctypes.c_int64), ("stride_teacher", ctypes.c_int64), ("stride_index", ctypes.c_int64),
+                ("dtype", ctypes.c_int32), ("teacher_dtype", ctypes.c_int32), ("index_dtype", ctypes.c_int32),
+                ("temperature", ctypes.c_double)]
+
+
 STATE_BYTES = ctypes.sizeof(NB200State)
 
 # Every symbol include/neptune_b200.h declares, with (restype, argtypes).
 _vp, _i64, _int, _dbl = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_double
+_attn, _strides = ctypes.POINTER(NB200AttnArgs), ctypes.POINTER(NB200AttnStrides)
+_norm, _distill = ctypes.POINTER(NB200NormArgs), ctypes.POINTER(NB200DistillArgs)
 SIGNATURES = {
     "nb200_last_error": (ctypes.c_char_p, []),
     "nb200_version": (ctypes.c_char_p, []),
@@ -79,6 +108,14 @@ SIGNATURES = {
     "nb200_segment_pool": (_int, [_vp, _int, _i64, _i64, _i64, _i64, _vp, _int, _i64, _i64, _int, _int,
                                   ctypes.c_uint32, _vp, _vp, _vp]),
     "nb200_attention": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _int, ctypes.c_float, _vp]),
+    "nb200_attention_fwd": (_int, [_attn, _strides, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "nb200_attention_bwd_work_bytes": (_i64, [_attn]),
+    "nb200_attention_bwd": (_int, [_attn, _strides, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "nb200_gated_norm": (_int, [_norm, _int, _vp, _vp, _vp, _vp]),
+    "nb200_gated_norm_bwd_work_bytes": (_i64, [_norm]),
+    "nb200_gated_norm_bwd": (_int, [_norm, _int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "nb200_distill_loss": (_int, [_distill, _vp, _vp, _vp, _vp]),
+    "nb200_distill_loss_bwd": (_int, [_distill, _vp, _i64, _vp, _vp, _vp]),
 }
 
 _LOCK = threading.Lock()

@@ -1,9 +1,13 @@
-"""Fused single-pass attention on the sm_100a tensor cores (nb200_attention).
+"""Fused attention on the sm_100a tensor cores, forward (nb200_attention_fwd) and backward
+(nb200_attention_bwd).
 
-O = softmax(scale * Q K^T [+ causal mask]) V per (batch, head) with bf16 Q, K, V, O of shape
-[B, H, S, D], fp32 scores and an fp32 online max/sum repair (the exp(c - s) rescale of the
-repaired fold applied to attention rows), and optionally the fp32 natural log-sum-exp of each
-query row's scaled scores, [B, H, S].
+O = softmax(scale * Q K^T [+ masks]) V per (batch, head) with bf16 Q, O of shape [B, H, S, D] and
+K, V of shape [B, H_kv, S, D] (H a multiple of H_kv: query head h reads key/value head
+h // (H // H_kv)), fp32 scores and an fp32 online max/sum repair (the exp(c - s) rescale of the
+repaired fold applied to attention rows), and optionally the fp32 natural log-sum-exp of each query
+row's scaled scores, [B, H, S]. `seq_lens` [B] gives the tokens of each batch element: queries and
+keys past them are masked, their rows of O and of the gradients are zero and their log-sum-exp is
+-inf, whatever the tensors hold there.
 
 The reference has no attention kernel (its roadmap declares one out of scope); the contract here
 follows torch.nn.functional.scaled_dot_product_attention with is_causal (key index <= query
@@ -13,16 +17,17 @@ kernel is not built for.
 """
 from __future__ import annotations
 
+import ctypes
 import math
 
 from neptune_opt_b200 import _lib
-from neptune_opt_b200.template import _on_device, current_stream
+from neptune_opt_b200.template import _is_metadata, _on_device, current_stream
 
 HEAD_DIMS = (128,)
 OP_NAME = "neptune_b200::attention"
 
 
-def validate_attention_inputs(q, k, v, scale):
+def validate_attention_inputs(q, k, v, scale, seq_lens=None):
     import torch
 
     for name, t in (("q", q), ("k", k), ("v", v)):
@@ -32,8 +37,10 @@ def validate_attention_inputs(q, k, v, scale):
             raise TypeError(f"attention: {name} must be bfloat16, got {t.dtype}")
         if t.dim() != 4:
             raise ValueError(f"attention: {name} must be [batch, heads, seq, head_dim], got {tuple(t.shape)}")
-    if q.shape != k.shape or q.shape != v.shape:
+    if k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[2:] != k.shape[2:]:
         raise ValueError(f"attention: q, k, v shapes differ: {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    if q.shape[1] != k.shape[1] and (k.shape[1] == 0 or q.shape[1] % k.shape[1]):
+        raise ValueError(f"attention: {q.shape[1]} query heads cannot share {k.shape[1]} key/value heads")
     if q.device != k.device or q.device != v.device:
         raise ValueError("attention: q, k, v must be on one device")
     if q.device.type != "cuda" and q.device.type != "meta":
@@ -41,34 +48,134 @@ def validate_attention_inputs(q, k, v, scale):
     d = q.shape[-1]
     if d not in HEAD_DIMS:
         raise NotImplementedError(f"attention: head_dim {d} is not supported (built for {HEAD_DIMS})")
+    if seq_lens is not None:
+        if not isinstance(seq_lens, torch.Tensor) or seq_lens.dtype != torch.int32:
+            raise TypeError("attention: seq_lens must be an int32 tensor")
+        if tuple(seq_lens.shape) != (q.shape[0],) or seq_lens.device != q.device or not seq_lens.is_contiguous():
+            raise ValueError("attention: seq_lens must be a contiguous [batch] tensor on the device of q")
     s = 1.0 / math.sqrt(d) if scale is None else float(scale)
     if not (math.isfinite(s) and s > 0.0):
         raise ValueError(f"attention: scale must be finite and positive, got {scale}")
     return s
 
 
-def launch_attention(q, k, v, o, lse, *, causal: bool, scale: float) -> None:
-    """One nb200_attention call on the current stream of q's device (all tensors contiguous)."""
-    lib = _lib.load()
+def _rows(t):
+    """t itself when the kernels' copies can read its rows (unit stride in a row, 16-byte multiples
+    between rows, heads and batch elements, 16-byte aligned base), else a contiguous copy."""
+    import torch
+
+    sizes, strides = t.shape, t.stride()
+    if strides[3] == 1 and t.data_ptr() % 16 == 0 and all(
+            sizes[i] <= 1 or (strides[i] > 0 and strides[i] % 8 == 0) for i in range(3)):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _args(q, k, causal, scale, seq_lens):
     b, h, s, d = q.shape
+    return _lib.NB200AttnArgs(b, h, k.shape[1], s, d, seq_lens.data_ptr() if seq_lens is not None else None,
+                              1 if causal else 0, scale)
+
+
+def _strides(*tensors):
+    return (_lib.NB200AttnStrides * len(tensors))(*[t.stride()[:3] for t in tensors])
+
+
+def launch_attention(q, k, v, o, lse, *, causal: bool, scale: float, seq_lens=None) -> None:
+    """One nb200_attention_fwd call on the current stream of q's device."""
+    lib = _lib.load()
     with _on_device(q.device):
-        rc = lib.nb200_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
-                                 lse.data_ptr() if lse is not None else None, b, h, s, d, 1 if causal else 0,
-                                 scale, current_stream(q.device))
+        rc = lib.nb200_attention_fwd(ctypes.byref(_args(q, k, causal, scale, seq_lens)), _strides(q, k, v, o),
+                                     q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+                                     lse.data_ptr() if lse is not None else None, current_stream(q.device))
     _lib.check(rc, "nb200_attention")
 
 
-def run_attention(q, k, v, *, causal: bool = False, scale=None, return_lse: bool = False):
-    """Fresh O (and LSE when asked) for contiguous copies of q, k, v."""
+def _forward(q, k, v, causal, scale, seq_lens, with_lse):
     import torch
 
-    sc = validate_attention_inputs(q, k, v, scale)
-    q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
-    o = torch.empty_like(q)
-    lse = torch.empty(q.shape[:-1], device=q.device, dtype=torch.float32) if return_lse else None
-    if q.device.type != "meta" and q.numel():
-        launch_attention(q, k, v, o, lse, causal=causal, scale=sc)
+    o = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    lse = torch.empty(q.shape[:-1], device=q.device, dtype=torch.float32) if with_lse else None
+    if not _is_metadata(q) and q.numel():
+        launch_attention(_rows(q), _rows(k), _rows(v), o, lse, causal=causal, scale=scale, seq_lens=seq_lens)
+    return o, lse
+
+
+def run_attention(q, k, v, *, causal: bool = False, scale=None, return_lse: bool = False, seq_lens=None):
+    """Fresh contiguous O (and LSE when asked). With gradients enabled and wanted, O carries them (LSE
+    does not)."""
+    import torch
+
+    sc = validate_attention_inputs(q, k, v, scale, seq_lens)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        o, lse = _function().apply(q, k, v, causal, sc, seq_lens)
+    else:
+        o, lse = _forward(q, k, v, causal, sc, seq_lens, return_lse)
     return (o, lse) if return_lse else o
+
+
+def attention_backward(q, k, v, o, lse, grad_out, *, causal: bool = False, scale=None, seq_lens=None):
+    """(dq, dk, dv) of `run_attention`'s O for the gradient grad_out of it, from the saved O and LSE.
+
+    The probabilities are recomputed; dk and dv of a shared key/value head sum over its query heads.
+    The result does not depend on scheduling. Gradients keep the memory layout of their inputs."""
+    import torch
+
+    sc = validate_attention_inputs(q, k, v, scale, seq_lens)
+    for name, t in (("o", o), ("grad_out", grad_out)):
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.bfloat16:
+            raise TypeError(f"attention_backward: {name} must be a bfloat16 tensor")
+        if t.shape != q.shape or t.device != q.device:
+            raise ValueError(f"attention_backward: {name} must have the shape and device of q")
+    if not isinstance(lse, torch.Tensor) or lse.dtype != torch.float32:
+        raise TypeError("attention_backward: lse must be a float32 tensor")
+    if lse.shape != q.shape[:-1] or lse.device != q.device:
+        raise ValueError("attention_backward: lse must be [batch, heads, seq] on the device of q")
+    if _is_metadata(q) or q.numel() == 0:
+        return torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v)
+    q, k, v, o, grad_out, lse = _rows(q), _rows(k), _rows(v), _rows(o), _rows(grad_out), lse.contiguous()
+    dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    lib = _lib.load()
+    args = _args(q, k, causal, sc, seq_lens)
+    nbytes = lib.nb200_attention_bwd_work_bytes(ctypes.byref(args))
+    work = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=q.device)
+    with _on_device(q.device):
+        rc = lib.nb200_attention_bwd(ctypes.byref(args), _strides(q, k, v, o, grad_out, dq, dk, dv), q.data_ptr(),
+                                     k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), grad_out.data_ptr(),
+                                     dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), work.data_ptr(), work.numel(),
+                                     current_stream(q.device))
+    _lib.check(rc, "nb200_attention_bwd")
+    return dq, dk, dv
+
+
+_FUNCTION = None
+
+
+def _function():
+    global _FUNCTION
+    if _FUNCTION is not None:
+        return _FUNCTION
+    import torch
+
+    class Attention(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, q, k, v, causal, scale, seq_lens):
+            o, lse = _forward(q, k, v, causal, scale, seq_lens, True)
+            ctx.save_for_backward(q, k, v, o, lse, seq_lens)
+            ctx.causal, ctx.scale = causal, scale
+            ctx.mark_non_differentiable(lse)
+            return o, lse
+
+        @staticmethod
+        @torch.autograd.function.once_differentiable
+        def backward(ctx, grad_out, _):
+            q, k, v, o, lse, seq_lens = ctx.saved_tensors
+            grads = attention_backward(q, k, v, o, lse, grad_out, causal=ctx.causal, scale=ctx.scale,
+                                       seq_lens=seq_lens)
+            return (*grads, None, None, None)
+
+    _FUNCTION = Attention
+    return _FUNCTION
 
 
 _OP = None

@@ -1,0 +1,209 @@
+"""The norms around a transformer block, fused with the block's gate and residual scale
+(nb200_gated_norm, nb200_gated_norm_bwd).
+
+    z = post_weight * x * rsqrt(mean(x^2) + eps)          x is the block's output (z = x without the weight)
+    y = residual + residual_scale * a(gate) * z           a: identity, tanh or sigmoid (1 without a gate)
+    h = pre_weight * y * rsqrt(mean(y^2) + eps)           the next block's input (None without the weight)
+
+One pass over x and residual, everything in fp32, each result rounded once (h from the unrounded y).
+Gradients are those of that function; weight and shared-gate gradients are fp32 column sums added in
+a fixed order. The reference's RMSNorm (neptune_codegen/emitters.py:549-627) is the inner norm alone,
+forward only, with its own rounding stages: `rms_norm` keeps those.
+
+x and residual are [..., width] in float32, bfloat16 or float16, gate and weights of the same dtype.
+gate is [width], or has x's rank with leading dimensions equal to x's followed by ones (one gate row
+per sequence, or per token). Errors follow the backend's convention: TypeError for dtypes, ValueError
+for devices, shapes and parameters, NotImplementedError past the kernels' width.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+from neptune_opt_b200 import _lib
+from neptune_opt_b200.template import _is_metadata, _on_device, current_stream, dtype_code
+
+GATE_ACTS = {"none": 0, "tanh": 1, "sigmoid": 2}
+MAX_WIDTH = 16384
+
+
+def _rows_per_gate(x, gate) -> int:
+    """Consecutive rows of x that share one row of the gate."""
+    if gate.dim() == 1:
+        return math.prod(x.shape[:-1])
+    lead, shared, n = x.shape[:-1], gate.shape[:-1], 0
+    if gate.dim() == x.dim():
+        while n < len(lead) and shared[n] == lead[n]:
+            n += 1
+        if all(s == 1 for s in shared[n:]):
+            return math.prod(lead[n:])
+    raise ValueError(f"gated_residual_norm: gate {tuple(gate.shape)} does not broadcast over rows of {tuple(x.shape)}")
+
+
+def validate_gated_norm_inputs(x, residual, gate, post_weight, pre_weight, gate_act, residual_scale, eps=1.0):
+    """Metadata-only contract; returns the rows that share a gate row."""
+    import torch
+
+    what = "gated_residual_norm"
+    for name, t in (("x", x), ("residual", residual), ("gate", gate), ("post_weight", post_weight),
+                    ("pre_weight", pre_weight)):
+        if t is None and name not in ("x", "residual"):
+            continue
+        if not isinstance(t, torch.Tensor) or t.layout != torch.strided:
+            raise TypeError(f"{what}: {name} must be a strided tensor")
+        if t.dtype not in (torch.float32, torch.bfloat16, torch.float16) or t.dtype != x.dtype:
+            raise TypeError(f"{what}: {name} must share x's float32/bfloat16/float16 dtype, got {t.dtype}")
+        if t.device != x.device:
+            raise ValueError(f"{what}: {name} must be on the device of x")
+    if x.device.type not in ("cuda", "meta"):
+        raise ValueError(f"{what}: inputs must be CUDA tensors, got {x.device}")
+    if x.dim() < 1 or x.shape[-1] < 1 or x.shape != residual.shape:
+        raise ValueError(f"{what}: x {tuple(x.shape)} and residual {tuple(residual.shape)} must be one [..., width]")
+    for name, t in (("post_weight", post_weight), ("pre_weight", pre_weight)):
+        if t is not None and tuple(t.shape) != (x.shape[-1],):
+            raise ValueError(f"{what}: {name} must be [{x.shape[-1]}], got {tuple(t.shape)}")
+    if post_weight is None and pre_weight is None:
+        raise ValueError(f"{what}: neither post_weight nor pre_weight is given")
+    if gate is not None and (gate.dim() < 1 or gate.shape[-1] != x.shape[-1]):
+        raise ValueError(f"{what}: gate must be [..., {x.shape[-1]}], got {tuple(gate.shape)}")
+    if gate_act not in GATE_ACTS:
+        raise ValueError(f"{what}: gate_act must be one of {sorted(GATE_ACTS)}, got {gate_act!r}")
+    if not math.isfinite(residual_scale):
+        raise ValueError(f"{what}: residual_scale must be finite")
+    if not (math.isfinite(eps) and eps > 0):
+        raise ValueError(f"{what}: eps must be finite and positive")
+    if x.shape[-1] > MAX_WIDTH:
+        raise NotImplementedError(f"{what}: width {x.shape[-1]} exceeds {MAX_WIDTH}")
+    return 1 if gate is None else _rows_per_gate(x, gate)
+
+
+def _flat(t):
+    """[rows, width] of t with unit column stride (a copy only when no such view exists)."""
+    t2 = t.reshape(-1, t.shape[-1])
+    if t2.stride(1) != 1 and t2.shape[1] != 1 or t2.stride(0) < 0:
+        t2 = t2.contiguous()
+    return t2
+
+
+def _args(x, residual, gate, post_weight, pre_weight, per_gate, gate_act, residual_scale, eps):
+    """(nb200_norm_args, the tensors whose memory it names)."""
+    keep = [None if t is None else _flat(t) for t in (x, residual, gate)]
+    keep += [None if w is None else w.contiguous() for w in (post_weight, pre_weight)]
+    x2 = keep[0]
+    a = _lib.NB200NormArgs(*[None if t is None else t.data_ptr() for t in keep], x2.shape[0], x2.shape[1],
+                           x2.stride(0), keep[1].stride(0), 0 if gate is None else keep[2].stride(0), 0, 0, per_gate,
+                           GATE_ACTS[gate_act], residual_scale, eps)
+    return a, keep
+
+
+def run_gated_residual_norm(x, residual, gate=None, *, post_weight=None, pre_weight=None, gate_act: str = "none",
+                            residual_scale: float = 1.0, eps: float = 1e-6):
+    """(y, h, rstd): fresh contiguous results in x's dtype (h is None without pre_weight) and the fp32
+    reciprocal norms [..., 2] that the backward pass takes."""
+    import torch
+
+    per_gate = validate_gated_norm_inputs(x, residual, gate, post_weight, pre_weight, gate_act, residual_scale, eps)
+    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    h = torch.empty(x.shape, device=x.device, dtype=x.dtype) if pre_weight is not None else None
+    rstd = torch.empty((*x.shape[:-1], 2), device=x.device, dtype=torch.float32)
+    if _is_metadata(x) or x.numel() == 0:
+        return y, h, rstd
+    a, keep = _args(x, residual, gate, post_weight, pre_weight, per_gate, gate_act, residual_scale, eps)
+    lib = _lib.load()
+    with _on_device(x.device):
+        rc = lib.nb200_gated_norm(ctypes.byref(a), dtype_code(x.dtype), y.data_ptr(),
+                                  None if h is None else h.data_ptr(), rstd.data_ptr(), current_stream(x.device))
+    _lib.check(rc, "nb200_gated_norm")
+    return y, h, rstd
+
+
+def gated_residual_norm_backward(grad_y, grad_h, x, residual, gate, rstd, *, post_weight=None, pre_weight=None,
+                                 gate_act: str = "none", residual_scale: float = 1.0):
+    """(dx, dresidual, dgate, dpost_weight, dpre_weight) for the gradients of y and h (either may be
+    None); None in the place of an input that is absent. dgate sums over the rows that share a gate row."""
+    import torch
+
+    per_gate = validate_gated_norm_inputs(x, residual, gate, post_weight, pre_weight, gate_act, residual_scale)
+    if grad_h is not None and pre_weight is None:
+        raise ValueError("gated_residual_norm_backward: grad_h without pre_weight")
+    for name, t in (("grad_y", grad_y), ("grad_h", grad_h)):
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor) or t.dtype != x.dtype:
+            raise TypeError(f"gated_residual_norm_backward: {name} must be a tensor of x's dtype")
+        if t.shape != x.shape or t.device != x.device:
+            raise ValueError(f"gated_residual_norm_backward: {name} must have the shape and device of x")
+    if not isinstance(rstd, torch.Tensor) or rstd.dtype != torch.float32:
+        raise TypeError("gated_residual_norm_backward: rstd must be a float32 tensor")
+    if tuple(rstd.shape) != (*x.shape[:-1], 2) or rstd.device != x.device:
+        raise ValueError("gated_residual_norm_backward: rstd must be [..., 2] on the device of x")
+
+    def fresh(t):
+        return None if t is None else torch.empty(t.shape, device=t.device, dtype=t.dtype)
+
+    grads = [fresh(t) for t in (x, residual, gate, post_weight, pre_weight)]
+    if _is_metadata(x) or x.numel() == 0:
+        return tuple(None if g is None else g.zero_() for g in grads)
+    a, keep = _args(x, residual, gate, post_weight, pre_weight, per_gate, gate_act, residual_scale, 1.0)
+    gy, gh = (None if t is None else _flat(t) for t in (grad_y, grad_h))
+    a.stride_grad_y = 0 if gy is None else gy.stride(0)
+    a.stride_grad_h = 0 if gh is None else gh.stride(0)
+    lib = _lib.load()
+    nbytes = lib.nb200_gated_norm_bwd_work_bytes(ctypes.byref(a))
+    work = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=x.device)
+    rstd = rstd.contiguous()
+
+    def ptr(t):
+        return None if t is None else t.data_ptr()
+
+    with _on_device(x.device):
+        rc = lib.nb200_gated_norm_bwd(ctypes.byref(a), dtype_code(x.dtype), ptr(rstd), ptr(gy), ptr(gh),
+                                      *[ptr(g) for g in grads], ptr(work), work.numel(), current_stream(x.device))
+    _lib.check(rc, "nb200_gated_norm_bwd")
+    return tuple(grads)
+
+
+_FUNCTION = None
+
+
+def _function():
+    global _FUNCTION
+    if _FUNCTION is not None:
+        return _FUNCTION
+    import torch
+
+    class GatedResidualNorm(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, residual, gate, post_weight, pre_weight, gate_act, residual_scale, eps):
+            y, h, rstd = run_gated_residual_norm(x, residual, gate, post_weight=post_weight, pre_weight=pre_weight,
+                                                 gate_act=gate_act, residual_scale=residual_scale, eps=eps)
+            ctx.save_for_backward(x, residual, gate, post_weight, pre_weight, rstd)
+            ctx.gate_act, ctx.residual_scale = gate_act, residual_scale
+            ctx.set_materialize_grads(False)
+            return y, h
+
+        @staticmethod
+        @torch.autograd.function.once_differentiable
+        def backward(ctx, grad_y, grad_h):
+            x, residual, gate, post_weight, pre_weight, rstd = ctx.saved_tensors
+            grads = gated_residual_norm_backward(grad_y, grad_h, x, residual, gate, rstd, post_weight=post_weight,
+                                                 pre_weight=pre_weight, gate_act=ctx.gate_act,
+                                                 residual_scale=ctx.residual_scale)
+            return (*grads, None, None, None)
+
+    _FUNCTION = GatedResidualNorm
+    return _FUNCTION
+
+
+def gated_residual_norm(x, residual, gate=None, *, post_weight=None, pre_weight=None, gate_act: str = "none",
+                        residual_scale: float = 1.0, eps: float = 1e-6):
+    """(y, h): the residual stream after a block and the next block's normalised input (None without
+    pre_weight). Differentiable in every tensor argument."""
+    import torch
+
+    tensors = (x, residual, gate, post_weight, pre_weight)
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
+        validate_gated_norm_inputs(*tensors, gate_act, residual_scale, eps)
+        return _function().apply(*tensors, gate_act, residual_scale, eps)
+    return run_gated_residual_norm(x, residual, gate, post_weight=post_weight, pre_weight=pre_weight,
+                                   gate_act=gate_act, residual_scale=residual_scale, eps=eps)[:2]

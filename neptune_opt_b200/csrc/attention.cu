@@ -1,5 +1,6 @@
-// Fused single-pass attention forward, O = softmax(scale * Q K^T [+ causal mask]) V, bf16 in and
-// out, fp32 scores and online max/sum repair, on the sm_100a tensor cores.
+// Fused single-pass attention forward, O = softmax(scale * Q K^T [+ masks]) V, bf16 in and out, fp32
+// scores and online max/sum repair, on the sm_100a tensor cores. Query heads may share key/value
+// heads; a batch element may hold fewer tokens than the tensors (the rest is masked).
 //
 // One CTA owns 256 query rows of one (batch, head): two query tiles of 128 rows, one tensor-memory
 // lane per row. The K/V sequence streams through a ring of shared-memory stages filled by
@@ -29,24 +30,16 @@
 // attention fault word and the CTA's abort flag; the other roles stop at their next wait, the
 // producer waits for the copies it issued, the MMA thread waits for its MMAs, and the CTA frees
 // its tensor memory and exits with the output unwritten.
-#include <cudaTypedefs.h>
-
 #include <mutex>
 
-#include "common.cuh"
-#include "launch.h"
-#include "fastmath.cuh"
-#include "tcgen05.cuh"
+#include "attn.cuh"
 
 namespace nb200 {
 namespace {
 
-static __device__ unsigned int g_attn_fault = 0u;
-
 constexpr int kRows = 128;   // query rows per tile (= TMEM lanes)
 constexpr int kQTiles = 2;   // query tiles per CTA
 constexpr int kKeys = 128;   // keys per K/V tile
-constexpr int kDim = 128;    // head dimension
 constexpr int kStages = 5;   // K/V ring stages; each holds one K or one V tile
 constexpr uint32_t kTileBytes = kRows * kDim * 2;  // 32 KB per Q, K or V tile
 constexpr uint32_t kHalfBytes = kTileBytes / 2;    // one 64-column half: the TMA box
@@ -78,7 +71,6 @@ static_assert(kPParts == 2 || kPParts == 4 || kPParts == 8, "P parts");
 constexpr float kRescaleSlack = 8.f;          // keep a stale max while the new one is < 2^8 above it
 constexpr uint32_t kIdescQK = tc::idesc_bf16(128, 128, false);
 constexpr uint32_t kIdescPV = tc::idesc_bf16(128, 128, true);
-constexpr long long kWaitCycles = 1ll << 31;
 
 // Shared-memory layout (offsets from a 1024-byte aligned base).
 constexpr uint32_t kOffQ = 0;                                // kQTiles tiles
@@ -91,6 +83,7 @@ struct Bars {
     uint64_t s_full[kQTiles];
     uint64_t p_full[kQTiles][kPParts];  // per part of P (128 / kPParts keys each)
     uint64_t o_final;
+    uint64_t tail;  // the last V tile's copy, when rows of it are masked before it is published
     uint32_t tmem_base;
     int abort;
 };
@@ -98,54 +91,16 @@ constexpr uint32_t kSmemBytes = kOffBar + sizeof(Bars) + 1024;  // + alignment s
 
 struct AttnArgs {
     int S;        // sequence length (queries = keys)
-    int BH;       // batch * heads
+    int H;        // query heads
+    int group;    // query heads that share a key/value head
+    const int* lens;  // tokens of each batch element, nullable
+    int64_t ob, oh, os;  // strides of o
+    __nv_bfloat16* o;
     int nqb;      // query blocks of kQTiles * kRows rows per (batch, head)
     int causal;
     float sl2;    // scale * log2(e)
     float* lse;   // [BH, S] natural log-sum-exp, nullable
 };
-
-// Bounded wait on phase `parity` of `bar`. Gives up early when another role has aborted the CTA.
-// (Inline on purpose: a called function would need one register budget for roles that run under
-// different setmaxnreg limits.)
-__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* abort) {
-    if (mbar_try_wait(bar, parity)) return true;
-    const long long t0 = clock64();
-    for (uint32_t i = 1; i < (1u << 30); ++i) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if ((i & 255u) == 0) {
-            if (*abort) return false;
-            if (clock64() - t0 > kWaitCycles) break;
-        }
-    }
-    atomicOr(&g_attn_fault, 2u);
-    *abort = 1;
-    return false;
-}
-
-// Position in the K/V stage ring: stage index and the parity of its current fill.
-struct Ring {
-    int s = 0;
-    uint32_t ph = 0;
-    __device__ __forceinline__ void next() {
-        if (++s == kStages) {
-            s = 0;
-            ph ^= 1u;
-        }
-    }
-};
-
-// Bounded wait used while shutting down: ignores the abort flag (outstanding copies and MMAs
-// must land before the CTA exits) but still gives up after the same limit.
-__device__ __forceinline__ void drain_bar(uint64_t* bar, uint32_t parity) {
-    if (mbar_try_wait(bar, parity)) return;
-    const long long t0 = clock64();
-    for (uint32_t i = 1; i < (1u << 30); ++i) {
-        if (mbar_try_wait(bar, parity)) return;
-        if ((i & 255u) == 0 && clock64() - t0 > kWaitCycles) break;
-    }
-    atomicOr(&g_attn_fault, 2u);
-}
 
 // P for part qp of this row's keys: p = 2^(s * sl2 - m) on the special-function unit,
 // rounded to bf16 into TMEM (one column per key pair, the lower key in the low half), fp32 p added
@@ -178,35 +133,59 @@ __device__ __forceinline__ void p_part(const float* s, int qp, uint64_t sl2, uin
     }
 }
 
+// The whole warp calls it; lane 0 issues. With tail > 0 only that many rows of the last V tile belong
+// to the sequence: what lies past them is zeroed before the tile is published, because a masked
+// probability of 0 times an infinity or NaN there would still poison the product.
 __device__ __forceinline__ void producer(const CUtensorMap* mq, const CUtensorMap* mk, const CUtensorMap* mv,
-                                         uint8_t* smem, Bars* b, int bh, int q0, int n) {
+                                         uint8_t* smem, Bars* b, int head, int kv_head, int batch, int q0, int n,
+                                         int tail, int lane) {
     volatile int* abort = &b->abort;
-    tc::prefetch_map(mq);
-    tc::prefetch_map(mk);
-    tc::prefetch_map(mv);
-    for (int t = 0; t < kQTiles; ++t) {
-        uint8_t* dst = smem + kOffQ + t * kTileBytes;
-        mbar_expect_tx(&b->q_full[t], kTileBytes);
-        tc::tma_load_3d(dst, mq, 0, q0 + t * kRows, bh, &b->q_full[t]);
-        tc::tma_load_3d(dst + kHalfBytes, mq, kDim / 2, q0 + t * kRows, bh, &b->q_full[t]);
+    if (lane == 0) {
+        tc::prefetch_map(mq);
+        tc::prefetch_map(mk);
+        tc::prefetch_map(mv);
+        for (int t = 0; t < kQTiles; ++t) {
+            uint8_t* dst = smem + kOffQ + t * kTileBytes;
+            mbar_expect_tx(&b->q_full[t], kTileBytes);
+            tc::tma_load_4d(dst, mq, 0, q0 + t * kRows, head, batch, &b->q_full[t]);
+            tc::tma_load_4d(dst + kHalfBytes, mq, kDim / 2, q0 + t * kRows, head, batch, &b->q_full[t]);
+        }
     }
-    int it = 0;
-    Ring r;
-    for (; it < 2 * n; ++it, r.next()) {
-        const int s = r.s;
-        if (!wait_bar(&b->kv_empty[s], r.ph ^ 1u, abort)) break;
+    auto load = [&](int it, int s, uint64_t* bar) {
         uint8_t* dst = smem + kOffKV + s * kTileBytes;
         const CUtensorMap* m = (it & 1) ? mv : mk;
         const int row = (it >> 1) * kKeys;
-        mbar_expect_tx(&b->kv_full[s], kTileBytes);
-        tc::tma_load_3d(dst, m, 0, row, bh, &b->kv_full[s]);
-        tc::tma_load_3d(dst + kHalfBytes, m, kDim / 2, row, bh, &b->kv_full[s]);
+        mbar_expect_tx(bar, kTileBytes);
+        tc::tma_load_4d(dst, m, 0, row, kv_head, batch, bar);
+        tc::tma_load_4d(dst + kHalfBytes, m, kDim / 2, row, kv_head, batch, bar);
+    };
+    int it = 0;
+    Ring<kStages> r;
+    bool ok = true;
+    for (const int whole = tail ? 2 * n - 1 : 2 * n; it < whole; ++it, r.next()) {
+        ok = lane != 0 || wait_bar(&b->kv_empty[r.s], r.ph ^ 1u, abort);
+        if (!ok) break;
+        if (lane == 0) load(it, r.s, &b->kv_full[r.s]);
+    }
+    ok = __all_sync(0xffffffffu, ok);
+    if (tail && ok) {
+        ok = lane != 0 || wait_bar(&b->kv_empty[r.s], r.ph ^ 1u, abort);
+        if (lane == 0 && ok) load(it, r.s, &b->tail);
+        ok = __all_sync(0xffffffffu, ok) && __all_sync(0xffffffffu, wait_bar(&b->tail, 0, abort));
+        if (ok) {
+            zero_tail(smem + kOffKV + r.s * kTileBytes, kKeys, tail, lane);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&b->kv_full[r.s]);
+            ++it;
+        }
     }
     // Every copy issued into this CTA's shared memory lands before the CTA may exit: wait for the
     // last phase filled in each stage (`it` tiles were issued, stage s got those with index = s
     // mod kStages).
-    for (int t = 0; t < kQTiles; ++t) drain_bar(&b->q_full[t], 0);
-    for (int s = 0; s < kStages && s < it; ++s) drain_bar(&b->kv_full[s], ((it - 1 - s) / kStages) & 1u);
+    if (lane == 0) {
+        for (int t = 0; t < kQTiles; ++t) drain_bar(&b->q_full[t], 0);
+        for (int s = 0; s < kStages && s < it; ++s) drain_bar(&b->kv_full[s], ((it - 1 - s) / kStages) & 1u);
+    }
 }
 
 // n K/V tiles in the unit; query tile 0 uses the first n0 of them (n0 = n, or n - 1 under a causal
@@ -266,7 +245,7 @@ __device__ __forceinline__ void mma_issuer(uint8_t* smem, Bars* b, uint32_t tmem
         return true;
     };
     // kr: the next K tile's stage, vr: the next V tile's stage (tiles alternate K_0, V_0, K_1, ...).
-    Ring kr, vr;
+    Ring<kStages> kr, vr;
     vr.next();
     bool ok = wait_bar(&b->q_full[0], 0, abort) && wait_bar(&b->q_full[1], 0, abort) &&
               wait_bar(&b->kv_full[kr.s], kr.ph, abort);
@@ -310,13 +289,13 @@ __device__ __forceinline__ void mma_issuer(uint8_t* smem, Bars* b, uint32_t tmem
 }
 
 __device__ __forceinline__ void softmax_tile(const CUtensorMap* mo, uint8_t* smem, Bars* b, uint32_t tmem,
-                                             const AttnArgs& a, int bh, int q0, int n) {
+                                             const AttnArgs& a, int head, int batch, int len, int q0, int n) {
     volatile int* abort = &b->abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int t = warp >> 2, wq = warp & 3;
     const int r = wq * 32 + lane;  // row inside the tile = TMEM lane
     const int qrow = q0 + t * kRows + r;
-    const int lim = a.causal ? min(qrow, a.S - 1) : a.S - 1;  // last key this row attends to
+    const int lim = a.causal ? min(qrow, len - 1) : len - 1;  // last key this row attends to
     const uint32_t lanes = (uint32_t)(wq * 32) << 16;
     const uint32_t tS = tmem + lanes + kColS0 + 128 * t;
     const uint32_t tP = tS + kColP;
@@ -389,6 +368,7 @@ __device__ __forceinline__ void softmax_tile(const CUtensorMap* mo, uint8_t* sme
     // the O tensor map expects, then one TMA store per warp for its 32 rows.
     uint8_t* stage = smem + kOffQ + t * kTileBytes;
     const float inv = 1.f / l;
+    const bool live = qrow < len;  // rows past the sequence read out as zero, whatever q held there
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
         uint32_t v[32];
@@ -396,7 +376,7 @@ __device__ __forceinline__ void softmax_tile(const CUtensorMap* mo, uint8_t* sme
         uint32_t pk[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-            pk[i] = tc::pack_bf16(__uint_as_float(v[2 * i]) * inv, __uint_as_float(v[2 * i + 1]) * inv);
+            pk[i] = live ? tc::pack_bf16(__uint_as_float(v[2 * i]) * inv, __uint_as_float(v[2 * i + 1]) * inv) : 0u;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             const int ch = 4 * c + q;  // 16-byte chunk of the 256-byte row
@@ -404,13 +384,14 @@ __device__ __forceinline__ void softmax_tile(const CUtensorMap* mo, uint8_t* sme
             *reinterpret_cast<uint4*>(dst) = make_uint4(pk[4 * q], pk[4 * q + 1], pk[4 * q + 2], pk[4 * q + 3]);
         }
     }
-    if (a.lse && qrow < a.S) a.lse[(size_t)bh * a.S + qrow] = (m + log2f(l)) * 0.69314718055994531f;
+    if (a.lse && qrow < a.S)
+        a.lse[((size_t)batch * a.H + head) * a.S + qrow] = live ? (m + log2f(l)) * 0.69314718055994531f : -NB200_INF;
     fence_proxy_async();
     __syncwarp();
     const int row0 = q0 + t * kRows + wq * 32;
     if (lane == 0 && row0 < a.S) {
-        tc::tma_store_3d(mo, stage + wq * 32 * 128, 0, row0, bh);
-        tc::tma_store_3d(mo, stage + kHalfBytes + wq * 32 * 128, kDim / 2, row0, bh);
+        tc::tma_store_4d(mo, stage + wq * 32 * 128, 0, row0, head, batch);
+        tc::tma_store_4d(mo, stage + kHalfBytes + wq * 32 * 128, kDim / 2, row0, head, batch);
         tc::bulk_commit();
         tc::bulk_wait_read();
     }
@@ -431,10 +412,23 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int bh = (int)(blockIdx.x / (unsigned)a.nqb);
     const int qb = a.nqb - 1 - (int)(blockIdx.x % (unsigned)a.nqb);
     const int q0 = qb * kQTiles * kRows;
-    const int kv_end = a.causal ? min(q0 + kQTiles * kRows, a.S) : a.S;
+    const int batch = bh / a.H, head = bh % a.H;
+    const int len = tokens_of(a.lens, batch, a.S);
+    if (q0 >= len) {  // no query of this block belongs to the sequence
+        const int rows = min(kQTiles * kRows, a.S - q0);
+        for (int i = threadIdx.x; i < rows * (kDim / 8); i += kThreads)
+            *reinterpret_cast<uint4*>(a.o + batch * a.ob + head * a.oh + (q0 + i / (kDim / 8)) * a.os +
+                                      i % (kDim / 8) * 8) = make_uint4(0u, 0u, 0u, 0u);
+        if (a.lse)
+            for (int i = threadIdx.x; i < rows; i += kThreads) a.lse[(size_t)bh * a.S + q0 + i] = -NB200_INF;
+        return;
+    }
+    const int kv_end = a.causal ? min(q0 + kQTiles * kRows, len) : len;
     const int n = (kv_end + kKeys - 1) / kKeys;
     // Query tile 0 of a causal unit ends 128 rows earlier: its last K/V tile would be fully masked.
-    const int n0 = a.causal ? (min(q0 + kRows, a.S) + kKeys - 1) / kKeys : n;
+    const int n0 = a.causal ? (min(q0 + kRows, len) + kKeys - 1) / kKeys : n;
+    // Rows of the last V tile inside the sequence, when the tensor holds more rows past them.
+    const int tail = n * kKeys > len && len < a.S ? len - (n - 1) * kKeys : 0;
 
     if (threadIdx.x == 0) {
         for (int t = 0; t < kQTiles; ++t) {
@@ -447,6 +441,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&b->kv_empty[s], 1);
         }
         mbar_init(&b->o_final, 1);
+        mbar_init(&b->tail, 1);
         b->abort = 0;
         fence_barrier_init();
     }
@@ -463,13 +458,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     // branch); both end at barrier 0, after which the MMA warp frees the tensor memory.
     if (warp < 8) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
-        softmax_tile(&mo, smem, b, tmem, a, bh, q0, warp < 4 ? n0 : n);
+        softmax_tile(&mo, smem, b, tmem, a, head, batch, len, q0, warp < 4 ? n0 : n);
         tc::fence_before();
         asm volatile("bar.sync 0;" ::: "memory");
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));
         if (warp == kLoadWarp) {
-            if (lane == 0) producer(&mq, &mk, &mv, smem, b, bh, q0, n);
+            producer(&mq, &mk, &mv, smem, b, head, head / a.group, batch, q0, n, tail, lane);
             __syncwarp();
         } else if (warp == kMmaWarp) {
             if (lane == 0) mma_issuer(smem, b, tmem, n0, n);
@@ -490,7 +485,9 @@ std::once_flag g_encode_once;
 std::mutex g_attr_mutex;
 bool g_attr_set[64] = {false};
 
-int get_encoder() {
+}  // namespace
+
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder(const char* what) {
     std::call_once(g_encode_once, [] {
         void* fn = nullptr;
         cudaDriverEntryPointQueryResult q;
@@ -499,69 +496,27 @@ int get_encoder() {
             g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
         cudaGetLastError();
     });
-    if (!g_encode) {
-        set_error("nb200_attention: the driver does not provide cuTensorMapEncodeTiled");
-        return NB200_ERR_LAUNCH;
-    }
-    return NB200_OK;
+    if (!g_encode) set_error("%s: the driver does not provide cuTensorMapEncodeTiled", what);
+    return g_encode;
 }
 
-// [BH, S, D] bf16 viewed as a 3-D tensor map with a {64, box_rows, 1} box and 128-byte swizzle.
-int encode_map(CUtensorMap* map, const void* base, int64_t BH, int64_t S, uint32_t box_rows, const char* what) {
-    const cuuint64_t dims[3] = {(cuuint64_t)kDim, (cuuint64_t)S, (cuuint64_t)BH};
-    const cuuint64_t strides[2] = {(cuuint64_t)kDim * 2, (cuuint64_t)S * kDim * 2};
-    const cuuint32_t box[3] = {kDim / 2, box_rows, 1};
-    const cuuint32_t estr[3] = {1, 1, 1};
-    const CUresult rc = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides,
-                                 box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (rc != CUDA_SUCCESS) {
-        set_error("nb200_attention: cannot describe %s as a tensor map (CUresult %d)", what, (int)rc);
-        return NB200_ERR_ARG;
-    }
-    return NB200_OK;
-}
+int attn_fault_take(unsigned int* bits) { return take_attn_fault(bits); }
 
-}  // namespace
-
-int attn_fault_take(unsigned int* bits) {
-    unsigned int v = 0, zero = 0;
-    if (cudaMemcpyFromSymbol(&v, g_attn_fault, sizeof(v)) != cudaSuccess ||
-        cudaMemcpyToSymbol(g_attn_fault, &zero, sizeof(zero)) != cudaSuccess) {
-        set_error("cannot read the attention fault word: %s", cudaGetErrorString(cudaGetLastError()));
-        return NB200_ERR_LAUNCH;
-    }
-    *bits = v;
-    return NB200_OK;
-}
-
-int launch_attention(const void* q, const void* k, const void* v, void* o, float* lse, int64_t B, int64_t H,
-                     int64_t S, int64_t D, int causal, float scale, cudaStream_t st) {
-    if (D != kDim) {
-        set_error("nb200_attention: head_dim %lld is not supported (this kernel is built for %d)", (long long)D, kDim);
-        return NB200_ERR_UNSUPPORTED;
-    }
-    if (!(scale > 0.f)) {
-        set_error("nb200_attention: scale must be positive");
-        return NB200_ERR_ARG;
-    }
-    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) ||
-        (lse && (reinterpret_cast<uintptr_t>(lse) & 3u))) {
-        set_error("nb200_attention: q, k, v, o must be 16-byte aligned and lse 4-byte aligned");
-        return NB200_ERR_ARG;
-    }
-    const int64_t BH = B * H;
-    const int64_t nqb = (S + kQTiles * kRows - 1) / (kQTiles * kRows);
-    if (S > (int64_t)1 << 30 || BH > (int64_t)1 << 30 || BH * nqb > 0x7fffffffLL) {
-        set_error("nb200_attention: batch*heads=%lld, seq=%lld exceed the kernel's index range", (long long)BH,
-                  (long long)S);
+int launch_attention(const nb200_attn_args& n, const nb200_attn_strides* strides, const void* q, const void* k,
+                     const void* v, void* o, float* lse, cudaStream_t st) {
+    const char* what = "nb200_attention";
+    const int64_t nqb = (n.seq + kQTiles * kRows - 1) / (kQTiles * kRows);
+    if (n.batch * n.heads * nqb > 0x7fffffffLL) {
+        set_error("%s: batch*heads=%lld, seq=%lld exceed the kernel's index range", what,
+                  (long long)(n.batch * n.heads), (long long)n.seq);
         return NB200_ERR_CAPACITY;
     }
-    int rc = get_encoder();
-    if (rc) return rc;
     CUtensorMap mq, mk, mv, mo;
-    if ((rc = encode_map(&mq, q, BH, S, kRows, "q")) || (rc = encode_map(&mk, k, BH, S, kKeys, "k")) ||
-        (rc = encode_map(&mv, v, BH, S, kKeys, "v")) || (rc = encode_map(&mo, o, BH, S, 32, "o")))
+    int rc;
+    if ((rc = encode_rows(&mq, what, "q", q, n.batch, n.heads, n.seq, strides[0], kRows)) ||
+        (rc = encode_rows(&mk, what, "k", k, n.batch, n.kv_heads, n.seq, strides[1], kKeys)) ||
+        (rc = encode_rows(&mv, what, "v", v, n.batch, n.kv_heads, n.seq, strides[2], kKeys)) ||
+        (rc = encode_rows(&mo, what, "o", o, n.batch, n.heads, n.seq, strides[3], 32)))
         return rc;
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
@@ -582,13 +537,19 @@ int launch_attention(const void* q, const void* k, const void* v, void* o, float
         }
     }
     AttnArgs a;
-    a.S = (int)S;
-    a.BH = (int)BH;
+    a.S = (int)n.seq;
+    a.H = (int)n.heads;
+    a.group = (int)(n.heads / n.kv_heads);
+    a.lens = n.seq_lens;
+    a.ob = strides[3].batch;
+    a.oh = strides[3].head;
+    a.os = strides[3].seq;
+    a.o = static_cast<__nv_bfloat16*>(o);
     a.nqb = (int)nqb;
-    a.causal = causal ? 1 : 0;
-    a.sl2 = scale * 1.4426950408889634f;
+    a.causal = n.causal ? 1 : 0;
+    a.sl2 = n.scale * 1.4426950408889634f;
     a.lse = lse;
-    attn_fwd_kernel<<<(unsigned)(BH * nqb), kThreads, kSmemBytes, st>>>(mq, mk, mv, mo, a);
+    attn_fwd_kernel<<<(unsigned)(n.batch * n.heads * nqb), kThreads, kSmemBytes, st>>>(mq, mk, mv, mo, a);
     count_launch();
     return finish_launch("nb200_attention");
 }

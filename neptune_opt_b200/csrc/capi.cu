@@ -59,6 +59,88 @@ namespace {
 
 bool valid_dtype(int d) { return d == NB200_F32 || d == NB200_BF16 || d == NB200_F16; }
 
+// Sizes, scale and the strides of `count` tensors in the order q, k, v, o, grad_o, dq, dk, dv.
+int check_attention(const char* what, const nb200_attn_args* a, const nb200_attn_strides* s, int count) {
+    if (!a || !s) { set_error("%s: null pointer", what); return NB200_ERR_ARG; }
+    if (a->batch < 0 || a->heads < 0 || a->seq < 0) { set_error("%s: negative size", what); return NB200_ERR_ARG; }
+    if (a->batch == 0 || a->heads == 0 || a->seq == 0) return NB200_OK;
+    if (a->kv_heads < 1 || a->heads % a->kv_heads) {
+        set_error("%s: %lld query heads cannot share %lld key/value heads", what, (long long)a->heads,
+                  (long long)a->kv_heads);
+        return NB200_ERR_ARG;
+    }
+    if (!std::isfinite(a->scale)) { set_error("%s: scale must be finite", what); return NB200_ERR_ARG; }
+    if (a->head_dim != 128) {
+        set_error("%s: head_dim %lld is not supported (the kernels are built for 128)", what, (long long)a->head_dim);
+        return NB200_ERR_UNSUPPORTED;
+    }
+    if (!(a->scale > 0.f)) { set_error("%s: scale must be positive", what); return NB200_ERR_ARG; }
+    const int64_t most = (int64_t)1 << 30;
+    if (a->seq > most || a->batch > most || a->heads > most || a->batch * a->heads > most) {
+        set_error("%s: batch*heads=%lld*%lld, seq=%lld exceed the kernel's index range", what, (long long)a->batch,
+                  (long long)a->heads, (long long)a->seq);
+        return NB200_ERR_CAPACITY;
+    }
+    // The copies' limits: multiples of 16 bytes, below 2^40 bytes.
+    auto bad = [](int64_t stride, int64_t size) { return size > 1 && (stride < 8 || stride % 8 || stride >= (int64_t)1 << 39); };
+    for (int i = 0; i < count; ++i) {
+        const bool kv = i == 1 || i == 2 || i >= 6;
+        if (bad(s[i].batch, a->batch) || bad(s[i].head, kv ? a->kv_heads : a->heads) || bad(s[i].seq, a->seq)) {
+            set_error("%s: strides must be positive multiples of 8 elements (tensor %d)", what, i);
+            return NB200_ERR_ARG;
+        }
+    }
+    return NB200_OK;
+}
+
+int check_attention_pointers(const char* what, const void* const* tensors, int count, const float* lse,
+                             const int32_t* seq_lens) {
+    for (int i = 0; i < count; ++i) {
+        if (!tensors[i]) { set_error("%s: null pointer", what); return NB200_ERR_ARG; }
+        if (!aligned16(tensors[i])) { set_error("%s: tensors must be 16-byte aligned", what); return NB200_ERR_ARG; }
+    }
+    if (((uintptr_t)lse | (uintptr_t)seq_lens) & 3u) {
+        set_error("%s: lse and seq_lens must be 4-byte aligned", what);
+        return NB200_ERR_ARG;
+    }
+    return NB200_OK;
+}
+
+int check_norm(const char* what, const nb200_norm_args* a, int dtype, bool with_eps) {
+    if (!a) { set_error("%s: null pointer", what); return NB200_ERR_ARG; }
+    if (!valid_dtype(dtype)) { set_error("%s: unsupported dtype %d", what, dtype); return NB200_ERR_ARG; }
+    if (a->rows < 0 || a->width < 1) { set_error("%s: need rows >= 0 and width >= 1", what); return NB200_ERR_ARG; }
+    if (a->rows > 0x7fffffffLL) { set_error("%s: too many rows", what); return NB200_ERR_CAPACITY; }
+    if (a->gate && (a->rows_per_gate < 1 || a->rows % a->rows_per_gate)) {
+        set_error("%s: %lld rows are not whole groups of %lld", what, (long long)a->rows, (long long)a->rows_per_gate);
+        return NB200_ERR_ARG;
+    }
+    if (a->gate_act < NB200_GATE_NONE || a->gate_act > NB200_GATE_SIGMOID || !std::isfinite(a->scale) ||
+        (with_eps && !(std::isfinite(a->eps) && a->eps > 0))) {
+        set_error("%s: unknown gate activation, or scale or eps out of range", what);
+        return NB200_ERR_ARG;
+    }
+    return NB200_OK;
+}
+
+int check_distill(const char* what, const nb200_distill_args* a) {
+    if (!a) { set_error("%s: null pointer", what); return NB200_ERR_ARG; }
+    if (!valid_dtype(a->dtype) || !valid_dtype(a->teacher_dtype) ||
+        (a->index_dtype != NB200_I32 && a->index_dtype != NB200_I64)) {
+        set_error("%s: unsupported dtype", what);
+        return NB200_ERR_ARG;
+    }
+    if (a->rows < 0 || a->vocab < 1 || a->top < 0) {
+        set_error("%s: need rows >= 0, vocab >= 1 and top >= 0", what);
+        return NB200_ERR_ARG;
+    }
+    if (!(std::isfinite(a->temperature) && a->temperature > 0)) {
+        set_error("%s: temperature must be finite and positive", what);
+        return NB200_ERR_ARG;
+    }
+    return NB200_OK;
+}
+
 // Declared-parameter checks of the reference's certificate (algebra.py:285-302): every declared
 // scalar finite, T/beta/N/eps strictly positive, tiny nonnegative.
 int check_params(int sk, const nb200_params* q, nb200_params* out) {
@@ -130,11 +212,12 @@ uint64_t nb200_launch_count(void) { return g_launches.load(std::memory_order_rel
 
 int nb200_stream_fault(uint32_t* bits) {
     if (!bits) { set_error("nb200_stream_fault: null pointer"); return NB200_ERR_ARG; }
-    unsigned int v = 0, w = 0, x = 0;
+    unsigned int v = 0, w = 0, x = 0, y = 0;
     int rc = stream_fault_take(&v);
     if (rc == NB200_OK) rc = attn_fault_take(&w);
     if (rc == NB200_OK) rc = peer_fault_take(&x);
-    *bits = v | w | x;
+    if (rc == NB200_OK) rc = attn_bwd_fault_take(&y);
+    *bits = v | w | x | y;
     return rc;
 }
 
@@ -430,11 +513,108 @@ int nb200_ipc_close(void* base) {
 
 int nb200_attention(const void* q, const void* k, const void* v, void* o, float* lse, int64_t batch,
                     int64_t heads, int64_t seq, int64_t head_dim, int causal, float scale, void* stream) {
-    if (batch < 0 || heads < 0 || seq < 0) { set_error("nb200_attention: negative size"); return NB200_ERR_ARG; }
-    if (batch * heads * seq == 0) return NB200_OK;
-    if (!q || !k || !v || !o) { set_error("nb200_attention: null pointer"); return NB200_ERR_ARG; }
-    if (!std::isfinite(scale)) { set_error("nb200_attention: scale must be finite"); return NB200_ERR_ARG; }
-    return launch_attention(q, k, v, o, lse, batch, heads, seq, head_dim, causal, scale, (cudaStream_t)stream);
+    const nb200_attn_args a = {batch, heads, heads, seq, head_dim, nullptr, causal, scale};
+    const nb200_attn_strides s = {heads * seq * head_dim, seq * head_dim, head_dim};
+    const nb200_attn_strides all[4] = {s, s, s, s};
+    return nb200_attention_fwd(&a, all, q, k, v, o, lse, stream);
+}
+
+int nb200_attention_fwd(const nb200_attn_args* args, const nb200_attn_strides* strides, const void* q, const void* k,
+                        const void* v, void* o, float* lse, void* stream) {
+    int rc = check_attention("nb200_attention", args, strides, 4);
+    if (rc) return rc;
+    if (args->batch * args->heads * args->seq == 0) return NB200_OK;
+    const void* tensors[4] = {q, k, v, o};
+    if ((rc = check_attention_pointers("nb200_attention", tensors, 4, lse, args->seq_lens))) return rc;
+    return launch_attention(*args, strides, q, k, v, o, lse, (cudaStream_t)stream);
+}
+
+int64_t nb200_attention_bwd_work_bytes(const nb200_attn_args* args) {
+    const nb200_attn_strides none[8] = {};
+    const int rc = check_attention("nb200_attention_bwd", args, none, 0);
+    return rc ? rc : attention_bwd_work_bytes(*args);
+}
+
+int nb200_attention_bwd(const nb200_attn_args* args, const nb200_attn_strides* strides, const void* q, const void* k,
+                        const void* v, const void* o, const float* lse, const void* grad_o, void* dq, void* dk,
+                        void* dv, void* work, int64_t work_bytes, void* stream) {
+    int rc = check_attention("nb200_attention_bwd", args, strides, 8);
+    if (rc) return rc;
+    if (args->batch * args->heads * args->seq == 0) return NB200_OK;
+    const void* tensors[8] = {q, k, v, o, grad_o, dq, dk, dv};
+    if ((rc = check_attention_pointers("nb200_attention_bwd", tensors, 8, lse, args->seq_lens))) return rc;
+    if (!lse) { set_error("nb200_attention_bwd: null pointer"); return NB200_ERR_ARG; }
+    if (!work || !aligned16(work) || work_bytes < attention_bwd_work_bytes(*args)) {
+        set_error("nb200_attention_bwd: work must hold %lld bytes, 16-byte aligned",
+                  (long long)attention_bwd_work_bytes(*args));
+        return NB200_ERR_ARG;
+    }
+    return launch_attention_bwd(*args, strides, q, k, v, o, lse, grad_o, dq, dk, dv, work, (cudaStream_t)stream);
+}
+
+int nb200_gated_norm(const nb200_norm_args* args, int dtype, void* y, void* h, float* rstd, void* stream) {
+    const int rc = check_norm("nb200_gated_norm", args, dtype, true);
+    if (rc) return rc;
+    if (args->rows == 0) return NB200_OK;
+    if (!args->x || !args->residual || !y || !rstd || (args->pre_weight && !h)) {
+        set_error("nb200_gated_norm: null pointer");
+        return NB200_ERR_ARG;
+    }
+    return launch_norm_fwd(*args, dtype, y, h, rstd, (cudaStream_t)stream);
+}
+
+int64_t nb200_gated_norm_bwd_work_bytes(const nb200_norm_args* args) {
+    const int rc = check_norm("nb200_gated_norm_bwd", args, NB200_F32, false);
+    if (rc) return rc;
+    return args->rows ? norm_bwd_work_bytes(*args) : 0;
+}
+
+int nb200_gated_norm_bwd(const nb200_norm_args* args, int dtype, const float* rstd, const void* grad_y,
+                         const void* grad_h, void* dx, void* dresidual, void* dgate, void* dpost, void* dpre,
+                         void* work, int64_t work_bytes, void* stream) {
+    const int rc = check_norm("nb200_gated_norm_bwd", args, dtype, false);
+    if (rc) return rc;
+    if (args->rows == 0) return NB200_OK;
+    if (!args->x || !args->residual || !rstd || !dx || !dresidual) {
+        set_error("nb200_gated_norm_bwd: null pointer");
+        return NB200_ERR_ARG;
+    }
+    if ((dgate && !args->gate) || (dpost && !args->post_weight) || (dpre && !args->pre_weight) ||
+        (grad_h && !args->pre_weight)) {
+        set_error("nb200_gated_norm_bwd: a gradient of an input that is absent");
+        return NB200_ERR_ARG;
+    }
+    if (!work || !aligned16(work) || work_bytes < norm_bwd_work_bytes(*args)) {
+        set_error("nb200_gated_norm_bwd: work must hold %lld bytes, 16-byte aligned",
+                  (long long)norm_bwd_work_bytes(*args));
+        return NB200_ERR_ARG;
+    }
+    return launch_norm_bwd(*args, dtype, rstd, grad_y, grad_h, dx, dresidual, dgate, dpost, dpre,
+                           static_cast<float*>(work), (cudaStream_t)stream);
+}
+
+int nb200_distill_loss(const nb200_distill_args* args, const float* teacher_lse, float* loss, float* stats,
+                       void* stream) {
+    const int rc = check_distill("nb200_distill_loss", args);
+    if (rc) return rc;
+    if (args->rows == 0) return NB200_OK;
+    if (!args->x || (args->top && (!args->teacher || !args->index)) || !loss || !stats) {
+        set_error("nb200_distill_loss: null pointer");
+        return NB200_ERR_ARG;
+    }
+    return launch_distill_fwd(*args, teacher_lse, loss, stats, (cudaStream_t)stream);
+}
+
+int nb200_distill_loss_bwd(const nb200_distill_args* args, const float* grad, int64_t stride_grad, const float* stats,
+                           void* dx, void* stream) {
+    const int rc = check_distill("nb200_distill_loss_bwd", args);
+    if (rc) return rc;
+    if (args->rows == 0) return NB200_OK;
+    if (!args->x || (args->top && (!args->teacher || !args->index)) || !grad || !stats || !dx || stride_grad < 0) {
+        set_error("nb200_distill_loss_bwd: null pointer or negative stride");
+        return NB200_ERR_ARG;
+    }
+    return launch_distill_bwd(*args, grad, stride_grad, stats, dx, (cudaStream_t)stream);
 }
 
 }  // extern "C"

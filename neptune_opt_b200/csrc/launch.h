@@ -74,9 +74,23 @@ int stream_span(int sk, const Params& p, const void* x, int dtype, int64_t rows,
                 int finalize, const nb200_launch* L, cudaStream_t st);
 int stream_fault_take(unsigned int* bits);
 int attn_fault_take(unsigned int* bits);
+int attn_bwd_fault_take(unsigned int* bits);
 
-int launch_attention(const void* q, const void* k, const void* v, void* o, float* lse,
-                     int64_t B, int64_t H, int64_t S, int64_t D, int causal, float scale,
-                     cudaStream_t st);
+int launch_attention(const nb200_attn_args& a, const nb200_attn_strides* strides, const void* q, const void* k,
+                     const void* v, void* o, float* lse, cudaStream_t st);
+int64_t attention_bwd_work_bytes(const nb200_attn_args& a);
+int launch_attention_bwd(const nb200_attn_args& a, const nb200_attn_strides* strides, const void* q, const void* k,
+                         const void* v, const void* o, const float* lse, const void* grad_o, void* dq, void* dk,
+                         void* dv, void* work, cudaStream_t st);
+
+int launch_norm_fwd(const nb200_norm_args& a, int dtype, void* y, void* h, float* rstd, cudaStream_t st);
+int64_t norm_bwd_work_bytes(const nb200_norm_args& a);
+int launch_norm_bwd(const nb200_norm_args& a, int dtype, const float* rstd, const void* dy, const void* dh, void* dx,
+                    void* dres, void* dgate, void* dw1, void* dw2, float* work, cudaStream_t st);
+
+int launch_distill_fwd(const nb200_distill_args& a, const float* teacher_lse, float* loss, float* stats,
+                       cudaStream_t st);
+int launch_distill_bwd(const nb200_distill_args& a, const float* grad, int64_t stride_grad, const float* stats,
+                       void* dx, cudaStream_t st);
 
 }  // namespace nb200
