@@ -30,8 +30,6 @@
 // attention fault word and the CTA's abort flag; the other roles stop at their next wait, the
 // producer waits for the copies it issued, the MMA thread waits for its MMAs, and the CTA frees
 // its tensor memory and exits with the output unwritten.
-#include <mutex>
-
 #include "attn.cuh"
 
 namespace nb200 {
@@ -482,8 +480,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 // ------------------------------------------------------------------ host side
 PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
 std::once_flag g_encode_once;
-std::mutex g_attr_mutex;
-bool g_attr_set[64] = {false};
+SharedLimit g_shared;
 
 }  // namespace
 
@@ -518,24 +515,7 @@ int launch_attention(const nb200_attn_args& n, const nb200_attn_strides* strides
         (rc = encode_rows(&mv, what, "v", v, n.batch, n.kv_heads, n.seq, strides[2], kKeys)) ||
         (rc = encode_rows(&mo, what, "o", o, n.batch, n.heads, n.seq, strides[3], 32)))
         return rc;
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
-        cudaGetLastError();
-        set_error("nb200_attention: no usable current CUDA device");
-        return NB200_ERR_LAUNCH;
-    }
-    {
-        std::lock_guard<std::mutex> lock(g_attr_mutex);
-        if (!g_attr_set[dev]) {
-            if (cudaFuncSetAttribute(attn_fwd_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes) !=
-                cudaSuccess) {
-                set_error("nb200_attention: cannot reserve %u bytes of shared memory: %s", kSmemBytes,
-                          cudaGetErrorString(cudaGetLastError()));
-                return NB200_ERR_LAUNCH;
-            }
-            g_attr_set[dev] = true;
-        }
-    }
+    if ((rc = g_shared.raise(what, attn_fwd_kernel, kSmemBytes))) return rc;
     AttnArgs a;
     a.S = (int)n.seq;
     a.H = (int)n.heads;
