@@ -169,7 +169,9 @@ __device__ __forceinline__ void producer(const CUtensorMap* mq, const CUtensorMa
     if (tail && ok) {
         ok = lane != 0 || wait_bar(&b->kv_empty[r.s], r.ph ^ 1u, abort);
         if (lane == 0 && ok) load(it, r.s, &b->tail);
-        ok = __all_sync(0xffffffffu, ok) && __all_sync(0xffffffffu, wait_bar(&b->tail, 0, abort));
+        const bool sent = __all_sync(0xffffffffu, ok);
+        ok = sent && __all_sync(0xffffffffu, wait_bar(&b->tail, 0, abort));
+        if (sent && !ok && lane == 0) drain_bar(&b->tail, 0);
         if (ok) {
             zero_tail(smem + kOffKV + r.s * kTileBytes, kKeys, tail, lane);
             __syncwarp();

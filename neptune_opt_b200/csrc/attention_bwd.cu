@@ -11,20 +11,25 @@
 // remainder, which keeps 16 bits; it runs at most four steps a head, so that costs next to nothing.
 //
 // Two kinds of CTA in one launch. A key CTA owns 128 keys of one key/value head and streams Q and dO in
-// steps of 64 queries over every query head that shares it (4 products a step); a query CTA owns 128
-// queries of one head and streams K and V in steps of 64 keys (3 products). Together 7 products where
+// steps of 128 queries over every query head that shares it (4 products a step); a query CTA owns 128
+// queries of one head and streams K and V in steps of 128 keys (3 products). Together 7 products where
 // the mathematics needs 5: S and dO V^T are formed twice, but no gradient is summed across CTAs, so
 // there are no atomics, no fp32 copy of dQ in memory, and the result does not depend on scheduling.
+// Steps of 64 (two score stages, N = 64 products) were measured at half the rate: an N = 64 product takes
+// the tensor pipe as long as one of N = 128 (bf16 [8,32,4096,128]: 9.6 ms).
 //
-// Both kinds have one row (a key or a query) per TMEM lane, two score stages, and the same roles:
-//   warps 0-3 / 4-7   even / odd steps: read S and dP (64 columns each), form P and dS, store them as
-//                     bf16 into the stage's S columns for the products that follow
-//   warp 8            issues the products:  S, dP of step i+2 after those that use P, dS of step i
+// Both kinds have one row (a key or a query) per TMEM lane and the same roles:
+//   warps 0-3 / 4-7   columns 0-63 / 64-127 of the scores: read S and dP, form P and dS, store them as
+//                     bf16 into TMEM, the A operand of the products that sum them
+//   warp 8            issues the products
 //   warp 9            fills the ring of streamed tiles by TMA
-// TMEM (512 columns): query CTA  Q 0-63, dO 64-127 (both as A operands), dQ 128-255, then per stage S and dP;
-// key CTA  dV 0-127, dK 128-255, S of both stages 256-383, dP 384-447, V 448-511 (A operand); K, the A
-// operand of S, is in shared memory. An A operand in TMEM halves what a product of 64 columns reads of
-// shared memory, which otherwise bounds it (6 KB a 16-wide step against 128 B a cycle).
+//
+// Key CTA.  TMEM: dV 0-127, dK 128-255, S 256-383 (P over it), dP 384-511 (dS over it). K and V are in
+// shared memory. Order of the products: dV(i), S(i+1), dK(i), dP(i+1); while the tensor pipe works on one
+// pair the warps work on the other: P(i+1) from S(i+1) during dK(i), dP(i+1), and dS(i) during dV(i), S(i+1).
+// Query CTA.  TMEM: dQ 0-127, S 128-255, dP 256-383, dS 384-447, dO 448-511 (A operand). Q is in shared
+// memory. S and dP of step j+1 are issued as soon as the warps hold step j in registers, dQ(j) when dS(j)
+// is stored: the exponentials of a step (1024 cycles of the special-function unit) run under the products.
 //
 // Every wait is bounded; one that runs out sets the attention fault bit and the CTA's abort flag, the
 // roles stop at their next wait and the outputs stay unwritten.
@@ -34,49 +39,56 @@ namespace nb200 {
 namespace {
 
 constexpr int kRows = 128;  // rows a CTA owns (= TMEM lanes)
-constexpr int kStep = 64;   // streamed rows a step
-constexpr int kStages = 5;  // ring of streamed tiles
-constexpr uint32_t kTileBytes = kStep * kDim * 2;  // 16 KB
+constexpr int kStep = 128;  // streamed rows a step
+constexpr int kStages = 5;  // ring of streamed tiles, which alternate K, V (or Q, dO)
+constexpr uint32_t kTileBytes = kStep * kDim * 2;  // 32 KB
 constexpr uint32_t kHalfBytes = kTileBytes / 2;    // 64 columns: the TMA box
 constexpr uint32_t kStatBytes = kStep * 4;         // one fp32 per streamed row
-constexpr uint32_t kStageBytes = 2 * kTileBytes + 1024;  // two tiles and two statistics rows
-constexpr uint32_t kFillBytes = 2 * kTileBytes;
-constexpr uint32_t kOwnBytes = 2 * kTileBytes;     // a key CTA's K tile: two halves of 128 rows
-constexpr uint32_t kOffOwn = 0;
-constexpr uint32_t kOffRing = kOffOwn + kOwnBytes;
-constexpr uint32_t kOffBar = kOffRing + kStages * kStageBytes;
+constexpr uint32_t kOffOwn = 0;                    // K and V of a key CTA, Q of a query CTA
+constexpr uint32_t kOffRing = kOffOwn + 2 * kTileBytes;
+constexpr uint32_t kOffStat = kOffRing + kStages * kTileBytes;  // two steps of two statistics rows
+constexpr uint32_t kOffBar = kOffStat + 2 * 2 * kStatBytes;
 constexpr int kMmaWarp = 8;
-constexpr int kThreads = 320;  // warp 9, the last, is the producer
+constexpr int kLoadWarp = 9;
+constexpr int kThreads = 384;  // warps 10-11 only complete the third warpgroup for the register split
+// Register split (setmaxnreg, per warpgroup), within what the block is launched with.
+constexpr int kLaunchRegs = 168;
+constexpr int kRegsSoftmax = 216;
+constexpr int kRegsControl = 72;
+static_assert(2 * 128 * kRegsSoftmax + 128 * kRegsControl <= kThreads * kLaunchRegs, "register split");
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kIdescScores = tc::idesc_bf16(128, kStep, false);
 constexpr uint32_t kIdescGrads = tc::idesc_bf16(128, kDim, true);
-// Query CTA: A operands, accumulator and stages.
-constexpr uint32_t kColQ = 0, kColDO = 64, kColDQ = 128, kColStageQ = 256;  // stage: S, then dP at + 64
-// Key CTA.
-constexpr uint32_t kColDV = 0, kColDK = 128, kColStageK = 256, kColDP = 384, kColV = 448;
+constexpr uint32_t kColDV = 0, kColDK = 128, kColKeyS = 256, kColKeyDP = 384;
+constexpr uint32_t kColDQ = 0, kColQueryS = 128, kColQueryDP = 256, kColDS = 384, kColDO = 448;
 
 struct Bars {
     uint64_t full[kStages];
     uint64_t empty[kStages];
-    uint64_t scores[2];   // S and dP of a stage are in TMEM
-    uint64_t grads[2];    // P and dS of a stage are in TMEM (one arrival per warp)
-    uint64_t dp_read;     // a key CTA's one dP buffer has been read (one arrival per warp)
-    uint64_t own;         // the CTA's own operands: K in shared memory
-    uint64_t own_tmem;    // ... and the A operands in TMEM (one arrival per warp)
+    uint64_t s_full;       // S is in TMEM (a query CTA: S and dP)
+    uint64_t dp_full;      // dP is in TMEM (key CTA)
+    uint64_t p_full[2];    // P of a column half is in TMEM (one arrival per warp)
+    uint64_t ds_full[2];   // dS of a column half
+    uint64_t read;         // a query CTA's S and dP are in registers (one arrival per warp)
+    uint64_t ds_free;      // a query CTA's dS has been consumed
+    uint64_t stat_full[2], stat_empty[2];  // statistics of a key CTA's step
+    uint64_t own;          // the CTA's own operands in shared memory
+    uint64_t own_tmem;     // ... and in TMEM (one arrival per warp)
     uint64_t done;
-    uint64_t tail;        // a streamed tile with masked rows, before it is published
+    uint64_t tail;         // a streamed tile with masked rows, before it is published
     uint32_t tmem_base;
     int abort;
 };
-constexpr uint32_t kSmemBytes = kOffBar + sizeof(Bars) + 1024;  // + alignment slack
+constexpr uint32_t kSmemBytes = kOffBar + sizeof(Bars);
+static_assert(kSmemBytes <= 232448, "shared memory of a CTA");
 
 struct BwdArgs {
-    int S, Spad, H, Hk, group, key_ctas, key_blocks, query_blocks, causal;
+    int S, Spad, H, Hk, group, key_ctas, blocks, causal;
     float scale, sl2;
     const int* lens;
-    const __nv_bfloat16 *q, *v, *go;
+    const __nv_bfloat16* go;
     __nv_bfloat16 *dq, *dk, *dv;
-    nb200_attn_strides sq, sv, sgo, sdq, sdk, sdv;
+    nb200_attn_strides sgo, sdq, sdk, sdv;
     const float* nlse2;   // [batch, heads, Spad]: -lse log2(e), -inf where the row sees nothing
     const float* ndelta;  // [batch, heads, Spad]: -delta
 };
@@ -129,8 +141,19 @@ __global__ void __launch_bounds__(kStatThreads) bwd_stats_kernel(StatArgs a) {
 }
 
 // ------------------------------------------------------------------ products
-// S-shaped product of a stage: 128 rows x kStep columns over the head dimension, eight K = 16 steps of
-// 32 bytes inside a half's 128-byte rows. A from TMEM.
+// Scores: 128 rows x 128 streamed rows over the head dimension, eight K = 16 steps of 32 bytes inside a
+// half's 128-byte rows. Both operands in shared memory, or A in TMEM (8 columns a step).
+__device__ __forceinline__ void scores_ss(uint32_t d, uint64_t a, uint64_t b) {
+    constexpr uint32_t h = kHalfBytes >> 4;
+    tc::mma_ss_at<0>(d, a, b, kIdescScores, 0u);
+    tc::mma_ss_at<2>(d, a, b, kIdescScores, 1u);
+    tc::mma_ss_at<4>(d, a, b, kIdescScores, 1u);
+    tc::mma_ss_at<6>(d, a, b, kIdescScores, 1u);
+    tc::mma_ss_at<h + 0>(d, a, b, kIdescScores, 1u);
+    tc::mma_ss_at<h + 2>(d, a, b, kIdescScores, 1u);
+    tc::mma_ss_at<h + 4>(d, a, b, kIdescScores, 1u);
+    tc::mma_ss_at<h + 6>(d, a, b, kIdescScores, 1u);
+}
 __device__ __forceinline__ void scores_ts(uint32_t d, uint32_t a, uint64_t b) {
     constexpr uint32_t h = kHalfBytes >> 4;
     tc::mma_ts_at<0, 0>(d, a, b, kIdescScores, 0u);
@@ -142,127 +165,118 @@ __device__ __forceinline__ void scores_ts(uint32_t d, uint32_t a, uint64_t b) {
     tc::mma_ts_at<48, h + 4>(d, a, b, kIdescScores, 1u);
     tc::mma_ts_at<56, h + 6>(d, a, b, kIdescScores, 1u);
 }
-// The same with A in shared memory (halves of 128 rows).
-__device__ __forceinline__ void scores_ss(uint32_t d, uint64_t a, uint64_t b) {
-    constexpr uint32_t h = kHalfBytes >> 4, g = kTileBytes >> 4;
-    tc::mma_ss_at<0, 0>(d, a, b, kIdescScores, 0u);
-    tc::mma_ss_at<2, 2>(d, a, b, kIdescScores, 1u);
-    tc::mma_ss_at<4, 4>(d, a, b, kIdescScores, 1u);
-    tc::mma_ss_at<6, 6>(d, a, b, kIdescScores, 1u);
-    tc::mma_ss_at<g + 0, h + 0>(d, a, b, kIdescScores, 1u);
-    tc::mma_ss_at<g + 2, h + 2>(d, a, b, kIdescScores, 1u);
-    tc::mma_ss_at<g + 4, h + 4>(d, a, b, kIdescScores, 1u);
-    tc::mma_ss_at<g + 6, h + 6>(d, a, b, kIdescScores, 1u);
-}
-// Gradient-shaped product: 128 rows x 128 head columns (+)= A[128, kStep] (bf16 in TMEM) * streamed tile,
-// read MN-major: 16 streamed rows = 2048 bytes a K = 16 step, the second 64 columns one half further.
-__device__ __forceinline__ void grads_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t acc) {
+// Half of a gradient product: 128 rows x 128 head columns (+)= A[128, 64] (bf16 in TMEM) * 64 rows of a
+// streamed tile, read MN-major: 16 streamed rows = 2048 bytes a K = 16 step.
+__device__ __forceinline__ void grads_ts(uint32_t d, uint32_t a, uint64_t tile, int half, uint32_t acc) {
+    const uint64_t b = tile + half * 512;
     tc::mma_ts_at<0, 0>(d, a, b, kIdescGrads, acc);
     tc::mma_ts_at<8, 128>(d, a, b, kIdescGrads, 1u);
     tc::mma_ts_at<16, 256>(d, a, b, kIdescGrads, 1u);
     tc::mma_ts_at<24, 384>(d, a, b, kIdescGrads, 1u);
 }
 
-// Descriptors of the streamed tiles in the ring: as K-major and as MN-major B operands.
+// Descriptors of the ring's tiles, as K-major and as MN-major B operands (the second 64 head columns one
+// half further).
 struct RingDesc {
-    uint64_t k, mn;
+    uint64_t k0, mn0;
     __device__ __forceinline__ explicit RingDesc(uint8_t* smem)
-        : k(tc::sw128_desc(smem_u32(smem + kOffRing), 16, 1024)),
-          mn(tc::sw128_desc(smem_u32(smem + kOffRing), kHalfBytes, 1024)) {}
-    // tile 0: K or Q, tile 1: V or dO
-    __device__ __forceinline__ static uint64_t step(int s, int tile) {
-        return (uint64_t)((s * kStageBytes + tile * kTileBytes) >> 4);
-    }
+        : k0(tc::sw128_desc(smem_u32(smem + kOffRing), 16, 1024)),
+          mn0(tc::sw128_desc(smem_u32(smem + kOffRing), kHalfBytes, 1024)) {}
+    __device__ __forceinline__ uint64_t k(int s) const { return k0 + ((s * kTileBytes) >> 4); }
+    __device__ __forceinline__ uint64_t mn(int s) const { return mn0 + ((s * kTileBytes) >> 4); }
 };
+
+// Waits for both column halves of an operand as they are stored and issues their half products.
+__device__ __forceinline__ bool grads(uint64_t* ready, uint32_t parity, uint32_t d, uint32_t a, uint32_t half_cols,
+                                      uint32_t lo, uint64_t tile, bool acc, bool pair, volatile int* abort) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        if (!wait_bar(&ready[h], parity, abort)) return false;
+        tc::fence_after();
+        grads_ts(d, a + h * half_cols, tile, h, acc || h ? 1u : 0u);
+        if (pair) grads_ts(d, lo + h * 64, tile, h, 1u);
+    }
+    return true;
+}
 
 __device__ __forceinline__ void issue_query(uint8_t* smem, Bars* b, uint32_t tmem, int n, bool pair) {
     volatile int* abort = &b->abort;
     const RingDesc rd(smem);
-    Ring<kStages> front, back;  // next tile for S and dP; next tile for dQ
-    bool ok = wait_bar(&b->own_tmem, 0, abort);
-    auto scores = [&](int st) {
-        if (!wait_bar(&b->full[front.s], front.ph, abort)) return false;
+    const uint64_t own = tc::sw128_desc(smem_u32(smem + kOffOwn), 16, 1024);
+    Ring<kStages> k, v, back;  // next K and V tile for S and dP; next K tile for dQ
+    v.next();
+    auto scores = [&]() {
+        if (!wait_bar(&b->full[k.s], k.ph, abort)) return false;
         tc::fence_after();
-        const uint32_t d = tmem + kColStageQ + 128 * st;
-        scores_ts(d, tmem + kColQ, rd.k + RingDesc::step(front.s, 0));
-        scores_ts(d + 64, tmem + kColDO, rd.k + RingDesc::step(front.s, 1));
-        tc::commit(&b->scores[st]);
-        front.next();
+        scores_ss(tmem + kColQueryS, own, rd.k(k.s));
+        if (!wait_bar(&b->full[v.s], v.ph, abort)) return false;
+        tc::fence_after();
+        scores_ts(tmem + kColQueryDP, tmem + kColDO, rd.k(v.s));
+        tc::commit(&b->s_full);
+        tc::commit(&b->empty[v.s]);
+        k.next(), k.next(), v.next(), v.next();
         return true;
     };
-    ok = ok && scores(0);
-    if (ok && n > 1) ok = scores(1);
+    bool ok = wait_bar(&b->own_tmem, 0, abort) && wait_bar(&b->own, 0, abort) && scores();
     for (int j = 0; ok && j < n; ++j) {
-        const int st = j & 1;
-        if (!(ok = wait_bar(&b->grads[st], (j >> 1) & 1u, abort))) break;
-        tc::fence_after();
-        const uint32_t ds = tmem + kColStageQ + 128 * st;
-        grads_ts(tmem + kColDQ, ds, rd.mn + RingDesc::step(back.s, 0), j > 0);
-        if (pair) grads_ts(tmem + kColDQ, ds + 32, rd.mn + RingDesc::step(back.s, 0), 1u);
+        const uint32_t ph = j & 1u;
+        if (j + 1 < n && !(ok = wait_bar(&b->read, ph, abort) && scores())) break;
+        if (!(ok = grads(b->ds_full, ph, tmem + kColDQ, tmem + kColDS, 32, tmem + kColQueryS, rd.mn(back.s), j > 0,
+                         pair, abort)))
+            break;
+        tc::commit(&b->ds_free);
         tc::commit(&b->empty[back.s]);
-        back.next();
-        if (j + 2 < n) ok = scores(st);
+        back.next(), back.next();
     }
     tc::commit(&b->done);
     drain_bar(&b->done, 0);
 }
 
-// With pairs the remainders of P and dS take the dP buffer, so the next dP waits for the products of this
-// step: S and dP of one step are issued at a time instead of two.
 __device__ __forceinline__ void issue_key(uint8_t* smem, Bars* b, uint32_t tmem, int n, bool pair) {
     volatile int* abort = &b->abort;
     const RingDesc rd(smem);
     const uint64_t own = tc::sw128_desc(smem_u32(smem + kOffOwn), 16, 1024);
-    Ring<kStages> front, back;
-    bool ok = wait_bar(&b->own_tmem, 0, abort) && wait_bar(&b->own, 0, abort);
-    // S and dP of step i; the one dP buffer is free once the warps have read step i - 1 out of it.
-    auto scores = [&](int i) {
-        if (!wait_bar(&b->full[front.s], front.ph, abort)) return false;
+    Ring<kStages> q, go;  // the tiles of this step; S and dP of the next step run one step ahead
+    go.next();
+    auto scores = [&](const Ring<kStages>& r, uint64_t a, uint32_t d, uint64_t* bar) {
+        if (!wait_bar(&b->full[r.s], r.ph, abort)) return false;
         tc::fence_after();
-        scores_ss(tmem + kColStageK + 64 * (i & 1), own, rd.k + RingDesc::step(front.s, 0));
-        if (i > 0 && !wait_bar(&b->dp_read, (i - 1) & 1u, abort)) return false;
-        tc::fence_after();
-        scores_ts(tmem + kColDP, tmem + kColV, rd.k + RingDesc::step(front.s, 1));
-        tc::commit(&b->scores[i & 1]);
-        front.next();
+        scores_ss(d, a, rd.k(r.s));
+        tc::commit(bar);
         return true;
     };
-    const int ahead = pair ? 1 : 2;
-    ok = ok && scores(0);
-    if (ok && n > 1 && !pair) ok = scores(1);
+    const uint32_t s = tmem + kColKeyS, dp = tmem + kColKeyDP;
+    const uint64_t own_v = own + (kTileBytes >> 4);
+    bool ok = wait_bar(&b->own, 0, abort) && scores(q, own, s, &b->s_full) && scores(go, own_v, dp, &b->dp_full);
     for (int i = 0; ok && i < n; ++i) {
-        const int st = i & 1;
-        if (!(ok = wait_bar(&b->grads[st], (i >> 1) & 1u, abort))) break;
-        tc::fence_after();
-        const uint32_t p = tmem + kColStageK + 64 * st;
-        grads_ts(tmem + kColDV, p, rd.mn + RingDesc::step(back.s, 1), i > 0);
-        grads_ts(tmem + kColDK, p + 32, rd.mn + RingDesc::step(back.s, 0), i > 0);
-        if (pair) {
-            grads_ts(tmem + kColDV, tmem + kColDP, rd.mn + RingDesc::step(back.s, 1), 1u);
-            grads_ts(tmem + kColDK, tmem + kColDP + 32, rd.mn + RingDesc::step(back.s, 0), 1u);
-        }
-        tc::commit(&b->empty[back.s]);
-        back.next();
-        if (i + ahead < n) ok = scores(i + ahead);
+        const uint32_t ph = i & 1u;
+        const bool more = i + 1 < n;
+        Ring<kStages> q1 = q, go1 = go;
+        q1.next(), q1.next(), go1.next(), go1.next();
+        if (!(ok = grads(b->p_full, ph, tmem + kColDV, s, 64, s + 32, rd.mn(go.s), i > 0, pair, abort))) break;
+        tc::commit(&b->empty[go.s]);
+        if (more && !(ok = scores(q1, own, s, &b->s_full))) break;
+        if (!(ok = grads(b->ds_full, ph, tmem + kColDK, dp, 64, dp + 32, rd.mn(q.s), i > 0, pair, abort))) break;
+        tc::commit(&b->empty[q.s]);
+        if (more && !(ok = scores(go1, own_v, dp, &b->dp_full))) break;
+        q = q1;
+        go = go1;
     }
     tc::commit(&b->done);
     drain_bar(&b->done, 0);
 }
 
 // ------------------------------------------------------------------ the CTA's own operands
-// One row of 128 bf16 per lane into 64 TMEM columns (two elements a column); zeros without a row.
+// 64 bf16 of a row per lane into 32 TMEM columns (two elements a column); zeros without a row.
 __device__ __forceinline__ void own_row(uint32_t col, const __nv_bfloat16* row) {
+    uint32_t w[32];
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-        uint32_t w[32];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const uint4 u = row ? ld_keep(row + 64 * c + 8 * i) : make_uint4(0u, 0u, 0u, 0u);
-            w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
-        }
-        __syncwarp();
-        tc::tmem_st32(col + 32 * c, w);
+    for (int i = 0; i < 8; ++i) {
+        const uint4 u = row ? ld_keep(row + 8 * i) : make_uint4(0u, 0u, 0u, 0u);
+        w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
     }
+    __syncwarp();
+    tc::tmem_st32(col, w);
 }
 
 // kCols accumulator columns of this lane's row, times `scale`, to `row` as bf16 (zeros if the row is
@@ -311,24 +325,24 @@ __device__ __forceinline__ void query_warps(Bars* b, uint32_t tmem, const BwdArg
     const int row = q0 + (warp & 3) * 32 + lane;
     const bool live = row < len;
     const uint32_t t = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const __nv_bfloat16* src = half ? a.go + offset(a.sgo, batch, head, row) : a.q + offset(a.sq, batch, head, row);
-    own_row(t + (half ? kColDO : kColQ), live ? src : nullptr);
+    own_row(t + kColDO + 32 * half, live ? a.go + offset(a.sgo, batch, head, row) + 64 * half : nullptr);
     tc::tmem_wait_st();
     publish(&b->own_tmem, lane);
     const int64_t stat = ((int64_t)batch * a.H + head) * a.Spad + row;
     const float nl = live ? a.nlse2[stat] : -NB200_INF, nd = live ? a.ndelta[stat] : 0.f;
     const uint64_t nl2 = f2(nl, nl), nd2 = f2(nd, nd), sl2 = f2(a.sl2, a.sl2);
-    const int lim = a.causal ? min(row, len - 1) : len - 1;  // last key this row sees
-    const uint32_t tS = t + kColStageQ + 128 * half;
+    const int lim = (a.causal ? min(row, len - 1) : len - 1) - 64 * half;  // last key this row sees, from column 0 on
+    const uint32_t tS = t + kColQueryS + 64 * half, tDS = t + kColDS + 32 * half;
     bool ok = true;
-    for (int j = half; j < n; j += 2) {
-        if (!(ok = __all_sync(0xffffffffu, wait_bar(&b->scores[half], (j >> 1) & 1u, abort)))) break;
+    for (int j = 0; j < n; ++j) {
+        if (!(ok = __all_sync(0xffffffffu, wait_bar(&b->s_full, j & 1u, abort)))) break;
         tc::fence_after();
         uint32_t s[64], d[64];
         tc::tmem_ld64(tS, s);
-        tc::tmem_ld64(tS + 64, d);
+        tc::tmem_ld64(tS + (kColQueryDP - kColQueryS), d);
+        publish(&b->read, lane);
         const int room = lim - j * kStep;  // columns past it are masked
-        if (__any_sync(0xffffffffu, room < kStep - 1)) {
+        if (__any_sync(0xffffffffu, room < 63)) {
 #pragma unroll
             for (int c = 0; c < 64; ++c)
                 if (c > room) s[c] = __float_as_uint(-NB200_INF);
@@ -341,10 +355,12 @@ __device__ __forceinline__ void query_warps(Bars* b, uint32_t tmem, const BwdArg
             const uint64_t g = mul2(p, add2(f2(__uint_as_float(d[2 * c]), __uint_as_float(d[2 * c + 1])), nd2));
             round_pair<kPair>(g, w[c], lo[c]);
         }
-        tc::tmem_st32(tS, w);
-        if constexpr (kPair) tc::tmem_st32(tS + 32, lo);
+        if (j > 0 && !(ok = __all_sync(0xffffffffu, wait_bar(&b->ds_free, (j - 1) & 1u, abort)))) break;
+        tc::tmem_st32(tDS, w);
+        // Remainders go over S: a CTA that has them runs one step, so no further S is on its way.
+        if constexpr (kPair) tc::tmem_st32(tS, lo);
         tc::tmem_wait_st();
-        publish(&b->grads[half], lane);
+        publish(&b->ds_full[half], lane);
     }
     if (ok) ok = __all_sync(0xffffffffu, wait_bar(&b->done, 0, abort));
     if (!ok) return;
@@ -361,59 +377,57 @@ __device__ __forceinline__ void key_warps(uint8_t* smem, Bars* b, uint32_t tmem,
     const int row = k0 + (warp & 3) * 32 + lane;
     const bool live = row < len;
     const uint32_t t = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    if (half == 0) {
-        own_row(t + kColV, live ? a.v + offset(a.sv, batch, head, row) : nullptr);
-        tc::tmem_wait_st();
-    }
-    publish(&b->own_tmem, lane);
     const uint64_t sl2 = f2(a.sl2, a.sl2);
-    const uint32_t tS = t + kColStageK + 64 * half;
-    Ring<kStages> r;
-    if (half) r.next();
+    const uint32_t tS = t + kColKeyS + 64 * half, tDP = t + kColKeyDP + 64 * half;
     bool ok = true;
-    int step = first + half;  // query step inside its head
-    for (int i = half; i < n; i += 2, step += 2) {
-        while (step >= first + per_head) step -= per_head;
-        ok = wait_bar(&b->scores[half], (i >> 1) & 1u, abort) && wait_bar(&b->full[r.s], r.ph, abort);
+    for (int i = 0, step = first; i < n; ++i) {
+        const uint32_t ph = i & 1u;
+        ok = wait_bar(&b->s_full, ph, abort) && wait_bar(&b->stat_full[ph], (i >> 1) & 1u, abort);
         if (!(ok = __all_sync(0xffffffffu, ok))) break;
         tc::fence_after();
-        uint32_t s[64], d[64];
-        tc::tmem_ld64(t + kColDP, d);
-        publish(&b->dp_read, lane);
+        const float4* nl = reinterpret_cast<const float4*>(smem + kOffStat + ph * 2 * kStatBytes) + 16 * half;
+        const float4* nd = nl + kStep / 4;
+        uint32_t s[64], w[32], lo[32];
         tc::tmem_ld64(tS, s);
-        const int hidden = a.causal ? row - step * kStep : 0;  // columns before it are masked
+        const int hidden = a.causal ? row - step * kStep - 64 * half : 0;  // columns before it are masked
         if (__any_sync(0xffffffffu, hidden > 0)) {
 #pragma unroll
             for (int c = 0; c < 64; ++c)
                 if (c < hidden) s[c] = __float_as_uint(-NB200_INF);
         }
-        const float4* nl = reinterpret_cast<const float4*>(smem + kOffRing + r.s * kStageBytes + 2 * kTileBytes);
-        const float4* nd = nl + kStep / 4;
-        uint32_t w[32], plo[32], wlo[32];
 #pragma unroll
-        for (int c = 0; c < 16; ++c) {
-            const float4 l4 = nl[c], d4 = nd[c];
-            const uint64_t l2[2] = {f2(l4.x, l4.y), f2(l4.z, l4.w)}, e2[2] = {f2(d4.x, d4.y), f2(d4.z, d4.w)};
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int k = 4 * c + 2 * e;
-                const uint64_t x = fma2(f2(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), sl2, l2[e]);
-                const uint64_t p = f2(ex2_ftz(f2lo(x)), ex2_ftz(f2hi(x)));
-                const uint64_t g = mul2(p, add2(f2(__uint_as_float(d[k]), __uint_as_float(d[k + 1])), e2[e]));
-                round_pair<kPair>(p, s[k / 2], plo[k / 2]);
-                round_pair<kPair>(g, w[k / 2], wlo[k / 2]);
-            }
+        for (int c = 0; c < 32; ++c) {
+            const float4 l4 = nl[c / 2];
+            const uint64_t l2 = c & 1 ? f2(l4.z, l4.w) : f2(l4.x, l4.y);
+            const uint64_t x = fma2(f2(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1])), sl2, l2);
+            const uint64_t p = f2(ex2_ftz(f2lo(x)), ex2_ftz(f2hi(x)));
+            s[2 * c] = __float_as_uint(f2lo(p));
+            s[2 * c + 1] = __float_as_uint(f2hi(p));
+            round_pair<kPair>(p, w[c], lo[c]);
         }
-        tc::tmem_st32(tS, s);
-        tc::tmem_st32(tS + 32, w);
-        if constexpr (kPair) {
-            tc::tmem_st32(t + kColDP, plo);
-            tc::tmem_st32(t + kColDP + 32, wlo);
-        }
+        tc::tmem_st32(tS, w);
+        if constexpr (kPair) tc::tmem_st32(tS + 32, lo);
         tc::tmem_wait_st();
-        publish(&b->grads[half], lane);
-        r.next();
-        r.next();
+        publish(&b->p_full[half], lane);
+
+        if (!(ok = __all_sync(0xffffffffu, wait_bar(&b->dp_full, ph, abort)))) break;
+        tc::fence_after();
+        uint32_t d[64];
+        tc::tmem_ld64(tDP, d);
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+            const float4 d4 = nd[c / 2];
+            const uint64_t nd2 = c & 1 ? f2(d4.z, d4.w) : f2(d4.x, d4.y);
+            const uint64_t p = f2(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1]));
+            const uint64_t g = mul2(p, add2(f2(__uint_as_float(d[2 * c]), __uint_as_float(d[2 * c + 1])), nd2));
+            round_pair<kPair>(g, w[c], lo[c]);
+        }
+        tc::tmem_st32(tDP, w);
+        if constexpr (kPair) tc::tmem_st32(tDP + 32, lo);
+        tc::tmem_wait_st();
+        publish(&b->ds_full[half], lane);
+        if (lane == 0) mbar_arrive(&b->stat_empty[ph]);
+        if (++step == first + per_head) step = first;
     }
     if (ok) ok = __all_sync(0xffffffffu, wait_bar(&b->done, 0, abort));
     if (!ok) return;
@@ -424,59 +438,69 @@ __device__ __forceinline__ void key_warps(uint8_t* smem, Bars* b, uint32_t tmem,
 }
 
 // ------------------------------------------------------------------ producer (a whole warp; lane 0 issues)
-// Streams n tile pairs: steps first .. first + per_head - 1 of heads head0, head0 + 1, ... Rows past the
-// sequence in a head's last step are zeroed before the step is published (`tail` rows remain; 0: none
+__device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* m, int row, int head, int batch,
+                                          uint64_t* bar) {
+    tc::tma_load_4d(dst, m, 0, row, head, batch, bar);
+    tc::tma_load_4d(dst + kHalfBytes, m, kDim / 2, row, head, batch, bar);
+}
+
+// Streams n steps of two tiles: steps first .. first + per_head - 1 of heads head0, head0 + 1, ... Rows past
+// the sequence in a head's last step are zeroed before the tile is published (`tail` rows remain; 0: none
 // to zero): they enter sums over the streamed rows, where a coefficient of 0 times an infinity or NaN
-// would still poison the result. With statistics (a key CTA) their two rows come along.
+// would still poison the result. A key CTA's steps come with their rows' statistics.
 __device__ __forceinline__ void produce(const CUtensorMap* mx, const CUtensorMap* my, uint8_t* smem, Bars* b,
-                                        int batch, int head0, int first, int per_head, int n, int tail,
-                                        const float* nlse2, const float* ndelta, const BwdArgs& a, int lane) {
+                                        int batch, int head0, int first, int per_head, int n, int tail, bool stats,
+                                        const BwdArgs& a, int lane) {
     volatile int* abort = &b->abort;
     Ring<kStages> r;
     int it = 0, head = head0, step = first;
     uint32_t tail_ph = 0;
     bool ok = true;
-    for (; it < n; ++it, r.next()) {
-        ok = __all_sync(0xffffffffu, lane != 0 || wait_bar(&b->empty[r.s], r.ph ^ 1u, abort));
-        if (!ok) break;
-        uint8_t* dst = smem + kOffRing + r.s * kStageBytes;
-        const bool cut = tail && step == first + per_head - 1;
+    for (; it < 2 * n; ++it, r.next()) {
+        const int i = it >> 1;
+        const bool second = it & 1, cut = tail && step == first + per_head - 1;
+        ok = lane != 0 || wait_bar(&b->empty[r.s], r.ph ^ 1u, abort);
+        if (ok && lane == 0 && stats && !second) ok = wait_bar(&b->stat_empty[i & 1], ((i >> 1) & 1u) ^ 1u, abort);
+        if (!(ok = __all_sync(0xffffffffu, ok))) break;
+        uint8_t* dst = smem + kOffRing + r.s * kTileBytes;
         if (lane == 0) {
             uint64_t* bar = cut ? &b->tail : &b->full[r.s];
-            mbar_expect_tx(bar, kFillBytes + (nlse2 ? 2 * kStatBytes : 0));
-            const int row = step * kStep;
-            tc::tma_load_4d(dst, mx, 0, row, head, batch, bar);
-            tc::tma_load_4d(dst + kHalfBytes, mx, kDim / 2, row, head, batch, bar);
-            tc::tma_load_4d(dst + kTileBytes, my, 0, row, head, batch, bar);
-            tc::tma_load_4d(dst + kTileBytes + kHalfBytes, my, kDim / 2, row, head, batch, bar);
-            if (nlse2) {
-                const int64_t at = ((int64_t)batch * a.H + head) * a.Spad + row;
-                bulk_load(dst + 2 * kTileBytes, nlse2 + at, kStatBytes, bar);
-                bulk_load(dst + 2 * kTileBytes + kStatBytes, ndelta + at, kStatBytes, bar);
+            mbar_expect_tx(bar, kTileBytes);
+            load_tile(dst, second ? my : mx, step * kStep, head, batch, bar);
+            if (stats && !second) {
+                const int64_t at = ((int64_t)batch * a.H + head) * a.Spad + step * kStep;
+                uint8_t* to = smem + kOffStat + (i & 1) * 2 * kStatBytes;
+                mbar_expect_tx(&b->stat_full[i & 1], 2 * kStatBytes);
+                bulk_load(to, a.nlse2 + at, kStatBytes, &b->stat_full[i & 1]);
+                bulk_load(to + kStatBytes, a.ndelta + at, kStatBytes, &b->stat_full[i & 1]);
             }
         }
         if (cut) {
-            ok = __all_sync(0xffffffffu, wait_bar(&b->tail, tail_ph, abort));
-            if (!ok) break;
+            if (!(ok = __all_sync(0xffffffffu, wait_bar(&b->tail, tail_ph, abort)))) {
+                if (lane == 0) drain_bar(&b->tail, tail_ph);
+                break;
+            }
             tail_ph ^= 1u;
             zero_tail(dst, kStep, tail, lane);
-            zero_tail(dst + kTileBytes, kStep, tail, lane);
             __syncwarp();
             if (lane == 0) mbar_arrive(&b->full[r.s]);
         }
-        if (++step == first + per_head) {
+        if (second && ++step == first + per_head) {
             step = first;
             ++head;
         }
     }
     // Every copy lands before the CTA may exit.
-    if (lane == 0)
+    if (lane == 0) {
         for (int s = 0; s < kStages && s < it; ++s) drain_bar(&b->full[s], ((it - 1 - s) / kStages) & 1u);
+        const int steps = (it + 1) / 2;
+        for (int s = 0; stats && s < 2 && s < steps; ++s) drain_bar(&b->stat_full[s], ((steps - 1 - s) / 2) & 1u);
+        drain_bar(&b->own, 0);
+    }
 }
 
 __global__ void __launch_bounds__(kThreads, 1) attn_bwd_kernel(const __grid_constant__ Maps m, const BwdArgs a) {
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    extern __shared__ __align__(1024) uint8_t smem[];
     Bars* b = reinterpret_cast<Bars*>(smem + kOffBar);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -484,7 +508,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_kernel(const __grid_cons
     // through L2; under a causal mask the longest of a head come first.
     const bool keys = (int)blockIdx.x < a.key_ctas;
     const int id = keys ? blockIdx.x : blockIdx.x - a.key_ctas;
-    const int blocks = keys ? a.key_blocks : a.query_blocks, heads = keys ? a.Hk : a.H;
+    const int blocks = a.blocks, heads = keys ? a.Hk : a.H;
     const int batch = id / blocks / heads, head = id / blocks % heads;
     const int row0 = (keys ? id % blocks : blocks - 1 - id % blocks) * kRows;
 
@@ -494,15 +518,22 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_kernel(const __grid_cons
             mbar_init(&b->empty[s], 1);
         }
         for (int s = 0; s < 2; ++s) {
-            mbar_init(&b->scores[s], 1);
-            mbar_init(&b->grads[s], 4);
+            mbar_init(&b->p_full[s], 4);
+            mbar_init(&b->ds_full[s], 4);
+            mbar_init(&b->stat_full[s], 1);
+            mbar_init(&b->stat_empty[s], 8);
         }
-        mbar_init(&b->dp_read, 4);
+        mbar_init(&b->s_full, 1);
+        mbar_init(&b->dp_full, 1);
+        mbar_init(&b->read, 8);
+        mbar_init(&b->ds_free, 1);
         mbar_init(&b->own, 1);
         mbar_init(&b->own_tmem, 8);
         mbar_init(&b->done, 1);
         mbar_init(&b->tail, 1);
-        b->abort = 0;
+        // The swizzled tiles need 1024-byte alignment; a base without it would compute nonsense.
+        b->abort = (smem_u32(smem) & 1023u) != 0;
+        if (b->abort) atomicOr(&g_attn_fault, 2u);
         fence_barrier_init();
         tc::prefetch_map(&m.q);
         tc::prefetch_map(&m.k);
@@ -542,32 +573,34 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_kernel(const __grid_cons
     __syncthreads();
     tc::fence_after();
     const uint32_t tmem = b->tmem_base;
-
-    if (warp < 8) {
+    if (b->abort) {
+        // nothing was issued
+    } else if (warp < 8) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
         if (keys && pair) key_warps<true>(smem, b, tmem, a, batch, head, len, row0, first, per_head, n);
         else if (keys) key_warps<false>(smem, b, tmem, a, batch, head, len, row0, first, per_head, n);
         else if (pair) query_warps<true>(b, tmem, a, batch, head, len, row0, n);
         else query_warps<false>(b, tmem, a, batch, head, len, row0, n);
-    } else if (warp == kMmaWarp) {
-        if (lane == 0) {
-            if (keys) issue_key(smem, b, tmem, n, pair);
-            else issue_query(smem, b, tmem, n, pair);
-        }
-    } else if (keys) {
-        if (lane == 0) {
-            uint8_t* own = smem + kOffOwn;
-            mbar_expect_tx(&b->own, kOwnBytes);
-            for (int h = 0; h < 2; ++h)
-                for (int r = 0; r < 2; ++r)
-                    tc::tma_load_4d(own + h * kTileBytes + r * kHalfBytes, &m.k, h * kDim / 2, row0 + r * kStep, head,
-                                    batch, &b->own);
-        }
-        produce(&m.q, &m.go, smem, b, batch, head * a.group, first, per_head, n, tail, a.nlse2, a.ndelta, a, lane);
-        if (lane == 0) drain_bar(&b->own, 0);
     } else {
-        produce(&m.k, &m.v, smem, b, batch, head / a.group, 0, per_head, n, tail, nullptr, nullptr, a, lane);
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));
+        if (warp == kMmaWarp) {
+            if (lane == 0) {
+                if (keys) issue_key(smem, b, tmem, n, pair);
+                else issue_query(smem, b, tmem, n, pair);
+            }
+        } else if (warp == kLoadWarp) {
+            if (lane == 0) {
+                uint8_t* own = smem + kOffOwn;
+                mbar_expect_tx(&b->own, keys ? 2 * kTileBytes : kTileBytes);
+                load_tile(own, keys ? &m.k : &m.q, row0, head, batch, &b->own);
+                if (keys) load_tile(own + kTileBytes, &m.v, row0, head, batch, &b->own);
+            }
+            __syncwarp();
+            if (keys) produce(&m.q, &m.go, smem, b, batch, head * a.group, first, per_head, n, tail, true, a, lane);
+            else produce(&m.k, &m.v, smem, b, batch, head / a.group, 0, per_head, n, tail, false, a, lane);
+        }
+        __syncwarp();
     }
-    __syncwarp();
     tc::fence_before();
     __syncthreads();
     if (warp == kMmaWarp) {
@@ -629,19 +662,15 @@ int launch_attention_bwd(const nb200_attn_args& n, const nb200_attn_strides* str
     a.Hk = (int)n.kv_heads;
     a.group = (int)(n.heads / n.kv_heads);
     a.key_ctas = (int)(n.batch * n.kv_heads * blocks);
-    a.key_blocks = a.query_blocks = (int)blocks;
+    a.blocks = (int)blocks;
     a.causal = n.causal ? 1 : 0;
     a.scale = n.scale;
     a.sl2 = n.scale * 1.4426950408889634f;
     a.lens = n.seq_lens;
-    a.q = static_cast<const B*>(q);
-    a.v = static_cast<const B*>(v);
     a.go = static_cast<const B*>(grad_o);
     a.dq = static_cast<B*>(dq);
     a.dk = static_cast<B*>(dk);
     a.dv = static_cast<B*>(dv);
-    a.sq = strides[0];
-    a.sv = strides[2];
     a.sgo = strides[4];
     a.sdq = strides[5];
     a.sdk = strides[6];
