@@ -40,13 +40,18 @@ namespace {
 
 constexpr int kRows = 128;  // rows a CTA owns (= TMEM lanes)
 constexpr int kStep = 128;  // streamed rows a step
-constexpr int kStages = 5;  // ring of streamed tiles, which alternate K, V (or Q, dO)
+// Rings of streamed tiles, which alternate K, V (or Q, dO): what the CTA's own operands leave of the
+// shared memory. A query CTA needs six: V(j+1) would otherwise wait for K(j-1), that is for dQ(j-1).
+constexpr int kKeyStages = 5;
+constexpr int kQueryStages = 6;
 constexpr uint32_t kTileBytes = kStep * kDim * 2;  // 32 KB
 constexpr uint32_t kHalfBytes = kTileBytes / 2;    // 64 columns: the TMA box
 constexpr uint32_t kStatBytes = kStep * 4;         // one fp32 per streamed row
-constexpr uint32_t kOffOwn = 0;                    // K and V of a key CTA, Q of a query CTA
-constexpr uint32_t kOffRing = kOffOwn + 2 * kTileBytes;
-constexpr uint32_t kOffStat = kOffRing + kStages * kTileBytes;  // two steps of two statistics rows
+constexpr uint32_t kOffOwn = 0;  // K and V of a key CTA, Q of a query CTA; the ring follows
+constexpr uint32_t kOffKeyRing = kOffOwn + 2 * kTileBytes;
+constexpr uint32_t kOffQueryRing = kOffOwn + kTileBytes;
+constexpr uint32_t kOffStat = kOffKeyRing + kKeyStages * kTileBytes;  // two steps of two statistics rows
+static_assert(kOffQueryRing + kQueryStages * kTileBytes == kOffStat, "rings end together");
 constexpr uint32_t kOffBar = kOffStat + 2 * 2 * kStatBytes;
 constexpr int kMmaWarp = 8;
 constexpr int kLoadWarp = 9;
@@ -63,8 +68,8 @@ constexpr uint32_t kColDV = 0, kColDK = 128, kColKeyS = 256, kColKeyDP = 384;
 constexpr uint32_t kColDQ = 0, kColQueryS = 128, kColQueryDP = 256, kColDS = 384, kColDO = 448;
 
 struct Bars {
-    uint64_t full[kStages];
-    uint64_t empty[kStages];
+    uint64_t full[kQueryStages];
+    uint64_t empty[kQueryStages];
     uint64_t s_full;       // S is in TMEM (a query CTA: S and dP)
     uint64_t dp_full;      // dP is in TMEM (key CTA)
     uint64_t p_full[2];    // P of a column half is in TMEM (one arrival per warp)
@@ -179,9 +184,8 @@ __device__ __forceinline__ void grads_ts(uint32_t d, uint32_t a, uint64_t tile, 
 // half further).
 struct RingDesc {
     uint64_t k0, mn0;
-    __device__ __forceinline__ explicit RingDesc(uint8_t* smem)
-        : k0(tc::sw128_desc(smem_u32(smem + kOffRing), 16, 1024)),
-          mn0(tc::sw128_desc(smem_u32(smem + kOffRing), kHalfBytes, 1024)) {}
+    __device__ __forceinline__ explicit RingDesc(uint8_t* ring)
+        : k0(tc::sw128_desc(smem_u32(ring), 16, 1024)), mn0(tc::sw128_desc(smem_u32(ring), kHalfBytes, 1024)) {}
     __device__ __forceinline__ uint64_t k(int s) const { return k0 + ((s * kTileBytes) >> 4); }
     __device__ __forceinline__ uint64_t mn(int s) const { return mn0 + ((s * kTileBytes) >> 4); }
 };
@@ -201,9 +205,9 @@ __device__ __forceinline__ bool grads(uint64_t* ready, uint32_t parity, uint32_t
 
 __device__ __forceinline__ void issue_query(uint8_t* smem, Bars* b, uint32_t tmem, int n, bool pair) {
     volatile int* abort = &b->abort;
-    const RingDesc rd(smem);
+    const RingDesc rd(smem + kOffQueryRing);
     const uint64_t own = tc::sw128_desc(smem_u32(smem + kOffOwn), 16, 1024);
-    Ring<kStages> k, v, back;  // next K and V tile for S and dP; next K tile for dQ
+    Ring<kQueryStages> k, v, back;  // next K and V tile for S and dP; next K tile for dQ
     v.next();
     auto scores = [&]() {
         if (!wait_bar(&b->full[k.s], k.ph, abort)) return false;
@@ -234,11 +238,11 @@ __device__ __forceinline__ void issue_query(uint8_t* smem, Bars* b, uint32_t tme
 
 __device__ __forceinline__ void issue_key(uint8_t* smem, Bars* b, uint32_t tmem, int n, bool pair) {
     volatile int* abort = &b->abort;
-    const RingDesc rd(smem);
+    const RingDesc rd(smem + kOffKeyRing);
     const uint64_t own = tc::sw128_desc(smem_u32(smem + kOffOwn), 16, 1024);
-    Ring<kStages> q, go;  // the tiles of this step; S and dP of the next step run one step ahead
+    Ring<kKeyStages> q, go;  // the tiles of this step; S and dP of the next step run one step ahead
     go.next();
-    auto scores = [&](const Ring<kStages>& r, uint64_t a, uint32_t d, uint64_t* bar) {
+    auto scores = [&](const Ring<kKeyStages>& r, uint64_t a, uint32_t d, uint64_t* bar) {
         if (!wait_bar(&b->full[r.s], r.ph, abort)) return false;
         tc::fence_after();
         scores_ss(d, a, rd.k(r.s));
@@ -251,7 +255,7 @@ __device__ __forceinline__ void issue_key(uint8_t* smem, Bars* b, uint32_t tmem,
     for (int i = 0; ok && i < n; ++i) {
         const uint32_t ph = i & 1u;
         const bool more = i + 1 < n;
-        Ring<kStages> q1 = q, go1 = go;
+        Ring<kKeyStages> q1 = q, go1 = go;
         q1.next(), q1.next(), go1.next(), go1.next();
         if (!(ok = grads(b->p_full, ph, tmem + kColDV, s, 64, s + 32, rd.mn(go.s), i > 0, pair, abort))) break;
         tc::commit(&b->empty[go.s]);
@@ -396,14 +400,18 @@ __device__ __forceinline__ void key_warps(uint8_t* smem, Bars* b, uint32_t tmem,
                 if (c < hidden) s[c] = __float_as_uint(-NB200_INF);
         }
 #pragma unroll
-        for (int c = 0; c < 32; ++c) {
+        for (int c = 0; c < 32; c += 2) {
             const float4 l4 = nl[c / 2];
-            const uint64_t l2 = c & 1 ? f2(l4.z, l4.w) : f2(l4.x, l4.y);
-            const uint64_t x = fma2(f2(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1])), sl2, l2);
-            const uint64_t p = f2(ex2_ftz(f2lo(x)), ex2_ftz(f2hi(x)));
-            s[2 * c] = __float_as_uint(f2lo(p));
-            s[2 * c + 1] = __float_as_uint(f2hi(p));
-            round_pair<kPair>(p, w[c], lo[c]);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int k = 2 * (c + e);
+                const uint64_t x = fma2(f2(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), sl2,
+                                        e ? f2(l4.z, l4.w) : f2(l4.x, l4.y));
+                const uint64_t p = f2(ex2_ftz(f2lo(x)), ex2_ftz(f2hi(x)));
+                s[k] = __float_as_uint(f2lo(p));
+                s[k + 1] = __float_as_uint(f2hi(p));
+                round_pair<kPair>(p, w[c + e], lo[c + e]);
+            }
         }
         tc::tmem_st32(tS, w);
         if constexpr (kPair) tc::tmem_st32(tS + 32, lo);
@@ -415,12 +423,16 @@ __device__ __forceinline__ void key_warps(uint8_t* smem, Bars* b, uint32_t tmem,
         uint32_t d[64];
         tc::tmem_ld64(tDP, d);
 #pragma unroll
-        for (int c = 0; c < 32; ++c) {
+        for (int c = 0; c < 32; c += 2) {
             const float4 d4 = nd[c / 2];
-            const uint64_t nd2 = c & 1 ? f2(d4.z, d4.w) : f2(d4.x, d4.y);
-            const uint64_t p = f2(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1]));
-            const uint64_t g = mul2(p, add2(f2(__uint_as_float(d[2 * c]), __uint_as_float(d[2 * c + 1])), nd2));
-            round_pair<kPair>(g, w[c], lo[c]);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int k = 2 * (c + e);
+                const uint64_t p = f2(__uint_as_float(s[k]), __uint_as_float(s[k + 1]));
+                const uint64_t g = mul2(p, add2(f2(__uint_as_float(d[k]), __uint_as_float(d[k + 1])),
+                                                e ? f2(d4.z, d4.w) : f2(d4.x, d4.y)));
+                round_pair<kPair>(g, w[c + e], lo[c + e]);
+            }
         }
         tc::tmem_st32(tDP, w);
         if constexpr (kPair) tc::tmem_st32(tDP + 32, lo);
@@ -448,9 +460,11 @@ __device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* m, in
 // the sequence in a head's last step are zeroed before the tile is published (`tail` rows remain; 0: none
 // to zero): they enter sums over the streamed rows, where a coefficient of 0 times an infinity or NaN
 // would still poison the result. A key CTA's steps come with their rows' statistics.
+template <bool kKeys>
 __device__ __forceinline__ void produce(const CUtensorMap* mx, const CUtensorMap* my, uint8_t* smem, Bars* b,
-                                        int batch, int head0, int first, int per_head, int n, int tail, bool stats,
+                                        int batch, int head0, int first, int per_head, int n, int tail,
                                         const BwdArgs& a, int lane) {
+    constexpr int kStages = kKeys ? kKeyStages : kQueryStages;
     volatile int* abort = &b->abort;
     Ring<kStages> r;
     int it = 0, head = head0, step = first;
@@ -460,14 +474,14 @@ __device__ __forceinline__ void produce(const CUtensorMap* mx, const CUtensorMap
         const int i = it >> 1;
         const bool second = it & 1, cut = tail && step == first + per_head - 1;
         ok = lane != 0 || wait_bar(&b->empty[r.s], r.ph ^ 1u, abort);
-        if (ok && lane == 0 && stats && !second) ok = wait_bar(&b->stat_empty[i & 1], ((i >> 1) & 1u) ^ 1u, abort);
+        if (kKeys && ok && lane == 0 && !second) ok = wait_bar(&b->stat_empty[i & 1], ((i >> 1) & 1u) ^ 1u, abort);
         if (!(ok = __all_sync(0xffffffffu, ok))) break;
-        uint8_t* dst = smem + kOffRing + r.s * kTileBytes;
+        uint8_t* dst = smem + (kKeys ? kOffKeyRing : kOffQueryRing) + r.s * kTileBytes;
         if (lane == 0) {
             uint64_t* bar = cut ? &b->tail : &b->full[r.s];
             mbar_expect_tx(bar, kTileBytes);
             load_tile(dst, second ? my : mx, step * kStep, head, batch, bar);
-            if (stats && !second) {
+            if (kKeys && !second) {
                 const int64_t at = ((int64_t)batch * a.H + head) * a.Spad + step * kStep;
                 uint8_t* to = smem + kOffStat + (i & 1) * 2 * kStatBytes;
                 mbar_expect_tx(&b->stat_full[i & 1], 2 * kStatBytes);
@@ -494,7 +508,7 @@ __device__ __forceinline__ void produce(const CUtensorMap* mx, const CUtensorMap
     if (lane == 0) {
         for (int s = 0; s < kStages && s < it; ++s) drain_bar(&b->full[s], ((it - 1 - s) / kStages) & 1u);
         const int steps = (it + 1) / 2;
-        for (int s = 0; stats && s < 2 && s < steps; ++s) drain_bar(&b->stat_full[s], ((steps - 1 - s) / 2) & 1u);
+        for (int s = 0; kKeys && s < 2 && s < steps; ++s) drain_bar(&b->stat_full[s], ((steps - 1 - s) / 2) & 1u);
         drain_bar(&b->own, 0);
     }
 }
@@ -513,7 +527,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_kernel(const __grid_cons
     const int row0 = (keys ? id % blocks : blocks - 1 - id % blocks) * kRows;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kStages; ++s) {
+        for (int s = 0; s < kQueryStages; ++s) {
             mbar_init(&b->full[s], 1);
             mbar_init(&b->empty[s], 1);
         }
@@ -584,7 +598,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_kernel(const __grid_cons
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));
         if (warp == kMmaWarp) {
-            if (lane == 0) {
+            if (tc::elect_one()) {
                 if (keys) issue_key(smem, b, tmem, n, pair);
                 else issue_query(smem, b, tmem, n, pair);
             }
@@ -596,8 +610,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_kernel(const __grid_cons
                 if (keys) load_tile(own + kTileBytes, &m.v, row0, head, batch, &b->own);
             }
             __syncwarp();
-            if (keys) produce(&m.q, &m.go, smem, b, batch, head * a.group, first, per_head, n, tail, true, a, lane);
-            else produce(&m.k, &m.v, smem, b, batch, head / a.group, 0, per_head, n, tail, false, a, lane);
+            if (keys) produce<true>(&m.q, &m.go, smem, b, batch, head * a.group, first, per_head, n, tail, a, lane);
+            else produce<false>(&m.k, &m.v, smem, b, batch, head / a.group, 0, per_head, n, tail, a, lane);
         }
         __syncwarp();
     }

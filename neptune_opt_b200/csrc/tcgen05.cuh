@@ -66,6 +66,15 @@ __device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t ncols) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
 }
 
+// True in one lane of a converged warp. The products are issued under this predicate and not under a lane
+// test: the compiler knows that one thread is active behind it and builds the operands in uniform
+// registers; behind `lane == 0` every MMA took about 138 cycles to issue, twice its time on the pipe.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}\n" : "=r"(r));
+    return r != 0;
+}
+
 // Ordering of tcgen05 operations across a thread synchronisation (barrier, mbarrier).
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
