@@ -467,7 +467,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             producer(&mq, &mk, &mv, smem, b, head, head / a.group, batch, q0, n, tail, lane);
             __syncwarp();
         } else if (warp == kMmaWarp) {
-            if (lane == 0) mma_issuer(smem, b, tmem, n0, n);
+            if (tc::elect_one()) mma_issuer(smem, b, tmem, n0, n);
             __syncwarp();
         }
         tc::fence_before();

@@ -15,8 +15,6 @@
 // queries of one head and streams K and V in steps of 128 keys (3 products). Together 7 products where
 // the mathematics needs 5: S and dO V^T are formed twice, but no gradient is summed across CTAs, so
 // there are no atomics, no fp32 copy of dQ in memory, and the result does not depend on scheduling.
-// Steps of 64 (two score stages, N = 64 products) were measured at half the rate: an N = 64 product takes
-// the tensor pipe as long as one of N = 128 (bf16 [8,32,4096,128]: 9.6 ms).
 //
 // Both kinds have one row (a key or a query) per TMEM lane and the same roles:
 //   warps 0-3 / 4-7   columns 0-63 / 64-127 of the scores: read S and dP, form P and dS, store them as

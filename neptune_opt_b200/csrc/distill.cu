@@ -8,16 +8,17 @@
 //
 // An index outside [0, vocab) marks an entry that was not kept. A row without kept entries has loss 0
 // and gradient 0 whatever its logits hold.
+#include <cmath>
 #include <type_traits>
 
 #include "common.cuh"
+#include "fastmath.cuh"
 #include "launch.h"
 
 namespace nb200 {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kMaxTop = 256;  // entries a row may keep: one per thread
+constexpr int kMaxTop = 256;  // entries a row may keep: one per thread of its CTA
 
 struct Row {  // what both directions read of the teacher
     const void* teacher;
@@ -42,50 +43,150 @@ struct Row {  // what both directions read of the teacher
     }
 };
 
-// Merge of two (maximum, sum of exp(x - maximum)) states; -inf maxima carry a zero sum.
-__device__ __forceinline__ void merge(float& m, float& s, float m2, float s2) {
-    const float mm = fmaxf(m, m2);
-    const float a = m == mm ? s : s * expf(m - mm);
-    const float b = m2 == mm ? s2 : s2 * expf(m2 - mm);
-    m = mm;
-    s = a + b;
+// Elements before the first 16-byte boundary at or after p.
+template <typename T>
+__device__ __forceinline__ int64_t lead(const T* p) {
+    return (int64_t)((16 - (reinterpret_cast<uintptr_t>(p) & 15u)) & 15u) / (int64_t)sizeof(T);
+}
+
+// Running (maximum, sum of 2^(x log2 e - maximum)) of x = logits / T, the maximum in the log2 domain. -inf
+// maxima carry a zero sum.
+struct LogSum {
+    float m = -HUGE_VALF, s = 0.f;
+    __device__ __forceinline__ static float shift(float m) { return m == -NB200_INF ? 0.f : m; }
+    __device__ __forceinline__ void merge(float m2, float s2) {
+        const float t = fmaxf(m, m2), c = shift(t);
+        s = s * ex2_ftz(m - c) + s2 * ex2_ftz(m2 - c);
+        m = t;
+    }
+    // E values, already in the log2 domain.
+    template <int E>
+    __device__ __forceinline__ void add(const float* x) {
+        float t[4] = {m, x[0], x[0], x[0]};
+#pragma unroll
+        for (int i = 0; i < E; ++i) t[i & 3] = fmaxf(t[i & 3], x[i]);
+        const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), c = shift(top);
+        float a[4] = {s * ex2_ftz(m - c), 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < E; ++i) a[i & 3] += ex2_ftz(x[i] - c);
+        s = (a[0] + a[1]) + (a[2] + a[3]);
+        m = top;
+    }
+};
+
+// ------------------------------------------------------------------ forward
+// One cluster of CTAs per row (one CTA when there are rows enough): each folds a share of the row's 16-byte
+// vectors, the states meet in the first CTA's shared memory, and that CTA takes the kept entries, which
+// it fetched before the fold. One pass over the logits, no scratch.
+constexpr int kFwdThreads = 512;
+constexpr int kMaxCluster = 16;
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Stores v at p's place in the shared memory of the cluster's first CTA.
+__device__ __forceinline__ void store_first(float* p, float v) {
+    uint32_t to;
+    const uint32_t local = static_cast<uint32_t>(__cvta_generic_to_shared(p));
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(to) : "r"(local));
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(v) : "memory");
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kFwdThreads)
     distill_fwd_kernel(const T* x, int64_t stride, Row r, const float* teacher_lse, float* loss, float* stats) {
-    __shared__ float buf[64], sm[32], ss[32];
-    const int64_t row = blockIdx.x;
+    constexpr int V = Elem<T>::V, U = 4;  // U vectors in flight per thread
+    __shared__ float buf[64], sm[32], ss[32], cm[kMaxCluster], cs[kMaxCluster];
+    const uint32_t rank = cluster_rank(), size = cluster_size();
+    const int64_t row = blockIdx.x / size;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const T* xr = x + row * stride;
-    float m = -NB200_INF, s = 0.f;
-    for (int64_t c = t; c < r.vocab; c += kThreads) merge(m, s, Elem<T>::to_f(xr[c]) * r.inv_t, 1.f);
-    for (int o = 16; o > 0; o >>= 1)
-        merge(m, s, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o));
+    // The kept entries, one per thread.
+    int64_t at = -1;
+    float tl = -NB200_INF, xl = 0.f;
+    if (rank == 0 && t < r.top) {
+        at = r.at(row, t);
+        if (at >= 0) {
+            tl = r.logit(row, t);
+            xl = Elem<T>::to_f(xr[at]) * r.inv_t;
+        }
+    }
+    constexpr float kL2e = 1.4426950408889634f;
+    const float scale = r.inv_t * kL2e;
+    LogSum acc;
+    const int64_t head = min(lead(xr), r.vocab), nv = (r.vocab - head) / V, tail = head + nv * V;
+    int64_t v0, v1;
+    split_range(nv, size, rank, v0, v1);
+    const uint4* p = reinterpret_cast<const uint4*>(xr + head);
+    auto fold = [&](const uint4& u) {
+        float f[V];
+        Elem<T>::unpack(u, f);
+#pragma unroll
+        for (int e = 0; e < V; ++e) f[e] *= scale;
+        acc.add<V>(f);
+    };
+    int64_t v = v0 + t;
+    for (; v + (U - 1) * kFwdThreads < v1; v += U * kFwdThreads) {
+        uint4 u[U];
+#pragma unroll
+        for (int k = 0; k < U; ++k) u[k] = ld_stream(p + v + k * kFwdThreads);
+#pragma unroll
+        for (int k = 0; k < U; ++k) fold(u[k]);
+    }
+    for (; v < v1; v += kFwdThreads) fold(ld_stream(p + v));
+    if (rank == 0) {  // what lies outside the vectors: fewer than 2 V elements
+        if (t < head) {
+            const float f = Elem<T>::to_f(xr[t]) * scale;
+            acc.add<1>(&f);
+        } else if (t >= 32 && tail + t - 32 < r.vocab) {
+            const float f = Elem<T>::to_f(xr[tail + t - 32]) * scale;
+            acc.add<1>(&f);
+        }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const float m2 = __shfl_xor_sync(0xffffffffu, acc.m, o), s2 = __shfl_xor_sync(0xffffffffu, acc.s, o);
+        acc.merge(m2, s2);
+    }
     if (lane == 0) {
-        sm[warp] = m;
-        ss[warp] = s;
+        sm[warp] = acc.m;
+        ss[warp] = acc.s;
     }
     __syncthreads();
-    m = sm[0];
-    s = ss[0];
-    for (int w = 1; w < kThreads / 32; ++w) merge(m, s, sm[w], ss[w]);
-    const float lse = m + logf(s);
-    // The kept entries, one per thread.
+    acc = LogSum{};
+    for (int w = 0; w < kFwdThreads / 32; ++w) acc.merge(sm[w], ss[w]);
+    if (size > 1) {
+        if (t == 0) {
+            store_first(&cm[rank], acc.m);
+            store_first(&cs[rank], acc.s);
+        }
+        cluster_sync();
+        if (rank != 0) return;
+        acc = LogSum{};
+        for (uint32_t c = 0; c < size; ++c) acc.merge(cm[c], cs[c]);
+    }
+    const float lse = (acc.m + log2f(acc.s)) * 0.69314718055994531f;
     Group<true> g{buf, 0};
-    const int64_t at = t < r.top ? r.at(row, t) : -1;
-    const float tl = at >= 0 ? r.logit(row, t) : -NB200_INF;
     float z;
     if (teacher_lse) {
         z = teacher_lse[row];
     } else {
-        const float top = g.reduce(tl, RED_MAX), shift = top == -NB200_INF ? 0.f : top;
-        z = shift + logf(g.reduce(expf(tl - shift), RED_SUM));
+        const float top = g.reduce(tl, RED_MAX), c = LogSum::shift(top);
+        z = c + logf(g.reduce(expf(tl - c), RED_SUM));
     }
-    const float p = at >= 0 ? expf(tl - z) : 0.f;
-    const float mass = g.reduce(p, RED_SUM);
-    const float d = at >= 0 && p != 0.f ? p * ((tl - z) - (Elem<T>::to_f(xr[at]) * r.inv_t - lse)) : 0.f;
-    const float l = g.reduce(d, RED_SUM);
+    const float pr = at >= 0 ? expf(tl - z) : 0.f;
+    const float mass = g.reduce(pr, RED_SUM);
+    const float l = g.reduce(at >= 0 && pr != 0.f ? pr * ((tl - z) - (xl - lse)) : 0.f, RED_SUM);
     if (t == 0) {
         loss[row] = l;
         stats[3 * row] = lse;
@@ -94,34 +195,83 @@ __global__ void __launch_bounds__(kThreads)
     }
 }
 
+// CTAs per row: enough for two on every SM, no more than leaves each at least one round of loads.
 template <typename T>
-__global__ void __launch_bounds__(kThreads)
+int cluster_for(int64_t rows, int64_t vocab) {
+    const int64_t round = (int64_t)kFwdThreads * Elem<T>::V;
+    int c = 1;
+    while (c < kMaxCluster && rows * c < 2 * sm_count() && vocab >= 2 * c * round) c *= 2;
+    return c;
+}
+
+// ------------------------------------------------------------------ backward
+// One CTA per row and chunk of columns: write the softmax part of the chunk, then the chunk's kept
+// columns once more with their probabilities taken off.
+constexpr int kBwdThreads = 256;
+constexpr int kChunk = 16384;  // columns
+static_assert(kMaxTop <= kBwdThreads && kMaxTop <= kFwdThreads, "one kept entry per thread");
+
+template <typename T>
+__global__ void __launch_bounds__(kBwdThreads)
     distill_bwd_kernel(const float* grad, int64_t grad_stride, const T* x, int64_t stride, Row r, const float* stats,
-                       T* dx) {
+                       int chunks, T* dx) {
+    constexpr int V = Elem<T>::V, U = 4;
     __shared__ int64_t at[kMaxTop];
     __shared__ float p[kMaxTop];
-    const int64_t row = blockIdx.x;
+    const int64_t row = blockIdx.x / chunks, c0 = (int64_t)(blockIdx.x % chunks) * kChunk;
+    const int64_t c1 = min(c0 + kChunk, r.vocab);
     const int t = threadIdx.x;
     const float lse = stats[3 * row], z = stats[3 * row + 1], mass = stats[3 * row + 2];
     const float w = grad[row * grad_stride] * r.inv_t;
     const T* xr = x + row * stride;
     T* dr = dx + row * r.vocab;
-    at[t] = t < r.top ? r.at(row, t) : -1;
-    p[t] = at[t] >= 0 ? expf(r.logit(row, t) - z) : 0.f;
-    const bool any = __syncthreads_or(at[t] >= 0);
-    for (int64_t c = t; c < r.vocab; c += kThreads)
-        dr[c] = Elem<T>::from_f(any ? w * (mass * expf(Elem<T>::to_f(xr[c]) * r.inv_t - lse)) : 0.f);
+    const int64_t mine = t < r.top ? r.at(row, t) : -1;
+    const float pm = mine >= 0 ? expf(r.logit(row, t) - z) : 0.f;
+    if (t < r.top) {
+        at[t] = mine;
+        p[t] = pm;
+    }
+    const bool any = __syncthreads_or(mine >= 0);
+    constexpr float kL2e = 1.4426950408889634f;
+    const float wm = w * mass;
+    // w mass q, the difference taken before the change of base so that large logits keep their digits; a
+    // row without kept entries is 0 whatever its logits hold.
+    auto soft = [&](float f) { return any ? wm * ex2_ftz(fmaf(f, r.inv_t, -lse) * kL2e) : 0.f; };
+    const int64_t head = min(lead(dr + c0), c1 - c0);
+    const bool together = lead(xr + c0) == lead(dr + c0);  // both sides meet the same 16-byte boundaries
+    const int64_t nv = together ? (c1 - c0 - head) / V : 0;
+    const uint4* src = reinterpret_cast<const uint4*>(xr + c0 + head);
+    uint4* dst = reinterpret_cast<uint4*>(dr + c0 + head);
+    auto one = [&](const uint4& u, int64_t v) {
+        float f[V];
+        Elem<T>::unpack(u, f);
+#pragma unroll
+        for (int e = 0; e < V; ++e) f[e] = soft(f[e]);
+        __stcs(dst + v, Elem<T>::pack(f));
+    };
+    int64_t v = t;
+    for (; v + (U - 1) * kBwdThreads < nv; v += U * kBwdThreads) {
+        uint4 u[U];
+#pragma unroll
+        for (int k = 0; k < U; ++k) u[k] = ld_stream(src + v + k * kBwdThreads);
+#pragma unroll
+        for (int k = 0; k < U; ++k) one(u[k], v + k * kBwdThreads);
+    }
+    for (; v < nv; v += kBwdThreads) one(ld_stream(src + v), v);
+    if (t < head) dr[c0 + t] = Elem<T>::from_f(soft(Elem<T>::to_f(xr[c0 + t])));
+    for (int64_t c = c0 + head + nv * V + t; c < c1; c += kBwdThreads)
+        dr[c] = Elem<T>::from_f(soft(Elem<T>::to_f(xr[c])));
     __syncthreads();
-    // The kept columns again, by the first entry that names each: entries of one column add in order.
-    if (at[t] >= 0) {
+    // By the first entry that names a column: entries of one column add in order.
+    if (mine >= c0 && mine < c1) {
         float sum = 0.f;
         bool first = true;
         for (int j = 0; j < r.top; ++j) {
-            if (at[j] != at[t]) continue;
+            if (at[j] != mine) continue;
             first = first && j >= t;
             sum += p[j];
         }
-        if (first) dr[at[t]] = Elem<T>::from_f(w * (mass * expf(Elem<T>::to_f(xr[at[t]]) * r.inv_t - lse) - sum));
+        if (first) dr[mine] = Elem<T>::from_f(soft(Elem<T>::to_f(xr[mine])) - w * sum);
     }
 }
 
@@ -144,8 +294,9 @@ int check_sizes(const char* what, const nb200_distill_args& a) {
         set_error("%s: %lld kept logits per row exceed the kernel's %d", what, (long long)a.top, kMaxTop);
         return NB200_ERR_CAPACITY;
     }
-    if (a.rows > 0x7fffffffLL) {
-        set_error("%s: %lld rows exceed the kernel's index range", what, (long long)a.rows);
+    if (a.rows * ((a.vocab + kChunk - 1) / kChunk) > 0x7fffffffLL || a.rows > 0x7fffffffLL / kMaxCluster) {
+        set_error("%s: %lld rows of %lld exceed the kernel's index range", what, (long long)a.rows,
+                  (long long)a.vocab);
         return NB200_ERR_CAPACITY;
     }
     return NB200_OK;
@@ -159,7 +310,21 @@ int launch_distill_fwd(const nb200_distill_args& a, const float* teacher_lse, fl
     if (rc) return rc;
     const Row r = make_row(a);
     auto go = [&](auto* x) {
-        distill_fwd_kernel<<<(unsigned)a.rows, kThreads, 0, st>>>(x, a.stride_x, r, teacher_lse, loss, stats);
+        using T = std::remove_const_t<std::remove_pointer_t<decltype(x)>>;
+        const auto kernel = distill_fwd_kernel<T>;
+        const int size = cluster_for<T>(a.rows, a.vocab);
+        if (size > 8) cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)(a.rows * size));
+        cfg.blockDim = dim3(kFwdThreads);
+        cfg.stream = st;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = size;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        cudaLaunchKernelEx(&cfg, kernel, x, a.stride_x, r, teacher_lse, loss, stats);
     };
     if (a.dtype == NB200_F32) go(static_cast<const float*>(a.x));
     else if (a.dtype == NB200_BF16) go(static_cast<const __nv_bfloat16*>(a.x));
@@ -175,8 +340,9 @@ int launch_distill_bwd(const nb200_distill_args& a, const float* grad, int64_t s
     const Row r = make_row(a);
     auto go = [&](auto* d) {
         using T = std::remove_pointer_t<decltype(d)>;
-        distill_bwd_kernel<T><<<(unsigned)a.rows, kThreads, 0, st>>>(grad, stride_grad, static_cast<const T*>(a.x),
-                                                                     a.stride_x, r, stats, d);
+        const int chunks = (int)((a.vocab + kChunk - 1) / kChunk);
+        distill_bwd_kernel<T><<<(unsigned)(a.rows * chunks), kBwdThreads, 0, st>>>(
+            grad, stride_grad, static_cast<const T*>(a.x), a.stride_x, r, stats, chunks, d);
     };
     if (a.dtype == NB200_F32) go(static_cast<float*>(dx));
     else if (a.dtype == NB200_BF16) go(static_cast<__nv_bfloat16*>(dx));
