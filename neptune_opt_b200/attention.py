@@ -22,6 +22,7 @@ import math
 
 from neptune_opt_b200 import _lib
 from neptune_opt_b200.template import _is_metadata, _on_device, current_stream
+from neptune_opt_b200.torch_op import cxx_op
 
 HEAD_DIMS = (128,)
 OP_NAME = "neptune_b200::attention"
@@ -133,19 +134,7 @@ def attention_backward(q, k, v, o, lse, grad_out, *, causal: bool = False, scale
         raise ValueError("attention_backward: lse must be [batch, heads, seq] on the device of q")
     if _is_metadata(q) or q.numel() == 0:
         return torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v)
-    q, k, v, o, grad_out, lse = _rows(q), _rows(k), _rows(v), _rows(o), _rows(grad_out), lse.contiguous()
-    dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
-    lib = _lib.load()
-    args = _args(q, k, causal, sc, seq_lens)
-    nbytes = lib.nb200_attention_bwd_work_bytes(ctypes.byref(args))
-    work = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=q.device)
-    with _on_device(q.device):
-        rc = lib.nb200_attention_bwd(ctypes.byref(args), _strides(q, k, v, o, grad_out, dq, dk, dv), q.data_ptr(),
-                                     k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), grad_out.data_ptr(),
-                                     dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), work.data_ptr(), work.numel(),
-                                     current_stream(q.device))
-    _lib.check(rc, "nb200_attention_bwd")
-    return dq, dk, dv
+    return cxx_op("attention_bwd")(q, k, v, o, lse, grad_out, seq_lens, causal, sc)
 
 
 _FUNCTION = None

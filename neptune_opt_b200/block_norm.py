@@ -17,11 +17,10 @@ for devices, shapes and parameters, NotImplementedError past the kernels' width.
 """
 from __future__ import annotations
 
-import ctypes
 import math
 
-from neptune_opt_b200 import _lib
-from neptune_opt_b200.template import _is_metadata, _on_device, current_stream, dtype_code
+from neptune_opt_b200.template import _is_metadata
+from neptune_opt_b200.torch_op import cxx_op
 
 GATE_ACTS = {"none": 0, "tanh": 1, "sigmoid": 2}
 MAX_WIDTH = 16384
@@ -77,25 +76,6 @@ def validate_gated_norm_inputs(x, residual, gate, post_weight, pre_weight, gate_
     return 1 if gate is None else _rows_per_gate(x, gate)
 
 
-def _flat(t):
-    """[rows, width] of t with unit column stride (a copy only when no such view exists)."""
-    t2 = t.reshape(-1, t.shape[-1])
-    if t2.stride(1) != 1 and t2.shape[1] != 1 or t2.stride(0) < 0:
-        t2 = t2.contiguous()
-    return t2
-
-
-def _args(x, residual, gate, post_weight, pre_weight, per_gate, gate_act, residual_scale, eps):
-    """(nb200_norm_args, the tensors whose memory it names)."""
-    keep = [None if t is None else _flat(t) for t in (x, residual, gate)]
-    keep += [None if w is None else w.contiguous() for w in (post_weight, pre_weight)]
-    x2 = keep[0]
-    a = _lib.NB200NormArgs(*[None if t is None else t.data_ptr() for t in keep], x2.shape[0], x2.shape[1],
-                           x2.stride(0), keep[1].stride(0), 0 if gate is None else keep[2].stride(0), 0, 0, per_gate,
-                           GATE_ACTS[gate_act], residual_scale, eps)
-    return a, keep
-
-
 def run_gated_residual_norm(x, residual, gate=None, *, post_weight=None, pre_weight=None, gate_act: str = "none",
                             residual_scale: float = 1.0, eps: float = 1e-6):
     """(y, h, rstd): fresh contiguous results in x's dtype (h is None without pre_weight) and the fp32
@@ -103,18 +83,12 @@ def run_gated_residual_norm(x, residual, gate=None, *, post_weight=None, pre_wei
     import torch
 
     per_gate = validate_gated_norm_inputs(x, residual, gate, post_weight, pre_weight, gate_act, residual_scale, eps)
+    if not _is_metadata(x) and x.numel():
+        return cxx_op("gated_norm")(x, residual, gate, post_weight, pre_weight, per_gate, GATE_ACTS[gate_act],
+                                    residual_scale, eps)
     y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
     h = torch.empty(x.shape, device=x.device, dtype=x.dtype) if pre_weight is not None else None
-    rstd = torch.empty((*x.shape[:-1], 2), device=x.device, dtype=torch.float32)
-    if _is_metadata(x) or x.numel() == 0:
-        return y, h, rstd
-    a, keep = _args(x, residual, gate, post_weight, pre_weight, per_gate, gate_act, residual_scale, eps)
-    lib = _lib.load()
-    with _on_device(x.device):
-        rc = lib.nb200_gated_norm(ctypes.byref(a), dtype_code(x.dtype), y.data_ptr(),
-                                  None if h is None else h.data_ptr(), rstd.data_ptr(), current_stream(x.device))
-    _lib.check(rc, "nb200_gated_norm")
-    return y, h, rstd
+    return y, h, torch.empty((*x.shape[:-1], 2), device=x.device, dtype=torch.float32)
 
 
 def gated_residual_norm_backward(grad_y, grad_h, x, residual, gate, rstd, *, post_weight=None, pre_weight=None,
@@ -138,29 +112,11 @@ def gated_residual_norm_backward(grad_y, grad_h, x, residual, gate, rstd, *, pos
     if tuple(rstd.shape) != (*x.shape[:-1], 2) or rstd.device != x.device:
         raise ValueError("gated_residual_norm_backward: rstd must be [..., 2] on the device of x")
 
-    def fresh(t):
-        return None if t is None else torch.empty(t.shape, device=t.device, dtype=t.dtype)
-
-    grads = [fresh(t) for t in (x, residual, gate, post_weight, pre_weight)]
-    if _is_metadata(x) or x.numel() == 0:
-        return tuple(None if g is None else g.zero_() for g in grads)
-    a, keep = _args(x, residual, gate, post_weight, pre_weight, per_gate, gate_act, residual_scale, 1.0)
-    gy, gh = (None if t is None else _flat(t) for t in (grad_y, grad_h))
-    a.stride_grad_y = 0 if gy is None else gy.stride(0)
-    a.stride_grad_h = 0 if gh is None else gh.stride(0)
-    lib = _lib.load()
-    nbytes = lib.nb200_gated_norm_bwd_work_bytes(ctypes.byref(a))
-    work = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=x.device)
-    rstd = rstd.contiguous()
-
-    def ptr(t):
-        return None if t is None else t.data_ptr()
-
-    with _on_device(x.device):
-        rc = lib.nb200_gated_norm_bwd(ctypes.byref(a), dtype_code(x.dtype), ptr(rstd), ptr(gy), ptr(gh),
-                                      *[ptr(g) for g in grads], ptr(work), work.numel(), current_stream(x.device))
-    _lib.check(rc, "nb200_gated_norm_bwd")
-    return tuple(grads)
+    if not _is_metadata(x) and x.numel():
+        return cxx_op("gated_norm_bwd")(grad_y, grad_h, x, residual, gate, rstd, post_weight, pre_weight, per_gate,
+                                        GATE_ACTS[gate_act], residual_scale)
+    return tuple(None if t is None else torch.zeros(t.shape, device=t.device, dtype=t.dtype)
+                 for t in (x, residual, gate, post_weight, pre_weight))
 
 
 _FUNCTION = None

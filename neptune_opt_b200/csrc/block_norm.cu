@@ -18,6 +18,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "fastmath.cuh"
 #include "launch.h"
 
 namespace nb200 {
@@ -49,64 +50,141 @@ __device__ __forceinline__ float gate_value(float g, int kind, float& slope) {
 }
 
 // A row is held by a warp (CTA false, kWarpRows of them in a CTA) or a whole CTA, E = NV * V elements a
-// thread; t is the thread's place in its row, item the row (forward) or chunk (backward) it works on.
-template <bool CTA>
-struct Place {
+// thread, computed as packed fp32 pairs. A unit (warp or CTA) works through consecutive rows, so that the
+// weights stay in registers and a gate row is read and put through its activation once per group.
+template <typename T, int NV, bool VEC, bool CTA>
+struct Rows {
+    using CH = Chunk<T, NV, VEC>;
+    static constexpr int V = CH::V, P = CH::E / 2;  // P pairs a thread
     int t, G;
-    int64_t item, items;
-    __device__ __forceinline__ Place() {
+    int64_t unit, width;
+    float4* buf;  // 2 x 32 entries of shared memory when CTA
+    int phase = 0;
+
+    __device__ __forceinline__ Rows(int64_t w, float4* b) : width(w), buf(b) {
         t = threadIdx.x;
         G = blockDim.x;
-        item = CTA ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-        items = CTA ? (int64_t)gridDim.x : (int64_t)gridDim.x * blockDim.y;
+        unit = CTA ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+    }
+    __device__ __forceinline__ void load(CH& c, const T* row, bool stream) const { c.load(row, 1, 0, width, t, G, stream); }
+    __device__ __forceinline__ static uint64_t pair(const CH& c, int i) { return f2(c.get(2 * i), c.get(2 * i + 1)); }
+    __device__ __forceinline__ void store(T* row, const uint64_t* v) const {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            float f[V];
+#pragma unroll
+            for (int j = 0; j < V / 2; ++j) {
+                f[2 * j] = f2lo(v[k * V / 2 + j]);
+                f[2 * j + 1] = f2hi(v[k * V / 2 + j]);
+            }
+            store_vec<T, NV, VEC>(row, f, k, 0, width, t, G, VEC);
+        }
+    }
+    // Sums of up to three values over the row's threads, in every thread: warp shuffles, then the warps' sums
+    // in warp order (one barrier; the two buffers alternate).
+    template <int N>
+    __device__ __forceinline__ void sum(float* v) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = warp_sum(v[i]);
+        if constexpr (CTA) {
+            float4* slot = buf + (phase ^= 1) * 32;
+            const int warps = G >> 5;
+            if ((t & 31) == 0) slot[t >> 5] = make_float4(v[0], N > 1 ? v[1] : 0.f, N > 2 ? v[2] : 0.f, 0.f);
+            __syncthreads();
+            float4 w = (t & 31) < warps ? slot[t & 31] : make_float4(0.f, 0.f, 0.f, 0.f);
+            v[0] = warp_sum(w.x);
+            if (N > 1) v[1] = warp_sum(w.y);
+            if (N > 2) v[2] = warp_sum(w.z);
+        }
+    }
+};
+
+// Position of a unit in its rows: the rows left of the current gate group.
+struct GatePos {
+    int64_t index, left;
+    __device__ __forceinline__ GatePos(int64_t row, int64_t group) : index(row / group) {
+        left = group - (row - index * group);
+    }
+    // Moves to the next row; true when that row starts another group.
+    __device__ __forceinline__ bool next(int64_t group) {
+        if (--left) return false;
+        left = group;
+        ++index;
+        return true;
     }
 };
 
 template <typename T, int NV, bool VEC, bool CTA, int kThreads>
-__global__ void __launch_bounds__(kThreads) norm_fwd_kernel(const T* x, const T* res, const T* gate, const T* w1, const T* w2, Norm n, T* y,
-                                T* h, float* rstd) {
-    using CH = Chunk<T, NV, VEC>;
-    constexpr int V = CH::V, E = CH::E;
-    __shared__ float buf[64];
-    const Place<CTA> at;
-    Group<CTA> grp{buf, 0};
-    CH c1, c2;
-    if (w1) c1.load(w1, 1, 0, n.width, at.t, at.G, false);
-    if (w2) c2.load(w2, 1, 0, n.width, at.t, at.G, false);
-    for (int64_t row = at.item; row < n.rows; row += at.items) {
-        CH cx, cr, cg;
-        cx.load(x + row * n.sx, 1, 0, n.width, at.t, at.G, true);
-        cr.load(res + row * n.sr, 1, 0, n.width, at.t, at.G, true);
-        if (gate) cg.load(gate + row / n.group * n.sg, 1, 0, n.width, at.t, at.G, false);
-        float s = 0.f, r1 = 1.f, r2 = 1.f;
+__global__ void __launch_bounds__(kThreads) norm_fwd_kernel(const T* x, const T* res, const T* gate, const T* w1,
+                                                            const T* w2, Norm n, int64_t per_unit, T* y, T* h,
+                                                            float* rstd) {
+    using R = Rows<T, NV, VEC, CTA>;
+    using CH = typename R::CH;
+    constexpr int P = R::P;
+    __shared__ float4 buf[CTA ? 64 : 1];
+    R r(n.width, buf);
+    int64_t row = r.unit * per_unit;
+    const int64_t end = min(row + per_unit, n.rows);
+    if (row >= end) return;
+    CH c1, c2, cx, cr, cg;
+    if (w1) r.load(c1, w1, false);
+    if (w2) r.load(c2, w2, false);
+    r.load(cx, x + row * n.sx, true);
+    r.load(cr, res + row * n.sr, true);
+    GatePos g(row, n.group);
+    if (gate) r.load(cg, gate + g.index * n.sg, false);
+    bool fresh = true;
+    uint64_t b[P];  // scale * a(gate) * post weight
+    for (; row < end; ++row) {
+        if (fresh) {
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                float slope;
+                const uint64_t a = gate ? f2(n.scale * gate_value(cg.get(2 * i), n.act, slope),
+                                             n.scale * gate_value(cg.get(2 * i + 1), n.act, slope))
+                                        : f2(n.scale, n.scale);
+                b[i] = w1 ? mul2(a, R::pair(c1, i)) : a;
+            }
+        }
+        // The next row is on its way while this one is reduced.
+        CH nx, nr;
+        fresh = false;
+        if (row + 1 < end) {
+            r.load(nx, x + (row + 1) * n.sx, true);
+            r.load(nr, res + (row + 1) * n.sr, true);
+            if (gate && g.next(n.group)) {
+                r.load(cg, gate + g.index * n.sg, false);
+                fresh = true;
+            }
+        }
+        float r1 = 1.f, r2 = 1.f;
+        uint64_t acc = 0;
         if (w1) {
 #pragma unroll
-            for (int i = 0; i < E; ++i) s = fmaf(cx.get(i), cx.get(i), s);
-            r1 = rsqrtf(grp.reduce(s, RED_SUM) * n.inv_n + n.eps);
+            for (int i = 0; i < P; ++i) acc = fma2(R::pair(cx, i), R::pair(cx, i), acc);
+            float s = f2lo(acc) + f2hi(acc);
+            r.template sum<1>(&s);
+            r1 = rsqrtf(s * n.inv_n + n.eps);
         }
-        float v[E];
-        s = 0.f;
+        uint64_t v[P];
+        acc = 0;
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-            float z = cx.get(i), slope;
-            if (w1) z *= r1 * c1.get(i);
-            v[i] = fmaf(n.scale * (gate ? gate_value(cg.get(i), n.act, slope) : 1.f), z, cr.get(i));
-            s = fmaf(v[i], v[i], s);
+        for (int i = 0; i < P; ++i) {
+            v[i] = fma2(b[i], mul2(R::pair(cx, i), f2(r1, r1)), R::pair(cr, i));
+            acc = fma2(v[i], v[i], acc);
         }
-        if (w2) r2 = rsqrtf(grp.reduce(s, RED_SUM) * n.inv_n + n.eps);
-#pragma unroll
-        for (int k = 0; k < NV; ++k) store_vec<T, NV, VEC>(y + row * n.width, v + k * V, k, 0, n.width, at.t, at.G, VEC);
+        r.store(y + row * n.width, v);
         if (w2) {
+            float s = f2lo(acc) + f2hi(acc);
+            r.template sum<1>(&s);
+            r2 = rsqrtf(s * n.inv_n + n.eps);
 #pragma unroll
-            for (int i = 0; i < E; ++i) v[i] *= r2 * c2.get(i);
-#pragma unroll
-            for (int k = 0; k < NV; ++k)
-                store_vec<T, NV, VEC>(h + row * n.width, v + k * V, k, 0, n.width, at.t, at.G, VEC);
+            for (int i = 0; i < P; ++i) v[i] = mul2(v[i], mul2(R::pair(c2, i), f2(r2, r2)));
+            r.store(h + row * n.width, v);
         }
-        if (at.t == 0) {
-            rstd[2 * row] = r1;
-            rstd[2 * row + 1] = r2;
-        }
+        if (r.t == 0) *reinterpret_cast<float2*>(rstd + 2 * row) = make_float2(r1, r2);
+        cx = nx;
+        cr = nr;
     }
 }
 
@@ -122,7 +200,9 @@ struct Chunks {
     }
 };
 
-Chunks make_chunks(const Norm& n, int64_t target) {
+Chunks make_chunks(const Norm& n) {
+    // Two CTAs on every SM, each unit of which holds one chunk.
+    const int64_t target = 2 * sm_count() * (n.width > 512 ? 1 : kWarpRows);
     const int64_t want = (n.rows + target - 1) / target;  // rows per chunk
     Chunks c;
     if (n.group > want) {
@@ -138,105 +218,143 @@ Chunks make_chunks(const Norm& n, int64_t target) {
 }
 
 // One fp32 row of a chunk's column sums.
-template <typename T, int NV, bool VEC>
-__device__ __forceinline__ void store_part(float* part, const float* acc, int64_t width, int t, int G) {
-    using CH = Chunk<T, NV, VEC>;
+template <typename R>
+__device__ __forceinline__ void store_part(float* part, const uint64_t* acc, const R& r) {
 #pragma unroll
-    for (int i = 0; i < CH::E; ++i) {
-        const int64_t c = CH::col_of(0, t, G, i);
-        if (c < width) part[c] = acc[i];
+    for (int i = 0; i < 2 * R::P; ++i) {
+        const int64_t c = R::CH::col_of(0, r.t, r.G, i);
+        if (c < r.width) part[c] = i & 1 ? f2hi(acc[i / 2]) : f2lo(acc[i / 2]);
     }
 }
 
+// Both row statistics come from one round of sums: with c = scale a w1 xhat,
+//   n m2 = sum t yhat,   n m1 = sum c dY = sum c (dy + r2 t) - r2 m2 sum c yhat.
+// Within a gate group the gate and post-weight gradients share one column sum, G = sum xhat dY:
+// dgate = scale a' w1 G and dw1 += scale a G.
 template <typename T, int NV, bool VEC, bool CTA, int kThreads>
-__global__ void __launch_bounds__(kThreads) norm_bwd_kernel(const T* dy, const T* dh, const T* x, const T* res, const T* gate, const T* w1,
-                                const T* w2, const float* rstd, Norm n, Chunks ch, T* dx, T* dres, T* dgate,
-                                float* part1, float* part2, float* partg) {
-    using CH = Chunk<T, NV, VEC>;
-    constexpr int V = CH::V, E = CH::E;
-    __shared__ float buf[64];
-    const Place<CTA> at;
-    Group<CTA> grp{buf, 0};
-    if (at.item >= ch.count) return;
+__global__ void __launch_bounds__(kThreads)
+    norm_bwd_kernel(const T* dy, const T* dh, const T* x, const T* res, const T* gate, const T* w1, const T* w2,
+                    const float* rstd, Norm n, Chunks ch, T* dx, T* dres, T* dgate, float* part1, float* part2,
+                    float* partg) {
+    using R = Rows<T, NV, VEC, CTA>;
+    using CH = typename R::CH;
+    constexpr int P = R::P;
+    __shared__ float4 buf[CTA ? 64 : 1];
+    pdl_trigger();
+    R r(n.width, buf);
+    if (r.unit >= ch.count) return;
     int64_t row, end;
-    ch.range(at.item, n, row, end);
-    CH c1, c2;
-    if (w1) c1.load(w1, 1, 0, n.width, at.t, at.G, false);
-    if (w2) c2.load(w2, 1, 0, n.width, at.t, at.G, false);
-    float a1[E], a2[E], ag[E];
+    ch.range(r.unit, n, row, end);
+    CH c1, c2, cg;
+    if (w1) r.load(c1, w1, false);
+    if (w2) r.load(c2, w2, false);
+    uint64_t b[P], G[P], a1[P], a2[P];
 #pragma unroll
-    for (int i = 0; i < E; ++i) a1[i] = a2[i] = ag[i] = 0.f;
+    for (int i = 0; i < P; ++i) G[i] = a1[i] = a2[i] = 0;
+    GatePos g(row, n.group);
+    bool fresh = true;
     for (; row < end; ++row) {
-        CH cx, cr, cg, cdy, cdh;
-        cx.load(x + row * n.sx, 1, 0, n.width, at.t, at.G, true);
-        cr.load(res + row * n.sr, 1, 0, n.width, at.t, at.G, true);
-        if (gate) cg.load(gate + row / n.group * n.sg, 1, 0, n.width, at.t, at.G, false);
-        if (dy) cdy.load(dy + row * n.sdy, 1, 0, n.width, at.t, at.G, true);
-        if (dh) cdh.load(dh + row * n.sdh, 1, 0, n.width, at.t, at.G, true);
-        const float r1 = w1 ? rstd[2 * row] : 1.f, r2 = w2 ? rstd[2 * row + 1] : 1.f;
-        float xhat[E], a[E], yhat[E], d[E];
-        float s = 0.f, slope;
+        CH cx, cr, cdy, cdh;
+        r.load(cx, x + row * n.sx, true);
+        r.load(cr, res + row * n.sr, true);
+        if (dy) r.load(cdy, dy + row * n.sdy, true);
+        if (dh) r.load(cdh, dh + row * n.sdh, true);
+        const float2 rs = *reinterpret_cast<const float2*>(rstd + 2 * row);
+        if (fresh) {
+            if (gate) r.load(cg, gate + g.index * n.sg, false);
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-            xhat[i] = cx.get(i) * r1;
-            a[i] = n.scale * (gate ? gate_value(cg.get(i), n.act, slope) : 1.f);
-            yhat[i] = fmaf(a[i], w1 ? xhat[i] * c1.get(i) : xhat[i], cr.get(i)) * r2;
-            d[i] = dh && w2 ? cdh.get(i) * c2.get(i) : 0.f;
-            s = fmaf(d[i], yhat[i], s);
-        }
-        const float m2 = w2 ? grp.reduce(s, RED_SUM) * n.inv_n : 0.f;
-        s = 0.f;
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-            d[i] = fmaf(r2, d[i] - yhat[i] * m2, dy ? cdy.get(i) : 0.f);
-            if (dh) a2[i] = fmaf(cdh.get(i), yhat[i], a2[i]);
-            const float dz = a[i] * d[i];
-            a1[i] = fmaf(dz, xhat[i], a1[i]);
-            if (w1) s = fmaf(dz * c1.get(i), xhat[i], s);
-        }
-        if (gate) {
-            const bool whole = !partg && (row + 1) % n.group == 0;
-#pragma unroll
-            for (int i = 0; i < E; ++i) {
-                gate_value(cg.get(i), n.act, slope);
-                ag[i] = fmaf(n.scale * slope * (w1 ? xhat[i] * c1.get(i) : xhat[i]), d[i], ag[i]);
-            }
-            if (whole) {
-                T* out = dgate + row / n.group * n.width;
-#pragma unroll
-                for (int k = 0; k < NV; ++k)
-                    store_vec<T, NV, VEC>(out, ag + k * V, k, 0, n.width, at.t, at.G, VEC);
-#pragma unroll
-                for (int i = 0; i < E; ++i) ag[i] = 0.f;
+            for (int i = 0; i < P; ++i) {
+                float slope;
+                const uint64_t a = gate ? f2(n.scale * gate_value(cg.get(2 * i), n.act, slope),
+                                             n.scale * gate_value(cg.get(2 * i + 1), n.act, slope))
+                                        : f2(n.scale, n.scale);
+                b[i] = w1 ? mul2(a, R::pair(c1, i)) : a;
             }
         }
+        const float r1 = w1 ? rs.x : 1.f, r2 = w2 ? rs.y : 1.f;
+        const uint64_t r1p = f2(r1, r1), r2p = f2(r2, r2);
+        uint64_t yhat[P], e[P];  // e = dy + r2 t
+        uint64_t s1 = 0, s2 = 0, s3 = 0;
 #pragma unroll
-        for (int k = 0; k < NV; ++k)
-            store_vec<T, NV, VEC>(dres + row * n.width, d + k * V, k, 0, n.width, at.t, at.G, VEC);
-        const float m1 = w1 ? grp.reduce(s, RED_SUM) * n.inv_n : 0.f;
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-            const float u = a[i] * d[i];
-            d[i] = w1 ? r1 * (u * c1.get(i) - xhat[i] * m1) : u;
+        for (int i = 0; i < P; ++i) {
+            const uint64_t c = mul2(b[i], mul2(R::pair(cx, i), r1p));
+            yhat[i] = mul2(add2(c, R::pair(cr, i)), r2p);
+            const uint64_t t = dh ? mul2(R::pair(cdh, i), R::pair(c2, i)) : 0;
+            e[i] = fma2(t, r2p, dy ? R::pair(cdy, i) : 0);
+            s1 = fma2(t, yhat[i], s1);
+            s2 = fma2(c, e[i], s2);
+            s3 = fma2(c, yhat[i], s3);
         }
+        float s[3] = {f2lo(s1) + f2hi(s1), f2lo(s2) + f2hi(s2), f2lo(s3) + f2hi(s3)};
+        r.template sum<3>(s);
+        const float k2 = r2 * s[0] * n.inv_n, m1 = (s[1] - k2 * s[2]) * n.inv_n;  // k2 = r2 m2
+        const uint64_t k2p = f2(-k2, -k2), k1p = f2(w1 ? -m1 : 0.f, w1 ? -m1 : 0.f);
 #pragma unroll
-        for (int k = 0; k < NV; ++k)
-            store_vec<T, NV, VEC>(dx + row * n.width, d + k * V, k, 0, n.width, at.t, at.G, VEC);
+        for (int i = 0; i < P; ++i) {
+            const uint64_t xhat = mul2(R::pair(cx, i), r1p);
+            if (w2) e[i] = fma2(yhat[i], k2p, e[i]);  // dY
+            if (dh) a2[i] = fma2(R::pair(cdh, i), yhat[i], a2[i]);
+            G[i] = fma2(xhat, e[i], G[i]);
+            yhat[i] = mul2(fma2(xhat, k1p, mul2(b[i], e[i])), r1p);  // dx
+        }
+        r.store(dres + row * n.width, e);
+        r.store(dx + row * n.width, yhat);
+        // The end of a gate group, or of the chunk.
+        fresh = gate && g.next(n.group);
+        if (fresh || row + 1 == end) {
+            const bool direct = gate && !partg;
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                float da[2] = {0.f, 0.f};
+                uint64_t a = f2(n.scale, n.scale);
+                if (gate) {
+                    const float lo = gate_value(cg.get(2 * i), n.act, da[0]);
+                    const float hi = gate_value(cg.get(2 * i + 1), n.act, da[1]);
+                    a = mul2(a, f2(lo, hi));
+                }
+                a1[i] = fma2(a, G[i], a1[i]);
+                G[i] = mul2(G[i], mul2(f2(n.scale * da[0], n.scale * da[1]), w1 ? R::pair(c1, i) : f2(1.f, 1.f)));
+            }
+            if (direct) r.store(dgate + (g.index - (fresh ? 1 : 0)) * n.width, G);
+            if (row + 1 == end) break;
+#pragma unroll
+            for (int i = 0; i < P; ++i) G[i] = 0;
+        }
     }
-    if (part1) store_part<T, NV, VEC>(part1 + at.item * n.width, a1, n.width, at.t, at.G);
-    if (part2) store_part<T, NV, VEC>(part2 + at.item * n.width, a2, n.width, at.t, at.G);
-    if (partg) store_part<T, NV, VEC>(partg + at.item * n.width, ag, n.width, at.t, at.G);
+    if (part1) store_part(part1 + r.unit * n.width, a1, r);
+    if (part2) store_part(part2 + r.unit * n.width, a2, r);
+    if (partg) store_part(partg + r.unit * n.width, G, r);
 }
 
-// out[g, c] = sum over the chunks of group g, in order, of part[chunk, c].
+// Column sums over chunks, in an order that depends on their number alone: out row blockIdx.y is dpost,
+// dpre, then the gate rows. kSumRows threads of a column each add every kSumRows-th chunk, then meet.
+constexpr int kSumCols = 32, kSumRows = 16;
 template <typename T>
-__global__ void __launch_bounds__(256) norm_sum_kernel(const float* part, int64_t chunks, int64_t width, T* out) {
-    const int64_t c = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (c >= width) return;
-    const float* p = part + (int64_t)blockIdx.y * chunks * width + c;
+struct Sums {
+    const float* part[3];  // of dpost, dpre, dgate; null: not wanted
+    T* out[3];
+    int64_t chunks, per_group, width;
+};
+template <typename T>
+__global__ void __launch_bounds__(kSumCols* kSumRows) norm_sum_kernel(Sums<T> a) {
+    __shared__ float buf[kSumRows][kSumCols];
+    pdl_wait();
+    const int64_t c = (int64_t)blockIdx.x * kSumCols + threadIdx.x;
+    const int which = min((int)blockIdx.y, 2);
+    const int64_t group = (int64_t)blockIdx.y - which;
+    if (!a.part[which]) return;
+    const int64_t chunks = which == 2 ? a.per_group : a.chunks;
+    const float* p = a.part[which] + group * chunks * a.width + c;
     float s = 0.f;
-    for (int64_t i = 0; i < chunks; ++i) s += p[i * width];
-    out[(int64_t)blockIdx.y * width + c] = Elem<T>::from_f(s);
+    if (c < a.width) {
+#pragma unroll 4
+        for (int64_t i = threadIdx.y; i < chunks; i += kSumRows) s += p[i * a.width];
+    }
+    buf[threadIdx.y][threadIdx.x] = s;
+    __syncthreads();
+    if (threadIdx.y || c >= a.width) return;
+    for (int i = 1; i < kSumRows; ++i) s += buf[i][threadIdx.x];
+    a.out[which][group * a.width + c] = Elem<T>::from_f(s);
 }
 
 // Threads of a row and elements of a thread: a warp holds up to 512 elements, a CTA of at most 512
@@ -310,16 +428,16 @@ int norm_fwd(const nb200_norm_args& a, T* y, T* h, float* rstd, cudaStream_t st)
     dispatch(s, [&](auto cta, auto e, auto vec, auto most) {
         auto kernel = norm_fwd_kernel<T, decltype(e)::value / Elem<T>::V, decltype(vec)::value, decltype(cta)::value,
                                       decltype(most)::value>;
-        const int grid = persistent_grid(kernel, s.threads * per, 0, (n.rows + per - 1) / per, 0);
-        kernel<<<grid, dim3(s.threads, per), 0, st>>>(
+        // Units enough to fill the GPU, each with an equal share of consecutive rows.
+        const int64_t units = per * (int64_t)persistent_grid(kernel, s.threads * per, 0, (n.rows + per - 1) / per, 0);
+        const int64_t share = (n.rows + units - 1) / units;
+        kernel<<<(unsigned)((n.rows + share * per - 1) / (share * per)), dim3(s.threads, per), 0, st>>>(
             static_cast<const T*>(a.x), static_cast<const T*>(a.residual), static_cast<const T*>(a.gate),
-            static_cast<const T*>(a.post_weight), static_cast<const T*>(a.pre_weight), n, y, h, rstd);
+            static_cast<const T*>(a.post_weight), static_cast<const T*>(a.pre_weight), n, share, y, h, rstd);
     });
     count_launch();
     return finish_launch("nb200_gated_norm");
 }
-
-constexpr int64_t kChunkTarget = 592;
 
 template <typename T>
 int norm_bwd(const nb200_norm_args& a, const float* rstd, const T* dy, const T* dh, T* dx, T* dres, T* dgate, T* dw1,
@@ -332,7 +450,7 @@ int norm_bwd(const nb200_norm_args& a, const float* rstd, const T* dy, const T* 
                     aligned16(dx) && aligned16(dres) && (!dgate || aligned16(dgate));
     const Shape s = make_shape(n.width, es, al);
     const int per = s.cta ? 1 : kWarpRows;
-    const Chunks ch = make_chunks(n, kChunkTarget);
+    const Chunks ch = make_chunks(n);
     const int64_t size = ch.count * n.width;
     float* p1 = dw1 ? work : nullptr;
     float* p2 = dw2 ? work + size : nullptr;
@@ -346,14 +464,21 @@ int norm_bwd(const nb200_norm_args& a, const float* rstd, const T* dy, const T* 
             p1, p2, pg);
     });
     count_launch();
-    auto sum = [&](const float* part, int64_t groups, int64_t chunks, T* out) {
-        norm_sum_kernel<T><<<dim3((unsigned)((n.width + 255) / 256), (unsigned)groups), 256, 0, st>>>(part, chunks,
-                                                                                                      n.width, out);
+    if (p1 || p2 || pg) {
+        const Sums<T> sums = {{p1, p2, pg}, {dw1, dw2, dgate}, ch.count, ch.per_group, n.width};
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)((n.width + kSumCols - 1) / kSumCols),
+                           (unsigned)(2 + (pg ? ch.count / ch.per_group : 0)));
+        cfg.blockDim = dim3(kSumCols, kSumRows);
+        cfg.stream = st;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        cudaLaunchKernelEx(&cfg, norm_sum_kernel<T>, sums);
         count_launch();
-    };
-    if (p1) sum(p1, 1, ch.count, dw1);
-    if (p2) sum(p2, 1, ch.count, dw2);
-    if (pg) sum(pg, ch.count / ch.per_group, ch.per_group, dgate);
+    }
     return finish_launch("nb200_gated_norm_bwd");
 }
 
@@ -370,7 +495,7 @@ int launch_norm_fwd(const nb200_norm_args& a, int dtype, void* y, void* h, float
 
 int64_t norm_bwd_work_bytes(const nb200_norm_args& a) {
     const Norm n = make_norm(a);
-    return 3 * make_chunks(n, kChunkTarget).count * n.width * (int64_t)sizeof(float);
+    return 3 * make_chunks(n).count * n.width * (int64_t)sizeof(float);
 }
 
 int launch_norm_bwd(const nb200_norm_args& a, int dtype, const float* rstd, const void* dy, const void* dh, void* dx,

@@ -20,6 +20,19 @@
 //   segment_status_word(int device) -> Tensor      the per-device int32 word itself, for launches
 //                                                  made through the C ABI by other host code
 //   attention(Tensor q, Tensor k, Tensor v, bool causal, float scale) -> (Tensor o, Tensor lse)
+// The training operators (CUDA kernels only; the Python layer checks the whole contract, the ops what
+// memory safety needs, and an absent optional result is an undefined tensor):
+//   attention_bwd(Tensor q, Tensor k, Tensor v, Tensor o, Tensor lse, Tensor grad_o, Tensor? seq_lens,
+//                 bool causal, float scale) -> (Tensor dq, Tensor dk, Tensor dv)
+//   gated_norm(Tensor x, Tensor residual, Tensor? gate, Tensor? post, Tensor? pre, int rows_per_gate,
+//              int act, float scale, float eps) -> (Tensor y, Tensor h, Tensor rstd)
+//   gated_norm_bwd(Tensor? grad_y, Tensor? grad_h, Tensor x, Tensor residual, Tensor? gate, Tensor rstd,
+//                  Tensor? post, Tensor? pre, int rows_per_gate, int act, float scale)
+//              -> (Tensor dx, Tensor dresidual, Tensor dgate, Tensor dpost, Tensor dpre)
+//   distill_loss(Tensor x, Tensor teacher, Tensor index, float temperature, Tensor? teacher_lse)
+//              -> (Tensor loss, Tensor stats)
+//   distill_loss_bwd(Tensor grad, Tensor x, Tensor teacher, Tensor index, Tensor stats,
+//                    float temperature) -> Tensor
 //
 // libneptune_b200.so is opened at the first call from the directory this library lives in, so
 // the two files only need to sit side by side.
@@ -51,6 +64,13 @@ struct Api {
     decltype(&nb200_segment_spans) segment_spans;
     decltype(&nb200_segment_pool) segment_pool;
     decltype(&nb200_attention) attention;
+    decltype(&nb200_attention_bwd_work_bytes) attention_bwd_work_bytes;
+    decltype(&nb200_attention_bwd) attention_bwd;
+    decltype(&nb200_gated_norm) gated_norm;
+    decltype(&nb200_gated_norm_bwd_work_bytes) gated_norm_bwd_work_bytes;
+    decltype(&nb200_gated_norm_bwd) gated_norm_bwd;
+    decltype(&nb200_distill_loss) distill_loss;
+    decltype(&nb200_distill_loss_bwd) distill_loss_bwd;
 };
 
 std::string own_directory() {
@@ -86,6 +106,13 @@ const Api& api() {
         bind(h, "nb200_segment_spans", a.segment_spans);
         bind(h, "nb200_segment_pool", a.segment_pool);
         bind(h, "nb200_attention", a.attention);
+        bind(h, "nb200_attention_bwd_work_bytes", a.attention_bwd_work_bytes);
+        bind(h, "nb200_attention_bwd", a.attention_bwd);
+        bind(h, "nb200_gated_norm", a.gated_norm);
+        bind(h, "nb200_gated_norm_bwd_work_bytes", a.gated_norm_bwd_work_bytes);
+        bind(h, "nb200_gated_norm_bwd", a.gated_norm_bwd);
+        bind(h, "nb200_distill_loss", a.distill_loss);
+        bind(h, "nb200_distill_loss_bwd", a.distill_loss_bwd);
     });
     return a;
 }
@@ -314,6 +341,236 @@ std::tuple<at::Tensor, at::Tensor> attention_cuda(const at::Tensor& q, const at:
     return {o, lse};
 }
 
+// ------------------------------------------------------------------ training operators
+using OptTensor = std::optional<at::Tensor>;
+
+bool present(const OptTensor& t) { return t.has_value() && t->defined(); }
+
+// t itself when the attention kernels' copies can read its rows (unit stride in a row, positive 16-byte
+// multiples between rows, heads and batch elements, 16-byte aligned base), else a contiguous copy.
+at::Tensor attn_rows(const at::Tensor& t) {
+    bool ok = t.stride(3) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+    for (int i = 0; i < 3; ++i) ok = ok && (t.size(i) <= 1 || (t.stride(i) > 0 && t.stride(i) % 8 == 0));
+    return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+nb200_attn_strides attn_strides(const at::Tensor& t) { return {t.stride(0), t.stride(1), t.stride(2)}; }
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_bwd_cuda(const at::Tensor& q_, const at::Tensor& k_,
+                                                                  const at::Tensor& v_, const at::Tensor& o_,
+                                                                  const at::Tensor& lse_, const at::Tensor& go_,
+                                                                  const OptTensor& seq_lens, bool causal,
+                                                                  double scale) {
+    const char* what = "nb200.attention_bwd";
+    for (const at::Tensor* t : {&q_, &k_, &v_, &o_, &go_}) {
+        check_cuda(*t, what);
+        TORCH_CHECK_TYPE(t->scalar_type() == at::kBFloat16, what, ": q, k, v, o, grad_o must be bfloat16");
+        TORCH_CHECK_VALUE(t->dim() == 4 && t->device() == q_.device(), what, ": tensors must be 4-D on one device");
+    }
+    check_cuda(lse_, what);
+    TORCH_CHECK_VALUE(q_.sizes() == o_.sizes() && q_.sizes() == go_.sizes() && k_.sizes() == v_.sizes() &&
+                          q_.size(0) == k_.size(0) && q_.size(2) == k_.size(2) && q_.size(3) == k_.size(3),
+                      what, ": shapes differ");
+    TORCH_CHECK_VALUE(lse_.scalar_type() == at::kFloat && lse_.sizes() == q_.sizes().slice(0, 3), what,
+                      ": lse must be float32 [batch, heads, seq]");
+    c10::cuda::CUDAGuard guard(q_.device());
+    const at::Tensor q = attn_rows(q_), k = attn_rows(k_), v = attn_rows(v_), o = attn_rows(o_), go = attn_rows(go_);
+    const at::Tensor lse = lse_.contiguous();
+    at::Tensor dq = at::empty_like(q), dk = at::empty_like(k), dv = at::empty_like(v);
+    nb200_attn_args a = {q.size(0), q.size(1), k.size(1), q.size(2), q.size(3), nullptr, causal ? 1 : 0, (float)scale};
+    if (present(seq_lens)) {
+        check_cuda(*seq_lens, what);
+        TORCH_CHECK_VALUE(seq_lens->scalar_type() == at::kInt && seq_lens->dim() == 1 &&
+                              seq_lens->size(0) == q.size(0) && seq_lens->is_contiguous(),
+                          what, ": seq_lens must be contiguous int32 [batch]");
+        a.seq_lens = seq_lens->data_ptr<int32_t>();
+    }
+    const nb200_attn_strides strides[8] = {attn_strides(q),  attn_strides(k),  attn_strides(v),  attn_strides(o),
+                                           attn_strides(go), attn_strides(dq), attn_strides(dk), attn_strides(dv)};
+    const int64_t bytes = api().attention_bwd_work_bytes(&a);
+    if (bytes < 0) check((int)bytes, what);
+    at::Tensor work = at::empty({std::max<int64_t>(bytes, 16)}, q.options().dtype(at::kByte));
+    check(api().attention_bwd(&a, strides, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+                              lse.data_ptr<float>(), go.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                              work.data_ptr(), work.numel(), stream_of(q)),
+          what);
+    return {dq, dk, dv};
+}
+
+// [rows, last] of t with unit column stride: a copy only when no such view exists.
+at::Tensor unit_rows(const at::Tensor& t, int64_t rows) {
+    at::Tensor f = t.dim() == 2 && t.size(0) == rows ? t : t.reshape({rows, t.size(-1)});
+    return (f.stride(1) == 1 || f.size(1) == 1) && f.stride(0) >= 0 ? f : f.contiguous();
+}
+
+// The descriptor of a gated norm's inputs and the tensors whose memory it names.
+struct NormInputs {
+    nb200_norm_args a = {};
+    int dtype;
+    int64_t rows;
+    std::vector<at::Tensor> keep;
+    const void* row_input(const at::Tensor& t, const at::Tensor& like, int64_t n, int64_t* stride, const char* what) {
+        check_cuda(t, what);
+        TORCH_CHECK_TYPE(t.scalar_type() == like.scalar_type(), what, ": tensors must share one dtype");
+        TORCH_CHECK_VALUE(t.device() == like.device() && t.dim() >= 1 && t.size(-1) == like.size(-1) &&
+                              t.numel() == n * like.size(-1),
+                          what, ": tensors must be [..., width] on one device");
+        keep.push_back(unit_rows(t, n));
+        *stride = keep.back().stride(0);
+        return keep.back().data_ptr();
+    }
+    const void* weight(const OptTensor& t, const at::Tensor& like, const char* what) {
+        if (!present(t)) return nullptr;
+        check_cuda(*t, what);
+        TORCH_CHECK_TYPE(t->scalar_type() == like.scalar_type(), what, ": weights must have x's dtype");
+        TORCH_CHECK_VALUE(t->device() == like.device() && t->dim() == 1 && t->size(0) == like.size(-1), what,
+                          ": weights must be 1-D with x's last dimension");
+        keep.push_back(t->contiguous());
+        return keep.back().data_ptr();
+    }
+    NormInputs(const at::Tensor& x, const at::Tensor& residual, const OptTensor& gate, const OptTensor& post,
+               const OptTensor& pre, int64_t rows_per_gate, int64_t act, double scale, double eps, const char* what) {
+        dtype = dtype_code(x);
+        TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1 && rows_per_gate >= 1, what, ": x must be [..., width]");
+        rows = x.numel() / x.size(-1);
+        keep.reserve(7);
+        a.rows = rows;
+        a.width = x.size(-1);
+        a.x = row_input(x, x, rows, &a.stride_x, what);
+        a.residual = row_input(residual, x, rows, &a.stride_residual, what);
+        a.rows_per_gate = rows_per_gate;
+        if (present(gate)) {
+            TORCH_CHECK_VALUE(rows % rows_per_gate == 0, what, ": gate rows do not divide x's rows");
+            a.gate = row_input(*gate, x, rows / rows_per_gate, &a.stride_gate, what);
+        }
+        a.post_weight = weight(post, x, what);
+        a.pre_weight = weight(pre, x, what);
+        a.gate_act = (int32_t)act;
+        a.scale = scale;
+        a.eps = eps;
+    }
+};
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> gated_norm_cuda(const at::Tensor& x, const at::Tensor& residual,
+                                                               const OptTensor& gate, const OptTensor& post,
+                                                               const OptTensor& pre, int64_t rows_per_gate, int64_t act,
+                                                               double scale, double eps) {
+    const char* what = "nb200.gated_norm";
+    c10::cuda::CUDAGuard guard(x.device());
+    const NormInputs in(x, residual, gate, post, pre, rows_per_gate, act, scale, eps, what);
+    at::Tensor y = at::empty(x.sizes(), x.options()), h;
+    if (present(pre)) h = at::empty(x.sizes(), x.options());
+    std::vector<int64_t> shape = lead_shape(x, false);
+    shape.push_back(2);
+    at::Tensor rstd = at::empty(shape, x.options().dtype(at::kFloat));
+    check(api().gated_norm(&in.a, in.dtype, y.data_ptr(), h.defined() ? h.data_ptr() : nullptr, rstd.data_ptr<float>(),
+                           stream_of(x)),
+          what);
+    return {y, h, rstd};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> gated_norm_bwd_cuda(
+    const OptTensor& gy, const OptTensor& gh, const at::Tensor& x, const at::Tensor& residual, const OptTensor& gate,
+    const at::Tensor& rstd_, const OptTensor& post, const OptTensor& pre, int64_t rows_per_gate, int64_t act,
+    double scale) {
+    const char* what = "nb200.gated_norm_bwd";
+    c10::cuda::CUDAGuard guard(x.device());
+    NormInputs in(x, residual, gate, post, pre, rows_per_gate, act, scale, 1.0, what);
+    check_cuda(rstd_, what);
+    TORCH_CHECK_VALUE(rstd_.scalar_type() == at::kFloat && rstd_.numel() == 2 * in.rows, what,
+                      ": rstd must be float32 [..., 2]");
+    const at::Tensor rstd = rstd_.contiguous();
+    const void* dy = present(gy) ? in.row_input(*gy, x, in.rows, &in.a.stride_grad_y, what) : nullptr;
+    const void* dh = present(gh) ? in.row_input(*gh, x, in.rows, &in.a.stride_grad_h, what) : nullptr;
+    auto fresh = [&](const OptTensor& t) { return present(t) ? at::empty(t->sizes(), t->options()) : at::Tensor(); };
+    at::Tensor dx = at::empty(x.sizes(), x.options()), dr = at::empty(x.sizes(), x.options());
+    at::Tensor dgate = fresh(gate), dpost = fresh(post), dpre = fresh(pre);
+    auto ptr = [](const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+    const int64_t bytes = api().gated_norm_bwd_work_bytes(&in.a);
+    if (bytes < 0) check((int)bytes, what);
+    at::Tensor work = at::empty({std::max<int64_t>(bytes, 16)}, x.options().dtype(at::kByte));
+    check(api().gated_norm_bwd(&in.a, in.dtype, rstd.data_ptr<float>(), dy, dh, dx.data_ptr(), dr.data_ptr(),
+                               ptr(dgate), ptr(dpost), ptr(dpre), work.data_ptr(), work.numel(), stream_of(x)),
+          what);
+    return {dx, dr, dgate, dpost, dpre};
+}
+
+// The descriptor of a distillation loss's inputs and the tensors whose memory it names.
+struct DistillInputs {
+    nb200_distill_args a = {};
+    at::Tensor x, teacher, index;
+    DistillInputs(const at::Tensor& x_, const at::Tensor& teacher_, const at::Tensor& index_, double temperature,
+                  const char* what) {
+        check_cuda(x_, what);
+        check_cuda(teacher_, what);
+        check_cuda(index_, what);
+        TORCH_CHECK_VALUE(x_.dim() >= 1 && x_.size(-1) >= 1 && teacher_.sizes() == index_.sizes() &&
+                              teacher_.dim() == x_.dim() && teacher_.device() == x_.device() &&
+                              index_.device() == x_.device(),
+                          what, ": logits [..., vocab], teacher and index [..., top] on one device");
+        a.rows = x_.numel() / x_.size(-1);
+        a.vocab = x_.size(-1);
+        a.top = teacher_.size(-1);
+        TORCH_CHECK_VALUE(teacher_.numel() == a.rows * a.top, what, ": teacher rows differ from the logits'");
+        x = unit_rows(x_, a.rows);
+        teacher = unit_rows(teacher_, a.rows);
+        index = unit_rows(index_, a.rows);
+        a.x = x.data_ptr();
+        a.teacher = teacher.data_ptr();
+        a.index = index.data_ptr();
+        a.stride_x = x.stride(0);
+        a.stride_teacher = teacher.stride(0);
+        a.stride_index = index.stride(0);
+        a.dtype = dtype_code(x);
+        a.teacher_dtype = dtype_code(teacher);
+        a.index_dtype = index_code(index);
+        a.temperature = temperature;
+    }
+};
+
+std::tuple<at::Tensor, at::Tensor> distill_loss_cuda(const at::Tensor& x, const at::Tensor& teacher,
+                                                     const at::Tensor& index, double temperature,
+                                                     const OptTensor& teacher_lse) {
+    const char* what = "nb200.distill_loss";
+    c10::cuda::CUDAGuard guard(x.device());
+    const DistillInputs in(x, teacher, index, temperature, what);
+    std::vector<int64_t> shape = lead_shape(x, false);
+    const auto f32 = x.options().dtype(at::kFloat);
+    at::Tensor loss = at::empty(shape, f32), z;
+    shape.push_back(3);
+    at::Tensor stats = at::empty(shape, f32);
+    if (present(teacher_lse)) {
+        check_cuda(*teacher_lse, what);
+        TORCH_CHECK_VALUE(teacher_lse->scalar_type() == at::kFloat && teacher_lse->numel() == in.a.rows, what,
+                          ": teacher_lse must be float32 [...]");
+        z = teacher_lse->contiguous();
+    }
+    check(api().distill_loss(&in.a, z.defined() ? z.data_ptr<float>() : nullptr, loss.data_ptr<float>(),
+                             stats.data_ptr<float>(), stream_of(x)),
+          what);
+    return {loss, stats};
+}
+
+at::Tensor distill_loss_bwd_cuda(const at::Tensor& grad_, const at::Tensor& x, const at::Tensor& teacher,
+                                 const at::Tensor& index, const at::Tensor& stats_, double temperature) {
+    const char* what = "nb200.distill_loss_bwd";
+    c10::cuda::CUDAGuard guard(x.device());
+    const DistillInputs in(x, teacher, index, temperature, what);
+    check_cuda(grad_, what);
+    check_cuda(stats_, what);
+    TORCH_CHECK_VALUE(grad_.scalar_type() == at::kFloat && grad_.numel() == in.a.rows &&
+                          stats_.scalar_type() == at::kFloat && stats_.numel() == 3 * in.a.rows,
+                      what, ": grad must be float32 [...], stats float32 [..., 3]");
+    at::Tensor grad = grad_.reshape({-1});
+    if (grad.stride(0) < 0) grad = grad.contiguous();
+    const at::Tensor stats = stats_.contiguous();
+    at::Tensor dx = at::empty(x.sizes(), x.options());
+    check(api().distill_loss_bwd(&in.a, grad.data_ptr<float>(), grad.stride(0), stats.data_ptr<float>(), dx.data_ptr(),
+                                 stream_of(x)),
+          what);
+    return dx;
+}
+
 // ------------------------------------------------------------------ Meta kernels (shapes only)
 // Symbolic sizes throughout, so graphs exported with dynamic dimensions trace through these ops.
 std::vector<c10::SymInt> lead_sym_shape(const at::Tensor& x, bool keepdim) {
@@ -420,6 +677,24 @@ TORCH_LIBRARY(nb200, m) {
     m.def("segment_status(int device, bool clear) -> int", &segment_status);
     m.def("segment_status_word(int device) -> Tensor", &segment_status_word);
     m.def("attention(Tensor q, Tensor k, Tensor v, bool causal, float scale) -> (Tensor, Tensor)");
+    m.def("attention_bwd(Tensor q, Tensor k, Tensor v, Tensor o, Tensor lse, Tensor grad_o, Tensor? seq_lens, "
+          "bool causal, float scale) -> (Tensor, Tensor, Tensor)");
+    m.def("gated_norm(Tensor x, Tensor residual, Tensor? gate, Tensor? post, Tensor? pre, int rows_per_gate, int act, "
+          "float scale, float eps) -> (Tensor, Tensor, Tensor)");
+    m.def("gated_norm_bwd(Tensor? grad_y, Tensor? grad_h, Tensor x, Tensor residual, Tensor? gate, Tensor rstd, "
+          "Tensor? post, Tensor? pre, int rows_per_gate, int act, float scale) "
+          "-> (Tensor, Tensor, Tensor, Tensor, Tensor)");
+    m.def("distill_loss(Tensor x, Tensor teacher, Tensor index, float temperature, Tensor? teacher_lse) "
+          "-> (Tensor, Tensor)");
+    m.def("distill_loss_bwd(Tensor grad, Tensor x, Tensor teacher, Tensor index, Tensor stats, float temperature) "
+          "-> Tensor");
+}
+
+// The training operators are their own gradients' building blocks: autograd records nothing for them (the
+// Python layer's autograd functions call them).
+TORCH_LIBRARY_IMPL(nb200, Autograd, m) {
+    for (const char* op : {"attention_bwd", "gated_norm", "gated_norm_bwd", "distill_loss", "distill_loss_bwd"})
+        m.impl(op, torch::CppFunction::makeFallthrough());
 }
 
 TORCH_LIBRARY_IMPL(nb200, CUDA, m) {
@@ -429,6 +704,11 @@ TORCH_LIBRARY_IMPL(nb200, CUDA, m) {
     m.impl("rms_norm", &rms_cuda);
     m.impl("segment_pool", &segment_cuda);
     m.impl("attention", &attention_cuda);
+    m.impl("attention_bwd", &attention_bwd_cuda);
+    m.impl("gated_norm", &gated_norm_cuda);
+    m.impl("gated_norm_bwd", &gated_norm_bwd_cuda);
+    m.impl("distill_loss", &distill_loss_cuda);
+    m.impl("distill_loss_bwd", &distill_loss_bwd_cuda);
 }
 
 TORCH_LIBRARY_IMPL(nb200, Meta, m) {

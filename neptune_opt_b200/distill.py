@@ -18,11 +18,10 @@ parameters, NotImplementedError past the kernels' kept entries per row.
 """
 from __future__ import annotations
 
-import ctypes
 import math
 
-from neptune_opt_b200 import _lib
-from neptune_opt_b200.template import _is_metadata, _on_device, current_stream, dtype_code
+from neptune_opt_b200.template import _is_metadata
+from neptune_opt_b200.torch_op import cxx_op
 
 MAX_TOP = 256
 
@@ -60,24 +59,6 @@ def validate_distill_inputs(logits, teacher_logits, teacher_index, temperature, 
         raise NotImplementedError(f"{what}: {teacher_logits.shape[-1]} kept logits per row exceed {MAX_TOP}")
 
 
-def _flat(t, rows):
-    """[rows, last] of t with unit column stride (a copy only when no such view exists)."""
-    t2 = t.reshape(rows, t.shape[-1])
-    if t2.stride(1) != 1 and t2.shape[1] > 1 or t2.stride(0) < 0:
-        t2 = t2.contiguous()
-    return t2
-
-
-def _args(logits, teacher_logits, teacher_index, temperature):
-    """(nb200_distill_args, the tensors whose memory it names)."""
-    rows = math.prod(logits.shape[:-1])
-    x, t, i = keep = [_flat(a, rows) for a in (logits, teacher_logits, teacher_index)]
-    a = _lib.NB200DistillArgs(x.data_ptr(), t.data_ptr(), i.data_ptr(), rows, x.shape[1], t.shape[1], x.stride(0),
-                              t.stride(0), i.stride(0), dtype_code(x.dtype), dtype_code(t.dtype),
-                              _lib.INDEX_CODES[str(i.dtype).removeprefix("torch.")], temperature)
-    return a, keep
-
-
 def run_distill_loss(logits, teacher_logits, teacher_index, *, temperature: float = 1.0, teacher_lse=None):
     """(loss [...], stats [..., 3]) in fp32; stats holds each row's logsumexp(logits / T), teacher
     normaliser Z and kept mass, which the backward pass takes. teacher_lse [...] is the teacher's
@@ -85,18 +66,10 @@ def run_distill_loss(logits, teacher_logits, teacher_index, *, temperature: floa
     import torch
 
     validate_distill_inputs(logits, teacher_logits, teacher_index, temperature, teacher_lse)
-    loss = torch.empty(logits.shape[:-1], device=logits.device, dtype=torch.float32)
-    stats = torch.empty((*logits.shape[:-1], 3), device=logits.device, dtype=torch.float32)
-    if _is_metadata(logits) or loss.numel() == 0:
-        return loss, stats
-    a, keep = _args(logits, teacher_logits, teacher_index, temperature)
-    z = None if teacher_lse is None else teacher_lse.contiguous()
-    lib = _lib.load()
-    with _on_device(logits.device):
-        rc = lib.nb200_distill_loss(ctypes.byref(a), None if z is None else z.data_ptr(), loss.data_ptr(),
-                                    stats.data_ptr(), current_stream(logits.device))
-    _lib.check(rc, "nb200_distill_loss")
-    return loss, stats
+    if not _is_metadata(logits) and logits.numel():
+        return cxx_op("distill_loss")(logits, teacher_logits, teacher_index, temperature, teacher_lse)
+    return (torch.empty(logits.shape[:-1], device=logits.device, dtype=torch.float32),
+            torch.empty((*logits.shape[:-1], 3), device=logits.device, dtype=torch.float32))
 
 
 def distill_loss_backward(grad, logits, teacher_logits, teacher_index, stats, *, temperature: float = 1.0):
@@ -110,17 +83,9 @@ def distill_loss_backward(grad, logits, teacher_logits, teacher_index, stats, *,
             raise TypeError(f"distill_loss_backward: {name} must be a float32 tensor")
         if tuple(t.shape) != tuple(shape) or t.device != logits.device:
             raise ValueError(f"distill_loss_backward: {name} must be {tuple(shape)} on the device of logits")
-    dx = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
-    if _is_metadata(logits) or dx.numel() == 0:
-        return dx
-    a, keep = _args(logits, teacher_logits, teacher_index, temperature)
-    grad, stats = grad.reshape(-1), stats.contiguous()
-    lib = _lib.load()
-    with _on_device(logits.device):
-        rc = lib.nb200_distill_loss_bwd(ctypes.byref(a), grad.data_ptr(), grad.stride(0), stats.data_ptr(),
-                                        dx.data_ptr(), current_stream(logits.device))
-    _lib.check(rc, "nb200_distill_loss_bwd")
-    return dx
+    if not _is_metadata(logits) and logits.numel():
+        return cxx_op("distill_loss_bwd")(grad, logits, teacher_logits, teacher_index, stats, temperature)
+    return torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
 
 
 _FUNCTION = None

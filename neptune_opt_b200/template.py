@@ -63,9 +63,13 @@ def _row_last_layout(x):
 
 
 def _is_metadata(x) -> bool:
+    import torch
+
+    if type(x) is torch.Tensor:
+        return x.is_meta
     from torch._subclasses.fake_tensor import FakeTensor
 
-    return isinstance(x, FakeTensor) or x.device.type == "meta"
+    return isinstance(x, FakeTensor) or x.is_meta
 
 
 _DTYPE_CODES: dict = {}

@@ -56,6 +56,17 @@ def _nb200():
     return torch.ops.nb200
 
 
+_CXX_OPS: dict[str, object] = {}
+
+
+def cxx_op(name: str):
+    """The overload of a C++-registered nb200 op (resolved once)."""
+    op = _CXX_OPS.get(name)
+    if op is None:
+        op = _CXX_OPS[name] = getattr(_nb200(), name).default
+    return op
+
+
 def _tracing(*tensors) -> bool:
     """True while fake, meta or functional tensors trace the op (export, AOTInductor, FakeTensorMode)."""
     from torch._subclasses.fake_tensor import FakeTensor
