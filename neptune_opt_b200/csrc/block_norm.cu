@@ -58,10 +58,10 @@ struct Rows {
     static constexpr int V = CH::V, P = CH::E / 2;  // P pairs a thread
     int t, G;
     int64_t unit, width;
-    float4* buf;  // 2 x 32 entries of shared memory when CTA
+    float* buf;  // 2 x 4 x 32 entries of shared memory when CTA
     int phase = 0;
 
-    __device__ __forceinline__ Rows(int64_t w, float4* b) : width(w), buf(b) {
+    __device__ __forceinline__ Rows(int64_t w, float* b) : width(w), buf(b) {
         t = threadIdx.x;
         G = blockDim.x;
         unit = CTA ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
@@ -80,22 +80,42 @@ struct Rows {
             store_vec<T, NV, VEC>(row, f, k, 0, width, t, G, VEC);
         }
     }
-    // Sums of up to three values over the row's threads, in every thread: warp shuffles, then the warps' sums
-    // in warp order (one barrier; the two buffers alternate).
-    template <int N>
-    __device__ __forceinline__ void sum(float* v) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = warp_sum(v[i]);
+    // The sum of v over the row's threads, in every thread: warp shuffles, then the warps' sums (one
+    // barrier; the two buffers alternate).
+    __device__ __forceinline__ float sum(float v) {
+        v = warp_sum(v);
         if constexpr (CTA) {
-            float4* slot = buf + (phase ^= 1) * 32;
-            const int warps = G >> 5;
-            if ((t & 31) == 0) slot[t >> 5] = make_float4(v[0], N > 1 ? v[1] : 0.f, N > 2 ? v[2] : 0.f, 0.f);
+            float* slot = buf + (phase ^= 1) * 4 * 32;
+            if ((t & 31) == 0) slot[t >> 5] = v;
             __syncthreads();
-            float4 w = (t & 31) < warps ? slot[t & 31] : make_float4(0.f, 0.f, 0.f, 0.f);
-            v[0] = warp_sum(w.x);
-            if (N > 1) v[1] = warp_sum(w.y);
-            if (N > 2) v[2] = warp_sum(w.z);
+            v = warp_sum((t & 31) < (G >> 5) ? slot[t & 31] : 0.f);
         }
+        return v;
+    }
+    // Three sums at once. Each of the first two shuffle rounds halves the number of values a lane carries (it
+    // keeps its half of them and adds the partner's), so six shuffles do what fifteen would.
+    __device__ __forceinline__ void sum3(float& a, float& b, float& c) {
+        const bool hi = t & 16, odd = t & 8;
+        float k0 = hi ? c : a, k1 = hi ? 0.f : b;  // kept: (a, b) below lane 16, (c, -) above
+        k0 += __shfl_xor_sync(0xffffffffu, hi ? a : c, 16);
+        k1 += __shfl_xor_sync(0xffffffffu, hi ? b : 0.f, 16);
+        float v = odd ? k1 : k0;  // lanes 0-7 a, 8-15 b, 16-23 c
+        v += __shfl_xor_sync(0xffffffffu, odd ? k0 : k1, 8);
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        if constexpr (CTA) {
+            float* slot = buf + (phase ^= 1) * 4 * 32;
+            const int which = (t & 31) >> 3, warps = G >> 5;
+            if ((t & 7) == 0) slot[which * 32 + (t >> 5)] = v;
+            __syncthreads();
+            v = 0.f;
+            for (int w = t & 7; w < warps; w += 8) v += slot[which * 32 + w];
+#pragma unroll
+            for (int o = 4; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        }
+        a = __shfl_sync(0xffffffffu, v, 0);
+        b = __shfl_sync(0xffffffffu, v, 8);
+        c = __shfl_sync(0xffffffffu, v, 16);
     }
 };
 
@@ -115,13 +135,13 @@ struct GatePos {
 };
 
 template <typename T, int NV, bool VEC, bool CTA, int kThreads>
-__global__ void __launch_bounds__(kThreads) norm_fwd_kernel(const T* x, const T* res, const T* gate, const T* w1,
-                                                            const T* w2, Norm n, int64_t per_unit, T* y, T* h,
-                                                            float* rstd) {
+__global__ void __launch_bounds__(kThreads, NV * Elem<T>::V == 8 ? 1024 / kThreads : 1)
+    norm_fwd_kernel(const T* x, const T* res, const T* gate, const T* w1, const T* w2, Norm n, int64_t per_unit, T* y,
+                    T* h, float* rstd) {
     using R = Rows<T, NV, VEC, CTA>;
     using CH = typename R::CH;
     constexpr int P = R::P;
-    __shared__ float4 buf[CTA ? 64 : 1];
+    __shared__ float buf[CTA ? 256 : 1];
     R r(n.width, buf);
     int64_t row = r.unit * per_unit;
     const int64_t end = min(row + per_unit, n.rows);
@@ -163,7 +183,7 @@ __global__ void __launch_bounds__(kThreads) norm_fwd_kernel(const T* x, const T*
 #pragma unroll
             for (int i = 0; i < P; ++i) acc = fma2(R::pair(cx, i), R::pair(cx, i), acc);
             float s = f2lo(acc) + f2hi(acc);
-            r.template sum<1>(&s);
+            s = r.sum(s);
             r1 = rsqrtf(s * n.inv_n + n.eps);
         }
         uint64_t v[P];
@@ -176,7 +196,7 @@ __global__ void __launch_bounds__(kThreads) norm_fwd_kernel(const T* x, const T*
         r.store(y + row * n.width, v);
         if (w2) {
             float s = f2lo(acc) + f2hi(acc);
-            r.template sum<1>(&s);
+            s = r.sum(s);
             r2 = rsqrtf(s * n.inv_n + n.eps);
 #pragma unroll
             for (int i = 0; i < P; ++i) v[i] = mul2(v[i], mul2(R::pair(c2, i), f2(r2, r2)));
@@ -232,14 +252,14 @@ __device__ __forceinline__ void store_part(float* part, const uint64_t* acc, con
 // Within a gate group the gate and post-weight gradients share one column sum, G = sum xhat dY:
 // dgate = scale a' w1 G and dw1 += scale a G.
 template <typename T, int NV, bool VEC, bool CTA, int kThreads>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, NV * Elem<T>::V == 8 ? 1024 / kThreads : 1)
     norm_bwd_kernel(const T* dy, const T* dh, const T* x, const T* res, const T* gate, const T* w1, const T* w2,
                     const float* rstd, Norm n, Chunks ch, T* dx, T* dres, T* dgate, float* part1, float* part2,
                     float* partg) {
     using R = Rows<T, NV, VEC, CTA>;
     using CH = typename R::CH;
     constexpr int P = R::P;
-    __shared__ float4 buf[CTA ? 64 : 1];
+    __shared__ float buf[CTA ? 256 : 1];
     pdl_trigger();
     R r(n.width, buf);
     if (r.unit >= ch.count) return;
@@ -248,9 +268,19 @@ __global__ void __launch_bounds__(kThreads)
     CH c1, c2, cg;
     if (w1) r.load(c1, w1, false);
     if (w2) r.load(c2, w2, false);
-    uint64_t b[P], G[P], a1[P], a2[P];
+    // The post weight's sums are touched once per gate group and live in shared memory, for the wide shapes
+    // the pre weight's as well: registers decide how many rows an SM has in flight.
+    constexpr bool kWide = P > 4;
+    extern __shared__ uint64_t shared_acc[];
+    uint64_t* a1 = shared_acc + (CTA ? 0 : threadIdx.y * r.G * P) + r.t;
+    uint64_t* a2s = a1 + (CTA ? 1 : kWarpRows) * r.G * P;
+    uint64_t b[P], G[P], a2[P];
 #pragma unroll
-    for (int i = 0; i < P; ++i) G[i] = a1[i] = a2[i] = 0;
+    for (int i = 0; i < P; ++i) {
+        G[i] = a2[i] = 0;
+        a1[i * r.G] = 0;
+        if (kWide) a2s[i * r.G] = 0;
+    }
     GatePos g(row, n.group);
     bool fresh = true;
     for (; row < end; ++row) {
@@ -285,15 +315,18 @@ __global__ void __launch_bounds__(kThreads)
             s2 = fma2(c, e[i], s2);
             s3 = fma2(c, yhat[i], s3);
         }
-        float s[3] = {f2lo(s1) + f2hi(s1), f2lo(s2) + f2hi(s2), f2lo(s3) + f2hi(s3)};
-        r.template sum<3>(s);
-        const float k2 = r2 * s[0] * n.inv_n, m1 = (s[1] - k2 * s[2]) * n.inv_n;  // k2 = r2 m2
+        float t1 = f2lo(s1) + f2hi(s1), t2 = f2lo(s2) + f2hi(s2), t3 = f2lo(s3) + f2hi(s3);
+        r.sum3(t1, t2, t3);
+        const float k2 = r2 * t1 * n.inv_n, m1 = (t2 - k2 * t3) * n.inv_n;  // k2 = r2 m2
         const uint64_t k2p = f2(-k2, -k2), k1p = f2(w1 ? -m1 : 0.f, w1 ? -m1 : 0.f);
 #pragma unroll
         for (int i = 0; i < P; ++i) {
             const uint64_t xhat = mul2(R::pair(cx, i), r1p);
             if (w2) e[i] = fma2(yhat[i], k2p, e[i]);  // dY
-            if (dh) a2[i] = fma2(R::pair(cdh, i), yhat[i], a2[i]);
+            if (dh) {
+                if (kWide) a2s[i * r.G] = fma2(R::pair(cdh, i), yhat[i], a2s[i * r.G]);
+                else a2[i] = fma2(R::pair(cdh, i), yhat[i], a2[i]);
+            }
             G[i] = fma2(xhat, e[i], G[i]);
             yhat[i] = mul2(fma2(xhat, k1p, mul2(b[i], e[i])), r1p);  // dx
         }
@@ -312,7 +345,7 @@ __global__ void __launch_bounds__(kThreads)
                     const float hi = gate_value(cg.get(2 * i + 1), n.act, da[1]);
                     a = mul2(a, f2(lo, hi));
                 }
-                a1[i] = fma2(a, G[i], a1[i]);
+                a1[i * r.G] = fma2(a, G[i], a1[i * r.G]);
                 G[i] = mul2(G[i], mul2(f2(n.scale * da[0], n.scale * da[1]), w1 ? R::pair(c1, i) : f2(1.f, 1.f)));
             }
             if (direct) r.store(dgate + (g.index - (fresh ? 1 : 0)) * n.width, G);
@@ -321,8 +354,17 @@ __global__ void __launch_bounds__(kThreads)
             for (int i = 0; i < P; ++i) G[i] = 0;
         }
     }
-    if (part1) store_part(part1 + r.unit * n.width, a1, r);
-    if (part2) store_part(part2 + r.unit * n.width, a2, r);
+    if (part2) {
+#pragma unroll
+        for (int i = 0; i < P; ++i)
+            if (kWide) a2[i] = a2s[i * r.G];
+        store_part(part2 + r.unit * n.width, a2, r);
+    }
+    if (part1) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) b[i] = a1[i * r.G];
+        store_part(part1 + r.unit * n.width, b, r);
+    }
     if (partg) store_part(partg + r.unit * n.width, G, r);
 }
 
@@ -458,7 +500,9 @@ int norm_bwd(const nb200_norm_args& a, const float* rstd, const T* dy, const T* 
     dispatch(s, [&](auto cta, auto e, auto vec, auto most) {
         auto kernel = norm_bwd_kernel<T, decltype(e)::value / Elem<T>::V, decltype(vec)::value, decltype(cta)::value,
                                       decltype(most)::value>;
-        kernel<<<(unsigned)((ch.count + per - 1) / per), dim3(s.threads, per), 0, st>>>(
+        const int smem = (s.wide ? 2 : 1) * per * s.threads * decltype(e)::value * (int)sizeof(float);
+        if (smem > 48 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        kernel<<<(unsigned)((ch.count + per - 1) / per), dim3(s.threads, per), smem, st>>>(
             dy, dh, static_cast<const T*>(a.x), static_cast<const T*>(a.residual), static_cast<const T*>(a.gate),
             static_cast<const T*>(a.post_weight), static_cast<const T*>(a.pre_weight), rstd, n, ch, dx, dres, dgate,
             p1, p2, pg);
