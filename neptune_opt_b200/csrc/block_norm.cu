@@ -15,6 +15,7 @@
 // gate groups, whose gate gradients it writes itself, or a part of one group. Weight gradients (and the
 // gate's, when a group spans chunks) leave as one fp32 row per chunk, summed in chunk order by a
 // second kernel, so results do not depend on scheduling.
+#include <algorithm>
 #include <type_traits>
 
 #include "common.cuh"
@@ -251,30 +252,38 @@ __device__ __forceinline__ void store_part(float* part, const uint64_t* acc, con
 //   n m2 = sum t yhat,   n m1 = sum c dY = sum c (dy + r2 t) - r2 m2 sum c yhat.
 // Within a gate group the gate and post-weight gradients share one column sum, G = sum xhat dY:
 // dgate = scale a' w1 G and dw1 += scale a G.
+//
+// The next row's four operands are on their way in registers while a row is computed (AHEAD, 8 elements a
+// thread). That takes one CTA of 512 threads per SM; two at 64 registers a thread, with or without a ring of
+// bulk copies in shared memory in place of the registers, spilled and ran slower (bf16 [16384, 4096]: 250
+// and 294 us).
 template <typename T, int NV, bool VEC, bool CTA, int kThreads>
-__global__ void __launch_bounds__(kThreads, NV * Elem<T>::V == 8 ? 1024 / kThreads : 1)
+__global__ void __launch_bounds__(kThreads)
     norm_bwd_kernel(const T* dy, const T* dh, const T* x, const T* res, const T* gate, const T* w1, const T* w2,
                     const float* rstd, Norm n, Chunks ch, T* dx, T* dres, T* dgate, float* part1, float* part2,
                     float* partg) {
     using R = Rows<T, NV, VEC, CTA>;
     using CH = typename R::CH;
     constexpr int P = R::P;
+    constexpr bool AHEAD = P == 4;
     __shared__ float buf[CTA ? 256 : 1];
-    pdl_trigger();
+    extern __shared__ __align__(16) uint8_t dyn[];
     R r(n.width, buf);
+    // What a thread keeps across rows but touches little lives in shared memory, in slots of its own: b = scale
+    // a(gate) w1 and the post weight's sums (touched once per gate group), for the wide shapes the pre
+    // weight's sums as well. Gate and post weight are read again where a group ends.
+    constexpr bool kWide = P > 4;
+    const int slots = (CTA ? 1 : kWarpRows) * r.G * P;
+    uint64_t* bs = reinterpret_cast<uint64_t*>(dyn) + (CTA ? 0 : threadIdx.y * r.G * P) + r.t;
+    uint64_t* a1 = bs + slots;
+    uint64_t* a2s = a1 + slots;
+    pdl_trigger();
     if (r.unit >= ch.count) return;
     int64_t row, end;
     ch.range(r.unit, n, row, end);
-    CH c1, c2, cg;
-    if (w1) r.load(c1, w1, false);
+    CH c2;
     if (w2) r.load(c2, w2, false);
-    // The post weight's sums are touched once per gate group and live in shared memory, for the wide shapes
-    // the pre weight's as well: registers decide how many rows an SM has in flight.
-    constexpr bool kWide = P > 4;
-    extern __shared__ uint64_t shared_acc[];
-    uint64_t* a1 = shared_acc + (CTA ? 0 : threadIdx.y * r.G * P) + r.t;
-    uint64_t* a2s = a1 + (CTA ? 1 : kWarpRows) * r.G * P;
-    uint64_t b[P], G[P], a2[P];
+    uint64_t G[P], a2[P];
 #pragma unroll
     for (int i = 0; i < P; ++i) {
         G[i] = a2[i] = 0;
@@ -283,14 +292,23 @@ __global__ void __launch_bounds__(kThreads, NV * Elem<T>::V == 8 ? 1024 / kThrea
     }
     GatePos g(row, n.group);
     bool fresh = true;
+    CH nx, nr, ndy, ndh;
+    float2 nrs;
+    auto fetch = [&](int64_t i) {
+        nrs = *reinterpret_cast<const float2*>(rstd + 2 * i);
+        r.load(nx, x + i * n.sx, true);
+        r.load(nr, res + i * n.sr, true);
+        if (dy) r.load(ndy, dy + i * n.sdy, true);
+        if (dh) r.load(ndh, dh + i * n.sdh, true);
+    };
+    if (AHEAD) fetch(row);
     for (; row < end; ++row) {
-        CH cx, cr, cdy, cdh;
-        r.load(cx, x + row * n.sx, true);
-        r.load(cr, res + row * n.sr, true);
-        if (dy) r.load(cdy, dy + row * n.sdy, true);
-        if (dh) r.load(cdh, dh + row * n.sdh, true);
-        const float2 rs = *reinterpret_cast<const float2*>(rstd + 2 * row);
+        if (!AHEAD) fetch(row);
+        const CH cx = nx, cr = nr, cdy = ndy, cdh = ndh;
+        const float2 rs = nrs;
         if (fresh) {
+            CH c1, cg;
+            if (w1) r.load(c1, w1, false);
             if (gate) r.load(cg, gate + g.index * n.sg, false);
 #pragma unroll
             for (int i = 0; i < P; ++i) {
@@ -298,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, NV * Elem<T>::V == 8 ? 1024 / kThrea
                 const uint64_t a = gate ? f2(n.scale * gate_value(cg.get(2 * i), n.act, slope),
                                              n.scale * gate_value(cg.get(2 * i + 1), n.act, slope))
                                         : f2(n.scale, n.scale);
-                b[i] = w1 ? mul2(a, R::pair(c1, i)) : a;
+                bs[i * r.G] = w1 ? mul2(a, R::pair(c1, i)) : a;
             }
         }
         const float r1 = w1 ? rs.x : 1.f, r2 = w2 ? rs.y : 1.f;
@@ -307,7 +325,7 @@ __global__ void __launch_bounds__(kThreads, NV * Elem<T>::V == 8 ? 1024 / kThrea
         uint64_t s1 = 0, s2 = 0, s3 = 0;
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-            const uint64_t c = mul2(b[i], mul2(R::pair(cx, i), r1p));
+            const uint64_t c = mul2(bs[i * r.G], mul2(R::pair(cx, i), r1p));
             yhat[i] = mul2(add2(c, R::pair(cr, i)), r2p);
             const uint64_t t = dh ? mul2(R::pair(cdh, i), R::pair(c2, i)) : 0;
             e[i] = fma2(t, r2p, dy ? R::pair(cdy, i) : 0);
@@ -315,6 +333,8 @@ __global__ void __launch_bounds__(kThreads, NV * Elem<T>::V == 8 ? 1024 / kThrea
             s2 = fma2(c, e[i], s2);
             s3 = fma2(c, yhat[i], s3);
         }
+        // Issued here, the loads cover the sums' latency.
+        if (AHEAD && row + 1 < end) fetch(row + 1);
         float t1 = f2lo(s1) + f2hi(s1), t2 = f2lo(s2) + f2hi(s2), t3 = f2lo(s3) + f2hi(s3);
         r.sum3(t1, t2, t3);
         const float k2 = r2 * t1 * n.inv_n, m1 = (t2 - k2 * t3) * n.inv_n;  // k2 = r2 m2
@@ -328,7 +348,7 @@ __global__ void __launch_bounds__(kThreads, NV * Elem<T>::V == 8 ? 1024 / kThrea
                 else a2[i] = fma2(R::pair(cdh, i), yhat[i], a2[i]);
             }
             G[i] = fma2(xhat, e[i], G[i]);
-            yhat[i] = mul2(fma2(xhat, k1p, mul2(b[i], e[i])), r1p);  // dx
+            yhat[i] = mul2(fma2(xhat, k1p, mul2(bs[i * r.G], e[i])), r1p);  // dx
         }
         r.store(dres + row * n.width, e);
         r.store(dx + row * n.width, yhat);
@@ -336,6 +356,10 @@ __global__ void __launch_bounds__(kThreads, NV * Elem<T>::V == 8 ? 1024 / kThrea
         fresh = gate && g.next(n.group);
         if (fresh || row + 1 == end) {
             const bool direct = gate && !partg;
+            const int64_t ended = g.index - (fresh ? 1 : 0);
+            CH c1, cg;
+            if (w1) r.load(c1, w1, false);
+            if (gate) r.load(cg, gate + ended * n.sg, false);
 #pragma unroll
             for (int i = 0; i < P; ++i) {
                 float da[2] = {0.f, 0.f};
@@ -348,7 +372,7 @@ __global__ void __launch_bounds__(kThreads, NV * Elem<T>::V == 8 ? 1024 / kThrea
                 a1[i * r.G] = fma2(a, G[i], a1[i * r.G]);
                 G[i] = mul2(G[i], mul2(f2(n.scale * da[0], n.scale * da[1]), w1 ? R::pair(c1, i) : f2(1.f, 1.f)));
             }
-            if (direct) r.store(dgate + (g.index - (fresh ? 1 : 0)) * n.width, G);
+            if (direct) r.store(dgate + ended * n.width, G);
             if (row + 1 == end) break;
 #pragma unroll
             for (int i = 0; i < P; ++i) G[i] = 0;
@@ -362,8 +386,8 @@ __global__ void __launch_bounds__(kThreads, NV * Elem<T>::V == 8 ? 1024 / kThrea
     }
     if (part1) {
 #pragma unroll
-        for (int i = 0; i < P; ++i) b[i] = a1[i * r.G];
-        store_part(part1 + r.unit * n.width, b, r);
+        for (int i = 0; i < P; ++i) a2[i] = a1[i * r.G];
+        store_part(part1 + r.unit * n.width, a2, r);
     }
     if (partg) store_part(partg + r.unit * n.width, G, r);
 }
@@ -500,7 +524,7 @@ int norm_bwd(const nb200_norm_args& a, const float* rstd, const T* dy, const T* 
     dispatch(s, [&](auto cta, auto e, auto vec, auto most) {
         auto kernel = norm_bwd_kernel<T, decltype(e)::value / Elem<T>::V, decltype(vec)::value, decltype(cta)::value,
                                       decltype(most)::value>;
-        const int smem = (s.wide ? 2 : 1) * per * s.threads * decltype(e)::value * (int)sizeof(float);
+        const int smem = (s.wide ? 3 : 2) * per * s.threads * decltype(e)::value * (int)sizeof(float);
         if (smem > 48 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         kernel<<<(unsigned)((ch.count + per - 1) / per), dim3(s.threads, per), smem, st>>>(
             dy, dh, static_cast<const T*>(a.x), static_cast<const T*>(a.residual), static_cast<const T*>(a.gate),

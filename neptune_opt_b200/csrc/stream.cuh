@@ -12,8 +12,8 @@
 
 namespace nb200 {
 
-// Set (bitwise OR) by streaming kernels whose bounded wait ran out; read and cleared by the host
-// (stream.cu, the one translation unit that includes this header).
+// Set (bitwise OR) by streaming kernels whose bounded wait ran out; one word per kernel file, read and
+// cleared by the host.
 static __device__ unsigned int g_stream_fault = 0u;
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
