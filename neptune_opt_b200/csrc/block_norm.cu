@@ -34,20 +34,16 @@ struct Norm {
     int act;
 };
 
-// a(g) and its derivative.
-__device__ __forceinline__ float gate_value(float g, int kind, float& slope) {
-    if (kind == NB200_GATE_TANH) {
-        const float a = tanhf(g);
-        slope = 1.f - a * a;
-        return a;
-    }
-    if (kind == NB200_GATE_SIGMOID) {
-        const float a = 1.f / (1.f + expf(-g));
-        slope = a * (1.f - a);
-        return a;
-    }
-    slope = 1.f;
+// a(g), and its derivative in terms of a.
+__device__ __forceinline__ float gate_value(float g, int kind) {
+    if (kind == NB200_GATE_TANH) return tanhf(g);
+    if (kind == NB200_GATE_SIGMOID) return 1.f / (1.f + expf(-g));
     return g;
+}
+__device__ __forceinline__ float gate_slope(float a, int kind) {
+    if (kind == NB200_GATE_TANH) return 1.f - a * a;
+    if (kind == NB200_GATE_SIGMOID) return a * (1.f - a);
+    return 1.f;
 }
 
 // A row is held by a warp (CTA false, kWarpRows of them in a CTA) or a whole CTA, E = NV * V elements a
@@ -160,9 +156,8 @@ __global__ void __launch_bounds__(kThreads, NV * Elem<T>::V == 8 ? 1024 / kThrea
         if (fresh) {
 #pragma unroll
             for (int i = 0; i < P; ++i) {
-                float slope;
-                const uint64_t a = gate ? f2(n.scale * gate_value(cg.get(2 * i), n.act, slope),
-                                             n.scale * gate_value(cg.get(2 * i + 1), n.act, slope))
+                const uint64_t a = gate ? f2(n.scale * gate_value(cg.get(2 * i), n.act),
+                                             n.scale * gate_value(cg.get(2 * i + 1), n.act))
                                         : f2(n.scale, n.scale);
                 b[i] = w1 ? mul2(a, R::pair(c1, i)) : a;
             }
@@ -269,14 +264,13 @@ __global__ void __launch_bounds__(kThreads)
     __shared__ float buf[CTA ? 256 : 1];
     extern __shared__ __align__(16) uint8_t dyn[];
     R r(n.width, buf);
-    // What a thread keeps across rows but touches little lives in shared memory, in slots of its own: b = scale
-    // a(gate) w1 and the post weight's sums (touched once per gate group), for the wide shapes the pre
-    // weight's sums as well. Gate and post weight are read again where a group ends.
-    constexpr bool kWide = P > 4;
+    // What a thread keeps across rows but touches little lives in shared memory, in slots of its own: scale
+    // What a thread keeps across rows but touches little lives in shared memory, in slots of its own:
+    // a(gate), b = scale a(gate) w1 and the post weight's sums (touched once per gate group).
     const int slots = (CTA ? 1 : kWarpRows) * r.G * P;
     uint64_t* bs = reinterpret_cast<uint64_t*>(dyn) + (CTA ? 0 : threadIdx.y * r.G * P) + r.t;
-    uint64_t* a1 = bs + slots;
-    uint64_t* a2s = a1 + slots;
+    uint64_t* as = bs + slots;
+    uint64_t* a1 = as + slots;
     pdl_trigger();
     if (r.unit >= ch.count) return;
     int64_t row, end;
@@ -288,7 +282,6 @@ __global__ void __launch_bounds__(kThreads)
     for (int i = 0; i < P; ++i) {
         G[i] = a2[i] = 0;
         a1[i * r.G] = 0;
-        if (kWide) a2s[i * r.G] = 0;
     }
     GatePos g(row, n.group);
     bool fresh = true;
@@ -312,10 +305,10 @@ __global__ void __launch_bounds__(kThreads)
             if (gate) r.load(cg, gate + g.index * n.sg, false);
 #pragma unroll
             for (int i = 0; i < P; ++i) {
-                float slope;
-                const uint64_t a = gate ? f2(n.scale * gate_value(cg.get(2 * i), n.act, slope),
-                                             n.scale * gate_value(cg.get(2 * i + 1), n.act, slope))
-                                        : f2(n.scale, n.scale);
+                const uint64_t v = gate ? f2(gate_value(cg.get(2 * i), n.act), gate_value(cg.get(2 * i + 1), n.act))
+                                        : f2(1.f, 1.f);
+                const uint64_t a = mul2(v, f2(n.scale, n.scale));
+                as[i * r.G] = v;
                 bs[i * r.G] = w1 ? mul2(a, R::pair(c1, i)) : a;
             }
         }
@@ -332,9 +325,17 @@ __global__ void __launch_bounds__(kThreads)
             s1 = fma2(t, yhat[i], s1);
             s2 = fma2(c, e[i], s2);
             s3 = fma2(c, yhat[i], s3);
+            if (dh) a2[i] = fma2(R::pair(cdh, i), yhat[i], a2[i]);
         }
         // Issued here, the loads cover the sums' latency.
         if (AHEAD && row + 1 < end) fetch(row + 1);
+        if (gate && g.left == 1 && row + 1 < end && (r.t & 7) == 0)
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                const int64_t c = CH::col_of(0, r.t, r.G, k * R::V);
+                if (c < n.width)
+                    asm volatile("prefetch.global.L2 [%0];" ::"l"(gate + (g.index + 1) * n.sg + c));
+            }
         float t1 = f2lo(s1) + f2hi(s1), t2 = f2lo(s2) + f2hi(s2), t3 = f2lo(s3) + f2hi(s3);
         r.sum3(t1, t2, t3);
         const float k2 = r2 * t1 * n.inv_n, m1 = (t2 - k2 * t3) * n.inv_n;  // k2 = r2 m2
@@ -343,10 +344,6 @@ __global__ void __launch_bounds__(kThreads)
         for (int i = 0; i < P; ++i) {
             const uint64_t xhat = mul2(R::pair(cx, i), r1p);
             if (w2) e[i] = fma2(yhat[i], k2p, e[i]);  // dY
-            if (dh) {
-                if (kWide) a2s[i * r.G] = fma2(R::pair(cdh, i), yhat[i], a2s[i * r.G]);
-                else a2[i] = fma2(R::pair(cdh, i), yhat[i], a2[i]);
-            }
             G[i] = fma2(xhat, e[i], G[i]);
             yhat[i] = mul2(fma2(xhat, k1p, mul2(bs[i * r.G], e[i])), r1p);  // dx
         }
@@ -357,20 +354,14 @@ __global__ void __launch_bounds__(kThreads)
         if (fresh || row + 1 == end) {
             const bool direct = gate && !partg;
             const int64_t ended = g.index - (fresh ? 1 : 0);
-            CH c1, cg;
+            CH c1;
             if (w1) r.load(c1, w1, false);
-            if (gate) r.load(cg, gate + ended * n.sg, false);
 #pragma unroll
             for (int i = 0; i < P; ++i) {
-                float da[2] = {0.f, 0.f};
-                uint64_t a = f2(n.scale, n.scale);
-                if (gate) {
-                    const float lo = gate_value(cg.get(2 * i), n.act, da[0]);
-                    const float hi = gate_value(cg.get(2 * i + 1), n.act, da[1]);
-                    a = mul2(a, f2(lo, hi));
-                }
-                a1[i * r.G] = fma2(a, G[i], a1[i * r.G]);
-                G[i] = mul2(G[i], mul2(f2(n.scale * da[0], n.scale * da[1]), w1 ? R::pair(c1, i) : f2(1.f, 1.f)));
+                const uint64_t a = as[i * r.G], g1 = mul2(G[i], f2(n.scale, n.scale));
+                a1[i * r.G] = fma2(a, g1, a1[i * r.G]);
+                G[i] = mul2(g1, f2(gate_slope(f2lo(a), n.act), gate_slope(f2hi(a), n.act)));
+                if (w1) G[i] = mul2(G[i], R::pair(c1, i));
             }
             if (direct) r.store(dgate + ended * n.width, G);
             if (row + 1 == end) break;
@@ -378,12 +369,7 @@ __global__ void __launch_bounds__(kThreads)
             for (int i = 0; i < P; ++i) G[i] = 0;
         }
     }
-    if (part2) {
-#pragma unroll
-        for (int i = 0; i < P; ++i)
-            if (kWide) a2[i] = a2s[i * r.G];
-        store_part(part2 + r.unit * n.width, a2, r);
-    }
+    if (part2) store_part(part2 + r.unit * n.width, a2, r);
     if (part1) {
 #pragma unroll
         for (int i = 0; i < P; ++i) a2[i] = a1[i * r.G];
@@ -524,8 +510,8 @@ int norm_bwd(const nb200_norm_args& a, const float* rstd, const T* dy, const T* 
     dispatch(s, [&](auto cta, auto e, auto vec, auto most) {
         auto kernel = norm_bwd_kernel<T, decltype(e)::value / Elem<T>::V, decltype(vec)::value, decltype(cta)::value,
                                       decltype(most)::value>;
-        const int smem = (s.wide ? 3 : 2) * per * s.threads * decltype(e)::value * (int)sizeof(float);
-        if (smem > 48 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        const int smem = 3 * per * s.threads * decltype(e)::value * (int)sizeof(float);
+        if (smem > 40 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         kernel<<<(unsigned)((ch.count + per - 1) / per), dim3(s.threads, per), smem, st>>>(
             dy, dh, static_cast<const T*>(a.x), static_cast<const T*>(a.residual), static_cast<const T*>(a.gate),
             static_cast<const T*>(a.post_weight), static_cast<const T*>(a.pre_weight), rstd, n, ch, dx, dres, dgate,
