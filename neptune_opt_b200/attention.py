@@ -22,7 +22,7 @@ import math
 
 from neptune_opt_b200 import _lib
 from neptune_opt_b200.template import _is_metadata, _on_device, current_stream
-from neptune_opt_b200.torch_op import cxx_op
+from neptune_opt_b200.torch_op import on_cuda, run_cxx
 
 HEAD_DIMS = (128,)
 OP_NAME = "neptune_b200::attention"
@@ -122,7 +122,18 @@ def attention_backward(q, k, v, o, lse, grad_out, *, causal: bool = False, scale
     The result does not depend on scheduling. Gradients keep the memory layout of their inputs."""
     import torch
 
-    sc = validate_attention_inputs(q, k, v, scale, seq_lens)
+    if on_cuda(q):
+        sc = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
+        return run_cxx("attention_bwd", (q, k, v, o, lse, grad_out, seq_lens, causal, sc),
+                       _validate_backward, q, k, v, o, lse, grad_out, scale, seq_lens)
+    _validate_backward(q, k, v, o, lse, grad_out, scale, seq_lens)
+    return torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v)
+
+
+def _validate_backward(q, k, v, o, lse, grad_out, scale, seq_lens):
+    import torch
+
+    validate_attention_inputs(q, k, v, scale, seq_lens)
     for name, t in (("o", o), ("grad_out", grad_out)):
         if not isinstance(t, torch.Tensor) or t.dtype != torch.bfloat16:
             raise TypeError(f"attention_backward: {name} must be a bfloat16 tensor")
@@ -132,9 +143,6 @@ def attention_backward(q, k, v, o, lse, grad_out, *, causal: bool = False, scale
         raise TypeError("attention_backward: lse must be a float32 tensor")
     if lse.shape != q.shape[:-1] or lse.device != q.device:
         raise ValueError("attention_backward: lse must be [batch, heads, seq] on the device of q")
-    if _is_metadata(q) or q.numel() == 0:
-        return torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v)
-    return cxx_op("attention_bwd")(q, k, v, o, lse, grad_out, seq_lens, causal, sc)
 
 
 _FUNCTION = None

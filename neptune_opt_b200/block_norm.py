@@ -19,28 +19,26 @@ from __future__ import annotations
 
 import math
 
-from neptune_opt_b200.template import _is_metadata
-from neptune_opt_b200.torch_op import cxx_op
+from neptune_opt_b200.torch_op import on_cuda, run_cxx
 
 GATE_ACTS = {"none": 0, "tanh": 1, "sigmoid": 2}
 MAX_WIDTH = 16384
 
 
-def _rows_per_gate(x, gate) -> int:
-    """Consecutive rows of x that share one row of the gate."""
+def _broadcasts(x, gate) -> bool:
+    """Whether the gate is one row, or x's leading dimensions followed by ones."""
     if gate.dim() == 1:
-        return math.prod(x.shape[:-1])
-    lead, shared, n = x.shape[:-1], gate.shape[:-1], 0
-    if gate.dim() == x.dim():
-        while n < len(lead) and shared[n] == lead[n]:
-            n += 1
-        if all(s == 1 for s in shared[n:]):
-            return math.prod(lead[n:])
-    raise ValueError(f"gated_residual_norm: gate {tuple(gate.shape)} does not broadcast over rows of {tuple(x.shape)}")
+        return True
+    if gate.dim() != x.dim():
+        return False
+    n = 0
+    while n < x.dim() - 1 and gate.shape[n] == x.shape[n]:
+        n += 1
+    return all(s == 1 for s in gate.shape[n:-1])
 
 
 def validate_gated_norm_inputs(x, residual, gate, post_weight, pre_weight, gate_act, residual_scale, eps=1.0):
-    """Metadata-only contract; returns the rows that share a gate row."""
+    """Metadata-only contract."""
     import torch
 
     what = "gated_residual_norm"
@@ -65,6 +63,8 @@ def validate_gated_norm_inputs(x, residual, gate, post_weight, pre_weight, gate_
         raise ValueError(f"{what}: neither post_weight nor pre_weight is given")
     if gate is not None and (gate.dim() < 1 or gate.shape[-1] != x.shape[-1]):
         raise ValueError(f"{what}: gate must be [..., {x.shape[-1]}], got {tuple(gate.shape)}")
+    if gate is not None and not _broadcasts(x, gate):
+        raise ValueError(f"{what}: gate {tuple(gate.shape)} does not broadcast over the rows of {tuple(x.shape)}")
     if gate_act not in GATE_ACTS:
         raise ValueError(f"{what}: gate_act must be one of {sorted(GATE_ACTS)}, got {gate_act!r}")
     if not math.isfinite(residual_scale):
@@ -73,7 +73,6 @@ def validate_gated_norm_inputs(x, residual, gate, post_weight, pre_weight, gate_
         raise ValueError(f"{what}: eps must be finite and positive")
     if x.shape[-1] > MAX_WIDTH:
         raise NotImplementedError(f"{what}: width {x.shape[-1]} exceeds {MAX_WIDTH}")
-    return 1 if gate is None else _rows_per_gate(x, gate)
 
 
 def run_gated_residual_norm(x, residual, gate=None, *, post_weight=None, pre_weight=None, gate_act: str = "none",
@@ -82,10 +81,11 @@ def run_gated_residual_norm(x, residual, gate=None, *, post_weight=None, pre_wei
     reciprocal norms [..., 2] that the backward pass takes."""
     import torch
 
-    per_gate = validate_gated_norm_inputs(x, residual, gate, post_weight, pre_weight, gate_act, residual_scale, eps)
-    if not _is_metadata(x) and x.numel():
-        return cxx_op("gated_norm")(x, residual, gate, post_weight, pre_weight, per_gate, GATE_ACTS[gate_act],
-                                    residual_scale, eps)
+    contract = (x, residual, gate, post_weight, pre_weight, gate_act, residual_scale, eps)
+    if on_cuda(x):
+        return run_cxx("gated_norm", (x, residual, gate, post_weight, pre_weight, GATE_ACTS.get(gate_act, -1),
+                                      residual_scale, eps), validate_gated_norm_inputs, *contract)
+    validate_gated_norm_inputs(*contract)
     y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
     h = torch.empty(x.shape, device=x.device, dtype=x.dtype) if pre_weight is not None else None
     return y, h, torch.empty((*x.shape[:-1], 2), device=x.device, dtype=torch.float32)
@@ -97,7 +97,19 @@ def gated_residual_norm_backward(grad_y, grad_h, x, residual, gate, rstd, *, pos
     None); None in the place of an input that is absent. dgate sums over the rows that share a gate row."""
     import torch
 
-    per_gate = validate_gated_norm_inputs(x, residual, gate, post_weight, pre_weight, gate_act, residual_scale)
+    contract = (grad_y, grad_h, x, residual, gate, rstd, post_weight, pre_weight, gate_act, residual_scale)
+    if on_cuda(x):
+        return run_cxx("gated_norm_bwd", (grad_y, grad_h, x, residual, gate, rstd, post_weight, pre_weight,
+                                          GATE_ACTS.get(gate_act, -1), residual_scale), _validate_backward, *contract)
+    _validate_backward(*contract)
+    return tuple(None if t is None else torch.zeros(t.shape, device=t.device, dtype=t.dtype)
+                 for t in (x, residual, gate, post_weight, pre_weight))
+
+
+def _validate_backward(grad_y, grad_h, x, residual, gate, rstd, post_weight, pre_weight, gate_act, residual_scale):
+    import torch
+
+    validate_gated_norm_inputs(x, residual, gate, post_weight, pre_weight, gate_act, residual_scale)
     if grad_h is not None and pre_weight is None:
         raise ValueError("gated_residual_norm_backward: grad_h without pre_weight")
     for name, t in (("grad_y", grad_y), ("grad_h", grad_h)):
@@ -111,12 +123,6 @@ def gated_residual_norm_backward(grad_y, grad_h, x, residual, gate, rstd, *, pos
         raise TypeError("gated_residual_norm_backward: rstd must be a float32 tensor")
     if tuple(rstd.shape) != (*x.shape[:-1], 2) or rstd.device != x.device:
         raise ValueError("gated_residual_norm_backward: rstd must be [..., 2] on the device of x")
-
-    if not _is_metadata(x) and x.numel():
-        return cxx_op("gated_norm_bwd")(grad_y, grad_h, x, residual, gate, rstd, post_weight, pre_weight, per_gate,
-                                        GATE_ACTS[gate_act], residual_scale)
-    return tuple(None if t is None else torch.zeros(t.shape, device=t.device, dtype=t.dtype)
-                 for t in (x, residual, gate, post_weight, pre_weight))
 
 
 _FUNCTION = None

@@ -128,22 +128,25 @@ __global__ void __launch_bounds__(kFwdThreads)
     int64_t v0, v1;
     split_range(nv, size, rank, v0, v1);
     const uint4* p = reinterpret_cast<const uint4*>(xr + head);
-    auto fold = [&](const uint4& u) {
-        float f[V];
-        Elem<T>::unpack(u, f);
-#pragma unroll
-        for (int e = 0; e < V; ++e) f[e] *= scale;
-        acc.add<V>(f);
-    };
     int64_t v = v0 + t;
     for (; v + (U - 1) * kFwdThreads < v1; v += U * kFwdThreads) {
         uint4 u[U];
 #pragma unroll
         for (int k = 0; k < U; ++k) u[k] = ld_stream(p + v + k * kFwdThreads);
+        float f[U * V];
 #pragma unroll
-        for (int k = 0; k < U; ++k) fold(u[k]);
+        for (int k = 0; k < U; ++k) Elem<T>::unpack(u[k], f + k * V);
+#pragma unroll
+        for (int e = 0; e < U * V; ++e) f[e] *= scale;
+        acc.add<U * V>(f);
     }
-    for (; v < v1; v += kFwdThreads) fold(ld_stream(p + v));
+    for (; v < v1; v += kFwdThreads) {
+        float f[V];
+        Elem<T>::unpack(ld_stream(p + v), f);
+#pragma unroll
+        for (int e = 0; e < V; ++e) f[e] *= scale;
+        acc.add<V>(f);
+    }
     if (rank == 0) {  // what lies outside the vectors: fewer than 2 V elements
         if (t < head) {
             const float f = Elem<T>::to_f(xr[t]) * scale;

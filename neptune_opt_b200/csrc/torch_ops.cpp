@@ -20,14 +20,14 @@
 //   segment_status_word(int device) -> Tensor      the per-device int32 word itself, for launches
 //                                                  made through the C ABI by other host code
 //   attention(Tensor q, Tensor k, Tensor v, bool causal, float scale) -> (Tensor o, Tensor lse)
-// The training operators (CUDA kernels only; the Python layer checks the whole contract, the ops what
-// memory safety needs, and an absent optional result is an undefined tensor):
+// The training operators (CUDA kernels only, which check the whole contract of the Python functions; an
+// absent optional result is an undefined tensor):
 //   attention_bwd(Tensor q, Tensor k, Tensor v, Tensor o, Tensor lse, Tensor grad_o, Tensor? seq_lens,
 //                 bool causal, float scale) -> (Tensor dq, Tensor dk, Tensor dv)
-//   gated_norm(Tensor x, Tensor residual, Tensor? gate, Tensor? post, Tensor? pre, int rows_per_gate,
-//              int act, float scale, float eps) -> (Tensor y, Tensor h, Tensor rstd)
+//   gated_norm(Tensor x, Tensor residual, Tensor? gate, Tensor? post, Tensor? pre, int act, float scale,
+//              float eps) -> (Tensor y, Tensor h, Tensor rstd)
 //   gated_norm_bwd(Tensor? grad_y, Tensor? grad_h, Tensor x, Tensor residual, Tensor? gate, Tensor rstd,
-//                  Tensor? post, Tensor? pre, int rows_per_gate, int act, float scale)
+//                  Tensor? post, Tensor? pre, int act, float scale)
 //              -> (Tensor dx, Tensor dresidual, Tensor dgate, Tensor dpost, Tensor dpre)
 //   distill_loss(Tensor x, Tensor teacher, Tensor index, float temperature, Tensor? teacher_lse)
 //              -> (Tensor loss, Tensor stats)
@@ -344,6 +344,10 @@ std::tuple<at::Tensor, at::Tensor> attention_cuda(const at::Tensor& q, const at:
 // ------------------------------------------------------------------ training operators
 using OptTensor = std::optional<at::Tensor>;
 
+void check_strided(const at::Tensor& t, const char* what) {
+    TORCH_CHECK_TYPE(t.layout() == at::kStrided, what, ": tensors must be strided");
+}
+
 bool present(const OptTensor& t) { return t.has_value() && t->defined(); }
 
 // t itself when the attention kernels' copies can read its rows (unit stride in a row, positive 16-byte
@@ -363,26 +367,27 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_bwd_cuda(const at::Tens
                                                                   double scale) {
     const char* what = "nb200.attention_bwd";
     for (const at::Tensor* t : {&q_, &k_, &v_, &o_, &go_}) {
-        check_cuda(*t, what);
+        check_strided(*t, what);
         TORCH_CHECK_TYPE(t->scalar_type() == at::kBFloat16, what, ": q, k, v, o, grad_o must be bfloat16");
         TORCH_CHECK_VALUE(t->dim() == 4 && t->device() == q_.device(), what, ": tensors must be 4-D on one device");
     }
-    check_cuda(lse_, what);
+    check_cuda(q_, what);
+    TORCH_CHECK_TYPE(lse_.scalar_type() == at::kFloat, what, ": lse must be float32");
     TORCH_CHECK_VALUE(q_.sizes() == o_.sizes() && q_.sizes() == go_.sizes() && k_.sizes() == v_.sizes() &&
                           q_.size(0) == k_.size(0) && q_.size(2) == k_.size(2) && q_.size(3) == k_.size(3),
                       what, ": shapes differ");
-    TORCH_CHECK_VALUE(lse_.scalar_type() == at::kFloat && lse_.sizes() == q_.sizes().slice(0, 3), what,
-                      ": lse must be float32 [batch, heads, seq]");
+    TORCH_CHECK_VALUE(lse_.device() == q_.device() && lse_.sizes() == q_.sizes().slice(0, 3), what,
+                      ": lse must be [batch, heads, seq]");
     c10::cuda::CUDAGuard guard(q_.device());
     const at::Tensor q = attn_rows(q_), k = attn_rows(k_), v = attn_rows(v_), o = attn_rows(o_), go = attn_rows(go_);
     const at::Tensor lse = lse_.contiguous();
     at::Tensor dq = at::empty_like(q), dk = at::empty_like(k), dv = at::empty_like(v);
     nb200_attn_args a = {q.size(0), q.size(1), k.size(1), q.size(2), q.size(3), nullptr, causal ? 1 : 0, (float)scale};
     if (present(seq_lens)) {
-        check_cuda(*seq_lens, what);
-        TORCH_CHECK_VALUE(seq_lens->scalar_type() == at::kInt && seq_lens->dim() == 1 &&
+        TORCH_CHECK_TYPE(seq_lens->scalar_type() == at::kInt, what, ": seq_lens must be int32");
+        TORCH_CHECK_VALUE(seq_lens->device() == q.device() && seq_lens->dim() == 1 &&
                               seq_lens->size(0) == q.size(0) && seq_lens->is_contiguous(),
-                          what, ": seq_lens must be contiguous int32 [batch]");
+                          what, ": seq_lens must be contiguous [batch] on the device of q");
         a.seq_lens = seq_lens->data_ptr<int32_t>();
     }
     const nb200_attn_strides strides[8] = {attn_strides(q),  attn_strides(k),  attn_strides(v),  attn_strides(o),
@@ -403,45 +408,69 @@ at::Tensor unit_rows(const at::Tensor& t, int64_t rows) {
     return (f.stride(1) == 1 || f.size(1) == 1) && f.stride(0) >= 0 ? f : f.contiguous();
 }
 
+// Consecutive rows of x that share one row of the gate: all of them for a 1-D gate, otherwise those under the
+// gate's trailing ones (its leading dimensions are x's).
+int64_t rows_per_gate(const at::Tensor& x, const at::Tensor& gate, const char* what) {
+    const int64_t lead = x.dim() - 1;
+    int64_t n = 0, rows = 1;
+    if (gate.dim() != 1) {
+        TORCH_CHECK_VALUE(gate.dim() == x.dim(), what, ": gate does not broadcast over the rows of x");
+        while (n < lead && gate.size(n) == x.size(n)) ++n;
+        for (int64_t d = n; d < lead; ++d)
+            TORCH_CHECK_VALUE(gate.size(d) == 1, what, ": gate does not broadcast over the rows of x");
+    }
+    for (int64_t d = n; d < lead; ++d) rows *= x.size(d);
+    return rows;
+}
+
 // The descriptor of a gated norm's inputs and the tensors whose memory it names.
 struct NormInputs {
     nb200_norm_args a = {};
     int dtype;
     int64_t rows;
     std::vector<at::Tensor> keep;
-    const void* row_input(const at::Tensor& t, const at::Tensor& like, int64_t n, int64_t* stride, const char* what) {
-        check_cuda(t, what);
+    static void same_kind(const at::Tensor& t, const at::Tensor& like, const char* what) {
+        check_strided(t, what);
         TORCH_CHECK_TYPE(t.scalar_type() == like.scalar_type(), what, ": tensors must share one dtype");
-        TORCH_CHECK_VALUE(t.device() == like.device() && t.dim() >= 1 && t.size(-1) == like.size(-1) &&
-                              t.numel() == n * like.size(-1),
-                          what, ": tensors must be [..., width] on one device");
+        TORCH_CHECK_VALUE(t.device() == like.device(), what, ": tensors must be on one CUDA device");
+    }
+    const void* row_input(const at::Tensor& t, int64_t n, int64_t* stride) {
         keep.push_back(unit_rows(t, n));
         *stride = keep.back().stride(0);
         return keep.back().data_ptr();
     }
-    const void* weight(const OptTensor& t, const at::Tensor& like, const char* what) {
+    const void* like_x(const at::Tensor& t, const at::Tensor& x, int64_t* stride, const char* what) {
+        same_kind(t, x, what);
+        TORCH_CHECK_VALUE(t.sizes() == x.sizes(), what, ": residual and gradients must have x's shape");
+        return row_input(t, rows, stride);
+    }
+    const void* weight(const OptTensor& t, const at::Tensor& x, const char* what) {
         if (!present(t)) return nullptr;
-        check_cuda(*t, what);
-        TORCH_CHECK_TYPE(t->scalar_type() == like.scalar_type(), what, ": weights must have x's dtype");
-        TORCH_CHECK_VALUE(t->device() == like.device() && t->dim() == 1 && t->size(0) == like.size(-1), what,
+        same_kind(*t, x, what);
+        TORCH_CHECK_VALUE(t->dim() == 1 && t->size(0) == x.size(-1), what,
                           ": weights must be 1-D with x's last dimension");
         keep.push_back(t->contiguous());
         return keep.back().data_ptr();
     }
     NormInputs(const at::Tensor& x, const at::Tensor& residual, const OptTensor& gate, const OptTensor& post,
-               const OptTensor& pre, int64_t rows_per_gate, int64_t act, double scale, double eps, const char* what) {
+               const OptTensor& pre, int64_t act, double scale, double eps, const char* what) {
+        check_strided(x, what);
+        check_cuda(x, what);
         dtype = dtype_code(x);
-        TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1 && rows_per_gate >= 1, what, ": x must be [..., width]");
+        TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1, what, ": x must be [..., width]");
+        TORCH_CHECK_VALUE(present(post) || present(pre), what, ": neither weight is given");
         rows = x.numel() / x.size(-1);
         keep.reserve(7);
         a.rows = rows;
         a.width = x.size(-1);
-        a.x = row_input(x, x, rows, &a.stride_x, what);
-        a.residual = row_input(residual, x, rows, &a.stride_residual, what);
-        a.rows_per_gate = rows_per_gate;
+        a.x = row_input(x, rows, &a.stride_x);
+        a.residual = like_x(residual, x, &a.stride_residual, what);
+        a.rows_per_gate = 1;
         if (present(gate)) {
-            TORCH_CHECK_VALUE(rows % rows_per_gate == 0, what, ": gate rows do not divide x's rows");
-            a.gate = row_input(*gate, x, rows / rows_per_gate, &a.stride_gate, what);
+            same_kind(*gate, x, what);
+            TORCH_CHECK_VALUE(gate->dim() >= 1 && gate->size(-1) == x.size(-1), what, ": gate must be [..., width]");
+            a.rows_per_gate = rows_per_gate(x, *gate, what);
+            a.gate = row_input(*gate, rows / a.rows_per_gate, &a.stride_gate);
         }
         a.post_weight = weight(post, x, what);
         a.pre_weight = weight(pre, x, what);
@@ -453,11 +482,11 @@ struct NormInputs {
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor> gated_norm_cuda(const at::Tensor& x, const at::Tensor& residual,
                                                                const OptTensor& gate, const OptTensor& post,
-                                                               const OptTensor& pre, int64_t rows_per_gate, int64_t act,
-                                                               double scale, double eps) {
+                                                               const OptTensor& pre, int64_t act, double scale,
+                                                               double eps) {
     const char* what = "nb200.gated_norm";
+    const NormInputs in(x, residual, gate, post, pre, act, scale, eps, what);
     c10::cuda::CUDAGuard guard(x.device());
-    const NormInputs in(x, residual, gate, post, pre, rows_per_gate, act, scale, eps, what);
     at::Tensor y = at::empty(x.sizes(), x.options()), h;
     if (present(pre)) h = at::empty(x.sizes(), x.options());
     std::vector<int64_t> shape = lead_shape(x, false);
@@ -471,17 +500,17 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> gated_norm_cuda(const at::Tensor&
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> gated_norm_bwd_cuda(
     const OptTensor& gy, const OptTensor& gh, const at::Tensor& x, const at::Tensor& residual, const OptTensor& gate,
-    const at::Tensor& rstd_, const OptTensor& post, const OptTensor& pre, int64_t rows_per_gate, int64_t act,
-    double scale) {
+    const at::Tensor& rstd_, const OptTensor& post, const OptTensor& pre, int64_t act, double scale) {
     const char* what = "nb200.gated_norm_bwd";
+    NormInputs in(x, residual, gate, post, pre, act, scale, 1.0, what);
     c10::cuda::CUDAGuard guard(x.device());
-    NormInputs in(x, residual, gate, post, pre, rows_per_gate, act, scale, 1.0, what);
-    check_cuda(rstd_, what);
-    TORCH_CHECK_VALUE(rstd_.scalar_type() == at::kFloat && rstd_.numel() == 2 * in.rows, what,
-                      ": rstd must be float32 [..., 2]");
+    TORCH_CHECK_TYPE(rstd_.scalar_type() == at::kFloat, what, ": rstd must be float32");
+    TORCH_CHECK_VALUE(rstd_.device() == x.device() && rstd_.dim() == x.dim() && rstd_.size(-1) == 2 &&
+                          rstd_.sizes().slice(0, x.dim() - 1) == x.sizes().slice(0, x.dim() - 1),
+                      what, ": rstd must be [..., 2]");
     const at::Tensor rstd = rstd_.contiguous();
-    const void* dy = present(gy) ? in.row_input(*gy, x, in.rows, &in.a.stride_grad_y, what) : nullptr;
-    const void* dh = present(gh) ? in.row_input(*gh, x, in.rows, &in.a.stride_grad_h, what) : nullptr;
+    const void* dy = present(gy) ? in.like_x(*gy, x, &in.a.stride_grad_y, what) : nullptr;
+    const void* dh = present(gh) ? in.like_x(*gh, x, &in.a.stride_grad_h, what) : nullptr;
     auto fresh = [&](const OptTensor& t) { return present(t) ? at::empty(t->sizes(), t->options()) : at::Tensor(); };
     at::Tensor dx = at::empty(x.sizes(), x.options()), dr = at::empty(x.sizes(), x.options());
     at::Tensor dgate = fresh(gate), dpost = fresh(post), dpre = fresh(pre);
@@ -501,17 +530,20 @@ struct DistillInputs {
     at::Tensor x, teacher, index;
     DistillInputs(const at::Tensor& x_, const at::Tensor& teacher_, const at::Tensor& index_, double temperature,
                   const char* what) {
+        for (const at::Tensor* t : {&x_, &teacher_, &index_}) check_strided(*t, what);
         check_cuda(x_, what);
-        check_cuda(teacher_, what);
-        check_cuda(index_, what);
+        a.dtype = dtype_code(x_);
+        a.teacher_dtype = dtype_code(teacher_);
+        a.index_dtype = index_code(index_);
         TORCH_CHECK_VALUE(x_.dim() >= 1 && x_.size(-1) >= 1 && teacher_.sizes() == index_.sizes() &&
-                              teacher_.dim() == x_.dim() && teacher_.device() == x_.device() &&
-                              index_.device() == x_.device(),
-                          what, ": logits [..., vocab], teacher and index [..., top] on one device");
+                              teacher_.dim() == x_.dim() &&
+                              teacher_.sizes().slice(0, x_.dim() - 1) == x_.sizes().slice(0, x_.dim() - 1),
+                          what, ": logits must be [..., vocab], teacher and index [..., top] over the same rows");
+        TORCH_CHECK_VALUE(teacher_.device() == x_.device() && index_.device() == x_.device(), what,
+                          ": tensors must be on one CUDA device");
         a.rows = x_.numel() / x_.size(-1);
         a.vocab = x_.size(-1);
         a.top = teacher_.size(-1);
-        TORCH_CHECK_VALUE(teacher_.numel() == a.rows * a.top, what, ": teacher rows differ from the logits'");
         x = unit_rows(x_, a.rows);
         teacher = unit_rows(teacher_, a.rows);
         index = unit_rows(index_, a.rows);
@@ -521,9 +553,6 @@ struct DistillInputs {
         a.stride_x = x.stride(0);
         a.stride_teacher = teacher.stride(0);
         a.stride_index = index.stride(0);
-        a.dtype = dtype_code(x);
-        a.teacher_dtype = dtype_code(teacher);
-        a.index_dtype = index_code(index);
         a.temperature = temperature;
     }
 };
@@ -532,17 +561,17 @@ std::tuple<at::Tensor, at::Tensor> distill_loss_cuda(const at::Tensor& x, const 
                                                      const at::Tensor& index, double temperature,
                                                      const OptTensor& teacher_lse) {
     const char* what = "nb200.distill_loss";
-    c10::cuda::CUDAGuard guard(x.device());
     const DistillInputs in(x, teacher, index, temperature, what);
+    c10::cuda::CUDAGuard guard(x.device());
     std::vector<int64_t> shape = lead_shape(x, false);
     const auto f32 = x.options().dtype(at::kFloat);
     at::Tensor loss = at::empty(shape, f32), z;
     shape.push_back(3);
     at::Tensor stats = at::empty(shape, f32);
     if (present(teacher_lse)) {
-        check_cuda(*teacher_lse, what);
-        TORCH_CHECK_VALUE(teacher_lse->scalar_type() == at::kFloat && teacher_lse->numel() == in.a.rows, what,
-                          ": teacher_lse must be float32 [...]");
+        TORCH_CHECK_TYPE(teacher_lse->scalar_type() == at::kFloat, what, ": teacher_lse must be float32");
+        TORCH_CHECK_VALUE(teacher_lse->device() == x.device() && teacher_lse->sizes() == loss.sizes(), what,
+                          ": teacher_lse must be [...] over the logits' rows");
         z = teacher_lse->contiguous();
     }
     check(api().distill_loss(&in.a, z.defined() ? z.data_ptr<float>() : nullptr, loss.data_ptr<float>(),
@@ -554,13 +583,15 @@ std::tuple<at::Tensor, at::Tensor> distill_loss_cuda(const at::Tensor& x, const 
 at::Tensor distill_loss_bwd_cuda(const at::Tensor& grad_, const at::Tensor& x, const at::Tensor& teacher,
                                  const at::Tensor& index, const at::Tensor& stats_, double temperature) {
     const char* what = "nb200.distill_loss_bwd";
-    c10::cuda::CUDAGuard guard(x.device());
     const DistillInputs in(x, teacher, index, temperature, what);
-    check_cuda(grad_, what);
-    check_cuda(stats_, what);
-    TORCH_CHECK_VALUE(grad_.scalar_type() == at::kFloat && grad_.numel() == in.a.rows &&
-                          stats_.scalar_type() == at::kFloat && stats_.numel() == 3 * in.a.rows,
-                      what, ": grad must be float32 [...], stats float32 [..., 3]");
+    c10::cuda::CUDAGuard guard(x.device());
+    const auto lead = x.sizes().slice(0, x.dim() - 1);
+    TORCH_CHECK_TYPE(grad_.scalar_type() == at::kFloat && stats_.scalar_type() == at::kFloat, what,
+                     ": grad and stats must be float32");
+    TORCH_CHECK_VALUE(grad_.sizes() == lead && stats_.dim() == x.dim() && stats_.size(-1) == 3 &&
+                          stats_.sizes().slice(0, x.dim() - 1) == lead && grad_.device() == x.device() &&
+                          stats_.device() == x.device(),
+                      what, ": grad must be [...], stats [..., 3] over the logits' rows");
     at::Tensor grad = grad_.reshape({-1});
     if (grad.stride(0) < 0) grad = grad.contiguous();
     const at::Tensor stats = stats_.contiguous();
@@ -679,10 +710,10 @@ TORCH_LIBRARY(nb200, m) {
     m.def("attention(Tensor q, Tensor k, Tensor v, bool causal, float scale) -> (Tensor, Tensor)");
     m.def("attention_bwd(Tensor q, Tensor k, Tensor v, Tensor o, Tensor lse, Tensor grad_o, Tensor? seq_lens, "
           "bool causal, float scale) -> (Tensor, Tensor, Tensor)");
-    m.def("gated_norm(Tensor x, Tensor residual, Tensor? gate, Tensor? post, Tensor? pre, int rows_per_gate, int act, "
+    m.def("gated_norm(Tensor x, Tensor residual, Tensor? gate, Tensor? post, Tensor? pre, int act, "
           "float scale, float eps) -> (Tensor, Tensor, Tensor)");
     m.def("gated_norm_bwd(Tensor? grad_y, Tensor? grad_h, Tensor x, Tensor residual, Tensor? gate, Tensor rstd, "
-          "Tensor? post, Tensor? pre, int rows_per_gate, int act, float scale) "
+          "Tensor? post, Tensor? pre, int act, float scale) "
           "-> (Tensor, Tensor, Tensor, Tensor, Tensor)");
     m.def("distill_loss(Tensor x, Tensor teacher, Tensor index, float temperature, Tensor? teacher_lse) "
           "-> (Tensor, Tensor)");

@@ -20,8 +20,7 @@ from __future__ import annotations
 
 import math
 
-from neptune_opt_b200.template import _is_metadata
-from neptune_opt_b200.torch_op import cxx_op
+from neptune_opt_b200.torch_op import on_cuda, run_cxx
 
 MAX_TOP = 256
 
@@ -65,9 +64,10 @@ def run_distill_loss(logits, teacher_logits, teacher_index, *, temperature: floa
     logsumexp(t / T) over its whole vocabulary; without it the kept entries are normalised to mass 1."""
     import torch
 
-    validate_distill_inputs(logits, teacher_logits, teacher_index, temperature, teacher_lse)
-    if not _is_metadata(logits) and logits.numel():
-        return cxx_op("distill_loss")(logits, teacher_logits, teacher_index, temperature, teacher_lse)
+    contract = (logits, teacher_logits, teacher_index, temperature, teacher_lse)
+    if on_cuda(logits):
+        return run_cxx("distill_loss", contract, validate_distill_inputs, *contract)
+    validate_distill_inputs(*contract)
     return (torch.empty(logits.shape[:-1], device=logits.device, dtype=torch.float32),
             torch.empty((*logits.shape[:-1], 3), device=logits.device, dtype=torch.float32))
 
@@ -77,15 +77,22 @@ def distill_loss_backward(grad, logits, teacher_logits, teacher_index, stats, *,
     the forward pass's stats."""
     import torch
 
+    contract = (grad, logits, teacher_logits, teacher_index, stats, temperature)
+    if on_cuda(logits):
+        return run_cxx("distill_loss_bwd", contract, _validate_backward, *contract)
+    _validate_backward(*contract)
+    return torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
+
+
+def _validate_backward(grad, logits, teacher_logits, teacher_index, stats, temperature):
+    import torch
+
     validate_distill_inputs(logits, teacher_logits, teacher_index, temperature)
     for name, t, shape in (("grad", grad, logits.shape[:-1]), ("stats", stats, (*logits.shape[:-1], 3))):
         if not isinstance(t, torch.Tensor) or t.dtype != torch.float32:
             raise TypeError(f"distill_loss_backward: {name} must be a float32 tensor")
         if tuple(t.shape) != tuple(shape) or t.device != logits.device:
             raise ValueError(f"distill_loss_backward: {name} must be {tuple(shape)} on the device of logits")
-    if not _is_metadata(logits) and logits.numel():
-        return cxx_op("distill_loss_bwd")(grad, logits, teacher_logits, teacher_index, stats, temperature)
-    return torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
 
 
 _FUNCTION = None

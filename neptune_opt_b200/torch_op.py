@@ -67,6 +67,23 @@ def cxx_op(name: str):
     return op
 
 
+def run_cxx(name: str, args: tuple, validate, *validate_args):
+    """A C++-registered op on real CUDA tensors. The op checks the whole contract, so a call costs no
+    Python checks; when it refuses, `validate` runs to raise the error in the function's own words."""
+    try:
+        return cxx_op(name)(*args)
+    except (RuntimeError, TypeError, ValueError, NotImplementedError):
+        validate(*validate_args)
+        raise
+
+
+def on_cuda(t) -> bool:
+    """A real (not fake, not meta) CUDA tensor with elements: what the kernels run on."""
+    import torch
+
+    return type(t) in (torch.Tensor, torch.nn.Parameter) and t.is_cuda and t.numel() > 0
+
+
 def _tracing(*tensors) -> bool:
     """True while fake, meta or functional tensors trace the op (export, AOTInductor, FakeTensorMode)."""
     from torch._subclasses.fake_tensor import FakeTensor
