@@ -19,6 +19,7 @@ namespace nb200 {
 namespace {
 
 constexpr int kMaxTop = 256;  // entries a row may keep: one per thread of its CTA
+constexpr float kL2e = 1.4426950408889634f;
 
 struct Row {  // what both directions read of the teacher
     const void* teacher;
@@ -49,35 +50,55 @@ __device__ __forceinline__ int64_t lead(const T* p) {
     return (int64_t)((16 - (reinterpret_cast<uintptr_t>(p) & 15u)) & 15u) / (int64_t)sizeof(T);
 }
 
-// Running (maximum, sum of 2^(x log2 e - maximum)) of x = logits / T, the maximum in the log2 domain. -inf
-// maxima carry a zero sum.
+// Running state of a row: s = sum of 2^(x scale - c) with scale = log2(e) / T and c the largest x scale so far,
+// rounded; c is the exact shift of every term, so its rounding costs nothing. A row of -inf alone keeps
+// c = -inf and s = 0.
 struct LogSum {
-    float m = -HUGE_VALF, s = 0.f;
-    __device__ __forceinline__ static float shift(float m) { return m == -NB200_INF ? 0.f : m; }
-    __device__ __forceinline__ void merge(float m2, float s2) {
-        const float t = fmaxf(m, m2), c = shift(t);
-        s = s * ex2_ftz(m - c) + s2 * ex2_ftz(m2 - c);
-        m = t;
+    float c = -HUGE_VALF, s = 0.f;
+    __device__ __forceinline__ static float shift(float c) { return c == -NB200_INF ? 0.f : c; }
+    __device__ __forceinline__ void merge(float c2, float s2) {
+        const float t = fmaxf(c, c2), m = shift(t);
+        s = s * ex2_ftz(c - m) + s2 * ex2_ftz(c2 - m);
+        c = t;
     }
-    // E values, already in the log2 domain.
+    __device__ __forceinline__ void merge_warp(int from) {
+        for (int o = from; o > 0; o >>= 1) {
+            const float c2 = __shfl_xor_sync(0xffffffffu, c, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+            merge(c2, s2);
+        }
+    }
+    // E logits (E even): half an instruction each for the maximum, the exponent and the sum (three-input max,
+    // packed pairs), one exponential each, one more for the whole batch.
     template <int E>
-    __device__ __forceinline__ void add(const float* x) {
-        float t[4] = {m, x[0], x[0], x[0]};
+    __device__ __forceinline__ void add(const float* x, float scale) {
+        float t0 = x[0], t1 = x[1];
 #pragma unroll
-        for (int i = 0; i < E; ++i) t[i & 3] = fmaxf(t[i & 3], x[i]);
-        const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), c = shift(top);
-        float a[4] = {s * ex2_ftz(m - c), 0.f, 0.f, 0.f};
+        for (int i = 2; i + 3 < E; i += 4) {
+            t0 = max3(t0, x[i], x[i + 1]);
+            t1 = max3(t1, x[i + 2], x[i + 3]);
+        }
+        if (E % 4 == 0) t0 = max3(t0, x[E - 2], x[E - 1]);
+        const float top = fmaxf(c, fmaxf(t0, t1) * scale), m = shift(top);
+        const uint64_t scale2 = f2(scale, scale), m2 = f2(-m, -m);
+        uint64_t a0 = f2(s * ex2_ftz(c - m), 0.f), a1 = 0;
 #pragma unroll
-        for (int i = 0; i < E; ++i) a[i & 3] += ex2_ftz(x[i] - c);
-        s = (a[0] + a[1]) + (a[2] + a[3]);
-        m = top;
+        for (int i = 0; i < E; i += 2) {
+            const uint64_t e = fma2(f2(x[i], x[i + 1]), scale2, m2);
+            const uint64_t p = f2(ex2_ftz(f2lo(e)), ex2_ftz(f2hi(e)));
+            if (i & 2) a1 = add2(a1, p);
+            else a0 = add2(a0, p);
+        }
+        const uint64_t a = add2(a0, a1);
+        s = f2lo(a) + f2hi(a);
+        c = top;
     }
+    __device__ __forceinline__ void add_one(float x, float scale) { merge(x * scale, x == -NB200_INF ? 0.f : 1.f); }
 };
 
 // ------------------------------------------------------------------ forward
 // One cluster of CTAs per row (one CTA when there are rows enough): each folds a share of the row's 16-byte
-// vectors, the states meet in the first CTA's shared memory, and that CTA takes the kept entries, which
-// it fetched before the fold. One pass over the logits, no scratch.
+// vectors, the states meet in the first CTA's shared memory, and that CTA's first warp takes the kept
+// entries, which were fetched before the fold. One pass over the logits, no scratch.
 constexpr int kFwdThreads = 512;
 constexpr int kMaxCluster = 16;
 
@@ -106,22 +127,17 @@ template <typename T>
 __global__ void __launch_bounds__(kFwdThreads)
     distill_fwd_kernel(const T* x, int64_t stride, Row r, const float* teacher_lse, float* loss, float* stats) {
     constexpr int V = Elem<T>::V, U = 4;  // U vectors in flight per thread
-    __shared__ float buf[64], sm[32], ss[32], cm[kMaxCluster], cs[kMaxCluster];
+    __shared__ float ec[32], es[32], cc[kMaxCluster], cs[kMaxCluster], teach[kMaxTop], stud[kMaxTop];
     const uint32_t rank = cluster_rank(), size = cluster_size();
     const int64_t row = blockIdx.x / size;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const T* xr = x + row * stride;
-    // The kept entries, one per thread.
-    int64_t at = -1;
-    float tl = -NB200_INF, xl = 0.f;
+    // The kept entries, one per thread: t_j / T (-inf: not kept, its probability is 0) and x / T.
     if (rank == 0 && t < r.top) {
-        at = r.at(row, t);
-        if (at >= 0) {
-            tl = r.logit(row, t);
-            xl = Elem<T>::to_f(xr[at]) * r.inv_t;
-        }
+        const int64_t at = r.at(row, t);
+        teach[t] = at >= 0 ? r.logit(row, t) : -NB200_INF;
+        stud[t] = at >= 0 ? Elem<T>::to_f(xr[at]) * r.inv_t : 0.f;
     }
-    constexpr float kL2e = 1.4426950408889634f;
     const float scale = r.inv_t * kL2e;
     LogSum acc;
     const int64_t head = min(lead(xr), r.vocab), nv = (r.vocab - head) / V, tail = head + nv * V;
@@ -136,61 +152,66 @@ __global__ void __launch_bounds__(kFwdThreads)
         float f[U * V];
 #pragma unroll
         for (int k = 0; k < U; ++k) Elem<T>::unpack(u[k], f + k * V);
-#pragma unroll
-        for (int e = 0; e < U * V; ++e) f[e] *= scale;
-        acc.add<U * V>(f);
+        acc.add<U * V>(f, scale);
     }
     for (; v < v1; v += kFwdThreads) {
         float f[V];
         Elem<T>::unpack(ld_stream(p + v), f);
-#pragma unroll
-        for (int e = 0; e < V; ++e) f[e] *= scale;
-        acc.add<V>(f);
+        acc.add<V>(f, scale);
     }
     if (rank == 0) {  // what lies outside the vectors: fewer than 2 V elements
-        if (t < head) {
-            const float f = Elem<T>::to_f(xr[t]) * scale;
-            acc.add<1>(&f);
-        } else if (t >= 32 && tail + t - 32 < r.vocab) {
-            const float f = Elem<T>::to_f(xr[tail + t - 32]) * scale;
-            acc.add<1>(&f);
-        }
+        if (t < head) acc.add_one(Elem<T>::to_f(xr[t]), scale);
+        else if (t >= 32 && tail + t - 32 < r.vocab) acc.add_one(Elem<T>::to_f(xr[tail + t - 32]), scale);
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const float m2 = __shfl_xor_sync(0xffffffffu, acc.m, o), s2 = __shfl_xor_sync(0xffffffffu, acc.s, o);
-        acc.merge(m2, s2);
-    }
+    acc.merge_warp(16);
     if (lane == 0) {
-        sm[warp] = acc.m;
-        ss[warp] = acc.s;
+        ec[warp] = acc.c;
+        es[warp] = acc.s;
     }
     __syncthreads();
-    acc = LogSum{};
-    for (int w = 0; w < kFwdThreads / 32; ++w) acc.merge(sm[w], ss[w]);
-    if (size > 1) {
-        if (t == 0) {
-            store_first(&cm[rank], acc.m);
+    if (warp == 0) {
+        acc = LogSum{};
+        if (lane < kFwdThreads / 32) acc.merge(ec[lane], es[lane]);
+        acc.merge_warp(16);
+        if (size > 1 && lane == 0) {
+            store_first(&cc[rank], acc.c);
             store_first(&cs[rank], acc.s);
         }
+    }
+    if (size > 1) {
+        __syncwarp();
         cluster_sync();
         if (rank != 0) return;
-        acc = LogSum{};
-        for (uint32_t c = 0; c < size; ++c) acc.merge(cm[c], cs[c]);
+        if (warp == 0) {
+            acc = LogSum{};
+            if (lane < size) acc.merge(cc[lane], cs[lane]);
+            acc.merge_warp(16);
+        }
     }
-    const float lse = (acc.m + log2f(acc.s)) * 0.69314718055994531f;
-    Group<true> g{buf, 0};
+    if (warp != 0) return;
+    // The first warp takes the kept entries.
+    const float lse = (acc.c + log2f(acc.s)) * 0.69314718055994531f;
     float z;
     if (teacher_lse) {
         z = teacher_lse[row];
     } else {
-        const float top = g.reduce(tl, RED_MAX), c = LogSum::shift(top);
-        z = c + logf(g.reduce(expf(tl - c), RED_SUM));
+        float top = -NB200_INF, sum = 0.f;
+        for (int j = lane; j < r.top; j += 32) top = fmaxf(top, teach[j]);
+        top = warp_max(top);
+        const float c = LogSum::shift(top);
+        for (int j = lane; j < r.top; j += 32) sum += expf(teach[j] - c);
+        z = c + logf(warp_sum(sum));
     }
-    const float pr = at >= 0 ? expf(tl - z) : 0.f;
-    const float mass = g.reduce(pr, RED_SUM);
-    const float l = g.reduce(at >= 0 && pr != 0.f ? pr * ((tl - z) - (xl - lse)) : 0.f, RED_SUM);
-    if (t == 0) {
+    float mass = 0.f, l = 0.f;
+    for (int j = lane; j < r.top; j += 32) {
+        if (teach[j] == -NB200_INF) continue;
+        const float q = expf(teach[j] - z);
+        mass += q;
+        if (q != 0.f) l += q * ((teach[j] - z) - (stud[j] - lse));
+    }
+    mass = warp_sum(mass);
+    l = warp_sum(l);
+    if (lane == 0) {
         loss[row] = l;
         stats[3 * row] = lse;
         stats[3 * row + 1] = z;
@@ -235,7 +256,6 @@ __global__ void __launch_bounds__(kBwdThreads)
         p[t] = pm;
     }
     const bool any = __syncthreads_or(mine >= 0);
-    constexpr float kL2e = 1.4426950408889634f;
     const float wm = w * mass;
     // w mass q, the difference taken before the change of base so that large logits keep their digits; a
     // row without kept entries is 0 whatever its logits hold.
