@@ -46,25 +46,95 @@ __device__ __forceinline__ float gate_slope(float a, int kind) {
     return 1.f;
 }
 
+// NV 16-byte vectors' worth of a row's elements, zero past the row.
+template <typename T, int NV>
+struct Vecs {
+    static constexpr int V = Elem<T>::V, P = NV * V / 2;
+    uint4 raw[NV];
+    __device__ __forceinline__ float get(int i) const { return Elem<T>::lane(raw[i / V], i % V); }
+    __device__ __forceinline__ uint64_t pair(int i) const { return f2(get(2 * i), get(2 * i + 1)); }
+};
+
 // A row is held by a warp (CTA false, kWarpRows of them in a CTA) or a whole CTA, E = NV * V elements a
 // thread, computed as packed fp32 pairs. A unit (warp or CTA) works through consecutive rows, so that the
 // weights stay in registers and a gate row is read and put through its activation once per group.
-template <typename T, int NV, bool VEC, bool CTA>
+//
+// Element i of thread t is column (t + (i / V) G) V + i % V. Rows of 16-bit elements that do not start on a
+// 16-byte boundary (ALIGNED false: odd widths, slices) move in 16-byte vectors as well. All threads of a row are off by the same number of bytes: a load takes the two aligned vectors it
+// straddles (never one without a byte of the row) and shifts; a store passes its last elements to the next
+// lane, which writes the aligned vector they begin, and the few elements at the ends of a warp's span go one
+// by one (bf16 [16384, 3001] 431 us backward; 795 us element by element). Such rows of fp32 go element by
+// element, column t + i G, which was the faster there ([3003, 1001] 36 us, 54 us by vectors).
+template <typename T, int NV, bool ALIGNED, bool CTA>
 struct Rows {
-    using CH = Chunk<T, NV, VEC>;
-    static constexpr int V = CH::V, P = CH::E / 2;  // P pairs a thread
+    using CH = Vecs<T, NV>;
+    static constexpr int V = CH::V, P = CH::P;  // P pairs a thread
+    static constexpr bool SCALAR = !ALIGNED && sizeof(T) == 4;
     int t, G;
-    int64_t unit, width;
+    int64_t unit;
+    int width;
     float* buf;  // 2 x 4 x 32 entries of shared memory when CTA
     int phase = 0;
 
-    __device__ __forceinline__ Rows(int64_t w, float* b) : width(w), buf(b) {
+    __device__ __forceinline__ Rows(int64_t w, float* b) : width((int)w), buf(b) {
         t = threadIdx.x;
         G = blockDim.x;
         unit = CTA ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
     }
-    __device__ __forceinline__ void load(CH& c, const T* row, bool stream) const { c.load(row, 1, 0, width, t, G, stream); }
-    __device__ __forceinline__ static uint64_t pair(const CH& c, int i) { return f2(c.get(2 * i), c.get(2 * i + 1)); }
+    __device__ __forceinline__ int col(int k) const { return (t + k * G) * V; }  // of vector k
+    __device__ __forceinline__ int col_of(int i) const { return SCALAR ? t + i * G : col(i / V) + i % V; }
+    __device__ __forceinline__ static uint4 fetch(const void* p, bool stream) { return stream ? ld_stream(p) : ld_keep(p); }
+    __device__ __forceinline__ void load(CH& c, const T* row, bool stream) const {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int at = col(k);
+            if constexpr (ALIGNED) {
+                if (at < width) c.raw[k] = fetch(row + at, stream);
+                else c.raw[k] = make_uint4(0u, 0u, 0u, 0u);
+            } else if constexpr (SCALAR) {
+                uint32_t w[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int i = col_of(4 * k + j);
+                    w[j] = i < width ? __float_as_uint(row[i]) : 0u;
+                }
+                c.raw[k] = make_uint4(w[0], w[1], w[2], w[3]);
+            } else if (at >= width) {
+                c.raw[k] = make_uint4(0u, 0u, 0u, 0u);
+            } else {
+                const uintptr_t a = reinterpret_cast<uintptr_t>(row + at);
+                const uint32_t off = (uint32_t)a & 15u;  // the same for every thread of the row
+                const char* p = reinterpret_cast<const char*>(a - off);
+                uint4 lo = fetch(p, stream), hi = make_uint4(0u, 0u, 0u, 0u);
+                if (off && p + 16 < reinterpret_cast<const char*>(row + width)) hi = fetch(p + 16, stream);
+                c.raw[k] = shift_down(lo, hi, off);
+                if (at + V > width) keep_first(c.raw[k], width - at);
+            }
+        }
+    }
+    // 16 bytes from byte `off` of lo:hi.
+    __device__ __forceinline__ static uint4 shift_down(const uint4& lo, const uint4& hi, uint32_t off) {
+        uint32_t w[7] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z};
+        const uint32_t last = hi.w;
+        if (off & 8u) {
+            w[0] = w[2], w[1] = w[3], w[2] = w[4], w[3] = w[5], w[4] = w[6], w[5] = last;
+        }
+        if (off & 4u) {
+            w[0] = w[1], w[1] = w[2], w[2] = w[3], w[3] = w[4], w[4] = w[5];
+        }
+        const uint32_t bits = (off & 2u) * 8u;
+        return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits),
+                          __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
+    }
+    __device__ __forceinline__ static void keep_first(uint4& u, int n) {
+        uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (2 * i >= n) w[i] = 0u;
+            else if (2 * i + 1 >= n) w[i] &= 0xffffu;
+        }
+        u = make_uint4(w[0], w[1], w[2], w[3]);
+    }
     __device__ __forceinline__ void store(T* row, const uint64_t* v) const {
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
@@ -74,7 +144,46 @@ struct Rows {
                 f[2 * j] = f2lo(v[k * V / 2 + j]);
                 f[2 * j + 1] = f2hi(v[k * V / 2 + j]);
             }
-            store_vec<T, NV, VEC>(row, f, k, 0, width, t, G, VEC);
+            const int at = col(k);
+            if constexpr (ALIGNED) {
+                if (at < width) st_stream(row + at, Elem<T>::pack(f));
+            } else if constexpr (SCALAR) {
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    if (col_of(k * V + j) < width) row[col_of(k * V + j)] = f[j];
+            } else {
+                store_shifted(row, at, Elem<T>::pack(f));
+            }
+        }
+    }
+    // Whole warps come here. `own` elements at the start of a vector share their aligned 16 bytes with the last
+    // `pass` elements of the lane below.
+    __device__ __forceinline__ void store_shifted(T* row, int at, const uint4& u) const {
+        const uintptr_t a = reinterpret_cast<uintptr_t>(row) + (uintptr_t)at * sizeof(T);
+        const uint32_t off = (uint32_t)a & 15u;
+        const int pass = off / (int)sizeof(T), own = V - pass, lane = t & 31;
+        const int valid = max(0, min(V, width - at)), above = max(0, min(V, width - at - V));
+        uint4 below;
+        below.x = __shfl_up_sync(0xffffffffu, u.x, 1);
+        below.y = __shfl_up_sync(0xffffffffu, u.y, 1);
+        below.z = __shfl_up_sync(0xffffffffu, u.z, 1);
+        below.w = __shfl_up_sync(0xffffffffu, u.w, 1);
+        if ((lane > 0 || pass == 0) && valid >= own)
+            st_stream(reinterpret_cast<void*>(a - off), pass ? shift_down(below, u, 16u - off) : u);
+        // Elements no whole vector takes: the head of a warp's first lane, the tail of its last, the row's end.
+        uint32_t single = 0;
+        if (lane == 0 ? pass != 0 : valid < own) single |= (1u << own) - 1u;
+        if (pass && (lane == 31 || above < own)) single |= ((1u << V) - 1u) & ~((1u << own) - 1u);
+        if (pass == 0 && valid == V) single = 0;
+        if (pass == 0 && valid < V) single = (1u << V) - 1u;
+        single &= (1u << valid) - 1u;
+        if (__any_sync(0xffffffffu, single)) {
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                if (!(single >> j & 1u)) continue;
+                reinterpret_cast<uint16_t*>(row)[at + j] = (uint16_t)(w[j / 2] >> (16 * (j & 1)));
+            }
         }
     }
     // The sum of v over the row's threads, in every thread: warp shuffles, then the warps' sums (one
@@ -131,11 +240,11 @@ struct GatePos {
     }
 };
 
-template <typename T, int NV, bool VEC, bool CTA, int kThreads>
-__global__ void __launch_bounds__(kThreads, NV * Elem<T>::V == 8 ? 1024 / kThreads : 1)
+template <typename T, int NV, bool ALIGNED, bool CTA, int kThreads>
+__global__ void __launch_bounds__(kThreads, (CTA || ALIGNED) && NV * Elem<T>::V == 8 ? 1024 / kThreads : 1)
     norm_fwd_kernel(const T* x, const T* res, const T* gate, const T* w1, const T* w2, Norm n, int64_t per_unit, T* y,
                     T* h, float* rstd) {
-    using R = Rows<T, NV, VEC, CTA>;
+    using R = Rows<T, NV, ALIGNED, CTA>;
     using CH = typename R::CH;
     constexpr int P = R::P;
     __shared__ float buf[CTA ? 256 : 1];
@@ -159,7 +268,7 @@ __global__ void __launch_bounds__(kThreads, NV * Elem<T>::V == 8 ? 1024 / kThrea
                 const uint64_t a = gate ? f2(n.scale * gate_value(cg.get(2 * i), n.act),
                                              n.scale * gate_value(cg.get(2 * i + 1), n.act))
                                         : f2(n.scale, n.scale);
-                b[i] = w1 ? mul2(a, R::pair(c1, i)) : a;
+                b[i] = w1 ? mul2(a, c1.pair(i)) : a;
             }
         }
         // The next row is on its way while this one is reduced.
@@ -177,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, NV * Elem<T>::V == 8 ? 1024 / kThrea
         uint64_t acc = 0;
         if (w1) {
 #pragma unroll
-            for (int i = 0; i < P; ++i) acc = fma2(R::pair(cx, i), R::pair(cx, i), acc);
+            for (int i = 0; i < P; ++i) acc = fma2(cx.pair(i), cx.pair(i), acc);
             float s = f2lo(acc) + f2hi(acc);
             s = r.sum(s);
             r1 = rsqrtf(s * n.inv_n + n.eps);
@@ -186,7 +295,7 @@ __global__ void __launch_bounds__(kThreads, NV * Elem<T>::V == 8 ? 1024 / kThrea
         acc = 0;
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-            v[i] = fma2(b[i], mul2(R::pair(cx, i), f2(r1, r1)), R::pair(cr, i));
+            v[i] = fma2(b[i], mul2(cx.pair(i), f2(r1, r1)), cr.pair(i));
             acc = fma2(v[i], v[i], acc);
         }
         r.store(y + row * n.width, v);
@@ -195,13 +304,29 @@ __global__ void __launch_bounds__(kThreads, NV * Elem<T>::V == 8 ? 1024 / kThrea
             s = r.sum(s);
             r2 = rsqrtf(s * n.inv_n + n.eps);
 #pragma unroll
-            for (int i = 0; i < P; ++i) v[i] = mul2(v[i], mul2(R::pair(c2, i), f2(r2, r2)));
+            for (int i = 0; i < P; ++i) v[i] = mul2(v[i], mul2(c2.pair(i), f2(r2, r2)));
             r.store(h + row * n.width, v);
         }
         if (r.t == 0) *reinterpret_cast<float2*>(rstd + 2 * row) = make_float2(r1, r2);
         cx = nx;
         cr = nr;
     }
+}
+
+// Threads of a row and elements of a thread: a warp of 8 holds up to 256 elements, a CTA of at most 512 threads up
+// to 4096 (8 a thread) or 8192 (16), a CTA of 1024 the rest.
+struct Shape {
+    bool cta, aligned;
+    int e, threads;
+};
+
+Shape make_shape(int64_t width) {
+    Shape s;
+    s.aligned = false;
+    s.cta = width > 256;
+    s.e = width <= 4096 ? 8 : 16;
+    s.threads = s.cta ? (int)((width + 32 * s.e - 1) / (32 * s.e)) * 32 : 32;
+    return s;
 }
 
 // How the backward pass cuts the rows: `per_group` chunks of each gate group, or (per_group 1) chunks
@@ -217,17 +342,20 @@ struct Chunks {
 };
 
 Chunks make_chunks(const Norm& n) {
-    // Two CTAs on every SM, each unit of which holds one chunk.
-    const int64_t target = 2 * sm_count() * (n.width > 512 ? 1 : kWarpRows);
-    const int64_t want = (n.rows + target - 1) / target;  // rows per chunk
+    // 512 threads on every SM, about what fits one at a time, and one chunk for each unit of them: more chunks
+    // mean more partial sums to write and add (bf16 [32768, 1024] 95 us, with twice as many 103).
+    const Shape s = make_shape(n.width);
+    const int64_t target = (int64_t)sm_count() * (s.cta ? std::max(1, 512 / s.threads) : 2 * kWarpRows);
+    const int64_t groups = n.rows / n.group;
     Chunks c;
-    if (n.group > want) {
-        c.rows = want;
-        c.per_group = (n.group + want - 1) / want;
-        c.count = n.rows / n.group * c.per_group;
+    if (groups < target) {  // a part of a group each, at most `target` in all
+        c.per_group = std::min(n.group, std::max<int64_t>(1, target / groups));
+        c.rows = (n.group + c.per_group - 1) / c.per_group;
+        c.per_group = (n.group + c.rows - 1) / c.rows;
+        c.count = groups * c.per_group;
     } else {
         c.per_group = 1;
-        c.rows = (want + n.group - 1) / n.group * n.group;
+        c.rows = (groups + target - 1) / target * n.group;
         c.count = (n.rows + c.rows - 1) / c.rows;
     }
     return c;
@@ -238,7 +366,7 @@ template <typename R>
 __device__ __forceinline__ void store_part(float* part, const uint64_t* acc, const R& r) {
 #pragma unroll
     for (int i = 0; i < 2 * R::P; ++i) {
-        const int64_t c = R::CH::col_of(0, r.t, r.G, i);
+        const int c = r.col_of(i);
         if (c < r.width) part[c] = i & 1 ? f2hi(acc[i / 2]) : f2lo(acc[i / 2]);
     }
 }
@@ -252,12 +380,12 @@ __device__ __forceinline__ void store_part(float* part, const uint64_t* acc, con
 // thread). That takes one CTA of 512 threads per SM; two at 64 registers a thread, with or without a ring of
 // bulk copies in shared memory in place of the registers, spilled and ran slower (bf16 [16384, 4096]: 250
 // and 294 us).
-template <typename T, int NV, bool VEC, bool CTA, int kThreads>
+template <typename T, int NV, bool ALIGNED, bool CTA, int kThreads>
 __global__ void __launch_bounds__(kThreads)
     norm_bwd_kernel(const T* dy, const T* dh, const T* x, const T* res, const T* gate, const T* w1, const T* w2,
                     const float* rstd, Norm n, Chunks ch, T* dx, T* dres, T* dgate, float* part1, float* part2,
                     float* partg) {
-    using R = Rows<T, NV, VEC, CTA>;
+    using R = Rows<T, NV, ALIGNED, CTA>;
     using CH = typename R::CH;
     constexpr int P = R::P;
     constexpr bool AHEAD = P == 4;
@@ -309,7 +437,7 @@ __global__ void __launch_bounds__(kThreads)
                                         : f2(1.f, 1.f);
                 const uint64_t a = mul2(v, f2(n.scale, n.scale));
                 as[i * r.G] = v;
-                bs[i * r.G] = w1 ? mul2(a, R::pair(c1, i)) : a;
+                bs[i * r.G] = w1 ? mul2(a, c1.pair(i)) : a;
             }
         }
         const float r1 = w1 ? rs.x : 1.f, r2 = w2 ? rs.y : 1.f;
@@ -318,23 +446,22 @@ __global__ void __launch_bounds__(kThreads)
         uint64_t s1 = 0, s2 = 0, s3 = 0;
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-            const uint64_t c = mul2(bs[i * r.G], mul2(R::pair(cx, i), r1p));
-            yhat[i] = mul2(add2(c, R::pair(cr, i)), r2p);
-            const uint64_t t = dh ? mul2(R::pair(cdh, i), R::pair(c2, i)) : 0;
-            e[i] = fma2(t, r2p, dy ? R::pair(cdy, i) : 0);
+            const uint64_t c = mul2(bs[i * r.G], mul2(cx.pair(i), r1p));
+            yhat[i] = mul2(add2(c, cr.pair(i)), r2p);
+            const uint64_t t = dh ? mul2(cdh.pair(i), c2.pair(i)) : 0;
+            e[i] = fma2(t, r2p, dy ? cdy.pair(i) : 0);
             s1 = fma2(t, yhat[i], s1);
             s2 = fma2(c, e[i], s2);
             s3 = fma2(c, yhat[i], s3);
-            if (dh) a2[i] = fma2(R::pair(cdh, i), yhat[i], a2[i]);
+            if (dh) a2[i] = fma2(cdh.pair(i), yhat[i], a2[i]);
         }
         // Issued here, the loads cover the sums' latency.
         if (AHEAD && row + 1 < end) fetch(row + 1);
         if (gate && g.left == 1 && row + 1 < end && (r.t & 7) == 0)
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
-                const int64_t c = CH::col_of(0, r.t, r.G, k * R::V);
-                if (c < n.width)
-                    asm volatile("prefetch.global.L2 [%0];" ::"l"(gate + (g.index + 1) * n.sg + c));
+                if (r.col(k) < r.width)
+                    asm volatile("prefetch.global.L2 [%0];" ::"l"(gate + (g.index + 1) * n.sg + r.col(k)));
             }
         float t1 = f2lo(s1) + f2hi(s1), t2 = f2lo(s2) + f2hi(s2), t3 = f2lo(s3) + f2hi(s3);
         r.sum3(t1, t2, t3);
@@ -342,7 +469,7 @@ __global__ void __launch_bounds__(kThreads)
         const uint64_t k2p = f2(-k2, -k2), k1p = f2(w1 ? -m1 : 0.f, w1 ? -m1 : 0.f);
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-            const uint64_t xhat = mul2(R::pair(cx, i), r1p);
+            const uint64_t xhat = mul2(cx.pair(i), r1p);
             if (w2) e[i] = fma2(yhat[i], k2p, e[i]);  // dY
             G[i] = fma2(xhat, e[i], G[i]);
             yhat[i] = mul2(fma2(xhat, k1p, mul2(bs[i * r.G], e[i])), r1p);  // dx
@@ -361,7 +488,7 @@ __global__ void __launch_bounds__(kThreads)
                 const uint64_t a = as[i * r.G], g1 = mul2(G[i], f2(n.scale, n.scale));
                 a1[i * r.G] = fma2(a, g1, a1[i * r.G]);
                 G[i] = mul2(g1, f2(gate_slope(f2lo(a), n.act), gate_slope(f2hi(a), n.act)));
-                if (w1) G[i] = mul2(G[i], R::pair(c1, i));
+                if (w1) G[i] = mul2(G[i], c1.pair(i));
             }
             if (direct) r.store(dgate + ended * n.width, G);
             if (row + 1 == end) break;
@@ -409,38 +536,19 @@ __global__ void __launch_bounds__(kSumCols* kSumRows) norm_sum_kernel(Sums<T> a)
     a.out[which][group * a.width + c] = Elem<T>::from_f(s);
 }
 
-// Threads of a row and elements of a thread: a warp holds up to 512 elements, a CTA of at most 512
-// threads up to 4096 (8 a thread) or 8192 (16), a CTA of 1024 the rest.
-struct Shape {
-    bool cta, vec, wide, huge;
-    int threads;
-};
-
-Shape make_shape(int64_t width, int esize, bool aligned) {
-    Shape s;
-    s.vec = aligned && width * esize % 16 == 0;
-    s.cta = width > 512;
-    s.wide = s.cta ? width > 4096 : width > 256;
-    s.huge = width > 8192;
-    const int e = s.wide ? 16 : 8;
-    s.threads = s.cta ? (int)((width + 32 * e - 1) / (32 * e)) * 32 : 32;
-    return s;
-}
-
-// f(CTA, E, VEC, most threads) with the shape's compile-time values.
+// f(CTA, E, ALIGNED, most threads) with the shape's compile-time values.
 template <typename F>
 void dispatch(const Shape& s, F&& f) {
-    auto vec = [&](auto cta, auto e, auto most) {
-        if (s.vec) f(cta, e, std::true_type{}, most);
+    auto pick = [&](auto cta, auto e, auto most) {
+        if (s.aligned) f(cta, e, std::true_type{}, most);
         else f(cta, e, std::false_type{}, most);
     };
     using E8 = std::integral_constant<int, 8>;
     using E16 = std::integral_constant<int, 16>;
-    if (!s.cta && !s.wide) vec(std::false_type{}, E8{}, std::integral_constant<int, 32 * kWarpRows>{});
-    else if (!s.cta) vec(std::false_type{}, E16{}, std::integral_constant<int, 32 * kWarpRows>{});
-    else if (!s.wide) vec(std::true_type{}, E8{}, std::integral_constant<int, 512>{});
-    else if (!s.huge) vec(std::true_type{}, E16{}, std::integral_constant<int, 512>{});
-    else vec(std::true_type{}, E16{}, std::integral_constant<int, 1024>{});
+    if (!s.cta) pick(std::false_type{}, E8{}, std::integral_constant<int, 32 * kWarpRows>{});
+    else if (s.e == 8) pick(std::true_type{}, E8{}, std::integral_constant<int, 512>{});
+    else if (s.threads <= 512) pick(std::true_type{}, E16{}, std::integral_constant<int, 512>{});
+    else pick(std::true_type{}, E16{}, std::integral_constant<int, 1024>{});
 }
 
 bool rows_aligned(const void* p, int64_t stride, int esize) { return !p || (aligned16(p) && stride * esize % 16 == 0); }
@@ -475,10 +583,11 @@ int norm_fwd(const nb200_norm_args& a, T* y, T* h, float* rstd, cudaStream_t st)
     const bool al = rows_aligned(a.x, n.sx, es) && rows_aligned(a.residual, n.sr, es) &&
                     rows_aligned(a.gate, n.sg, es) && rows_aligned(a.post_weight, 0, es) &&
                     rows_aligned(a.pre_weight, 0, es) && aligned16(y) && (!h || aligned16(h));
-    const Shape s = make_shape(n.width, es, al);
+    Shape s = make_shape(n.width);
+    s.aligned = al && n.width * es % 16 == 0;
     const int per = s.cta ? 1 : kWarpRows;
-    dispatch(s, [&](auto cta, auto e, auto vec, auto most) {
-        auto kernel = norm_fwd_kernel<T, decltype(e)::value / Elem<T>::V, decltype(vec)::value, decltype(cta)::value,
+    dispatch(s, [&](auto cta, auto e, auto aligned, auto most) {
+        auto kernel = norm_fwd_kernel<T, decltype(e)::value / Elem<T>::V, decltype(aligned)::value, decltype(cta)::value,
                                       decltype(most)::value>;
         // Units enough to fill the GPU, each with an equal share of consecutive rows.
         const int64_t units = per * (int64_t)persistent_grid(kernel, s.threads * per, 0, (n.rows + per - 1) / per, 0);
@@ -500,15 +609,16 @@ int norm_bwd(const nb200_norm_args& a, const float* rstd, const T* dy, const T* 
                     rows_aligned(a.gate, n.sg, es) && rows_aligned(a.post_weight, 0, es) &&
                     rows_aligned(a.pre_weight, 0, es) && rows_aligned(dy, n.sdy, es) && rows_aligned(dh, n.sdh, es) &&
                     aligned16(dx) && aligned16(dres) && (!dgate || aligned16(dgate));
-    const Shape s = make_shape(n.width, es, al);
+    Shape s = make_shape(n.width);
+    s.aligned = al && n.width * es % 16 == 0;
     const int per = s.cta ? 1 : kWarpRows;
     const Chunks ch = make_chunks(n);
     const int64_t size = ch.count * n.width;
     float* p1 = dw1 ? work : nullptr;
     float* p2 = dw2 ? work + size : nullptr;
     float* pg = dgate && ch.per_group > 1 ? work + 2 * size : nullptr;
-    dispatch(s, [&](auto cta, auto e, auto vec, auto most) {
-        auto kernel = norm_bwd_kernel<T, decltype(e)::value / Elem<T>::V, decltype(vec)::value, decltype(cta)::value,
+    dispatch(s, [&](auto cta, auto e, auto aligned, auto most) {
+        auto kernel = norm_bwd_kernel<T, decltype(e)::value / Elem<T>::V, decltype(aligned)::value, decltype(cta)::value,
                                       decltype(most)::value>;
         const int smem = 3 * per * s.threads * decltype(e)::value * (int)sizeof(float);
         if (smem > 40 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
