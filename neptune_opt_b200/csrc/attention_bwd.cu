@@ -29,8 +29,14 @@
 // memory. S and dP of step j+1 are issued as soon as the warps hold step j in registers, dQ(j) when dS(j)
 // is stored: the exponentials of a step (1024 cycles of the special-function unit) run under the products.
 //
+// Where a few key CTAs would run far longer than the rest (shared heads: a key CTA streams every query head
+// of its group), each is cut into `parts` CTAs of consecutive steps whose fp32 sums a third kernel adds in
+// order and rounds.
+//
 // Every wait is bounded; one that runs out sets the attention fault bit and the CTA's abort flag, the
 // roles stop at their next wait and the outputs stay unwritten.
+#include <algorithm>
+
 #include "attn.cuh"
 
 namespace nb200 {
@@ -86,7 +92,7 @@ constexpr uint32_t kSmemBytes = kOffBar + sizeof(Bars);
 static_assert(kSmemBytes <= 232448, "shared memory of a CTA");
 
 struct BwdArgs {
-    int S, Spad, H, Hk, group, key_ctas, blocks, causal;
+    int S, Spad, H, Hk, group, parts, key_ctas, blocks, causal;
     float scale, sl2;
     const int* lens;
     const __nv_bfloat16* go;
@@ -94,6 +100,8 @@ struct BwdArgs {
     nb200_attn_strides sgo, sdq, sdk, sdv;
     const float* nlse2;   // [batch, heads, Spad]: -lse log2(e), -inf where the row sees nothing
     const float* ndelta;  // [batch, heads, Spad]: -delta
+    float *part_k, *part_v;  // [parts, batch, kv_heads, S, 128], with parts > 1
+    int64_t part_rows;       // batch * kv_heads * S
 };
 
 struct Maps {
@@ -304,6 +312,20 @@ __device__ __forceinline__ void write_row(uint32_t col, __nv_bfloat16* row, bool
     }
 }
 
+// The same as fp32, unscaled.
+__device__ __forceinline__ void write_row_f32(uint32_t col, float* row) {
+#pragma unroll
+    for (int c = 0; c < kDim / 32; ++c) {
+        uint32_t v[32];
+        __syncwarp();
+        tc::tmem_ld32(col + 32 * c, v);
+        if (!row) continue;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            *reinterpret_cast<uint4*>(row + 32 * c + 4 * i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    }
+}
+
 // Two fp32 values as bf16 pairs: rounded, and (kPair) what the rounding left.
 template <bool kPair>
 __device__ __forceinline__ void round_pair(uint64_t x, uint32_t& hi, uint32_t& lo) {
@@ -373,7 +395,7 @@ __device__ __forceinline__ void query_warps(Bars* b, uint32_t tmem, const BwdArg
 
 template <bool kPair>
 __device__ __forceinline__ void key_warps(uint8_t* smem, Bars* b, uint32_t tmem, const BwdArgs& a, int batch, int head,
-                                          int len, int k0, int first, int per_head, int n) {
+                                          int len, int k0, int first, int per_head, int skip, int n, int part) {
     volatile int* abort = &b->abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = warp >> 2;
     const int row = k0 + (warp & 3) * 32 + lane;
@@ -382,7 +404,7 @@ __device__ __forceinline__ void key_warps(uint8_t* smem, Bars* b, uint32_t tmem,
     const uint64_t sl2 = f2(a.sl2, a.sl2);
     const uint32_t tS = t + kColKeyS + 64 * half, tDP = t + kColKeyDP + 64 * half;
     bool ok = true;
-    for (int i = 0, step = first; i < n; ++i) {
+    for (int i = 0, step = first + skip % per_head; i < n; ++i) {
         const uint32_t ph = i & 1u;
         ok = wait_bar(&b->s_full, ph, abort) && wait_bar(&b->stat_full[ph], (i >> 1) & 1u, abort);
         if (!(ok = __all_sync(0xffffffffu, ok))) break;
@@ -442,6 +464,11 @@ __device__ __forceinline__ void key_warps(uint8_t* smem, Bars* b, uint32_t tmem,
     if (ok) ok = __all_sync(0xffffffffu, wait_bar(&b->done, 0, abort));
     if (!ok) return;
     tc::fence_after();
+    if (a.parts > 1) {
+        const int64_t at = part * a.part_rows + ((int64_t)batch * a.Hk + head) * a.S + row;
+        write_row_f32(t + (half ? kColDK : kColDV), live ? (half ? a.part_k : a.part_v) + at * kDim : nullptr);
+        return;
+    }
     const nb200_attn_strides& so = half ? a.sdk : a.sdv;
     __nv_bfloat16* out = row < a.S ? (half ? a.dk : a.dv) + offset(so, batch, head, row) : nullptr;
     write_row<128>(t + (half ? kColDK : kColDV), out, live, half ? a.scale : 1.f);
@@ -454,18 +481,19 @@ __device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* m, in
     tc::tma_load_4d(dst + kHalfBytes, m, kDim / 2, row, head, batch, bar);
 }
 
-// Streams n steps of two tiles: steps first .. first + per_head - 1 of heads head0, head0 + 1, ... Rows past
+// Streams n steps of two tiles from step `skip` on of steps first .. first + per_head - 1 of heads head0, head0 + 1,
+// ... Rows past
 // the sequence in a head's last step are zeroed before the tile is published (`tail` rows remain; 0: none
 // to zero): they enter sums over the streamed rows, where a coefficient of 0 times an infinity or NaN
 // would still poison the result. A key CTA's steps come with their rows' statistics.
 template <bool kKeys>
 __device__ __forceinline__ void produce(const CUtensorMap* mx, const CUtensorMap* my, uint8_t* smem, Bars* b,
-                                        int batch, int head0, int first, int per_head, int n, int tail,
+                                        int batch, int head0, int first, int per_head, int skip, int n, int tail,
                                         const BwdArgs& a, int lane) {
     constexpr int kStages = kKeys ? kKeyStages : kQueryStages;
     volatile int* abort = &b->abort;
     Ring<kStages> r;
-    int it = 0, head = head0, step = first;
+    int it = 0, head = head0 + skip / per_head, step = first + skip % per_head;
     uint32_t tail_ph = 0;
     bool ok = true;
     for (; it < 2 * n; ++it, r.next()) {
@@ -519,7 +547,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_kernel(const __grid_cons
     // Head-major order in both parts, so that the CTAs that run side by side share their streamed tiles
     // through L2; under a causal mask the longest of a head come first.
     const bool keys = (int)blockIdx.x < a.key_ctas;
-    const int id = keys ? blockIdx.x : blockIdx.x - a.key_ctas;
+    const int part = keys ? blockIdx.x % a.parts : 0;
+    const int id = keys ? blockIdx.x / a.parts : blockIdx.x - a.key_ctas;
     const int blocks = a.blocks, heads = keys ? a.Hk : a.H;
     const int batch = id / blocks / heads, head = id / blocks % heads;
     const int row0 = (keys ? id % blocks : blocks - 1 - id % blocks) * kRows;
@@ -555,6 +584,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_kernel(const __grid_cons
     pdl_wait();
     const int len = tokens_of(a.lens, batch, a.S);
     if (row0 >= len) {  // none of the CTA's rows belongs to the sequence
+        if (keys && a.parts > 1) return;
         const int rows = min(kRows, a.S - row0);
         for (int i = threadIdx.x; i < rows * (kDim / 8); i += kThreads) {
             const int r = row0 + i / (kDim / 8), c = i % (kDim / 8) * 8;
@@ -572,7 +602,17 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_kernel(const __grid_cons
     const int first = keys && a.causal ? row0 / kStep : 0;
     const int end = !keys && a.causal ? min(row0 + kRows, len) : len;
     const int per_head = (end + kStep - 1) / kStep - first;
-    const int n = keys ? a.group * per_head : per_head;
+    const int all = keys ? a.group * per_head : per_head;
+    const int skip = keys ? (int)((int64_t)all * part / a.parts) : 0;
+    const int n = keys ? (int)((int64_t)all * (part + 1) / a.parts) - skip : all;
+    if (n == 0) {  // a part without steps: its sums are zero
+        for (int i = threadIdx.x; i < min(kRows, len - row0) * (kDim / 4); i += kThreads) {
+            const int64_t at = (part * a.part_rows + ((int64_t)batch * a.Hk + head) * a.S + row0) * kDim + 4 * i;
+            *reinterpret_cast<uint4*>(a.part_k + at) = *reinterpret_cast<uint4*>(a.part_v + at) =
+                make_uint4(0u, 0u, 0u, 0u);
+        }
+        return;
+    }
     const int tail = (first + per_head) * kStep > len && len < a.S ? len - (first + per_head - 1) * kStep : 0;
     // Some row's sum has fewer than kRows terms: queries that see few keys, keys few queries see.
     const bool pair = a.causal ? (keys ? row0 + 2 * kRows > len : row0 == 0) : len < kRows;
@@ -589,8 +629,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_kernel(const __grid_cons
         // nothing was issued
     } else if (warp < 8) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
-        if (keys && pair) key_warps<true>(smem, b, tmem, a, batch, head, len, row0, first, per_head, n);
-        else if (keys) key_warps<false>(smem, b, tmem, a, batch, head, len, row0, first, per_head, n);
+        if (keys && pair) key_warps<true>(smem, b, tmem, a, batch, head, len, row0, first, per_head, skip, n, part);
+        else if (keys) key_warps<false>(smem, b, tmem, a, batch, head, len, row0, first, per_head, skip, n, part);
         else if (pair) query_warps<true>(b, tmem, a, batch, head, len, row0, n);
         else query_warps<false>(b, tmem, a, batch, head, len, row0, n);
     } else {
@@ -608,8 +648,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_kernel(const __grid_cons
                 if (keys) load_tile(own + kTileBytes, &m.v, row0, head, batch, &b->own);
             }
             __syncwarp();
-            if (keys) produce<true>(&m.q, &m.go, smem, b, batch, head * a.group, first, per_head, n, tail, a, lane);
-            else produce<false>(&m.k, &m.v, smem, b, batch, head / a.group, 0, per_head, n, tail, a, lane);
+            if (keys) produce<true>(&m.q, &m.go, smem, b, batch, head * a.group, first, per_head, skip, n, tail, a, lane);
+            else produce<false>(&m.k, &m.v, smem, b, batch, head / a.group, 0, per_head, 0, n, tail, a, lane);
         }
         __syncwarp();
     }
@@ -621,16 +661,51 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_kernel(const __grid_cons
     }
 }
 
+// dK and dV from the parts' sums, in part order; a warp per row, four columns a lane.
+constexpr int kJoinRows = 8;
+__global__ void __launch_bounds__(32 * kJoinRows) bwd_join_kernel(BwdArgs a) {
+    pdl_wait();
+    const int64_t row = (int64_t)blockIdx.x * kJoinRows + (threadIdx.x >> 5);
+    if (row >= a.part_rows) return;
+    const int lane = threadIdx.x & 31, i = (int)(row % a.S), head = (int)(row / a.S % a.Hk);
+    const int batch = (int)(row / a.S / a.Hk);
+    float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
+    if (i < tokens_of(a.lens, batch, a.S))
+        for (int p = 0; p < a.parts; ++p) {
+            const int64_t at = ((p * a.part_rows + row) * kDim) / 4 + lane;
+            const float4 x = reinterpret_cast<const float4*>(a.part_k)[at], y = reinterpret_cast<const float4*>(a.part_v)[at];
+            k.x += x.x, k.y += x.y, k.z += x.z, k.w += x.w;
+            v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
+        }
+    *reinterpret_cast<uint2*>(a.dk + offset(a.sdk, batch, head, i) + 4 * lane) =
+        make_uint2(tc::pack_bf16(k.x * a.scale, k.y * a.scale), tc::pack_bf16(k.z * a.scale, k.w * a.scale));
+    *reinterpret_cast<uint2*>(a.dv + offset(a.sdv, batch, head, i) + 4 * lane) =
+        make_uint2(tc::pack_bf16(v.x, v.y), tc::pack_bf16(v.z, v.w));
+}
+
 SharedLimit g_shared;
 
 int64_t padded(int64_t seq) { return (seq + kStep - 1) / kStep * kStep; }
+
+// CTAs a key block is cut into. A step of a key CTA takes about 3 units of time, one of a query CTA 2; the longest
+// key CTA should not take much longer than an SM's share of all steps, nor a part run fewer than 4 steps.
+// bf16 [4, 16 heads on 4, 1000, 128] causal: 68 us with one part, PARTS_US with four.
+int parts_of(const nb200_attn_args& n) {
+    const int64_t blocks = (n.seq + kRows - 1) / kRows, group = n.heads / n.kv_heads;
+    const int64_t pairs = n.causal ? blocks * (blocks + 1) / 2 : blocks * blocks;  // (key block, query step)
+    const int64_t share = 5 * n.batch * n.heads * pairs / sm_count(), longest = 3 * group * blocks;
+    const int64_t most = group * blocks / 4;
+    return (int)std::max<int64_t>(1, std::min(most, longest / std::max<int64_t>(share, 1)));
+}
 
 }  // namespace
 
 int attn_bwd_fault_take(unsigned int* bits) { return take_attn_fault(bits); }
 
 int64_t attention_bwd_work_bytes(const nb200_attn_args& n) {
-    return 2 * n.batch * n.heads * padded(n.seq) * (int64_t)sizeof(float);
+    const int64_t parts = parts_of(n);
+    return 2 * (int64_t)sizeof(float) *
+           (n.batch * n.heads * padded(n.seq) + (parts > 1 ? parts * n.batch * n.kv_heads * n.seq * kDim : 0));
 }
 
 int launch_attention_bwd(const nb200_attn_args& n, const nb200_attn_strides* strides, const void* q, const void* k,
@@ -639,7 +714,8 @@ int launch_attention_bwd(const nb200_attn_args& n, const nb200_attn_strides* str
     const char* what = "nb200_attention_bwd";
     using B = __nv_bfloat16;
     const int64_t blocks = (n.seq + kRows - 1) / kRows, pad = padded(n.seq), rows = n.batch * n.heads * pad;
-    const int64_t ctas = n.batch * (n.heads + n.kv_heads) * blocks, stat_ctas = (rows + kStatRows - 1) / kStatRows;
+    const int64_t parts = parts_of(n), part_rows = n.batch * n.kv_heads * n.seq;
+    const int64_t ctas = n.batch * (n.heads + n.kv_heads * parts) * blocks, stat_ctas = (rows + kStatRows - 1) / kStatRows;
     if (ctas > 0x7fffffffLL || stat_ctas > 0x7fffffffLL) {
         set_error("%s: batch*heads=%lld, seq=%lld exceed the kernel's index range", what,
                   (long long)(n.batch * n.heads), (long long)n.seq);
@@ -673,7 +749,11 @@ int launch_attention_bwd(const nb200_attn_args& n, const nb200_attn_strides* str
     a.H = (int)n.heads;
     a.Hk = (int)n.kv_heads;
     a.group = (int)(n.heads / n.kv_heads);
-    a.key_ctas = (int)(n.batch * n.kv_heads * blocks);
+    a.parts = (int)parts;
+    a.key_ctas = (int)(n.batch * n.kv_heads * blocks * parts);
+    a.part_k = s.ndelta + rows;
+    a.part_v = a.part_k + parts * part_rows * kDim;
+    a.part_rows = part_rows;
     a.blocks = (int)blocks;
     a.causal = n.causal ? 1 : 0;
     a.scale = n.scale;
@@ -691,6 +771,10 @@ int launch_attention_bwd(const nb200_attn_args& n, const nb200_attn_strides* str
     a.ndelta = s.ndelta;
     launch_pdl(attn_bwd_kernel, (unsigned)ctas, kThreads, kSmemBytes, st, m, a);
     count_launch(2);
+    if (parts > 1) {
+        launch_pdl(bwd_join_kernel, (unsigned)((part_rows + kJoinRows - 1) / kJoinRows), 32 * kJoinRows, 0, st, a);
+        count_launch();
+    }
     return finish_launch(what);
 }
 
