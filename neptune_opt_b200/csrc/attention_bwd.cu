@@ -35,6 +35,8 @@
 //
 // Every wait is bounded; one that runs out sets the attention fault bit and the CTA's abort flag, the
 // roles stop at their next wait and the outputs stay unwritten.
+#include <stddef.h>
+
 #include <algorithm>
 
 #include "attn.cuh"
@@ -62,8 +64,8 @@ constexpr int kLoadWarp = 9;
 constexpr int kThreads = 384;  // warps 10-11 only complete the third warpgroup for the register split
 // Register split (setmaxnreg, per warpgroup), within what the block is launched with.
 constexpr int kLaunchRegs = 168;
-constexpr int kRegsSoftmax = 216;
-constexpr int kRegsControl = 72;
+constexpr int kRegsSoftmax = 208;
+constexpr int kRegsControl = 88;
 static_assert(2 * 128 * kRegsSoftmax + 128 * kRegsControl <= kThreads * kLaunchRegs, "register split");
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kIdescScores = tc::idesc_bf16(128, kStep, false);
@@ -72,22 +74,29 @@ constexpr uint32_t kColDV = 0, kColDK = 128, kColKeyS = 256, kColKeyDP = 384;
 constexpr uint32_t kColDQ = 0, kColQueryS = 128, kColQueryDP = 256, kColDS = 384, kColDO = 448;
 
 struct Bars {
+    // one arrival a phase
     uint64_t full[kQueryStages];
     uint64_t empty[kQueryStages];
-    uint64_t s_full;       // S is in TMEM (a query CTA: S and dP)
-    uint64_t dp_full;      // dP is in TMEM (key CTA)
-    uint64_t p_full[2];    // P of a column half is in TMEM (one arrival per warp)
-    uint64_t ds_full[2];   // dS of a column half
-    uint64_t read;         // a query CTA's S and dP are in registers (one arrival per warp)
-    uint64_t ds_free;      // a query CTA's dS has been consumed
-    uint64_t stat_full[2], stat_empty[2];  // statistics of a key CTA's step
-    uint64_t own;          // the CTA's own operands in shared memory
-    uint64_t own_tmem;     // ... and in TMEM (one arrival per warp)
+    uint64_t s_full;        // S is in TMEM (a query CTA: S and dP)
+    uint64_t dp_full;       // dP is in TMEM (key CTA)
+    uint64_t ds_free;       // a query CTA's dS has been consumed
+    uint64_t stat_full[2];  // statistics of a key CTA's step
+    uint64_t own;           // the CTA's own operands in shared memory
     uint64_t done;
-    uint64_t tail;         // a streamed tile with masked rows, before it is published
+    uint64_t tail;          // a streamed tile with masked rows, before it is published
+    // one arrival from each of four warps
+    uint64_t p_full[2];     // P of a column half is in TMEM
+    uint64_t ds_full[2];    // dS of a column half
+    // one arrival from each of eight warps
+    uint64_t read;          // a query CTA's S and dP are in registers
+    uint64_t stat_empty[2];
+    uint64_t own_tmem;      // the own operand in TMEM
     uint32_t tmem_base;
     int abort;
 };
+constexpr int kFourArrivals = offsetof(Bars, p_full) / 8, kEightArrivals = offsetof(Bars, read) / 8;
+constexpr int kBarriers = offsetof(Bars, tmem_base) / 8;
+static_assert(kBarriers <= 32, "one lane sets up one barrier");
 constexpr uint32_t kSmemBytes = kOffBar + sizeof(Bars);
 static_assert(kSmemBytes <= 232448, "shared memory of a CTA");
 
@@ -105,7 +114,8 @@ struct BwdArgs {
 };
 
 struct Maps {
-    CUtensorMap q, k, v, go;
+    CUtensorMap q, k, v, go;   // boxes of kStep rows
+    CUtensorMap dq, dk, dv;    // boxes of 32 rows: what one warp stores
 };
 
 __device__ __forceinline__ int64_t offset(const nb200_attn_strides& s, int64_t b, int64_t h, int64_t i) {
@@ -215,10 +225,11 @@ __device__ __forceinline__ void issue_query(uint8_t* smem, Bars* b, uint32_t tme
     const uint64_t own = tc::sw128_desc(smem_u32(smem + kOffOwn), 16, 1024);
     Ring<kQueryStages> k, v, back;  // next K and V tile for S and dP; next K tile for dQ
     v.next();
-    auto scores = [&]() {
+    auto scores = [&](bool first) {
         if (!wait_bar(&b->full[k.s], k.ph, abort)) return false;
         tc::fence_after();
         scores_ss(tmem + kColQueryS, own, rd.k(k.s));
+        if (first && !wait_bar(&b->own_tmem, 0, abort)) return false;
         if (!wait_bar(&b->full[v.s], v.ph, abort)) return false;
         tc::fence_after();
         scores_ts(tmem + kColQueryDP, tmem + kColDO, rd.k(v.s));
@@ -227,10 +238,10 @@ __device__ __forceinline__ void issue_query(uint8_t* smem, Bars* b, uint32_t tme
         k.next(), k.next(), v.next(), v.next();
         return true;
     };
-    bool ok = wait_bar(&b->own_tmem, 0, abort) && wait_bar(&b->own, 0, abort) && scores();
+    bool ok = wait_bar(&b->own, 0, abort) && scores(true);
     for (int j = 0; ok && j < n; ++j) {
         const uint32_t ph = j & 1u;
-        if (j + 1 < n && !(ok = wait_bar(&b->read, ph, abort) && scores())) break;
+        if (j + 1 < n && !(ok = wait_bar(&b->read, ph, abort) && scores(false))) break;
         if (!(ok = grads(b->ds_full, ph, tmem + kColDQ, tmem + kColDS, 32, tmem + kColQueryS, rd.mn(back.s), j > 0,
                          pair, abort)))
             break;
@@ -277,28 +288,34 @@ __device__ __forceinline__ void issue_key(uint8_t* smem, Bars* b, uint32_t tmem,
 }
 
 // ------------------------------------------------------------------ the CTA's own operands
-// 64 bf16 of a row per lane into 32 TMEM columns (two elements a column); zeros without a row.
-__device__ __forceinline__ void own_row(uint32_t col, const __nv_bfloat16* row) {
-    uint32_t w[32];
+// What a softmax thread of a query CTA fetches for itself, on its way while the CTA sets up: 64 columns of its
+// row of dO (zeros without a row) and, once the kernel before is through, the row's statistics.
+struct QueryRow {
+    uint32_t go[32];
+    float nl, nd;
+    __device__ __forceinline__ void load(const BwdArgs& a, int batch, int head, int len, int q0) {
+        const int warp = threadIdx.x >> 5, row = q0 + (warp & 3) * 32 + (threadIdx.x & 31);
+        const bool live = row < len;
+        const __nv_bfloat16* src = a.go + offset(a.sgo, batch, head, row) + 64 * (warp >> 2);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const uint4 u = row ? ld_keep(row + 8 * i) : make_uint4(0u, 0u, 0u, 0u);
-        w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
+        for (int i = 0; i < 8; ++i) {
+            const uint4 u = live ? ld_keep(src + 8 * i) : make_uint4(0u, 0u, 0u, 0u);
+            go[4 * i] = u.x, go[4 * i + 1] = u.y, go[4 * i + 2] = u.z, go[4 * i + 3] = u.w;
+        }
+        pdl_wait();
+        const int64_t stat = ((int64_t)batch * a.H + head) * a.Spad + row;
+        nl = live ? a.nlse2[stat] : -NB200_INF;
+        nd = live ? a.ndelta[stat] : 0.f;
     }
-    __syncwarp();
-    tc::tmem_st32(col, w);
-}
+};
 
-// kCols accumulator columns of this lane's row, times `scale`, to `row` as bf16 (zeros if the row is
-// masked; nothing without a row).
-template <int kCols>
-__device__ __forceinline__ void write_row(uint32_t col, __nv_bfloat16* row, bool live, float scale) {
+// 64 accumulator columns of this lane's row, times `scale`, as bf16 into row r of half `h` of a staged tile, in the
+// swizzle the tensor maps expect (zeros if the row is masked).
+__device__ __forceinline__ void stage_half(uint32_t col, uint8_t* tile, int h, int r, bool live, float scale) {
 #pragma unroll
-    for (int c = 0; c < kCols / 32; ++c) {
+    for (int c = 0; c < 2; ++c) {
         uint32_t v[32];
-        __syncwarp();
         tc::tmem_ld32(col + 32 * c, v);
-        if (!row) continue;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             uint32_t w[4];
@@ -307,12 +324,26 @@ __device__ __forceinline__ void write_row(uint32_t col, __nv_bfloat16* row, bool
                 w[e] = live ? tc::pack_bf16(__uint_as_float(v[8 * i + 2 * e]) * scale,
                                             __uint_as_float(v[8 * i + 2 * e + 1]) * scale)
                             : 0u;
-            *reinterpret_cast<uint4*>(row + 32 * c + 8 * i) = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4*>(tile + h * kHalfBytes + r * 128 + (((4 * c + i) ^ (r & 7)) << 4)) =
+                make_uint4(w[0], w[1], w[2], w[3]);
         }
     }
 }
+// Stores halves h0 .. h1 - 1 of this warp's 32 staged rows; rows past the tensor are not written.
+__device__ __forceinline__ void store_rows(const CUtensorMap* m, const uint8_t* tile, int h0, int h1, int quarter,
+                                           int row, int seq, int head, int batch, int lane) {
+    fence_proxy_async();
+    __syncwarp();
+    if (lane == 0 && row < seq) {
+        for (int h = h0; h < h1; ++h)
+            tc::tma_store_4d(m, tile + h * kHalfBytes + quarter * 32 * 128, h * kDim / 2, row, head, batch);
+        tc::bulk_commit();
+        tc::bulk_wait_read();
+    }
+    __syncwarp();
+}
 
-// The same as fp32, unscaled.
+// The 128 accumulator columns of this lane's row as fp32 (nothing without a row).
 __device__ __forceinline__ void write_row_f32(uint32_t col, float* row) {
 #pragma unroll
     for (int c = 0; c < kDim / 32; ++c) {
@@ -342,19 +373,18 @@ __device__ __forceinline__ void publish(uint64_t* bar, int lane) {
 
 // ------------------------------------------------------------------ softmax warps
 template <bool kPair>
-__device__ __forceinline__ void query_warps(Bars* b, uint32_t tmem, const BwdArgs& a, int batch, int head, int len,
-                                            int q0, int n) {
+__device__ __forceinline__ void query_warps(const Maps& m, uint8_t* smem, Bars* b, uint32_t tmem, const BwdArgs& a,
+                                            const QueryRow& own, int batch, int head, int len, int q0, int n) {
     volatile int* abort = &b->abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = warp >> 2;
     const int row = q0 + (warp & 3) * 32 + lane;
     const bool live = row < len;
     const uint32_t t = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    own_row(t + kColDO + 32 * half, live ? a.go + offset(a.sgo, batch, head, row) + 64 * half : nullptr);
+    __syncwarp();
+    tc::tmem_st32(t + kColDO + 32 * half, own.go);
     tc::tmem_wait_st();
     publish(&b->own_tmem, lane);
-    const int64_t stat = ((int64_t)batch * a.H + head) * a.Spad + row;
-    const float nl = live ? a.nlse2[stat] : -NB200_INF, nd = live ? a.ndelta[stat] : 0.f;
-    const uint64_t nl2 = f2(nl, nl), nd2 = f2(nd, nd), sl2 = f2(a.sl2, a.sl2);
+    const uint64_t nl2 = f2(own.nl, own.nl), nd2 = f2(own.nd, own.nd), sl2 = f2(a.sl2, a.sl2);
     const int lim = (a.causal ? min(row, len - 1) : len - 1) - 64 * half;  // last key this row sees, from column 0 on
     const uint32_t tS = t + kColQueryS + 64 * half, tDS = t + kColDS + 32 * half;
     bool ok = true;
@@ -389,12 +419,14 @@ __device__ __forceinline__ void query_warps(Bars* b, uint32_t tmem, const BwdArg
     if (ok) ok = __all_sync(0xffffffffu, wait_bar(&b->done, 0, abort));
     if (!ok) return;
     tc::fence_after();
-    __nv_bfloat16* out = row < a.S ? a.dq + offset(a.sdq, batch, head, row) + 64 * half : nullptr;
-    write_row<64>(t + kColDQ + 64 * half, out, live, a.scale);
+    // Every streamed tile has been consumed: the ring's first tile stages dQ.
+    uint8_t* tile = smem + kOffQueryRing;
+    stage_half(t + kColDQ + 64 * half, tile, half, row - q0, live, a.scale);
+    store_rows(&m.dq, tile, half, half + 1, warp & 3, q0 + (warp & 3) * 32, a.S, head, batch, lane);
 }
 
 template <bool kPair>
-__device__ __forceinline__ void key_warps(uint8_t* smem, Bars* b, uint32_t tmem, const BwdArgs& a, int batch, int head,
+__device__ __forceinline__ void key_warps(const Maps& m, uint8_t* smem, Bars* b, uint32_t tmem, const BwdArgs& a, int batch, int head,
                                           int len, int k0, int first, int per_head, int skip, int n, int part) {
     volatile int* abort = &b->abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = warp >> 2;
@@ -469,9 +501,10 @@ __device__ __forceinline__ void key_warps(uint8_t* smem, Bars* b, uint32_t tmem,
         write_row_f32(t + (half ? kColDK : kColDV), live ? (half ? a.part_k : a.part_v) + at * kDim : nullptr);
         return;
     }
-    const nb200_attn_strides& so = half ? a.sdk : a.sdv;
-    __nv_bfloat16* out = row < a.S ? (half ? a.dk : a.dv) + offset(so, batch, head, row) : nullptr;
-    write_row<128>(t + (half ? kColDK : kColDV), out, live, half ? a.scale : 1.f);
+    uint8_t* tile = smem + kOffKeyRing + half * kTileBytes;
+    for (int h = 0; h < 2; ++h)
+        stage_half(t + (half ? kColDK : kColDV) + 64 * h, tile, h, row - k0, live, half ? a.scale : 1.f);
+    store_rows(half ? &m.dk : &m.dv, tile, 0, 2, warp & 3, k0 + (warp & 3) * 32, a.S, head, batch, lane);
 }
 
 // ------------------------------------------------------------------ producer (a whole warp; lane 0 issues)
@@ -482,62 +515,92 @@ __device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* m, in
 }
 
 // Streams n steps of two tiles from step `skip` on of steps first .. first + per_head - 1 of heads head0, head0 + 1,
-// ... Rows past
-// the sequence in a head's last step are zeroed before the tile is published (`tail` rows remain; 0: none
-// to zero): they enter sums over the streamed rows, where a coefficient of 0 times an infinity or NaN
+// ... Rows past the sequence in a head's last step are zeroed before the tile is published (`tail` rows remain;
+// 0: none to zero): they enter sums over the streamed rows, where a coefficient of 0 times an infinity or NaN
 // would still poison the result. A key CTA's steps come with their rows' statistics.
 template <bool kKeys>
-__device__ __forceinline__ void produce(const CUtensorMap* mx, const CUtensorMap* my, uint8_t* smem, Bars* b,
-                                        int batch, int head0, int first, int per_head, int skip, int n, int tail,
-                                        const BwdArgs& a, int lane) {
-    constexpr int kStages = kKeys ? kKeyStages : kQueryStages;
-    volatile int* abort = &b->abort;
-    Ring<kStages> r;
-    int it = 0, head = head0 + skip / per_head, step = first + skip % per_head;
+struct Producer {
+    static constexpr int kStages = kKeys ? kKeyStages : kQueryStages;
+    const CUtensorMap *mx, *my;
+    uint8_t* smem;
+    Bars* b;
+    int batch, first, per_head, tiles, tail;
+    const BwdArgs& a;
+    int head, step, it = 0;
     uint32_t tail_ph = 0;
     bool ok = true;
-    for (; it < 2 * n; ++it, r.next()) {
-        const int i = it >> 1;
-        const bool second = it & 1, cut = tail && step == first + per_head - 1;
-        ok = lane != 0 || wait_bar(&b->empty[r.s], r.ph ^ 1u, abort);
-        if (kKeys && ok && lane == 0 && !second) ok = wait_bar(&b->stat_empty[i & 1], ((i >> 1) & 1u) ^ 1u, abort);
-        if (!(ok = __all_sync(0xffffffffu, ok))) break;
-        uint8_t* dst = smem + (kKeys ? kOffKeyRing : kOffQueryRing) + r.s * kTileBytes;
-        if (lane == 0) {
-            uint64_t* bar = cut ? &b->tail : &b->full[r.s];
-            mbar_expect_tx(bar, kTileBytes);
-            load_tile(dst, second ? my : mx, step * kStep, head, batch, bar);
-            if (kKeys && !second) {
-                const int64_t at = ((int64_t)batch * a.H + head) * a.Spad + step * kStep;
-                uint8_t* to = smem + kOffStat + (i & 1) * 2 * kStatBytes;
-                mbar_expect_tx(&b->stat_full[i & 1], 2 * kStatBytes);
-                bulk_load(to, a.nlse2 + at, kStatBytes, &b->stat_full[i & 1]);
-                bulk_load(to + kStatBytes, a.ndelta + at, kStatBytes, &b->stat_full[i & 1]);
+    Ring<kStages> r;
+
+    __device__ __forceinline__ Producer(const CUtensorMap* mx_, const CUtensorMap* my_, uint8_t* smem_, Bars* b_, int batch_,
+                                        int head0, int first_, int per_head_, int skip, int n, int tail_,
+                                        const BwdArgs& a_)
+        : mx(mx_), my(my_), smem(smem_), b(b_), batch(batch_), first(first_), per_head(per_head_), tiles(2 * n),
+          tail(tail_), a(a_), head(head0 + skip / per_head_), step(first_ + skip % per_head_) {}
+
+    // Issues tiles up to number `end`; ahead of the CTA's first barrier (`early`) only those nothing waits for.
+    __device__ __forceinline__ void run(int end, bool early, int lane) {
+        volatile int* abort = &b->abort;
+        for (; ok && it < end; ++it, r.next()) {
+            const int i = it >> 1;
+            const bool second = it & 1, cut = tail && step == first + per_head - 1;
+            if (early && cut) return;
+            ok = lane != 0 || wait_bar(&b->empty[r.s], r.ph ^ 1u, abort);
+            if (kKeys && ok && lane == 0 && !second) ok = wait_bar(&b->stat_empty[i & 1], ((i >> 1) & 1u) ^ 1u, abort);
+            if (!(ok = __all_sync(0xffffffffu, ok))) return;
+            uint8_t* dst = smem + (kKeys ? kOffKeyRing : kOffQueryRing) + r.s * kTileBytes;
+            if (lane == 0) {
+                uint64_t* bar = cut ? &b->tail : &b->full[r.s];
+                mbar_expect_tx(bar, kTileBytes);
+                load_tile(dst, second ? my : mx, step * kStep, head, batch, bar);
+                if (kKeys && !second) {
+                    const int64_t at = ((int64_t)batch * a.H + head) * a.Spad + step * kStep;
+                    uint8_t* to = smem + kOffStat + (i & 1) * 2 * kStatBytes;
+                    mbar_expect_tx(&b->stat_full[i & 1], 2 * kStatBytes);
+                    bulk_load(to, a.nlse2 + at, kStatBytes, &b->stat_full[i & 1]);
+                    bulk_load(to + kStatBytes, a.ndelta + at, kStatBytes, &b->stat_full[i & 1]);
+                }
             }
-        }
-        if (cut) {
-            if (!(ok = __all_sync(0xffffffffu, wait_bar(&b->tail, tail_ph, abort)))) {
-                if (lane == 0) drain_bar(&b->tail, tail_ph);
-                break;
+            if (cut) {
+                if (!(ok = __all_sync(0xffffffffu, wait_bar(&b->tail, tail_ph, abort)))) {
+                    if (lane == 0) drain_bar(&b->tail, tail_ph);
+                    return;
+                }
+                tail_ph ^= 1u;
+                zero_tail(dst, kStep, tail, lane);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&b->full[r.s]);
             }
-            tail_ph ^= 1u;
-            zero_tail(dst, kStep, tail, lane);
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&b->full[r.s]);
-        }
-        if (second && ++step == first + per_head) {
-            step = first;
-            ++head;
+            if (second && ++step == first + per_head) {
+                step = first;
+                ++head;
+            }
         }
     }
     // Every copy lands before the CTA may exit.
-    if (lane == 0) {
+    __device__ __forceinline__ void drain(int lane) {
+        if (lane != 0) return;
         for (int s = 0; s < kStages && s < it; ++s) drain_bar(&b->full[s], ((it - 1 - s) / kStages) & 1u);
         const int steps = (it + 1) / 2;
         for (int s = 0; kKeys && s < 2 && s < steps; ++s) drain_bar(&b->stat_full[s], ((steps - 1 - s) / 2) & 1u);
         drain_bar(&b->own, 0);
     }
+};
+
+// A whole warp: one lane per barrier.
+__device__ __forceinline__ void init_barriers(Bars* b, bool aligned, int lane) {
+    if (lane < kBarriers)
+        mbar_init(reinterpret_cast<uint64_t*>(b) + lane, lane < kFourArrivals ? 1 : lane < kEightArrivals ? 4 : 8);
+    if (lane == 0) {
+        b->abort = !aligned;
+        if (!aligned) atomicOr(&g_attn_fault, 2u);
+    }
+    fence_barrier_init();
+    fence_proxy_async();
+    __syncwarp();
 }
+
+// One barrier for the whole CTA, met by its roles at different places.
+__device__ __forceinline__ void cta_sync() { asm volatile("bar.sync 0;" ::: "memory"); }
 
 __global__ void __launch_bounds__(kThreads, 1) attn_bwd_kernel(const __grid_constant__ Maps m, const BwdArgs a) {
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -547,41 +610,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_kernel(const __grid_cons
     // Head-major order in both parts, so that the CTAs that run side by side share their streamed tiles
     // through L2; under a causal mask the longest of a head come first.
     const bool keys = (int)blockIdx.x < a.key_ctas;
-    const int part = keys ? blockIdx.x % a.parts : 0;
-    const int id = keys ? blockIdx.x / a.parts : blockIdx.x - a.key_ctas;
-    const int blocks = a.blocks, heads = keys ? a.Hk : a.H;
-    const int batch = id / blocks / heads, head = id / blocks % heads;
-    const int row0 = (keys ? id % blocks : blocks - 1 - id % blocks) * kRows;
+    const unsigned part = keys ? blockIdx.x % (unsigned)a.parts : 0u;
+    const unsigned id = keys ? blockIdx.x / (unsigned)a.parts : blockIdx.x - a.key_ctas;
+    const unsigned bh = id / (unsigned)a.blocks, block = id - bh * a.blocks, heads = keys ? a.Hk : a.H;
+    const int batch = (int)(bh / heads), head = (int)(bh - batch * heads);
+    const int row0 = (int)(keys ? block : a.blocks - 1 - block) * kRows;
 
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < kQueryStages; ++s) {
-            mbar_init(&b->full[s], 1);
-            mbar_init(&b->empty[s], 1);
-        }
-        for (int s = 0; s < 2; ++s) {
-            mbar_init(&b->p_full[s], 4);
-            mbar_init(&b->ds_full[s], 4);
-            mbar_init(&b->stat_full[s], 1);
-            mbar_init(&b->stat_empty[s], 8);
-        }
-        mbar_init(&b->s_full, 1);
-        mbar_init(&b->dp_full, 1);
-        mbar_init(&b->read, 8);
-        mbar_init(&b->ds_free, 1);
-        mbar_init(&b->own, 1);
-        mbar_init(&b->own_tmem, 8);
-        mbar_init(&b->done, 1);
-        mbar_init(&b->tail, 1);
-        // The swizzled tiles need 1024-byte alignment; a base without it would compute nonsense.
-        b->abort = (smem_u32(smem) & 1023u) != 0;
-        if (b->abort) atomicOr(&g_attn_fault, 2u);
-        fence_barrier_init();
-        tc::prefetch_map(&m.q);
-        tc::prefetch_map(&m.k);
-        tc::prefetch_map(&m.v);
-        tc::prefetch_map(&m.go);
-    }
-    pdl_wait();
+    // Only the statistics come from the kernel before this one: everything else may be read while that one drains.
     const int len = tokens_of(a.lens, batch, a.S);
     if (row0 >= len) {  // none of the CTA's rows belongs to the sequence
         if (keys && a.parts > 1) return;
@@ -603,8 +638,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_kernel(const __grid_cons
     const int end = !keys && a.causal ? min(row0 + kRows, len) : len;
     const int per_head = (end + kStep - 1) / kStep - first;
     const int all = keys ? a.group * per_head : per_head;
-    const int skip = keys ? (int)((int64_t)all * part / a.parts) : 0;
-    const int n = keys ? (int)((int64_t)all * (part + 1) / a.parts) - skip : all;
+    const bool cut = keys && a.parts > 1;
+    const int skip = cut ? (int)((int64_t)all * part / a.parts) : 0;
+    const int n = cut ? (int)((int64_t)all * (part + 1) / a.parts) - skip : all;
     if (n == 0) {  // a part without steps: its sums are zero
         for (int i = threadIdx.x; i < min(kRows, len - row0) * (kDim / 4); i += kThreads) {
             const int64_t at = (part * a.part_rows + ((int64_t)batch * a.Hk + head) * a.S + row0) * kDim + 4 * i;
@@ -617,47 +653,70 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_kernel(const __grid_cons
     // Some row's sum has fewer than kRows terms: queries that see few keys, keys few queries see.
     const bool pair = a.causal ? (keys ? row0 + 2 * kRows > len : row0 == 0) : len < kRows;
 
-    if (warp == kMmaWarp) {
-        tc::tmem_alloc(&b->tmem_base, kTmemCols);
-        tc::tmem_relinquish();
-    }
-    tc::fence_before();
-    __syncthreads();
-    tc::fence_after();
-    const uint32_t tmem = b->tmem_base;
-    if (b->abort) {
-        // nothing was issued
-    } else if (warp < 8) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
-        if (keys && pair) key_warps<true>(smem, b, tmem, a, batch, head, len, row0, first, per_head, skip, n, part);
-        else if (keys) key_warps<false>(smem, b, tmem, a, batch, head, len, row0, first, per_head, skip, n, part);
-        else if (pair) query_warps<true>(b, tmem, a, batch, head, len, row0, n);
-        else query_warps<false>(b, tmem, a, batch, head, len, row0, n);
+    // The control warpgroup gives its registers up before any softmax warp asks for them.
+    if (warp >= kMmaWarp) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));
+
+    // The producer sets up the barriers and sends for the first tiles before the CTA's first barrier; the tiles'
+    // way to shared memory (1 to 2 us) then overlaps the allocation of the tensor memory.
+    auto produce = [&](auto& p) {
+        init_barriers(b, (smem_u32(smem) & 1023u) == 0, lane);  // the swizzled tiles need the alignment
+        if (lane == 0 && !b->abort) {
+            uint8_t* own = smem + kOffOwn;
+            mbar_expect_tx(&b->own, keys ? 2 * kTileBytes : kTileBytes);
+            load_tile(own, keys ? &m.k : &m.q, row0, head, batch, &b->own);
+            if (keys) load_tile(own + kTileBytes, &m.v, row0, head, batch, &b->own);
+        }
+        __syncwarp();
+        if (keys) pdl_wait();
+        if (!b->abort) p.run(2, true, lane);  // the first step
+        __syncwarp();
+        cta_sync();
+        if (!b->abort) {
+            p.run(p.tiles, false, lane);
+            p.drain(lane);
+        }
+    };
+    if (warp == kLoadWarp) {
+        if (keys) {
+            Producer<true> p(&m.q, &m.go, smem, b, batch, head * a.group, first, per_head, skip, n, tail, a);
+            produce(p);
+        } else {
+            Producer<false> p(&m.k, &m.v, smem, b, batch, head / a.group, 0, per_head, 0, n, tail, a);
+            produce(p);
+        }
+        __syncwarp();
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));
         if (warp == kMmaWarp) {
+            tc::tmem_alloc(&b->tmem_base, kTmemCols);
+            tc::tmem_relinquish();
+        }
+        QueryRow own;
+        if (warp < 8 && !keys) own.load(a, batch, head, len, row0);
+        tc::fence_before();
+        cta_sync();
+        tc::fence_after();
+        const uint32_t tmem = b->tmem_base;
+        if (b->abort) {
+            // nothing was issued
+        } else if (warp < 8) {
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+            if (keys && pair) key_warps<true>(m, smem, b, tmem, a, batch, head, len, row0, first, per_head, skip, n, part);
+            else if (keys) key_warps<false>(m, smem, b, tmem, a, batch, head, len, row0, first, per_head, skip, n, part);
+            else if (pair) query_warps<true>(m, smem, b, tmem, a, own, batch, head, len, row0, n);
+            else query_warps<false>(m, smem, b, tmem, a, own, batch, head, len, row0, n);
+        } else if (warp == kMmaWarp) {
             if (tc::elect_one()) {
                 if (keys) issue_key(smem, b, tmem, n, pair);
                 else issue_query(smem, b, tmem, n, pair);
             }
-        } else if (warp == kLoadWarp) {
-            if (lane == 0) {
-                uint8_t* own = smem + kOffOwn;
-                mbar_expect_tx(&b->own, keys ? 2 * kTileBytes : kTileBytes);
-                load_tile(own, keys ? &m.k : &m.q, row0, head, batch, &b->own);
-                if (keys) load_tile(own + kTileBytes, &m.v, row0, head, batch, &b->own);
-            }
             __syncwarp();
-            if (keys) produce<true>(&m.q, &m.go, smem, b, batch, head * a.group, first, per_head, skip, n, tail, a, lane);
-            else produce<false>(&m.k, &m.v, smem, b, batch, head / a.group, 0, per_head, 0, n, tail, a, lane);
         }
-        __syncwarp();
     }
     tc::fence_before();
-    __syncthreads();
+    cta_sync();
     if (warp == kMmaWarp) {
         tc::fence_after();
-        tc::tmem_dealloc(tmem, kTmemCols);
+        tc::tmem_dealloc(b->tmem_base, kTmemCols);
     }
 }
 
@@ -687,15 +746,17 @@ SharedLimit g_shared;
 
 int64_t padded(int64_t seq) { return (seq + kStep - 1) / kStep * kStep; }
 
-// CTAs a key block is cut into. A step of a key CTA takes about 3 units of time, one of a query CTA 2; the longest
-// key CTA should not take much longer than an SM's share of all steps, nor a part run fewer than 4 steps.
-// bf16 [4, 16 heads on 4, 1000, 128] causal: 68 us with one part, PARTS_US with four.
+// CTAs a key block is cut into, so that the longest runs about as long as an SM's share of all the work (within a
+// quarter of it), and no fewer than 4 steps. Units of 0.57 us: a step of a key CTA takes 3, one of a query CTA 2, and every CTA about
+// 9 or 8 besides (set-up, the way of the first tiles, the epilogue). bf16 causal [1, 32 heads on 1, 4096, 128]
+// 1.59 ms uncut, 0.41 ms with 4 parts; [1, 8 on 1, 2048, 128] 207 and 62 us (76 us with
+// 21 parts); not causal [1, 8 on 1, 8192, 128] 865 and 691 us (2 parts).
 int parts_of(const nb200_attn_args& n) {
     const int64_t blocks = (n.seq + kRows - 1) / kRows, group = n.heads / n.kv_heads;
-    const int64_t pairs = n.causal ? blocks * (blocks + 1) / 2 : blocks * blocks;  // (key block, query step)
-    const int64_t share = 5 * n.batch * n.heads * pairs / sm_count(), longest = 3 * group * blocks;
-    const int64_t most = group * blocks / 4;
-    return (int)std::max<int64_t>(1, std::min(most, longest / std::max<int64_t>(share, 1)));
+    const int64_t pairs = n.causal ? blocks * (blocks + 1) / 2 : blocks * blocks;  // (block, step) of one head
+    const int64_t work = n.batch * (n.heads * (5 * pairs + 8 * blocks) + 9 * n.kv_heads * blocks);
+    const int64_t share = std::max<int64_t>(work / sm_count(), 1), longest = 3 * group * blocks;
+    return (int)std::max<int64_t>(1, std::min(group * blocks / 4, (4 * longest + 5 * share - 1) / (5 * share)));
 }
 
 }  // namespace
@@ -727,6 +788,9 @@ int launch_attention_bwd(const nb200_attn_args& n, const nb200_attn_strides* str
         (rc = encode_rows(&m.k, what, "k", k, n.batch, n.kv_heads, n.seq, strides[1], kStep)) ||
         (rc = encode_rows(&m.v, what, "v", v, n.batch, n.kv_heads, n.seq, strides[2], kStep)) ||
         (rc = encode_rows(&m.go, what, "grad_o", grad_o, n.batch, n.heads, n.seq, strides[4], kStep)) ||
+        (rc = encode_rows(&m.dq, what, "dq", dq, n.batch, n.heads, n.seq, strides[5], 32)) ||
+        (rc = encode_rows(&m.dk, what, "dk", dk, n.batch, n.kv_heads, n.seq, strides[6], 32)) ||
+        (rc = encode_rows(&m.dv, what, "dv", dv, n.batch, n.kv_heads, n.seq, strides[7], 32)) ||
         (rc = g_shared.raise(what, attn_bwd_kernel, kSmemBytes)))
         return rc;
     StatArgs s;
