@@ -29,7 +29,8 @@ constexpr int kMaxWidth = 16384;
 constexpr int kWarpRows = 8;  // rows a CTA of the warp-per-row form holds
 
 struct Norm {
-    int64_t rows, width, sx, sr, sg, sdy, sdh, group;
+    int64_t rows, width, sx, sr, sg, sdy, sdh;
+    uint32_t group;  // rows that share a gate row
     float scale, eps, inv_n;
     int act;
 };
@@ -59,20 +60,28 @@ struct Vecs {
 // thread, computed as packed fp32 pairs. A unit (warp or CTA) works through consecutive rows, so that the
 // weights stay in registers and a gate row is read and put through its activation once per group.
 //
-// Element i of thread t is column (t + (i / V) G) V + i % V. Rows of 16-bit elements that do not start on a
-// 16-byte boundary (ALIGNED false: odd widths, slices) move in 16-byte vectors as well. All threads of a row are off by the same number of bytes: a load takes the two aligned vectors it
-// straddles (never one without a byte of the row) and shifts; a store passes its last elements to the next
-// lane, which writes the aligned vector they begin, and the few elements at the ends of a warp's span go one
-// by one (bf16 [16384, 3001] 431 us backward; 795 us element by element). Such rows of fp32 go element by
-// element, column t + i G, which was the faster there ([3003, 1001] 36 us, 54 us by vectors).
-template <typename T, int NV, bool ALIGNED, bool CTA>
+// Element i of thread t is column (t + (i / V) G) V + i % V, less `lead` columns where rows do not start on a
+// 16-byte boundary. Three forms:
+//  ALIGNED  every row of every tensor starts on a 16-byte boundary and is whole vectors.
+//  LINED    widths off the vector size, tensors laid out alike (contiguous ones are): all tensors' rows are off the
+//           boundary by the same amount, which repeats every `step` rows (8 at most). A unit takes rows of one
+//           residue, so that its vectors are aligned in every row, its columns stay the same, and only the
+//           first and the last vector of a row are partial.
+//  ANY      anything else (slices): 16-bit rows move in vectors that each thread shifts (the two aligned
+//           vectors it straddles, never one without a byte of the row; a store passes its last elements
+//           to the next lane, which writes the aligned vector they begin, and the few elements at the ends of a
+//           warp's span go one by one), fp32 rows go element by element, column t + i G.
+// bf16 [16384, 3001], backward: 193 us lined up, 427 us by shifted vectors, 795 us element by element.
+enum Form { ALIGNED, LINED, ANY };
+
+template <typename T, int NV, Form FORM, bool CTA>
 struct Rows {
     using CH = Vecs<T, NV>;
     static constexpr int V = CH::V, P = CH::P;  // P pairs a thread
-    static constexpr bool SCALAR = !ALIGNED && sizeof(T) == 4;
+    static constexpr bool SCALAR = FORM == ANY && sizeof(T) == 4;
     int t, G;
     int64_t unit;
-    int width;
+    int width, lead = 0;
     float* buf;  // 2 x 4 x 32 entries of shared memory when CTA
     int phase = 0;
 
@@ -81,15 +90,25 @@ struct Rows {
         G = blockDim.x;
         unit = CTA ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
     }
-    __device__ __forceinline__ int col(int k) const { return (t + k * G) * V; }  // of vector k
+    // Columns ahead of the first whole vector: `row` is any row this unit works on.
+    __device__ __forceinline__ void line_up(const T* row) {
+        if (FORM == LINED) lead = (int)((reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(T));
+    }
+    __device__ __forceinline__ int col(int k) const { return (t + k * G) * V - (FORM == LINED ? lead : 0); }  // of vector k
     __device__ __forceinline__ int col_of(int i) const { return SCALAR ? t + i * G : col(i / V) + i % V; }
+    __device__ __forceinline__ bool holds(int c) const { return c < width && (FORM != LINED || c >= 0); }
     __device__ __forceinline__ static uint4 fetch(const void* p, bool stream) { return stream ? ld_stream(p) : ld_keep(p); }
+    // A row of one of the tensors the form speaks of; `finish` before use. (Clearing the partial vectors here would
+    // make their warps wait for a prefetched row as soon as it is sent for.)
     __device__ __forceinline__ void load(CH& c, const T* row, bool stream) const {
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const int at = col(k);
-            if constexpr (ALIGNED) {
+            if constexpr (FORM == ALIGNED) {
                 if (at < width) c.raw[k] = fetch(row + at, stream);
+                else c.raw[k] = make_uint4(0u, 0u, 0u, 0u);
+            } else if constexpr (FORM == LINED) {
+                if (at < width && at + V > 0) c.raw[k] = fetch(row + at, stream);
                 else c.raw[k] = make_uint4(0u, 0u, 0u, 0u);
             } else if constexpr (SCALAR) {
                 uint32_t w[4];
@@ -108,7 +127,30 @@ struct Rows {
                 uint4 lo = fetch(p, stream), hi = make_uint4(0u, 0u, 0u, 0u);
                 if (off && p + 16 < reinterpret_cast<const char*>(row + width)) hi = fetch(p + 16, stream);
                 c.raw[k] = shift_down(lo, hi, off);
-                if (at + V > width) keep_first(c.raw[k], width - at);
+                if (at + V > width) keep_range(c.raw[k], 0, width - at);
+            }
+        }
+    }
+    __device__ __forceinline__ void finish(CH& c) const {
+        if constexpr (FORM == LINED) {
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                const int at = col(k);
+                if (at < 0 || at + V > width) keep_range(c.raw[k], -at, width - at);
+            }
+        }
+    }
+    // A weight or a shared gate row, which need not be laid out like the rows.
+    __device__ __forceinline__ void load_shared(CH& c, const T* row) const {
+        if constexpr (FORM != LINED) {
+            load(c, row, false);
+        } else {
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                float f[V];
+#pragma unroll
+                for (int j = 0; j < V; ++j) f[j] = holds(col(k) + j) ? Elem<T>::to_f(row[col(k) + j]) : 0.f;
+                c.raw[k] = Elem<T>::pack(f);
             }
         }
     }
@@ -126,14 +168,21 @@ struct Rows {
         return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits),
                           __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
     }
-    __device__ __forceinline__ static void keep_first(uint4& u, int n) {
+    // Zeroes every element outside [from, to).
+    __device__ __forceinline__ static void keep_range(uint4& u, int from, int to) {
         uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (2 * i >= n) w[i] = 0u;
-            else if (2 * i + 1 >= n) w[i] &= 0xffffu;
+        for (int j = 0; j < V; ++j) {
+            if (j >= from && j < to) continue;
+            if constexpr (V == 4) w[j] = 0u;
+            else w[j / 2] &= j & 1 ? 0xffffu : 0xffff0000u;
         }
         u = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    __device__ __forceinline__ static void put(T* row, int c, const uint4& u, int j) {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+        if constexpr (V == 4) reinterpret_cast<uint32_t*>(row)[c] = w[j];
+        else reinterpret_cast<uint16_t*>(row)[c] = (uint16_t)(w[j / 2] >> (16 * (j & 1)));
     }
     __device__ __forceinline__ void store(T* row, const uint64_t* v) const {
 #pragma unroll
@@ -145,12 +194,21 @@ struct Rows {
                 f[2 * j + 1] = f2hi(v[k * V / 2 + j]);
             }
             const int at = col(k);
-            if constexpr (ALIGNED) {
+            if constexpr (FORM == ALIGNED) {
                 if (at < width) st_stream(row + at, Elem<T>::pack(f));
             } else if constexpr (SCALAR) {
 #pragma unroll
                 for (int j = 0; j < V; ++j)
                     if (col_of(k * V + j) < width) row[col_of(k * V + j)] = f[j];
+            } else if constexpr (FORM == LINED) {
+                const uint4 u = Elem<T>::pack(f);
+                if (at >= 0 && at + V <= width) {
+                    st_stream(row + at, u);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < V; ++j)
+                        if (holds(at + j)) put(row, at + j, u, j);
+                }
             } else {
                 store_shifted(row, at, Elem<T>::pack(f));
             }
@@ -168,22 +226,16 @@ struct Rows {
         below.y = __shfl_up_sync(0xffffffffu, u.y, 1);
         below.z = __shfl_up_sync(0xffffffffu, u.z, 1);
         below.w = __shfl_up_sync(0xffffffffu, u.w, 1);
-        if ((lane > 0 || pass == 0) && valid >= own)
-            st_stream(reinterpret_cast<void*>(a - off), pass ? shift_down(below, u, 16u - off) : u);
+        const bool whole = (lane > 0 || pass == 0) && valid >= own;
+        if (whole) st_stream(reinterpret_cast<void*>(a - off), pass ? shift_down(below, u, 16u - off) : u);
         // Elements no whole vector takes: the head of a warp's first lane, the tail of its last, the row's end.
-        uint32_t single = 0;
-        if (lane == 0 ? pass != 0 : valid < own) single |= (1u << own) - 1u;
+        uint32_t single = whole ? 0u : (1u << own) - 1u;
         if (pass && (lane == 31 || above < own)) single |= ((1u << V) - 1u) & ~((1u << own) - 1u);
-        if (pass == 0 && valid == V) single = 0;
-        if (pass == 0 && valid < V) single = (1u << V) - 1u;
         single &= (1u << valid) - 1u;
         if (__any_sync(0xffffffffu, single)) {
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                if (!(single >> j & 1u)) continue;
-                reinterpret_cast<uint16_t*>(row)[at + j] = (uint16_t)(w[j / 2] >> (16 * (j & 1)));
-            }
+            for (int j = 0; j < V; ++j)
+                if (single >> j & 1u) put(row, at + j, u, j);
         }
     }
     // The sum of v over the row's threads, in every thread: warp shuffles, then the warps' sums (one
@@ -225,43 +277,92 @@ struct Rows {
     }
 };
 
-// Position of a unit in its rows: the rows left of the current gate group.
-struct GatePos {
-    int64_t index, left;
-    __device__ __forceinline__ GatePos(int64_t row, int64_t group) : index(row / group) {
-        left = group - (row - index * group);
-    }
-    // Moves to the next row; true when that row starts another group.
-    __device__ __forceinline__ bool next(int64_t group) {
-        if (--left) return false;
-        left = group;
-        ++index;
-        return true;
+// Threads of a row and elements of a thread: a warp of 8 holds up to 256 elements, a CTA of at most 512 threads up
+// to 4096 (8 a thread) or 8192 (16), a CTA of 1024 the rest.
+struct Shape {
+    bool cta;
+    Form form;
+    int e, threads;
+};
+
+Shape make_shape(int64_t width, Form form) {
+    Shape s;
+    s.form = form;
+    const int64_t span = form == LINED ? width + 7 : width;  // columns ahead of the first vector
+    s.cta = span > 256;
+    s.e = span <= 4096 ? 8 : 16;
+    s.threads = s.cta ? (int)((span + 32 * s.e - 1) / (32 * s.e)) * 32 : 32;
+    return s;
+}
+
+// How the rows are cut into units' shares. Rows are planned in groups of `group` (all rows, unless whole gate groups
+// have to stay together), per_group units each; `step` units take turns at consecutive rows.
+struct Chunks {
+    int64_t group, per_group, rows, step, count;
+    __device__ __forceinline__ void range(int64_t i, const Norm& n, uint32_t& r0, uint32_t& r1) const {
+        const int64_t g = i / per_group, u = i - g * per_group, base = g * group;
+        const int64_t from = base + u / step * (rows * step), to = from + rows * step;
+        r0 = (uint32_t)(from + u % step);
+        r1 = (uint32_t)min(min(to, base + group), n.rows);
     }
 };
 
-template <typename T, int NV, bool ALIGNED, bool CTA, int kThreads>
-__global__ void __launch_bounds__(kThreads, (CTA || ALIGNED) && NV * Elem<T>::V == 8 ? 1024 / kThreads : 1)
-    norm_fwd_kernel(const T* x, const T* res, const T* gate, const T* w1, const T* w2, Norm n, int64_t per_unit, T* y,
-                    T* h, float* rstd) {
-    using R = Rows<T, NV, ALIGNED, CTA>;
+Chunks make_chunks(const Norm& n, int64_t group, int64_t target, int64_t step) {
+    Chunks c;
+    c.step = step;
+    const int64_t groups = n.rows / group;
+    if (groups < target || step > 1) {  // parts of a group, at most `target` in all unless that is less than `step` each
+        const int64_t turns = std::min((group + step - 1) / step, std::max<int64_t>(1, target / groups / step));
+        c.group = group;
+        c.rows = (group + turns * step - 1) / (turns * step);
+        c.per_group = (group + c.rows * step - 1) / (c.rows * step) * step;
+        c.count = groups * c.per_group;
+    } else {  // whole groups
+        c.group = c.rows = (groups + target - 1) / target * group;
+        c.per_group = 1;
+        c.count = (n.rows + c.rows - 1) / c.rows;
+    }
+    return c;
+}
+
+// A gate row: laid out like the rows when every row has its own.
+template <typename R, typename T>
+__device__ __forceinline__ void load_gate(const R& r, typename R::CH& c, const T* gate, const Norm& n, uint32_t index) {
+    if (n.group == 1) {
+        r.load(c, gate + index * n.sg, false);
+        r.finish(c);
+    } else {
+        r.load_shared(c, gate + index * n.sg);
+    }
+}
+
+template <typename T, int NV, Form FORM, bool CTA, int kThreads>
+__global__ void __launch_bounds__(kThreads, (CTA || FORM == ALIGNED) && NV * Elem<T>::V == 8 ? 1024 / kThreads : 1)
+    norm_fwd_kernel(const T* x, const T* res, const T* gate, const T* w1, const T* w2, Norm n, Chunks ch, T* y, T* h,
+                    float* rstd) {
+    using R = Rows<T, NV, FORM, CTA>;
     using CH = typename R::CH;
     constexpr int P = R::P;
     __shared__ float buf[CTA ? 256 : 1];
     R r(n.width, buf);
-    int64_t row = r.unit * per_unit;
-    const int64_t end = min(row + per_unit, n.rows);
+    if (r.unit >= ch.count) return;
+    uint32_t row, end;
+    ch.range(r.unit, n, row, end);
     if (row >= end) return;
+    r.line_up(x + row * n.sx);
     CH c1, c2, cx, cr, cg;
-    if (w1) r.load(c1, w1, false);
-    if (w2) r.load(c2, w2, false);
+    if (w1) r.load_shared(c1, w1);
+    if (w2) r.load_shared(c2, w2);
     r.load(cx, x + row * n.sx, true);
     r.load(cr, res + row * n.sr, true);
-    GatePos g(row, n.group);
-    if (gate) r.load(cg, gate + g.index * n.sg, false);
+    uint32_t index = 0;
+    if (gate) {
+        index = row / n.group;
+        load_gate(r, cg, gate, n, index);
+    }
     bool fresh = true;
     uint64_t b[P];  // scale * a(gate) * post weight
-    for (; row < end; ++row) {
+    for (; row < end; row += ch.step) {
         if (fresh) {
 #pragma unroll
             for (int i = 0; i < P; ++i) {
@@ -271,14 +372,18 @@ __global__ void __launch_bounds__(kThreads, (CTA || ALIGNED) && NV * Elem<T>::V 
                 b[i] = w1 ? mul2(a, c1.pair(i)) : a;
             }
         }
+        r.finish(cx);
+        r.finish(cr);
         // The next row is on its way while this one is reduced.
         CH nx, nr;
         fresh = false;
-        if (row + 1 < end) {
-            r.load(nx, x + (row + 1) * n.sx, true);
-            r.load(nr, res + (row + 1) * n.sr, true);
-            if (gate && g.next(n.group)) {
-                r.load(cg, gate + g.index * n.sg, false);
+        const uint32_t next = row + ch.step;
+        if (next < end) {
+            r.load(nx, x + next * n.sx, true);
+            r.load(nr, res + next * n.sr, true);
+            if (gate && next / n.group != index) {
+                index = next / n.group;
+                load_gate(r, cg, gate, n, index);
                 fresh = true;
             }
         }
@@ -298,67 +403,19 @@ __global__ void __launch_bounds__(kThreads, (CTA || ALIGNED) && NV * Elem<T>::V 
             v[i] = fma2(b[i], mul2(cx.pair(i), f2(r1, r1)), cr.pair(i));
             acc = fma2(v[i], v[i], acc);
         }
-        r.store(y + row * n.width, v);
+        r.store(y + (int64_t)row * n.width, v);
         if (w2) {
             float s = f2lo(acc) + f2hi(acc);
             s = r.sum(s);
             r2 = rsqrtf(s * n.inv_n + n.eps);
 #pragma unroll
             for (int i = 0; i < P; ++i) v[i] = mul2(v[i], mul2(c2.pair(i), f2(r2, r2)));
-            r.store(h + row * n.width, v);
+            r.store(h + (int64_t)row * n.width, v);
         }
-        if (r.t == 0) *reinterpret_cast<float2*>(rstd + 2 * row) = make_float2(r1, r2);
+        if (r.t == 0) *reinterpret_cast<float2*>(rstd + 2 * (int64_t)row) = make_float2(r1, r2);
         cx = nx;
         cr = nr;
     }
-}
-
-// Threads of a row and elements of a thread: a warp of 8 holds up to 256 elements, a CTA of at most 512 threads up
-// to 4096 (8 a thread) or 8192 (16), a CTA of 1024 the rest.
-struct Shape {
-    bool cta, aligned;
-    int e, threads;
-};
-
-Shape make_shape(int64_t width) {
-    Shape s;
-    s.aligned = false;
-    s.cta = width > 256;
-    s.e = width <= 4096 ? 8 : 16;
-    s.threads = s.cta ? (int)((width + 32 * s.e - 1) / (32 * s.e)) * 32 : 32;
-    return s;
-}
-
-// How the backward pass cuts the rows: `per_group` chunks of each gate group, or (per_group 1) chunks
-// of whole groups.
-struct Chunks {
-    int64_t rows, per_group, count;
-    __device__ __forceinline__ void range(int64_t i, const Norm& n, int64_t& r0, int64_t& r1) const {
-        const int64_t base = i / per_group * (per_group > 1 ? n.group : rows);
-        const int64_t end = per_group > 1 ? base + n.group : n.rows;
-        r0 = base + i % per_group * rows;
-        r1 = r0 + rows < end ? r0 + rows : end;
-    }
-};
-
-Chunks make_chunks(const Norm& n) {
-    // 512 threads on every SM, about what fits one at a time, and one chunk for each unit of them: more chunks
-    // mean more partial sums to write and add (bf16 [32768, 1024] 95 us, with twice as many 103).
-    const Shape s = make_shape(n.width);
-    const int64_t target = (int64_t)sm_count() * (s.cta ? std::max(1, 512 / s.threads) : 2 * kWarpRows);
-    const int64_t groups = n.rows / n.group;
-    Chunks c;
-    if (groups < target) {  // a part of a group each, at most `target` in all
-        c.per_group = std::min(n.group, std::max<int64_t>(1, target / groups));
-        c.rows = (n.group + c.per_group - 1) / c.per_group;
-        c.per_group = (n.group + c.rows - 1) / c.rows;
-        c.count = groups * c.per_group;
-    } else {
-        c.per_group = 1;
-        c.rows = (groups + target - 1) / target * n.group;
-        c.count = (n.rows + c.rows - 1) / c.rows;
-    }
-    return c;
 }
 
 // One fp32 row of a chunk's column sums.
@@ -367,7 +424,7 @@ __device__ __forceinline__ void store_part(float* part, const uint64_t* acc, con
 #pragma unroll
     for (int i = 0; i < 2 * R::P; ++i) {
         const int c = r.col_of(i);
-        if (c < r.width) part[c] = i & 1 ? f2hi(acc[i / 2]) : f2lo(acc[i / 2]);
+        if (r.holds(c)) part[c] = i & 1 ? f2hi(acc[i / 2]) : f2lo(acc[i / 2]);
     }
 }
 
@@ -380,12 +437,12 @@ __device__ __forceinline__ void store_part(float* part, const uint64_t* acc, con
 // thread). That takes one CTA of 512 threads per SM; two at 64 registers a thread, with or without a ring of
 // bulk copies in shared memory in place of the registers, spilled and ran slower (bf16 [16384, 4096]: 250
 // and 294 us).
-template <typename T, int NV, bool ALIGNED, bool CTA, int kThreads>
+template <typename T, int NV, Form FORM, bool CTA, int kThreads>
 __global__ void __launch_bounds__(kThreads)
     norm_bwd_kernel(const T* dy, const T* dh, const T* x, const T* res, const T* gate, const T* w1, const T* w2,
                     const float* rstd, Norm n, Chunks ch, T* dx, T* dres, T* dgate, float* part1, float* part2,
                     float* partg) {
-    using R = Rows<T, NV, ALIGNED, CTA>;
+    using R = Rows<T, NV, FORM, CTA>;
     using CH = typename R::CH;
     constexpr int P = R::P;
     constexpr bool AHEAD = P == 4;
@@ -401,36 +458,43 @@ __global__ void __launch_bounds__(kThreads)
     uint64_t* a1 = as + slots;
     pdl_trigger();
     if (r.unit >= ch.count) return;
-    int64_t row, end;
+    uint32_t row, end;
     ch.range(r.unit, n, row, end);
+    r.line_up(x + row * n.sx);
     CH c2;
-    if (w2) r.load(c2, w2, false);
+    if (w2) r.load_shared(c2, w2);
     uint64_t G[P], a2[P];
 #pragma unroll
     for (int i = 0; i < P; ++i) {
         G[i] = a2[i] = 0;
         a1[i * r.G] = 0;
     }
-    GatePos g(row, n.group);
+    uint32_t index = gate ? row / n.group : 0u;
     bool fresh = true;
     CH nx, nr, ndy, ndh;
     float2 nrs;
-    auto fetch = [&](int64_t i) {
-        nrs = *reinterpret_cast<const float2*>(rstd + 2 * i);
+    auto fetch = [&](uint32_t i) {
+        nrs = *reinterpret_cast<const float2*>(rstd + 2 * (int64_t)i);
         r.load(nx, x + i * n.sx, true);
         r.load(nr, res + i * n.sr, true);
         if (dy) r.load(ndy, dy + i * n.sdy, true);
         if (dh) r.load(ndh, dh + i * n.sdh, true);
     };
-    if (AHEAD) fetch(row);
-    for (; row < end; ++row) {
+    if (AHEAD && row < end) fetch(row);
+    for (; row < end; row += ch.step) {
+        const uint32_t next = row + ch.step, next_index = gate ? next / n.group : 0u;
+        const bool last = next >= end;
         if (!AHEAD) fetch(row);
-        const CH cx = nx, cr = nr, cdy = ndy, cdh = ndh;
+        CH cx = nx, cr = nr, cdy = ndy, cdh = ndh;
+        r.finish(cx);
+        r.finish(cr);
+        if (dy) r.finish(cdy);
+        if (dh) r.finish(cdh);
         const float2 rs = nrs;
         if (fresh) {
             CH c1, cg;
-            if (w1) r.load(c1, w1, false);
-            if (gate) r.load(cg, gate + g.index * n.sg, false);
+            if (w1) r.load_shared(c1, w1);
+            if (gate) load_gate(r, cg, gate, n, index);
 #pragma unroll
             for (int i = 0; i < P; ++i) {
                 const uint64_t v = gate ? f2(gate_value(cg.get(2 * i), n.act), gate_value(cg.get(2 * i + 1), n.act))
@@ -456,12 +520,12 @@ __global__ void __launch_bounds__(kThreads)
             if (dh) a2[i] = fma2(cdh.pair(i), yhat[i], a2[i]);
         }
         // Issued here, the loads cover the sums' latency.
-        if (AHEAD && row + 1 < end) fetch(row + 1);
-        if (gate && g.left == 1 && row + 1 < end && (r.t & 7) == 0)
+        if (AHEAD && !last) fetch(next);
+        if (gate && next_index != index && !last && (r.t & 7) == 0)
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
-                if (r.col(k) < r.width)
-                    asm volatile("prefetch.global.L2 [%0];" ::"l"(gate + (g.index + 1) * n.sg + r.col(k)));
+                if (r.holds(r.col(k)))
+                    asm volatile("prefetch.global.L2 [%0];" ::"l"(gate + next_index * n.sg + r.col(k)));
             }
         float t1 = f2lo(s1) + f2hi(s1), t2 = f2lo(s2) + f2hi(s2), t3 = f2lo(s3) + f2hi(s3);
         r.sum3(t1, t2, t3);
@@ -474,15 +538,13 @@ __global__ void __launch_bounds__(kThreads)
             G[i] = fma2(xhat, e[i], G[i]);
             yhat[i] = mul2(fma2(xhat, k1p, mul2(bs[i * r.G], e[i])), r1p);  // dx
         }
-        r.store(dres + row * n.width, e);
-        r.store(dx + row * n.width, yhat);
+        r.store(dres + (int64_t)row * n.width, e);
+        r.store(dx + (int64_t)row * n.width, yhat);
         // The end of a gate group, or of the chunk.
-        fresh = gate && g.next(n.group);
-        if (fresh || row + 1 == end) {
-            const bool direct = gate && !partg;
-            const int64_t ended = g.index - (fresh ? 1 : 0);
+        fresh = gate && next_index != index;
+        if (fresh || last) {
             CH c1;
-            if (w1) r.load(c1, w1, false);
+            if (w1) r.load_shared(c1, w1);
 #pragma unroll
             for (int i = 0; i < P; ++i) {
                 const uint64_t a = as[i * r.G], g1 = mul2(G[i], f2(n.scale, n.scale));
@@ -490,8 +552,9 @@ __global__ void __launch_bounds__(kThreads)
                 G[i] = mul2(g1, f2(gate_slope(f2lo(a), n.act), gate_slope(f2hi(a), n.act)));
                 if (w1) G[i] = mul2(G[i], c1.pair(i));
             }
-            if (direct) r.store(dgate + ended * n.width, G);
-            if (row + 1 == end) break;
+            if (dgate && !partg) r.store(dgate + index * n.width, G);
+            index = next_index;
+            if (last) break;
 #pragma unroll
             for (int i = 0; i < P; ++i) G[i] = 0;
         }
@@ -536,12 +599,13 @@ __global__ void __launch_bounds__(kSumCols* kSumRows) norm_sum_kernel(Sums<T> a)
     a.out[which][group * a.width + c] = Elem<T>::from_f(s);
 }
 
-// f(CTA, E, ALIGNED, most threads) with the shape's compile-time values.
+// f(CTA, E, FORM, most threads) with the shape's compile-time values.
 template <typename F>
 void dispatch(const Shape& s, F&& f) {
     auto pick = [&](auto cta, auto e, auto most) {
-        if (s.aligned) f(cta, e, std::true_type{}, most);
-        else f(cta, e, std::false_type{}, most);
+        if (s.form == ALIGNED) f(cta, e, std::integral_constant<Form, ALIGNED>{}, most);
+        else if (s.form == LINED) f(cta, e, std::integral_constant<Form, LINED>{}, most);
+        else f(cta, e, std::integral_constant<Form, ANY>{}, most);
     };
     using E8 = std::integral_constant<int, 8>;
     using E16 = std::integral_constant<int, 16>;
@@ -551,7 +615,27 @@ void dispatch(const Shape& s, F&& f) {
     else pick(std::true_type{}, E16{}, std::integral_constant<int, 1024>{});
 }
 
-bool rows_aligned(const void* p, int64_t stride, int esize) { return !p || (aligned16(p) && stride * esize % 16 == 0); }
+// What the rows of several tensors have in common: where they start within 16 bytes.
+struct Layout {
+    bool aligned = true, alike = true, any = false;
+    uintptr_t base = 0;
+    int64_t pitch = 0;
+    void add(const void* p, int64_t stride, int esize) {
+        if (!p) return;
+        const uintptr_t at = reinterpret_cast<uintptr_t>(p) & 15u;
+        const int64_t bytes = stride * esize & 15;
+        aligned = aligned && at == 0 && bytes == 0;
+        if (any) alike = alike && at == base && bytes == pitch;
+        any = true;
+        base = at;
+        pitch = bytes;
+    }
+    int64_t step() const {  // rows until the offset repeats
+        int64_t n = 1;
+        while (n * pitch & 15) n *= 2;
+        return n;
+    }
+};
 
 int check_width(const char* what, int64_t width) {
     if (width <= kMaxWidth) return NB200_OK;
@@ -568,7 +652,7 @@ Norm make_norm(const nb200_norm_args& a) {
     n.sg = a.stride_gate;
     n.sdy = a.stride_grad_y;
     n.sdh = a.stride_grad_h;
-    n.group = a.gate ? a.rows_per_gate : 1;
+    n.group = a.gate ? (uint32_t)a.rows_per_gate : 1u;
     n.scale = (float)a.scale;
     n.eps = (float)a.eps;
     n.inv_n = 1.f / (float)a.width;
@@ -576,28 +660,56 @@ Norm make_norm(const nb200_norm_args& a) {
     return n;
 }
 
+// The form of a call whose row tensors have layout `l`, all tensors together `all`. Lined-up rows may need one
+// vector more than a CTA holds.
+Form pick_form(const Norm& n, const Layout& l, const Layout& all, int esize) {
+    if (all.aligned && n.width * esize % 16 == 0) return ALIGNED;
+    return l.alike && make_shape(n.width, LINED).threads <= 1024 ? LINED : ANY;
+}
+
 template <typename T>
 int norm_fwd(const nb200_norm_args& a, T* y, T* h, float* rstd, cudaStream_t st) {
     const Norm n = make_norm(a);
     constexpr int es = sizeof(T);
-    const bool al = rows_aligned(a.x, n.sx, es) && rows_aligned(a.residual, n.sr, es) &&
-                    rows_aligned(a.gate, n.sg, es) && rows_aligned(a.post_weight, 0, es) &&
-                    rows_aligned(a.pre_weight, 0, es) && aligned16(y) && (!h || aligned16(h));
-    Shape s = make_shape(n.width);
-    s.aligned = al && n.width * es % 16 == 0;
+    Layout l;
+    l.add(a.x, n.sx, es);
+    l.add(a.residual, n.sr, es);
+    l.add(y, n.width, es);
+    l.add(h, n.width, es);
+    if (n.group == 1) l.add(a.gate, n.sg, es);
+    Layout all = l;  // the shared rows count for ALIGNED
+    if (n.group > 1) all.add(a.gate, n.sg, es);
+    all.add(a.post_weight, 0, es);
+    all.add(a.pre_weight, 0, es);
+    const Shape s = make_shape(n.width, pick_form(n, l, all, es));
     const int per = s.cta ? 1 : kWarpRows;
-    dispatch(s, [&](auto cta, auto e, auto aligned, auto most) {
-        auto kernel = norm_fwd_kernel<T, decltype(e)::value / Elem<T>::V, decltype(aligned)::value, decltype(cta)::value,
+    dispatch(s, [&](auto cta, auto e, auto form, auto most) {
+        auto kernel = norm_fwd_kernel<T, decltype(e)::value / Elem<T>::V, decltype(form)::value, decltype(cta)::value,
                                       decltype(most)::value>;
-        // Units enough to fill the GPU, each with an equal share of consecutive rows.
+        // Units enough to fill the GPU, each with an equal share of the rows.
         const int64_t units = per * (int64_t)persistent_grid(kernel, s.threads * per, 0, (n.rows + per - 1) / per, 0);
-        const int64_t share = (n.rows + units - 1) / units;
-        kernel<<<(unsigned)((n.rows + share * per - 1) / (share * per)), dim3(s.threads, per), 0, st>>>(
+        const Chunks ch = make_chunks(n, n.rows, units, s.form == LINED ? l.step() : 1);
+        kernel<<<(unsigned)((ch.count + per - 1) / per), dim3(s.threads, per), 0, st>>>(
             static_cast<const T*>(a.x), static_cast<const T*>(a.residual), static_cast<const T*>(a.gate),
-            static_cast<const T*>(a.post_weight), static_cast<const T*>(a.pre_weight), n, share, y, h, rstd);
+            static_cast<const T*>(a.post_weight), static_cast<const T*>(a.pre_weight), n, ch, y, h, rstd);
     });
     count_launch();
     return finish_launch("nb200_gated_norm");
+}
+
+// 512 threads on every SM, about what fits one at a time, and one chunk for each unit of them: more chunks mean
+// more partial sums to write and add (bf16 [32768, 1024] 95 us, with twice as many 103). Gate groups of more than
+// one row stay apart, so that a unit's gate gradients are of one group, or of whole ones.
+int64_t bwd_target(const Shape& s) {
+    return (int64_t)sm_count() * (s.cta ? std::max(1, 512 / s.threads) : 2 * kWarpRows);
+}
+Chunks bwd_chunks(const Norm& n, const Shape& s, int64_t step) {
+    return make_chunks(n, n.group > 1 ? n.group : n.rows, bwd_target(s), step);
+}
+// Lined-up rows cut every gate group at least `step` ways: not where many small groups would make that far more
+// units (and partial sums) than the GPU needs.
+bool lined_pays(const Norm& n, int64_t step) {
+    return n.group == 1 || n.rows / n.group * step <= 2 * bwd_target(make_shape(n.width, LINED));
 }
 
 template <typename T>
@@ -605,20 +717,35 @@ int norm_bwd(const nb200_norm_args& a, const float* rstd, const T* dy, const T* 
              T* dw2, float* work, cudaStream_t st) {
     const Norm n = make_norm(a);
     constexpr int es = sizeof(T);
-    const bool al = rows_aligned(a.x, n.sx, es) && rows_aligned(a.residual, n.sr, es) &&
-                    rows_aligned(a.gate, n.sg, es) && rows_aligned(a.post_weight, 0, es) &&
-                    rows_aligned(a.pre_weight, 0, es) && rows_aligned(dy, n.sdy, es) && rows_aligned(dh, n.sdh, es) &&
-                    aligned16(dx) && aligned16(dres) && (!dgate || aligned16(dgate));
-    Shape s = make_shape(n.width);
-    s.aligned = al && n.width * es % 16 == 0;
+    Layout l;
+    l.add(a.x, n.sx, es);
+    l.add(a.residual, n.sr, es);
+    l.add(dy, n.sdy, es);
+    l.add(dh, n.sdh, es);
+    l.add(dx, n.width, es);
+    l.add(dres, n.width, es);
+    if (n.group == 1) {
+        l.add(a.gate, n.sg, es);
+        l.add(dgate, n.width, es);
+    }
+    Layout all = l;
+    if (n.group > 1) {
+        all.add(a.gate, n.sg, es);
+        all.add(dgate, n.width, es);
+    }
+    all.add(a.post_weight, 0, es);
+    all.add(a.pre_weight, 0, es);
+    Form form = pick_form(n, l, all, es);
+    if (form == LINED && !lined_pays(n, l.step())) form = ANY;
+    const Shape s = make_shape(n.width, form);
     const int per = s.cta ? 1 : kWarpRows;
-    const Chunks ch = make_chunks(n);
+    const Chunks ch = bwd_chunks(n, s, s.form == LINED ? l.step() : 1);
     const int64_t size = ch.count * n.width;
     float* p1 = dw1 ? work : nullptr;
     float* p2 = dw2 ? work + size : nullptr;
-    float* pg = dgate && ch.per_group > 1 ? work + 2 * size : nullptr;
-    dispatch(s, [&](auto cta, auto e, auto aligned, auto most) {
-        auto kernel = norm_bwd_kernel<T, decltype(e)::value / Elem<T>::V, decltype(aligned)::value, decltype(cta)::value,
+    float* pg = dgate && n.group > 1 && ch.per_group > 1 ? work + 2 * size : nullptr;
+    dispatch(s, [&](auto cta, auto e, auto f, auto most) {
+        auto kernel = norm_bwd_kernel<T, decltype(e)::value / Elem<T>::V, decltype(f)::value, decltype(cta)::value,
                                       decltype(most)::value>;
         const int smem = 3 * per * s.threads * decltype(e)::value * (int)sizeof(float);
         if (smem > 40 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
@@ -658,8 +785,12 @@ int launch_norm_fwd(const nb200_norm_args& a, int dtype, void* y, void* h, float
 }
 
 int64_t norm_bwd_work_bytes(const nb200_norm_args& a) {
+    // The form depends on the pointers: room for the form that cuts finest.
     const Norm n = make_norm(a);
-    return 3 * make_chunks(n).count * n.width * (int64_t)sizeof(float);
+    int64_t count = bwd_chunks(n, make_shape(n.width, ALIGNED), 1).count;
+    for (int64_t step = 1; step <= 8; step *= 2)
+        if (lined_pays(n, step)) count = std::max(count, bwd_chunks(n, make_shape(n.width, LINED), step).count);
+    return 3 * count * n.width * (int64_t)sizeof(float);
 }
 
 int launch_norm_bwd(const nb200_norm_args& a, int dtype, const float* rstd, const void* dy, const void* dh, void* dx,

@@ -250,3 +250,26 @@ def test_empty_and_other_stream():
     with torch.cuda.stream(side):
         _run_and_check(_make((64, 640), "bfloat16", "full", 2), "bfloat16", label="stream")
     side.synchronize()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("gate", ["none", "channel", "sequence", "full"])
+@pytest.mark.parametrize("shape", [(1, 1, 333), (2, 9, 1001), (3, 700, 77), (400, 3, 259), (2, 4, 4099), (1, 5, 8197),
+                                   (600, 2, 514), (1, 3, 16383)])
+def test_rows_off_the_vector_boundary(shape, gate, dtype):
+    """Contiguous rows whose offsets repeat every 2 to 8 rows, alone and in groups that share a gate."""
+    _run_and_check(_make(shape, dtype, gate, 31), dtype, "sigmoid", 0.8, label=f"{shape} {gate} {dtype}")
+
+
+def test_slices_off_the_vector_boundary():
+    """Rows with an aligned pitch and an unaligned start: tensors laid out alike, then each on its own."""
+    import torch
+
+    for same in (True, False):
+        s = _make((6, 11, 520), "bfloat16", "sequence", 9)
+        for i, name in enumerate(("x", "residual", "gy", "gh")):
+            room = torch.zeros(6, 11, 528, dtype=torch.bfloat16, device="cuda")
+            at = 3 if same else 1 + 2 * i
+            room[..., at:at + 520] = s[name]
+            s[name] = room[..., at:at + 520]
+        _run_and_check(s, "bfloat16", "tanh", label=f"slices {same}")
