@@ -686,9 +686,10 @@ int norm_fwd(const nb200_norm_args& a, T* y, T* h, float* rstd, cudaStream_t st)
     dispatch(s, [&](auto cta, auto e, auto form, auto most) {
         auto kernel = norm_fwd_kernel<T, decltype(e)::value / Elem<T>::V, decltype(form)::value, decltype(cta)::value,
                                       decltype(most)::value>;
-        // Units enough to fill the GPU, each with an equal share of the rows.
-        const int64_t units = per * (int64_t)persistent_grid(kernel, s.threads * per, 0, (n.rows + per - 1) / per, 0);
-        const Chunks ch = make_chunks(n, n.rows, units, s.form == LINED ? l.step() : 1);
+        // Units enough to fill the GPU (1024 threads of 64 registers on an SM, or 512 of 128), each with an equal share
+        // of the rows.
+        const int64_t ctas = (int64_t)sm_count() * std::max(1, (s.e == 8 ? 1024 : 512) / (s.threads * per));
+        const Chunks ch = make_chunks(n, n.rows, ctas * per, s.form == LINED ? l.step() : 1);
         kernel<<<(unsigned)((ch.count + per - 1) / per), dim3(s.threads, per), 0, st>>>(
             static_cast<const T*>(a.x), static_cast<const T*>(a.residual), static_cast<const T*>(a.gate),
             static_cast<const T*>(a.post_weight), static_cast<const T*>(a.pre_weight), n, ch, y, h, rstd);

@@ -404,7 +404,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_bwd_cuda(const at::Tens
 
 // [rows, last] of t with unit column stride: a copy only when no such view exists.
 at::Tensor unit_rows(const at::Tensor& t, int64_t rows) {
-    at::Tensor f = t.dim() == 2 && t.size(0) == rows ? t : t.reshape({rows, t.size(-1)});
+    at::Tensor f = t.dim() == 2 ? t : t.reshape({rows, t.size(-1)});
     return (f.stride(1) == 1 || f.size(1) == 1) && f.stride(0) >= 0 ? f : f.contiguous();
 }
 
@@ -435,6 +435,10 @@ struct NormInputs {
         TORCH_CHECK_VALUE(t.device() == like.device(), what, ": tensors must be on one CUDA device");
     }
     const void* row_input(const at::Tensor& t, int64_t n, int64_t* stride) {
+        if (t.is_contiguous()) {
+            *stride = t.size(-1);
+            return t.data_ptr();
+        }
         keep.push_back(unit_rows(t, n));
         *stride = keep.back().stride(0);
         return keep.back().data_ptr();
@@ -449,6 +453,7 @@ struct NormInputs {
         same_kind(*t, x, what);
         TORCH_CHECK_VALUE(t->dim() == 1 && t->size(0) == x.size(-1), what,
                           ": weights must be 1-D with x's last dimension");
+        if (t->is_contiguous()) return t->data_ptr();
         keep.push_back(t->contiguous());
         return keep.back().data_ptr();
     }
