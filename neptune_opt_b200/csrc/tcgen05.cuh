@@ -1,5 +1,5 @@
 // sm_100a tensor-core (tcgen05), tensor-memory (TMEM) and tensor-map copy (TMA) primitives, as
-// inline PTX. Used by the fused attention kernel.
+// inline PTX. Used by the attention kernels.
 //
 // Conventions:
 //  * tcgen05.mma is issued by one thread; its completion is observed through tcgen05.commit, which
