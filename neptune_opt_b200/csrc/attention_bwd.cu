@@ -625,6 +625,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_kernel(const __grid_cons
     // Only the statistics come from the kernel before this one: everything else may be read while that one drains.
     const int len = tokens_of(a.lens, batch, a.S);
     if (row0 >= len) {  // none of the CTA's rows belongs to the sequence
+        pdl_wait();  // so that this grid never ends before the one ahead of it
         if (keys && a.parts > 1) return;
         const int rows = min(kRows, a.S - row0);
         for (int i = threadIdx.x; i < rows * (kDim / 8); i += kThreads) {
@@ -648,6 +649,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_kernel(const __grid_cons
     const int skip = cut ? (int)((int64_t)all * part / a.parts) : 0;
     const int n = cut ? (int)((int64_t)all * (part + 1) / a.parts) - skip : all;
     if (n == 0) {  // a part without steps: its sums are zero
+        pdl_wait();
         for (int i = threadIdx.x; i < min(kRows, len - row0) * (kDim / 4); i += kThreads) {
             const int64_t at = (part * a.part_rows + ((int64_t)batch * a.Hk + head) * a.S + row0) * kDim + 4 * i;
             *reinterpret_cast<uint4*>(a.part_k + at) = *reinterpret_cast<uint4*>(a.part_v + at) =

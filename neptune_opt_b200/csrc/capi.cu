@@ -556,8 +556,8 @@ int nb200_gated_norm(const nb200_norm_args* args, int dtype, void* y, void* h, f
     const int rc = check_norm("nb200_gated_norm", args, dtype, true);
     if (rc) return rc;
     if (args->rows == 0) return NB200_OK;
-    if (!args->x || !args->residual || !y || !rstd || (args->pre_weight && !h)) {
-        set_error("nb200_gated_norm: null pointer");
+    if (!args->x || !args->residual || !y || !rstd || (args->pre_weight && !h) || ((uintptr_t)rstd & 7u)) {
+        set_error("nb200_gated_norm: null pointer, or rstd not 8-byte aligned");
         return NB200_ERR_ARG;
     }
     return launch_norm_fwd(*args, dtype, y, h, rstd, (cudaStream_t)stream);
@@ -575,8 +575,8 @@ int nb200_gated_norm_bwd(const nb200_norm_args* args, int dtype, const float* rs
     const int rc = check_norm("nb200_gated_norm_bwd", args, dtype, false);
     if (rc) return rc;
     if (args->rows == 0) return NB200_OK;
-    if (!args->x || !args->residual || !rstd || !dx || !dresidual) {
-        set_error("nb200_gated_norm_bwd: null pointer");
+    if (!args->x || !args->residual || !rstd || !dx || !dresidual || ((uintptr_t)rstd & 7u)) {
+        set_error("nb200_gated_norm_bwd: null pointer, or rstd not 8-byte aligned");
         return NB200_ERR_ARG;
     }
     if ((dgate && !args->gate) || (dpost && !args->post_weight) || (dpre && !args->pre_weight) ||

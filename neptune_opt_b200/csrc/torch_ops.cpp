@@ -513,7 +513,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> gated_nor
     TORCH_CHECK_VALUE(rstd_.device() == x.device() && rstd_.dim() == x.dim() && rstd_.size(-1) == 2 &&
                           rstd_.sizes().slice(0, x.dim() - 1) == x.sizes().slice(0, x.dim() - 1),
                       what, ": rstd must be [..., 2]");
-    const at::Tensor rstd = rstd_.contiguous();
+    const bool whole = rstd_.is_contiguous() && reinterpret_cast<uintptr_t>(rstd_.data_ptr()) % 8 == 0;
+    const at::Tensor rstd = whole ? rstd_ : rstd_.clone(at::MemoryFormat::Contiguous);
     const void* dy = present(gy) ? in.like_x(*gy, x, &in.a.stride_grad_y, what) : nullptr;
     const void* dh = present(gh) ? in.like_x(*gh, x, &in.a.stride_grad_h, what) : nullptr;
     auto fresh = [&](const OptTensor& t) { return present(t) ? at::empty(t->sizes(), t->options()) : at::Tensor(); };

@@ -285,3 +285,20 @@ def test_other_stream_and_empty():
     none = torch.empty(0, 2, 5, D, dtype=torch.bfloat16, device="cuda")
     out = NB.attention_backward(none, none, none, none, torch.empty(0, 2, 5, device="cuda"), none)
     assert [t.shape for t in out] == [none.shape] * 3
+
+
+@pytest.mark.parametrize("lens", [[100, 2000], [1, 0], [129, 1]])
+def test_parts_without_steps(lens):
+    """A long tensor with short sequences: key blocks are cut into more parts than they have steps."""
+    import torch
+
+    import neptune_opt_b200 as NB
+
+    for shape, causal in (((2, 1, 1, 2000), False), ((2, 4, 1, 2000), True)):
+        q, k, v, g = _make(shape, 77)
+        dev = _lens_of(lens, 2, 2000)
+        o, lse = NB.attention(q, k, v, causal=causal, return_lse=True, seq_lens=dev)
+        grads = NB.attention_backward(q, k, v, o, lse, g, causal=causal, seq_lens=dev)
+        _check_all(q, k, v, o, lse, g, grads, lens, causal, 1.0 / math.sqrt(D), f"{shape} {lens}")
+        again = NB.attention_backward(q, k, v, o, lse, g, causal=causal, seq_lens=dev)
+        assert all(torch.equal(a, c) for a, c in zip(grads, again))

@@ -273,3 +273,19 @@ def test_slices_off_the_vector_boundary():
             room[..., at:at + 520] = s[name]
             s[name] = room[..., at:at + 520]
         _run_and_check(s, "bfloat16", "tanh", label=f"slices {same}")
+
+
+def test_reciprocal_norms_off_their_boundary():
+    import torch
+
+    import neptune_opt_b200 as NB
+
+    s = _make((5, 96), "float32", "channel", 4)
+    kw = {"post_weight": s["post"], "pre_weight": s["pre"]}
+    rstd = NB.run_gated_residual_norm(s["x"], s["residual"], s["gate"], **kw)[2]
+    room = torch.empty(11, device="cuda")
+    room[1:] = rstd.flatten()
+    args = (s["gy"], s["gh"], s["x"], s["residual"], s["gate"])
+    want = NB.gated_residual_norm_backward(*args, rstd, **kw)
+    got = NB.gated_residual_norm_backward(*args, room[1:].view(5, 2), **kw)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
