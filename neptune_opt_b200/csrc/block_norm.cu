@@ -21,6 +21,7 @@
 #include "common.cuh"
 #include "fastmath.cuh"
 #include "launch.h"
+#include "stream.cuh"
 
 namespace nb200 {
 namespace {
@@ -433,23 +434,27 @@ __device__ __forceinline__ void store_part(float* part, const uint64_t* acc, con
 // Within a gate group the gate and post-weight gradients share one column sum, G = sum xhat dY:
 // dgate = scale a' w1 G and dw1 += scale a G.
 //
-// The next row's four operands are on their way in registers while a row is computed (AHEAD, 8 elements a
-// thread). That takes one CTA of 512 threads per SM; two at 64 registers a thread, with or without a ring of
-// bulk copies in shared memory in place of the registers, spilled and ran slower (bf16 [16384, 4096]: 250
-// and 294 us).
-template <typename T, int NV, Form FORM, bool CTA, int kThreads>
+// A row's four operands come through a ring of shared-memory stages filled by bulk copies (RING: the CTA form of
+// ALIGNED rows, where three stages fit), rows ahead of their use and without registers or issue slots; without a
+// ring the next row waits in registers (AHEAD). bf16 [16384, 4096]: 170 us with the ring, 181 us in registers;
+// with two stages it lost ([8192, 8192] 283 us against 238), and for LINED rows too ([16384, 3001] 202 against 193).
+// One CTA of 512 threads per SM either way: two, at 64 registers a thread, spilled (250 us).
+constexpr int kMaxRing = 4;
+
+template <typename T, int NV, Form FORM, bool CTA, bool RING, int kThreads>
 __global__ void __launch_bounds__(kThreads)
     norm_bwd_kernel(const T* dy, const T* dh, const T* x, const T* res, const T* gate, const T* w1, const T* w2,
-                    const float* rstd, Norm n, Chunks ch, T* dx, T* dres, T* dgate, float* part1, float* part2,
-                    float* partg) {
+                    const float* rstd, Norm n, Chunks ch, int stages, T* dx, T* dres, T* dgate, float* part1,
+                    float* part2, float* partg) {
+    static_assert(!RING || (CTA && FORM == ALIGNED), "the ring holds whole aligned rows");
     using R = Rows<T, NV, FORM, CTA>;
     using CH = typename R::CH;
     constexpr int P = R::P;
-    constexpr bool AHEAD = P == 4;
+    constexpr bool AHEAD = !RING && P == 4;
     __shared__ float buf[CTA ? 256 : 1];
+    __shared__ uint64_t full[RING ? kMaxRing : 1];
     extern __shared__ __align__(16) uint8_t dyn[];
     R r(n.width, buf);
-    // What a thread keeps across rows but touches little lives in shared memory, in slots of its own: scale
     // What a thread keeps across rows but touches little lives in shared memory, in slots of its own:
     // a(gate), b = scale a(gate) w1 and the post weight's sums (touched once per gate group).
     const int slots = (CTA ? 1 : kWarpRows) * r.G * P;
@@ -461,6 +466,31 @@ __global__ void __launch_bounds__(kThreads)
     uint32_t row, end;
     ch.range(r.unit, n, row, end);
     r.line_up(x + row * n.sx);
+    // Stage s holds the vectors of x, residual, dy and dh that cover one row.
+    uint8_t* ring = reinterpret_cast<uint8_t*>(bs - r.t + 3 * slots);
+    const uint32_t bytes = r.width * (uint32_t)sizeof(T);
+    auto fill = [&](int s, uint32_t i) {  // one thread
+        uint8_t* to = ring + s * 4 * bytes;
+        mbar_expect_tx(&full[s], (2 + (dy ? 1 : 0) + (dh ? 1 : 0)) * bytes);
+        bulk_load(to, x + i * n.sx, bytes, &full[s]);
+        bulk_load(to + bytes, res + i * n.sr, bytes, &full[s]);
+        if (dy) bulk_load(to + 2 * bytes, dy + i * n.sdy, bytes, &full[s]);
+        if (dh) bulk_load(to + 3 * bytes, dh + i * n.sdh, bytes, &full[s]);
+    };
+    int stage = 0;
+    uint32_t parity = 0;
+    bool primed = false;  // a row has been taken out of the ring
+    bool arrived = true;  // false once a wait has run out: the rest runs through without waiting
+    if constexpr (RING) {
+        if (threadIdx.x == 0) {
+            for (int s = 0; s < stages; ++s) mbar_init(&full[s], 1);
+            fence_barrier_init();
+            fence_proxy_async();
+            for (int s = 0; s < stages; ++s)
+                if (row + s * ch.step < end) fill(s, row + s * (uint32_t)ch.step);
+        }
+        __syncthreads();
+    }
     CH c2;
     if (w2) r.load_shared(c2, w2);
     uint64_t G[P], a2[P];
@@ -473,18 +503,34 @@ __global__ void __launch_bounds__(kThreads)
     bool fresh = true;
     CH nx, nr, ndy, ndh;
     float2 nrs;
+    auto statistics = [&](uint32_t i) { nrs = *reinterpret_cast<const float2*>(rstd + 2 * (int64_t)i); };
     auto fetch = [&](uint32_t i) {
-        nrs = *reinterpret_cast<const float2*>(rstd + 2 * (int64_t)i);
+        statistics(i);
         r.load(nx, x + i * n.sx, true);
         r.load(nr, res + i * n.sr, true);
         if (dy) r.load(ndy, dy + i * n.sdy, true);
         if (dh) r.load(ndh, dh + i * n.sdh, true);
     };
     if (AHEAD && row < end) fetch(row);
+    if (RING && row < end) statistics(row);
     for (; row < end; row += ch.step) {
         const uint32_t next = row + ch.step, next_index = gate ? next / n.group : 0u;
         const bool last = next >= end;
-        if (!AHEAD) fetch(row);
+        if (!AHEAD && !RING) fetch(row);
+        if constexpr (RING) {
+            arrived = arrived && mbar_wait(&full[stage], parity);
+            auto staged = [&](CH& c, int i) {
+#pragma unroll
+                for (int k = 0; k < NV; ++k) {
+                    const uint4* p = reinterpret_cast<const uint4*>(ring + (stage * 4 + i) * bytes) + r.t + k * r.G;
+                    c.raw[k] = r.col(k) < r.width ? *p : make_uint4(0u, 0u, 0u, 0u);
+                }
+            };
+            staged(nx, 0);
+            staged(nr, 1);
+            if (dy) staged(ndy, 2);
+            if (dh) staged(ndh, 3);
+        }
         CH cx = nx, cr = nr, cdy = ndy, cdh = ndh;
         r.finish(cx);
         r.finish(cr);
@@ -521,6 +567,7 @@ __global__ void __launch_bounds__(kThreads)
         }
         // Issued here, the loads cover the sums' latency.
         if (AHEAD && !last) fetch(next);
+        if (RING && !last) statistics(next);
         if (gate && next_index != index && !last && (r.t & 7) == 0)
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
@@ -529,6 +576,17 @@ __global__ void __launch_bounds__(kThreads)
             }
         float t1 = f2lo(s1) + f2hi(s1), t2 = f2lo(s2) + f2hi(s2), t3 = f2lo(s3) + f2hi(s3);
         r.sum3(t1, t2, t3);
+        if constexpr (RING) {
+            // Past the barrier in there, every thread is done with the previous row: its stage takes the row that is
+            // `stages` behind it.
+            const uint32_t ahead = row + (uint32_t)ch.step * (stages - 1);
+            if (threadIdx.x == 0 && primed && ahead < end) fill(stage ? stage - 1 : stages - 1, ahead);
+            primed = true;
+            if (++stage == stages) {
+                stage = 0;
+                parity ^= 1u;
+            }
+        }
         const float k2 = r2 * t1 * n.inv_n, m1 = (t2 - k2 * t3) * n.inv_n;  // k2 = r2 m2
         const uint64_t k2p = f2(-k2, -k2), k1p = f2(w1 ? -m1 : 0.f, w1 ? -m1 : 0.f);
 #pragma unroll
@@ -559,6 +617,9 @@ __global__ void __launch_bounds__(kThreads)
             for (int i = 0; i < P; ++i) G[i] = 0;
         }
     }
+    if (RING && !arrived && threadIdx.x == 0)  // copies may still be on their way: wait for them, again with a limit
+        for (int s = 0; s < stages; ++s)
+            for (uint32_t ph = 0; ph < 2; ++ph) mbar_wait(&full[s], ph);
     if (part2) store_part(part2 + r.unit * n.width, a2, r);
     if (part1) {
 #pragma unroll
@@ -746,13 +807,27 @@ int norm_bwd(const nb200_norm_args& a, const float* rstd, const T* dy, const T* 
     float* p2 = dw2 ? work + size : nullptr;
     float* pg = dgate && n.group > 1 && ch.per_group > 1 ? work + 2 * size : nullptr;
     dispatch(s, [&](auto cta, auto e, auto f, auto most) {
-        auto kernel = norm_bwd_kernel<T, decltype(e)::value / Elem<T>::V, decltype(f)::value, decltype(cta)::value,
-                                      decltype(most)::value>;
-        const int smem = 3 * per * s.threads * decltype(e)::value * (int)sizeof(float);
+        constexpr int kNV = decltype(e)::value / Elem<T>::V, kMost = decltype(most)::value;
+        constexpr Form kForm = decltype(f)::value;
+        constexpr bool kCta = decltype(cta)::value;
+        auto kernel = norm_bwd_kernel<T, kNV, kForm, kCta, false, kMost>;
+        int smem = 3 * per * s.threads * decltype(e)::value * (int)sizeof(float), stages = 0;
+        if constexpr (kCta && kForm == ALIGNED && kMost == 512) {
+            // What the CTAs that share an SM leave of its shared memory (228 KB, 1 KB of it reserved for each) beside
+            // their accumulators and the kernel's own 1.1 KB.
+            const int room = 233472 / std::max(1, 512 / s.threads) - 1024 - 1280 - smem;
+            const int stage = 4 * (int)n.width * es;
+            stages = std::min(kMaxRing, room / stage);
+            if (stages >= 3) {
+                kernel = norm_bwd_kernel<T, kNV, kForm, kCta, true, kMost>;
+                smem += stages * stage;
+            }
+        }
         if (smem > 40 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         kernel<<<(unsigned)((ch.count + per - 1) / per), dim3(s.threads, per), smem, st>>>(
             dy, dh, static_cast<const T*>(a.x), static_cast<const T*>(a.residual), static_cast<const T*>(a.gate),
-            static_cast<const T*>(a.post_weight), static_cast<const T*>(a.pre_weight), rstd, n, ch, dx, dres, dgate,
+            static_cast<const T*>(a.post_weight), static_cast<const T*>(a.pre_weight), rstd, n, ch, stages, dx, dres,
+            dgate,
             p1, p2, pg);
     });
     count_launch();
@@ -775,6 +850,17 @@ int norm_bwd(const nb200_norm_args& a, const float* rstd, const T* dy, const T* 
 }
 
 }  // namespace
+
+int norm_fault_take(unsigned int* bits) {
+    unsigned int v = 0, zero = 0;
+    if (cudaMemcpyFromSymbol(&v, g_stream_fault, sizeof(v)) != cudaSuccess ||
+        cudaMemcpyToSymbol(g_stream_fault, &zero, sizeof(zero)) != cudaSuccess) {
+        set_error("cannot read the gated norm's fault word: %s", cudaGetErrorString(cudaGetLastError()));
+        return NB200_ERR_LAUNCH;
+    }
+    *bits = v;
+    return NB200_OK;
+}
 
 int launch_norm_fwd(const nb200_norm_args& a, int dtype, void* y, void* h, float* rstd, cudaStream_t st) {
     const int rc = check_width("nb200_gated_norm", a.width);

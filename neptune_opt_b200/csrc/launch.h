@@ -75,6 +75,7 @@ int stream_span(int sk, const Params& p, const void* x, int dtype, int64_t rows,
 int stream_fault_take(unsigned int* bits);
 int attn_fault_take(unsigned int* bits);
 int attn_bwd_fault_take(unsigned int* bits);
+int norm_fault_take(unsigned int* bits);
 
 int launch_attention(const nb200_attn_args& a, const nb200_attn_strides* strides, const void* q, const void* k,
                      const void* v, void* o, float* lse, cudaStream_t st);
