@@ -8,6 +8,7 @@
 //
 // An index outside [0, vocab) marks an entry that was not kept. A row without kept entries has loss 0
 // and gradient 0 whatever its logits hold.
+#include <algorithm>
 #include <cmath>
 #include <type_traits>
 
@@ -18,8 +19,24 @@
 namespace nb200 {
 namespace {
 
-constexpr int kMaxTop = 256;  // entries a row may keep: one per thread of its CTA
+constexpr int kMaxTop = 256;  // entries a row may keep
 constexpr float kL2e = 1.4426950408889634f;
+// A CTA of 256 threads takes a row, or a chunk of one (bf16 [4096, 131072] forward 164 us, 6.5 TB/s; 191 us with 512
+// and 175 us with 128). Narrow rows, where there are many, go to a warp each, kWarpRows of them in a CTA: there a CTA's
+// launch and barriers count for more than its loads (bf16, CTA -> warp: [8192, 1000] 39 -> 15 us forward, 30 -> 19 us
+// backward; [8192, 10007] 62 -> 40 us forward, but 81 -> 89 us backward). With fewer rows the warps leave SMs idle:
+// [1200, 5000] 9.7 -> 8.1 and 10.0 -> 8.7 us, but [600, 5000] 6.1 -> 6.8 and 5.5 -> 7.7 us.
+constexpr int kWide = 256, kWarpRows = 8;
+constexpr int64_t kNarrowFwd = 16384, kNarrowBwd = 8192;  // columns
+
+bool narrow_rows(int64_t rows, int64_t vocab, int64_t most) { return vocab <= most && vocab <= 5 * rows; }
+
+// A barrier of the threads that share a row.
+template <int kThreads>
+__device__ __forceinline__ void row_sync() {
+    if constexpr (kThreads == 32) __syncwarp();
+    else __syncthreads();
+}
 
 struct Row {  // what both directions read of the teacher
     const void* teacher;
@@ -96,11 +113,9 @@ struct LogSum {
 };
 
 // ------------------------------------------------------------------ forward
-// One cluster of CTAs per row (one CTA when there are rows enough): each folds a share of the row's 16-byte
+// One cluster of CTAs per row (one CTA, or a warp, when there are rows enough): each folds a share of the row's 16-byte
 // vectors, the states meet in the first CTA's shared memory, and that CTA's first warp takes the kept
 // entries, which were fetched before the fold. One pass over the logits, no scratch.
-// 256 threads: bf16 [4096, 131072] 164 us (6.5 TB/s); 191 us with 512 and 175 us with 128.
-constexpr int kFwdThreads = 256;
 constexpr int kMaxCluster = 16;
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -124,20 +139,24 @@ __device__ __forceinline__ void store_first(float* p, float v) {
     asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(v) : "memory");
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kFwdThreads)
-    distill_fwd_kernel(const T* x, int64_t stride, Row r, const float* teacher_lse, float* loss, float* stats) {
-    constexpr int V = Elem<T>::V, U = 4;  // U vectors in flight per thread
-    __shared__ float ec[32], es[32], cc[kMaxCluster], cs[kMaxCluster], teach[kMaxTop], stud[kMaxTop];
-    const uint32_t rank = cluster_rank(), size = cluster_size();
-    const int64_t row = blockIdx.x / size;
+template <typename T, int kThreads>
+__global__ void __launch_bounds__(kWide)
+    distill_fwd_kernel(const T* x, int64_t rows, int64_t stride, Row r, const float* teacher_lse, float* loss,
+                       float* stats) {
+    constexpr int V = Elem<T>::V, U = 4, kRows = kWide / kThreads;  // U vectors in flight per thread
+    __shared__ float ec[32], es[32], cc[kMaxCluster], cs[kMaxCluster], teach_[kRows][kMaxTop], stud_[kRows][kMaxTop];
+    const int sub = kRows > 1 ? threadIdx.y : 0;  // which of the CTA's rows
+    float *teach = teach_[sub], *stud = stud_[sub];
+    const uint32_t rank = kRows > 1 ? 0 : cluster_rank(), size = kRows > 1 ? 1 : cluster_size();
+    const int64_t row = (int64_t)(blockIdx.x / size) * kRows + sub;
+    if (kRows > 1 && row >= rows) return;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const T* xr = x + row * stride;
-    // The kept entries, one per thread: t_j / T (-inf: not kept, its probability is 0) and x / T.
-    if (rank == 0 && t < r.top) {
-        const int64_t at = r.at(row, t);
-        teach[t] = at >= 0 ? r.logit(row, t) : -NB200_INF;
-        stud[t] = at >= 0 ? Elem<T>::to_f(xr[at]) * r.inv_t : 0.f;
+    // The kept entries: t_j / T (-inf: not kept, its probability is 0) and x / T.
+    for (int j = rank == 0 ? t : r.top; j < r.top; j += kThreads) {
+        const int64_t at = r.at(row, j);
+        teach[j] = at >= 0 ? r.logit(row, j) : -NB200_INF;
+        stud[j] = at >= 0 ? Elem<T>::to_f(xr[at]) * r.inv_t : 0.f;
     }
     const float scale = r.inv_t * kL2e;
     LogSum acc;
@@ -146,33 +165,33 @@ __global__ void __launch_bounds__(kFwdThreads)
     split_range(nv, size, rank, v0, v1);
     const uint4* p = reinterpret_cast<const uint4*>(xr + head);
     int64_t v = v0 + t;
-    for (; v + (U - 1) * kFwdThreads < v1; v += U * kFwdThreads) {
+    for (; v + (U - 1) * kThreads < v1; v += U * kThreads) {
         uint4 u[U];
 #pragma unroll
-        for (int k = 0; k < U; ++k) u[k] = ld_stream(p + v + k * kFwdThreads);
+        for (int k = 0; k < U; ++k) u[k] = ld_stream(p + v + k * kThreads);
         float f[U * V];
 #pragma unroll
         for (int k = 0; k < U; ++k) Elem<T>::unpack(u[k], f + k * V);
         acc.add<U * V>(f, scale);
     }
-    for (; v < v1; v += kFwdThreads) {
+    for (; v < v1; v += kThreads) {
         float f[V];
         Elem<T>::unpack(ld_stream(p + v), f);
         acc.add<V>(f, scale);
     }
     if (rank == 0) {  // what lies outside the vectors: fewer than 2 V elements
         if (t < head) acc.add_one(Elem<T>::to_f(xr[t]), scale);
-        else if (t >= 32 && tail + t - 32 < r.vocab) acc.add_one(Elem<T>::to_f(xr[tail + t - 32]), scale);
+        if (tail + t < r.vocab) acc.add_one(Elem<T>::to_f(xr[tail + t]), scale);
     }
     acc.merge_warp(16);
-    if (lane == 0) {
+    if (kThreads > 32 && lane == 0) {
         ec[warp] = acc.c;
         es[warp] = acc.s;
     }
-    __syncthreads();
-    if (warp == 0) {
+    row_sync<kThreads>();
+    if (kThreads > 32 && warp == 0) {
         acc = LogSum{};
-        if (lane < kFwdThreads / 32) acc.merge(ec[lane], es[lane]);
+        if (lane < kThreads / 32) acc.merge(ec[lane], es[lane]);
         acc.merge_warp(16);
         if (size > 1 && lane == 0) {
             store_first(&cc[rank], acc.c);
@@ -225,79 +244,91 @@ __global__ void __launch_bounds__(kFwdThreads)
 // [1024, 50001] 24.9, 29.1, 45.3 us; [160, 131072] 20.5, 15.6, 14.7 us.
 template <typename T>
 int cluster_for(int64_t rows, int64_t vocab) {
-    const int64_t round = (int64_t)kFwdThreads * Elem<T>::V;
+    const int64_t round = (int64_t)kWide * Elem<T>::V;
     int c = 1;
     while (c < kMaxCluster && rows * c < 4 * sm_count() && vocab >= 2 * c * round) c *= 2;
     return c;
 }
 
 // ------------------------------------------------------------------ backward
-// One CTA per row and chunk of columns: write the softmax part of the chunk, then the chunk's kept
+// One CTA, or a warp, per row and chunk of columns: write the softmax part of the chunk, then the chunk's kept
 // columns once more with their probabilities taken off.
-constexpr int kBwdThreads = 256;
-constexpr int kChunk = 16384;  // columns
-static_assert(kMaxTop <= kBwdThreads && kMaxTop <= kFwdThreads, "one kept entry per thread");
+constexpr int kChunk = 16384;   // columns, at most
+constexpr int kChunkLeast = 2048;
 
-template <typename T>
-__global__ void __launch_bounds__(kBwdThreads)
-    distill_bwd_kernel(const float* grad, int64_t grad_stride, const T* x, int64_t stride, Row r, const float* stats,
-                       int chunks, T* dx) {
-    constexpr int V = Elem<T>::V, U = 4;
-    __shared__ int64_t at[kMaxTop];
-    __shared__ float p[kMaxTop];
-    const int64_t row = blockIdx.x / chunks, c0 = (int64_t)(blockIdx.x % chunks) * kChunk;
-    const int64_t c1 = min(c0 + kChunk, r.vocab);
-    const int t = threadIdx.x;
+template <typename T, int kThreads>
+__global__ void __launch_bounds__(kWide)
+    distill_bwd_kernel(const float* grad, int64_t grad_stride, const T* x, int64_t rows, int64_t stride, Row r,
+                       const float* stats, unsigned chunks, int64_t chunk, T* dx) {
+    constexpr int V = Elem<T>::V, U = 4, kRows = kWide / kThreads;
+    __shared__ __align__(16) int at_[kRows][kMaxTop];  // the entry's column in the chunk, -1 outside it
+    __shared__ float p_[kRows][kMaxTop];
+    const int sub = kRows > 1 ? threadIdx.y : 0;  // which of the CTA's rows
+    int* at = at_[sub];
+    float* p = p_[sub];
+    const unsigned item = blockIdx.x * kRows + sub;
+    const int64_t row = item / chunks, c0 = item % chunks * chunk;
+    if (kRows > 1 && row >= rows) return;
+    const int n = (int)min(chunk, r.vocab - c0), t = threadIdx.x;
     const float lse = stats[3 * row], z = stats[3 * row + 1], mass = stats[3 * row + 2];
-    const float w = grad[row * grad_stride] * r.inv_t;
-    const T* xr = x + row * stride;
-    T* dr = dx + row * r.vocab;
-    const int64_t mine = t < r.top ? r.at(row, t) : -1;
-    const float pm = mine >= 0 ? expf(r.logit(row, t) - z) : 0.f;
-    if (t < r.top) {
-        at[t] = mine;
-        p[t] = pm;
+    const float w = grad[row * grad_stride] * r.inv_t, wm = w * mass;
+    const T* xr = x + row * stride + c0;
+    T* dr = dx + row * r.vocab + c0;
+    bool mine = false;
+    for (int j = t; j < (r.top + 3 & ~3); j += kThreads) {
+        const int64_t c = j < r.top ? r.at(row, j) : -1;
+        mine = mine || c >= 0;
+        at[j] = c >= c0 && c < c0 + n ? (int)(c - c0) : -1;
+        p[j] = c >= 0 ? expf(r.logit(row, j) - z) : 0.f;
     }
-    const bool any = __syncthreads_or(mine >= 0);
-    const float wm = w * mass;
+    bool any;
+    if constexpr (kThreads == 32) any = __any_sync(0xffffffffu, mine);
+    else any = __syncthreads_or(mine);
+    row_sync<kThreads>();
     // w mass q, the difference taken before the change of base so that large logits keep their digits; a
     // row without kept entries is 0 whatever its logits hold.
     auto soft = [&](float f) { return any ? wm * ex2_ftz(fmaf(f, r.inv_t, -lse) * kL2e) : 0.f; };
-    const int64_t head = min(lead(dr + c0), c1 - c0);
-    const bool together = lead(xr + c0) == lead(dr + c0);  // both sides meet the same 16-byte boundaries
-    const int64_t nv = together ? (c1 - c0 - head) / V : 0;
-    const uint4* src = reinterpret_cast<const uint4*>(xr + c0 + head);
-    uint4* dst = reinterpret_cast<uint4*>(dr + c0 + head);
-    auto one = [&](const uint4& u, int64_t v) {
-        float f[V];
-        Elem<T>::unpack(u, f);
-#pragma unroll
-        for (int e = 0; e < V; ++e) f[e] = soft(f[e]);
-        __stcs(dst + v, Elem<T>::pack(f));
-    };
-    int64_t v = t;
-    for (; v + (U - 1) * kBwdThreads < nv; v += U * kBwdThreads) {
+    const int head = (int)min(lead(dr), (int64_t)n);
+    const bool together = lead(xr) == lead(dr);  // both sides meet the same 16-byte boundaries
+    const int nv = together ? (n - head) / V : 0;
+    const uint4* src = reinterpret_cast<const uint4*>(xr + head);
+    uint4* dst = reinterpret_cast<uint4*>(dr + head);
+    for (int v = t; v < nv; v += U * kThreads) {
         uint4 u[U];
 #pragma unroll
-        for (int k = 0; k < U; ++k) u[k] = ld_stream(src + v + k * kBwdThreads);
+        for (int k = 0; k < U; ++k)
+            if (v + k * kThreads < nv) u[k] = ld_stream(src + v + k * kThreads);
 #pragma unroll
-        for (int k = 0; k < U; ++k) one(u[k], v + k * kBwdThreads);
+        for (int k = 0; k < U; ++k) {
+            if (v + k * kThreads >= nv) break;
+            float f[V];
+            Elem<T>::unpack(u[k], f);
+#pragma unroll
+            for (int e = 0; e < V; ++e) f[e] = soft(f[e]);
+            __stcs(dst + v + k * kThreads, Elem<T>::pack(f));
+        }
     }
-    for (; v < nv; v += kBwdThreads) one(ld_stream(src + v), v);
-    if (t < head) dr[c0 + t] = Elem<T>::from_f(soft(Elem<T>::to_f(xr[c0 + t])));
-    for (int64_t c = c0 + head + nv * V + t; c < c1; c += kBwdThreads)
-        dr[c] = Elem<T>::from_f(soft(Elem<T>::to_f(xr[c])));
-    __syncthreads();
+    if (t < head) dr[t] = Elem<T>::from_f(soft(Elem<T>::to_f(xr[t])));
+    for (int c = head + nv * V + t; c < n; c += kThreads) dr[c] = Elem<T>::from_f(soft(Elem<T>::to_f(xr[c])));
+    row_sync<kThreads>();
     // By the first entry that names a column: entries of one column add in order.
-    if (mine >= c0 && mine < c1) {
+    for (int j = t; j < r.top; j += kThreads) {
+        const int c = at[j];
+        if (c < 0) continue;
         float sum = 0.f;
         bool first = true;
-        for (int j = 0; j < r.top; ++j) {
-            if (at[j] != mine) continue;
-            first = first && j >= t;
-            sum += p[j];
+        for (int i = 0; i < r.top; i += 4) {
+            const int4 o = *reinterpret_cast<const int4*>(at + i);
+            if (o.x != c && o.y != c && o.z != c && o.w != c) continue;
+            const int a[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (a[e] == c) {
+                    first = first && i + e >= j;
+                    sum += p[i + e];
+                }
         }
-        if (first) dr[mine] = Elem<T>::from_f(soft(Elem<T>::to_f(xr[mine])) - w * sum);
+        if (first) dr[c] = Elem<T>::from_f(soft(Elem<T>::to_f(xr[c])) - w * sum);
     }
 }
 
@@ -320,7 +351,7 @@ int check_sizes(const char* what, const nb200_distill_args& a) {
         set_error("%s: %lld kept logits per row exceed the kernel's %d", what, (long long)a.top, kMaxTop);
         return NB200_ERR_CAPACITY;
     }
-    if (a.rows * ((a.vocab + kChunk - 1) / kChunk) > 0x7fffffffLL || a.rows > 0x7fffffffLL / kMaxCluster) {
+    if (a.rows * ((a.vocab + kChunkLeast - 1) / kChunkLeast) > 0x7fffffffLL || a.rows > 0x7fffffffLL / kMaxCluster) {
         set_error("%s: %lld rows of %lld exceed the kernel's index range", what, (long long)a.rows,
                   (long long)a.vocab);
         return NB200_ERR_CAPACITY;
@@ -337,12 +368,13 @@ int launch_distill_fwd(const nb200_distill_args& a, const float* teacher_lse, fl
     const Row r = make_row(a);
     auto go = [&](auto* x) {
         using T = std::remove_const_t<std::remove_pointer_t<decltype(x)>>;
-        const auto kernel = distill_fwd_kernel<T>;
-        const int size = cluster_for<T>(a.rows, a.vocab);
+        const bool narrow = narrow_rows(a.rows, a.vocab, kNarrowFwd);
+        const auto kernel = narrow ? distill_fwd_kernel<T, 32> : distill_fwd_kernel<T, kWide>;
+        const int size = narrow ? 1 : cluster_for<T>(a.rows, a.vocab);
         if (size > 8) cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)(a.rows * size));
-        cfg.blockDim = dim3(kFwdThreads);
+        cfg.gridDim = dim3((unsigned)(narrow ? (a.rows + kWarpRows - 1) / kWarpRows : a.rows * size));
+        cfg.blockDim = narrow ? dim3(32, kWarpRows) : dim3(kWide);
         cfg.stream = st;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -350,7 +382,7 @@ int launch_distill_fwd(const nb200_distill_args& a, const float* teacher_lse, fl
         attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
-        cudaLaunchKernelEx(&cfg, kernel, x, a.stride_x, r, teacher_lse, loss, stats);
+        cudaLaunchKernelEx(&cfg, kernel, x, a.rows, a.stride_x, r, teacher_lse, loss, stats);
     };
     if (a.dtype == NB200_F32) go(static_cast<const float*>(a.x));
     else if (a.dtype == NB200_BF16) go(static_cast<const __nv_bfloat16*>(a.x));
@@ -366,9 +398,17 @@ int launch_distill_bwd(const nb200_distill_args& a, const float* grad, int64_t s
     const Row r = make_row(a);
     auto go = [&](auto* d) {
         using T = std::remove_pointer_t<decltype(d)>;
-        const int chunks = (int)((a.vocab + kChunk - 1) / kChunk);
-        distill_bwd_kernel<T><<<(unsigned)(a.rows * chunks), kBwdThreads, 0, st>>>(
-            grad, stride_grad, static_cast<const T*>(a.x), a.stride_x, r, stats, chunks, d);
+        // Equal chunks of whole 128-byte lines, four CTAs on every SM where rows are few and wide enough.
+        const int64_t want = (4 * (int64_t)sm_count() + a.rows - 1) / a.rows, least = (a.vocab + kChunk - 1) / kChunk;
+        const int64_t cut = std::max(least, std::min(want, a.vocab / kChunkLeast));
+        const int64_t chunk = ((a.vocab + cut - 1) / cut + 63) / 64 * 64, chunks = (a.vocab + chunk - 1) / chunk;
+        const bool narrow = narrow_rows(a.rows, a.vocab, kNarrowBwd);
+        const auto kernel = narrow ? distill_bwd_kernel<T, 32> : distill_bwd_kernel<T, kWide>;
+        const int64_t items = a.rows * chunks;
+        kernel<<<(unsigned)(narrow ? (items + kWarpRows - 1) / kWarpRows : items),
+                 narrow ? dim3(32, kWarpRows) : dim3(kWide), 0, st>>>(grad, stride_grad, static_cast<const T*>(a.x),
+                                                                     a.rows, a.stride_x, r, stats, (unsigned)chunks,
+                                                                     chunk, d);
     };
     if (a.dtype == NB200_F32) go(static_cast<float*>(dx));
     else if (a.dtype == NB200_BF16) go(static_cast<__nv_bfloat16*>(dx));

@@ -122,6 +122,40 @@ def test_rows_without_entries_and_repeated_entries():
     assert stats[0, 1] == -math.inf and stats[0, 2] == 0
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("shape", [(1003, 500, 12), (401, 2003, 256), (1643, 8189, 64), (3281, 16381, 33)])
+def test_many_narrow_rows(shape, dtype):
+    """Row counts that are no multiple of a CTA's, with rows of every kind side by side."""
+    import torch
+
+    x, t, index, grad = _make(*shape, dtype, 9)
+    rows, vocab, top = shape
+    index[5::7, top // 2:] = -1      # entries that were not kept, and what sits in them
+    t[5::7, top // 2:] = math.nan
+    index[3::11, 4:8] = index[3::11, :1]  # one column named five times
+    x[2::13, vocab // 2:] = -math.inf     # half the vocabulary masked
+    index[2::13] = torch.arange(top, device="cuda")
+    x[-1, vocab // 3:] = torch.finfo(x.dtype).min
+    index[-1] = torch.arange(top, device="cuda")
+    index[0] = vocab                 # nothing kept
+    # Where an entry of NaN was kept after all (the steps above meet in some rows), loss and gradient are NaN.
+    import neptune_opt_b200 as NB
+
+    bad = ((index >= 0) & (index < vocab) & t.isnan()).any(-1)
+    loss, stats = NB.run_distill_loss(x, t, index)
+    dx = NB.distill_loss_backward(grad, x, t, index, stats)
+    assert bad.any() and torch.equal(loss.isnan(), bad)
+    assert dx[bad].isnan().all() and not dx[~bad].isnan().any()
+    for first, temperature in ((0, 1.0), (1, 0.7)):
+        keep = ~bad[first:]
+        ref, bound, _ = _forward_ref(x[first:], t[first:], index[first:], temperature)
+        got, stats = NB.run_distill_loss(x[first:], t[first:], index[first:].int(), temperature=temperature)
+        assert ((got.double() - ref).abs() <= bound)[keep].all(), f"{shape} loss"
+        dx = NB.distill_loss_backward(grad[first:], x[first:], t[first:], index[first:], stats, temperature=temperature)
+        rdx, mag = _backward_ref(grad[first:], x[first:], t[first:], index[first:], stats, temperature)
+        assert ((dx.double() - rdx).abs() <= UNIT[dtype] * rdx.abs() + 2.0 ** -14 * mag + TINY[dtype])[keep].all(), shape
+
+
 def test_no_entries_at_all():
     import torch
 
