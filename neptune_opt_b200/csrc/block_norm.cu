@@ -74,12 +74,16 @@ struct Vecs {
 //           warp's span go one by one), fp32 rows go element by element, column t + i G.
 // bf16 [16384, 3001], backward: 193 us lined up, 427 us by shifted vectors, 795 us element by element.
 enum Form { ALIGNED, LINED, ANY };
+template <typename T, Form FORM>
+constexpr bool kScalar = FORM == ANY && sizeof(T) == 4;
 
-template <typename T, int NV, Form FORM, bool CTA>
+// KEEP: stored rows stay in L2 for whoever reads them next, ahead of what streams past (bf16 [16384, 4096] forward
+// 97.4 us, 99.6 stored as they stream; the backward, which writes less than it reads, is as fast either way and
+// leaves L2 to its partial sums).
+template <typename T, int NV, Form FORM, bool CTA, bool KEEP>
 struct Rows {
     using CH = Vecs<T, NV>;
     static constexpr int V = CH::V, P = CH::P;  // P pairs a thread
-    static constexpr bool SCALAR = FORM == ANY && sizeof(T) == 4;
     int t, G;
     int64_t unit;
     int width, lead = 0;
@@ -96,7 +100,7 @@ struct Rows {
         if (FORM == LINED) lead = (int)((reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(T));
     }
     __device__ __forceinline__ int col(int k) const { return (t + k * G) * V - (FORM == LINED ? lead : 0); }  // of vector k
-    __device__ __forceinline__ int col_of(int i) const { return SCALAR ? t + i * G : col(i / V) + i % V; }
+    __device__ __forceinline__ int col_of(int i) const { return kScalar<T, FORM> ? t + i * G : col(i / V) + i % V; }
     __device__ __forceinline__ bool holds(int c) const { return c < width && (FORM != LINED || c >= 0); }
     __device__ __forceinline__ static uint4 fetch(const void* p, bool stream) { return stream ? ld_stream(p) : ld_keep(p); }
     // A row of one of the tensors the form speaks of; `finish` before use. (Clearing the partial vectors here would
@@ -111,7 +115,7 @@ struct Rows {
             } else if constexpr (FORM == LINED) {
                 if (at < width && at + V > 0) c.raw[k] = fetch(row + at, stream);
                 else c.raw[k] = make_uint4(0u, 0u, 0u, 0u);
-            } else if constexpr (SCALAR) {
+            } else if constexpr (kScalar<T, FORM>) {
                 uint32_t w[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -185,6 +189,10 @@ struct Rows {
         if constexpr (V == 4) reinterpret_cast<uint32_t*>(row)[c] = w[j];
         else reinterpret_cast<uint16_t*>(row)[c] = (uint16_t)(w[j / 2] >> (16 * (j & 1)));
     }
+    __device__ __forceinline__ static void put_vec(void* p, const uint4& u) {
+        if (KEEP) *reinterpret_cast<uint4*>(p) = u;
+        else st_stream(p, u);
+    }
     __device__ __forceinline__ void store(T* row, const uint64_t* v) const {
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
@@ -196,15 +204,15 @@ struct Rows {
             }
             const int at = col(k);
             if constexpr (FORM == ALIGNED) {
-                if (at < width) st_stream(row + at, Elem<T>::pack(f));
-            } else if constexpr (SCALAR) {
+                if (at < width) put_vec(row + at, Elem<T>::pack(f));
+            } else if constexpr (kScalar<T, FORM>) {
 #pragma unroll
                 for (int j = 0; j < V; ++j)
                     if (col_of(k * V + j) < width) row[col_of(k * V + j)] = f[j];
             } else if constexpr (FORM == LINED) {
                 const uint4 u = Elem<T>::pack(f);
                 if (at >= 0 && at + V <= width) {
-                    st_stream(row + at, u);
+                    put_vec(row + at, u);
                 } else {
 #pragma unroll
                     for (int j = 0; j < V; ++j)
@@ -228,7 +236,7 @@ struct Rows {
         below.z = __shfl_up_sync(0xffffffffu, u.z, 1);
         below.w = __shfl_up_sync(0xffffffffu, u.w, 1);
         const bool whole = (lane > 0 || pass == 0) && valid >= own;
-        if (whole) st_stream(reinterpret_cast<void*>(a - off), pass ? shift_down(below, u, 16u - off) : u);
+        if (whole) put_vec(reinterpret_cast<void*>(a - off), pass ? shift_down(below, u, 16u - off) : u);
         // Elements no whole vector takes: the head of a warp's first lane, the tail of its last, the row's end.
         uint32_t single = whole ? 0u : (1u << own) - 1u;
         if (pass && (lane == 31 || above < own)) single |= ((1u << V) - 1u) & ~((1u << own) - 1u);
@@ -341,7 +349,7 @@ template <typename T, int NV, Form FORM, bool CTA, int kThreads>
 __global__ void __launch_bounds__(kThreads, (CTA || FORM == ALIGNED) && NV * Elem<T>::V == 8 ? 1024 / kThreads : 1)
     norm_fwd_kernel(const T* x, const T* res, const T* gate, const T* w1, const T* w2, Norm n, Chunks ch, T* y, T* h,
                     float* rstd) {
-    using R = Rows<T, NV, FORM, CTA>;
+    using R = Rows<T, NV, FORM, CTA, true>;
     using CH = typename R::CH;
     constexpr int P = R::P;
     __shared__ float buf[CTA ? 256 : 1];
@@ -447,7 +455,7 @@ __global__ void __launch_bounds__(kThreads)
                     const float* rstd, Norm n, Chunks ch, int stages, T* dx, T* dres, T* dgate, float* part1,
                     float* part2, float* partg) {
     static_assert(!RING || (CTA && FORM == ALIGNED), "the ring holds whole aligned rows");
-    using R = Rows<T, NV, FORM, CTA>;
+    using R = Rows<T, NV, FORM, CTA, false>;
     using CH = typename R::CH;
     constexpr int P = R::P;
     constexpr bool AHEAD = !RING && P == 4;
@@ -750,7 +758,16 @@ int norm_fwd(const nb200_norm_args& a, T* y, T* h, float* rstd, cudaStream_t st)
         // Units enough to fill the GPU (1024 threads of 64 registers on an SM, or 512 of 128), each with an equal share
         // of the rows.
         const int64_t ctas = (int64_t)sm_count() * std::max(1, (s.e == 8 ? 1024 : 512) / (s.threads * per));
-        const Chunks ch = make_chunks(n, n.rows, ctas * per, s.form == LINED ? l.step() : 1);
+        const int64_t target = ctas * per, multiple = s.form == LINED ? l.step() : 1;
+        Chunks ch = make_chunks(n, n.rows, target, multiple);  // a run of rows for each
+        // Better, all units of a gate group take turns row by row: together they sweep through neighbouring rows (bf16
+        // [16384, 4096] 99.6 us, runs 101.8; [8192, 8192] 104 and 107). Not where that makes a unit's share larger, nor
+        // across gate groups, whose activations it would compute anew every few rows (64 groups of 256: 150 us, runs
+        // 102). The backward, with more to fetch for each row, does not gain (bf16 [16384, 4096] 170.5 us, runs 168.7).
+        const int64_t group = n.group > 1 ? n.group : n.rows, all_units = target / (n.rows / group);
+        const Chunks turns = make_chunks(
+            n, group, target, std::max<int64_t>(1, std::min(all_units, group) / multiple) * multiple);
+        if (turns.rows <= ch.rows) ch = turns;
         kernel<<<(unsigned)((ch.count + per - 1) / per), dim3(s.threads, per), 0, st>>>(
             static_cast<const T*>(a.x), static_cast<const T*>(a.residual), static_cast<const T*>(a.gate),
             static_cast<const T*>(a.post_weight), static_cast<const T*>(a.pre_weight), n, ch, y, h, rstd);
