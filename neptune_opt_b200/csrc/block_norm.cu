@@ -36,10 +36,14 @@ struct Norm {
     int act;
 };
 
-// a(g), and its derivative in terms of a.
+// a(g), and its derivative in terms of a. The sigmoid's division is good to 2 ulp (and gives 0 where expf overflows):
+// a gate row for each row, bf16 [16384, 4096] forward 148 us, rounded exactly 161 us; fp32 [16384, 1000] backward
+// 103 us and 124 us. The fp32 forward kernel has no registers to spare and takes the exact one (EXACT), with which it
+// spills less inside its loop ([16384, 2048] 91 us, else 95 us).
+template <bool EXACT>
 __device__ __forceinline__ float gate_value(float g, int kind) {
     if (kind == NB200_GATE_TANH) return tanhf(g);
-    if (kind == NB200_GATE_SIGMOID) return 1.f / (1.f + expf(-g));
+    if (kind == NB200_GATE_SIGMOID) return EXACT ? 1.f / (1.f + expf(-g)) : __fdividef(1.f, 1.f + expf(-g));
     return g;
 }
 __device__ __forceinline__ float gate_slope(float a, int kind) {
@@ -99,10 +103,12 @@ struct Rows {
     __device__ __forceinline__ void line_up(const T* row) {
         if (FORM == LINED) lead = (int)((reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(T));
     }
-    __device__ __forceinline__ int col(int k) const { return (t + k * G) * V - (FORM == LINED ? lead : 0); }  // of vector k
+    __device__ __forceinline__ int col(int k) const { return (t + k * G) * V - (FORM == LINED ? lead : 0); }
     __device__ __forceinline__ int col_of(int i) const { return kScalar<T, FORM> ? t + i * G : col(i / V) + i % V; }
     __device__ __forceinline__ bool holds(int c) const { return c < width && (FORM != LINED || c >= 0); }
-    __device__ __forceinline__ static uint4 fetch(const void* p, bool stream) { return stream ? ld_stream(p) : ld_keep(p); }
+    __device__ __forceinline__ static uint4 fetch(const void* p, bool stream) {
+        return stream ? ld_stream(p) : ld_keep(p);
+    }
     // A row of one of the tensors the form speaks of; `finish` before use. (Clearing the partial vectors here would
     // make their warps wait for a prefetched row as soon as it is sent for.)
     __device__ __forceinline__ void load(CH& c, const T* row, bool stream) const {
@@ -320,7 +326,7 @@ Chunks make_chunks(const Norm& n, int64_t group, int64_t target, int64_t step) {
     Chunks c;
     c.step = step;
     const int64_t groups = n.rows / group;
-    if (groups < target || step > 1) {  // parts of a group, at most `target` in all unless that is less than `step` each
+    if (groups < target || step > 1) {  // parts of a group: at most `target` in all, or `step` for each group
         const int64_t turns = std::min((group + step - 1) / step, std::max<int64_t>(1, target / groups / step));
         c.group = group;
         c.rows = (group + turns * step - 1) / (turns * step);
@@ -334,15 +340,11 @@ Chunks make_chunks(const Norm& n, int64_t group, int64_t target, int64_t step) {
     return c;
 }
 
-// A gate row: laid out like the rows when every row has its own.
+// A gate row: laid out like the rows when every row has its own; `finish` before use.
 template <typename R, typename T>
 __device__ __forceinline__ void load_gate(const R& r, typename R::CH& c, const T* gate, const Norm& n, uint32_t index) {
-    if (n.group == 1) {
-        r.load(c, gate + index * n.sg, false);
-        r.finish(c);
-    } else {
-        r.load_shared(c, gate + index * n.sg);
-    }
+    if (n.group == 1) r.load(c, gate + index * n.sg, true);
+    else r.load_shared(c, gate + index * n.sg);
 }
 
 template <typename T, int NV, Form FORM, bool CTA, int kThreads>
@@ -373,10 +375,11 @@ __global__ void __launch_bounds__(kThreads, (CTA || FORM == ALIGNED) && NV * Ele
     uint64_t b[P];  // scale * a(gate) * post weight
     for (; row < end; row += ch.step) {
         if (fresh) {
+            if (gate) r.finish(cg);
 #pragma unroll
             for (int i = 0; i < P; ++i) {
-                const uint64_t a = gate ? f2(n.scale * gate_value(cg.get(2 * i), n.act),
-                                             n.scale * gate_value(cg.get(2 * i + 1), n.act))
+                const uint64_t a = gate ? f2(n.scale * gate_value<sizeof(T) == 4>(cg.get(2 * i), n.act),
+                                             n.scale * gate_value<sizeof(T) == 4>(cg.get(2 * i + 1), n.act))
                                         : f2(n.scale, n.scale);
                 b[i] = w1 ? mul2(a, c1.pair(i)) : a;
             }
@@ -442,11 +445,12 @@ __device__ __forceinline__ void store_part(float* part, const uint64_t* acc, con
 // Within a gate group the gate and post-weight gradients share one column sum, G = sum xhat dY:
 // dgate = scale a' w1 G and dw1 += scale a G.
 //
-// A row's four operands come through a ring of shared-memory stages filled by bulk copies (RING: the CTA form of
-// ALIGNED rows, where three stages fit), rows ahead of their use and without registers or issue slots; without a
-// ring the next row waits in registers (AHEAD). bf16 [16384, 4096]: 170 us with the ring, 181 us in registers;
-// with two stages it lost ([8192, 8192] 283 us against 238), and for LINED rows too ([16384, 3001] 202 against 193).
-// One CTA of 512 threads per SM either way: two, at 64 registers a thread, spilled (250 us).
+// A row's operands (its own gate row among them) come through a ring of shared-memory stages filled by bulk copies
+// (RING: the CTA form of ALIGNED rows, where the stages fit), rows ahead of their use and without registers or issue
+// slots; without a ring the next row waits in registers, where a thread's share of it is 8 elements (AHEAD). bf16
+// [16384, 4096]: 161 us with the ring, 179 us in registers. Two stages beat no prefetch (bf16 [8192, 8192] 228 us and
+// 243) but not registers (fp32 [4096, 4096] 103 us and 76), and LINED rows lost by a ring ([16384, 3001] 202 us
+// against 193). One CTA of 512 threads per SM either way: two, at 64 registers a thread, spilled (250 us).
 constexpr int kMaxRing = 4;
 
 template <typename T, int NV, Form FORM, bool CTA, bool RING, int kThreads>
@@ -474,16 +478,19 @@ __global__ void __launch_bounds__(kThreads)
     uint32_t row, end;
     ch.range(r.unit, n, row, end);
     r.line_up(x + row * n.sx);
-    // Stage s holds the vectors of x, residual, dy and dh that cover one row.
+    const bool own = gate && n.group == 1;  // a gate row for each row: it comes along with the row
+    // Stage s holds the vectors of x, residual, dy, dh and the gate that cover one row.
     uint8_t* ring = reinterpret_cast<uint8_t*>(bs - r.t + 3 * slots);
     const uint32_t bytes = r.width * (uint32_t)sizeof(T);
+    const uint32_t pitch = (own ? 5 : 4) * bytes;
     auto fill = [&](int s, uint32_t i) {  // one thread
-        uint8_t* to = ring + s * 4 * bytes;
-        mbar_expect_tx(&full[s], (2 + (dy ? 1 : 0) + (dh ? 1 : 0)) * bytes);
+        uint8_t* to = ring + s * pitch;
+        mbar_expect_tx(&full[s], (2 + (dy ? 1 : 0) + (dh ? 1 : 0) + (own ? 1 : 0)) * bytes);
         bulk_load(to, x + i * n.sx, bytes, &full[s]);
         bulk_load(to + bytes, res + i * n.sr, bytes, &full[s]);
         if (dy) bulk_load(to + 2 * bytes, dy + i * n.sdy, bytes, &full[s]);
         if (dh) bulk_load(to + 3 * bytes, dh + i * n.sdh, bytes, &full[s]);
+        if (own) bulk_load(to + 4 * bytes, gate + i * n.sg, bytes, &full[s]);
     };
     int stage = 0;
     uint32_t parity = 0;
@@ -499,7 +506,8 @@ __global__ void __launch_bounds__(kThreads)
         }
         __syncthreads();
     }
-    CH c2;
+    CH c1, c2;
+    if (w1) r.load_shared(c1, w1);
     if (w2) r.load_shared(c2, w2);
     uint64_t G[P], a2[P];
 #pragma unroll
@@ -509,7 +517,7 @@ __global__ void __launch_bounds__(kThreads)
     }
     uint32_t index = gate ? row / n.group : 0u;
     bool fresh = true;
-    CH nx, nr, ndy, ndh;
+    CH nx, nr, ndy, ndh, ng;
     float2 nrs;
     auto statistics = [&](uint32_t i) { nrs = *reinterpret_cast<const float2*>(rstd + 2 * (int64_t)i); };
     auto fetch = [&](uint32_t i) {
@@ -518,6 +526,7 @@ __global__ void __launch_bounds__(kThreads)
         r.load(nr, res + i * n.sr, true);
         if (dy) r.load(ndy, dy + i * n.sdy, true);
         if (dh) r.load(ndh, dh + i * n.sdh, true);
+        if (own) r.load(ng, gate + i * n.sg, true);
     };
     if (AHEAD && row < end) fetch(row);
     if (RING && row < end) statistics(row);
@@ -530,7 +539,7 @@ __global__ void __launch_bounds__(kThreads)
             auto staged = [&](CH& c, int i) {
 #pragma unroll
                 for (int k = 0; k < NV; ++k) {
-                    const uint4* p = reinterpret_cast<const uint4*>(ring + (stage * 4 + i) * bytes) + r.t + k * r.G;
+                    const uint4* p = reinterpret_cast<const uint4*>(ring + stage * pitch + i * bytes) + r.t + k * r.G;
                     c.raw[k] = r.col(k) < r.width ? *p : make_uint4(0u, 0u, 0u, 0u);
                 }
             };
@@ -538,6 +547,7 @@ __global__ void __launch_bounds__(kThreads)
             staged(nr, 1);
             if (dy) staged(ndy, 2);
             if (dh) staged(ndh, 3);
+            if (own) staged(ng, 4);
         }
         CH cx = nx, cr = nr, cdy = ndy, cdh = ndh;
         r.finish(cx);
@@ -546,12 +556,13 @@ __global__ void __launch_bounds__(kThreads)
         if (dh) r.finish(cdh);
         const float2 rs = nrs;
         if (fresh) {
-            CH c1, cg;
-            if (w1) r.load_shared(c1, w1);
-            if (gate) load_gate(r, cg, gate, n, index);
+            CH cg = ng;
+            if (gate && !own) load_gate(r, cg, gate, n, index);
+            if (gate) r.finish(cg);
 #pragma unroll
             for (int i = 0; i < P; ++i) {
-                const uint64_t v = gate ? f2(gate_value(cg.get(2 * i), n.act), gate_value(cg.get(2 * i + 1), n.act))
+                const uint64_t v = gate ? f2(gate_value<false>(cg.get(2 * i), n.act),
+                                             gate_value<false>(cg.get(2 * i + 1), n.act))
                                         : f2(1.f, 1.f);
                 const uint64_t a = mul2(v, f2(n.scale, n.scale));
                 as[i * r.G] = v;
@@ -576,7 +587,7 @@ __global__ void __launch_bounds__(kThreads)
         // Issued here, the loads cover the sums' latency.
         if (AHEAD && !last) fetch(next);
         if (RING && !last) statistics(next);
-        if (gate && next_index != index && !last && (r.t & 7) == 0)
+        if (gate && !own && next_index != index && !last && (r.t & 7) == 0)
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
                 if (r.holds(r.col(k)))
@@ -609,8 +620,6 @@ __global__ void __launch_bounds__(kThreads)
         // The end of a gate group, or of the chunk.
         fresh = gate && next_index != index;
         if (fresh || last) {
-            CH c1;
-            if (w1) r.load_shared(c1, w1);
 #pragma unroll
             for (int i = 0; i < P; ++i) {
                 const uint64_t a = as[i * r.G], g1 = mul2(G[i], f2(n.scale, n.scale));
@@ -833,9 +842,9 @@ int norm_bwd(const nb200_norm_args& a, const float* rstd, const T* dy, const T* 
             // What the CTAs that share an SM leave of its shared memory (228 KB, 1 KB of it reserved for each) beside
             // their accumulators and the kernel's own 1.1 KB.
             const int room = 233472 / std::max(1, 512 / s.threads) - 1024 - 1280 - smem;
-            const int stage = 4 * (int)n.width * es;
+            const int stage = (a.gate && n.group == 1 ? 5 : 4) * (int)n.width * es;
             stages = std::min(kMaxRing, room / stage);
-            if (stages >= 3) {
+            if (stages >= (s.e == 8 ? 3 : 2)) {
                 kernel = norm_bwd_kernel<T, kNV, kForm, kCta, true, kMost>;
                 smem += stages * stage;
             }
