@@ -23,13 +23,16 @@ constexpr int kMaxTop = 256;  // entries a row may keep
 constexpr float kL2e = 1.4426950408889634f;
 // A CTA of 256 threads takes a row, or a chunk of one (bf16 [4096, 131072] forward 164 us, 6.5 TB/s; 191 us with 512
 // and 175 us with 128). Narrow rows, where there are many, go to a warp each, kWarpRows of them in a CTA: there a CTA's
-// launch and barriers count for more than its loads (bf16, CTA -> warp: [8192, 1000] 39 -> 15 us forward, 30 -> 19 us
-// backward; [8192, 10007] 62 -> 40 us forward, but 81 -> 89 us backward). With fewer rows the warps leave SMs idle:
-// [1200, 5000] 9.7 -> 8.1 and 10.0 -> 8.7 us, but [600, 5000] 6.1 -> 6.8 and 5.5 -> 7.7 us.
+// launch and barriers count for more than its loads (CTA -> warp, forward: bf16 [8192, 1000] 39 -> 15 us,
+// [8192, 10007] 62 -> 40, [8192, 32001] 105 -> 99, fp32 [8192, 32000] 152 -> 164; backward: bf16 [8192, 1000] 30 -> 19,
+// [8192, 10007] 81 -> 89). With fewer rows the warps leave SMs idle: [1200, 5000] 9.7 -> 8.1 and 10.0 -> 8.7 us, but
+// [600, 5000] 6.1 -> 6.8 and 5.5 -> 7.7 us.
 constexpr int kWide = 256, kWarpRows = 8;
-constexpr int64_t kNarrowFwd = 16384, kNarrowBwd = 8192;  // columns
+constexpr int64_t kNarrowFwd = 65536, kNarrowBwd = 16384;  // bytes of a row
 
-bool narrow_rows(int64_t rows, int64_t vocab, int64_t most) { return vocab <= most && vocab <= 5 * rows; }
+bool narrow_rows(const nb200_distill_args& a, int64_t most, int64_t esize) {
+    return a.vocab * esize <= most && a.vocab <= 5 * a.rows;
+}
 
 // A barrier of the threads that share a row.
 template <int kThreads>
@@ -368,7 +371,7 @@ int launch_distill_fwd(const nb200_distill_args& a, const float* teacher_lse, fl
     const Row r = make_row(a);
     auto go = [&](auto* x) {
         using T = std::remove_const_t<std::remove_pointer_t<decltype(x)>>;
-        const bool narrow = narrow_rows(a.rows, a.vocab, kNarrowFwd);
+        const bool narrow = narrow_rows(a, kNarrowFwd, sizeof(T));
         const auto kernel = narrow ? distill_fwd_kernel<T, 32> : distill_fwd_kernel<T, kWide>;
         const int size = narrow ? 1 : cluster_for<T>(a.rows, a.vocab);
         if (size > 8) cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
@@ -402,7 +405,7 @@ int launch_distill_bwd(const nb200_distill_args& a, const float* grad, int64_t s
         const int64_t want = (4 * (int64_t)sm_count() + a.rows - 1) / a.rows, least = (a.vocab + kChunk - 1) / kChunk;
         const int64_t cut = std::max(least, std::min(want, a.vocab / kChunkLeast));
         const int64_t chunk = ((a.vocab + cut - 1) / cut + 63) / 64 * 64, chunks = (a.vocab + chunk - 1) / chunk;
-        const bool narrow = narrow_rows(a.rows, a.vocab, kNarrowBwd);
+        const bool narrow = narrow_rows(a, kNarrowBwd, sizeof(T));
         const auto kernel = narrow ? distill_bwd_kernel<T, 32> : distill_bwd_kernel<T, kWide>;
         const int64_t items = a.rows * chunks;
         kernel<<<(unsigned)(narrow ? (items + kWarpRows - 1) / kWarpRows : items),
