@@ -165,6 +165,21 @@ def test_absent_parts(without):
     _run_and_check(s, "bfloat16", label=without)
 
 
+@pytest.mark.parametrize("without", ["", "post", "pre", "gy", "gh"])
+@pytest.mark.parametrize("gate", ["none", "channel", "sequence", "full"])
+@pytest.mark.parametrize("shape,dtype", [((2, 1000, 1024), "bfloat16"), ((3, 400, 768), "float32"),
+                                         ((1, 701, 8192), "float16"), ((7, 200, 2056), "bfloat16")])
+def test_rows_fetched_ahead(shape, dtype, gate, without):
+    """Aligned rows, many for each CTA, so that every stage they pass through is used again."""
+    s = _make(shape, dtype, gate, 17)
+    if without:
+        s[without] = None
+    if s["pre"] is None:
+        s["gh"] = None
+    _run_and_check(s, dtype, "sigmoid" if gate == "full" else "tanh" if gate != "none" else "none", 0.7,
+                   label=f"{shape} {gate} without {without}")
+
+
 def test_many_rows_and_one_row():
     _run_and_check(_make((1, 128), "float32", "channel", 1), "float32", label="one row")
     _run_and_check(_make((40001, 72), "bfloat16", "channel", 2), "bfloat16", label="many rows")
