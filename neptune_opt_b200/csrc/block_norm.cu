@@ -76,7 +76,7 @@ struct Vecs {
 //           vectors it straddles, never one without a byte of the row; a store passes its last elements
 //           to the next lane, which writes the aligned vector they begin, and the few elements at the ends of a
 //           warp's span go one by one), fp32 rows go element by element, column t + i G.
-// bf16 [16384, 3001], backward: 193 us lined up, 427 us by shifted vectors, 795 us element by element.
+// bf16 [16384, 3001], backward: 195 us lined up, 427 us by shifted vectors, 795 us element by element.
 enum Form { ALIGNED, LINED, ANY };
 template <typename T, Form FORM>
 constexpr bool kScalar = FORM == ANY && sizeof(T) == 4;
@@ -450,7 +450,7 @@ __device__ __forceinline__ void store_part(float* part, const uint64_t* acc, con
 // slots; without a ring the next row waits in registers, where a thread's share of it is 8 elements (AHEAD). bf16
 // [16384, 4096]: 161 us with the ring, 179 us in registers. Two stages beat no prefetch (bf16 [8192, 8192] 228 us and
 // 243) but not registers (fp32 [4096, 4096] 103 us and 76), and LINED rows lost by a ring ([16384, 3001] 202 us
-// against 193). One CTA of 512 threads per SM either way: two, at 64 registers a thread, spilled (250 us).
+// against 195). One CTA of 512 threads per SM either way: two, at 64 registers a thread, spilled (250 us).
 constexpr int kMaxRing = 4;
 
 template <typename T, int NV, Form FORM, bool CTA, bool RING, int kThreads>
@@ -786,7 +786,7 @@ int norm_fwd(const nb200_norm_args& a, T* y, T* h, float* rstd, cudaStream_t st)
 }
 
 // 512 threads on every SM, about what fits one at a time, and one chunk for each unit of them: more chunks mean
-// more partial sums to write and add (bf16 [32768, 1024] 95 us, with twice as many 103). Gate groups of more than
+// more partial sums to write and add (bf16 [32768, 1024] 91 us, with twice as many 105). Gate groups of more than
 // one row stay apart, so that a unit's gate gradients are of one group, or of whole ones.
 int64_t bwd_target(const Shape& s) {
     return (int64_t)sm_count() * (s.cta ? std::max(1, 512 / s.threads) : 2 * kWarpRows);
