@@ -51,6 +51,17 @@ inline void launch_pdl(void (*kernel)(KArgs...), unsigned grid, unsigned block, 
     cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 
+// ------------------------------------------------------------------ clusters
+// A CTA may touch another's shared memory only once that CTA is known to run. Every thread arrives at
+// the kernel's entry, which waits for nothing, and waits just before the first remote access, when the
+// others have long arrived. A kernel of single CTAs (a cluster of one) may call both as well.
+__device__ __forceinline__ void cluster_arrive_started() {
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait_started() {
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 inline size_t dtype_size(int dtype) { return dtype == NB200_F32 ? 4 : 2; }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

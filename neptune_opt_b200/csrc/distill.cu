@@ -153,6 +153,7 @@ __global__ void __launch_bounds__(kWide)
     const uint32_t rank = kRows > 1 ? 0 : cluster_rank(), size = kRows > 1 ? 1 : cluster_size();
     const int64_t row = (int64_t)(blockIdx.x / size) * kRows + sub;
     if (kRows > 1 && row >= rows) return;
+    if (size > 1) cluster_arrive_started();
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const T* xr = x + row * stride;
     // The kept entries: t_j / T (-inf: not kept, its probability is 0) and x / T.
@@ -191,6 +192,7 @@ __global__ void __launch_bounds__(kWide)
         ec[warp] = acc.c;
         es[warp] = acc.s;
     }
+    if (size > 1) cluster_wait_started();
     row_sync<kThreads>();
     if (kThreads > 32 && warp == 0) {
         acc = LogSum{};
