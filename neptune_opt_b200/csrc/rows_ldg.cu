@@ -225,10 +225,10 @@ template int launch_ldg_span<__half>(int, const Params&, const __half*, int64_t,
 // cluster per row), each CTA folding a contiguous column range of the row with its 8 warps (4 KB
 // register sub-blocks and a running lane state, as the span kernel), its warps' states merged in
 // ascending warp order. The C CTA states then meet in the leader CTA's shared memory through
-// distributed shared memory (st.shared::cluster after mapa), one cluster barrier, and the leader
-// merges them in ascending CTA rank -- the split plan's certified order with the CTA ranges as
-// chunks -- and finalises. No scratch in global memory and no second launch; a single row is
-// spread over C SMs instead of one.
+// distributed shared memory (st.shared::cluster after mapa, once all of them are known to run), one
+// cluster barrier, and the leader merges them in ascending CTA rank -- the split plan's certified
+// order with the CTA ranges as chunks -- and finalises. No scratch in global memory and no second
+// launch; a single row is spread over C SMs instead of one.
 constexpr int kClThreads = 256;
 constexpr int kClWarps = kClThreads / 32;
 constexpr int kClMax = 16;
@@ -274,6 +274,7 @@ __global__ void __launch_bounds__(kClThreads) cluster_fold_kernel(const T* __res
     constexpr bool kFast = S == NB200_LOGSUMEXP && sizeof(T) == 2;
     __shared__ float4 cta_state[kClMax];
     __shared__ float4 warp_state[kClWarps];
+    cluster_arrive_started();
     pdl_wait();
     pdl_trigger();
     const uint32_t crank = cluster_rank(), csize = cluster_size();
@@ -297,6 +298,7 @@ __global__ void __launch_bounds__(kClThreads) cluster_fold_kernel(const T* __res
         const St w = warp_merge<S>(run, lane, p);
         if (lane == 0) warp_state[warp] = make_float4(w.m, w.acc, __int_as_float(w.seen), __int_as_float(w.status));
     }
+    cluster_wait_started();
     __syncthreads();
     if (threadIdx.x == 0) {
         St c = empty_state();
@@ -335,6 +337,7 @@ __global__ void __launch_bounds__(kClThreads) cluster_rms_kernel(const T* __rest
     constexpr int V = Elem<T>::V;
     __shared__ float part[kClMax];
     __shared__ float warp_sum_s[kClWarps];
+    cluster_arrive_started();
     pdl_wait();
     pdl_trigger();
     const uint32_t crank = cluster_rank(), csize = cluster_size();
@@ -370,6 +373,7 @@ __global__ void __launch_bounds__(kClThreads) cluster_rms_kernel(const T* __rest
     const unsigned long long a = add_f32x2(acc[0], acc[1]);
     const float t = warp_sum(__fadd_rn(lo_f(a), hi_f(a)));
     if ((threadIdx.x & 31) == 0) warp_sum_s[threadIdx.x >> 5] = t;
+    cluster_wait_started();
     __syncthreads();
     if (threadIdx.x < csize) {  // thread r sends this CTA's partial sum to cluster CTA r
         float cta = 0.f;
