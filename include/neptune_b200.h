@@ -326,7 +326,8 @@ int nb200_attention_bwd(const nb200_attn_args* args, const nb200_attn_strides* s
  * post weight), and h = pre_weight * y rsqrt(mean y^2 + eps) (not computed without a pre weight).
  * x and residual are [rows, width] with unit column stride; gate (nullable) holds one row per
  * rows_per_gate consecutive rows; weights are contiguous [width]; everything is of one dtype. y, h and
- * every gradient are contiguous. All of it is computed in fp32 and rounded once, h from the
+ * every gradient are contiguous; pointers need their elements' alignment only, and each its own (the
+ * rows move faster where all start on a 16-byte boundary, or alike). All of it is computed in fp32 and rounded once, h from the
  * unrounded y. rstd is fp32 [rows, 2], 8-byte aligned: the two reciprocal norms (1 where a weight is absent).
  * width <= 16384 (else NB200_ERR_CAPACITY); rows a multiple of rows_per_gate. No counterpart in the
  * reference, whose RMSNorm is forward only (neptune_codegen/emitters.py:549-627). */

@@ -165,6 +165,16 @@ struct Rows {
             }
         }
     }
+    // The gradient of a shared gate row: laid out by its own pointer, as load_shared's rows are.
+    __device__ __forceinline__ void store_shared(T* row, const uint64_t* v) const {
+        if constexpr (FORM != LINED) {
+            store(row, v);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 2 * P; ++i)
+                if (holds(col_of(i))) row[col_of(i)] = Elem<T>::from_f(i & 1 ? f2hi(v[i / 2]) : f2lo(v[i / 2]));
+        }
+    }
     // 16 bytes from byte `off` of lo:hi.
     __device__ __forceinline__ static uint4 shift_down(const uint4& lo, const uint4& hi, uint32_t off) {
         uint32_t w[7] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z};
@@ -627,7 +637,10 @@ __global__ void __launch_bounds__(kThreads)
                 G[i] = mul2(g1, f2(gate_slope(f2lo(a), n.act), gate_slope(f2hi(a), n.act)));
                 if (w1) G[i] = mul2(G[i], c1.pair(i));
             }
-            if (dgate && !partg) r.store(dgate + index * n.width, G);
+            if (dgate && !partg) {
+                if (own) r.store(dgate + index * n.width, G);
+                else r.store_shared(dgate + index * n.width, G);
+            }
             index = next_index;
             if (last) break;
 #pragma unroll
