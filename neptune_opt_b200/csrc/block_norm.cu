@@ -505,9 +505,12 @@ __global__ void __launch_bounds__(kThreads)
     int stage = 0;
     uint32_t parity = 0;
     bool primed = false;  // a row has been taken out of the ring
-    bool arrived = true;  // false once a wait has run out: the rest runs through without waiting
+    // A wait that ran out, for rows of even and odd number: written ahead of the row's barrier and read past it, so
+    // all threads stop at the same row.
+    __shared__ int ran_out[RING ? 2 : 1];
     if constexpr (RING) {
         if (threadIdx.x == 0) {
+            ran_out[0] = ran_out[1] = 0;
             for (int s = 0; s < stages; ++s) mbar_init(&full[s], 1);
             fence_barrier_init();
             fence_proxy_async();
@@ -545,7 +548,7 @@ __global__ void __launch_bounds__(kThreads)
         const bool last = next >= end;
         if (!AHEAD && !RING) fetch(row);
         if constexpr (RING) {
-            arrived = arrived && mbar_wait(&full[stage], parity);
+            if (!mbar_wait(&full[stage], parity)) ran_out[r.phase] = 1;
             auto staged = [&](CH& c, int i) {
 #pragma unroll
                 for (int k = 0; k < NV; ++k) {
@@ -606,6 +609,7 @@ __global__ void __launch_bounds__(kThreads)
         float t1 = f2lo(s1) + f2hi(s1), t2 = f2lo(s2) + f2hi(s2), t3 = f2lo(s3) + f2hi(s3);
         r.sum3(t1, t2, t3);
         if constexpr (RING) {
+            if (ran_out[r.phase ^ 1]) break;
             // Past the barrier in there, every thread is done with the previous row: its stage takes the row that is
             // `stages` behind it.
             const uint32_t ahead = row + (uint32_t)ch.step * (stages - 1);
@@ -647,9 +651,23 @@ __global__ void __launch_bounds__(kThreads)
             for (int i = 0; i < P; ++i) G[i] = 0;
         }
     }
-    if (RING && !arrived && threadIdx.x == 0)  // copies may still be on their way: wait for them, again with a limit
-        for (int s = 0; s < stages; ++s)
-            for (uint32_t ph = 0; ph < 2; ++ph) mbar_wait(&full[s], ph);
+    if (RING && (ran_out[0] | ran_out[1])) {
+        // This row and those behind it stay unwritten, and what was added up is no sum. What is on its way lands before
+        // the CTA may exit (again with a limit): this row's stage and those that were filled ahead.
+        if (threadIdx.x == 0)
+            for (int k = 0; k < stages - (primed ? 1 : 0) && row + k * (uint32_t)ch.step < end; ++k) {
+                mbar_wait(&full[stage], parity);
+                if (++stage == stages) {
+                    stage = 0;
+                    parity ^= 1u;
+                }
+            }
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            a2[i] = G[i] = f2(NB200_NAN, NB200_NAN);
+            a1[i * r.G] = a2[i];
+        }
+    }
     if (part2) store_part(part2 + r.unit * n.width, a2, r);
     if (part1) {
 #pragma unroll
