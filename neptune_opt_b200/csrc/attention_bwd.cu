@@ -568,7 +568,10 @@ struct Producer {
             }
             if (cut) {
                 if (!(ok = __all_sync(0xffffffffu, wait_bar(&b->tail, tail_ph, abort)))) {
-                    if (lane == 0) drain_bar(&b->tail, tail_ph);
+                    if (lane == 0) {
+                        drain_bar(&b->tail, tail_ph);
+                        if (kKeys && !second) drain_bar(&b->stat_full[i & 1], (i >> 1) & 1u);  // came with this tile
+                    }
                     return;
                 }
                 tail_ph ^= 1u;
@@ -668,7 +671,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_kernel(const __grid_cons
     // way to shared memory (1 to 2 us) then overlaps the allocation of the tensor memory.
     auto produce = [&](auto& p) {
         init_barriers(b, (smem_u32(smem) & 1023u) == 0, lane);  // the swizzled tiles need the alignment
-        if (lane == 0 && !b->abort) {
+        const bool issue = !b->abort;  // nobody else writes it before the CTA's first barrier
+        if (lane == 0 && issue) {
             uint8_t* own = smem + kOffOwn;
             mbar_expect_tx(&b->own, keys ? 2 * kTileBytes : kTileBytes);
             load_tile(own, keys ? &m.k : &m.q, row0, head, batch, &b->own);
@@ -676,10 +680,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_kernel(const __grid_cons
         }
         __syncwarp();
         if (keys) pdl_wait();
-        if (!b->abort) p.run(2, true, lane);  // the first step
+        if (issue) p.run(2, true, lane);  // the first step
         __syncwarp();
         cta_sync();
-        if (!b->abort) {
+        if (issue) {
             p.run(p.tiles, false, lane);
             p.drain(lane);
         }
