@@ -4,8 +4,6 @@
 
 #include <cudaTypedefs.h>
 
-#include <mutex>
-
 #include "common.cuh"
 #include "launch.h"
 #include "fastmath.cuh"
@@ -81,31 +79,6 @@ __device__ __forceinline__ void zero_tail(uint8_t* tile, int rows, int row, int 
 // ------------------------------------------------------------------ host side
 // cuTensorMapEncodeTiled, or null with an error recorded.
 PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder(const char* what);
-
-// Lets `kernel` use `bytes` of dynamic shared memory on the current device (done once per device and
-// kernel; `done` holds what was set).
-struct SharedLimit {
-    std::mutex mutex;
-    bool done[64] = {false};
-    template <typename K>
-    int raise(const char* what, K kernel, uint32_t bytes) {
-        int dev = 0;
-        if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
-            cudaGetLastError();
-            set_error("%s: no usable current CUDA device", what);
-            return NB200_ERR_LAUNCH;
-        }
-        std::lock_guard<std::mutex> lock(mutex);
-        if (done[dev]) return NB200_OK;
-        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) {
-            set_error("%s: cannot reserve %u bytes of shared memory: %s", what, bytes,
-                      cudaGetErrorString(cudaGetLastError()));
-            return NB200_ERR_LAUNCH;
-        }
-        done[dev] = true;
-        return NB200_OK;
-    }
-};
 
 // A [batch, heads, seq, 128] bf16 tensor as a 4-D tensor map with a {64, box_rows, 1, 1} box and
 // 128-byte swizzle. The stride of a dimension of one element is never used and may be anything.

@@ -462,6 +462,8 @@ __device__ __forceinline__ void store_part(float* part, const uint64_t* acc, con
 // 243) but not registers (fp32 [4096, 4096] 103 us and 76), and LINED rows lost by a ring ([16384, 3001] 202 us
 // against 195). One CTA of 512 threads per SM either way: two, at 64 registers a thread, spilled (250 us).
 constexpr int kMaxRing = 4;
+constexpr int kSmShared = 233472;  // shared memory of an SM, 228 KB
+constexpr int kCtaShared = 1024 + 1280;  // what is reserved for each CTA, and the kernel's own 1.1 KB
 
 template <typename T, int NV, Form FORM, bool CTA, bool RING, int kThreads>
 __global__ void __launch_bounds__(kThreads)
@@ -863,30 +865,37 @@ int norm_bwd(const nb200_norm_args& a, const float* rstd, const T* dy, const T* 
     float* p1 = dw1 ? work : nullptr;
     float* p2 = dw2 ? work + size : nullptr;
     float* pg = dgate && n.group > 1 && ch.per_group > 1 ? work + 2 * size : nullptr;
+    int rc = NB200_OK;
     dispatch(s, [&](auto cta, auto e, auto f, auto most) {
         constexpr int kNV = decltype(e)::value / Elem<T>::V, kMost = decltype(most)::value;
         constexpr Form kForm = decltype(f)::value;
         constexpr bool kCta = decltype(cta)::value;
         auto kernel = norm_bwd_kernel<T, kNV, kForm, kCta, false, kMost>;
         int smem = 3 * per * s.threads * decltype(e)::value * (int)sizeof(float), stages = 0;
+        constexpr uint32_t kSlots = 3 * kMost * decltype(e)::value * sizeof(float);  // the most of them
+        static SharedLimit limits[2];  // of this instance's two kernels
+        bool ring = false;
         if constexpr (kCta && kForm == ALIGNED && kMost == 512) {
-            // What the CTAs that share an SM leave of its shared memory (228 KB, 1 KB of it reserved for each) beside
-            // their accumulators and the kernel's own 1.1 KB.
-            const int room = 233472 / std::max(1, 512 / s.threads) - 1024 - 1280 - smem;
+            // What the CTAs that share an SM leave of its shared memory beside their accumulators.
+            const int room = kSmShared / std::max(1, 512 / s.threads) - kCtaShared - smem;
             const int stage = (a.gate && n.group == 1 ? 5 : 4) * (int)n.width * es;
             stages = std::min(kMaxRing, room / stage);
             if (stages >= (s.e == 8 ? 3 : 2)) {
                 kernel = norm_bwd_kernel<T, kNV, kForm, kCta, true, kMost>;
                 smem += stages * stage;
+                ring = true;
             }
         }
-        if (smem > 40 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (smem > 40 * 1024 &&
+            (rc = limits[ring].raise("nb200_gated_norm_bwd", kernel, ring ? kSmShared - kCtaShared : kSlots)))
+            return;
         kernel<<<(unsigned)((ch.count + per - 1) / per), dim3(s.threads, per), smem, st>>>(
             dy, dh, static_cast<const T*>(a.x), static_cast<const T*>(a.residual), static_cast<const T*>(a.gate),
             static_cast<const T*>(a.post_weight), static_cast<const T*>(a.pre_weight), rstd, n, ch, stages, dx, dres,
             dgate,
             p1, p2, pg);
     });
+    if (rc) return rc;
     count_launch();
     if (p1 || p2 || pg) {
         const Sums<T> sums = {{p1, p2, pg}, {dw1, dw2, dgate}, ch.count, ch.per_group, n.width};

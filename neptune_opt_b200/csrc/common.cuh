@@ -11,6 +11,7 @@
 #include <stdint.h>
 
 #include <atomic>
+#include <mutex>
 
 #include "../../include/neptune_b200.h"
 
@@ -279,6 +280,32 @@ __device__ __forceinline__ void store_vec(T* out_row, const float* f, int k, int
         }
     }
 }
+
+// Lets `kernel` use up to `bytes` of dynamic shared memory on the current device: done once per device
+// and kernel (`done` holds where), with the most any call of it asks for, so that no thread takes away
+// what another is about to launch with.
+struct SharedLimit {
+    std::mutex mutex;
+    bool done[64] = {false};
+    template <typename K>
+    int raise(const char* what, K kernel, uint32_t bytes) {
+        int dev = 0;
+        if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
+            cudaGetLastError();
+            set_error("%s: no usable current CUDA device", what);
+            return NB200_ERR_LAUNCH;
+        }
+        std::lock_guard<std::mutex> lock(mutex);
+        if (done[dev]) return NB200_OK;
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) {
+            set_error("%s: cannot reserve %u bytes of shared memory: %s", what, bytes,
+                      cudaGetErrorString(cudaGetLastError()));
+            return NB200_ERR_LAUNCH;
+        }
+        done[dev] = true;
+        return NB200_OK;
+    }
+};
 
 // Persistent grid: enough CTAs to fill every SM at the occupancy the kernel reaches.
 template <typename K>
