@@ -207,10 +207,10 @@ constexpr uint32_t kSmemBudget = 224 * 1024;
 inline uint32_t align_up(uint32_t v, uint32_t a) { return (v + a - 1) / a * a; }
 
 template <typename K>
-int ensure_smem(K kernel, uint32_t bytes) {
+int ensure_smem(K kernel, uint32_t bytes) {  // the same limit in every call: threads do not lower each other's
     static_assert(sizeof(K) > 0, "");
     if (bytes <= 48 * 1024) return NB200_OK;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBudget) != cudaSuccess) {
         cudaGetLastError();
         set_error("cannot reserve %u bytes of shared memory", bytes);
         return NB200_ERR_LAUNCH;

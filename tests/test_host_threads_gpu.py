@@ -44,3 +44,34 @@ def test_gated_norm_backward_of_several_widths():
     for t in threads:
         t.join()
     assert not wrong, wrong[:3]
+
+
+def test_streamed_softmax_of_several_widths():
+    """The same of the streaming row kernel."""
+    import torch
+
+    import neptune_opt_b200._lib as L
+
+    lib, wrong = L.load(), []
+    launch = L.launch_struct(L.VARIANT_STREAM)
+
+    def work(width):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            x = torch.randn(8, width, device="cuda")
+            y, lse = torch.empty_like(x), torch.empty(8, device="cuda")
+            p = [ctypes.c_void_p(t.data_ptr()) for t in (x, y, lse)]
+            st = ctypes.c_void_p(stream.cuda_stream)
+            for _ in range(3000):
+                rc = lib.nb200_softmax(0, p[0], 0, 8, width, width, 1, p[1], p[2], ctypes.byref(launch), st)
+                if rc:
+                    wrong.append((width, rc, L.last_error()))
+                    return
+            stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(w,)) for w in (1024, 2048, 4096, 5120, 6144, 3584)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong[:3]
