@@ -533,7 +533,8 @@ int nb200_attention_fwd(const nb200_attn_args* args, const nb200_attn_strides* s
 int64_t nb200_attention_bwd_work_bytes(const nb200_attn_args* args) {
     const nb200_attn_strides none[8] = {};
     const int rc = check_attention("nb200_attention_bwd", args, none, 0);
-    return rc ? rc : attention_bwd_work_bytes(*args);
+    if (rc) return rc;
+    return args->batch * args->heads * args->seq ? attention_bwd_work_bytes(*args) : 0;
 }
 
 int nb200_attention_bwd(const nb200_attn_args* args, const nb200_attn_strides* strides, const void* q, const void* k,
