@@ -474,8 +474,8 @@ struct NormInputs {
         if (present(gate)) {
             same_kind(*gate, x, what);
             TORCH_CHECK_VALUE(gate->dim() >= 1 && gate->size(-1) == x.size(-1), what, ": gate must be [..., width]");
-            a.rows_per_gate = rows_per_gate(x, *gate, what);
-            a.gate = row_input(*gate, rows / a.rows_per_gate, &a.stride_gate);
+            a.rows_per_gate = std::max<int64_t>(rows_per_gate(x, *gate, what), 1);  // x may have no rows
+            a.gate = row_input(*gate, gate->numel() / gate->size(-1), &a.stride_gate);
         }
         a.post_weight = weight(post, x, what);
         a.pre_weight = weight(pre, x, what);
@@ -517,7 +517,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> gated_nor
     const at::Tensor rstd = whole ? rstd_ : rstd_.clone(at::MemoryFormat::Contiguous);
     const void* dy = present(gy) ? in.like_x(*gy, x, &in.a.stride_grad_y, what) : nullptr;
     const void* dh = present(gh) ? in.like_x(*gh, x, &in.a.stride_grad_h, what) : nullptr;
-    auto fresh = [&](const OptTensor& t) { return present(t) ? at::empty(t->sizes(), t->options()) : at::Tensor(); };
+    auto fresh = [&](const OptTensor& t) {  // sums over no rows are zero
+        if (!present(t)) return at::Tensor();
+        return in.rows ? at::empty(t->sizes(), t->options()) : at::zeros(t->sizes(), t->options());
+    };
     at::Tensor dx = at::empty(x.sizes(), x.options()), dr = at::empty(x.sizes(), x.options());
     at::Tensor dgate = fresh(gate), dpost = fresh(post), dpre = fresh(pre);
     auto ptr = [](const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
