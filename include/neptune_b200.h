@@ -356,11 +356,11 @@ int nb200_gated_norm_bwd(const nb200_norm_args* args, int dtype, const float* rs
 /* ------------------------------------------------------------------ distillation loss
  * Per row: p_j = exp(teacher_j / T - Z) over the kept entries, Z = logsumexp of their teacher_j / T
  * (teacher_lse null) or teacher_lse[row]; q = softmax(x / T); loss = sum_j p_j (log p_j - log q at
- * index_j); stats = {logsumexp(x / T), Z, sum_j p_j}. An index outside [0, vocab) marks an entry
- * that is not kept; a row without kept entries has loss 0 and gradient 0. x is [rows, vocab] and
- * teacher, index [rows, top], unit column stride; top <= 256 (else NB200_ERR_CAPACITY). loss and
- * teacher_lse are fp32 [rows], stats fp32 [rows, 3], contiguous. Built on the reference's logsumexp
- * skeleton (neptune_codegen/library.py:19); the reference has no loss and no gradient. */
+ * index_j); stats = {logsumexp(x / T), Z, sum_j p_j}. An index outside [0, vocab), or a teacher logit
+ * of -inf, marks an entry that is not kept; a row without kept entries has loss 0 and gradient 0. x is
+ * [rows, vocab] and teacher, index [rows, top], unit column stride; top <= 256 (else
+ * NB200_ERR_CAPACITY). loss and teacher_lse are fp32 [rows], stats fp32 [rows, 3], contiguous. Built on
+ * the reference's logsumexp skeleton (neptune_codegen/library.py:19), which has no loss and no gradient. */
 typedef struct {
     const void *x, *teacher, *index;
     int64_t rows, vocab, top;

@@ -6,8 +6,8 @@
 //   loss = sum_j p_j (log p_j - log q[idx_j])
 //   dx_c = g / T * (mass q_c - sum_{j: idx_j = c} p_j),   mass = sum_j p_j
 //
-// An index outside [0, vocab) marks an entry that was not kept. A row without kept entries has loss 0
-// and gradient 0 whatever its logits hold.
+// An index outside [0, vocab) marks an entry that was not kept, and so does a teacher logit of -inf: its
+// probability is 0. A row without kept entries has loss 0 and gradient 0 whatever its logits hold.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -281,10 +281,12 @@ __global__ void __launch_bounds__(kWide)
     T* dr = dx + row * r.vocab + c0;
     bool mine = false;
     for (int j = t; j < (r.top + 3 & ~3); j += kThreads) {
-        const int64_t c = j < r.top ? r.at(row, j) : -1;
+        int64_t c = j < r.top ? r.at(row, j) : -1;
+        const float logit = c >= 0 ? r.logit(row, j) : -NB200_INF;
+        if (logit == -NB200_INF) c = -1;
         mine = mine || c >= 0;
         at[j] = c >= c0 && c < c0 + n ? (int)(c - c0) : -1;
-        p[j] = c >= 0 ? expf(r.logit(row, j) - z) : 0.f;
+        p[j] = c >= 0 ? expf(logit - z) : 0.f;
     }
     bool any;
     if constexpr (kThreads == 32) any = __any_sync(0xffffffffu, mine);

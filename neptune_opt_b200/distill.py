@@ -8,8 +8,9 @@ Per row of student logits x over the whole vocabulary, with kept teacher logits 
     loss = sum_j p_j (log p_j - log q[i_j])
     dx   = grad / T * (mass * q - scatter(p)),   mass = sum_j p_j
 
-An index outside [0, vocab) marks an entry that was not kept; a row without kept entries (a prompt
-token) has loss 0 and gradient 0 whatever its logits hold. Entries that name one column twice add.
+An index outside [0, vocab), or a teacher logit of -inf, marks an entry that was not kept; a row without
+kept entries (a prompt token) has loss 0 and gradient 0 whatever its logits hold. Entries that name one
+column twice add.
 The row's logsumexp is the reference's skeleton (neptune_codegen/library.py:19, :157); it has no loss
 and no gradient. Everything is fp32 inside; the gradient is rounded once to the logits' dtype.
 

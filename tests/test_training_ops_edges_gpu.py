@@ -44,3 +44,30 @@ def test_attention_and_distillation_ops_without_elements():
         assert loss.shape == (rows,) and stats.shape == (rows, 3) and not loss.any()
         dx = _ops().distill_loss_bwd(torch.ones(rows, device="cuda"), x, t, index, stats, 1.0)
         assert dx.shape == x.shape and not dx.any()
+
+
+@pytest.mark.parametrize("z", [False, True])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("rows,vocab", [(6, 500), (900, 300), (3, 70001)])
+def test_rows_whose_kept_teacher_logits_are_all_minus_infinity(rows, vocab, dtype, z):
+    """Rows padded with logits of -inf in place of index -1: loss and gradient are 0, whatever the student's logits
+    hold, and neighbouring rows are what they are without them. A CTA a row, a warp a row and a cluster a row."""
+    import math
+
+    import torch
+
+    import neptune_opt_b200 as NB
+    from test_distill_gpu import _make
+
+    x, t, index, grad = _make(rows, vocab, 8, dtype, 5)
+    lse = torch.logsumexp(t.float(), -1) + 0.2 if z else None
+    want, stats = NB.run_distill_loss(x, t, index, teacher_lse=lse)
+    dwant = NB.distill_loss_backward(grad, x, t, index, stats)
+    t[1::3] = -math.inf
+    index[1::3, 4:] = 0  # the usual padding: one column named again and again
+    x[1, 7] = math.nan
+    loss, stats = NB.run_distill_loss(x, t, index, teacher_lse=lse)
+    dx = NB.distill_loss_backward(grad, x, t, index, stats)
+    assert not loss[1::3].any() and not stats[1::3, 2].any() and not dx[1::3].any()
+    for first in (0, 2):
+        assert torch.equal(loss[first::3], want[first::3]) and torch.equal(dx[first::3], dwant[first::3])
