@@ -71,8 +71,9 @@ __device__ __forceinline__ int64_t lead(const T* p) {
 }
 
 // Running state of a row: s = sum of 2^(x scale - c) with scale = log2(e) / T and c the largest x scale so far,
-// rounded; c is the exact shift of every term, so its rounding costs nothing. A row of -inf alone keeps
-// c = -inf and s = 0.
+// rounded up; c is the exact shift of every term, so its rounding costs nothing, and no exponent is positive: rounded
+// to nearest, it can fall short of the product by more than fp32's 2^128 holds where a thread has met nothing but a
+// mask's -1e10 or below. A row of -inf alone keeps c = -inf and s = 0.
 struct LogSum {
     float c = -HUGE_VALF, s = 0.f;
     __device__ __forceinline__ static float shift(float c) { return c == -NB200_INF ? 0.f : c; }
@@ -98,7 +99,7 @@ struct LogSum {
             t1 = max3(t1, x[i + 2], x[i + 3]);
         }
         if (E % 4 == 0) t0 = max3(t0, x[E - 2], x[E - 1]);
-        const float top = fmaxf(c, fmaxf(t0, t1) * scale), m = shift(top);
+        const float top = fmaxf(c, __fmul_ru(fmaxf(t0, t1), scale)), m = shift(top);
         const uint64_t scale2 = f2(scale, scale), m2 = f2(-m, -m);
         uint64_t a0 = f2(s * ex2_ftz(c - m), 0.f), a1 = 0;
 #pragma unroll
@@ -112,7 +113,7 @@ struct LogSum {
         s = f2lo(a) + f2hi(a);
         c = top;
     }
-    __device__ __forceinline__ void add_one(float x, float scale) { merge(x * scale, x == -NB200_INF ? 0.f : 1.f); }
+    __device__ __forceinline__ void add_one(float x, float scale) { merge(__fmul_ru(x, scale), x == -NB200_INF ? 0.f : 1.f); }
 };
 
 // ------------------------------------------------------------------ forward
