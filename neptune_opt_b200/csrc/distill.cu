@@ -116,6 +116,22 @@ struct LogSum {
     __device__ __forceinline__ void add_one(float x, float scale) { merge(__fmul_ru(x, scale), x == -NB200_INF ? 0.f : 1.f); }
 };
 
+// Rows whose largest logit is that far from 0 (in base 2) are folded once more, by one warp: there c's own rounding
+// amounts to something. A mask that leaves a row nothing makes such rows, training does not.
+constexpr float kFar = 1048576.f;
+
+// The largest logit over T, and log sum exp((x - largest) / T), of a row with a finite largest logit; else NaN.
+template <typename T>
+__device__ __noinline__ float2 far_row(const T* x, int64_t vocab, float inv_t, int lane) {
+    float top = -NB200_INF, sum = 0.f;
+#pragma unroll 8
+    for (int64_t i = lane; i < vocab; i += 32) top = fmaxf(top, Elem<T>::to_f(x[i]));
+    top = warp_max(top);
+#pragma unroll 8
+    for (int64_t i = lane; i < vocab; i += 32) sum += expf((Elem<T>::to_f(x[i]) - top) * inv_t);
+    return make_float2(top * inv_t, logf(warp_sum(sum)));
+}
+
 // ------------------------------------------------------------------ forward
 // One cluster of CTAs per row (one CTA, or a warp, when there are rows enough): each folds a share of the row's 16-byte
 // vectors, the states meet in the first CTA's shared memory, and that CTA's first warp takes the kept
@@ -216,7 +232,13 @@ __global__ void __launch_bounds__(kWide)
     }
     if (warp != 0) return;
     // The first warp takes the kept entries.
-    const float lse = (acc.c + log2f(acc.s)) * 0.69314718055994531f;
+    // log sum exp(x / T) = base + rest, apart where the sum of both would lose what the rest says.
+    float base = 0.f, rest = (acc.c + log2f(acc.s)) * 0.69314718055994531f;
+    if (fabsf(acc.c) >= kFar && acc.c != -NB200_INF) {
+        const float2 far = far_row(xr, r.vocab, r.inv_t, lane);
+        base = far.x;
+        rest = far.y;
+    }
     float z;
     if (teacher_lse) {
         z = teacher_lse[row];
@@ -233,13 +255,13 @@ __global__ void __launch_bounds__(kWide)
         if (teach[j] == -NB200_INF) continue;
         const float q = expf(teach[j] - z);
         mass += q;
-        if (q != 0.f) l += q * ((teach[j] - z) - (stud[j] - lse));
+        if (q != 0.f) l += q * ((teach[j] - z) - ((stud[j] - base) - rest));
     }
     mass = warp_sum(mass);
     l = warp_sum(l);
     if (lane == 0) {
         loss[row] = l;
-        stats[3 * row] = lse;
+        stats[3 * row] = base + rest;
         stats[3 * row + 1] = z;
         stats[3 * row + 2] = mass;
     }

@@ -31,3 +31,44 @@ def test_part_of_the_vocabulary_masked(shape, dtype, temperature):
         index[i, 7] = vocab - 1 if i % 2 else -1
         t[i, 7] = t[i].min() - 1
     _run_and_check(x, t, index, grad, dtype, temperature, label=f"{shape} {dtype} {temperature}")
+
+
+@pytest.mark.parametrize("temperature", [1.0, 1.7, 2.0])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("rows,vocab", [(len(MASKS) + 8, 900), (900, 300), (len(MASKS) + 8, 70001)])
+def test_rows_that_a_mask_leaves_nothing(rows, vocab, dtype, temperature):
+    """All logits of a row are the mask (or its largest value): the student is uniform there, so the loss is
+    sum p log p + log of how many are level. That logarithm comes from an fp32 sum of equal terms, in chains of up to
+    1024 (2^-14); where no other path is taken, up to 2^20 in base 2, the logits themselves are held to 2^-24 of their
+    size, twice."""
+    import math
+
+    import torch
+
+    import neptune_opt_b200 as NB
+
+    x, t, index, _ = _make(rows, vocab, 8, dtype, 5)
+    info = torch.finfo(x.dtype)
+    want, wstats = NB.run_distill_loss(x, t, index, temperature=temperature)
+    masks = [m for m in MASKS if m >= info.min] + [info.min, info.max, 1e4]
+    for i, mask in enumerate(masks):
+        x[i] = mask
+    n = len(masks)
+    x[n] = -math.inf
+    x[n, :100] = info.min
+    index[n] = torch.arange(8, device="cuda")
+    x[n + 1] = -math.inf
+    x[n + 2] = -math.inf
+    x[n + 2, 5] = math.nan
+    x[n + 3, 5] = math.inf
+    loss, stats = NB.run_distill_loss(x, t, index, temperature=temperature)
+    p = torch.softmax(t.double() / temperature, -1)
+    for i in range(n + 1):
+        size = x[i, 0].abs().double().item() / temperature
+        ref = (p[i] * p[i].log()).sum().item() + math.log(100 if i == n else vocab)
+        tol = 2.0 ** -13 + (2.0 ** -22 * size if size * 1.45 < 2.0 ** 20 else 0.0)
+        assert abs(loss[i].item() - ref) <= tol, (i, x[i, 0].item(), loss[i].item(), ref, tol)
+        lse = x[i, 0].double().item() / temperature + math.log(100 if i == n else vocab)
+        assert abs(stats[i, 0].double().item() - lse) <= 2.0 ** -21 * abs(lse) + 2.0 ** -13, (i, x[i, 0].item())
+    assert stats[n + 1, 0] == -math.inf and stats[n + 2:n + 4, 0].isnan().all() and loss[n + 2:n + 4].isnan().all()
+    assert torch.equal(loss[n + 4:], want[n + 4:]) and torch.equal(stats[n + 4:], wstats[n + 4:])
