@@ -129,7 +129,7 @@ __device__ __noinline__ float2 far_row(const T* x, int64_t vocab, float inv_t, i
     top = warp_max(top);
 #pragma unroll 8
     for (int64_t i = lane; i < vocab; i += 32) sum += expf((Elem<T>::to_f(x[i]) - top) * inv_t);
-    return make_float2(top * inv_t, logf(warp_sum(sum)));
+    return make_float2(__fmul_rn(top, inv_t), logf(warp_sum(sum)));
 }
 
 // ------------------------------------------------------------------ forward
@@ -315,9 +315,10 @@ __global__ void __launch_bounds__(kWide)
     if constexpr (kThreads == 32) any = __any_sync(0xffffffffu, mine);
     else any = __syncthreads_or(mine);
     row_sync<kThreads>();
-    // w mass q, the difference taken before the change of base so that large logits keep their digits; a
-    // row without kept entries is 0 whatever its logits hold.
-    auto soft = [&](float f) { return any ? wm * ex2_ftz(fmaf(f, r.inv_t, -lse) * kL2e) : 0.f; };
+    // w mass q, the difference taken before the change of base so that large logits keep their digits, and from a
+    // rounded x / T as the forward pass's: an exact one less a lse of -1e30 is anything, up to 2^75. A row without kept
+    // entries is 0 whatever its logits hold.
+    auto soft = [&](float f) { return any ? wm * ex2_ftz((__fmul_rn(f, r.inv_t) - lse) * kL2e) : 0.f; };
     const int head = (int)min(lead(dr), (int64_t)n);
     const bool together = lead(xr) == lead(dr);  // both sides meet the same 16-byte boundaries
     const int nv = together ? (n - head) / V : 0;

@@ -72,3 +72,25 @@ def test_rows_that_a_mask_leaves_nothing(rows, vocab, dtype, temperature):
         assert abs(stats[i, 0].double().item() - lse) <= 2.0 ** -21 * abs(lse) + 2.0 ** -13, (i, x[i, 0].item())
     assert stats[n + 1, 0] == -math.inf and stats[n + 2:n + 4, 0].isnan().all() and loss[n + 2:n + 4].isnan().all()
     assert torch.equal(loss[n + 4:], want[n + 4:]) and torch.equal(stats[n + 4:], wstats[n + 4:])
+
+
+@pytest.mark.parametrize("temperature", [0.9, 1.0, 1.7, 3.0])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("rows,vocab", [(len(MASKS), 900), (900, 300)])
+def test_gradients_of_rows_that_a_mask_leaves_nothing(rows, vocab, dtype, temperature):
+    """The fp32 log-sum-exp of such a row says no more than the logits' size, so q is anything up to 1 there, and the
+    gradient at most grad / T (mass + sum p) = 2 grad / T."""
+    import torch
+
+    import neptune_opt_b200 as NB
+
+    x, t, index, grad = _make(rows, vocab, 8, dtype, 5)
+    plain = x.clone()
+    for i, mask in enumerate(MASKS):
+        x[i] = max(mask, -3e38 * min(temperature, 1.0))
+    _, stats = NB.run_distill_loss(x, t, index, temperature=temperature)
+    dx = NB.distill_loss_backward(grad, x, t, index, stats, temperature=temperature)
+    assert (dx.double().abs() <= 2.01 * grad.double().abs()[:, None] / temperature).all()
+    _, stats = NB.run_distill_loss(plain, t, index, temperature=temperature)
+    want = NB.distill_loss_backward(grad, plain, t, index, stats, temperature=temperature)
+    assert torch.equal(dx[len(MASKS):], want[len(MASKS):])
