@@ -37,7 +37,7 @@ import struct
 
 from neptune_opt_b200 import _lib, autotune
 from neptune_opt_b200.skeletons import SKELETONS, checked_params, param_defaults
-from neptune_opt_b200.template import (_on_device, _ptr, _row_last_layout, _validate_row_last,
+from neptune_opt_b200.template import (_is_metadata, _on_device, _ptr, _row_last_layout, _validate_row_last,
                                        current_stream, dtype_code, launch_reduction, launch_rms_norm,
                                        split_launch_shape, validate_plan, validate_rms_inputs)
 
@@ -78,10 +78,12 @@ def run_cxx(name: str, args: tuple, validate, *validate_args):
 
 
 def on_cuda(t) -> bool:
-    """A real (not fake, not meta) CUDA tensor with elements: what the kernels run on."""
+    """A real CUDA tensor (no fake, no meta one) with elements, whatever its Python type: what the kernels run on."""
     import torch
 
-    return type(t) in (torch.Tensor, torch.nn.Parameter) and t.is_cuda and t.numel() > 0
+    if type(t) not in (torch.Tensor, torch.nn.Parameter) and (not isinstance(t, torch.Tensor) or _is_metadata(t)):
+        return False
+    return t.is_cuda and t.numel() > 0
 
 
 def _tracing(*tensors) -> bool:

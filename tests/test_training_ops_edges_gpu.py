@@ -71,3 +71,48 @@ def test_rows_whose_kept_teacher_logits_are_all_minus_infinity(rows, vocab, dtyp
     assert not loss[1::3].any() and not stats[1::3, 2].any() and not dx[1::3].any()
     for first in (0, 2):
         assert torch.equal(loss[first::3], want[first::3]) and torch.equal(dx[first::3], dwant[first::3])
+
+
+def test_tensors_of_a_subclass_give_what_plain_ones_give():
+    import torch
+
+    import neptune_opt_b200 as NB
+
+    class Tagged(torch.Tensor):
+        pass
+
+    gen = torch.Generator(device="cuda").manual_seed(5)
+
+    def normal(*shape, dtype=torch.bfloat16):
+        return torch.randn(*shape, device="cuda", generator=gen).to(dtype)
+
+    def plain(t):
+        return t.as_subclass(torch.Tensor) if isinstance(t, torch.Tensor) else t
+
+    q, k, g = normal(2, 4, 90, 128), normal(2, 2, 90, 128), normal(2, 4, 90, 128)
+    x, r, gate, w, gy = normal(6, 9, 200), normal(6, 9, 200), normal(6, 1, 200), normal(200), normal(6, 9, 200)
+    logits, teacher = normal(9, 3001), normal(9, 8)
+    index = torch.randint(0, 3001, (9, 8), device="cuda", generator=gen)
+    weight = torch.rand(9, device="cuda", generator=gen)
+
+    def everything(kind):
+        def leaf(t):
+            return t.clone().as_subclass(kind).requires_grad_()
+
+        q_, k_, x_, r_, gate_, w_, l_ = (leaf(t) for t in (q, k, x, r, gate, w, logits))
+        o, lse = NB.attention(q_, k_, k_, causal=True, return_lse=True)
+        y, h = NB.gated_residual_norm(x_, r_, gate_, post_weight=w_, pre_weight=w_, gate_act="tanh")
+        loss = NB.distill_loss(l_, teacher.as_subclass(kind), index)
+        torch.autograd.backward([o, y, h, loss], [t.as_subclass(kind) for t in (g, gy, gy, weight)])
+        a = [t.as_subclass(kind) for t in (x, r, gate, w, logits, q, k, teacher)]
+        with torch.no_grad():
+            ys, hs, rstd = NB.run_gated_residual_norm(*a[:3], post_weight=a[3], pre_weight=a[3])
+            ls, stats = NB.run_distill_loss(a[4], a[7], index)
+            direct = (*NB.attention_backward(a[5], a[6], a[6], o, lse, g, causal=True),
+                      *NB.gated_residual_norm_backward(gy, None, *a[:3], rstd, post_weight=a[3], pre_weight=a[3]),
+                      NB.distill_loss_backward(weight, a[4], a[7], index, stats))
+        return [plain(t) for t in (o, lse, y, h, loss, q_.grad, k_.grad, x_.grad, r_.grad, gate_.grad, w_.grad, l_.grad,
+                                   ys, hs, rstd, ls, stats, *direct)]
+
+    want, got = everything(torch.Tensor), everything(Tagged)
+    assert len(got) == len(want) and all(torch.equal(a, b) for a, b in zip(got, want))

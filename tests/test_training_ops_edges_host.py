@@ -16,3 +16,46 @@ def test_attention_backward_needs_no_work_memory_for_an_empty_call(batch, heads,
     s = (L.NB200AttnStrides * 8)()
     null = ctypes.c_void_p(0)
     assert lib.nb200_attention_bwd(ctypes.byref(a), s, *[null] * 10, 0, null) == L.NB200_OK
+
+
+class _Reached(Exception):
+    """An op of the library was dispatched."""
+
+
+def _wrapper(*shape, dtype):
+    """A tensor of a subclass of its own that says it is on a CUDA device; its ops go to the subclass."""
+    import torch
+
+    class Wrapper(torch.Tensor):
+        @staticmethod
+        def __new__(cls):
+            return torch.Tensor._make_wrapper_subclass(cls, shape, dtype=dtype, device="cuda")
+
+        @classmethod
+        def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+            if func.namespace == "nb200":
+                raise _Reached(func)
+            raise NotImplementedError(func)
+
+    return Wrapper()
+
+
+def test_tensor_subclasses_reach_the_ops():
+    """A CUDA tensor is one whatever its Python type: its results come from the library, or its type refuses."""
+    import torch
+
+    import neptune_opt_b200 as NB
+
+    bf, f32 = torch.bfloat16, torch.float32
+    q, lse = _wrapper(1, 2, 8, 128, dtype=bf), _wrapper(1, 2, 8, dtype=f32)
+    x, w, rstd = _wrapper(4, 64, dtype=bf), _wrapper(64, dtype=bf), _wrapper(4, 2, dtype=f32)
+    t, i = _wrapper(4, 8, dtype=bf), _wrapper(4, 8, dtype=torch.int64)
+    loss, stats = _wrapper(4, dtype=f32), _wrapper(4, 3, dtype=f32)
+    for call in (lambda: NB.attention_backward(q, q, q, q, lse, q),
+                 lambda: NB.run_gated_residual_norm(x, x, pre_weight=w),
+                 lambda: NB.gated_residual_norm(x, x, post_weight=w),
+                 lambda: NB.gated_residual_norm_backward(x, None, x, x, None, rstd, post_weight=w),
+                 lambda: NB.run_distill_loss(x, t, i), lambda: NB.distill_loss(x, t, i),
+                 lambda: NB.distill_loss_backward(loss, x, t, i, stats)):
+        with pytest.raises(_Reached):
+            call()
