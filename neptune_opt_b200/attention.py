@@ -22,7 +22,7 @@ import math
 
 from neptune_opt_b200 import _lib
 from neptune_opt_b200.template import _is_metadata, _on_device, current_stream
-from neptune_opt_b200.torch_op import on_cuda, run_cxx
+from neptune_opt_b200.torch_op import run_cxx
 
 HEAD_DIMS = (128,)
 OP_NAME = "neptune_b200::attention"
@@ -58,6 +58,11 @@ def validate_attention_inputs(q, k, v, scale, seq_lens=None):
     if not (math.isfinite(s) and s > 0.0):
         raise ValueError(f"attention: scale must be finite and positive, got {scale}")
     return s
+
+
+def _scale(q, scale):
+    """The scale of a call, 1/sqrt(D) by default; what q is remains to be checked."""
+    return 1.0 / math.sqrt(max(q.shape[-1], 1)) if scale is None and getattr(q, "shape", ()) else scale
 
 
 def _rows(t):
@@ -120,14 +125,8 @@ def attention_backward(q, k, v, o, lse, grad_out, *, causal: bool = False, scale
 
     The probabilities are recomputed; dk and dv of a shared key/value head sum over its query heads.
     The result does not depend on scheduling. Gradients keep the memory layout of their inputs."""
-    import torch
-
-    if on_cuda(q):
-        sc = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
-        return run_cxx("attention_bwd", (q, k, v, o, lse, grad_out, seq_lens, causal, sc),
-                       _validate_backward, q, k, v, o, lse, grad_out, scale, seq_lens)
-    _validate_backward(q, k, v, o, lse, grad_out, scale, seq_lens)
-    return torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v)
+    return run_cxx("attention_bwd", q, (q, k, v, o, lse, grad_out, seq_lens, causal, _scale(q, scale)),
+                   _validate_backward, q, k, v, o, lse, grad_out, scale, seq_lens)
 
 
 def _validate_backward(q, k, v, o, lse, grad_out, scale, seq_lens):

@@ -19,7 +19,7 @@ from __future__ import annotations
 
 import math
 
-from neptune_opt_b200.torch_op import on_cuda, run_cxx
+from neptune_opt_b200.torch_op import distinct, run_cxx
 
 GATE_ACTS = {"none": 0, "tanh": 1, "sigmoid": 2}
 MAX_WIDTH = 16384
@@ -79,31 +79,22 @@ def run_gated_residual_norm(x, residual, gate=None, *, post_weight=None, pre_wei
                             residual_scale: float = 1.0, eps: float = 1e-6):
     """(y, h, rstd): fresh contiguous results in x's dtype (h is None without pre_weight) and the fp32
     reciprocal norms [..., 2] that the backward pass takes."""
-    import torch
-
-    contract = (x, residual, gate, post_weight, pre_weight, gate_act, residual_scale, eps)
-    if on_cuda(x):
-        return run_cxx("gated_norm", (x, residual, gate, post_weight, pre_weight, GATE_ACTS.get(gate_act, -1),
-                                      residual_scale, eps), validate_gated_norm_inputs, *contract)
-    validate_gated_norm_inputs(*contract)
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    h = torch.empty(x.shape, device=x.device, dtype=x.dtype) if pre_weight is not None else None
-    return y, h, torch.empty((*x.shape[:-1], 2), device=x.device, dtype=torch.float32)
+    y, h, rstd = run_cxx("gated_norm", x, (x, residual, gate, post_weight, pre_weight, GATE_ACTS.get(gate_act, -1),
+                                           residual_scale, eps), validate_gated_norm_inputs,
+                         x, residual, gate, post_weight, pre_weight, gate_act, residual_scale, eps)
+    return y, None if pre_weight is None else h, rstd
 
 
 def gated_residual_norm_backward(grad_y, grad_h, x, residual, gate, rstd, *, post_weight=None, pre_weight=None,
                                  gate_act: str = "none", residual_scale: float = 1.0):
     """(dx, dresidual, dgate, dpost_weight, dpre_weight) for the gradients of y and h (either may be
     None); None in the place of an input that is absent. dgate sums over the rows that share a gate row."""
-    import torch
-
-    contract = (grad_y, grad_h, x, residual, gate, rstd, post_weight, pre_weight, gate_act, residual_scale)
-    if on_cuda(x):
-        return run_cxx("gated_norm_bwd", (grad_y, grad_h, x, residual, gate, rstd, post_weight, pre_weight,
-                                          GATE_ACTS.get(gate_act, -1), residual_scale), _validate_backward, *contract)
-    _validate_backward(*contract)
-    return tuple(None if t is None else torch.zeros(t.shape, device=t.device, dtype=t.dtype)
-                 for t in (x, residual, gate, post_weight, pre_weight))
+    dx, dresidual, dgate, dpost, dpre = run_cxx(
+        "gated_norm_bwd", x, (grad_y, grad_h, x, residual, gate, rstd, post_weight, pre_weight,
+                              GATE_ACTS.get(gate_act, -1), residual_scale), _validate_backward,
+        grad_y, grad_h, x, residual, gate, rstd, post_weight, pre_weight, gate_act, residual_scale)
+    return (dx, dresidual, None if gate is None else dgate, None if post_weight is None else dpost,
+            None if pre_weight is None else dpre)
 
 
 def _validate_backward(grad_y, grad_h, x, residual, gate, rstd, post_weight, pre_weight, gate_act, residual_scale):
@@ -166,6 +157,6 @@ def gated_residual_norm(x, residual, gate=None, *, post_weight=None, pre_weight=
     tensors = (x, residual, gate, post_weight, pre_weight)
     if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
         validate_gated_norm_inputs(*tensors, gate_act, residual_scale, eps)
-        return _function().apply(*tensors, gate_act, residual_scale, eps)
+        return _function().apply(*distinct(*tensors), gate_act, residual_scale, eps)
     return run_gated_residual_norm(x, residual, gate, post_weight=post_weight, pre_weight=pre_weight,
                                    gate_act=gate_act, residual_scale=residual_scale, eps=eps)[:2]

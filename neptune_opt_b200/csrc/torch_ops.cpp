@@ -20,8 +20,8 @@
 //   segment_status_word(int device) -> Tensor      the per-device int32 word itself, for launches
 //                                                  made through the C ABI by other host code
 //   attention(Tensor q, Tensor k, Tensor v, bool causal, float scale) -> (Tensor o, Tensor lse)
-// The training operators (CUDA kernels only, which check the whole contract of the Python functions; an
-// absent optional result is an undefined tensor):
+// The training operators (their CUDA kernels check the whole contract of the Python functions; an absent
+// result is a tensor without elements, which graphs and packages can hold):
 //   attention_bwd(Tensor q, Tensor k, Tensor v, Tensor o, Tensor lse, Tensor grad_o, Tensor? seq_lens,
 //                 bool causal, float scale) -> (Tensor dq, Tensor dk, Tensor dv)
 //   gated_norm(Tensor x, Tensor residual, Tensor? gate, Tensor? post, Tensor? pre, int act, float scale,
@@ -349,13 +349,26 @@ void check_strided(const at::Tensor& t, const char* what) {
 }
 
 bool present(const OptTensor& t) { return t.has_value() && t->defined(); }
+// The result in the place of something absent.
+at::Tensor none_like(const at::Tensor& x) { return at::empty({0}, x.options()); }
 
-// t itself when the attention kernels' copies can read its rows (unit stride in a row, positive 16-byte
-// multiples between rows, heads and batch elements, 16-byte aligned base), else a contiguous copy.
+// Whether the attention kernels' copies can read rows of t's strides (unit stride in a row, positive 16-byte
+// multiples between rows, heads and batch elements); symbolic sizes too.
+bool rows_fit(const at::Tensor& t) {
+    const auto sizes = t.sym_sizes(), strides = t.sym_strides();
+    if (strides[3] != 1) return false;
+    for (int i = 0; i < 3; ++i)
+        if (sizes[i] > 1 && (strides[i] <= 0 || strides[i] % 8 != 0)) return false;
+    return true;
+}
+// t itself when the copies can read its rows (16-byte aligned base), else a contiguous copy.
 at::Tensor attn_rows(const at::Tensor& t) {
-    bool ok = t.stride(3) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
-    for (int i = 0; i < 3; ++i) ok = ok && (t.size(i) <= 1 || (t.stride(i) > 0 && t.stride(i) % 8 == 0));
+    const bool ok = rows_fit(t) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
     return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+// A gradient keeps the memory layout of its input.
+at::Tensor attn_grad(const at::Tensor& t) {
+    return rows_fit(t) ? at::empty_like(t) : at::empty_symint(t.sym_sizes(), t.options());
 }
 
 nb200_attn_strides attn_strides(const at::Tensor& t) { return {t.stride(0), t.stride(1), t.stride(2)}; }
@@ -381,7 +394,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_bwd_cuda(const at::Tens
     c10::cuda::CUDAGuard guard(q_.device());
     const at::Tensor q = attn_rows(q_), k = attn_rows(k_), v = attn_rows(v_), o = attn_rows(o_), go = attn_rows(go_);
     const at::Tensor lse = lse_.contiguous();
-    at::Tensor dq = at::empty_like(q), dk = at::empty_like(k), dv = at::empty_like(v);
+    at::Tensor dq = attn_grad(q_), dk = attn_grad(k_), dv = attn_grad(v_);
     nb200_attn_args a = {q.size(0), q.size(1), k.size(1), q.size(2), q.size(3), nullptr, causal ? 1 : 0, (float)scale};
     if (present(seq_lens)) {
         TORCH_CHECK_TYPE(seq_lens->scalar_type() == at::kInt, what, ": seq_lens must be int32");
@@ -492,12 +505,12 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> gated_norm_cuda(const at::Tensor&
     const char* what = "nb200.gated_norm";
     const NormInputs in(x, residual, gate, post, pre, act, scale, eps, what);
     c10::cuda::CUDAGuard guard(x.device());
-    at::Tensor y = at::empty(x.sizes(), x.options()), h;
-    if (present(pre)) h = at::empty(x.sizes(), x.options());
+    at::Tensor y = at::empty(x.sizes(), x.options());
+    at::Tensor h = present(pre) ? at::empty(x.sizes(), x.options()) : none_like(x);
     std::vector<int64_t> shape = lead_shape(x, false);
     shape.push_back(2);
     at::Tensor rstd = at::empty(shape, x.options().dtype(at::kFloat));
-    check(api().gated_norm(&in.a, in.dtype, y.data_ptr(), h.defined() ? h.data_ptr() : nullptr, rstd.data_ptr<float>(),
+    check(api().gated_norm(&in.a, in.dtype, y.data_ptr(), present(pre) ? h.data_ptr() : nullptr, rstd.data_ptr<float>(),
                            stream_of(x)),
           what);
     return {y, h, rstd};
@@ -518,17 +531,17 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> gated_nor
     const void* dy = present(gy) ? in.like_x(*gy, x, &in.a.stride_grad_y, what) : nullptr;
     const void* dh = present(gh) ? in.like_x(*gh, x, &in.a.stride_grad_h, what) : nullptr;
     auto fresh = [&](const OptTensor& t) {  // sums over no rows are zero
-        if (!present(t)) return at::Tensor();
+        if (!present(t)) return none_like(x);
         return in.rows ? at::empty(t->sizes(), t->options()) : at::zeros(t->sizes(), t->options());
     };
     at::Tensor dx = at::empty(x.sizes(), x.options()), dr = at::empty(x.sizes(), x.options());
     at::Tensor dgate = fresh(gate), dpost = fresh(post), dpre = fresh(pre);
-    auto ptr = [](const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+    auto ptr = [](const OptTensor& input, const at::Tensor& t) { return present(input) ? t.data_ptr() : nullptr; };
     const int64_t bytes = api().gated_norm_bwd_work_bytes(&in.a);
     if (bytes < 0) check((int)bytes, what);
     at::Tensor work = at::empty({std::max<int64_t>(bytes, 16)}, x.options().dtype(at::kByte));
     check(api().gated_norm_bwd(&in.a, in.dtype, rstd.data_ptr<float>(), dy, dh, dx.data_ptr(), dr.data_ptr(),
-                               ptr(dgate), ptr(dpost), ptr(dpre), work.data_ptr(), work.numel(), stream_of(x)),
+                               ptr(gate, dgate), ptr(post, dpost), ptr(pre, dpre), work.data_ptr(), work.numel(), stream_of(x)),
           what);
     return {dx, dr, dgate, dpost, dpre};
 }
@@ -644,6 +657,40 @@ std::tuple<at::Tensor, at::Tensor> attention_meta(const at::Tensor& q, const at:
     return {at::empty_symint(qs, q.options()),
             at::empty_symint(std::vector<c10::SymInt>(qs.begin(), qs.end() - 1), q.options().dtype(at::kFloat))};
 }
+// Of the training operators: the Python functions check the contract before a graph is traced.
+std::vector<c10::SymInt> lead_sym_shape_with(const at::Tensor& x, int64_t last) {
+    std::vector<c10::SymInt> v = lead_sym_shape(x, false);
+    v.emplace_back(last);
+    return v;
+}
+at::Tensor like_meta(const at::Tensor& x) { return at::empty_symint(x.sym_sizes(), x.options()); }
+at::Tensor like_meta(const OptTensor& t, const at::Tensor& x) { return present(t) ? like_meta(*t) : none_like(x); }
+std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_bwd_meta(const at::Tensor& q, const at::Tensor& k,
+                                                                  const at::Tensor& v, const at::Tensor&,
+                                                                  const at::Tensor&, const at::Tensor&,
+                                                                  const OptTensor&, bool, double) {
+    return {attn_grad(q), attn_grad(k), attn_grad(v)};
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor> gated_norm_meta(const at::Tensor& x, const at::Tensor&,
+                                                               const OptTensor&, const OptTensor&,
+                                                               const OptTensor& pre, int64_t, double, double) {
+    return {like_meta(x), present(pre) ? like_meta(x) : none_like(x),
+            at::empty_symint(lead_sym_shape_with(x, 2), x.options().dtype(at::kFloat))};
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> gated_norm_bwd_meta(
+    const OptTensor&, const OptTensor&, const at::Tensor& x, const at::Tensor&, const OptTensor& gate,
+    const at::Tensor&, const OptTensor& post, const OptTensor& pre, int64_t, double) {
+    return {like_meta(x), like_meta(x), like_meta(gate, x), like_meta(post, x), like_meta(pre, x)};
+}
+std::tuple<at::Tensor, at::Tensor> distill_loss_meta(const at::Tensor& x, const at::Tensor&, const at::Tensor&, double,
+                                                     const OptTensor&) {
+    const auto f32 = x.options().dtype(at::kFloat);
+    return {at::empty_symint(lead_sym_shape(x, false), f32), at::empty_symint(lead_sym_shape_with(x, 3), f32)};
+}
+at::Tensor distill_loss_bwd_meta(const at::Tensor&, const at::Tensor& x, const at::Tensor&, const at::Tensor&,
+                                 const at::Tensor&, double) {
+    return like_meta(x);
+}
 
 }  // namespace
 
@@ -758,4 +805,9 @@ TORCH_LIBRARY_IMPL(nb200, Meta, m) {
     m.impl("rms_norm", &rms_meta);
     m.impl("segment_pool", &segment_meta);
     m.impl("attention", &attention_meta);
+    m.impl("attention_bwd", &attention_bwd_meta);
+    m.impl("gated_norm", &gated_norm_meta);
+    m.impl("gated_norm_bwd", &gated_norm_bwd_meta);
+    m.impl("distill_loss", &distill_loss_meta);
+    m.impl("distill_loss_bwd", &distill_loss_bwd_meta);
 }

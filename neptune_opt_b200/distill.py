@@ -21,7 +21,7 @@ from __future__ import annotations
 
 import math
 
-from neptune_opt_b200.torch_op import on_cuda, run_cxx
+from neptune_opt_b200.torch_op import run_cxx
 
 MAX_TOP = 256
 
@@ -63,26 +63,15 @@ def run_distill_loss(logits, teacher_logits, teacher_index, *, temperature: floa
     """(loss [...], stats [..., 3]) in fp32; stats holds each row's logsumexp(logits / T), teacher
     normaliser Z and kept mass, which the backward pass takes. teacher_lse [...] is the teacher's
     logsumexp(t / T) over its whole vocabulary; without it the kept entries are normalised to mass 1."""
-    import torch
-
     contract = (logits, teacher_logits, teacher_index, temperature, teacher_lse)
-    if on_cuda(logits):
-        return run_cxx("distill_loss", contract, validate_distill_inputs, *contract)
-    validate_distill_inputs(*contract)
-    return (torch.empty(logits.shape[:-1], device=logits.device, dtype=torch.float32),
-            torch.empty((*logits.shape[:-1], 3), device=logits.device, dtype=torch.float32))
+    return run_cxx("distill_loss", logits, contract, validate_distill_inputs, *contract)
 
 
 def distill_loss_backward(grad, logits, teacher_logits, teacher_index, stats, *, temperature: float = 1.0):
     """Gradient of the logits (fresh, contiguous, their dtype) for the gradient of each row's loss, from
     the forward pass's stats."""
-    import torch
-
     contract = (grad, logits, teacher_logits, teacher_index, stats, temperature)
-    if on_cuda(logits):
-        return run_cxx("distill_loss_bwd", contract, _validate_backward, *contract)
-    _validate_backward(*contract)
-    return torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
+    return run_cxx("distill_loss_bwd", logits, contract, _validate_backward, *contract)
 
 
 def _validate_backward(grad, logits, teacher_logits, teacher_index, stats, temperature):

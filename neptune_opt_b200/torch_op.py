@@ -67,14 +67,28 @@ def cxx_op(name: str):
     return op
 
 
-def run_cxx(name: str, args: tuple, validate, *validate_args):
-    """A C++-registered op on real CUDA tensors. The op checks the whole contract, so a call costs no
-    Python checks; when it refuses, `validate` runs to raise the error in the function's own words."""
+def run_cxx(name: str, t, args: tuple, validate, *validate_args):
+    """A C++-registered op of t and others. On a real CUDA tensor t the op checks the whole contract, so a call
+    costs no Python checks; when it refuses, `validate` runs to raise the error in the function's own words.
+    On anything else `validate` comes first: it refuses tensors of other devices, and fake and meta ones go on
+    to the op's shape function, so that a graph traced through the call holds the op."""
+    if not on_cuda(t):
+        validate(*validate_args)
+        return cxx_op(name)(*args)
     try:
         return cxx_op(name)(*args)
     except (RuntimeError, TypeError, ValueError, NotImplementedError):
         validate(*validate_args)
         raise
+
+
+def distinct(*tensors) -> list:
+    """The tensors, one that comes again as a view of itself. (torch.compile keeps only one of the gradients of a
+    tensor that an autograd function takes in two places, as one weight for both norms.)"""
+    out = []
+    for t in tensors:
+        out.append(t.view_as(t) if t is not None and any(t is u for u in out) else t)
+    return out
 
 
 def on_cuda(t) -> bool:
