@@ -63,7 +63,7 @@ struct Api {
     decltype(&nb200_rms_norm) rms_norm;
     decltype(&nb200_segment_spans) segment_spans;
     decltype(&nb200_segment_pool) segment_pool;
-    decltype(&nb200_attention) attention;
+    decltype(&nb200_attention_fwd) attention_fwd;
     decltype(&nb200_attention_bwd_work_bytes) attention_bwd_work_bytes;
     decltype(&nb200_attention_bwd) attention_bwd;
     decltype(&nb200_gated_norm) gated_norm;
@@ -105,7 +105,7 @@ const Api& api() {
         bind(h, "nb200_rms_norm", a.rms_norm);
         bind(h, "nb200_segment_spans", a.segment_spans);
         bind(h, "nb200_segment_pool", a.segment_pool);
-        bind(h, "nb200_attention", a.attention);
+        bind(h, "nb200_attention_fwd", a.attention_fwd);
         bind(h, "nb200_attention_bwd_work_bytes", a.attention_bwd_work_bytes);
         bind(h, "nb200_attention_bwd", a.attention_bwd);
         bind(h, "nb200_gated_norm", a.gated_norm);
@@ -322,26 +322,7 @@ int64_t segment_status(int64_t device, bool clear) {
     return bits;
 }
 
-std::tuple<at::Tensor, at::Tensor> attention_cuda(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
-                                                  bool causal, double scale) {
-    check_cuda(q, "nb200.attention");
-    TORCH_CHECK_TYPE(q.scalar_type() == at::kBFloat16 && k.scalar_type() == at::kBFloat16 &&
-                         v.scalar_type() == at::kBFloat16,
-                     "nb200.attention: q, k, v must be bfloat16");
-    TORCH_CHECK_VALUE(q.dim() == 4 && q.sizes() == k.sizes() && q.sizes() == v.sizes(),
-                      "nb200.attention: q, k, v must share one [batch, heads, seq, head_dim] shape");
-    c10::cuda::CUDAGuard guard(q.device());
-    const at::Tensor qc = q.contiguous(), kc = k.contiguous(), vc = v.contiguous();
-    at::Tensor o = at::empty(q.sizes(), q.options());
-    at::Tensor lse = at::empty({q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
-    if (q.numel() == 0) return {o, lse};
-    check(api().attention(qc.data_ptr(), kc.data_ptr(), vc.data_ptr(), o.data_ptr(), lse.data_ptr<float>(), q.size(0),
-                          q.size(1), q.size(2), q.size(3), causal ? 1 : 0, (float)scale, stream_of(q)),
-          "nb200.attention");
-    return {o, lse};
-}
-
-// ------------------------------------------------------------------ training operators
+// ------------------------------------------------------------------ attention and the training operators
 using OptTensor = std::optional<at::Tensor>;
 
 void check_strided(const at::Tensor& t, const char* what) {
@@ -373,22 +354,54 @@ at::Tensor attn_grad(const at::Tensor& t) {
 
 nb200_attn_strides attn_strides(const at::Tensor& t) { return {t.stride(0), t.stride(1), t.stride(2)}; }
 
+// What the attention ops ask of q, k, v, symbolic sizes too: [batch, heads, seq, head_dim], k and v with a divisor of
+// q's heads.
+void check_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const char* what) {
+    for (const at::Tensor* t : {&q, &k, &v}) {
+        check_strided(*t, what);
+        TORCH_CHECK_TYPE(t->scalar_type() == at::kBFloat16, what, ": q, k, v must be bfloat16");
+        TORCH_CHECK_VALUE(t->dim() == 4 && t->device() == q.device(), what, ": q, k, v must be 4-D on one device");
+    }
+    const auto qs = q.sym_sizes(), ks = k.sym_sizes();
+    TORCH_CHECK_VALUE(ks == v.sym_sizes() && qs[0] == ks[0] && qs[2] == ks[2] && qs[3] == ks[3], what,
+                      ": the shapes of q, k, v differ");
+    TORCH_CHECK_VALUE(qs[1] == ks[1] || (ks[1] > 0 && qs[1] % ks[1] == 0), what, ": ", qs[1],
+                      " query heads cannot share ", ks[1], " key/value heads");
+}
+
+std::tuple<at::Tensor, at::Tensor> attention_cuda(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_,
+                                                  bool causal, double scale) {
+    const char* what = "nb200.attention";
+    check_cuda(q_, what);
+    check_attention(q_, k_, v_, what);
+    c10::cuda::CUDAGuard guard(q_.device());
+    const at::Tensor q = attn_rows(q_), k = attn_rows(k_), v = attn_rows(v_);
+    at::Tensor o = at::empty(q.sizes(), q.options());
+    at::Tensor lse = at::empty(q.sizes().slice(0, 3), q.options().dtype(at::kFloat));
+    const nb200_attn_args a = {q.size(0), q.size(1), k.size(1), q.size(2), q.size(3), nullptr, causal ? 1 : 0,
+                               (float)scale};
+    const nb200_attn_strides strides[4] = {attn_strides(q), attn_strides(k), attn_strides(v), attn_strides(o)};
+    check(api().attention_fwd(&a, strides, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+                              lse.data_ptr<float>(), stream_of(q)),
+          what);
+    return {o, lse};
+}
+
 std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_bwd_cuda(const at::Tensor& q_, const at::Tensor& k_,
                                                                   const at::Tensor& v_, const at::Tensor& o_,
                                                                   const at::Tensor& lse_, const at::Tensor& go_,
                                                                   const OptTensor& seq_lens, bool causal,
                                                                   double scale) {
     const char* what = "nb200.attention_bwd";
-    for (const at::Tensor* t : {&q_, &k_, &v_, &o_, &go_}) {
-        check_strided(*t, what);
-        TORCH_CHECK_TYPE(t->scalar_type() == at::kBFloat16, what, ": q, k, v, o, grad_o must be bfloat16");
-        TORCH_CHECK_VALUE(t->dim() == 4 && t->device() == q_.device(), what, ": tensors must be 4-D on one device");
-    }
     check_cuda(q_, what);
+    check_attention(q_, k_, v_, what);
+    for (const at::Tensor* t : {&o_, &go_}) {
+        check_strided(*t, what);
+        TORCH_CHECK_TYPE(t->scalar_type() == at::kBFloat16, what, ": o, grad_o must be bfloat16");
+        TORCH_CHECK_VALUE(t->device() == q_.device() && t->sizes() == q_.sizes(), what,
+                          ": o, grad_o must have the shape and device of q");
+    }
     TORCH_CHECK_TYPE(lse_.scalar_type() == at::kFloat, what, ": lse must be float32");
-    TORCH_CHECK_VALUE(q_.sizes() == o_.sizes() && q_.sizes() == go_.sizes() && k_.sizes() == v_.sizes() &&
-                          q_.size(0) == k_.size(0) && q_.size(2) == k_.size(2) && q_.size(3) == k_.size(3),
-                      what, ": shapes differ");
     TORCH_CHECK_VALUE(lse_.device() == q_.device() && lse_.sizes() == q_.sizes().slice(0, 3), what,
                       ": lse must be [batch, heads, seq]");
     c10::cuda::CUDAGuard guard(q_.device());
@@ -651,8 +664,9 @@ at::Tensor segment_meta(const at::Tensor& data, const at::Tensor& segments, bool
     for (size_t d = 1; d < ds.size(); ++d) shape.push_back(ds[d]);
     return at::empty_symint(shape, data.options());
 }
-std::tuple<at::Tensor, at::Tensor> attention_meta(const at::Tensor& q, const at::Tensor&, const at::Tensor&, bool,
+std::tuple<at::Tensor, at::Tensor> attention_meta(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, bool,
                                                   double) {
+    check_attention(q, k, v, "nb200.attention");
     const auto qs = q.sym_sizes();
     return {at::empty_symint(qs, q.options()),
             at::empty_symint(std::vector<c10::SymInt>(qs.begin(), qs.end() - 1), q.options().dtype(at::kFloat))};

@@ -99,3 +99,30 @@ def test_compiled_training_step():
 
     want, got = run(step), run(torch.compile(step, backend="aot_eager"))
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("layout", ["dense", "packed"])
+def test_attention_op_with_shared_heads(layout, tmp_path):
+    """The op a graph holds takes shared heads and strided tensors, eager, exported and packaged."""
+    import torch
+
+    import neptune_opt_b200 as NB
+    import neptune_opt_b200.aot as A
+
+    data = _inputs()
+    q, k, v = (data[n] for n in ("q", "k", "v"))
+    if layout == "packed":
+        q, k, v = torch.cat([q, k, v], 1).transpose(1, 2).contiguous().transpose(1, 2).split([4, 2, 2], 1)
+    op = NB.attention_op()
+
+    class Module(torch.nn.Module):
+        def forward(self, q, k, v):
+            return op(q, k, v, True, 0.1)
+
+    want = NB.attention(q, k, v, causal=True, scale=0.1, return_lse=True)
+    _same(op(q, k, v, True, 0.1), want)
+    ep = torch.export.export(Module(), (q, k, v))
+    _same(ep.module()(q, k, v), want)
+    for shims in (True, False):
+        package = A.compile_package(ep, str(tmp_path / f"attention{shims}.pt2"), shims=shims)
+        _same(torch._inductor.aoti_load_package(package)(q, k, v), want)

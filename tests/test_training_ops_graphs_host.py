@@ -130,3 +130,25 @@ def test_real_tensors_of_other_devices_are_still_refused():
         NB.run_gated_residual_norm(x, x, post_weight=torch.zeros(8))
     with pytest.raises(ValueError):
         NB.run_distill_loss(x, x, torch.zeros(2, 8, dtype=torch.int64))
+
+
+def test_the_attention_op_sees_what_its_kernel_takes():
+    """Shared key/value heads trace, and what no kernel takes is refused when it is traced, not when it runs."""
+    import torch
+
+    import neptune_opt_b200 as NB
+    import neptune_opt_b200.aot as A
+
+    A.load()
+
+    def meta(*shape, dtype=torch.bfloat16):
+        return torch.empty(*shape, dtype=dtype, device="meta")
+
+    q, k = meta(2, 8, 30, 128), meta(2, 2, 30, 128)
+    o, lse = NB.attention_op()(q, k, k, True, 0.1)
+    assert o.shape == q.shape and lse.shape == (2, 8, 30)
+    for bad in (meta(2, 3, 30, 128), meta(2, 2, 31, 128), meta(1, 2, 30, 128), meta(2, 30, 128), meta(2, 0, 30, 128)):
+        with pytest.raises(ValueError):
+            torch.ops.nb200.attention(q, bad, bad, True, 0.1)
+    with pytest.raises(TypeError):
+        torch.ops.nb200.attention(q, k.float(), k.float(), True, 0.1)
