@@ -21,8 +21,8 @@ import ctypes
 import math
 
 from neptune_opt_b200 import _lib
-from neptune_opt_b200.template import _is_metadata, _on_device, current_stream
-from neptune_opt_b200.torch_op import run_cxx
+from neptune_opt_b200.template import _on_device, current_stream
+from neptune_opt_b200.torch_op import cxx_op, distinct, run_cxx
 
 HEAD_DIMS = (128,)
 OP_NAME = "neptune_b200::attention"
@@ -65,18 +65,6 @@ def _scale(q, scale):
     return 1.0 / math.sqrt(max(q.shape[-1], 1)) if scale is None and getattr(q, "shape", ()) else scale
 
 
-def _rows(t):
-    """t itself when the kernels' copies can read its rows (unit stride in a row, 16-byte multiples
-    between rows, heads and batch elements, 16-byte aligned base), else a contiguous copy."""
-    import torch
-
-    sizes, strides = t.shape, t.stride()
-    if strides[3] == 1 and t.data_ptr() % 16 == 0 and all(
-            sizes[i] <= 1 or (strides[i] > 0 and strides[i] % 8 == 0) for i in range(3)):
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
-
-
 def _args(q, k, causal, scale, seq_lens):
     b, h, s, d = q.shape
     return _lib.NB200AttnArgs(b, h, k.shape[1], s, d, seq_lens.data_ptr() if seq_lens is not None else None,
@@ -88,7 +76,8 @@ def _strides(*tensors):
 
 
 def launch_attention(q, k, v, o, lse, *, causal: bool, scale: float, seq_lens=None) -> None:
-    """One nb200_attention_fwd call on the current stream of q's device."""
+    """One nb200_attention_fwd call into given tensors on the current stream of q's device (strides as the C entry
+    asks for them)."""
     lib = _lib.load()
     with _on_device(q.device):
         rc = lib.nb200_attention_fwd(ctypes.byref(_args(q, k, causal, scale, seq_lens)), _strides(q, k, v, o),
@@ -98,13 +87,9 @@ def launch_attention(q, k, v, o, lse, *, causal: bool, scale: float, seq_lens=No
 
 
 def _forward(q, k, v, causal, scale, seq_lens, with_lse):
-    import torch
-
-    o = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-    lse = torch.empty(q.shape[:-1], device=q.device, dtype=torch.float32) if with_lse else None
-    if not _is_metadata(q) and q.numel():
-        launch_attention(_rows(q), _rows(k), _rows(v), o, lse, causal=causal, scale=scale, seq_lens=seq_lens)
-    return o, lse
+    """(O, LSE or None). A graph traced through it holds the op."""
+    o, lse = cxx_op("attention_fwd")(q, k, v, seq_lens, causal, scale, with_lse)
+    return o, lse if with_lse else None
 
 
 def run_attention(q, k, v, *, causal: bool = False, scale=None, return_lse: bool = False, seq_lens=None):
@@ -114,7 +99,7 @@ def run_attention(q, k, v, *, causal: bool = False, scale=None, return_lse: bool
 
     sc = validate_attention_inputs(q, k, v, scale, seq_lens)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        o, lse = _function().apply(q, k, v, causal, sc, seq_lens)
+        o, lse = _function().apply(*distinct(q, k, v), causal, sc, seq_lens)
     else:
         o, lse = _forward(q, k, v, causal, sc, seq_lens, return_lse)
     return (o, lse) if return_lse else o

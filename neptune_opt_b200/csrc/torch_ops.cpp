@@ -22,6 +22,8 @@
 //   attention(Tensor q, Tensor k, Tensor v, bool causal, float scale) -> (Tensor o, Tensor lse)
 // The training operators (their CUDA kernels check the whole contract of the Python functions; an absent
 // result is a tensor without elements, which graphs and packages can hold):
+//   attention_fwd(Tensor q, Tensor k, Tensor v, Tensor? seq_lens, bool causal, float scale, bool with_lse)
+//              -> (Tensor o, Tensor lse)
 //   attention_bwd(Tensor q, Tensor k, Tensor v, Tensor o, Tensor lse, Tensor grad_o, Tensor? seq_lens,
 //                 bool causal, float scale) -> (Tensor dq, Tensor dk, Tensor dv)
 //   gated_norm(Tensor x, Tensor residual, Tensor? gate, Tensor? post, Tensor? pre, int act, float scale,
@@ -369,22 +371,37 @@ void check_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor&
                       " query heads cannot share ", ks[1], " key/value heads");
 }
 
-std::tuple<at::Tensor, at::Tensor> attention_cuda(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_,
-                                                  bool causal, double scale) {
-    const char* what = "nb200.attention";
+void check_seq_lens(const OptTensor& seq_lens, const at::Tensor& q, const char* what) {
+    if (!present(seq_lens)) return;
+    TORCH_CHECK_TYPE(seq_lens->scalar_type() == at::kInt, what, ": seq_lens must be int32");
+    TORCH_CHECK_VALUE(seq_lens->device() == q.device() && seq_lens->dim() == 1 && seq_lens->is_contiguous() &&
+                          seq_lens->sym_size(0) == q.sym_size(0),
+                      what, ": seq_lens must be contiguous [batch] on the device of q");
+}
+
+std::tuple<at::Tensor, at::Tensor> attention_fwd_cuda(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_,
+                                                      const OptTensor& seq_lens, bool causal, double scale,
+                                                      bool with_lse) {
+    const char* what = "nb200.attention_fwd";
     check_cuda(q_, what);
     check_attention(q_, k_, v_, what);
+    check_seq_lens(seq_lens, q_, what);
     c10::cuda::CUDAGuard guard(q_.device());
     const at::Tensor q = attn_rows(q_), k = attn_rows(k_), v = attn_rows(v_);
     at::Tensor o = at::empty(q.sizes(), q.options());
-    at::Tensor lse = at::empty(q.sizes().slice(0, 3), q.options().dtype(at::kFloat));
-    const nb200_attn_args a = {q.size(0), q.size(1), k.size(1), q.size(2), q.size(3), nullptr, causal ? 1 : 0,
-                               (float)scale};
+    const auto f32 = q.options().dtype(at::kFloat);
+    at::Tensor lse = with_lse ? at::empty(q.sizes().slice(0, 3), f32) : at::empty({0}, f32);
+    const nb200_attn_args a = {q.size(0), q.size(1), k.size(1), q.size(2), q.size(3),
+                               present(seq_lens) ? seq_lens->data_ptr<int32_t>() : nullptr, causal ? 1 : 0, (float)scale};
     const nb200_attn_strides strides[4] = {attn_strides(q), attn_strides(k), attn_strides(v), attn_strides(o)};
     check(api().attention_fwd(&a, strides, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
-                              lse.data_ptr<float>(), stream_of(q)),
+                              with_lse ? lse.data_ptr<float>() : nullptr, stream_of(q)),
           what);
     return {o, lse};
+}
+std::tuple<at::Tensor, at::Tensor> attention_cuda(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                                  bool causal, double scale) {
+    return attention_fwd_cuda(q, k, v, std::nullopt, causal, scale, true);
 }
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_bwd_cuda(const at::Tensor& q_, const at::Tensor& k_,
@@ -404,18 +421,13 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_bwd_cuda(const at::Tens
     TORCH_CHECK_TYPE(lse_.scalar_type() == at::kFloat, what, ": lse must be float32");
     TORCH_CHECK_VALUE(lse_.device() == q_.device() && lse_.sizes() == q_.sizes().slice(0, 3), what,
                       ": lse must be [batch, heads, seq]");
+    check_seq_lens(seq_lens, q_, what);
     c10::cuda::CUDAGuard guard(q_.device());
     const at::Tensor q = attn_rows(q_), k = attn_rows(k_), v = attn_rows(v_), o = attn_rows(o_), go = attn_rows(go_);
     const at::Tensor lse = lse_.contiguous();
     at::Tensor dq = attn_grad(q_), dk = attn_grad(k_), dv = attn_grad(v_);
     nb200_attn_args a = {q.size(0), q.size(1), k.size(1), q.size(2), q.size(3), nullptr, causal ? 1 : 0, (float)scale};
-    if (present(seq_lens)) {
-        TORCH_CHECK_TYPE(seq_lens->scalar_type() == at::kInt, what, ": seq_lens must be int32");
-        TORCH_CHECK_VALUE(seq_lens->device() == q.device() && seq_lens->dim() == 1 &&
-                              seq_lens->size(0) == q.size(0) && seq_lens->is_contiguous(),
-                          what, ": seq_lens must be contiguous [batch] on the device of q");
-        a.seq_lens = seq_lens->data_ptr<int32_t>();
-    }
+    if (present(seq_lens)) a.seq_lens = seq_lens->data_ptr<int32_t>();
     const nb200_attn_strides strides[8] = {attn_strides(q),  attn_strides(k),  attn_strides(v),  attn_strides(o),
                                            attn_strides(go), attn_strides(dq), attn_strides(dk), attn_strides(dv)};
     const int64_t bytes = api().attention_bwd_work_bytes(&a);
@@ -664,12 +676,18 @@ at::Tensor segment_meta(const at::Tensor& data, const at::Tensor& segments, bool
     for (size_t d = 1; d < ds.size(); ++d) shape.push_back(ds[d]);
     return at::empty_symint(shape, data.options());
 }
-std::tuple<at::Tensor, at::Tensor> attention_meta(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, bool,
-                                                  double) {
-    check_attention(q, k, v, "nb200.attention");
+std::tuple<at::Tensor, at::Tensor> attention_fwd_meta(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                                      const OptTensor& seq_lens, bool, double, bool with_lse) {
+    check_attention(q, k, v, "nb200.attention_fwd");
+    check_seq_lens(seq_lens, q, "nb200.attention_fwd");
     const auto qs = q.sym_sizes();
+    const auto f32 = q.options().dtype(at::kFloat);
     return {at::empty_symint(qs, q.options()),
-            at::empty_symint(std::vector<c10::SymInt>(qs.begin(), qs.end() - 1), q.options().dtype(at::kFloat))};
+            with_lse ? at::empty_symint(std::vector<c10::SymInt>(qs.begin(), qs.end() - 1), f32) : at::empty({0}, f32)};
+}
+std::tuple<at::Tensor, at::Tensor> attention_meta(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                                  bool causal, double scale) {
+    return attention_fwd_meta(q, k, v, std::nullopt, causal, scale, true);
 }
 // Of the training operators: the Python functions check the contract before a graph is traced.
 std::vector<c10::SymInt> lead_sym_shape_with(const at::Tensor& x, int64_t last) {
@@ -778,6 +796,8 @@ TORCH_LIBRARY(nb200, m) {
     m.def("segment_status(int device, bool clear) -> int", &segment_status);
     m.def("segment_status_word(int device) -> Tensor", &segment_status_word);
     m.def("attention(Tensor q, Tensor k, Tensor v, bool causal, float scale) -> (Tensor, Tensor)");
+    m.def("attention_fwd(Tensor q, Tensor k, Tensor v, Tensor? seq_lens, bool causal, float scale, bool with_lse) "
+          "-> (Tensor, Tensor)");
     m.def("attention_bwd(Tensor q, Tensor k, Tensor v, Tensor o, Tensor lse, Tensor grad_o, Tensor? seq_lens, "
           "bool causal, float scale) -> (Tensor, Tensor, Tensor)");
     m.def("gated_norm(Tensor x, Tensor residual, Tensor? gate, Tensor? post, Tensor? pre, int act, "
@@ -794,7 +814,7 @@ TORCH_LIBRARY(nb200, m) {
 // The training operators are their own gradients' building blocks: autograd records nothing for them (the
 // Python layer's autograd functions call them).
 TORCH_LIBRARY_IMPL(nb200, Autograd, m) {
-    for (const char* op : {"attention_bwd", "gated_norm", "gated_norm_bwd", "distill_loss", "distill_loss_bwd"})
+    for (const char* op : {"attention_fwd", "attention_bwd", "gated_norm", "gated_norm_bwd", "distill_loss", "distill_loss_bwd"})
         m.impl(op, torch::CppFunction::makeFallthrough());
 }
 
@@ -805,6 +825,7 @@ TORCH_LIBRARY_IMPL(nb200, CUDA, m) {
     m.impl("rms_norm", &rms_cuda);
     m.impl("segment_pool", &segment_cuda);
     m.impl("attention", &attention_cuda);
+    m.impl("attention_fwd", &attention_fwd_cuda);
     m.impl("attention_bwd", &attention_bwd_cuda);
     m.impl("gated_norm", &gated_norm_cuda);
     m.impl("gated_norm_bwd", &gated_norm_bwd_cuda);
@@ -819,6 +840,7 @@ TORCH_LIBRARY_IMPL(nb200, Meta, m) {
     m.impl("rms_norm", &rms_meta);
     m.impl("segment_pool", &segment_meta);
     m.impl("attention", &attention_meta);
+    m.impl("attention_fwd", &attention_fwd_meta);
     m.impl("attention_bwd", &attention_bwd_meta);
     m.impl("gated_norm", &gated_norm_meta);
     m.impl("gated_norm_bwd", &gated_norm_bwd_meta);

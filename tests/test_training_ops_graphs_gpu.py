@@ -19,7 +19,7 @@ def _inputs():
     return {"x": normal(4, 9, 200), "r": normal(4, 9, 200), "gate": normal(4, 1, 200), "w": normal(200),
             "logits": normal(9, 3001), "t": normal(9, 8), "row": torch.rand(9, device="cuda", generator=gen),
             "i": torch.randint(0, 3001, (9, 8), device="cuda", generator=gen),
-            "q": normal(2, 4, 90, 128), "k": normal(2, 2, 90, 128), "v": normal(2, 2, 90, 128), "g": normal(2, 4, 90, 128)}
+            "lens": torch.tensor([90, 33], dtype=torch.int32, device="cuda"), "q": normal(2, 4, 90, 128), "k": normal(2, 2, 90, 128), "v": normal(2, 2, 90, 128), "g": normal(2, 4, 90, 128)}
 
 
 def _modules():
@@ -48,7 +48,14 @@ def _modules():
             loss, stats = NB.run_distill_loss(logits, t, i, temperature=2.0)
             return loss, NB.distill_loss_backward(row, logits, t, i, stats, temperature=2.0)
 
-    return [Norm(), NormBackward(), Loss()]
+    class Attention(torch.nn.Module):
+        names = ("q", "k", "v", "g", "lens")
+
+        def forward(self, q, k, v, g, lens):
+            o, lse = NB.attention(q, k, v, causal=True, return_lse=True, seq_lens=lens)
+            return o, lse, NB.attention(q, q, q), *NB.attention_backward(q, k, v, o, lse, g, causal=True, seq_lens=lens)
+
+    return [Norm(), NormBackward(), Loss(), Attention()]
 
 
 def _same(a, b):
@@ -58,7 +65,7 @@ def _same(a, b):
     assert len(a) == len(b) and all(torch.equal(x, y) and x.stride() == y.stride() for x, y in zip(a, b))
 
 
-@pytest.mark.parametrize("which", [0, 1, 2])
+@pytest.mark.parametrize("which", [0, 1, 2, 3])
 def test_exported_compiled_and_packaged(which, tmp_path):
     import torch
 
@@ -99,6 +106,29 @@ def test_compiled_training_step():
 
     want, got = run(step), run(torch.compile(step, backend="aot_eager"))
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_compiled_attention_step():
+    """One projection as key and value: its gradient is the sum of both."""
+    import torch
+
+    import neptune_opt_b200 as NB
+
+    data = _inputs()
+
+    def run(f):
+        leaves = [data[n].clone().requires_grad_() for n in ("q", "k")]
+        o = f(*leaves)
+        o.backward(data["g"])
+        return [o.detach(), *(leaf.grad for leaf in leaves)]
+
+    def step(q, k):
+        return NB.attention(q, k, k, causal=True, seq_lens=data["lens"])
+
+    want = run(step)  # the first call makes the autograd function, which no graph holds
+    for backend in ("eager", "aot_eager"):
+        assert all(torch.equal(a, b) for a, b in zip(run(torch.compile(step, fullgraph=True, backend=backend)), want))
+        torch._dynamo.reset()
 
 
 @pytest.mark.parametrize("layout", ["dense", "packed"])

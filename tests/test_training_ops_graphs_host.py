@@ -152,3 +152,30 @@ def test_the_attention_op_sees_what_its_kernel_takes():
             torch.ops.nb200.attention(q, bad, bad, True, 0.1)
     with pytest.raises(TypeError):
         torch.ops.nb200.attention(q, k.float(), k.float(), True, 0.1)
+
+
+def test_attention_itself_exports():
+    """With everything the function takes: shared heads, lengths, the log-sum-exp, a symbolic batch."""
+    import torch
+
+    import neptune_opt_b200 as NB
+
+    _, e = _fakes()
+    q, k, lens = e(2, 4, 9, 128), e(2, 2, 9, 128), e(2, dtype=torch.int32)
+
+    class Plain(torch.nn.Module):
+        def forward(self, q, k, lens):
+            return NB.attention(q, k, k)
+
+    class Whole(torch.nn.Module):
+        def forward(self, q, k, lens):
+            return NB.attention(q, k, k, causal=True, scale=0.2, return_lse=True, seq_lens=lens)
+
+    batch = torch.export.Dim("batch", min=2, max=64)
+    for module, shapes in ((Plain(), [q.shape]), (Whole(), [q.shape, (2, 4, 9)])):
+        ep = torch.export.export(module, (q, k, lens), strict=False)
+        assert _ops(ep.graph) == ["nb200.attention_fwd.default"]
+        outputs = [n.meta["val"] for n in next(n for n in ep.graph.nodes if n.op == "output").args[0]]
+        assert [tuple(o.shape) for o in outputs] == [tuple(s) for s in shapes]
+        ep = torch.export.export(module, (q, k, lens), strict=False, dynamic_shapes=[{0: batch}] * 3)
+        assert _ops(ep.graph) == ["nb200.attention_fwd.default"]
