@@ -43,6 +43,7 @@
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/VariableTypeUtils.h>
 #include <torch/csrc/inductor/aoti_torch/utils.h>
 #include <torch/library.h>
 
@@ -812,10 +813,18 @@ TORCH_LIBRARY(nb200, m) {
 }
 
 // The training operators are their own gradients' building blocks: autograd records nothing for them (the
-// Python layer's autograd functions call them).
+// Python layer's autograd functions call them). A tangent of forward mode would be lost that way: it is refused.
+static void below_autograd(const c10::OperatorHandle& op, c10::DispatchKeySet keys, torch::jit::Stack* stack) {
+    for (const c10::IValue& v : torch::jit::last(*stack, op.schema().arguments().size()))
+        TORCH_CHECK_NOT_IMPLEMENTED(!v.isTensor() || !torch::autograd::isFwGradDefined(v.toTensor()),
+                                    op.schema().name(), " has no forward-mode derivative");
+    at::AutoDispatchBelowADInplaceOrView guard;
+    op.redispatchBoxed(keys & c10::after_ADInplaceOrView_keyset, stack);
+}
 TORCH_LIBRARY_IMPL(nb200, Autograd, m) {
-    for (const char* op : {"attention_fwd", "attention_bwd", "gated_norm", "gated_norm_bwd", "distill_loss", "distill_loss_bwd"})
-        m.impl(op, torch::CppFunction::makeFallthrough());
+    for (const char* op : {"attention_fwd", "attention_bwd", "gated_norm", "gated_norm_bwd", "distill_loss",
+                           "distill_loss_bwd"})
+        m.impl(op, torch::CppFunction::makeFromBoxedFunction<&below_autograd>());
 }
 
 TORCH_LIBRARY_IMPL(nb200, CUDA, m) {

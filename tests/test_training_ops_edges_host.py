@@ -59,3 +59,30 @@ def test_tensor_subclasses_reach_the_ops():
                  lambda: NB.distill_loss_backward(loss, x, t, i, stats)):
         with pytest.raises(_Reached):
             call()
+
+
+def test_forward_mode_is_refused():
+    """The operators have no tangents; a dual tensor is refused, not stripped of its own."""
+    import torch
+    import torch.autograd.forward_ad as forward
+
+    import neptune_opt_b200 as NB
+
+    def meta(*shape, dtype=torch.bfloat16):
+        return torch.empty(*shape, dtype=dtype, device="meta")
+
+    q, lse = meta(1, 2, 8, 128), meta(1, 2, 8, dtype=torch.float32)
+    x, w, rstd, t, i = meta(4, 64), meta(64), meta(4, 2, dtype=torch.float32), meta(4, 8), meta(4, 8, dtype=torch.int64)
+    row, stats = meta(4, dtype=torch.float32), meta(4, 3, dtype=torch.float32)
+    calls = [(q, lambda d: NB.attention(d, q, q)), (q, lambda d: NB.attention(q, q, d)),
+             (q, lambda d: NB.attention_backward(q, q, q, q, lse, d)),
+             (x, lambda d: NB.gated_residual_norm(d, x, pre_weight=w)), (w, lambda d: NB.gated_residual_norm(x, x, d, pre_weight=w)),
+             (x, lambda d: NB.run_gated_residual_norm(x, d, post_weight=w)),
+             (x, lambda d: NB.gated_residual_norm_backward(d, None, x, x, None, rstd, post_weight=w)),
+             (x, lambda d: NB.distill_loss(d, t, i)), (t, lambda d: NB.run_distill_loss(x, d, i)),
+             (row, lambda d: NB.distill_loss_backward(d, x, t, i, stats))]
+    for a, call in calls:
+        call(a)
+        for leaf in (a, a.clone().requires_grad_()):
+            with forward.dual_level(), pytest.raises((NotImplementedError, RuntimeError)):
+                call(forward.make_dual(leaf, torch.ones_like(a)))
