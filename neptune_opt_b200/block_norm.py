@@ -89,12 +89,18 @@ def gated_residual_norm_backward(grad_y, grad_h, x, residual, gate, rstd, *, pos
                                  gate_act: str = "none", residual_scale: float = 1.0):
     """(dx, dresidual, dgate, dpost_weight, dpre_weight) for the gradients of y and h (either may be
     None); None in the place of an input that is absent. dgate sums over the rows that share a gate row."""
-    dx, dresidual, dgate, dpost, dpre = run_cxx(
+    return _backward((True, True, True), grad_y, grad_h, x, residual, gate, rstd, post_weight, pre_weight, gate_act,
+                     residual_scale)
+
+
+def _backward(wanted, grad_y, grad_h, x, residual, gate, rstd, post_weight, pre_weight, gate_act, residual_scale):
+    """The gradients; of gate, post_weight and pre_weight those that are wanted, None for the others."""
+    dx, dresidual, *sums = run_cxx(
         "gated_norm_bwd", x, (grad_y, grad_h, x, residual, gate, rstd, post_weight, pre_weight,
-                              GATE_ACTS.get(gate_act, -1), residual_scale), _validate_backward,
+                              GATE_ACTS.get(gate_act, -1), residual_scale, *wanted), _validate_backward,
         grad_y, grad_h, x, residual, gate, rstd, post_weight, pre_weight, gate_act, residual_scale)
-    return (dx, dresidual, None if gate is None else dgate, None if post_weight is None else dpost,
-            None if pre_weight is None else dpre)
+    return (dx, dresidual, *(d if want and t is not None else None
+                             for want, t, d in zip(wanted, (gate, post_weight, pre_weight), sums)))
 
 
 def _validate_backward(grad_y, grad_h, x, residual, gate, rstd, post_weight, pre_weight, gate_act, residual_scale):
@@ -139,9 +145,8 @@ def _function():
         @torch.autograd.function.once_differentiable
         def backward(ctx, grad_y, grad_h):
             x, residual, gate, post_weight, pre_weight, rstd = ctx.saved_tensors
-            grads = gated_residual_norm_backward(grad_y, grad_h, x, residual, gate, rstd, post_weight=post_weight,
-                                                 pre_weight=pre_weight, gate_act=ctx.gate_act,
-                                                 residual_scale=ctx.residual_scale)
+            grads = _backward(ctx.needs_input_grad[2:5], grad_y, grad_h, x, residual, gate, rstd, post_weight,
+                              pre_weight, ctx.gate_act, ctx.residual_scale)
             return (*grads, None, None, None)
 
     _FUNCTION = GatedResidualNorm

@@ -29,7 +29,8 @@
 //   gated_norm(Tensor x, Tensor residual, Tensor? gate, Tensor? post, Tensor? pre, int act, float scale,
 //              float eps) -> (Tensor y, Tensor h, Tensor rstd)
 //   gated_norm_bwd(Tensor? grad_y, Tensor? grad_h, Tensor x, Tensor residual, Tensor? gate, Tensor rstd,
-//                  Tensor? post, Tensor? pre, int act, float scale)
+//                  Tensor? post, Tensor? pre, int act, float scale, bool want_gate=True, bool want_post=True,
+//                  bool want_pre=True)
 //              -> (Tensor dx, Tensor dresidual, Tensor dgate, Tensor dpost, Tensor dpre)
 //   distill_loss(Tensor x, Tensor teacher, Tensor index, float temperature, Tensor? teacher_lse)
 //              -> (Tensor loss, Tensor stats)
@@ -544,7 +545,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> gated_norm_cuda(const at::Tensor&
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> gated_norm_bwd_cuda(
     const OptTensor& gy, const OptTensor& gh, const at::Tensor& x, const at::Tensor& residual, const OptTensor& gate,
-    const at::Tensor& rstd_, const OptTensor& post, const OptTensor& pre, int64_t act, double scale) {
+    const at::Tensor& rstd_, const OptTensor& post, const OptTensor& pre, int64_t act, double scale, bool want_gate,
+    bool want_post, bool want_pre) {
     const char* what = "nb200.gated_norm_bwd";
     NormInputs in(x, residual, gate, post, pre, act, scale, 1.0, what);
     c10::cuda::CUDAGuard guard(x.device());
@@ -556,18 +558,20 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> gated_nor
     const at::Tensor rstd = whole ? rstd_ : rstd_.clone(at::MemoryFormat::Contiguous);
     const void* dy = present(gy) ? in.like_x(*gy, x, &in.a.stride_grad_y, what) : nullptr;
     const void* dh = present(gh) ? in.like_x(*gh, x, &in.a.stride_grad_h, what) : nullptr;
-    auto fresh = [&](const OptTensor& t) {  // sums over no rows are zero
-        if (!present(t)) return none_like(x);
+    auto fresh = [&](const OptTensor& t, bool want) {  // sums over no rows are zero
+        if (!present(t) || !want) return none_like(x);
         return in.rows ? at::empty(t->sizes(), t->options()) : at::zeros(t->sizes(), t->options());
     };
     at::Tensor dx = at::empty(x.sizes(), x.options()), dr = at::empty(x.sizes(), x.options());
-    at::Tensor dgate = fresh(gate), dpost = fresh(post), dpre = fresh(pre);
-    auto ptr = [](const OptTensor& input, const at::Tensor& t) { return present(input) ? t.data_ptr() : nullptr; };
+    at::Tensor dgate = fresh(gate, want_gate), dpost = fresh(post, want_post), dpre = fresh(pre, want_pre);
+    auto ptr = [](const OptTensor& t, bool want, const at::Tensor& d) {
+        return present(t) && want ? d.data_ptr() : nullptr;
+    };
     const int64_t bytes = api().gated_norm_bwd_work_bytes(&in.a);
     if (bytes < 0) check((int)bytes, what);
     at::Tensor work = at::empty({std::max<int64_t>(bytes, 16)}, x.options().dtype(at::kByte));
     check(api().gated_norm_bwd(&in.a, in.dtype, rstd.data_ptr<float>(), dy, dh, dx.data_ptr(), dr.data_ptr(),
-                               ptr(gate, dgate), ptr(post, dpost), ptr(pre, dpre), work.data_ptr(), work.numel(), stream_of(x)),
+                               ptr(gate, want_gate, dgate), ptr(post, want_post, dpost), ptr(pre, want_pre, dpre), work.data_ptr(), work.numel(), stream_of(x)),
           what);
     return {dx, dr, dgate, dpost, dpre};
 }
@@ -712,8 +716,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> gated_norm_meta(const at::Tensor&
 }
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> gated_norm_bwd_meta(
     const OptTensor&, const OptTensor&, const at::Tensor& x, const at::Tensor&, const OptTensor& gate,
-    const at::Tensor&, const OptTensor& post, const OptTensor& pre, int64_t, double) {
-    return {like_meta(x), like_meta(x), like_meta(gate, x), like_meta(post, x), like_meta(pre, x)};
+    const at::Tensor&, const OptTensor& post, const OptTensor& pre, int64_t, double, bool want_gate, bool want_post,
+    bool want_pre) {
+    return {like_meta(x), like_meta(x), want_gate ? like_meta(gate, x) : none_like(x),
+            want_post ? like_meta(post, x) : none_like(x), want_pre ? like_meta(pre, x) : none_like(x)};
 }
 std::tuple<at::Tensor, at::Tensor> distill_loss_meta(const at::Tensor& x, const at::Tensor&, const at::Tensor&, double,
                                                      const OptTensor&) {
@@ -804,7 +810,8 @@ TORCH_LIBRARY(nb200, m) {
     m.def("gated_norm(Tensor x, Tensor residual, Tensor? gate, Tensor? post, Tensor? pre, int act, "
           "float scale, float eps) -> (Tensor, Tensor, Tensor)");
     m.def("gated_norm_bwd(Tensor? grad_y, Tensor? grad_h, Tensor x, Tensor residual, Tensor? gate, Tensor rstd, "
-          "Tensor? post, Tensor? pre, int act, float scale) "
+          "Tensor? post, Tensor? pre, int act, float scale, bool want_gate=True, bool want_post=True, "
+          "bool want_pre=True) "
           "-> (Tensor, Tensor, Tensor, Tensor, Tensor)");
     m.def("distill_loss(Tensor x, Tensor teacher, Tensor index, float temperature, Tensor? teacher_lse) "
           "-> (Tensor, Tensor)");

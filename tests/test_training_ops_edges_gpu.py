@@ -116,3 +116,30 @@ def test_tensors_of_a_subclass_give_what_plain_ones_give():
 
     want, got = everything(torch.Tensor), everything(Tagged)
     assert len(got) == len(want) and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("frozen", ["gate", "post", "pre", "gate post pre"])
+@pytest.mark.parametrize("gate", ["channel", "sequence", "full"])
+def test_frozen_weights_leave_the_other_gradients_what_they_are(gate, frozen):
+    import torch
+
+    import neptune_opt_b200 as NB
+    from test_block_norm_gpu import _make
+
+    s = _make((5, 70, 384), "bfloat16", gate, 8)
+    names = ("x", "residual", "gate", "post", "pre")
+
+    def grads(frozen):
+        leaves = {n: s[n].clone().requires_grad_(n not in frozen) for n in names}
+        y, h = NB.gated_residual_norm(leaves["x"], leaves["residual"], leaves["gate"], post_weight=leaves["post"],
+                                      pre_weight=leaves["pre"], gate_act="tanh")
+        torch.cuda.synchronize()
+        before = NB.launch_count()
+        torch.autograd.backward([y, h], [s["gy"], s["gh"]])
+        return {n: leaf.grad for n, leaf in leaves.items()}, NB.launch_count() - before
+
+    want, launches = grads(())
+    got, fewer = grads(frozen.split())
+    for n in names:
+        assert got[n] is None if n in frozen.split() else torch.equal(got[n], want[n]), n
+    assert launches == 2 and fewer == (1 if len(frozen.split()) == 3 else 2)

@@ -86,3 +86,25 @@ def test_forward_mode_is_refused():
         for leaf in (a, a.clone().requires_grad_()):
             with forward.dual_level(), pytest.raises((NotImplementedError, RuntimeError)):
                 call(forward.make_dual(leaf, torch.ones_like(a)))
+
+
+def test_gradients_nobody_wants_are_not_made():
+    """Frozen weights and a constant gate: the backward pass asks for no sums, and makes no tensor of them."""
+    import torch
+
+    import neptune_opt_b200 as NB
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    def step(x, gate, w, train):
+        leaf = x.detach().requires_grad_()
+        w = w.detach().requires_grad_(train)
+        y, h = NB.gated_residual_norm(leaf, x, gate, post_weight=w, pre_weight=w.detach())
+        return torch.autograd.grad(h.sum() + y.sum(), [leaf, w] if train else [leaf])
+
+    x, w = torch.empty(4, 64, device="meta"), torch.empty(64, device="meta")
+    for train in (False, True):
+        graph = make_fx(lambda a, b, c: step(a, b, c, train))(x, x, w).graph
+        node = next(n for n in graph.nodes if "gated_norm_bwd" in str(n.target))
+        wanted = (list(node.args[10:]) + [True] * 3)[:3]
+        assert wanted == [False, train, False]
+        assert [tuple(v.shape) for v in node.meta["val"]] == [(4, 64), (4, 64), (0,), (64,) if train else (0,), (0,)]
