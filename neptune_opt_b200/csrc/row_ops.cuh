@@ -119,8 +119,8 @@ struct SoftmaxOp {
 
     // softmax of an fp32 row held whole in registers: the exponentials of the sum pass are kept
     // (over the row's own registers) and scaled by 1/sum for the output, so every element takes
-    // one exponential instead of two. Rows with a NaN or an infinity return false and take the
-    // general path below (exact status semantics).
+    // one exponential instead of two. Rows with a NaN, an infinity or a far maximum return false and
+    // take the general path below (exact status semantics).
     template <class Src>
     __device__ __forceinline__ bool softmax_in_registers(const Src& src, int64_t r, int lane) const {
         constexpr int NV = sizeof(src.r) / sizeof(uint4);
@@ -137,6 +137,7 @@ struct SoftmaxOp {
         }
         if (!__all_sync(0xffffffffu, probe == 0.f)) return false;
         const float m = warp_max(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+        if (far_max(m)) return false;
         const float nm = -m * kLog2e;
         uint4 e[NV];
         float acc[4] = {0.f, 0.f, 0.f, 0.f};

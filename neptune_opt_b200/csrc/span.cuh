@@ -30,8 +30,8 @@ __device__ __forceinline__ void load_block(RegRow<NV>& b, const uint4* base, int
         b.r[k] = (lane + 32 * k < b.nv) ? ld_stream(base + v0 + lane + 32 * k) : make_uint4(0u, 0u, 0u, 0u);
 }
 
-// 16-bit logsumexp sub-block: packed max with NaN propagation (a NaN or +inf in the block sends it
-// to the exact path), an online rescale of the lane's running sum when the block raises its max,
+// 16-bit logsumexp sub-block: packed max with NaN propagation (a NaN, +inf or far maximum in the block
+// sends it to the exact path), an online rescale of the lane's running sum when the block raises its max,
 // and 2^(x log2 e - m log2 e) on packed fp32 pairs. (Moving a share of the exponentials to an
 // FMA-pipe polynomial was measured slower here: this loop is bound by instruction issue, not by
 // the special-function unit.)
@@ -66,7 +66,7 @@ __device__ __forceinline__ void lse16_block(const RegRow<NV>& blk, St& run, cons
     });
     const uint64_t m2 = widen2<T>(max_nan2<T>(max_nan2<T>(mw[0], mw[1]), max_nan2<T>(mw[2], mw[3])));
     const float bm = fmaxf(f2lo(m2), f2hi(m2));
-    if (f2lo(m2) != f2lo(m2) || f2hi(m2) != f2hi(m2) || bm == NB200_INF) {  // NaN or +inf: exact status
+    if (f2lo(m2) != f2lo(m2) || f2hi(m2) != f2hi(m2) || far_max(bm)) {  // NaN, +inf or a far maximum: exact
         run = merge_fast<NB200_LOGSUMEXP>(run, lane_state<NB200_LOGSUMEXP, T>(blk, p), p);
         return;
     }
@@ -97,8 +97,8 @@ __device__ __forceinline__ void lse16_block(const RegRow<NV>& blk, St& run, cons
 // States of G whole 16-bit logsumexp items resident in `blk[g]`, each formed as row_state forms a
 // resident row (warp max first, every exponential against it, one warp sum; no repair) on packed
 // pairs: max.NaN on raw 16-bit pairs, exponent arguments and sums on fp32 pairs. The G items'
-// reductions interleave (one shuffle chain for all of them). A NaN or +inf anywhere in any of them
-// sends the warp to the exact lane-state merge for each item.
+// reductions interleave (one shuffle chain for all of them). A NaN, +inf or far maximum in any lane's
+// part of them sends the warp to the exact lane-state merge for each item.
 template <typename T, int NV, int G>
 __device__ __forceinline__ void lse16_rows_state(const RegRow<NV> (&blk)[G], St (&out)[G], const Params& p) {
     const uint32_t ninf = std::is_same<T, __half>::value ? 0xFC00FC00u : 0xFF80FF80u;
@@ -115,7 +115,7 @@ __device__ __forceinline__ void lse16_rows_state(const RegRow<NV> (&blk)[G], St 
         });
         const uint64_t m2 = widen2<T>(max_nan2<T>(max_nan2<T>(mw[0], mw[1]), max_nan2<T>(mw[2], mw[3])));
         m[g] = fmaxf(f2lo(m2), f2hi(m2));
-        exact |= f2lo(m2) != f2lo(m2) || f2hi(m2) != f2hi(m2) || m[g] == NB200_INF;
+        exact |= f2lo(m2) != f2lo(m2) || f2hi(m2) != f2hi(m2) || far_max(m[g]);
     }
     if (__any_sync(0xffffffffu, exact)) {
 #pragma unroll

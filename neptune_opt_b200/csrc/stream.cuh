@@ -85,6 +85,13 @@ constexpr float kLog2e = 1.4426950408889634f;
 // e^d for the fold's terms and repairs: exp(d) = 2^(d log2 e).
 __device__ __forceinline__ float fexp(float d) { return ex2(d * kLog2e); }
 
+// 2^(x log2 e - m log2 e) takes one multiply-add an element, from a product m log2 e that is rounded. Where the
+// maximum is this far from 0 (a lane, or a row, that a mask of -1e9 or below leaves nothing), that rounding is no
+// longer small against 1 (2^9 at 1e10, 2^76 at 1e30: infinite terms, and inf * 0 = NaN where states meet), and
+// terms are taken from x - m instead.
+constexpr float kFarMax = 1048576.f;
+__device__ __forceinline__ bool far_max(float m) { return fabsf(m) >= kFarMax && m != -NB200_INF; }
+
 // Per-lane state of the elements this lane holds in a staged block of `nv` 16-byte vectors
 // (vectors lane, lane + 32, ...). Same algebra as chunk_state, with the reductions lane-local.
 // Every reduction keeps V independent partials (one per position inside a 16-byte vector) so the
@@ -148,7 +155,7 @@ __device__ __forceinline__ St lane_state(const Src& src, const Params& p) {
             }
         });
         const float mall = combine_max<V>(mv);
-        if (combine_sum<V>(probe) == 0.f) {
+        if (combine_sum<V>(probe) == 0.f && !far_max(mall)) {
             const bool seen = mall != -NB200_INF;
             float a = 0.f;
             if (seen) {
@@ -164,7 +171,8 @@ __device__ __forceinline__ St lane_state(const Src& src, const Params& p) {
             }
             return St{mall, a, seen ? 1 : 0, 0};
         }
-        // A non-finite element is present: exact NaN / +inf status and the max over finite terms.
+        // A non-finite element is present, or the maximum is far: exact NaN / +inf status, the max over finite terms
+        // and every term from its distance to it.
         float m = -NB200_INF;
         int st = 0;
         src.for_each([&](const uint4& u, int) {
@@ -278,7 +286,7 @@ __device__ __forceinline__ St row_state(const Src& src, const Params& p) {
         });
         const float mall = warp_max(combine_max<V>(mv));
         const bool finite = __all_sync(0xffffffffu, combine_sum<V>(probe) == 0.f);
-        if (finite) {
+        if (finite && !far_max(mall)) {
             const bool seen = mall != -NB200_INF;
             float av[V];
 #pragma unroll
@@ -292,7 +300,7 @@ __device__ __forceinline__ St row_state(const Src& src, const Params& p) {
             }
             return St{mall, warp_sum(combine_sum<V>(av)), seen ? 1 : 0, 0};
         }
-        // a non-finite element: lane states with exact status, merged (rare path)
+        // a non-finite element or a far maximum: lane states with exact status, merged (rare path)
         return warp_merge<S>(lane_state<S, T>(src, p), src.lane, p);
     } else if constexpr (K::kind == K_MAXABS) {
         float mv[V], av[V];
