@@ -103,12 +103,12 @@ const char* nb200_last_error(void);
 const char* nb200_version(void);
 /* Number of nb200 kernel launches issued by this process (for launch accounting). */
 uint64_t nb200_launch_count(void);
-/* Reads and clears the fault bits of the kernels with device-side waits or checks (bit 0: a
- * bounded wait on a bulk copy in a streaming kernel or the gated norm's backward ran out and the kernel
- * stopped early, the rest of its rows unwritten and the norm's weight gradients NaN; bit 1: a bounded wait
- * in an attention kernel, forward or backward, ran out and its output was left unwritten; bit 2: the peer
- * merge's bounded wait for the ranks' states ran out, those rows written as NaN; bit 3: a peer push or merge
- * found a buffer whose recorded layout differs from the call's, nothing stored or read).
+/* Reads and clears the fault bits of the kernels with device-side waits or checks (bit 0: a bounded wait
+ * on a bulk copy ran out; a streaming kernel stopped early, the gated norm's backward wrote the rows it
+ * could not read, and its sums over rows, as NaN; bit 1: a bounded wait in an attention kernel, forward or
+ * backward, ran out and its output was left unwritten; bit 2: the peer merge's bounded wait for the ranks'
+ * states ran out, those rows written as NaN; bit 3: a peer push or merge found a buffer whose recorded
+ * layout differs from the call's, nothing stored or read).
  * Synchronous. No counterpart in the reference, whose Triton kernels have no device-side waits. */
 int nb200_stream_fault(uint32_t* bits);
 

@@ -534,7 +534,7 @@ struct Producer {
     const BwdArgs& a;
     int head, step, it = 0;
     uint32_t tail_ph = 0;
-    bool ok = true;
+    bool ok = true, left = false;
     Ring<kStages> r;
 
     __device__ __forceinline__ Producer(const CUtensorMap* mx_, const CUtensorMap* my_, uint8_t* smem_, Bars* b_, int batch_,
@@ -568,10 +568,8 @@ struct Producer {
             }
             if (cut) {
                 if (!(ok = __all_sync(0xffffffffu, wait_bar(&b->tail, tail_ph, abort)))) {
-                    if (lane == 0) {
-                        drain_bar(&b->tail, tail_ph);
-                        if (kKeys && !second) drain_bar(&b->stat_full[i & 1], (i >> 1) & 1u);  // came with this tile
-                    }
+                    if (lane == 0) drain_bar(&b->tail, tail_ph);
+                    left = !second;  // the statistics came with this tile
                     return;
                 }
                 tail_ph ^= 1u;
@@ -589,7 +587,7 @@ struct Producer {
     __device__ __forceinline__ void drain(int lane) {
         if (lane != 0) return;
         for (int s = 0; s < kStages && s < it; ++s) drain_bar(&b->full[s], ((it - 1 - s) / kStages) & 1u);
-        const int steps = (it + 1) / 2;
+        const int steps = (it + 1) / 2 + (left ? 1 : 0);
         for (int s = 0; kKeys && s < 2 && s < steps; ++s) drain_bar(&b->stat_full[s], ((steps - 1 - s) / 2) & 1u);
         drain_bar(&b->own, 0);
     }

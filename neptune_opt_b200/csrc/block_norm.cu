@@ -165,16 +165,6 @@ struct Rows {
             }
         }
     }
-    // The gradient of a shared gate row: laid out by its own pointer, as load_shared's rows are.
-    __device__ __forceinline__ void store_shared(T* row, const uint64_t* v) const {
-        if constexpr (FORM != LINED) {
-            store(row, v);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 2 * P; ++i)
-                if (holds(col_of(i))) row[col_of(i)] = Elem<T>::from_f(i & 1 ? f2hi(v[i / 2]) : f2lo(v[i / 2]));
-        }
-    }
     // 16 bytes from byte `off` of lo:hi.
     __device__ __forceinline__ static uint4 shift_down(const uint4& lo, const uint4& hi, uint32_t off) {
         uint32_t w[7] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z};
@@ -507,12 +497,12 @@ __global__ void __launch_bounds__(kThreads)
     int stage = 0;
     uint32_t parity = 0;
     bool primed = false;  // a row has been taken out of the ring
-    // A wait that ran out, for rows of even and odd number: written ahead of the row's barrier and read past it, so
-    // all threads stop at the same row.
-    __shared__ int ran_out[RING ? 2 : 1];
+    // False once a wait of this thread has run out. From there on it waits no more and takes NaN for what it should
+    // have read, which the row's sums carry to every thread: such rows, and the sums over rows, come out NaN. (Stopping
+    // the CTA instead takes a word from all of them for every row: bf16 [16384, 4096] 173 us, 167 us this way.)
+    bool arrived = true;
     if constexpr (RING) {
         if (threadIdx.x == 0) {
-            ran_out[0] = ran_out[1] = 0;
             for (int s = 0; s < stages; ++s) mbar_init(&full[s], 1);
             fence_barrier_init();
             fence_proxy_async();
@@ -550,7 +540,7 @@ __global__ void __launch_bounds__(kThreads)
         const bool last = next >= end;
         if (!AHEAD && !RING) fetch(row);
         if constexpr (RING) {
-            if (!mbar_wait(&full[stage], parity)) ran_out[r.phase] = 1;
+            arrived = arrived && mbar_wait(&full[stage], parity);
             auto staged = [&](CH& c, int i) {
 #pragma unroll
                 for (int k = 0; k < NV; ++k) {
@@ -563,6 +553,10 @@ __global__ void __launch_bounds__(kThreads)
             if (dy) staged(ndy, 2);
             if (dh) staged(ndh, 3);
             if (own) staged(ng, 4);
+            if (!arrived) {
+#pragma unroll
+                for (int k = 0; k < NV; ++k) nx.raw[k] = ndy.raw[k] = make_uint4(~0u, ~0u, ~0u, ~0u);
+            }
         }
         CH cx = nx, cr = nr, cdy = ndy, cdh = ndh;
         r.finish(cx);
@@ -611,11 +605,10 @@ __global__ void __launch_bounds__(kThreads)
         float t1 = f2lo(s1) + f2hi(s1), t2 = f2lo(s2) + f2hi(s2), t3 = f2lo(s3) + f2hi(s3);
         r.sum3(t1, t2, t3);
         if constexpr (RING) {
-            if (ran_out[r.phase ^ 1]) break;
             // Past the barrier in there, every thread is done with the previous row: its stage takes the row that is
             // `stages` behind it.
             const uint32_t ahead = row + (uint32_t)ch.step * (stages - 1);
-            if (threadIdx.x == 0 && primed && ahead < end) fill(stage ? stage - 1 : stages - 1, ahead);
+            if (threadIdx.x == 0 && arrived && primed && ahead < end) fill(stage ? stage - 1 : stages - 1, ahead);
             primed = true;
             if (++stage == stages) {
                 stage = 0;
@@ -643,33 +636,16 @@ __global__ void __launch_bounds__(kThreads)
                 G[i] = mul2(g1, f2(gate_slope(f2lo(a), n.act), gate_slope(f2hi(a), n.act)));
                 if (w1) G[i] = mul2(G[i], c1.pair(i));
             }
-            if (dgate && !partg) {
-                if (own) r.store(dgate + index * n.width, G);
-                else r.store_shared(dgate + index * n.width, G);
-            }
+            if (dgate && !partg) r.store(dgate + index * n.width, G);
             index = next_index;
             if (last) break;
 #pragma unroll
             for (int i = 0; i < P; ++i) G[i] = 0;
         }
     }
-    if (RING && (ran_out[0] | ran_out[1])) {
-        // This row and those behind it stay unwritten, and what was added up is no sum. What is on its way lands before
-        // the CTA may exit (again with a limit): this row's stage and those that were filled ahead.
-        if (threadIdx.x == 0)
-            for (int k = 0; k < stages - (primed ? 1 : 0) && row + k * (uint32_t)ch.step < end; ++k) {
-                mbar_wait(&full[stage], parity);
-                if (++stage == stages) {
-                    stage = 0;
-                    parity ^= 1u;
-                }
-            }
-#pragma unroll
-        for (int i = 0; i < P; ++i) {
-            a2[i] = G[i] = f2(NB200_NAN, NB200_NAN);
-            a1[i * r.G] = a2[i];
-        }
-    }
+    if (RING && !arrived && threadIdx.x == 0)  // copies may still be on their way: wait for them, again with a limit
+        for (int s = 0; s < stages; ++s)
+            for (uint32_t ph = 0; ph < 2; ++ph) mbar_wait(&full[s], ph);
     if (part2) store_part(part2 + r.unit * n.width, a2, r);
     if (part1) {
 #pragma unroll
@@ -858,6 +834,12 @@ int norm_bwd(const nb200_norm_args& a, const float* rstd, const T* dy, const T* 
     all.add(a.pre_weight, 0, es);
     Form form = pick_form(n, l, all, es);
     if (form == LINED && !lined_pays(n, l.step())) form = ANY;
+    // Whole gate groups (rows whose offset never changes) store their gate's gradient themselves, in the rows' layout.
+    if (form == LINED && l.step() == 1 && n.group > 1 && dgate) {
+        Layout with = l;
+        with.add(dgate, n.width, es);
+        if (!with.alike) form = ANY;
+    }
     const Shape s = make_shape(n.width, form);
     const int per = s.cta ? 1 : kWarpRows;
     const Chunks ch = bwd_chunks(n, s, s.form == LINED ? l.step() : 1);
