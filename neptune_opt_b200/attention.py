@@ -7,7 +7,8 @@ h // (H // H_kv)), fp32 scores and an fp32 online max/sum repair (the exp(c - s)
 repaired fold applied to attention rows), and optionally the fp32 natural log-sum-exp of each query
 row's scaled scores, [B, H, S]. `seq_lens` [B] gives the tokens of each batch element: queries and
 keys past them are masked, their rows of O and of the gradients are zero and their log-sum-exp is
--inf, whatever the tensors hold there.
+-inf, whatever the tensors hold there. Graphs traced through the functions (export, torch.compile) hold
+the C++ ops; forward-mode differentiation is refused.
 
 The reference has no attention kernel (its roadmap declares one out of scope); the contract here
 follows torch.nn.functional.scaled_dot_product_attention with is_causal (key index <= query

@@ -7,8 +7,9 @@
 
 One pass over x and residual, everything in fp32, each result rounded once (h from the unrounded y).
 Gradients are those of that function; weight and shared-gate gradients are fp32 column sums added in
-a fixed order. The reference's RMSNorm (neptune_codegen/emitters.py:549-627) is the inner norm alone,
-forward only, with its own rounding stages: `rms_norm` keeps those.
+a fixed order, and autograd asks only for those that are wanted. The reference's RMSNorm
+(neptune_codegen/emitters.py:549-627) is the inner norm alone, forward only, with its own rounding
+stages: `rms_norm` keeps those.
 
 x and residual are [..., width] in float32, bfloat16 or float16, gate and weights of the same dtype.
 gate is [width], or has x's rank with leading dimensions equal to x's followed by ones (one gate row

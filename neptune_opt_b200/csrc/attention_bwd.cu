@@ -33,8 +33,9 @@
 // of its group), each is cut into `parts` CTAs of consecutive steps whose fp32 sums a third kernel adds in
 // order and rounds.
 //
-// Measured on one B200, bf16: [8, 32, 4096, 128] 5.65 ms (973 TFLOP/s of the mathematics' 5 products, 1362 of
-// the 7 executed, 0.83 of the cuBLAS burst rate; 6.7 ms under continuous load, at the power cap). A key step
+// Measured on one B200, bf16: [8, 32, 4096, 128] 6.6 ms under continuous load, at the power cap (835 TFLOP/s of the
+// mathematics' 5 products, 1168 of the 7 executed, 0.86 of the sustained cuBLAS rate); a few passes from idle take
+// 5.65 ms (973, 1362 and 0.83 of the burst rate). A key step
 // takes 2930 cycles for 2048 of products, bound by shared memory (256 KB of operands, 64 KB of incoming tiles and
 // the statistics at 128 B a cycle); a query step 2000 for 1536, its exponentials and hand-offs about 1700. A
 // CTA costs 4 to 5 us besides its steps.

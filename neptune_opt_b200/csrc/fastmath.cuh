@@ -33,8 +33,9 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
-// 2^x on the special-function unit; subnormal results flush to zero (every caller adds them to a
-// sum that already holds the maximum's 2^0 = 1, where they vanish).
+// 2^x on the special-function unit (about 2 ulp); subnormal results flush to zero. The folds and forward
+// passes add them to a sum that holds the maximum's 2^0 = 1, where they vanish; the backward passes use them
+// as probabilities, of which those below 2^-126 become 0.
 __device__ __forceinline__ float ex2_ftz(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

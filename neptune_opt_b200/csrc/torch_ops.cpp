@@ -20,6 +20,7 @@
 //   segment_status_word(int device) -> Tensor      the per-device int32 word itself, for launches
 //                                                  made through the C ABI by other host code
 //   attention(Tensor q, Tensor k, Tensor v, bool causal, float scale) -> (Tensor o, Tensor lse)
+//                                                  (k and v may have fewer heads, a divisor of q's)
 // The training operators (their CUDA kernels check the whole contract of the Python functions; an absent
 // result is a tensor without elements, which graphs and packages can hold):
 //   attention_fwd(Tensor q, Tensor k, Tensor v, Tensor? seq_lens, bool causal, float scale, bool with_lse)
