@@ -80,10 +80,10 @@ def draw(rng):
         heads = kv_heads * rng.choice([1, 2, 3, 4, 5, 8, 16])
         dim, new = rng.choice([64, 128]), rng.choice([1, 1, 1, 2, 4, 7])
         prefix, cache = _log_int(rng, 1, 131072), max(new, _log_int(rng, 1, 8192))
-        # No dearer than the largest listed ones: the prefix's bytes, pairs of queries and keys, the caches' bytes.
-        pairs = 256 * 32 * 16384 // (heads * new)
-        prefix = min(prefix, 8 * 131072 * 128 // (kv_heads * dim), pairs)
-        most = min(256, pairs // max(prefix, cache), 256 * 8 * 512 * 128 // (kv_heads * cache * dim))
+        # No dearer than the largest listed ones: pairs of queries and keys, keys of the prefix and of all caches.
+        pairs, keys = 256 * 32 * 16384 // (heads * new), 8 * 131072 * 128 // (kv_heads * dim)
+        prefix = min(prefix, pairs, keys - cache)
+        most = min(256, pairs // max(prefix, cache), (keys - prefix) // cache)
         case = _attn("", rng.choice(["bfloat16", "float16"]), _log_int(rng, 1, max(1, most)), heads, kv_heads, dim,
                      prefix, cache, new, rng.random() < 0.5)
     elif op == "quantized_rms_norm":
