@@ -375,6 +375,78 @@ int nb200_distill_loss(const nb200_distill_args* args, const float* teacher_lse,
 int nb200_distill_loss_bwd(const nb200_distill_args* args, const float* grad, int64_t stride_grad,
                            const float* stats, void* dx, void* stream);
 
+/* ------------------------------------------------------------------ attention behind a shared prefix
+ * A few new tokens per sequence against a prefix that all sequences share and each sequence's own cache:
+ * o = softmax(scale q K^T) V with K, V the whole prefix followed by the sequence's own tokens up to the
+ * query's position. q is [batch, heads, tokens, head_dim], prefix_k, prefix_v [kv_heads, prefix, head_dim]
+ * (the batch stride is not used), k, v [batch, kv_heads, cache, head_dim], o contiguous like q, lse
+ * (nullable) fp32 [batch, heads, tokens], contiguous, the natural log-sum-exp of the scaled scores.
+ * seq_lens (nullable, device memory: every sequence fills its cache): own tokens of each sequence, the new
+ * ones included, read as clamped to [0, cache]. Query t stands at own position seq_lens[b] - tokens + t;
+ * one before its sequence's first token (a free slot) has a zero row of o and an lse of -inf, as has a row
+ * whose every score is -inf. What the caches hold at or past seq_lens does not matter. dtype NB200_BF16 or
+ * NB200_F16 for all tensors; probabilities are rounded to it for the product with V, all sums are fp32.
+ * head_dim 64 or 128 (else NB200_ERR_UNSUPPORTED); heads a multiple of kv_heads; bases and strides as for
+ * nb200_attention_fwd. prefix or cache may be 0. work: device memory, 16-byte aligned, of
+ * nb200_prefix_attention_work_bytes(args) bytes. The result does not depend on scheduling. No counterpart in
+ * the reference; the merge of partial results is its split plan's (neptune_codegen/algebra.py:348-403). */
+typedef struct {
+    int64_t batch, heads, kv_heads, tokens, head_dim, prefix, cache;
+    const int32_t* seq_lens;
+    int32_t dtype;
+    float scale;
+} nb200_prefix_attn_args;
+/* strides: of q, prefix_k, prefix_v, k, v. */
+int64_t nb200_prefix_attention_work_bytes(const nb200_prefix_attn_args* args);
+int nb200_prefix_attention(const nb200_prefix_attn_args* args, const nb200_attn_strides* strides, const void* q,
+                           const void* prefix_k, const void* prefix_v, const void* k, const void* v, void* o, float* lse,
+                           void* work, int64_t work_bytes, void* stream);
+
+/* ------------------------------------------------------------------ RMSNorm to 8 bits
+ * y = x + residual (y = x without a residual), h = weight * y rsqrt(mean y^2 + eps), and per row (group 0) or per
+ * group of `group` consecutive columns scale = max(max |h| / most, 2^-126), q = round(h / scale), saturating, with
+ * most = 448 (NB200_E4M3), 57344 (NB200_E5M2) or 127 (NB200_I8). All in fp32; y (written only with a residual) is
+ * rounded to dtype, h is taken from the unrounded y. A NaN in a row makes its scales NaN and its bytes NaN (0 in
+ * int8). x and residual are [rows, width] with unit column stride, weight contiguous [width], all of one dtype; q, y
+ * and scale ([rows] or [rows, width / group], fp32) are contiguous. Pointers need their elements' alignment only
+ * (rows that all start on 16-byte boundaries move faster). group is 0, 16, 32, 64 or 128 and divides width;
+ * width <= 16384 (else NB200_ERR_CAPACITY). The norm is the reference's (neptune_codegen/emitters.py:549-627)
+ * without its intermediate rounding; the reference has no 8-bit output. */
+typedef enum { NB200_E4M3 = 0, NB200_E5M2 = 1, NB200_I8 = 2 } nb200_byte_kind;
+typedef struct {
+    const void *x, *residual, *weight;
+    int64_t rows, width, group;
+    int64_t stride_x, stride_residual;                  /* elements between rows */
+    int32_t dtype, kind;
+    double eps;
+} nb200_norm8_args;
+int nb200_norm8(const nb200_norm8_args* args, void* q, float* scale, void* y, void* stream);
+
+/* ------------------------------------------------------------------ logits before sampling
+ * Per row, for each token of the vocabulary, in this order and in fp32, rounded once:
+ *   x > 0 ? x / repetition : x * repetition   if the token is in the row's history,
+ *   x - frequency * count - presence          if it is among the history's output tokens, count times,
+ *   x + the sum of its biases                 (in the order they are given),
+ *   x / temperature,
+ *   -inf                                      where its bit of allowed is 0.
+ * tokens (nullable with history = 0) is [rows, history]: the first token_lens[row] (null: all) are the row's
+ * history, of which the first prompt_lens[row] (null: none) are its prompt and the others its output. A token or
+ * bias index outside [0, vocab) is skipped. repetition, presence, frequency, temperature: fp32 [rows], each
+ * nullable (no such step); the caller keeps repetition and temperature positive. allowed (nullable) is
+ * [rows, ceil(vocab / 32)] int32, bit v % 32 of word v / 32. logits is [rows, vocab], out contiguous like it, of one
+ * dtype; every tensor has unit column stride. biases <= 1024 (else NB200_ERR_CAPACITY). No counterpart in the
+ * reference. */
+typedef struct {
+    const void *logits, *tokens, *bias_index;
+    const float* bias_value;
+    const int32_t *token_lens, *prompt_lens, *allowed;
+    const float *repetition, *presence, *frequency, *temperature;
+    int64_t rows, vocab, history, biases;
+    int64_t stride_logits, stride_tokens, stride_bias_index, stride_bias_value, stride_allowed; /* elements */
+    int32_t dtype, token_dtype, bias_dtype;
+} nb200_logits_args;
+int nb200_penalize_logits(const nb200_logits_args* args, void* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

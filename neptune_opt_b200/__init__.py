@@ -16,6 +16,11 @@ Training operators, differentiable through autograd and as explicit forward/back
 `attention(q, k, v, seq_lens=...)` / `attention_backward`, `gated_residual_norm(x, residual, gate,
 ...)` / `gated_residual_norm_backward` (the norms around a block with its gate and residual scale)
 and `distill_loss(logits, teacher_logits, teacher_index, ...)` / `distill_loss_backward`.
+
+Serving operators, for the decode step of a batch: `prefix_attention(q, prefix_k, prefix_v, k, v, seq_lens)`
+(new tokens against a prefix that all sequences share and their own caches), `quantized_rms_norm(x, weight,
+residual)` (residual sum, RMSNorm, 8-bit output with scales) and `penalize_logits(logits, tokens, ...)`
+(repetition penalties, biases, temperature and a grammar's mask).
 """
 from __future__ import annotations
 
@@ -25,6 +30,9 @@ from neptune_opt_b200.attention import attention_backward, attention_op, run_att
 from neptune_opt_b200.block_norm import (gated_residual_norm, gated_residual_norm_backward,  # noqa: F401
                                          run_gated_residual_norm)
 from neptune_opt_b200.distill import distill_loss, distill_loss_backward, run_distill_loss  # noqa: F401
+from neptune_opt_b200.logits import penalize_logits  # noqa: F401
+from neptune_opt_b200.prefix_attention import prefix_attention  # noqa: F401
+from neptune_opt_b200.quantized_norm import quantized_rms_norm  # noqa: F401
 from neptune_opt_b200.skeletons import (SKELETONS, all_registered, op_parameters, param_defaults,  # noqa: F401
                                         supported)
 from neptune_opt_b200.template import (MAX_SPLIT_PARTS, launch_reduction, run, run_l2_normalize,  # noqa: F401
@@ -95,7 +103,8 @@ __all__ = [
     "attention", "attention_backward", "attention_op", "run_attention", "distill_loss", "distill_loss_backward",
     "run_distill_loss", "gated_residual_norm", "gated_residual_norm_backward", "run_gated_residual_norm",
     "as_state_op", "as_triton_op", "autotune", "check_segment_status", "cuda_op_name", "l2_normalize",
-    "launch_count", "log_softmax", "op_handle", "op_parameters", "param_defaults", "rms_norm", "run",
+    "launch_count", "log_softmax", "op_handle", "op_parameters", "param_defaults", "penalize_logits",
+    "prefix_attention", "quantized_rms_norm", "rms_norm", "run",
     "run_l2_normalize", "run_rms_norm", "run_rms_norm_host", "run_segment_pool", "run_softmax", "run_softmax_lse",
     "segment_mean", "segment_op_handle", "segment_status", "segment_sum", "softmax", "softmax_op_handle",
     "split_launch_shape", "state_op_handle", "supported", "triton_op_name", "validate_rms_inputs",

@@ -68,12 +68,37 @@ class NB200DistillArgs(ctypes.Structure):
                 ("temperature", ctypes.c_double)]
 
 
+class NB200PrefixAttnArgs(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_int64), ("heads", ctypes.c_int64), ("kv_heads", ctypes.c_int64),
+                ("tokens", ctypes.c_int64), ("head_dim", ctypes.c_int64), ("prefix", ctypes.c_int64),
+                ("cache", ctypes.c_int64), ("seq_lens", ctypes.c_void_p), ("dtype", ctypes.c_int32),
+                ("scale", ctypes.c_float)]
+
+
+class NB200Norm8Args(ctypes.Structure):
+    _fields_ = [("x", ctypes.c_void_p), ("residual", ctypes.c_void_p), ("weight", ctypes.c_void_p),
+                ("rows", ctypes.c_int64), ("width", ctypes.c_int64), ("group", ctypes.c_int64),
+                ("stride_x", ctypes.c_int64), ("stride_residual", ctypes.c_int64), ("dtype", ctypes.c_int32),
+                ("kind", ctypes.c_int32), ("eps", ctypes.c_double)]
+
+
+class NB200LogitsArgs(ctypes.Structure):
+    _fields_ = [*((n, ctypes.c_void_p) for n in (
+                    "logits", "tokens", "bias_index", "bias_value", "token_lens", "prompt_lens", "allowed", "repetition",
+                    "presence", "frequency", "temperature")),
+                *((n, ctypes.c_int64) for n in (
+                    "rows", "vocab", "history", "biases", "stride_logits", "stride_tokens", "stride_bias_index",
+                    "stride_bias_value", "stride_allowed")),
+                *((n, ctypes.c_int32) for n in ("dtype", "token_dtype", "bias_dtype"))]
+
+
 STATE_BYTES = ctypes.sizeof(NB200State)
 
 # Every symbol include/neptune_b200.h declares, with (restype, argtypes).
 _vp, _i64, _int, _dbl = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_double
 _attn, _strides = ctypes.POINTER(NB200AttnArgs), ctypes.POINTER(NB200AttnStrides)
 _norm, _distill = ctypes.POINTER(NB200NormArgs), ctypes.POINTER(NB200DistillArgs)
+_prefix, _norm8, _logits = (ctypes.POINTER(t) for t in (NB200PrefixAttnArgs, NB200Norm8Args, NB200LogitsArgs))
 SIGNATURES = {
     "nb200_last_error": (ctypes.c_char_p, []),
     "nb200_version": (ctypes.c_char_p, []),
@@ -116,6 +141,10 @@ SIGNATURES = {
     "nb200_gated_norm_bwd": (_int, [_norm, _int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
     "nb200_distill_loss": (_int, [_distill, _vp, _vp, _vp, _vp]),
     "nb200_distill_loss_bwd": (_int, [_distill, _vp, _i64, _vp, _vp, _vp]),
+    "nb200_prefix_attention_work_bytes": (_i64, [_prefix]),
+    "nb200_prefix_attention": (_int, [_prefix, _strides, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "nb200_norm8": (_int, [_norm8, _vp, _vp, _vp, _vp]),
+    "nb200_penalize_logits": (_int, [_logits, _vp, _vp]),
 }
 
 _LOCK = threading.Lock()

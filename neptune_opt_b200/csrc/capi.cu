@@ -141,6 +141,109 @@ int check_distill(const char* what, const nb200_distill_args* a) {
     return NB200_OK;
 }
 
+int check_prefix_attention(const char* what, const nb200_prefix_attn_args* a, const nb200_attn_strides* s) {
+    if (!a || !s) { set_error("%s: null pointer", what); return NB200_ERR_ARG; }
+    if (a->dtype != NB200_BF16 && a->dtype != NB200_F16) {
+        set_error("%s: dtype must be bfloat16 or float16", what);
+        return NB200_ERR_ARG;
+    }
+    if (a->batch < 0 || a->heads < 0 || a->tokens < 0 || a->prefix < 0 || a->cache < 0) {
+        set_error("%s: negative size", what);
+        return NB200_ERR_ARG;
+    }
+    if (a->batch == 0 || a->heads == 0 || a->tokens == 0) return NB200_OK;
+    if (a->kv_heads < 1 || a->heads % a->kv_heads) {
+        set_error("%s: %lld query heads cannot share %lld key/value heads", what, (long long)a->heads,
+                  (long long)a->kv_heads);
+        return NB200_ERR_ARG;
+    }
+    if (a->head_dim != 64 && a->head_dim != 128) {
+        set_error("%s: head_dim %lld is not supported (the kernels are built for 64 and 128)", what,
+                  (long long)a->head_dim);
+        return NB200_ERR_UNSUPPORTED;
+    }
+    if (!std::isfinite(a->scale) || !(a->scale > 0.f)) {
+        set_error("%s: scale must be finite and positive", what);
+        return NB200_ERR_ARG;
+    }
+    const int64_t most = (int64_t)1 << 30;
+    if (a->batch > most || a->heads > most || a->tokens > most || a->prefix > most || a->cache > most ||
+        a->batch * a->heads > most || a->batch * a->heads * a->tokens > most) {
+        set_error("%s: batch=%lld, heads=%lld, tokens=%lld, prefix=%lld, cache=%lld exceed the kernel's index range", what,
+                  (long long)a->batch, (long long)a->heads, (long long)a->tokens, (long long)a->prefix,
+                  (long long)a->cache);
+        return NB200_ERR_CAPACITY;
+    }
+    // The copies' limits: multiples of 16 bytes, below 2^40 bytes.
+    auto bad = [](int64_t stride, int64_t size) { return size > 1 && (stride < 8 || stride % 8 || stride >= (int64_t)1 << 39); };
+    for (int i = 0; i < 5; ++i) {
+        const bool shared = i == 1 || i == 2;
+        const int64_t seq = i == 0 ? a->tokens : shared ? a->prefix : a->cache;
+        if (seq == 0) continue;
+        if ((!shared && bad(s[i].batch, a->batch)) || bad(s[i].head, i ? a->kv_heads : a->heads) || bad(s[i].seq, seq)) {
+            set_error("%s: strides must be positive multiples of 8 elements (tensor %d)", what, i);
+            return NB200_ERR_ARG;
+        }
+    }
+    return NB200_OK;
+}
+
+int check_norm8(const char* what, const nb200_norm8_args* a) {
+    if (!a) { set_error("%s: null pointer", what); return NB200_ERR_ARG; }
+    if (!valid_dtype(a->dtype)) { set_error("%s: unsupported dtype %d", what, a->dtype); return NB200_ERR_ARG; }
+    if (a->kind < NB200_E4M3 || a->kind > NB200_I8) {
+        set_error("%s: unknown 8-bit type %d", what, a->kind);
+        return NB200_ERR_ARG;
+    }
+    if (a->rows < 0 || a->width < 1) { set_error("%s: need rows >= 0 and width >= 1", what); return NB200_ERR_ARG; }
+    if (a->group != 0 && a->group != 16 && a->group != 32 && a->group != 64 && a->group != 128) {
+        set_error("%s: group must be 0, 16, 32, 64 or 128, got %lld", what, (long long)a->group);
+        return NB200_ERR_ARG;
+    }
+    if (a->group && a->width % a->group) {
+        set_error("%s: width %lld is not whole groups of %lld", what, (long long)a->width, (long long)a->group);
+        return NB200_ERR_ARG;
+    }
+    if (!std::isfinite(a->eps) || !((float)a->eps > 0.f) || !std::isfinite((float)a->eps)) {
+        set_error("%s: eps must be finite and positive in fp32", what);
+        return NB200_ERR_ARG;
+    }
+    if (a->width > 16384) {
+        set_error("%s: width %lld exceeds 16384", what, (long long)a->width);
+        return NB200_ERR_CAPACITY;
+    }
+    if (a->rows > 1 && (a->stride_x < 0 || (a->residual && a->stride_residual < 0))) {
+        set_error("%s: negative stride", what);
+        return NB200_ERR_ARG;
+    }
+    return NB200_OK;
+}
+
+int check_logits(const char* what, const nb200_logits_args* a) {
+    if (!a) { set_error("%s: null pointer", what); return NB200_ERR_ARG; }
+    auto index = [](int32_t d) { return d == NB200_I32 || d == NB200_I64; };
+    if (!valid_dtype(a->dtype) || (a->history && !index(a->token_dtype)) || (a->biases && !index(a->bias_dtype))) {
+        set_error("%s: unsupported dtype", what);
+        return NB200_ERR_ARG;
+    }
+    if (a->rows < 0 || a->vocab < 1 || a->history < 0 || a->biases < 0) {
+        set_error("%s: need rows >= 0, vocab >= 1, history >= 0 and biases >= 0", what);
+        return NB200_ERR_ARG;
+    }
+    const int64_t most = (int64_t)1 << 30;
+    if (a->rows > most || a->vocab > most || a->history > most || a->biases > 1024) {
+        set_error("%s: rows=%lld, vocab=%lld, history=%lld or biases=%lld (at most 1024) exceed the kernel's range", what,
+                  (long long)a->rows, (long long)a->vocab, (long long)a->history, (long long)a->biases);
+        return NB200_ERR_CAPACITY;
+    }
+    if (a->rows > 1 && (a->stride_logits < 0 || a->stride_tokens < 0 || a->stride_bias_index < 0 ||
+                        a->stride_bias_value < 0 || a->stride_allowed < 0)) {
+        set_error("%s: negative stride", what);
+        return NB200_ERR_ARG;
+    }
+    return NB200_OK;
+}
+
 // Declared-parameter checks of the reference's certificate (algebra.py:285-302): every declared
 // scalar finite, T/beta/N/eps strictly positive, tiny nonnegative.
 int check_params(int sk, const nb200_params* q, nb200_params* out) {
@@ -617,6 +720,64 @@ int nb200_distill_loss_bwd(const nb200_distill_args* args, const float* grad, in
         return NB200_ERR_ARG;
     }
     return launch_distill_bwd(*args, grad, stride_grad, stats, dx, (cudaStream_t)stream);
+}
+
+int64_t nb200_prefix_attention_work_bytes(const nb200_prefix_attn_args* args) {
+    const nb200_attn_strides any = {8, 8, 8};
+    const nb200_attn_strides strides[5] = {any, any, any, any, any};
+    const int rc = check_prefix_attention("nb200_prefix_attention", args, strides);
+    if (rc) return rc;
+    return args->batch * args->heads * args->tokens ? prefix_attention_work_bytes(*args) : 0;
+}
+
+int nb200_prefix_attention(const nb200_prefix_attn_args* args, const nb200_attn_strides* strides, const void* q,
+                           const void* prefix_k, const void* prefix_v, const void* k, const void* v, void* o, float* lse,
+                           void* work, int64_t work_bytes, void* stream) {
+    const char* what = "nb200_prefix_attention";
+    const int rc = check_prefix_attention(what, args, strides);
+    if (rc) return rc;
+    if (args->batch * args->heads * args->tokens == 0) return NB200_OK;
+    const void* tensors[6] = {q, o, prefix_k, prefix_v, k, v};
+    for (int i = 0; i < 6; ++i) {
+        if ((i == 2 || i == 3) ? args->prefix == 0 : i > 3 && args->cache == 0) continue;
+        if (!tensors[i] || !aligned16(tensors[i])) {
+            set_error("%s: null pointer, or a tensor is not 16-byte aligned", what);
+            return NB200_ERR_ARG;
+        }
+    }
+    if (((uintptr_t)lse | (uintptr_t)args->seq_lens) & 3u) {
+        set_error("%s: lse and seq_lens must be 4-byte aligned", what);
+        return NB200_ERR_ARG;
+    }
+    const int64_t need = prefix_attention_work_bytes(*args);
+    if (need && (!work || !aligned16(work) || work_bytes < need)) {
+        set_error("%s: work must hold %lld bytes, 16-byte aligned", what, (long long)need);
+        return NB200_ERR_ARG;
+    }
+    return launch_prefix_attention(*args, strides, q, prefix_k, prefix_v, k, v, o, lse, work, (cudaStream_t)stream);
+}
+
+int nb200_norm8(const nb200_norm8_args* args, void* q, float* scale, void* y, void* stream) {
+    const int rc = check_norm8("nb200_norm8", args);
+    if (rc) return rc;
+    if (args->rows == 0) return NB200_OK;
+    if (!args->x || !args->weight || !q || !scale || (args->residual && !y)) {
+        set_error("nb200_norm8: null pointer");
+        return NB200_ERR_ARG;
+    }
+    return launch_norm8(*args, q, scale, y, (cudaStream_t)stream);
+}
+
+int nb200_penalize_logits(const nb200_logits_args* args, void* out, void* stream) {
+    const int rc = check_logits("nb200_penalize_logits", args);
+    if (rc) return rc;
+    if (args->rows == 0) return NB200_OK;
+    if (!args->logits || !out || (args->history && !args->tokens) ||
+        (args->biases && (!args->bias_index || !args->bias_value))) {
+        set_error("nb200_penalize_logits: null pointer");
+        return NB200_ERR_ARG;
+    }
+    return launch_logits(*args, out, (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -94,4 +94,11 @@ int launch_distill_fwd(const nb200_distill_args& a, const float* teacher_lse, fl
 int launch_distill_bwd(const nb200_distill_args& a, const float* grad, int64_t stride_grad, const float* stats,
                        void* dx, cudaStream_t st);
 
+int64_t prefix_attention_work_bytes(const nb200_prefix_attn_args& a);
+int launch_prefix_attention(const nb200_prefix_attn_args& a, const nb200_attn_strides* strides, const void* q,
+                            const void* prefix_k, const void* prefix_v, const void* k, const void* v, void* o,
+                            float* lse, void* work, cudaStream_t st);
+int launch_norm8(const nb200_norm8_args& a, void* q, float* scale, void* y, cudaStream_t st);
+int launch_logits(const nb200_logits_args& a, void* out, cudaStream_t st);
+
 }  // namespace nb200

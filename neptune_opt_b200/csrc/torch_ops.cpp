@@ -37,6 +37,14 @@
 //              -> (Tensor loss, Tensor stats)
 //   distill_loss_bwd(Tensor grad, Tensor x, Tensor teacher, Tensor index, Tensor stats,
 //                    float temperature) -> Tensor
+// The serving operators (the same, but without a gradient: one that is asked for is refused):
+//   prefix_attention(Tensor q, Tensor prefix_k, Tensor prefix_v, Tensor k, Tensor v, Tensor? seq_lens, float scale,
+//                    bool with_lse) -> (Tensor o, Tensor lse)
+//   norm8(Tensor x, Tensor weight, Tensor? residual, int group, ScalarType dtype, float eps)
+//              -> (Tensor q, Tensor scale, Tensor y)
+//   penalize_logits(Tensor logits, Tensor? tokens, Tensor? token_lens, Tensor? prompt_lens, Tensor? repetition,
+//                   Tensor? presence, Tensor? frequency, Tensor? bias_index, Tensor? bias_value, Tensor? allowed,
+//                   Tensor? temperature) -> Tensor
 //
 // libneptune_b200.so is opened at the first call from the directory this library lives in, so
 // the two files only need to sit side by side.
@@ -76,6 +84,10 @@ struct Api {
     decltype(&nb200_gated_norm_bwd) gated_norm_bwd;
     decltype(&nb200_distill_loss) distill_loss;
     decltype(&nb200_distill_loss_bwd) distill_loss_bwd;
+    decltype(&nb200_prefix_attention_work_bytes) prefix_attention_work_bytes;
+    decltype(&nb200_prefix_attention) prefix_attention;
+    decltype(&nb200_norm8) norm8;
+    decltype(&nb200_penalize_logits) penalize_logits;
 };
 
 std::string own_directory() {
@@ -118,6 +130,10 @@ const Api& api() {
         bind(h, "nb200_gated_norm_bwd", a.gated_norm_bwd);
         bind(h, "nb200_distill_loss", a.distill_loss);
         bind(h, "nb200_distill_loss_bwd", a.distill_loss_bwd);
+        bind(h, "nb200_prefix_attention_work_bytes", a.prefix_attention_work_bytes);
+        bind(h, "nb200_prefix_attention", a.prefix_attention);
+        bind(h, "nb200_norm8", a.norm8);
+        bind(h, "nb200_penalize_logits", a.penalize_logits);
     });
     return a;
 }
@@ -655,6 +671,186 @@ at::Tensor distill_loss_bwd_cuda(const at::Tensor& grad_, const at::Tensor& x, c
     return dx;
 }
 
+// ------------------------------------------------------------------ the serving operators
+// What prefix_attention asks of its tensors, symbolic sizes too.
+void check_prefix_attention(const at::Tensor& q, const at::Tensor& pk, const at::Tensor& pv, const at::Tensor& k,
+                            const at::Tensor& v, const OptTensor& seq_lens, const char* what) {
+    for (const at::Tensor* t : {&q, &pk, &pv, &k, &v}) {
+        check_strided(*t, what);
+        TORCH_CHECK_TYPE(t->scalar_type() == q.scalar_type() &&
+                             (q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf),
+                         what, ": tensors must all be bfloat16 or all float16");
+        TORCH_CHECK_VALUE(t->device() == q.device(), what, ": tensors must be on one device");
+    }
+    TORCH_CHECK_VALUE(q.dim() == 4 && k.dim() == 4 && v.dim() == 4 && pk.dim() == 3 && pv.dim() == 3, what,
+                      ": q, k, v must be 4-D, prefix_k, prefix_v 3-D");
+    const auto qs = q.sym_sizes(), ks = k.sym_sizes(), ps = pk.sym_sizes();
+    TORCH_CHECK_VALUE(ks == v.sym_sizes() && ps == pv.sym_sizes() && qs[0] == ks[0] && qs[3] == ks[3] &&
+                          qs[3] == ps[2] && ks[1] == ps[0],
+                      what, ": the shapes differ");
+    TORCH_CHECK_VALUE(qs[1] == ks[1] || (ks[1] > 0 && qs[1] % ks[1] == 0), what, ": ", qs[1],
+                      " query heads cannot share ", ks[1], " key/value heads");
+    check_seq_lens(seq_lens, q, what);
+}
+
+std::tuple<at::Tensor, at::Tensor> prefix_attention_cuda(const at::Tensor& q_, const at::Tensor& pk_,
+                                                         const at::Tensor& pv_, const at::Tensor& k_,
+                                                         const at::Tensor& v_, const OptTensor& seq_lens, double scale,
+                                                         bool with_lse) {
+    const char* what = "nb200.prefix_attention";
+    check_cuda(q_, what);
+    check_prefix_attention(q_, pk_, pv_, k_, v_, seq_lens, what);
+    c10::cuda::CUDAGuard guard(q_.device());
+    const at::Tensor q = attn_rows(q_), pk = attn_rows(pk_.unsqueeze(0)), pv = attn_rows(pv_.unsqueeze(0));
+    const at::Tensor k = attn_rows(k_), v = attn_rows(v_);
+    at::Tensor o = at::empty(q.sizes(), q.options());
+    const auto f32 = q.options().dtype(at::kFloat);
+    at::Tensor lse = with_lse ? at::empty(q.sizes().slice(0, 3), f32) : at::empty({0}, f32);
+    const nb200_prefix_attn_args a = {q.size(0), q.size(1), k.size(1), q.size(2), q.size(3), pk.size(2), k.size(2),
+                                      present(seq_lens) ? seq_lens->data_ptr<int32_t>() : nullptr, dtype_code(q),
+                                      (float)scale};
+    const nb200_attn_strides strides[5] = {attn_strides(q), attn_strides(pk), attn_strides(pv), attn_strides(k),
+                                           attn_strides(v)};
+    const int64_t bytes = api().prefix_attention_work_bytes(&a);
+    if (bytes < 0) check((int)bytes, what);
+    at::Tensor work = at::empty({std::max<int64_t>(bytes, 16)}, q.options().dtype(at::kByte));
+    check(api().prefix_attention(&a, strides, q.data_ptr(), pk.data_ptr(), pv.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                 o.data_ptr(), with_lse ? lse.data_ptr<float>() : nullptr, work.data_ptr(),
+                                 work.numel(), stream_of(q)),
+          what);
+    return {o, lse};
+}
+
+int byte_kind(at::ScalarType t, const char* what) {
+    if (t == at::kFloat8_e4m3fn) return NB200_E4M3;
+    if (t == at::kFloat8_e5m2) return NB200_E5M2;
+    TORCH_CHECK_TYPE(t == at::kChar, what, ": dtype must be float8_e4m3fn, float8_e5m2 or int8, got ", t);
+    return NB200_I8;
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> norm8_cuda(const at::Tensor& x_, const at::Tensor& weight_,
+                                                          const OptTensor& residual_, int64_t group,
+                                                          at::ScalarType dtype, double eps) {
+    const char* what = "nb200.norm8";
+    check_strided(x_, what);
+    check_cuda(x_, what);
+    nb200_norm8_args a = {};
+    a.dtype = dtype_code(x_);
+    a.kind = byte_kind(dtype, what);
+    TORCH_CHECK_VALUE(x_.dim() >= 1 && x_.size(-1) >= 1, what, ": x must be [..., width]");
+    NormInputs::same_kind(weight_, x_, what);
+    TORCH_CHECK_VALUE(weight_.dim() == 1 && weight_.size(0) == x_.size(-1), what,
+                      ": weight must be 1-D with x's last dimension");
+    a.width = x_.size(-1);
+    a.rows = x_.numel() / a.width;
+    a.group = group;
+    a.eps = eps;
+    c10::cuda::CUDAGuard guard(x_.device());
+    const at::Tensor x = unit_rows(x_, a.rows), weight = weight_.contiguous();
+    at::Tensor residual, y;
+    a.x = x.data_ptr();
+    a.stride_x = x.stride(0);
+    a.weight = weight.data_ptr();
+    if (present(residual_)) {
+        NormInputs::same_kind(*residual_, x_, what);
+        TORCH_CHECK_VALUE(residual_->sizes() == x_.sizes(), what, ": residual must have x's shape");
+        residual = unit_rows(*residual_, a.rows);
+        a.residual = residual.data_ptr();
+        a.stride_residual = residual.stride(0);
+        y = at::empty(x_.sizes(), x_.options());
+    } else {
+        y = none_like(x_);
+    }
+    at::Tensor q = at::empty(x_.sizes(), x_.options().dtype(dtype));
+    std::vector<int64_t> shape = lead_shape(x_, false);
+    TORCH_CHECK_VALUE(group >= 0 && (group == 0 || a.width % group == 0), what, ": width ", a.width,
+                      " is not whole groups of ", group);
+    shape.push_back(group ? a.width / group : 1);
+    at::Tensor scale = at::empty(shape, x_.options().dtype(at::kFloat));
+    check(api().norm8(&a, q.data_ptr(), scale.data_ptr<float>(), a.residual ? y.data_ptr() : nullptr, stream_of(x_)),
+          what);
+    return {q, scale, y};
+}
+
+// The descriptor of the logits' inputs and the tensors whose memory it names.
+struct LogitsInputs {
+    nb200_logits_args a = {};
+    std::vector<at::Tensor> keep;
+    const at::Tensor& x;
+    const char* what;
+    // A tensor per row of the logits: [rows, columns] of the given type, or null.
+    const void* rows_of(const OptTensor& t, const char* name, int64_t* columns, int64_t* stride) {
+        if (!present(t)) return nullptr;
+        check_strided(*t, what);
+        TORCH_CHECK_VALUE(t->device() == x.device() && t->dim() == 2 && t->size(0) == a.rows, what, ": ", name,
+                          " must be [rows, ...] on the device of logits");
+        keep.push_back(unit_rows(*t, a.rows));
+        *columns = t->size(1);
+        *stride = keep.back().stride(0);
+        return keep.back().data_ptr();
+    }
+    template <typename T>
+    const T* per_row(const OptTensor& t, const char* name, at::ScalarType dtype) {
+        if (!present(t)) return nullptr;
+        check_strided(*t, what);
+        TORCH_CHECK_TYPE(t->scalar_type() == dtype, what, ": ", name, " must be ", dtype);
+        TORCH_CHECK_VALUE(t->device() == x.device() && t->dim() == 1 && t->size(0) == a.rows, what, ": ", name,
+                          " must be [rows] on the device of logits");
+        if (t->is_contiguous()) return t->data_ptr<T>();
+        keep.push_back(t->contiguous());
+        return keep.back().data_ptr<T>();
+    }
+    LogitsInputs(const at::Tensor& logits, const char* w) : x(logits), what(w) {
+        check_strided(x, what);
+        check_cuda(x, what);
+        a.dtype = dtype_code(x);
+        TORCH_CHECK_VALUE(x.dim() == 2 && x.size(1) >= 1, what, ": logits must be [rows, vocab]");
+        a.rows = x.size(0);
+        a.vocab = x.size(1);
+        keep.reserve(16);
+    }
+};
+
+at::Tensor penalize_logits_cuda(const at::Tensor& logits, const OptTensor& tokens, const OptTensor& token_lens,
+                                const OptTensor& prompt_lens, const OptTensor& repetition, const OptTensor& presence,
+                                const OptTensor& frequency, const OptTensor& bias_index, const OptTensor& bias_value,
+                                const OptTensor& allowed, const OptTensor& temperature) {
+    const char* what = "nb200.penalize_logits";
+    LogitsInputs in(logits, what);
+    nb200_logits_args& a = in.a;
+    c10::cuda::CUDAGuard guard(logits.device());
+    int64_t columns = 0;
+    a.logits = in.rows_of(logits, "logits", &columns, &a.stride_logits);
+    if (present(tokens)) a.token_dtype = index_code(*tokens);
+    a.tokens = in.rows_of(tokens, "tokens", &a.history, &a.stride_tokens);
+    a.token_lens = in.per_row<int32_t>(token_lens, "token_lens", at::kInt);
+    a.prompt_lens = in.per_row<int32_t>(prompt_lens, "prompt_lens", at::kInt);
+    a.repetition = in.per_row<float>(repetition, "repetition", at::kFloat);
+    a.presence = in.per_row<float>(presence, "presence", at::kFloat);
+    a.frequency = in.per_row<float>(frequency, "frequency", at::kFloat);
+    a.temperature = in.per_row<float>(temperature, "temperature", at::kFloat);
+    TORCH_CHECK_VALUE(present(tokens) || !(present(token_lens) || present(prompt_lens) || present(repetition) ||
+                                           present(presence) || present(frequency)),
+                      what, ": lengths or penalties without tokens");
+    TORCH_CHECK_VALUE(present(bias_index) == present(bias_value), what, ": bias_index and bias_value go together");
+    if (present(bias_index)) {
+        a.bias_dtype = index_code(*bias_index);
+        TORCH_CHECK_TYPE(bias_value->scalar_type() == at::kFloat, what, ": bias_value must be float32");
+        TORCH_CHECK_VALUE(bias_index->sizes() == bias_value->sizes(), what, ": the shapes of the biases differ");
+        a.bias_index = in.rows_of(bias_index, "bias_index", &a.biases, &a.stride_bias_index);
+        a.bias_value = static_cast<const float*>(in.rows_of(bias_value, "bias_value", &columns, &a.stride_bias_value));
+    }
+    if (present(allowed)) {
+        TORCH_CHECK_TYPE(allowed->scalar_type() == at::kInt, what, ": allowed must be int32");
+        a.allowed = static_cast<const int32_t*>(in.rows_of(allowed, "allowed", &columns, &a.stride_allowed));
+        TORCH_CHECK_VALUE(columns == (a.vocab + 31) / 32, what, ": allowed must hold ", (a.vocab + 31) / 32,
+                          " words a row, got ", columns);
+    }
+    at::Tensor out = at::empty(logits.sizes(), logits.options());
+    check(api().penalize_logits(&a, out.data_ptr(), stream_of(logits)), what);
+    return out;
+}
+
 // ------------------------------------------------------------------ Meta kernels (shapes only)
 // Symbolic sizes throughout, so graphs exported with dynamic dimensions trace through these ops.
 std::vector<c10::SymInt> lead_sym_shape(const at::Tensor& x, bool keepdim) {
@@ -730,6 +926,30 @@ std::tuple<at::Tensor, at::Tensor> distill_loss_meta(const at::Tensor& x, const 
 at::Tensor distill_loss_bwd_meta(const at::Tensor&, const at::Tensor& x, const at::Tensor&, const at::Tensor&,
                                  const at::Tensor&, double) {
     return like_meta(x);
+}
+std::tuple<at::Tensor, at::Tensor> prefix_attention_meta(const at::Tensor& q, const at::Tensor& pk,
+                                                         const at::Tensor& pv, const at::Tensor& k,
+                                                         const at::Tensor& v, const OptTensor& seq_lens, double,
+                                                         bool with_lse) {
+    check_prefix_attention(q, pk, pv, k, v, seq_lens, "nb200.prefix_attention");
+    const auto qs = q.sym_sizes();
+    const auto f32 = q.options().dtype(at::kFloat);
+    return {at::empty_symint(qs, q.options()),
+            with_lse ? at::empty_symint(std::vector<c10::SymInt>(qs.begin(), qs.end() - 1), f32) : at::empty({0}, f32)};
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor> norm8_meta(const at::Tensor& x, const at::Tensor&,
+                                                          const OptTensor& residual, int64_t group,
+                                                          at::ScalarType dtype, double) {
+    std::vector<c10::SymInt> shape = lead_sym_shape(x, false);
+    shape.emplace_back(group > 0 ? x.sym_size(-1) / group : c10::SymInt(1));
+    return {at::empty_symint(x.sym_sizes(), x.options().dtype(dtype)),
+            at::empty_symint(shape, x.options().dtype(at::kFloat)),
+            present(residual) ? like_meta(x) : none_like(x)};
+}
+at::Tensor penalize_logits_meta(const at::Tensor& logits, const OptTensor&, const OptTensor&, const OptTensor&,
+                                const OptTensor&, const OptTensor&, const OptTensor&, const OptTensor&,
+                                const OptTensor&, const OptTensor&, const OptTensor&) {
+    return like_meta(logits);
 }
 
 }  // namespace
@@ -818,6 +1038,13 @@ TORCH_LIBRARY(nb200, m) {
           "-> (Tensor, Tensor)");
     m.def("distill_loss_bwd(Tensor grad, Tensor x, Tensor teacher, Tensor index, Tensor stats, float temperature) "
           "-> Tensor");
+    m.def("prefix_attention(Tensor q, Tensor prefix_k, Tensor prefix_v, Tensor k, Tensor v, Tensor? seq_lens, "
+          "float scale, bool with_lse) -> (Tensor, Tensor)");
+    m.def("norm8(Tensor x, Tensor weight, Tensor? residual, int group, ScalarType dtype, float eps) "
+          "-> (Tensor, Tensor, Tensor)");
+    m.def("penalize_logits(Tensor logits, Tensor? tokens, Tensor? token_lens, Tensor? prompt_lens, "
+          "Tensor? repetition, Tensor? presence, Tensor? frequency, Tensor? bias_index, Tensor? bias_value, "
+          "Tensor? allowed, Tensor? temperature) -> Tensor");
 }
 
 // The training operators are their own gradients' building blocks: autograd records nothing for them (the
@@ -829,7 +1056,16 @@ static void below_autograd(const c10::OperatorHandle& op, c10::DispatchKeySet ke
     at::AutoDispatchBelowADInplaceOrView guard;
     op.redispatchBoxed(keys & c10::after_ADInplaceOrView_keyset, stack);
 }
+// The serving operators have no gradient; one that autograd would have to record is refused, not dropped.
+static void without_gradient(const c10::OperatorHandle& op, c10::DispatchKeySet keys, torch::jit::Stack* stack) {
+    for (const c10::IValue& v : torch::jit::last(*stack, op.schema().arguments().size()))
+        TORCH_CHECK_NOT_IMPLEMENTED(!v.isTensor() || !(at::GradMode::is_enabled() && v.toTensor().requires_grad()),
+                                    op.schema().name(), " has no gradient: call it under torch.no_grad()");
+    below_autograd(op, keys, stack);
+}
 TORCH_LIBRARY_IMPL(nb200, Autograd, m) {
+    for (const char* op : {"prefix_attention", "norm8", "penalize_logits"})
+        m.impl(op, torch::CppFunction::makeFromBoxedFunction<&without_gradient>());
     for (const char* op : {"attention_fwd", "attention_bwd", "gated_norm", "gated_norm_bwd", "distill_loss",
                            "distill_loss_bwd"})
         m.impl(op, torch::CppFunction::makeFromBoxedFunction<&below_autograd>());
@@ -848,6 +1084,9 @@ TORCH_LIBRARY_IMPL(nb200, CUDA, m) {
     m.impl("gated_norm_bwd", &gated_norm_bwd_cuda);
     m.impl("distill_loss", &distill_loss_cuda);
     m.impl("distill_loss_bwd", &distill_loss_bwd_cuda);
+    m.impl("prefix_attention", &prefix_attention_cuda);
+    m.impl("norm8", &norm8_cuda);
+    m.impl("penalize_logits", &penalize_logits_cuda);
 }
 
 TORCH_LIBRARY_IMPL(nb200, Meta, m) {
@@ -863,4 +1102,7 @@ TORCH_LIBRARY_IMPL(nb200, Meta, m) {
     m.impl("gated_norm_bwd", &gated_norm_bwd_meta);
     m.impl("distill_loss", &distill_loss_meta);
     m.impl("distill_loss_bwd", &distill_loss_bwd_meta);
+    m.impl("prefix_attention", &prefix_attention_meta);
+    m.impl("norm8", &norm8_meta);
+    m.impl("penalize_logits", &penalize_logits_meta);
 }
