@@ -12,13 +12,13 @@
 //
 // Rows. The query rows that share a key/value head are numbered r = (b G + g) T + t (G = query heads per
 // key/value head, T = new tokens): a sequence's rows are neighbours, and all B G T of them meet the prefix.
-#include <type_traits>
+#include <algorithm>
 
-#include "common.cuh"
-#include "launch.h"
+#include "prefix_attention.cuh"
 #include "stream.cuh"
 
 namespace nb200 {
+namespace prefix {
 namespace {
 
 constexpr int kWarps = 4;      // warps of a part kernel's CTA; each takes every fourth step of the keys
@@ -31,11 +31,10 @@ struct Keys {  // one source of keys and values (strides in elements)
 };
 
 struct PartArgs {
-    const void* q;
-    int64_t qb, qh, qt;
+    Query query;
     Keys src;
     const int* lens;     // own keys: tokens of each sequence (null: all); unused for the prefix
-    int kv_heads, group, tokens;
+    int kv_heads;
     int keys;            // keys of the source (the prefix, or the cache's length)
     int rows;            // query rows of a key/value head over all sequences
     int unit_rows;       // rows that share this source's keys: all, or a sequence's
@@ -75,12 +74,6 @@ __device__ __forceinline__ void ldmatrix4_t(uint32_t* r, uint32_t addr) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-// Probabilities are rounded to the inputs' type for the product with the values. They are at most 2^8 (see
-// the running maximum), so fp16 has room for 2^6 more: that keeps the probabilities of very many unlikely keys
-// above fp16's smallest value.
-template <typename T> constexpr float kLift = std::is_same<T, __half>::value ? 6.f : 0.f;
-constexpr float kSlack = 8.f;  // the running maximum may lag behind by 2^8
 
 __device__ __forceinline__ int tokens_of(const int* lens, int b, int keys) {
     return lens ? max(0, min(lens[b], keys)) : keys;
@@ -124,9 +117,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) part_kernel(const PartArgs a) 
         const int in = (lane >> 2) + 8 * i;
         const bool live = in < nrows;
         const int r = row0 + (live ? in : 0);
-        const int t = r % a.tokens, g = r / a.tokens % a.group, b = r / a.tokens / a.group;
-        limit[i] = OWN ? len - a.tokens + t : k1 - 1;
-        const T* q = static_cast<const T*>(a.q) + b * a.qb + (int64_t)(head * a.group + g) * a.qh + t * a.qt;
+        limit[i] = OWN ? len - a.query.tokens + r % a.query.tokens : k1 - 1;
+        const T* q = query_row<T>(a.query, head, r);
 #pragma unroll
         for (int s = 0; s < D / 16; ++s)
 #pragma unroll
@@ -357,8 +349,13 @@ Split plan_split(int64_t units, int64_t rows, int64_t keys) {
     return s;
 }
 
+// Up to this many query rows of a key/value head meet the prefix in the part kernel above; more go to the
+// tensor cores.
+constexpr int kMmaRows = 32;
+
 struct Plan {
     Split prefix, own;
+    bool tensor;          // the prefix runs on the tensor cores
     int64_t rows, pairs;  // query rows of a key/value head; pairs of a part over all heads
 };
 
@@ -366,7 +363,9 @@ Plan plan_of(const nb200_prefix_attn_args& a) {
     Plan p;
     const int64_t group = a.heads / a.kv_heads;
     p.rows = a.batch * group * a.tokens;
-    p.prefix = plan_split(a.kv_heads, p.rows, a.prefix);
+    p.tensor = a.prefix && p.rows > kMmaRows;
+    p.prefix = p.tensor ? Split{0, tensor_splits(a.kv_heads, p.rows, a.prefix), 0, 0}
+                        : plan_split(a.kv_heads, p.rows, a.prefix);
     p.own = plan_split(a.kv_heads * a.batch, group * a.tokens, a.cache);
     p.pairs = a.kv_heads * p.rows;
     return p;
@@ -393,10 +392,9 @@ int launch_all(const nb200_prefix_attn_args& n, const nb200_attn_strides* s, con
     float* part_o = work;
     float* part_lse = work + (int64_t)parts * plan.pairs * D;
     PartArgs a = {};
-    a.q = q;
-    a.qb = s[0].batch, a.qh = s[0].head, a.qt = s[0].seq;
+    a.query = {q, s[0].batch, s[0].head, s[0].seq, (int)(n.heads / n.kv_heads), (int)n.tokens};
     a.lens = n.seq_lens;
-    a.kv_heads = (int)n.kv_heads, a.group = (int)(n.heads / n.kv_heads), a.tokens = (int)n.tokens;
+    a.kv_heads = (int)n.kv_heads;
     a.rows = (int)plan.rows;
     a.sl2 = n.scale * 1.4426950408889634f;
     auto run = [&](const Split& sp, bool own, int64_t first) {
@@ -411,7 +409,7 @@ int launch_all(const nb200_prefix_attn_args& n, const nb200_attn_strides* s, con
         }
         if (own) {
             a.src = {k, v, s[3].batch, s[3].head, s[3].seq, s[4].batch, s[4].head, s[4].seq};
-            a.keys = (int)n.cache, a.unit_rows = a.group * a.tokens;
+            a.keys = (int)n.cache, a.unit_rows = a.query.group * a.query.tokens;
             return sp.mt == 1 ? launch_part<T, D, 1, true>(a, (unsigned)grid, limits[0], st)
                               : launch_part<T, D, 2, true>(a, (unsigned)grid, limits[1], st);
         }
@@ -421,14 +419,24 @@ int launch_all(const nb200_prefix_attn_args& n, const nb200_attn_strides* s, con
                           : launch_part<T, D, 2, false>(a, (unsigned)grid, limits[3], st);
     };
     int rc;
-    if ((rc = run(plan.prefix, false, 0)) || (rc = run(plan.own, true, plan.prefix.splits))) return rc;
-    const JoinArgs j = {part_o, part_lse, o, lse, n.seq_lens, a.kv_heads, a.group, a.tokens, a.rows, parts, (int)n.cache};
+    if (plan.tensor) {
+        const TensorPart t = {a.query, a.kv_heads, a.rows, (int)n.prefix, plan.prefix.splits, a.sl2, part_o, part_lse};
+        rc = launch_tensor_part(t, n.dtype, n.head_dim, pk, s[1], pv, s[2], st);
+    } else {
+        rc = run(plan.prefix, false, 0);
+    }
+    if (rc || (rc = run(plan.own, true, plan.prefix.splits))) return rc;
+    const JoinArgs j = {part_o, part_lse, o, lse, n.seq_lens, a.kv_heads, a.query.group, a.query.tokens, a.rows, parts,
+                        (int)n.cache};
     launch_pdl(join_kernel<T, D>, (unsigned)((plan.pairs + 7) / 8), 256, 0, st, j);
     count_launch();
     return finish_launch("nb200_prefix_attention");
 }
 
 }  // namespace
+}  // namespace prefix
+
+using namespace prefix;
 
 int64_t prefix_attention_work_bytes(const nb200_prefix_attn_args& a) {
     const Plan p = plan_of(a);

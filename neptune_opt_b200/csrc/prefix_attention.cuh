@@ -1,0 +1,46 @@
+// What the kernels of attention behind a shared prefix agree on: query rows, the keys of a part and where its
+// result goes (prefix_attention.cu has the mathematics).
+#pragma once
+
+#include <type_traits>
+
+#include "common.cuh"
+#include "launch.h"
+
+namespace nb200 {
+namespace prefix {
+
+struct Query {
+    const void* q;
+    int64_t qb, qh, qt;  // strides in elements
+    int group, tokens;   // query heads per key/value head, new tokens per sequence
+};
+
+// Query row r = (b group + g) tokens + t of key/value head `head`.
+template <typename T>
+__device__ __forceinline__ const T* query_row(const Query& a, int head, int r) {
+    const int t = r % a.tokens, g = r / a.tokens % a.group, b = r / a.tokens / a.group;
+    return static_cast<const T*>(a.q) + b * a.qb + (int64_t)(head * a.group + g) * a.qh + t * a.qt;
+}
+
+// Probabilities are rounded to the inputs' type for the product with the values. They are at most 2^8 (the
+// running maximum may lag behind by that much), so fp16 has room for 2^6 more: that keeps the probabilities of very
+// many unlikely keys above fp16's smallest value.
+constexpr float kSlack = 8.f;
+template <typename T> constexpr float kLift = std::is_same<T, __half>::value ? 6.f : 0.f;
+
+// The prefix on the tensor cores (prefix_attention_tc.cu): query rows of a key/value head in blocks of 256, the
+// prefix's tiles of 128 keys in `splits` nearly equal ranges. Results as of any part: o [splits][kv_heads][rows][D],
+// lse [splits][kv_heads][rows].
+struct TensorPart {
+    Query query;
+    int kv_heads, rows, keys, splits;
+    float sl2;
+    float *o, *lse;
+};
+int tensor_splits(int64_t kv_heads, int64_t rows, int64_t keys);
+int launch_tensor_part(const TensorPart& a, int dtype, int64_t head_dim, const void* k, const nb200_attn_strides& ks,
+                       const void* v, const nb200_attn_strides& vs, cudaStream_t st);
+
+}  // namespace prefix
+}  // namespace nb200
