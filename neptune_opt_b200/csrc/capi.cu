@@ -315,14 +315,15 @@ uint64_t nb200_launch_count(void) { return g_launches.load(std::memory_order_rel
 
 int nb200_stream_fault(uint32_t* bits) {
     if (!bits) { set_error("nb200_stream_fault: null pointer"); return NB200_ERR_ARG; }
-    unsigned int v = 0, w = 0, x = 0, y = 0, z = 0, p = 0;
+    unsigned int v = 0, w = 0, x = 0, y = 0, z = 0, p = 0, q = 0;
     int rc = stream_fault_take(&v);
     if (rc == NB200_OK) rc = attn_fault_take(&w);
     if (rc == NB200_OK) rc = peer_fault_take(&x);
     if (rc == NB200_OK) rc = attn_bwd_fault_take(&y);
     if (rc == NB200_OK) rc = norm_fault_take(&z);
     if (rc == NB200_OK) rc = prefix_fault_take(&p);
-    *bits = v | w | x | y | z | p;
+    if (rc == NB200_OK) rc = prefix_stream_fault_take(&q);
+    *bits = v | w | x | y | z | p | q;
     return rc;
 }
 

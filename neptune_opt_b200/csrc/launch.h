@@ -77,6 +77,7 @@ int attn_fault_take(unsigned int* bits);
 int attn_bwd_fault_take(unsigned int* bits);
 int norm_fault_take(unsigned int* bits);
 int prefix_fault_take(unsigned int* bits);
+int prefix_stream_fault_take(unsigned int* bits);
 
 int launch_attention(const nb200_attn_args& a, const nb200_attn_strides* strides, const void* q, const void* k,
                      const void* v, void* o, float* lse, cudaStream_t st);

@@ -17,8 +17,8 @@
 // for the caches, and for a prefix with few rows, where the bound is the keys' bytes; join_kernel.
 #include <algorithm>
 
+#include "attn.cuh"
 #include "prefix_attention.cuh"
-#include "stream.cuh"
 
 namespace nb200 {
 namespace prefix {
@@ -29,12 +29,7 @@ constexpr int kCtas = 2;       // its CTAs per SM
 constexpr int kStepKeys = 16;  // keys of a worker's step
 constexpr int kStages = 3;     // steps of a worker in shared memory: one in use, two in flight
 
-struct Keys {  // one source of keys and values (strides in elements)
-    const void *k, *v;
-    int64_t kb, kh, ks, vb, vh, vs;
-};
-
-// A unit of the stream kernel is a tile of 16 MT query rows and the keys they share: units of the prefix
+// A unit of the stream kernel is a tile of 8 NT query rows and the keys they share: units of the prefix
 // (key/value head, row tile; none when the prefix runs on the tensor cores), then units of the caches
 // (sequence, key/value head, row tile). All units' steps of 16 keys stand in one line, of which every worker
 // takes an equal piece, whatever the sequences' lengths are. A piece covers the end of one unit, whole units,
@@ -42,7 +37,6 @@ struct Keys {  // one source of keys and values (strides in elements)
 // span[u] says which workers had a share in u.
 struct StreamArgs {
     Query query;
-    Keys shared, own;
     const int* lens;  // tokens of each sequence (null: all of the cache)
     int batch, kv_heads, prefix, cache;
     int rows;                      // query rows of a key/value head over all sequences
@@ -56,26 +50,19 @@ struct StreamArgs {
 
 template <typename T> struct Mma;
 template <> struct Mma<__nv_bfloat16> {
-    __device__ __forceinline__ static void mul(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    __device__ __forceinline__ static void mul(float* d, const uint32_t* a, const uint32_t* b) {
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
     }
 };
 template <> struct Mma<__half> {
-    __device__ __forceinline__ static void mul(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    __device__ __forceinline__ static void mul(float* d, const uint32_t* a, const uint32_t* b) {
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
     }
 };
-
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void ldmatrix4(uint32_t* r, uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -84,12 +71,17 @@ __device__ __forceinline__ void ldmatrix4_t(uint32_t* r, uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
-__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-__device__ __forceinline__ int tokens_of(const int* lens, int b, int keys) {
-    return lens ? max(0, min(lens[b], keys)) : keys;
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {  // an 8 x 8 matrix of 16-bit values over the warp
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
+
 __device__ __forceinline__ int steps_of(int keys) { return (keys + kStepKeys - 1) / kStepKeys; }
+
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint64_t* bar) {
+    tc::tma_load_4d(reinterpret_cast<void*>(__cvta_shared_to_generic(dst)), map, c0, c1, c2, c3, bar);
+}
 
 // A position in the line of steps.
 struct Cursor {
@@ -172,18 +164,36 @@ __device__ __forceinline__ Cursor cursor_at(const StreamArgs& a, int64_t at) {
     return c;
 }
 
-// Every warp is a worker: it copies the keys and values of its steps into shared memory that no other warp
-// touches, two steps ahead and across the units' borders, and keeps the running maximum, sum and output of its
-// unit in registers. No barrier, no atomics.
-template <typename T, int D, int MT>
-__global__ void __launch_bounds__(kWarps * 32, kCtas) stream_kernel(const StreamArgs a) {
-    constexpr int kChunks = D / 8;                // 16-byte pieces of a row
-    constexpr uint32_t kTile = kStepKeys * D * 2; // K or V of a step
-    extern __shared__ __align__(128) uint8_t smem[];
+// Every warp is a worker: its lane 0 has the keys and values of the steps copied (TMA) into shared memory that no
+// other warp touches, two steps ahead and across the units' borders, and the warp keeps the running maximum, sum
+// and output of its unit in registers. No barrier, no atomics.
+//
+// The products are taken transposed, S^T = K Q^T and O^T = V^T P^T, with the keys (then the head dimension) along
+// the 16 rows of mma.sync and the query rows along its 8 columns: a unit of few query rows pays for 8, not 16, and the
+// fragments of K and V serve all NT column tiles.
+//
+// Every wait is bounded; one that runs out sets bit 1 of the fault word, and the worker waits (again with a limit) for
+// its copies and leaves its slots unwritten.
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kWarps * 32, kCtas)
+    stream_kernel(const __grid_constant__ CUtensorMap shared_k, const __grid_constant__ CUtensorMap shared_v,
+                  const __grid_constant__ CUtensorMap own_k, const __grid_constant__ CUtensorMap own_v,
+                  const StreamArgs a) {
+    constexpr uint32_t kBox = kStepKeys * 128;       // 64 columns of a step's keys, 128-byte swizzled
+    constexpr uint32_t kTile = kBox * (D / 64);      // K or V of a step
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t full[kWarps][kStages];
+    __shared__ int abort_flag[kWarps];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t mine = ((smem_u32(smem_raw) + 1023u) & ~1023u) + warp * (kStages * 2 * kTile);
+    if (lane == 0) {
+        for (int i = 0; i < kStages; ++i) mbar_init(&full[warp][i], 1);
+        abort_flag[warp] = 0;
+        fence_barrier_init();
+    }
     if (!a.beside) pdl_wait();
     pdl_trigger();
-    const int lane = threadIdx.x & 31;
-    const int worker = (int)blockIdx.x * kWarps + (threadIdx.x >> 5);
+    const int worker = (int)blockIdx.x * kWarps + warp;
     int64_t all;
     const int64_t share = share_of(a, (int64_t)gridDim.x * kWarps, all);
     const int64_t first = worker * share;
@@ -193,146 +203,151 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) stream_kernel(const Stream
         return;
     }
     int left = (int)min(share, all - first);  // steps to go
+    const int steps = left;
     Cursor use = cursor_at(a, first), get = use;
     int to_get = left;
 
-    const uint32_t mine = smem_addr(smem) + (threadIdx.x >> 5) * (kStages * 2 * kTile);
-    // The cursor's step into a stage. Keys past the end read as zero: what a cache holds behind a sequence must not
-    // reach the products.
-    auto copy = [&](int stage) {
-        if (to_get > 0) {
+    auto copy = [&](int stage) {  // the cursor's step into a stage
+        if (to_get <= 0) return;
+        if (lane == 0) {
             const bool shared = get.batch < 0;
-            const Keys& s = shared ? a.shared : a.own;
-            const T* kp = static_cast<const T*>(s.k) + (shared ? 0 : get.batch * s.kb) + get.head * s.kh;
-            const T* vp = static_cast<const T*>(s.v) + (shared ? 0 : get.batch * s.vb) + get.head * s.vh;
-            const int kb = get.step * kStepKeys;
-            const uint32_t at = mine + stage * (2 * kTile);
+            const CUtensorMap *mk = shared ? &shared_k : &own_k, *mv = shared ? &shared_v : &own_v;
+            const int b = shared ? 0 : get.batch, key = get.step * kStepKeys;
+            uint64_t* bar = &full[warp][stage];
+            mbar_expect_tx(bar, 2 * kTile);
 #pragma unroll
-            for (int c = lane; c < kStepKeys * kChunks; c += 32) {
-                const int row = c / kChunks, ch = c % kChunks;
-                const bool in = kb + row < get.keys;
-                const int64_t key = in ? kb + row : get.keys - 1;
-                const uint32_t off = (uint32_t)(row * D * 2 + ((ch ^ (row & 7)) << 4));
-                cp_async16(at + off, kp + key * s.ks + ch * 8, in ? 16 : 0);
-                cp_async16(at + kTile + off, vp + key * s.vs + ch * 8, in ? 16 : 0);
+            for (int h = 0; h < D / 64; ++h) {
+                tma_load(mine + stage * 2 * kTile + h * kBox, mk, 64 * h, key, get.head, b, bar);
+                tma_load(mine + stage * 2 * kTile + kTile + h * kBox, mv, 64 * h, key, get.head, b, bar);
             }
-            if (--to_get) get.next(a);
         }
-        cp_async_commit();
+        if (--to_get) get.next(a);
     };
+    __syncwarp();
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) copy(i);
 
-    // Row i of this lane's accumulators: lane / 4 + 8 i within the tile, i < 2 MT.
-    uint32_t qf[MT][D / 16][4];
-    int limit[2 * MT];  // last key the row sees
-    float o[MT][D / 8][4], m[2 * MT], l[2 * MT];
+    // Column tile n of this lane's accumulators: query rows 8 n + 2 (lane % 4) and the next one.
+    uint32_t qf[NT][D / 16][2];
+    int limit[NT][2], lowest = 0;  // last key a row sees; of the unit's rows, the least
+    float o[NT][D / 16][4], m[NT][2], l[NT][2];
     int nrows = 0;
     auto begin = [&] {
         const bool shared = use.batch < 0;
-        const int in_unit = use.tile * 16 * MT, own_rows = a.query.group * a.query.tokens;
+        const int in_unit = use.tile * 8 * NT, own_rows = a.query.group * a.query.tokens;
         const int row0 = (shared ? 0 : use.batch * own_rows) + in_unit;
-        nrows = min(16 * MT, (shared ? a.rows : own_rows) - in_unit);
+        nrows = min(8 * NT, (shared ? a.rows : own_rows) - in_unit);
+        lowest = shared ? use.keys - 1 : use.keys - a.query.tokens;
 #pragma unroll
-        for (int i = 0; i < 2 * MT; ++i) {
-            const int in = (lane >> 2) + 8 * i;
-            const bool live = in < nrows;
-            const int r = row0 + (live ? in : 0);
-            limit[i] = shared ? use.keys - 1 : use.keys - a.query.tokens + r % a.query.tokens;
-            const T* q = query_row<T>(a.query, use.head, r);
+        for (int n = 0; n < NT; ++n) {
+            const int in = 8 * n + (lane >> 2);
+            const T* q = query_row<T>(a.query, use.head, row0 + (in < nrows ? in : 0)) + 2 * (lane & 3);
 #pragma unroll
-            for (int s = 0; s < D / 16; ++s)
+            for (int d = 0; d < D / 16; ++d)
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
-                    qf[i / 2][s][i % 2 + 2 * h] =
-                        live ? *reinterpret_cast<const uint32_t*>(q + 16 * s + 8 * h + 2 * (lane & 3)) : 0u;
-            m[i] = -NB200_INF, l[i] = 0.f;
+                    qf[n][d][h] = in < nrows ? *reinterpret_cast<const uint32_t*>(q + 16 * d + 8 * h) : 0u;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                limit[n][e] = shared ? use.keys - 1 : lowest + (in_unit + 8 * n + 2 * (lane & 3) + e) % a.query.tokens;
+                m[n][e] = -NB200_INF, l[n][e] = 0.f;
+            }
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[n][d][e] = 0.f;
         }
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int c = 0; c < D / 8; ++c)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[i][c][e] = 0.f;
     };
     begin();
     if (lane == 0 && use.step == 0) a.span[use.unit(a)].x = worker;
 
-    for (int stage = 0;; stage = stage + 1 == kStages ? 0 : stage + 1) {
-        cp_async_wait<kStages - 2>();
-        __syncwarp();  // the step's data is there, and everyone has left the stage that is filled next
+    // This lane's address in a box: the row it loads for ldmatrix, and the swizzle of its 16-byte pieces.
+    const int k_row = lane & 15, k_piece = lane >> 4;                            // K: keys 0-15, then 8 columns on
+    const int v_row = (lane >> 4) * 8 + (lane & 7), v_piece = lane >> 3 & 1;     // V, transposed: columns, then keys
+    bool ok = true;
+    int stage = 0, done = 0;
+    uint32_t phase = 0;
+    for (;;) {
+        ok = __all_sync(0xffffffffu, wait_bar(&full[warp][stage], phase, &abort_flag[warp]));
+        if (!ok) break;
+        // Everyone has left the stage that is filled next.
         copy(stage == 0 ? kStages - 1 : stage - 1);
         const uint32_t ks = mine + stage * (2 * kTile), vs = ks + kTile;
         const int kb = use.step * kStepKeys;
-        float s[MT][2][4];
+        // What a cache holds behind a sequence must not reach the products: 0 times an infinity is none.
+        if (use.batch >= 0 && kb + kStepKeys > use.keys) {
+            for (int i = (use.keys - kb) * 8 + lane; i < kStepKeys * 8; i += 32)
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+                for (int h = 0; h < D / 64; ++h)
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(vs + h * kBox + i * 16), "r"(0u) : "memory");
+            fence_proxy_async();
+            __syncwarp();
+        }
+        float s[NT][4];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s[mt][e / 4][e % 4] = 0.f;
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) {
-            const int row = (lane >> 4) * 8 + (lane & 7), ch = 2 * d + (lane >> 3 & 1);
-            uint32_t b[4];
-            ldmatrix4(b, ks + row * D * 2 + ((ch ^ (row & 7)) << 4));
+            uint32_t f[4];
+            ldmatrix4(f, ks + (d / 4) * kBox + k_row * 128 + (((2 * (d % 4) + k_piece) ^ (k_row & 7)) << 4));
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                Mma<T>::mul(s[mt][0], qf[mt][d], b[0], b[1]);
-                Mma<T>::mul(s[mt][1], qf[mt][d], b[2], b[3]);
-            }
+            for (int n = 0; n < NT; ++n) Mma<T>::mul(s[n], f, qf[n][d]);
         }
-        // Scores in the log2 domain; keys past a row's last are masked.
-        float top[2 * MT];
+        // s[n][e]: key lane / 4 + 8 (e / 2), query row e % 2 of the lane's two.
+        if (kb + kStepKeys - 1 > lowest) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (kb + (lane >> 2) + 8 * (e / 2) > limit[n][e % 2]) s[n][e] = -NB200_INF;
+        }
         bool grow = false;
 #pragma unroll
-        for (int r = 0; r < 2 * MT; ++r) {
-            top[r] = -NB200_INF;
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                float& x = s[r / 2][e / 2][2 * (r % 2) + e % 2];
-                x = kb + 8 * (e / 2) + 2 * (lane & 3) + e % 2 <= limit[r] ? x * a.sl2 : -NB200_INF;
-                top[r] = fmaxf(top[r], x);
-            }
-            grow |= top[r] > m[r] + kSlack;
-        }
+            for (int e = 0; e < 2; ++e) grow |= fmaxf(s[n][e], s[n][e + 2]) * a.sl2 > m[n][e] + kSlack;
         if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-            for (int r = 0; r < 2 * MT; ++r) {
-                top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-                top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-                const float next = fmaxf(m[r], top[r]);
-                const float f = next == m[r] ? 1.f : ex2(m[r] - next);
-                m[r] = next;
-                l[r] *= f;
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int c = 0; c < D / 8; ++c) {
-                    o[r / 2][c][2 * (r % 2)] *= f;
-                    o[r / 2][c][2 * (r % 2) + 1] *= f;
+                for (int e = 0; e < 2; ++e) {
+                    float top = fmaxf(s[n][e], s[n][e + 2]) * a.sl2;
+#pragma unroll
+                    for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+                    const float next = fmaxf(m[n][e], top);
+                    const float f = next == m[n][e] ? 1.f : ex2(m[n][e] - next);
+                    m[n][e] = next;
+                    l[n][e] *= f;
+#pragma unroll
+                    for (int d = 0; d < D / 16; ++d) o[n][d][e] *= f, o[n][d][e + 2] *= f;
                 }
-            }
         }
-        uint32_t p[MT][4];
+        uint32_t p[NT][2];
 #pragma unroll
-        for (int r = 0; r < 2 * MT; ++r) {
-            const float ref = (m[r] == -NB200_INF ? 0.f : m[r]) - kLift<T>;
+        for (int n = 0; n < NT; ++n) {
+            float x[4];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const float x = ex2(s[r / 2][h][2 * (r % 2)] - ref), y = ex2(s[r / 2][h][2 * (r % 2) + 1] - ref);
-                l[r] += x + y;
-                p[r / 2][r % 2 + 2 * h] = Elem<T>::pack_word(x, y);
+            for (int e = 0; e < 2; ++e) {
+                const float ref = (m[n][e] == -NB200_INF ? 0.f : m[n][e]) - kLift<T>;
+                x[e] = ex2(fmaf(s[n][e], a.sl2, -ref));
+                x[e + 2] = ex2(fmaf(s[n][e + 2], a.sl2, -ref));
+                l[n][e] += x[e] + x[e + 2];
             }
+            p[n][0] = transpose8(Elem<T>::pack_word(x[0], x[1]));
+            p[n][1] = transpose8(Elem<T>::pack_word(x[2], x[3]));
         }
 #pragma unroll
-        for (int c = 0; c < D / 16; ++c) {
-            const int row = (lane >> 3 & 1) * 8 + (lane & 7), ch = 2 * c + (lane >> 4);
-            uint32_t b[4];
-            ldmatrix4_t(b, vs + row * D * 2 + ((ch ^ (row & 7)) << 4));
+        for (int d = 0; d < D / 16; ++d) {
+            uint32_t f[4];
+            ldmatrix4_t(f, vs + (d / 4) * kBox + v_row * 128 + (((2 * (d % 4) + v_piece) ^ (v_row & 7)) << 4));
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                Mma<T>::mul(o[mt][2 * c], p[mt], b[0], b[1]);
-                Mma<T>::mul(o[mt][2 * c + 1], p[mt], b[2], b[3]);
-            }
+            for (int n = 0; n < NT; ++n) Mma<T>::mul(o[n][d], f, p[n]);
         }
 
+        ++done;
+        if (++stage == kStages) stage = 0, phase ^= 1u;
         --left;
         const bool ends = use.step + 1 == use.steps;
         if (left && !ends) {
@@ -343,27 +358,32 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) stream_kernel(const Stream
         const int unit = use.unit(a);
         const int64_t slot = ((int64_t)worker + unit) * a.slot_rows;
 #pragma unroll
-        for (int r = 0; r < 2 * MT; ++r) {
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-            const int in = (lane >> 2) + 8 * r;
-            if (in < nrows) {
-                const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
-                float* dst = a.o + (slot + in) * D + 2 * (lane & 3);
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int c = 0; c < D / 8; ++c)
-                    *reinterpret_cast<float2*>(dst + 8 * c) =
-                        make_float2(o[r / 2][c][2 * (r % 2)] * inv, o[r / 2][c][2 * (r % 2) + 1] * inv);
-                if ((lane & 3) == 0) a.lse[slot + in] = l[r] == 0.f ? -NB200_INF : m[r] + log2f(l[r]) - kLift<T>;
+            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                for (int w = 4; w < 32; w <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], w);
+                const int in = 8 * n + 2 * (lane & 3) + e;
+                if (in < nrows) {
+                    const float inv = l[n][e] == 0.f ? 0.f : 1.f / l[n][e];
+                    float* dst = a.o + (slot + in) * D + (lane >> 2);
+#pragma unroll
+                    for (int d = 0; d < D / 16; ++d) {
+                        dst[16 * d] = o[n][d][e] * inv;
+                        dst[16 * d + 8] = o[n][d][e + 2] * inv;
+                    }
+                    if (lane < 4) a.lse[slot + in] = l[n][e] == 0.f ? -NB200_INF : m[n][e] + log2f(l[n][e]) - kLift<T>;
+                }
             }
-        }
         if (lane == 0 && ends) a.span[unit].y = worker;
         if (!left) break;
         use.next(a);
         if (lane == 0) a.span[use.unit(a)].x = worker;
         begin();
     }
-    cp_async_wait<0>();
+    // Every copy lands before the CTA may exit; `steps - to_get` were issued, of which `done` have been waited for.
+    if (!ok)
+        for (int i = done; i < steps - to_get; ++i) drain_bar(&full[warp][i % kStages], (i / kStages) & 1u);
     if (a.beside) pdl_wait();
 }
 
@@ -481,7 +501,7 @@ constexpr int kStreamRows = 32;
 
 struct Plan {
     int64_t rows;                  // query rows of a key/value head
-    int mt;                        // 16-row tiles of a unit
+    int nt;                        // 8-row tiles of a unit
     int splits;                    // of the prefix on the tensor cores (0: it is in the stream kernel, or empty)
     int64_t prefix_tiles, own_tiles, slot_rows, units, ctas;
     int64_t most_parts;            // parts of a row, at most
@@ -493,12 +513,13 @@ Plan plan_of(const nb200_prefix_attn_args& a) {
     Plan p = {};
     const int64_t own_rows = a.heads / a.kv_heads * a.tokens;
     p.rows = a.batch * own_rows;
-    p.mt = own_rows > 16 ? 2 : 1;
-    const int64_t tile = 16 * p.mt;
     if (a.prefix && p.rows > kStreamRows) p.splits = tensor_splits(a.kv_heads, p.rows, a.prefix);
+    const int64_t most = a.prefix && !p.splits ? p.rows : own_rows;
+    p.nt = most <= 8 ? 1 : most <= 16 ? 2 : 4;
+    const int64_t tile = 8 * p.nt;
     p.prefix_tiles = a.prefix && !p.splits ? (p.rows + tile - 1) / tile : 0;
     p.own_tiles = (own_rows + tile - 1) / tile;
-    p.slot_rows = std::min(tile, p.prefix_tiles ? p.rows : own_rows);
+    p.slot_rows = std::min(tile, most);
     p.units = a.kv_heads * (p.prefix_tiles + a.batch * p.own_tiles);
     const int64_t prefix_steps = p.prefix_tiles ? (a.prefix + kStepKeys - 1) / kStepKeys : 0;
     const int64_t own_steps = (a.cache + kStepKeys - 1) / kStepKeys;
@@ -520,13 +541,17 @@ Plan plan_of(const nb200_prefix_attn_args& a) {
     return p;
 }
 
-SharedLimit g_shared[8];
+SharedLimit g_shared[12];
 
-template <typename T, int D, int MT>
-int launch_stream(const StreamArgs& a, int64_t ctas, SharedLimit& limit, cudaStream_t st) {
-    constexpr uint32_t bytes = kWarps * kStages * 2 * kStepKeys * D * 2;
-    if (const int rc = limit.raise("nb200_prefix_attention", stream_kernel<T, D, MT>, bytes)) return rc;
-    launch_pdl(stream_kernel<T, D, MT>, (unsigned)ctas, kWarps * 32, bytes, st, a);
+struct Maps {
+    CUtensorMap shared_k, shared_v, own_k, own_v;
+};
+
+template <typename T, int D, int NT>
+int launch_stream(const Maps& m, const StreamArgs& a, int64_t ctas, SharedLimit& limit, cudaStream_t st) {
+    constexpr uint32_t bytes = kWarps * kStages * 2 * kStepKeys * D * 2 + 1024;  // + alignment slack
+    if (const int rc = limit.raise("nb200_prefix_attention", stream_kernel<T, D, NT>, bytes)) return rc;
+    launch_pdl(stream_kernel<T, D, NT>, (unsigned)ctas, kWarps * 32, bytes, st, m.shared_k, m.shared_v, m.own_k, m.own_v, a);
     count_launch();
     return finish_launch("nb200_prefix_attention");
 }
@@ -551,8 +576,14 @@ int launch_all(const nb200_prefix_attn_args& n, const nb200_attn_strides* s, con
     }
     StreamArgs a = {};
     a.query = query;
-    a.shared = {pk, pv, 0, s[1].head, s[1].seq, 0, s[2].head, s[2].seq};
-    a.own = {k, v, s[3].batch, s[3].head, s[3].seq, s[4].batch, s[4].head, s[4].seq};
+    Maps maps = {};
+    if (p.prefix_tiles &&
+        ((rc = encode_keys(&maps.shared_k, "prefix_k", pk, n.dtype, D, n.prefix, n.kv_heads, 1, s[1], kStepKeys)) ||
+         (rc = encode_keys(&maps.shared_v, "prefix_v", pv, n.dtype, D, n.prefix, n.kv_heads, 1, s[2], kStepKeys))))
+        return rc;
+    if (n.cache && ((rc = encode_keys(&maps.own_k, "k", k, n.dtype, D, n.cache, n.kv_heads, n.batch, s[3], kStepKeys)) ||
+                    (rc = encode_keys(&maps.own_v, "v", v, n.dtype, D, n.cache, n.kv_heads, n.batch, s[4], kStepKeys))))
+        return rc;
     a.lens = n.seq_lens;
     a.batch = (int)n.batch, a.kv_heads = (int)n.kv_heads, a.prefix = p.prefix_tiles ? (int)n.prefix : 0, a.cache = (int)n.cache;
     a.rows = (int)p.rows, a.prefix_tiles = (int)p.prefix_tiles, a.own_tiles = (int)p.own_tiles;
@@ -560,13 +591,15 @@ int launch_all(const nb200_prefix_attn_args& n, const nb200_attn_strides* s, con
     a.sl2 = sl2;
     a.o = at(p.o), a.lse = at(p.lse), a.span = reinterpret_cast<int2*>(at(p.span));
     a.beside = p.splits > 0;  // the tensor cores' kernel started after all that came before
-    rc = p.mt == 1 ? launch_stream<T, D, 1>(a, p.ctas, limits[0], st) : launch_stream<T, D, 2>(a, p.ctas, limits[1], st);
+    rc = p.nt == 1   ? launch_stream<T, D, 1>(maps, a, p.ctas, limits[0], st)
+         : p.nt == 2 ? launch_stream<T, D, 2>(maps, a, p.ctas, limits[1], st)
+                     : launch_stream<T, D, 4>(maps, a, p.ctas, limits[2], st);
     if (rc) return rc;
     JoinArgs j = {};
     j.tensor_o = at(p.tensor_o), j.tensor_lse = at(p.tensor_lse), j.o = a.o, j.lse = a.lse, j.span = a.span;
     j.out = o, j.out_lse = lse, j.lens = n.seq_lens;
     j.kv_heads = a.kv_heads, j.group = query.group, j.tokens = query.tokens, j.rows = a.rows, j.cache = a.cache;
-    j.splits = p.splits, j.prefix_tiles = a.prefix_tiles, j.own_tiles = a.own_tiles, j.tile_rows = 16 * p.mt;
+    j.splits = p.splits, j.prefix_tiles = a.prefix_tiles, j.own_tiles = a.own_tiles, j.tile_rows = 8 * p.nt;
     j.slot_rows = a.slot_rows;
     const int64_t rows = n.kv_heads * p.rows;
     // A warp per row while the rows fill the GPU and their parts are few.
@@ -579,11 +612,33 @@ int launch_all(const nb200_prefix_attn_args& n, const nb200_attn_strides* s, con
 }
 
 }  // namespace
+
+int encode_keys(CUtensorMap* map, const char* what, const void* base, int dtype, int64_t d, int64_t keys, int64_t heads,
+                int64_t batch, const nb200_attn_strides& s, uint32_t box_keys) {
+    const auto enc = tensor_map_encoder("nb200_prefix_attention");
+    if (!enc) return NB200_ERR_LAUNCH;
+    auto bytes = [d](int64_t stride, int64_t size) { return (cuuint64_t)(size > 1 ? stride * 2 : d * 2); };
+    const cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)keys, (cuuint64_t)heads, (cuuint64_t)batch};
+    const cuuint64_t strides[3] = {bytes(s.seq, keys), bytes(s.head, heads), bytes(s.batch, batch)};
+    const cuuint32_t box[4] = {64, box_keys, 1, 1}, one[4] = {1, 1, 1, 1};
+    const CUresult rc = enc(map, dtype == NB200_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+                            const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (rc != CUDA_SUCCESS) {
+        set_error("nb200_prefix_attention: cannot describe %s as a tensor map (CUresult %d)", what, (int)rc);
+        return NB200_ERR_ARG;
+    }
+    return NB200_OK;
+}
+
 }  // namespace prefix
 
 using namespace prefix;
 
 int64_t prefix_attention_work_bytes(const nb200_prefix_attn_args& a) { return plan_of(a).bytes; }
+
+int prefix_stream_fault_take(unsigned int* bits) { return take_attn_fault(bits); }
 
 int launch_prefix_attention(const nb200_prefix_attn_args& n, const nb200_attn_strides* s, const void* q, const void* pk,
                             const void* pv, const void* k, const void* v, void* o, float* lse, void* work,
@@ -592,9 +647,9 @@ int launch_prefix_attention(const nb200_prefix_attn_args& n, const nb200_attn_st
     if (n.dtype == NB200_BF16)
         return n.head_dim == 128
                    ? launch_all<__nv_bfloat16, 128>(n, s, q, pk, pv, k, v, o, lse, w, g_shared, st)
-                   : launch_all<__nv_bfloat16, 64>(n, s, q, pk, pv, k, v, o, lse, w, g_shared + 2, st);
-    return n.head_dim == 128 ? launch_all<__half, 128>(n, s, q, pk, pv, k, v, o, lse, w, g_shared + 4, st)
-                             : launch_all<__half, 64>(n, s, q, pk, pv, k, v, o, lse, w, g_shared + 6, st);
+                   : launch_all<__nv_bfloat16, 64>(n, s, q, pk, pv, k, v, o, lse, w, g_shared + 3, st);
+    return n.head_dim == 128 ? launch_all<__half, 128>(n, s, q, pk, pv, k, v, o, lse, w, g_shared + 6, st)
+                             : launch_all<__half, 64>(n, s, q, pk, pv, k, v, o, lse, w, g_shared + 9, st);
 }
 
 }  // namespace nb200

@@ -2,6 +2,8 @@
 // result goes (prefix_attention.cu has the mathematics).
 #pragma once
 
+#include <cuda.h>
+
 #include <type_traits>
 
 #include "common.cuh"
@@ -38,6 +40,11 @@ struct TensorPart {
     float sl2;
     float *o, *lse;
 };
+// [batch, heads, keys, D] as a tensor map with a {64, box_keys} box and 128-byte swizzle. The stride of a dimension of one
+// element is never used and may be anything.
+int encode_keys(CUtensorMap* map, const char* what, const void* base, int dtype, int64_t d, int64_t keys, int64_t heads,
+                int64_t batch, const nb200_attn_strides& s, uint32_t box_keys);
+
 int tensor_splits(int64_t kv_heads, int64_t rows, int64_t keys);
 int launch_tensor_part(const TensorPart& a, int dtype, int64_t head_dim, const void* k, const nb200_attn_strides& ks,
                        const void* v, const nb200_attn_strides& vs, cudaStream_t st);

@@ -444,27 +444,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
-// [kv_heads, keys, D] as a tensor map with a {64, 128} box of one head and 128-byte swizzle. The stride of a
-// dimension of one element is never used and may be anything.
-int encode(CUtensorMap* map, const char* what, const void* base, int dtype, int64_t d, int64_t keys, int64_t heads,
-           const nb200_attn_strides& s) {
-    const auto enc = tensor_map_encoder("nb200_prefix_attention");
-    if (!enc) return NB200_ERR_LAUNCH;
-    auto bytes = [d](int64_t stride, int64_t size) { return (cuuint64_t)(size > 1 ? stride * 2 : d * 2); };
-    const cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)keys, (cuuint64_t)heads, 1};
-    const cuuint64_t strides[3] = {bytes(s.seq, keys), bytes(s.head, heads), (cuuint64_t)(d * 2)};
-    const cuuint32_t box[4] = {64, kKeys, 1, 1}, one[4] = {1, 1, 1, 1};
-    const CUresult rc = enc(map, dtype == NB200_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
-                            const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (rc != CUDA_SUCCESS) {
-        set_error("nb200_prefix_attention: cannot describe %s as a tensor map (CUresult %d)", what, (int)rc);
-        return NB200_ERR_ARG;
-    }
-    return NB200_OK;
-}
-
 SharedLimit g_shared[4];
 
 template <typename T, int D>
@@ -497,8 +476,8 @@ int launch_tensor_part(const TensorPart& a, int dtype, int64_t head_dim, const v
                        const void* v, const nb200_attn_strides& vs, cudaStream_t st) {
     CUtensorMap mk, mv;
     int rc;
-    if ((rc = encode(&mk, "prefix_k", k, dtype, head_dim, a.keys, a.kv_heads, ks)) ||
-        (rc = encode(&mv, "prefix_v", v, dtype, head_dim, a.keys, a.kv_heads, vs)))
+    if ((rc = encode_keys(&mk, "prefix_k", k, dtype, head_dim, a.keys, a.kv_heads, 1, ks, kKeys)) ||
+        (rc = encode_keys(&mv, "prefix_v", v, dtype, head_dim, a.keys, a.kv_heads, 1, vs, kKeys)))
         return rc;
     if (dtype == NB200_BF16)
         return head_dim == 128 ? launch<__nv_bfloat16, 128>(mk, mv, a, g_shared[0], st)
