@@ -181,6 +181,9 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas)
                   const StreamArgs a) {
     constexpr uint32_t kBox = kStepKeys * 128;       // 64 columns of a step's keys, 128-byte swizzled
     constexpr uint32_t kTile = kBox * (D / 64);      // K or V of a step
+    // The next unit's query rows are loaded while this one's keys run, where there are registers to hold them:
+    // loaded between two units they would hold up the copies by a memory latency.
+    constexpr bool kAhead = NT <= 2;
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t full[kWarps][kStages];
     __shared__ int abort_flag[kWarps];
@@ -228,25 +231,33 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas)
     for (int i = 0; i < kStages - 1; ++i) copy(i);
 
     // Column tile n of this lane's accumulators: query rows 8 n + 2 (lane % 4) and the next one.
-    uint32_t qf[NT][D / 16][2];
+    uint32_t qf[NT][D / 16][2], next_q[kAhead ? NT : 1][D / 16][2];
     int limit[NT][2], lowest = 0;  // last key a row sees; of the unit's rows, the least
     float o[NT][D / 16][4], m[NT][2], l[NT][2];
     int nrows = 0;
-    auto begin = [&] {
-        const bool shared = use.batch < 0;
-        const int in_unit = use.tile * 8 * NT, own_rows = a.query.group * a.query.tokens;
-        const int row0 = (shared ? 0 : use.batch * own_rows) + in_unit;
-        nrows = min(8 * NT, (shared ? a.rows : own_rows) - in_unit);
-        lowest = shared ? use.keys - 1 : use.keys - a.query.tokens;
+    auto load_rows = [&](const Cursor& c, uint32_t(*q)[D / 16][2]) {
+        const bool shared = c.batch < 0;
+        const int own_rows = a.query.group * a.query.tokens;
+        const int row0 = (shared ? 0 : c.batch * own_rows) + c.tile * 8 * NT;
+        const int rows = (shared ? a.rows : own_rows) - c.tile * 8 * NT;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             const int in = 8 * n + (lane >> 2);
-            const T* q = query_row<T>(a.query, use.head, row0 + (in < nrows ? in : 0)) + 2 * (lane & 3);
+            const T* p = query_row<T>(a.query, c.head, row0 + (in < rows ? in : 0)) + 2 * (lane & 3);
 #pragma unroll
             for (int d = 0; d < D / 16; ++d)
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
-                    qf[n][d][h] = in < nrows ? *reinterpret_cast<const uint32_t*>(q + 16 * d + 8 * h) : 0u;
+                    q[n][d][h] = in < rows ? *reinterpret_cast<const uint32_t*>(p + 16 * d + 8 * h) : 0u;
+        }
+    };
+    auto begin = [&] {
+        const bool shared = use.batch < 0;
+        const int in_unit = use.tile * 8 * NT;
+        nrows = min(8 * NT, (shared ? a.rows : a.query.group * a.query.tokens) - in_unit);
+        lowest = shared ? use.keys - 1 : use.keys - a.query.tokens;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 limit[n][e] = shared ? use.keys - 1 : lowest + (in_unit + 8 * n + 2 * (lane & 3) + e) % a.query.tokens;
@@ -257,7 +268,14 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[n][d][e] = 0.f;
         }
+        if (kAhead && left > use.steps - use.step) {
+            Cursor c = use;
+            c.step = c.steps - 1;
+            c.next(a);
+            load_rows(c, next_q);
+        }
     };
+    load_rows(use, qf);
     begin();
     if (lane == 0 && use.step == 0) a.span[use.unit(a)].x = worker;
 
@@ -379,6 +397,14 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas)
         if (!left) break;
         use.next(a);
         if (lane == 0) a.span[use.unit(a)].x = worker;
+        if constexpr (kAhead) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int d = 0; d < D / 16; ++d) qf[n][d][0] = next_q[n][d][0], qf[n][d][1] = next_q[n][d][1];
+        } else {
+            load_rows(use, qf);
+        }
         begin();
     }
     // Every copy lands before the CTA may exit; `steps - to_get` were issued, of which `done` have been waited for.
@@ -404,10 +430,8 @@ struct JoinArgs {
 // sequence's first token (a free slot of the batch) reads out as zero with a log-sum-exp of -inf.
 template <typename T, int D, bool WIDE>
 __global__ void __launch_bounds__(256) join_kernel(const JoinArgs a) {
-    constexpr int E = D / 32, kTurns = WIDE ? 8 : 1;
+    constexpr int E = D / 32, kTurns = WIDE ? 8 : 1;  // parts of a turn are kTurns apart
     __shared__ float sh[WIDE ? 8 : 1][D], sh_sum[8];
-    pdl_wait();
-    pdl_trigger();
     const int64_t all = (int64_t)a.kv_heads * a.rows;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t id = WIDE ? blockIdx.x : (int64_t)blockIdx.x * 8 + warp;
@@ -415,55 +439,60 @@ __global__ void __launch_bounds__(256) join_kernel(const JoinArgs a) {
     const int head = (int)(id / a.rows), r = (int)(id % a.rows);
     const int t = r % a.tokens, g = r / a.tokens % a.group, b = r / a.tokens / a.group;
     const int64_t at = ((int64_t)b * a.kv_heads * a.group + head * a.group + g) * a.tokens + t;
+    // The lengths are older than the kernels ahead, which had them before this one could start.
     const int len = tokens_of(a.lens, b, a.cache);
+    pdl_wait();
+    pdl_trigger();
     float top = -NB200_INF, sum = 0.f, v[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) v[e] = 0.f;
     if (len - a.tokens + t >= 0) {
-        // Two runs of parts: rows `far + i far_step` of one array, `near + i near_step` of another.
+        // Two runs of parts: rows `far + i far_step` of one array, `near + i slot_rows` of another.
         const float *far_o = a.o, *far_lse = a.lse;
         int64_t far = 0, far_step = a.slot_rows;
         int nfar = 0;
-        if (a.splits) {
-            far_o = a.tensor_o, far_lse = a.tensor_lse, far = id, far_step = all, nfar = a.splits;
-        } else if (a.prefix_tiles) {
-            const int unit = head * a.prefix_tiles + r / a.tile_rows;
-            const int2 w = a.span[unit];
-            far = (int64_t)(w.x + unit) * a.slot_rows + r % a.tile_rows;
-            nfar = w.y - w.x + 1;
-        }
         const int in = r - b * a.group * a.tokens;
         const int unit = a.kv_heads * a.prefix_tiles + (b * a.kv_heads + head) * a.own_tiles + in / a.tile_rows;
         const int2 w = a.span[unit];
+        if (a.splits) {
+            far_o = a.tensor_o, far_lse = a.tensor_lse, far = id, far_step = all, nfar = a.splits;
+        } else if (a.prefix_tiles) {
+            const int shared = head * a.prefix_tiles + r / a.tile_rows;
+            const int2 u = a.span[shared];
+            far = (int64_t)(u.x + shared) * a.slot_rows + r % a.tile_rows;
+            nfar = u.y - u.x + 1;
+        }
         const int64_t near = (int64_t)(w.x + unit) * a.slot_rows + in % a.tile_rows;
         const int parts = nfar + w.y - w.x + 1;
         auto row_of = [&](int i) { return i < nfar ? far + i * far_step : near + (int64_t)(i - nfar) * a.slot_rows; };
         auto lse_of = [&](int i) { return i < parts ? (i < nfar ? far_lse : a.lse)[row_of(i)] : -NB200_INF; };
+        // Four o's in flight at a time, the first four before their weights are known.
+        float o[4][E];
+        auto load4 = [&](int i) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int part = min(i + k * kTurns, parts - 1);
+                const float* p = (part < nfar ? far_o : a.o) + row_of(part) * D + lane * E;
+                if constexpr (E == 4) *reinterpret_cast<float4*>(o[k]) = __ldg(reinterpret_cast<const float4*>(p));
+                else *reinterpret_cast<float2*>(o[k]) = __ldg(reinterpret_cast<const float2*>(p));
+            }
+        };
+        const int start = WIDE ? warp : 0;
+        load4(start);
         for (int i = lane; i < parts; i += 32) top = fmaxf(top, lse_of(i));
         top = warp_max(top);
-        for (int i0 = WIDE ? warp : 0; i0 < parts; i0 += 32 * kTurns) {
+        for (int i0 = start; i0 < parts; i0 += 32 * kTurns) {  // 32 parts, weighed by the 32 lanes
             const float x = lse_of(i0 + lane * kTurns);
             const float mine = x == -NB200_INF ? 0.f : ex2(x - top);  // NaN stays
             sum += mine;
-            // Four parts in flight; one without weight is not read.
             for (int i = 0; i < 32 && i0 + i * kTurns < parts; i += 4) {
-                float f[4], o[4][E];
+                if (i0 + i > start) load4(i0 + i * kTurns);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    f[k] = __shfl_sync(0xffffffffu, mine, i + k);
+                    const float f = __shfl_sync(0xffffffffu, mine, i + k);
 #pragma unroll
-                    for (int e = 0; e < E; ++e) o[k][e] = 0.f;
-                    if (f[k] != 0.f) {
-                        const int part = i0 + (i + k) * kTurns;
-                        const float* p = (part < nfar ? far_o : a.o) + row_of(part) * D + lane * E;
-                        if constexpr (E == 4) *reinterpret_cast<float4*>(o[k]) = __ldg(reinterpret_cast<const float4*>(p));
-                        else *reinterpret_cast<float2*>(o[k]) = __ldg(reinterpret_cast<const float2*>(p));
-                    }
+                    for (int e = 0; e < E; ++e) v[e] = f == 0.f ? v[e] : fmaf(f, o[k][e], v[e]);
                 }
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-#pragma unroll
-                    for (int e = 0; e < E; ++e) v[e] = fmaf(f[k], o[k][e], v[e]);
             }
         }
         sum = warp_sum(sum);

@@ -403,15 +403,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     pdl_trigger();
     // The query rows, into the 128-byte swizzled tiles that the products read; rows past the last are zero.
     if (warp < 8) {
+        // All copies of a thread in flight together: one after another their latencies took 15 us.
         const int rows = u.pair ? 2 * kRows : kRows;
         for (int i = threadIdx.x; i < rows * (D / 8); i += 256) {
             const int row = i / (D / 8), ch = i % (D / 8);
-            uint4 v = make_uint4(0u, 0u, 0u, 0u);
-            if (row < u.nrows) v = ld_keep(query_row<T>(a.query, u.head, u.row0 + row) + 8 * ch);
+            const T* src = query_row<T>(a.query, u.head, u.row0 + (row < u.nrows ? row : 0)) + 8 * ch;
             uint8_t* dst = smem + (row / kRows) * S::kTile + (ch >> 3) * S::kHalf + (row % kRows) * 128 +
                            (((ch & 7) ^ (row & 7)) << 4);
-            *reinterpret_cast<uint4*>(dst) = v;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src),
+                         "r"(row < u.nrows ? 16 : 0)
+                         : "memory");
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");
         fence_proxy_async();
     }
     tc::fence_before();
