@@ -28,11 +28,12 @@ constexpr int kWarps = 4;      // warps of a stream kernel's CTA, each a worker 
 constexpr int kCtas = 2;       // its CTAs per SM
 constexpr int kStepKeys = 16;  // keys of a worker's step
 constexpr int kStages = 3;     // steps of a worker in shared memory: one in use, two in flight
+constexpr int kEntry = 2;      // what a unit costs beside its steps, in steps
 
 // A unit of the stream kernel is a tile of 8 NT query rows and the keys they share: units of the prefix
 // (key/value head, row tile; none when the prefix runs on the tensor cores), then units of the caches
-// (sequence, key/value head, row tile). All units' steps of 16 keys stand in one line, of which every worker
-// takes an equal piece, whatever the sequences' lengths are. A piece covers the end of one unit, whole units,
+// (sequence, key/value head, row tile). All units' steps of 16 keys stand in one line, each unit's behind kEntry
+// places for its own start and end, and every worker takes an equal piece of the line, whatever the sequences' lengths are. A piece covers the end of one unit, whole units,
 // the beginning of another: worker w's result for unit u goes to slot w + u, which no other pair has, and
 // span[u] says which workers had a share in u.
 struct StreamArgs {
@@ -78,23 +79,26 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {  // an 8 x 8 matrix
 }
 
 __device__ __forceinline__ int steps_of(int keys) { return (keys + kStepKeys - 1) / kStepKeys; }
+// Places of a unit in the line.
+__device__ __forceinline__ int places_of(int keys) { return keys > 0 ? kEntry + steps_of(keys) : 0; }
 
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint64_t* bar) {
     tc::tma_load_4d(reinterpret_cast<void*>(__cvta_shared_to_generic(dst)), map, c0, c1, c2, c3, bar);
 }
 
-// A position in the line of steps.
+// A position in the line: a step of a unit, and how many places of the worker's piece are left from there on.
 struct Cursor {
     int batch;  // -1: a unit of the prefix
     int head, tile, step, steps, keys;
+    int left;   // <= 0: at the end
 
     __device__ __forceinline__ void sequence(const StreamArgs& a, int b) {
         batch = b, head = 0, tile = 0, keys = tokens_of(a.lens, b, a.cache), steps = steps_of(keys);
     }
-    // The next step; there is one.
-    __device__ __forceinline__ void next(const StreamArgs& a) {
-        if (++step < steps) return;
+    // The first step of the next unit; only while places are left.
+    __device__ __forceinline__ void next_unit(const StreamArgs& a) {
         step = 0;
+        left -= kEntry;
         if (++tile < (batch < 0 ? a.prefix_tiles : a.own_tiles)) return;
         tile = 0;
         if (++head < a.kv_heads) return;
@@ -102,65 +106,73 @@ struct Cursor {
         do sequence(a, ++b);
         while (steps == 0 && b + 1 < a.batch);
     }
+    __device__ __forceinline__ void next(const StreamArgs& a) {
+        --left;
+        if (++step == steps && left > 0) next_unit(a);
+    }
     __device__ __forceinline__ int unit(const StreamArgs& a) const {
         return batch < 0 ? head * a.prefix_tiles + tile
                          : a.kv_heads * a.prefix_tiles + (batch * a.kv_heads + head) * a.own_tiles + tile;
     }
 };
 
-// Steps per worker, and the cursor at step `at(per worker)`; a whole warp calls it.
+// The places of a worker's piece, and of the whole line; a whole warp calls it.
 __device__ __forceinline__ int64_t share_of(const StreamArgs& a, int64_t workers, int64_t& all) {
     const int lane = threadIdx.x & 31;
     int64_t own = 0;
     if (a.lens) {
-        for (int b = lane; b < a.batch; b += 32) own += steps_of(tokens_of(a.lens, b, a.cache));
+        for (int b = lane; b < a.batch; b += 32) own += places_of(tokens_of(a.lens, b, a.cache));
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) own += __shfl_xor_sync(0xffffffffu, own, o);
     } else {
-        own = (int64_t)a.batch * steps_of(a.cache);
+        own = (int64_t)a.batch * places_of(a.cache);
     }
-    all = (int64_t)a.kv_heads * ((int64_t)a.prefix_tiles * steps_of(a.prefix) + a.own_tiles * own);
+    all = (int64_t)a.kv_heads * ((int64_t)a.prefix_tiles * places_of(a.prefix) + a.own_tiles * own);
     return (all + workers - 1) / workers;
 }
-__device__ __forceinline__ Cursor cursor_at(const StreamArgs& a, int64_t at) {
+// The piece of `share` places from place `at` on (inside the line).
+__device__ __forceinline__ Cursor cursor_at(const StreamArgs& a, int64_t at, int share) {
     Cursor c;
-    const int64_t shared = (int64_t)a.kv_heads * a.prefix_tiles * steps_of(a.prefix);
+    const int64_t shared = (int64_t)a.kv_heads * a.prefix_tiles * places_of(a.prefix);
+    int unit, tiles;
     if (at < shared) {
-        c.batch = -1, c.keys = a.prefix, c.steps = steps_of(a.prefix);
-        const int unit = (int)(at / c.steps);
-        c.head = unit / a.prefix_tiles, c.tile = unit % a.prefix_tiles, c.step = (int)(at % c.steps);
-        return c;
-    }
-    at -= shared;
-    const int64_t each = (int64_t)a.kv_heads * a.own_tiles;
-    int b = 0;
-    if (a.lens) {  // 32 sequences at a time
-        const int lane = threadIdx.x & 31;
-        for (;; b += 32) {
-            const int64_t mine = b + lane < a.batch ? each * steps_of(tokens_of(a.lens, b + lane, a.cache)) : 0;
-            int64_t upto = mine;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= o) upto += x;
-            }
-            const unsigned past = __ballot_sync(0xffffffffu, upto > at);
-            if (past || b + 32 >= a.batch) {
-                const int pick = past ? __ffs(past) - 1 : 31;
-                at -= __shfl_sync(0xffffffffu, upto - mine, pick);
-                b += pick;
-                break;
-            }
-            at -= __shfl_sync(0xffffffffu, upto, 31);
-        }
+        c.batch = -1, c.keys = a.prefix, c.steps = steps_of(a.prefix), tiles = a.prefix_tiles;
     } else {
-        const int64_t steps = each * steps_of(a.cache);
-        b = (int)(at / steps);
-        at %= steps;
+        at -= shared;
+        tiles = a.own_tiles;
+        const int64_t each = (int64_t)a.kv_heads * tiles;
+        int b = 0;
+        if (a.lens) {  // 32 sequences at a time
+            const int lane = threadIdx.x & 31;
+            for (;; b += 32) {
+                const int64_t mine = b + lane < a.batch ? each * places_of(tokens_of(a.lens, b + lane, a.cache)) : 0;
+                int64_t upto = mine;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
+                    if (lane >= o) upto += x;
+                }
+                const unsigned past = __ballot_sync(0xffffffffu, upto > at);
+                if (past || b + 32 >= a.batch) {
+                    const int pick = past ? __ffs(past) - 1 : 31;
+                    at -= __shfl_sync(0xffffffffu, upto - mine, pick);
+                    b += pick;
+                    break;
+                }
+                at -= __shfl_sync(0xffffffffu, upto, 31);
+            }
+        } else {
+            const int64_t places = each * places_of(a.cache);
+            b = (int)(at / places);
+            at %= places;
+        }
+        c.sequence(a, b);
     }
-    c.sequence(a, b);
-    const int unit = (int)(at / c.steps);
-    c.head = unit / a.own_tiles, c.tile = unit % a.own_tiles, c.step = (int)(at % c.steps);
+    unit = (int)(at / (kEntry + c.steps));
+    c.head = unit / tiles, c.tile = unit % tiles;
+    const int place = (int)(at % (kEntry + c.steps)) - kEntry;
+    c.step = max(place, 0);
+    c.left = share - max(-place, 0);
     return c;
 }
 
@@ -201,17 +213,18 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas)
     const int64_t share = share_of(a, (int64_t)gridDim.x * kWarps, all);
     const int64_t first = worker * share;
     // The kernel that joins the parts waits for this one alone, so this one ends after the kernel ahead of it.
-    if (first >= all) {
+    Cursor use;
+    use.left = 0;
+    if (first < all) use = cursor_at(a, first, (int)min(share, all - first));
+    if (use.left <= 0) {
         if (a.beside) pdl_wait();
         return;
     }
-    int left = (int)min(share, all - first);  // steps to go
-    const int steps = left;
-    Cursor use = cursor_at(a, first), get = use;
-    int to_get = left;
+    Cursor get = use;
+    int sent = 0;
 
     auto copy = [&](int stage) {  // the cursor's step into a stage
-        if (to_get <= 0) return;
+        if (get.left <= 0) return;
         if (lane == 0) {
             const bool shared = get.batch < 0;
             const CUtensorMap *mk = shared ? &shared_k : &own_k, *mv = shared ? &shared_v : &own_v;
@@ -224,7 +237,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas)
                 tma_load(mine + stage * 2 * kTile + kTile + h * kBox, mv, 64 * h, key, get.head, b, bar);
             }
         }
-        if (--to_get) get.next(a);
+        ++sent;
+        get.next(a);
     };
     __syncwarp();
 #pragma unroll
@@ -242,13 +256,13 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas)
         const int rows = (shared ? a.rows : own_rows) - c.tile * 8 * NT;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const int in = 8 * n + (lane >> 2);
+            const int in = 8 * n + (lane >> 2);  // past the last row: the first one again, whose result is not stored
             const T* p = query_row<T>(a.query, c.head, row0 + (in < rows ? in : 0)) + 2 * (lane & 3);
 #pragma unroll
             for (int d = 0; d < D / 16; ++d)
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
-                    q[n][d][h] = in < rows ? *reinterpret_cast<const uint32_t*>(p + 16 * d + 8 * h) : 0u;
+                    q[n][d][h] = *reinterpret_cast<const uint32_t*>(p + 16 * d + 8 * h);
         }
     };
     auto begin = [&] {
@@ -268,10 +282,9 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[n][d][e] = 0.f;
         }
-        if (kAhead && left > use.steps - use.step) {
+        if (kAhead && use.left > use.steps - use.step) {
             Cursor c = use;
-            c.step = c.steps - 1;
-            c.next(a);
+            c.next_unit(a);
             load_rows(c, next_q);
         }
     };
@@ -366,10 +379,10 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas)
 
         ++done;
         if (++stage == kStages) stage = 0, phase ^= 1u;
-        --left;
         const bool ends = use.step + 1 == use.steps;
-        if (left && !ends) {
+        if (use.left > 1 && !ends) {
             ++use.step;
+            --use.left;
             continue;
         }
         // The worker's share of the unit is done.
@@ -394,8 +407,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas)
                 }
             }
         if (lane == 0 && ends) a.span[unit].y = worker;
-        if (!left) break;
         use.next(a);
+        if (use.left <= 0) break;
         if (lane == 0) a.span[use.unit(a)].x = worker;
         if constexpr (kAhead) {
 #pragma unroll
@@ -407,9 +420,9 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas)
         }
         begin();
     }
-    // Every copy lands before the CTA may exit; `steps - to_get` were issued, of which `done` have been waited for.
+    // Every copy lands before the CTA may exit; `sent` were issued, of which `done` have been waited for.
     if (!ok)
-        for (int i = done; i < steps - to_get; ++i) drain_bar(&full[warp][i % kStages], (i / kStages) & 1u);
+        for (int i = done; i < sent; ++i) drain_bar(&full[warp][i % kStages], (i / kStages) & 1u);
     if (a.beside) pdl_wait();
 }
 
@@ -550,8 +563,8 @@ Plan plan_of(const nb200_prefix_attn_args& a) {
     p.own_tiles = (own_rows + tile - 1) / tile;
     p.slot_rows = std::min(tile, most);
     p.units = a.kv_heads * (p.prefix_tiles + a.batch * p.own_tiles);
-    const int64_t prefix_steps = p.prefix_tiles ? (a.prefix + kStepKeys - 1) / kStepKeys : 0;
-    const int64_t own_steps = (a.cache + kStepKeys - 1) / kStepKeys;
+    auto places = [](int64_t keys) { return keys ? kEntry + (keys + kStepKeys - 1) / kStepKeys : 0; };
+    const int64_t prefix_steps = p.prefix_tiles ? places(a.prefix) : 0, own_steps = places(a.cache);
     const int64_t steps = a.kv_heads * (p.prefix_tiles * prefix_steps + a.batch * p.own_tiles * own_steps);
     p.ctas = std::max<int64_t>(1, std::min<int64_t>((steps + kWarps - 1) / kWarps, kCtas * (int64_t)sm_count()));
     const int64_t share = std::max<int64_t>(1, steps / (p.ctas * kWarps));
