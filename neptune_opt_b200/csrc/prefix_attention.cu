@@ -26,6 +26,10 @@ namespace {
 
 constexpr int kWarps = 4;      // warps of a stream kernel's CTA, each a worker of its own
 constexpr int kCtas = 2;       // its CTAs per SM
+#ifndef PIECES
+#define PIECES 3
+#endif
+constexpr int kPieces = PIECES;
 constexpr int kStepKeys = 16;  // keys of a worker's step
 constexpr int kStages = 3;     // steps of a worker in shared memory: one in use, two in flight
 constexpr int kEntry = 2;      // what a unit costs beside its steps, in steps
@@ -212,12 +216,14 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas)
     int64_t all;
     const int64_t share = share_of(a, (int64_t)gridDim.x * kWarps, all);
     const int64_t first = worker * share;
-    // The kernel that joins the parts waits for this one alone, so this one ends after the kernel ahead of it.
+    // The kernel that joins the parts waits for this one alone, so this one ends after the kernel ahead of it: its last
+    // CTA waits. (Were they all to wait, those that are done would hold their places against those to come.)
+    const bool waits = a.beside && blockIdx.x + 1 == gridDim.x;
     Cursor use;
     use.left = 0;
     if (first < all) use = cursor_at(a, first, (int)min(share, all - first));
     if (use.left <= 0) {
-        if (a.beside) pdl_wait();
+        if (waits) pdl_wait();
         return;
     }
     Cursor get = use;
@@ -423,7 +429,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas)
     // Every copy lands before the CTA may exit; `sent` were issued, of which `done` have been waited for.
     if (!ok)
         for (int i = done; i < sent; ++i) drain_bar(&full[warp][i % kStages], (i / kStages) & 1u);
-    if (a.beside) pdl_wait();
+    if (waits) pdl_wait();
 }
 
 struct JoinArgs {
@@ -555,7 +561,11 @@ Plan plan_of(const nb200_prefix_attn_args& a) {
     Plan p = {};
     const int64_t own_rows = a.heads / a.kv_heads * a.tokens;
     p.rows = a.batch * own_rows;
-    if (a.prefix && p.rows > kStreamRows) p.splits = tensor_splits(a.kv_heads, p.rows, a.prefix);
+    if (a.prefix && p.rows > kStreamRows) {
+        // With lengths that only the device knows, the caches are taken to be half full.
+        const int64_t bytes = a.batch * a.kv_heads * a.cache * a.head_dim * 4 / (a.seq_lens ? 2 : 1);
+        p.splits = tensor_splits(a.kv_heads, p.rows, a.prefix, bytes);
+    }
     const int64_t most = a.prefix && !p.splits ? p.rows : own_rows;
     p.nt = most <= 8 ? 1 : most <= 16 ? 2 : 4;
     const int64_t tile = 8 * p.nt;
@@ -566,7 +576,10 @@ Plan plan_of(const nb200_prefix_attn_args& a) {
     auto places = [](int64_t keys) { return keys ? kEntry + (keys + kStepKeys - 1) / kStepKeys : 0; };
     const int64_t prefix_steps = p.prefix_tiles ? places(a.prefix) : 0, own_steps = places(a.cache);
     const int64_t steps = a.kv_heads * (p.prefix_tiles * prefix_steps + a.batch * p.own_tiles * own_steps);
-    p.ctas = std::max<int64_t>(1, std::min<int64_t>((steps + kWarps - 1) / kWarps, kCtas * (int64_t)sm_count()));
+    // Beside the tensor cores' kernel, SMs become free at different times: shorter pieces, but of eight places at least.
+    p.ctas = kCtas * (int64_t)sm_count();
+    if (p.splits) p.ctas = std::max(p.ctas, std::min(kPieces * p.ctas, steps / (8 * kWarps)));
+    p.ctas = std::max<int64_t>(1, std::min<int64_t>((steps + kWarps - 1) / kWarps, p.ctas));
     const int64_t share = std::max<int64_t>(1, steps / (p.ctas * kWarps));
     p.most_parts = p.splits + (prefix_steps + own_steps) / share + 2;
     auto take = [&](int64_t floats) {

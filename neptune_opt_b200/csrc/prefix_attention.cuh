@@ -45,7 +45,8 @@ struct TensorPart {
 int encode_keys(CUtensorMap* map, const char* what, const void* base, int dtype, int64_t d, int64_t keys, int64_t heads,
                 int64_t batch, const nb200_attn_strides& s, uint32_t box_keys);
 
-int tensor_splits(int64_t kv_heads, int64_t rows, int64_t keys);
+// `other_bytes`: what the kernel beside it reads.
+int tensor_splits(int64_t kv_heads, int64_t rows, int64_t keys, int64_t other_bytes);
 int launch_tensor_part(const TensorPart& a, int dtype, int64_t head_dim, const void* k, const nb200_attn_strides& ks,
                        const void* v, const nb200_attn_strides& vs, cudaStream_t st);
 

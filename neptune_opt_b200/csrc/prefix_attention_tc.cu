@@ -47,6 +47,7 @@ template <int D> struct Shape {
 };
 
 struct Bars {
+    uint64_t q_full;
     uint64_t kv_full[8], kv_empty[8];
     uint64_t s_full[2], p_full[2][2];  // P is published in two halves of 64 keys
     uint64_t o_final;
@@ -165,8 +166,9 @@ __device__ __forceinline__ void mma_issuer(uint8_t* smem, Bars* b, uint32_t tmem
         tc::commit(&b->kv_empty[r.s]);
         r.next();
     };
-    bool ok = true;
-    if (u.pair) {
+    bool ok = wait_bar(&b->q_full, 0, abort);
+    if (!ok) {
+    } else if (u.pair) {
         if ((ok = arrived())) {
             scores(0);
             scores(1);
@@ -391,6 +393,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&b->kv_full[s], 1);
             mbar_init(&b->kv_empty[s], 1);
         }
+        mbar_init(&b->q_full, 8);  // one arrival per softmax warp
         mbar_init(&b->o_final, 1);
         b->abort = 0;
         fence_barrier_init();
@@ -399,11 +402,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::tmem_alloc(&b->tmem_base, kTmemCols);
         tc::tmem_relinquish();
     }
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tmem = b->tmem_base;
     pdl_wait();
     pdl_trigger();
-    // The query rows, into the 128-byte swizzled tiles that the products read; rows past the last are zero.
+    // Each role runs to the end of the kernel in its own branch (the register budget differs per branch); both
+    // end at barrier 0, after which the MMA warp frees the tensor memory.
     if (warp < 8) {
-        // All copies of a thread in flight together: one after another their latencies took 15 us.
+        // The query rows, into the 128-byte swizzled tiles that the products read, while the first K/V tiles come;
+        // rows past the last are zero. All copies of a thread in flight together: one after another their latencies took 15 us.
         const int rows = u.pair ? 2 * kRows : kRows;
         for (int i = threadIdx.x; i < rows * (D / 8); i += 256) {
             const int row = i / (D / 8), ch = i % (D / 8);
@@ -416,15 +425,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
         fence_proxy_async();
-    }
-    tc::fence_before();
-    __syncthreads();
-    tc::fence_after();
-    const uint32_t tmem = b->tmem_base;
-
-    // Each role runs to the end of the kernel in its own branch (the register budget differs per branch); both
-    // end at barrier 0, after which the MMA warp frees the tensor memory.
-    if (warp < 8) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&b->q_full);
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
         softmax_stream<T, D>(smem, b, tmem, a, u, split);
         tc::fence_before();
@@ -461,17 +463,22 @@ int launch(const CUtensorMap& mk, const CUtensorMap& mv, const TensorPart& a, Sh
 
 }  // namespace
 
-// Ranges of keys: the number that ends first, when a CTA takes its tiles and about four tiles' time for its
-// start and end, and one CTA runs on an SM.
-int tensor_splits(int64_t kv_heads, int64_t rows, int64_t keys) {
+// Ranges of keys. A CTA has an SM for itself, for about 8 us and 2 us a tile (1 us where its streams alternate); SMs
+// without one run the caches' workers beside it, which at the GPU's copy rate take 23 SM-us a MB. The number of ranges
+// for which both end first; the fewest of those, as every range is one more part to join.
+int tensor_splits(int64_t kv_heads, int64_t rows, int64_t keys, int64_t other_bytes) {
     const int64_t units = kv_heads * ((rows + 2 * kRows - 1) / (2 * kRows)), tiles = (keys + kKeys - 1) / kKeys;
-    const int64_t sms = sm_count();
+    const int64_t sms = sm_count(), per_tile = rows > kRows ? 2 : 1, other = other_bytes * 23 / 1000000;
     int64_t best = 1, least = INT64_MAX;
-    for (int64_t waves = 1; waves <= 4; ++waves) {
-        const int64_t s = std::max<int64_t>(1, std::min(waves * sms / units, tiles));
-        const int64_t cost = (units * s + sms - 1) / sms * ((tiles + s - 1) / s + 4);
+    auto consider = [&](int64_t s) {
+        if (s < 1 || s > tiles) return;
+        const int64_t each = 8 + per_tile * ((tiles + s - 1) / s);
+        const int64_t cost = std::max((units * s + sms - 1) / sms * each, (units * s * each + other) / sms);
         if (cost < least) best = s, least = cost;
-    }
+    };
+    const int64_t wave = std::max<int64_t>(1, sms / units);
+    for (int64_t i = 1; i <= 8; ++i) consider(wave * i / 8);
+    for (int64_t waves = 2; waves <= 4; ++waves) consider(waves * sms / units);
     return (int)best;
 }
 
