@@ -13,6 +13,8 @@
 // one write of the row's type and one byte.
 #include <cuda_fp8.h>
 
+#include <algorithm>
+
 #include "common.cuh"
 #include "launch.h"
 
@@ -199,7 +201,13 @@ int launch(const Norm8& a, cudaStream_t st) {
     constexpr int kThreads = TPR < 128 ? 128 : TPR;
     constexpr int kRows = TPR < 128 ? 128 / TPR : 1;
     auto kernel = norm8_kernel<T, GROUPED, VEC, TPR, NV>;
-    const int grid = persistent_grid(kernel, kThreads, 0, (a.rows + kRows - 1) / kRows, 0);
+    // As many CTAs as the GPU holds; asked once (the same for every device this library is built for).
+    static const int per_sm = [kernel] {
+        int n = 0;
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, kThreads, 0) != cudaSuccess || n < 1) n = 1;
+        return n;
+    }();
+    const int64_t grid = std::min((a.rows + kRows - 1) / kRows, (int64_t)per_sm * sm_count());
     launch_pdl(kernel, (unsigned)grid, kThreads, 0, st, a);
     count_launch();
     return finish_launch("nb200_norm8");

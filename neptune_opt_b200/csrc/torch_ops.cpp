@@ -51,6 +51,7 @@
 #include <dlfcn.h>
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/VariableTypeUtils.h>
@@ -672,6 +673,11 @@ at::Tensor distill_loss_bwd_cuda(const at::Tensor& grad_, const at::Tensor& x, c
 }
 
 // ------------------------------------------------------------------ the serving operators
+// A contiguous tensor on x's device, without the dispatcher's way to it: single-token calls are bound by the host.
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType dtype, const at::Tensor& x) {
+    return at::detail::empty_cuda(sizes, dtype, x.device(), std::nullopt);
+}
+
 // What prefix_attention asks of its tensors, symbolic sizes too.
 void check_prefix_attention(const at::Tensor& q, const at::Tensor& pk, const at::Tensor& pv, const at::Tensor& k,
                             const at::Tensor& v, const OptTensor& seq_lens, const char* what) {
@@ -693,6 +699,13 @@ void check_prefix_attention(const at::Tensor& q, const at::Tensor& pk, const at:
     check_seq_lens(seq_lens, q, what);
 }
 
+// As attn_rows, for [kv_heads, prefix, head_dim].
+at::Tensor prefix_rows(const at::Tensor& t) {
+    bool ok = t.stride(2) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+    for (int i = 0; i < 2; ++i) ok = ok && (t.size(i) <= 1 || (t.stride(i) > 0 && t.stride(i) % 8 == 0));
+    return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
 std::tuple<at::Tensor, at::Tensor> prefix_attention_cuda(const at::Tensor& q_, const at::Tensor& pk_,
                                                          const at::Tensor& pv_, const at::Tensor& k_,
                                                          const at::Tensor& v_, const OptTensor& seq_lens, double scale,
@@ -701,22 +714,20 @@ std::tuple<at::Tensor, at::Tensor> prefix_attention_cuda(const at::Tensor& q_, c
     check_cuda(q_, what);
     check_prefix_attention(q_, pk_, pv_, k_, v_, seq_lens, what);
     c10::cuda::CUDAGuard guard(q_.device());
-    const at::Tensor q = attn_rows(q_), pk = attn_rows(pk_.unsqueeze(0)), pv = attn_rows(pv_.unsqueeze(0));
-    const at::Tensor k = attn_rows(k_), v = attn_rows(v_);
-    at::Tensor o = at::empty(q.sizes(), q.options());
-    const auto f32 = q.options().dtype(at::kFloat);
-    at::Tensor lse = with_lse ? at::empty(q.sizes().slice(0, 3), f32) : at::empty({0}, f32);
-    const nb200_prefix_attn_args a = {q.size(0), q.size(1), k.size(1), q.size(2), q.size(3), pk.size(2), k.size(2),
+    const at::Tensor q = attn_rows(q_), k = attn_rows(k_), v = attn_rows(v_), pk = prefix_rows(pk_), pv = prefix_rows(pv_);
+    at::Tensor o = fresh(q.sizes(), q.scalar_type(), q);
+    at::Tensor lse = fresh(with_lse ? q.sizes().slice(0, 3) : at::IntArrayRef{0}, at::kFloat, q);
+    const nb200_prefix_attn_args a = {q.size(0), q.size(1), k.size(1), q.size(2), q.size(3), pk.size(1), k.size(2),
                                       present(seq_lens) ? seq_lens->data_ptr<int32_t>() : nullptr, dtype_code(q),
                                       (float)scale};
-    const nb200_attn_strides strides[5] = {attn_strides(q), attn_strides(pk), attn_strides(pv), attn_strides(k),
-                                           attn_strides(v)};
+    const nb200_attn_strides strides[5] = {attn_strides(q), {0, pk.stride(0), pk.stride(1)}, {0, pv.stride(0), pv.stride(1)},
+                                           attn_strides(k), attn_strides(v)};
     const int64_t bytes = api().prefix_attention_work_bytes(&a);
     if (bytes < 0) check((int)bytes, what);
-    at::Tensor work = at::empty({std::max<int64_t>(bytes, 16)}, q.options().dtype(at::kByte));
+    at::Tensor work = fresh({std::max<int64_t>(bytes, 16)}, at::kByte, q);
     check(api().prefix_attention(&a, strides, q.data_ptr(), pk.data_ptr(), pv.data_ptr(), k.data_ptr(), v.data_ptr(),
-                                 o.data_ptr(), with_lse ? lse.data_ptr<float>() : nullptr, work.data_ptr(),
-                                 work.numel(), stream_of(q)),
+                                 o.data_ptr(), with_lse ? lse.data_ptr<float>() : nullptr, work.data_ptr(), bytes,
+                                 stream_of(q)),
           what);
     return {o, lse};
 }
@@ -757,16 +768,16 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> norm8_cuda(const at::Tensor& x_, 
         residual = unit_rows(*residual_, a.rows);
         a.residual = residual.data_ptr();
         a.stride_residual = residual.stride(0);
-        y = at::empty(x_.sizes(), x_.options());
+        y = fresh(x_.sizes(), x_.scalar_type(), x_);
     } else {
-        y = none_like(x_);
+        y = fresh({0}, x_.scalar_type(), x_);
     }
-    at::Tensor q = at::empty(x_.sizes(), x_.options().dtype(dtype));
+    at::Tensor q = fresh(x_.sizes(), dtype, x_);
     std::vector<int64_t> shape = lead_shape(x_, false);
     TORCH_CHECK_VALUE(group >= 0 && (group == 0 || a.width % group == 0), what, ": width ", a.width,
                       " is not whole groups of ", group);
     shape.push_back(group ? a.width / group : 1);
-    at::Tensor scale = at::empty(shape, x_.options().dtype(at::kFloat));
+    at::Tensor scale = fresh(shape, at::kFloat, x_);
     check(api().norm8(&a, q.data_ptr(), scale.data_ptr<float>(), a.residual ? y.data_ptr() : nullptr, stream_of(x_)),
           what);
     return {q, scale, y};
@@ -846,7 +857,7 @@ at::Tensor penalize_logits_cuda(const at::Tensor& logits, const OptTensor& token
         TORCH_CHECK_VALUE(columns == (a.vocab + 31) / 32, what, ": allowed must hold ", (a.vocab + 31) / 32,
                           " words a row, got ", columns);
     }
-    at::Tensor out = at::empty(logits.sizes(), logits.options());
+    at::Tensor out = fresh(logits.sizes(), logits.scalar_type(), logits);
     check(api().penalize_logits(&a, out.data_ptr(), stream_of(logits)), what);
     return out;
 }
