@@ -434,7 +434,8 @@ int nb200_norm8(const nb200_norm8_args* args, void* q, float* scale, void* y, vo
  * bias index outside [0, vocab) is skipped. repetition, presence, frequency, temperature: fp32 [rows], each
  * nullable (no such step); the caller keeps repetition and temperature positive. allowed (nullable) is
  * [rows, ceil(vocab / 32)] int32, bit v % 32 of word v / 32. logits is [rows, vocab], out contiguous like it, of one
- * dtype; every tensor has unit column stride. biases <= 1024 (else NB200_ERR_CAPACITY). No counterpart in the
+ * dtype; every tensor has unit column stride. biases <= 1024 (else NB200_ERR_CAPACITY). work: device memory, 16-byte
+ * aligned, of nb200_penalize_logits_work_bytes(args) bytes (0 without history and biases). No counterpart in the
  * reference. */
 typedef struct {
     const void *logits, *tokens, *bias_index;
@@ -445,7 +446,8 @@ typedef struct {
     int64_t stride_logits, stride_tokens, stride_bias_index, stride_bias_value, stride_allowed; /* elements */
     int32_t dtype, token_dtype, bias_dtype;
 } nb200_logits_args;
-int nb200_penalize_logits(const nb200_logits_args* args, void* out, void* stream);
+int64_t nb200_penalize_logits_work_bytes(const nb200_logits_args* args);
+int nb200_penalize_logits(const nb200_logits_args* args, void* out, void* work, int64_t work_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -144,7 +144,8 @@ SIGNATURES = {
     "nb200_prefix_attention_work_bytes": (_i64, [_prefix]),
     "nb200_prefix_attention": (_int, [_prefix, _strides, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
     "nb200_norm8": (_int, [_norm8, _vp, _vp, _vp, _vp]),
-    "nb200_penalize_logits": (_int, [_logits, _vp, _vp]),
+    "nb200_penalize_logits_work_bytes": (_i64, [_logits]),
+    "nb200_penalize_logits": (_int, [_logits, _vp, _vp, _i64, _vp]),
 }
 
 _LOCK = threading.Lock()

@@ -770,7 +770,12 @@ int nb200_norm8(const nb200_norm8_args* args, void* q, float* scale, void* y, vo
     return launch_norm8(*args, q, scale, y, (cudaStream_t)stream);
 }
 
-int nb200_penalize_logits(const nb200_logits_args* args, void* out, void* stream) {
+int64_t nb200_penalize_logits_work_bytes(const nb200_logits_args* args) {
+    const int rc = check_logits("nb200_penalize_logits", args);
+    return rc ? rc : logits_work_bytes(*args);
+}
+
+int nb200_penalize_logits(const nb200_logits_args* args, void* out, void* work, int64_t work_bytes, void* stream) {
     const int rc = check_logits("nb200_penalize_logits", args);
     if (rc) return rc;
     if (args->rows == 0) return NB200_OK;
@@ -779,7 +784,12 @@ int nb200_penalize_logits(const nb200_logits_args* args, void* out, void* stream
         set_error("nb200_penalize_logits: null pointer");
         return NB200_ERR_ARG;
     }
-    return launch_logits(*args, out, (cudaStream_t)stream);
+    const int64_t need = logits_work_bytes(*args);
+    if (need && (!work || !aligned16(work) || work_bytes < need)) {
+        set_error("nb200_penalize_logits: work must hold %lld bytes, 16-byte aligned", (long long)need);
+        return NB200_ERR_ARG;
+    }
+    return launch_logits(*args, out, work, (cudaStream_t)stream);
 }
 
 }  // extern "C"

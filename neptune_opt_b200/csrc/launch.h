@@ -101,6 +101,7 @@ int launch_prefix_attention(const nb200_prefix_attn_args& a, const nb200_attn_st
                             const void* prefix_k, const void* prefix_v, const void* k, const void* v, void* o,
                             float* lse, void* work, cudaStream_t st);
 int launch_norm8(const nb200_norm8_args& a, void* q, float* scale, void* y, cudaStream_t st);
-int launch_logits(const nb200_logits_args& a, void* out, cudaStream_t st);
+int64_t logits_work_bytes(const nb200_logits_args& a);
+int launch_logits(const nb200_logits_args& a, void* out, void* work, cudaStream_t st);
 
 }  // namespace nb200

@@ -1,4 +1,4 @@
-// What a server does to the logits of each sequence before it samples, in one pass:
+// What a server does to the logits of each sequence before it samples:
 //
 //   x = l > 0 ? l / repetition : l * repetition    for tokens of the sequence's history (prompt or output)
 //   x -= frequency * count + presence              for tokens of its output, count = how often
@@ -6,167 +6,416 @@
 //   x /= temperature
 //   x = -inf                                       where the row's bit mask forbids the token
 //
-// A CTA owns one chunk of one row's vocabulary. It counts the row's history tokens of its chunk in shared
-// memory (integer atomics: no order changes the result), streams the chunk through registers and then
-// redoes the few biased tokens. The bound is HBM traffic, a read and a write of the logits; each chunk
-// reads the whole history again, from L2.
+// Nearly all tokens need only temperature and mask. The few that the history or the biases name are found first:
+// name_kernel marks them in bit maps of the vocabulary (one CTA per row; integer atomics, no order changes the result) and
+// leaves one entry for each, bucket by bucket of the vocabulary. sweep_kernel streams the logits through registers, tile by
+// tile, and writes a tile's named tokens once more while the tile's logits are in L1 and its results in L2.
+//
+// The bound is HBM traffic, a read and a write of the logits. Two other ways were built and measured on bf16
+// [512, 262144] with histories of 4096: counting in every tile of one kernel took 332 us (every tile reads the whole
+// history and waits for it), rewriting the named tokens behind the sweep 157 us (1% of the tokens, but a third of the
+// logits' sectors: they come from HBM a second time).
+#include <algorithm>
+
 #include "common.cuh"
 #include "launch.h"
 
 namespace nb200 {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr uint32_t kPrompt = 0x80000000u;  // beside the count of output tokens: the token is in the prompt
-
 struct Logits {
     nb200_logits_args n;
     void* out;
-    int chunk, chunks;
+    int tiles;             // of a row
+    int parts, range;      // CTAs of a row, each for `range` tokens of the vocabulary, that name tokens (0: there are none)
+    int slots;             // of a table of tokens that come again
+    int buckets, span;     // buckets of a row, each of 2^span tiles
+    int64_t most;          // entries of a part, at most
+    unsigned first;        // CTAs of the sweep that begin before the names are known
+    int* starts;           // [rows][parts][buckets + 1]: where a bucket's entries begin
+    uint4* entries;        // [rows][parts][most]: token, count in the output, bias, whether the history has it
 };
 
-struct RowParams {
-    float repetition, presence, frequency, inv_temperature;
+constexpr int kSweepThreads = 256, kSweepCtas = 6;  // an SM holds that many
+constexpr int kVectors = 4;  // of a thread, in flight together
+template <typename T> constexpr int kTileBits = 10 + (Elem<T>::V == 8 ? 3 : 2);
+template <typename T> constexpr int kTile = 1 << kTileBits<T>;
+static_assert(kTile<float> == kSweepThreads * kVectors * 4, "a tile is what a CTA's threads hold");
+
+// A row's pointers, and how many tokens lie before its first 16-byte boundary. Whole vectors start there, if input and
+// output share it; tile 0 holds the tokens before it, too.
+template <typename T>
+struct Row {
+    const T* x;
+    T* out;
+    const int32_t* allowed;
+    bool vec;
+    int head;
+    __device__ __forceinline__ Row(const Logits& a, int64_t row) {
+        const nb200_logits_args& n = a.n;
+        x = static_cast<const T*>(n.logits) + row * n.stride_logits;
+        out = static_cast<T*>(a.out) + row * n.vocab;
+        allowed = n.allowed ? n.allowed + row * n.stride_allowed : nullptr;
+        const uint32_t skew = (uint32_t)reinterpret_cast<uintptr_t>(x) & 15u;
+        vec = skew == ((uint32_t)reinterpret_cast<uintptr_t>(out) & 15u);
+        head = (int)min((int64_t)((16u - skew) & 15u) / (int64_t)sizeof(T), n.vocab);
+    }
 };
+
+// ------------------------------------------------------------------ the named tokens
+constexpr int kNameThreads = 512;
+// Counters of a bucket, for a warp to choose by its number: atomics on one address take their time one after another.
+constexpr int kCopies = 8;
+constexpr int kBiased = 1 << 30, kAlone = 1 << 29;  // beside a count: the token is biased, and not in the history
+constexpr int kTogether = 8;  // tokens of a thread on their way together
 
 __device__ __forceinline__ int64_t index_at(const void* p, int64_t i, int dtype) {
-    return dtype == NB200_I64 ? static_cast<const int64_t*>(p)[i] : static_cast<const int32_t*>(p)[i];
+    return dtype == NB200_I64 ? __ldg(static_cast<const long long*>(p) + i) : __ldg(static_cast<const int*>(p) + i);
 }
 
-// Penalties of one logit; c = its count and prompt bit.
-__device__ __forceinline__ float penalize(float x, uint32_t c, const RowParams& p) {
-    if (c == 0) return x;
-    x = x > 0.f ? x / p.repetition : x * p.repetition;
-    const uint32_t n = c & ~kPrompt;
-    return n ? x - p.frequency * (float)n - p.presence : x;
+// The finaliser of MurmurHash3 (Appleby): neighbours and arithmetic progressions spread like random numbers.
+__device__ __forceinline__ unsigned scatter(unsigned h) {
+    h = (h ^ (h >> 16)) * 0x85ebca6bu;
+    h = (h ^ (h >> 13)) * 0xc2b2ae35u;
+    return h ^ (h >> 16);
 }
 
-// 32 mask bits from token v on (those past the last word are 0).
-__device__ __forceinline__ uint32_t mask_bits(const int32_t* allowed, int64_t v, int64_t words) {
-    const int64_t w = v >> 5;
-    const uint32_t lo = (uint32_t)__ldg(allowed + w), hi = w + 1 < words ? (uint32_t)__ldg(allowed + w + 1) : 0u;
-    return __funnelshift_r(lo, hi, (uint32_t)v & 31u);
-}
-
-template <typename T, bool HISTORY>
-__global__ void __launch_bounds__(kThreads) logits_kernel(const Logits a) {
-    constexpr int V = Elem<T>::V;
-    extern __shared__ uint32_t counts[];
+// The named tokens of a row, or of `range` tokens of its vocabulary. A token's first mention sets its bit and makes its
+// entry, its first mention in the output sets another; only what comes again in the output, and what is biased, is kept
+// in a hash table with linear probing that the host makes large enough. (With all of them in the table the searches, a warp's longest
+// each time, made this kernel four times slower.) The kernel lives a few us, so latencies count: what a thread loads goes
+// out together, before the lengths are known.
+template <typename T>
+__global__ void __launch_bounds__(kNameThreads) name_kernel(const Logits a) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    const nb200_logits_args& n = a.n;
+    const int biases = (int)n.biases, words = (a.range + 127) / 128 * 4;
+    uint32_t* named = reinterpret_cast<uint32_t*>(smem);                  // [words]: bit v of the tokens that have an entry
+    uint32_t* put_out = named + words;                                    // [words]: those in the output
+    int* keys = reinterpret_cast<int*>(put_out + words);                  // [slots]: those tokens, -1 where empty
+    int* again = keys + a.slots;                                          // [slots]: how often after the first time, and flags
+    int* starts = again + a.slots;                                        // [buckets][kCopies], and the end
+    int* bias_token = starts + a.buckets * kCopies + 1;
+    float* bias_value = reinterpret_cast<float*>(bias_token + biases);
+    __shared__ int warp_sum[kNameThreads / 32 + 1], any_again, bias_again;
+    for (int i = threadIdx.x; i < words / 2; i += kNameThreads) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0u, 0u, 0u, 0u);
+    for (int i = threadIdx.x; i < a.slots; i += kNameThreads) keys[i] = -1, again[i] = 0;
+    const int counters = a.buckets * kCopies;
+    for (int i = threadIdx.x; i <= counters; i += kNameThreads) starts[i] = 0;
+    if (threadIdx.x == 0) any_again = bias_again = 0;
     pdl_wait();
     pdl_trigger();
-    const nb200_logits_args& n = a.n;
-    const int64_t row = blockIdx.x / (unsigned)a.chunks;
-    const int part = (int)(blockIdx.x % (unsigned)a.chunks);
-    const T* x = static_cast<const T*>(n.logits) + row * n.stride_logits;
-    T* out = static_cast<T*>(a.out) + row * n.vocab;
-    const int32_t* allowed = n.allowed ? n.allowed + row * n.stride_allowed : nullptr;
-    const int64_t words = (n.vocab + 31) / 32;
-    // Whole vectors start at the first 16-byte boundary of the row, where input and output share it.
-    const uint32_t skew = (uint32_t)reinterpret_cast<uintptr_t>(x) & 15u;
-    const bool vec = skew == ((uint32_t)reinterpret_cast<uintptr_t>(out) & 15u);
-    const int64_t head = min((int64_t)((16u - skew) & 15u) / (int64_t)sizeof(T), n.vocab);
-    const int64_t lo = part ? head + (int64_t)part * a.chunk : 0;
-    const int64_t hi = min(head + (int64_t)(part + 1) * a.chunk, n.vocab);
-    if (lo >= hi) return;
-
-    RowParams p;
-    p.repetition = n.repetition ? n.repetition[row] : 1.f;
-    p.presence = n.presence ? n.presence[row] : 0.f;
-    p.frequency = n.frequency ? n.frequency[row] : 0.f;
-    p.inv_temperature = n.temperature ? 1.f / n.temperature[row] : 1.f;
-
-    if constexpr (HISTORY) {
-        for (int i = threadIdx.x; i < (int)(hi - lo); i += kThreads) counts[i] = 0u;
-        __syncthreads();
-        const int64_t len = n.token_lens ? max((int64_t)0, min((int64_t)n.token_lens[row], n.history)) : n.history;
-        const int64_t prompt = n.prompt_lens ? n.prompt_lens[row] : 0;
-        for (int64_t i = threadIdx.x; i < len; i += kThreads) {
-            const int64_t v = index_at(n.tokens, row * n.stride_tokens + i, n.token_dtype);
-            if (v >= lo && v < hi) {
-                if (i < prompt) atomicOr(&counts[v - lo], kPrompt);
-                else atomicAdd(&counts[v - lo], 1u);
-            }
-        }
-        __syncthreads();
-    }
-    auto one = [&](int64_t v, float bias) {
-        float f = Elem<T>::to_f(x[v]);
-        if constexpr (HISTORY) f = penalize(f, counts[v - lo], p);
-        f = (f + bias) * p.inv_temperature;
-        if (allowed && !((uint32_t)allowed[v >> 5] >> (v & 31) & 1u)) f = -NB200_INF;
-        return Elem<T>::from_f(f);
-    };
-    if (vec) {
-        const int64_t body = part ? lo : head;
-        const int vectors = (int)((hi - body) / V);
-        if (!part)
-            for (int64_t v = threadIdx.x; v < head; v += kThreads) out[v] = one(v, 0.f);
-        for (int64_t v = body + (int64_t)vectors * V + threadIdx.x; v < hi; v += kThreads) out[v] = one(v, 0.f);
-        for (int i = threadIdx.x; i < vectors; i += kThreads) {
-            const int64_t v = body + (int64_t)i * V;
-            const uint4 raw = ld_stream(x + v);
-            const uint32_t ok = allowed ? mask_bits(allowed, v, words) : ~0u;
-            float f[V];
-            Elem<T>::unpack(raw, f);
+    const int64_t row = blockIdx.x / (unsigned)a.parts;
+    const int low = (int)(blockIdx.x % (unsigned)a.parts) * a.range;
+    const int64_t high = min((int64_t)low + a.range, n.vocab);
+    const Row<T> r(a, row);
+    const int64_t tokens = row * n.stride_tokens;
+    auto here = [&](int64_t v) { return v >= low && v < high ? (int)v : -1; };
+    int token[kTogether], bias[2];
+    auto load = [&](int64_t i0) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                if constexpr (HISTORY) f[j] = penalize(f[j], counts[v - lo + j], p);
-                f[j] = (ok >> j & 1u) ? f[j] * p.inv_temperature : -NB200_INF;
-            }
-            st_stream(out + v, Elem<T>::pack(f));
+        for (int k = 0; k < kTogether; ++k) {
+            const int64_t i = i0 + k * kNameThreads;
+            token[k] = i < n.history ? here(index_at(n.tokens, tokens + i, n.token_dtype)) : -1;
         }
-    } else {
-        for (int64_t v = lo + threadIdx.x; v < hi; v += kThreads) out[v] = one(v, 0.f);
+    };
+    load(threadIdx.x);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int i = threadIdx.x + k * kNameThreads;
+        bias[k] = i < biases ? here(index_at(n.bias_index, row * n.stride_bias_index + i, n.bias_dtype)) : -1;
+        if (i < biases) {
+            bias_token[i] = bias[k];
+            bias_value[i] = __ldg(n.bias_value + row * n.stride_bias_value + i);
+        }
     }
-    if (n.biases) {
-        __syncthreads();  // the chunk is written
-        const int64_t at = row * n.stride_bias_index, val = row * n.stride_bias_value;
-        for (int64_t i = threadIdx.x; i < n.biases; i += kThreads) {
-            const int64_t v = index_at(n.bias_index, at + i, n.bias_dtype);
-            if (v < lo || v >= hi) continue;
-            // The first entry of a token adds all of them, in their order.
-            bool first = true;
-            for (int64_t j = 0; j < i && first; ++j) first = index_at(n.bias_index, at + j, n.bias_dtype) != v;
-            if (!first) continue;
-            float bias = n.bias_value[val + i];
-            for (int64_t j = i + 1; j < n.biases; ++j)
-                if (index_at(n.bias_index, at + j, n.bias_dtype) == v) bias += n.bias_value[val + j];
-            out[v] = one(v, bias);
+    const int64_t len = n.token_lens ? min((int64_t)n.token_lens[row], n.history) : n.history;
+    const int64_t prompt = n.prompt_lens ? n.prompt_lens[row] : 0;
+    __syncthreads();
+
+    const int shift = a.span + kTileBits<T>, copy = threadIdx.x / 32 % kCopies;
+    auto place = [&](int v, int c) { return (max(v - r.head, 0) >> shift) * kCopies + c; };
+    auto bit = [&](int v) { return 1u << ((v - low) & 31); };
+    // Whether v's bit in a map was set; it is now.
+    auto mark = [&](uint32_t* map, int v) { return (atomicOr(&map[(v - low) >> 5], bit(v)) & bit(v)) != 0u; };
+    // An entry for v, if it has none yet: its rank in its bucket (of the copy that the warp counts in), else -1.
+    auto enter = [&](int v) { return v < 0 || mark(named, v) ? -1 : atomicAdd(&starts[place(v, copy)], 1); };
+    // The table's slot of v, which is put there unless only looked for; -1 where it is not.
+    auto slot_of = [&](int v, bool put) {
+        unsigned s = __umulhi(scatter((unsigned)v), (unsigned)a.slots);
+        for (;; s = s + 1u == (unsigned)a.slots ? 0u : s + 1u) {
+            int key = *reinterpret_cast<volatile int*>(keys + s);
+            if (key == -1 && put) key = atomicCAS(&keys[s], -1, v);
+            if (key == v || (key == -1 && put)) return (int)s;
+            if (key == -1) return -1;
+        }
+    };
+    int rank[kTogether], bias_rank[2];
+#pragma unroll
+    for (int k = 0; k < kTogether; ++k) rank[k] = -1;
+    for (int64_t i0 = threadIdx.x; i0 < len;) {
+#pragma unroll
+        for (int k = 0; k < kTogether; ++k) {
+            const int64_t i = i0 + k * kNameThreads;
+            if (i >= len) break;
+            const int v = token[k];
+            rank[k] = enter(v);
+            if (v >= 0 && i >= prompt && mark(put_out, v)) {
+                any_again = 1;
+                atomicAdd(&again[slot_of(v, true)], 1);
+            }
+        }
+        if ((i0 += kTogether * kNameThreads) < len) load(i0);
+    }
+    // A biased token's entry belongs to the history where that names it, else to the bias that makes it.
+    if (biases) {
+        int at[2] = {-1, -1};
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            if (bias[k] >= 0) {
+                at[k] = slot_of(bias[k], true);
+                if (atomicOr(&again[at[k]], kBiased) & kBiased) bias_again = 1;
+            }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            bias_rank[k] = enter(bias[k]);
+            if (bias_rank[k] >= 0) atomicOr(&again[at[k]], kAlone);
+        }
+    }
+    __syncthreads();
+    // Counts of the buckets to their first places: exclusive sums, kNameThreads counters at a time.
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int* out_starts = a.starts + blockIdx.x * (int64_t)(a.buckets + 1);
+    int before = 0;
+    for (int b0 = 0; b0 <= counters; b0 += kNameThreads) {
+        const int b = b0 + threadIdx.x, own = b <= counters ? starts[b] : 0;
+        int upto = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += x;
+        }
+        if (lane == 31) warp_sum[warp] = upto;
+        __syncthreads();
+        if (warp == 0) {
+            const int sum = lane < kNameThreads / 32 ? warp_sum[lane] : 0;
+            int all = sum;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, all, o);
+                if (lane >= o) all += x;
+            }
+            if (lane <= kNameThreads / 32) warp_sum[lane] = all - sum;  // the last one: of all
+        }
+        __syncthreads();
+        const int base = before + warp_sum[warp];
+        before += warp_sum[kNameThreads / 32];
+        if (b <= counters) {  // a bucket's copies follow each other
+            starts[b] = base + upto - own;
+            if (b % kCopies == 0) out_starts[b / kCopies] = base + upto - own;
+        }
+        __syncthreads();
+    }
+    uint4* entries = a.entries + blockIdx.x * a.most;
+    // The sum of a token's biases, in the order in which they are given.
+    auto bias_of = [&](int v) {
+        float sum = 0.f;
+        for (int j = 0; j < biases; ++j)
+            if (bias_token[j] == v) sum += bias_value[j];
+        return sum;
+    };
+    const bool held = len <= kTogether * kNameThreads;  // every token's first finder still holds it
+    auto leave = [&](int v, int rank, float b, bool history) {
+        int count = (put_out[(v - low) >> 5] & bit(v)) ? 1 : 0;
+        if (history && (any_again || biases)) {
+            const int s = slot_of(v, false), c = s < 0 ? 0 : again[s];
+            if (c & kAlone) return;
+            if (c & kBiased) b = bias_of(v);
+            count += c & ~(kBiased | kAlone);
+        }
+        // Without ranks any place of the bucket will do.
+        const int at = held ? starts[place(v, copy)] + rank : atomicAdd(&starts[place(v, 0)], 1);
+        entries[at] = make_uint4((uint32_t)v, (uint32_t)count, __float_as_uint(b), history);
+    };
+    if (held) {
+#pragma unroll
+        for (int k = 0; k < kTogether; ++k)
+            if (rank[k] >= 0) leave(token[k], rank[k], 0.f, true);
+    } else {
+#pragma unroll 1
+        for (int w = threadIdx.x; w < words; w += kNameThreads)
+            for (uint32_t left = named[w]; left; left &= left - 1u) leave(low + 32 * w + __ffs(left) - 1, 0, 0.f, true);
+    }
+    if (biases) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            if (bias_rank[k] >= 0)
+                leave(bias[k], bias_rank[k], bias_again ? bias_of(bias[k]) : bias_value[threadIdx.x + k * kNameThreads], false);
+    }
+}
+
+// ------------------------------------------------------------------ the sweep
+// The mask's bits of `count` tokens from v on, the first in bit 0.
+__device__ __forceinline__ uint32_t mask_bits(const int32_t* allowed, int64_t v, int count) {
+    const int shift = (int)(v & 31);
+    const uint32_t lo = (uint32_t)__ldg(allowed + (v >> 5));
+    return shift + count <= 32 ? lo >> shift : __funnelshift_r(lo, (uint32_t)__ldg(allowed + (v >> 5) + 1), shift);
+}
+
+// Temperature and mask of a tile, and all of it for its named tokens.
+template <typename T, bool NAMED>
+__global__ void __launch_bounds__(kSweepThreads, kSweepCtas) sweep_kernel(const Logits a) {
+    constexpr int V = Elem<T>::V;
+    if (!NAMED) {  // else the inputs are older than name_kernel, which had them before this one could start
+        pdl_wait();
+        pdl_trigger();
+    }
+    const nb200_logits_args& n = a.n;
+    const int64_t row = blockIdx.x / (unsigned)a.tiles;
+    const int tile = (int)(blockIdx.x % (unsigned)a.tiles);
+    const Row<T> r(a, row);
+    const int64_t lo = tile ? min(r.head + (int64_t)tile * kTile<T>, n.vocab) : 0;
+    const int64_t hi = min(r.head + (int64_t)(tile + 1) * kTile<T>, n.vocab);
+    const int64_t body = r.vec && !tile ? r.head : lo;
+    const int vectors = r.vec ? (int)((hi - body) / V) : 0;
+    uint4 raw[kVectors];
+    uint32_t ok[kVectors];
+#pragma unroll
+    for (int k = 0; k < kVectors; ++k) {
+        const int i = threadIdx.x + k * kSweepThreads;
+        if (i < vectors) {
+            raw[k] = NAMED ? ld_keep(r.x + body + (int64_t)i * V) : ld_stream(r.x + body + (int64_t)i * V);
+            ok[k] = r.allowed ? mask_bits(r.allowed, body + (int64_t)i * V, V) : ~0u;
+        }
+    }
+    const float inv = n.temperature ? 1.f / n.temperature[row] : 1.f;
+    // A CTA of the first wave runs beside name_kernel and waits for it only behind its tile. Those that come later find
+    // it done, and have their entries on the way with the logits.
+    const bool later = NAMED && blockIdx.x >= a.first;
+    const int* starts = a.starts + row * a.parts * (a.buckets + 1) + (NAMED ? tile >> a.span : 0);
+    const uint4* entries = a.entries + row * a.parts * a.most;
+    int e0 = 0, e1 = 0;
+    uint4 entry = make_uint4(0u, 0u, 0u, 0u);
+    auto look_up = [&] {
+        pdl_wait();
+        pdl_trigger();
+        e0 = starts[0], e1 = starts[1];
+        if (e0 + (int)threadIdx.x < e1) entry = entries[e0 + threadIdx.x];
+    };
+    if (later) look_up();
+#pragma unroll
+    for (int k = 0; k < kVectors; ++k) {
+        const int i = threadIdx.x + k * kSweepThreads;
+        if (i < vectors) {
+            float f[V];
+            Elem<T>::unpack(raw[k], f);
+#pragma unroll
+            for (int j = 0; j < V; ++j) f[j] = ok[k] >> j & 1u ? f[j] * inv : -NB200_INF;
+            const uint4 o = Elem<T>::pack(f);
+            if (NAMED) *reinterpret_cast<uint4*>(r.out + body + (int64_t)i * V) = o;
+            else st_stream(r.out + body + (int64_t)i * V, o);
+        }
+    }
+    // What lies before the first vector and behind the last one, or all of it.
+    auto allows = [&](int64_t v) { return !r.allowed || ((uint32_t)__ldg(r.allowed + (v >> 5)) >> (v & 31) & 1u); };
+    auto one = [&](int64_t v) { r.out[v] = Elem<T>::from_f(allows(v) ? Elem<T>::to_f(r.x[v]) * inv : -NB200_INF); };
+    for (int64_t v = lo + threadIdx.x; v < body; v += kSweepThreads) one(v);
+    for (int64_t v = body + (int64_t)vectors * V + threadIdx.x; v < hi; v += kSweepThreads) one(v);
+    if constexpr (NAMED) {
+        const float rep = n.repetition ? n.repetition[row] : 1.f, inv_rep = 1.f / rep;
+        const float freq = n.frequency ? n.frequency[row] : 0.f, pres = n.presence ? n.presence[row] : 0.f;
+        if (!later) look_up();
+        __syncthreads();  // the tile is written
+#pragma unroll 1
+        for (int part = 0;;) {
+#pragma unroll 1
+            for (int e = e0 + threadIdx.x; e < e1;) {
+                const int64_t v = entry.x;
+                if (v >= lo && v < hi) {  // and not of another tile of the bucket
+                    float f = Elem<T>::to_f(r.x[v]);
+                    if (entry.w) f *= f > 0.f ? inv_rep : rep;
+                    if (entry.y) f = f - freq * (float)entry.y - pres;
+                    f = (f + __uint_as_float(entry.z)) * inv;
+                    r.out[v] = Elem<T>::from_f(allows(v) ? f : -NB200_INF);
+                }
+                if ((e += kSweepThreads) < e1) entry = entries[e];
+            }
+            if (++part == a.parts) break;
+            starts += a.buckets + 1, entries += a.most;
+            e0 = starts[0], e1 = starts[1];
+            if (e0 + (int)threadIdx.x < e1) entry = entries[e0 + threadIdx.x];
         }
     }
 }
 
+// ------------------------------------------------------------------ host side
+constexpr int kMostBuckets = 256, kMostBiases = 1024;
+constexpr int kMostTable = 5120, kMostRange = 1 << 18;  // tokens of a CTA that may come again; of its bit maps
+constexpr int slots_of(int tokens) { return tokens * 8 / 5 + 8; }
+constexpr int name_bytes(int range, int slots, int buckets, int biases) {
+    return (range + 127) / 128 * 32 + slots * 8 + (buckets * kCopies + 1) * 4 + biases * 8;
+}
+static_assert(kMostBiases <= 2 * kNameThreads, "two biases a thread");
+static_assert(name_bytes(kMostRange, slots_of(kMostTable + kMostBiases), kMostBuckets, kMostBiases) <= 200 << 10, "shared memory");
 SharedLimit g_shared[3];
 
+// The shapes of a call, and the bytes of its workspace.
+int64_t plan(Logits& a, int tile) {
+    const nb200_logits_args& n = a.n;
+    a.tiles = (int)((n.vocab + tile - 1) / tile);
+    const int64_t entries = std::min(n.history + n.biases, n.vocab);
+    if (!entries) return 0;
+    // The table stays three eighths empty at least. Where it, or the bit maps, would be too large, the vocabulary is dealt
+    // out to as many CTAs as it takes for every token of a range to fit, whatever the history holds.
+    const int64_t fits = n.history / 2 <= kMostTable ? kMostRange : kMostTable;
+    a.parts = (int)((n.vocab + fits - 1) / fits);
+    a.range = (int)((n.vocab + a.parts - 1) / a.parts);
+    a.slots = slots_of((int)std::min<int64_t>(n.history / 2, a.range) + (int)n.biases);
+    a.most = std::min<int64_t>(entries, a.range);
+    while (((a.tiles - 1) >> a.span) >= kMostBuckets) ++a.span;
+    a.buckets = ((a.tiles - 1) >> a.span) + 1;
+    a.first = (unsigned)(kSweepCtas * sm_count());
+    return n.rows * a.parts * (a.most * 16 + (a.buckets + 1) * 4);
+}
+
+int tile_of(int dtype) { return dtype == NB200_F32 ? kTile<float> : kTile<__half>; }
+
 template <typename T>
-int launch(Logits a, SharedLimit& shared, cudaStream_t st) {
+int launch(const Logits& a, SharedLimit& shared, cudaStream_t st) {
     const char* what = "nb200_penalize_logits";
     const nb200_logits_args& n = a.n;
-    // Chunks of 16384 tokens (64 KB of counts, three CTAs an SM), shorter ones while the CTAs do not fill the GPU.
-    int chunk = 16384;
-    while (chunk > 2048 && n.rows * ((n.vocab + chunk - 1) / chunk) < 3 * (int64_t)sm_count()) chunk /= 2;
-    a.chunk = chunk;
-    a.chunks = (int)((n.vocab + chunk - 1) / chunk);
-    if (n.rows * a.chunks > 0x7fffffffLL) {
+    if (n.rows * std::max(a.tiles, a.parts) > 0x7fffffffLL) {
         set_error("%s: rows=%lld, vocab=%lld exceed the kernel's index range", what, (long long)n.rows, (long long)n.vocab);
         return NB200_ERR_CAPACITY;
     }
-    const unsigned grid = (unsigned)(n.rows * a.chunks);
-    if (n.history) {
-        const uint32_t bytes = (16384 + 16) * 4;
-        if (const int rc = shared.raise(what, logits_kernel<T, true>, bytes)) return rc;
-        launch_pdl(logits_kernel<T, true>, grid, kThreads, (size_t)(chunk + 16) * 4, st, a);
+    const unsigned grid = (unsigned)(n.rows * a.tiles);
+    if (a.parts) {
+        const int most = name_bytes(kMostRange, slots_of(kMostTable + kMostBiases), kMostBuckets, kMostBiases);
+        if (const int rc = shared.raise(what, name_kernel<T>, most)) return rc;
+        launch_pdl(name_kernel<T>, (unsigned)(n.rows * a.parts), kNameThreads,
+                   name_bytes(a.range, a.slots, a.buckets, (int)n.biases), st, a);
+        launch_pdl(sweep_kernel<T, true>, grid, kSweepThreads, 0, st, a);
+        count_launch(2);
     } else {
-        launch_pdl(logits_kernel<T, false>, grid, kThreads, 0, st, a);
+        launch_pdl(sweep_kernel<T, false>, grid, kSweepThreads, 0, st, a);
+        count_launch();
     }
-    count_launch();
     return finish_launch(what);
 }
 
 }  // namespace
 
-int launch_logits(const nb200_logits_args& n, void* out, cudaStream_t st) {
-    const Logits a = {n, out, 0, 0};
+int64_t logits_work_bytes(const nb200_logits_args& n) {
+    Logits a = {n};
+    return plan(a, tile_of(n.dtype));
+}
+
+int launch_logits(const nb200_logits_args& n, void* out, void* work, cudaStream_t st) {
+    Logits a = {n, out};
+    plan(a, tile_of(n.dtype));
+    a.entries = static_cast<uint4*>(work);
+    a.starts = reinterpret_cast<int*>(a.entries + n.rows * a.parts * a.most);
     if (n.dtype == NB200_F32) return launch<float>(a, g_shared[0], st);
     if (n.dtype == NB200_BF16) return launch<__nv_bfloat16>(a, g_shared[1], st);
     return launch<__half>(a, g_shared[2], st);

@@ -88,6 +88,7 @@ struct Api {
     decltype(&nb200_prefix_attention_work_bytes) prefix_attention_work_bytes;
     decltype(&nb200_prefix_attention) prefix_attention;
     decltype(&nb200_norm8) norm8;
+    decltype(&nb200_penalize_logits_work_bytes) penalize_logits_work_bytes;
     decltype(&nb200_penalize_logits) penalize_logits;
 };
 
@@ -134,6 +135,7 @@ const Api& api() {
         bind(h, "nb200_prefix_attention_work_bytes", a.prefix_attention_work_bytes);
         bind(h, "nb200_prefix_attention", a.prefix_attention);
         bind(h, "nb200_norm8", a.norm8);
+        bind(h, "nb200_penalize_logits_work_bytes", a.penalize_logits_work_bytes);
         bind(h, "nb200_penalize_logits", a.penalize_logits);
     });
     return a;
@@ -858,7 +860,11 @@ at::Tensor penalize_logits_cuda(const at::Tensor& logits, const OptTensor& token
                           " words a row, got ", columns);
     }
     at::Tensor out = fresh(logits.sizes(), logits.scalar_type(), logits);
-    check(api().penalize_logits(&a, out.data_ptr(), stream_of(logits)), what);
+    const int64_t bytes = api().penalize_logits_work_bytes(&a);
+    if (bytes < 0) check((int)bytes, what);
+    at::Tensor work;
+    if (bytes) work = fresh({bytes}, at::kByte, logits);
+    check(api().penalize_logits(&a, out.data_ptr(), bytes ? work.data_ptr() : nullptr, bytes, stream_of(logits)), what);
     return out;
 }
 

@@ -248,16 +248,19 @@ def test_c_logits_refuses_before_any_launch():
     lib = L.load()
 
     def call(rows=4, vocab=100, history=0, biases=0, dtype=1, tdt=1, bdt=1, logits=1 << 20, tokens=None, bi=None, bv=None,
-             out=FAKE, stride=100):
+             out=FAKE, stride=100, work=FAKE, nbytes=1 << 30):
         a = L.NB200LogitsArgs(logits, tokens, bi, bv, None, None, None, None, None, None, None, rows, vocab, history, biases,
                               stride, 0, 0, 0, 0, dtype, tdt, bdt)
-        return lib.nb200_penalize_logits(ctypes.byref(a), out, NULL)
+        return lib.nb200_penalize_logits(ctypes.byref(a), out, work, nbytes, NULL)
 
     assert call(rows=0, logits=None) == L.NB200_OK
     for bad in ({"rows": -1}, {"vocab": 0}, {"history": -1}, {"biases": -1}, {"dtype": 4}, {"history": 5}, {"biases": 5},
                 {"history": 5, "tokens": 1 << 20, "tdt": 2}, {"biases": 5, "bi": 1 << 20}, {"logits": None}, {"out": NULL},
-                {"biases": 5, "bi": 1 << 20, "bv": 1 << 20, "bdt": 9}, {"stride": -100}):
+                {"biases": 5, "bi": 1 << 20, "bv": 1 << 20, "bdt": 9}, {"stride": -100},
+                {"history": 5, "tokens": 1 << 20, "work": NULL}, {"history": 5, "tokens": 1 << 20, "work": ODD},
+                {"history": 5, "tokens": 1 << 20, "nbytes": 64}):
         assert call(**bad) == L.NB200_ERR_ARG, bad
     assert call(biases=1025, bi=1 << 20, bv=1 << 20) == L.NB200_ERR_CAPACITY
     assert call(vocab=(1 << 30) + 1) == L.NB200_ERR_CAPACITY
-    assert lib.nb200_penalize_logits(None, FAKE, NULL) == L.NB200_ERR_ARG
+    assert lib.nb200_penalize_logits(None, FAKE, FAKE, 1 << 30, NULL) == L.NB200_ERR_ARG
+    assert lib.nb200_penalize_logits_work_bytes(None) == L.NB200_ERR_ARG
