@@ -68,48 +68,61 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) norm8_kernel(const Norm
         for (int k = 0; k < NV; ++k)
             wv[k] = column(k, 0) < a.width ? ld_keep(weight + column(k, 0)) : make_uint4(0u, 0u, 0u, 0u);
     }
-    int phase = 0;
-    for (int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / TPR; row < a.rows;
-         row += (int64_t)gridDim.x * kRows, phase ^= 1) {
+    // A row's loads go out together, and with whole vectors the next row's as soon as this one's are unpacked: they are in
+    // flight while the row waits for its sums.
+    const int64_t first = (int64_t)blockIdx.x * kRows + threadIdx.x / TPR, stride = (int64_t)gridDim.x * kRows;
+    uint4 xv[VEC ? NV : 1], rv[VEC ? NV : 1];
+    auto load = [&](int64_t row) {
         const T* x = static_cast<const T*>(a.x) + row * a.stride_x;
         const T* r = a.residual ? static_cast<const T*>(a.residual) + row * a.stride_residual : nullptr;
+#pragma unroll
+        for (int k = 0; k < (VEC ? NV : 0); ++k) {
+            const bool in = column(k, 0) < a.width;
+            xv[k] = in ? ld_stream(x + column(k, 0)) : make_uint4(0u, 0u, 0u, 0u);
+            rv[k] = in && r ? ld_stream(r + column(k, 0)) : make_uint4(0u, 0u, 0u, 0u);
+        }
+    };
+    if (VEC && first < a.rows) load(first);
+    int phase = 0;
+    for (int64_t row = first; row < a.rows; row += stride, phase ^= 1) {
         T* yo = a.y ? static_cast<T*>(a.y) + row * a.width : nullptr;
         float y[NV * V], top[GROUPED ? NV : 1];
         float sum = 0.f;
         if constexpr (VEC) {
-            uint4 xv[NV], rv[NV];
-#pragma unroll
-            for (int k = 0; k < NV; ++k) {
-                const bool in = column(k, 0) < a.width;
-                xv[k] = in ? ld_stream(x + column(k, 0)) : make_uint4(0u, 0u, 0u, 0u);
-                rv[k] = in && r ? ld_stream(r + column(k, 0)) : make_uint4(0u, 0u, 0u, 0u);
-            }
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
                 float f[V];
                 Elem<T>::unpack(xv[k], y + k * V);
-                if (r) {
-                    Elem<T>::unpack(rv[k], f);
+                Elem<T>::unpack(rv[k], f);
 #pragma unroll
-                    for (int j = 0; j < V; ++j) y[k * V + j] += f[j];
-                }
-                if (yo && column(k, 0) < a.width)
-                    *reinterpret_cast<uint4*>(yo + column(k, 0)) = Elem<T>::pack(y + k * V);
+                for (int j = 0; j < V; ++j) y[k * V + j] += f[j];
             }
+            if (row + stride < a.rows) load(row + stride);
         } else {
+            const T* x = static_cast<const T*>(a.x) + row * a.stride_x;
+            const T* r = a.residual ? static_cast<const T*>(a.residual) + row * a.stride_residual : nullptr;
+            T xs[NV * V], rs[NV * V];
 #pragma unroll
-            for (int k = 0; k < NV; ++k)
+            for (int i = 0; i < NV * V; ++i) {
+                const int c = min(column(i / V, i % V), a.width - 1);
+                xs[i] = x[c];
+                rs[i] = r ? r[c] : Elem<T>::from_f(0.f);
+            }
 #pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const int c = column(k, j);
-                    float v = 0.f;
-                    if (c < a.width) {
-                        v = Elem<T>::to_f(x[c]);
-                        if (r) v += Elem<T>::to_f(r[c]);
-                        if (yo) yo[c] = Elem<T>::from_f(v);
-                    }
-                    y[k * V + j] = v;
+            for (int i = 0; i < NV * V; ++i)
+                y[i] = column(i / V, i % V) < a.width ? Elem<T>::to_f(xs[i]) + Elem<T>::to_f(rs[i]) : 0.f;
+        }
+        if (yo) {
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                if constexpr (VEC) {
+                    if (column(k, 0) < a.width) *reinterpret_cast<uint4*>(yo + column(k, 0)) = Elem<T>::pack(y + k * V);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < V; ++j)
+                        if (column(k, j) < a.width) yo[column(k, j)] = Elem<T>::from_f(y[k * V + j]);
                 }
+            }
         }
         // Sum of squares, then y becomes weight * y.
         float most = 0.f;
