@@ -79,11 +79,30 @@ __device__ __forceinline__ void unpack2(const uint4& u, uint64_t* p) {
     for (int j = 0; j < Elem<T>::V / 2; ++j) p[j] = f2(f[2 * j], f[2 * j + 1]);
 }
 
-// TPR threads per row (a warp, or the CTA), NV vectors of V columns each. Vector k of thread t holds the V
-// columns from (t + k TPR) V on. Without VEC (a row off the 16-byte boundary, or a width that is no multiple
-// of V) columns are loaded one by one, and with a scale per row they are dealt out singly, so that a warp's
-// accesses stay side by side.
-template <typename T, bool GROUPED, bool VEC, int TPR, int NV>
+// How a row's columns are dealt out. TPR threads (a warp, or the CTA) hold NV vectors of V columns each.
+//   WHOLE    every row starts on a 16-byte boundary and is whole vectors
+//   SHIFTED  rows of a width that is no multiple of V, one behind the other: vectors start on 16-byte boundaries all the
+//            same, and the first and the last one of a row hold columns of its neighbours, too, which are left out of the
+//            sums and not stored (nor loaded, behind the last rows). The cut depends on the
+//            row's number modulo `period` alone; a worker takes rows of one residue, and its weights stay in registers.
+//            (bf16 [16384, 4001] took 203 us column by column.)
+//   SINGLE   any strides: columns are moved one by one, with a scale per row side by side over the threads
+enum Layout { WHOLE, SHIFTED, SINGLE };
+
+// Elements [c, c + V) of a row as a vector, 0 outside of it.
+template <typename T>
+__device__ __forceinline__ uint4 gather(const T* row, int c, int width) {
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int j = 0; j < Elem<T>::V; ++j) {
+        if (c + j < 0 || c + j >= width) continue;
+        if constexpr (sizeof(T) == 4) w[j] = __float_as_uint(row[c + j]);
+        else w[j / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(row)[c + j] << (16 * (j & 1));
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <typename T, bool GROUPED, Layout L, int TPR, int NV>
 __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) norm8_kernel(const Norm8 a) {
     constexpr int V = Elem<T>::V;
     constexpr int kWarps = TPR / 32;
@@ -92,27 +111,40 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) norm8_kernel(const Norm
     pdl_wait();
     pdl_trigger();
     const int t = threadIdx.x % TPR, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    auto column = [&](int k, int j) { return VEC || GROUPED ? (t + k * TPR) * V + j : t + (k * V + j) * TPR; };
+    constexpr bool VEC = L != SINGLE;
+    const int64_t first = (int64_t)blockIdx.x * kRows + threadIdx.x / TPR, stride = (int64_t)gridDim.x * kRows;
+    // Columns that the first vector of this worker's rows has before them.
+    const int lead = L == SHIFTED ? (int)(first * a.width % V) : 0;
+    auto column = [&](int k, int j) { return VEC || GROUPED ? (t + k * TPR) * V + j - lead : t + (k * V + j) * TPR; };
+    // Whether vector k lies in the row as a whole.
+    auto whole = [&](int k) {
+        return L == SHIFTED ? column(k, 0) >= 0 && column(k, 0) + V <= a.width : column(k, 0) < a.width;
+    };
+    auto fetch = [&](const T* row, int k, bool last) {
+        if (L != SHIFTED ? whole(k) : column(k, 0) < a.width && (!last || whole(k))) return ld_stream(row + column(k, 0));
+        if (L == SHIFTED && last) return gather(row, column(k, 0), a.width);
+        return make_uint4(0u, 0u, 0u, 0u);
+    };
     // The weight stays in registers over the rows.
     uint4 wv[VEC ? NV : 1];
     const T* weight = static_cast<const T*>(a.weight);
     if constexpr (VEC) {
 #pragma unroll
-        for (int k = 0; k < NV; ++k)
-            wv[k] = column(k, 0) < a.width ? ld_keep(weight + column(k, 0)) : make_uint4(0u, 0u, 0u, 0u);
+        for (int k = 0; k < NV; ++k) {
+            if constexpr (L == SHIFTED) wv[k] = gather(weight, column(k, 0), a.width);
+            else wv[k] = whole(k) ? ld_keep(weight + column(k, 0)) : make_uint4(0u, 0u, 0u, 0u);
+        }
     }
     // A row's loads go out together, and with whole vectors the next row's as soon as this one's are unpacked: they are in
     // flight while the row waits for its sums.
-    const int64_t first = (int64_t)blockIdx.x * kRows + threadIdx.x / TPR, stride = (int64_t)gridDim.x * kRows;
     uint4 xv[VEC ? NV : 1], rv[VEC ? NV : 1];
     auto load = [&](int64_t row) {
         const T* x = static_cast<const T*>(a.x) + row * a.stride_x;
         const T* r = a.residual ? static_cast<const T*>(a.residual) + row * a.stride_residual : nullptr;
 #pragma unroll
         for (int k = 0; k < (VEC ? NV : 0); ++k) {
-            const bool in = column(k, 0) < a.width;
-            xv[k] = in ? ld_stream(x + column(k, 0)) : make_uint4(0u, 0u, 0u, 0u);
-            rv[k] = in && r ? ld_stream(r + column(k, 0)) : make_uint4(0u, 0u, 0u, 0u);
+            xv[k] = fetch(x, k, (a.rows - 1 - row) * a.stride_x < V);  // less than a vector behind the row
+            if (r) rv[k] = fetch(r, k, (a.rows - 1 - row) * a.stride_residual < V);
         }
     };
     if (VEC && first < a.rows) load(first);
@@ -132,6 +164,18 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) norm8_kernel(const Norm
 #pragma unroll
                     for (int j = 0; j < V / 2; ++j) y[k * V / 2 + j] = add2(y[k * V / 2 + j], f[j]);
                 }
+            }
+            if constexpr (L == SHIFTED) {
+#pragma unroll
+                for (int k = 0; k < NV; ++k)
+                    if (!whole(k)) {
+#pragma unroll
+                        for (int j = 0; j < V; j += 2) {
+                            uint64_t& p = y[(k * V + j) / 2];
+                            const int c = column(k, j);
+                            p = f2(c >= 0 && c < a.width ? f2lo(p) : 0.f, c + 1 >= 0 && c + 1 < a.width ? f2hi(p) : 0.f);
+                        }
+                    }
             }
             if (row + stride < a.rows) load(row + stride);
         } else {
@@ -160,12 +204,12 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) norm8_kernel(const Norm
                 float f[V];
 #pragma unroll
                 for (int j = 0; j < V; ++j) f[j] = value(y, k * V + j);
-                if constexpr (VEC) {
-                    if (column(k, 0) < a.width) *reinterpret_cast<uint4*>(yo + column(k, 0)) = Elem<T>::pack(f);
-                } else {
+                if (VEC && whole(k)) {
+                    *reinterpret_cast<uint4*>(yo + column(k, 0)) = Elem<T>::pack(f);
+                } else if (L != WHOLE) {
 #pragma unroll
                     for (int j = 0; j < V; ++j)
-                        if (column(k, j) < a.width) yo[column(k, j)] = Elem<T>::from_f(f[j]);
+                        if (column(k, j) >= 0 && column(k, j) < a.width) yo[column(k, j)] = Elem<T>::from_f(f[j]);
                 }
             }
         }
@@ -256,57 +300,62 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) norm8_kernel(const Norm
             }
             uint32_t w[V / 4];
             to_bytes<V>(x, w, a.kind);
-            if constexpr (VEC) {
-                if (column(k, 0) < a.width) {
-                    if constexpr (V == 8) *reinterpret_cast<uint2*>(q + column(k, 0)) = make_uint2(w[0], w[1]);
-                    else *reinterpret_cast<uint32_t*>(q + column(k, 0)) = w[0];
-                }
-            } else {
+            if (VEC && whole(k)) {
+                if constexpr (V == 8) *reinterpret_cast<uint2*>(q + column(k, 0)) = make_uint2(w[0], w[1]);
+                else *reinterpret_cast<uint32_t*>(q + column(k, 0)) = w[0];
+            } else if (L != WHOLE) {
 #pragma unroll
                 for (int j = 0; j < V; ++j)
-                    if (column(k, j) < a.width) q[column(k, j)] = (uint8_t)(w[j / 4] >> (8 * (j & 3)));
+                    if (column(k, j) >= 0 && column(k, j) < a.width) q[column(k, j)] = (uint8_t)(w[j / 4] >> (8 * (j & 3)));
             }
         }
     }
 }
 
-template <typename T, bool GROUPED, bool VEC, int TPR, int NV>
+template <typename T, bool GROUPED, Layout L, int TPR, int NV>
 int launch(const Norm8& a, cudaStream_t st) {
     constexpr int kThreads = TPR < 128 ? 128 : TPR;
     constexpr int kRows = TPR < 128 ? 128 / TPR : 1;
-    auto kernel = norm8_kernel<T, GROUPED, VEC, TPR, NV>;
+    auto kernel = norm8_kernel<T, GROUPED, L, TPR, NV>;
     // As many CTAs as the GPU holds; asked once (the same for every device this library is built for).
     static const int per_sm = [kernel] {
         int n = 0;
         if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, kThreads, 0) != cudaSuccess || n < 1) n = 1;
         return n;
     }();
-    const int64_t grid = std::min((a.rows + kRows - 1) / kRows, (int64_t)per_sm * sm_count());
+    int64_t grid = std::min((a.rows + kRows - 1) / kRows, (int64_t)per_sm * sm_count());
+    if (L == SHIFTED) grid = std::max<int64_t>(grid / 8, 1) * 8;  // rows of one residue modulo V to a worker
     launch_pdl(kernel, (unsigned)grid, kThreads, 0, st, a);
     count_launch();
     return finish_launch("nb200_norm8");
 }
 
-template <typename T, bool GROUPED, bool VEC>
+template <typename T, bool GROUPED, Layout L>
 int by_width(const Norm8& a, cudaStream_t st) {
     constexpr int V = Elem<T>::V;
-    const int n = a.width;
-    if (n <= 256) return launch<T, GROUPED, VEC, 32, 8 / V>(a, st);
-    if (n <= 1024) return launch<T, GROUPED, VEC, 32, 32 / V>(a, st);
-    if (n <= 2048) return launch<T, GROUPED, VEC, 128, 16 / V>(a, st);
-    if (n <= 4096) return launch<T, GROUPED, VEC, 128, 32 / V>(a, st);
-    if (n <= 8192) return launch<T, GROUPED, VEC, 256, 32 / V>(a, st);
-    return launch<T, GROUPED, VEC, 512, 32 / V>(a, st);
+    const int n = a.width + (L == SHIFTED ? V - 1 : 0);  // columns of a row's vectors, at most
+    if (n <= 256) return launch<T, GROUPED, L, 32, 8 / V>(a, st);
+    if (n <= 1024) return launch<T, GROUPED, L, 32, 32 / V>(a, st);
+    if (n <= 2048) return launch<T, GROUPED, L, 128, 16 / V>(a, st);
+    if (n <= 4096) return launch<T, GROUPED, L, 128, 32 / V>(a, st);
+    if (n <= 8192) return launch<T, GROUPED, L, 256, 32 / V>(a, st);
+    if (n <= 16384) return launch<T, GROUPED, L, 512, 32 / V>(a, st);
+    return launch<T, GROUPED, SINGLE, 512, 32 / V>(a, st);  // the last few columns before the limit, shifted
 }
 
 template <typename T>
 int by_layout(const Norm8& a, cudaStream_t st) {
     constexpr int V = Elem<T>::V;
-    const bool vec = a.width % V == 0 && a.stride_x % V == 0 && (!a.residual || a.stride_residual % V == 0) &&
-                     aligned16(a.x) && aligned16(a.residual) && aligned16(a.weight) && aligned16(a.y) &&
-                     (reinterpret_cast<uintptr_t>(a.q) & 7u) == 0;
-    if (a.group != a.width) return vec ? by_width<T, true, true>(a, st) : by_width<T, true, false>(a, st);
-    return vec ? by_width<T, false, true>(a, st) : by_width<T, false, false>(a, st);
+    auto alike = [&](int64_t stride) { return stride >= a.width && (stride - a.width) % V == 0; };  // cut as y's rows are
+    const bool one = a.rows == 1;
+    const bool base = aligned16(a.x) && aligned16(a.residual) && aligned16(a.y) && (reinterpret_cast<uintptr_t>(a.q) & 7u) == 0;
+    const bool vec = base && (one || alike(a.stride_x)) && (one || !a.residual || alike(a.stride_residual));
+    auto even = [&](int64_t stride) { return one || stride % V == 0; };
+    const bool whole = base && a.width % V == 0 && even(a.stride_x) && (!a.residual || even(a.stride_residual)) &&
+                       aligned16(a.weight);
+    if (a.group != a.width) return whole ? by_width<T, true, WHOLE>(a, st) : by_width<T, true, SINGLE>(a, st);
+    if (whole) return by_width<T, false, WHOLE>(a, st);
+    return vec ? by_width<T, false, SHIFTED>(a, st) : by_width<T, false, SINGLE>(a, st);
 }
 
 }  // namespace

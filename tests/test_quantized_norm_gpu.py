@@ -131,6 +131,39 @@ def test_layouts(dtype, group):
     assert bool(((a[1] - b[1]).abs() <= 2.0 ** -20 * b[1]).all()) and torch.equal(a[2], b[2])
 
 
+@pytest.mark.parametrize("dtype", list(HALF_STEP))
+@pytest.mark.parametrize("rows,width", [(1, 3), (2, 3), (9, 1), (5, 5), (3, 9), (17, 33), (8, 4001)])
+def test_rows_off_the_boundary_up_to_the_end_of_their_memory(dtype, rows, width):
+    """Odd rows one behind the other, and overlapping ones: what lies around a row is neither read as part of it nor
+    written. NaN on all sides of the inputs, sentinels around the outputs (through the C entry)."""
+    import ctypes
+
+    import torch
+
+    import neptune_opt_b200._lib as L
+
+    x, w, r = make((rows, width), dtype, rows * width)
+    dt, n = x.dtype, rows * width
+    pad = 64
+    room = {k: torch.full((n + 2 * pad,), math.nan, device="cuda", dtype=dt) for k in ("x", "r")}
+    for k, t in (("x", x), ("r", r)):
+        room[k][pad:pad + n] = t.flatten()
+    q = torch.full((n + 2 * pad,), 77, device="cuda", dtype=torch.uint8)
+    y = torch.full((n + 2 * pad,), 3.0, device="cuda", dtype=dt)
+    scale = torch.empty(rows, 1, device="cuda")
+    at = lambda t: t.data_ptr() + pad * t.element_size()  # noqa: E731
+    code = {"float32": 0, "bfloat16": 1, "float16": 2}[dtype]
+    a = L.NB200Norm8Args(at(room["x"]), at(room["r"]), w.data_ptr(), rows, width, 0, width, width, code, 0, 1e-6)
+    L.check(L.load().nb200_norm8(ctypes.byref(a), at(q), scale.data_ptr(), at(y),
+                                 ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)), "norm8")
+    got = q[pad:pad + n].view(torch.float8_e4m3fn).view(rows, width), scale, y[pad:pad + n].view(rows, width)
+    check(x, w, r, None, "float8_e4m3fn", got=got)
+    for t, v in ((q, 77), (y, 3.0)):
+        assert bool((t[:pad] == v).all()) and bool((t[pad + n:] == v).all())
+    windows = room["x"][pad:pad + n].as_strided((max(1, n - width), width), (1, 1))
+    check(windows, w, None, None, "int8")
+
+
 @pytest.mark.parametrize("kind", list(KINDS))
 @pytest.mark.parametrize("group", [None, 64])
 @pytest.mark.parametrize("width", [256, 4096])
