@@ -9,7 +9,7 @@
 // and the maxima are taken in the same sweep over registers and one reduction serves both. Every value is
 // read once and kept in registers as fp32 until it is quantised.
 //
-// A row belongs to one warp (up to 1024 columns) or to one CTA. The bound is HBM traffic, two reads and one write of the
+// A row belongs to one warp (up to 512 columns) or to one CTA. The bound is HBM traffic, two reads and one write of the
 // row's type and one byte, with issue slots close behind: the arithmetic runs on packed pairs, and what depends on the
 // 8-bit type or the group is decided once per vector (28 instructions a value before, about 10 now).
 #include <cuda_fp8.h>
@@ -335,7 +335,10 @@ int by_width(const Norm8& a, cudaStream_t st) {
     constexpr int V = Elem<T>::V;
     const int n = a.width + (L == SHIFTED ? V - 1 : 0);  // columns of a row's vectors, at most
     if (n <= 256) return launch<T, GROUPED, L, 32, 8 / V>(a, st);
-    if (n <= 1024) return launch<T, GROUPED, L, 32, 32 / V>(a, st);
+    if (n <= 512) return launch<T, GROUPED, L, 32, 16 / V>(a, st);
+    // From here on a CTA a row: bf16 [65536, 1024] 75 us (a warp a row 80), fp32 [3003, 1001] 7.8 us (10.8); at 512 columns it is
+    // the other way round (137 us, 100).
+    if (n <= 1024) return launch<T, GROUPED, L, 128, 8 / V>(a, st);
     if (n <= 2048) return launch<T, GROUPED, L, 128, 16 / V>(a, st);
     if (n <= 4096) return launch<T, GROUPED, L, 128, 32 / V>(a, st);
     if (n <= 8192) return launch<T, GROUPED, L, 256, 32 / V>(a, st);
