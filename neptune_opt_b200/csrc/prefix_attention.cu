@@ -26,10 +26,6 @@ namespace {
 
 constexpr int kWarps = 4;      // warps of a stream kernel's CTA, each a worker of its own
 constexpr int kCtas = 2;       // its CTAs per SM
-#ifndef PIECES
-#define PIECES 3
-#endif
-constexpr int kPieces = PIECES;
 constexpr int kStepKeys = 16;  // keys of a worker's step
 constexpr int kStages = 3;     // steps of a worker in shared memory: one in use, two in flight
 constexpr int kEntry = 2;      // what a unit costs beside its steps, in steps
@@ -120,63 +116,52 @@ struct Cursor {
     }
 };
 
-// The places of a worker's piece, and of the whole line; a whole warp calls it.
-__device__ __forceinline__ int64_t share_of(const StreamArgs& a, int64_t workers, int64_t& all) {
+// The piece of the line that a worker takes (a whole warp calls it). Each lane sums up the places of a run of sequences;
+// the run that holds the piece's first place is then walked by its lane.
+__device__ __forceinline__ Cursor piece_of(const StreamArgs& a, int worker, int workers) {
     const int lane = threadIdx.x & 31;
-    int64_t own = 0;
+    const int64_t each = (int64_t)a.kv_heads * a.own_tiles;  // units of a sequence
+    const int run = (a.batch + 31) / 32, b0 = min(lane * run, a.batch), b1 = min(b0 + run, a.batch);
+    int own = 0;  // places of the lane's sequences, for one unit of each
     if (a.lens) {
-        for (int b = lane; b < a.batch; b += 32) own += places_of(tokens_of(a.lens, b, a.cache));
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) own += __shfl_xor_sync(0xffffffffu, own, o);
+#pragma unroll 8
+        for (int b = b0; b < b1; ++b) own += places_of(tokens_of(a.lens, b, a.cache));
     } else {
-        own = (int64_t)a.batch * places_of(a.cache);
+        own = (b1 - b0) * places_of(a.cache);
     }
-    all = (int64_t)a.kv_heads * ((int64_t)a.prefix_tiles * places_of(a.prefix) + a.own_tiles * own);
-    return (all + workers - 1) / workers;
-}
-// The piece of `share` places from place `at` on (inside the line).
-__device__ __forceinline__ Cursor cursor_at(const StreamArgs& a, int64_t at, int share) {
-    Cursor c;
+    int upto = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += x;
+    }
     const int64_t shared = (int64_t)a.kv_heads * a.prefix_tiles * places_of(a.prefix);
-    int unit, tiles;
+    const int64_t all = shared + each * __shfl_sync(0xffffffffu, upto, 31);
+    const int64_t share = (all + workers - 1) / workers;
+    int64_t at = worker * share;
+    Cursor c;
+    c.left = 0;
+    if (at >= all) return c;
+    c.left = (int)min(share, all - at);
+    int tiles = a.prefix_tiles;
     if (at < shared) {
-        c.batch = -1, c.keys = a.prefix, c.steps = steps_of(a.prefix), tiles = a.prefix_tiles;
+        c.batch = -1, c.keys = a.prefix, c.steps = steps_of(a.prefix);
     } else {
         at -= shared;
         tiles = a.own_tiles;
-        const int64_t each = (int64_t)a.kv_heads * tiles;
-        int b = 0;
-        if (a.lens) {  // 32 sequences at a time
-            const int lane = threadIdx.x & 31;
-            for (;; b += 32) {
-                const int64_t mine = b + lane < a.batch ? each * places_of(tokens_of(a.lens, b + lane, a.cache)) : 0;
-                int64_t upto = mine;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
-                    if (lane >= o) upto += x;
-                }
-                const unsigned past = __ballot_sync(0xffffffffu, upto > at);
-                if (past || b + 32 >= a.batch) {
-                    const int pick = past ? __ffs(past) - 1 : 31;
-                    at -= __shfl_sync(0xffffffffu, upto - mine, pick);
-                    b += pick;
-                    break;
-                }
-                at -= __shfl_sync(0xffffffffu, upto, 31);
-            }
-        } else {
-            const int64_t places = each * places_of(a.cache);
-            b = (int)(at / places);
-            at %= places;
-        }
+        const int unit_at = (int)(at / each);  // the place, counted in one unit of each sequence
+        const int holder = __ffs(__ballot_sync(0xffffffffu, upto > unit_at)) - 1;
+        int b = b0, before = upto - own;
+        if (lane == holder)
+            for (int p; before + (p = places_of(tokens_of(a.lens, b, a.cache))) <= unit_at; ++b) before += p;
+        b = __shfl_sync(0xffffffffu, b, holder);
+        at -= each * __shfl_sync(0xffffffffu, before, holder);
         c.sequence(a, b);
     }
-    unit = (int)(at / (kEntry + c.steps));
+    const int places = kEntry + c.steps, unit = (int)(at / places), place = (int)(at - (int64_t)unit * places) - kEntry;
     c.head = unit / tiles, c.tile = unit % tiles;
-    const int place = (int)(at % (kEntry + c.steps)) - kEntry;
     c.step = max(place, 0);
-    c.left = share - max(-place, 0);
+    c.left -= max(-place, 0);
     return c;
 }
 
@@ -213,15 +198,10 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas)
     if (!a.beside) pdl_wait();
     pdl_trigger();
     const int worker = (int)blockIdx.x * kWarps + warp;
-    int64_t all;
-    const int64_t share = share_of(a, (int64_t)gridDim.x * kWarps, all);
-    const int64_t first = worker * share;
     // The kernel that joins the parts waits for this one alone, so this one ends after the kernel ahead of it: its last
     // CTA waits. (Were they all to wait, those that are done would hold their places against those to come.)
     const bool waits = a.beside && blockIdx.x + 1 == gridDim.x;
-    Cursor use;
-    use.left = 0;
-    if (first < all) use = cursor_at(a, first, (int)min(share, all - first));
+    Cursor use = piece_of(a, worker, (int)gridDim.x * kWarps);
     if (use.left <= 0) {
         if (waits) pdl_wait();
         return;
@@ -543,9 +523,10 @@ __global__ void __launch_bounds__(256) join_kernel(const JoinArgs a) {
 }
 
 // ------------------------------------------------------------------ host side
-// Up to this many query rows of a key/value head meet the prefix in the stream kernel; more go to the tensor
-// cores.
-constexpr int kStreamRows = 32;
+// Up to kStreamRows query rows of a key/value head meet the prefix in the stream kernel, and up to kFewRows if it is no
+// longer than kFewKeys; otherwise it goes to the tensor cores. bf16, 8 heads of 128: 4 rows, 8192 keys 12.4 us against 16.2;
+// 16 rows, 131072 keys 99 us against 90; 16 rows, 1000 keys 12.4 against 10.6, 300 keys 8.3 against 10.3.
+constexpr int kStreamRows = 8, kFewRows = 32, kFewKeys = 512;
 
 struct Plan {
     int64_t rows;                  // query rows of a key/value head
@@ -561,7 +542,7 @@ Plan plan_of(const nb200_prefix_attn_args& a) {
     Plan p = {};
     const int64_t own_rows = a.heads / a.kv_heads * a.tokens;
     p.rows = a.batch * own_rows;
-    if (a.prefix && p.rows > kStreamRows) {
+    if (a.prefix && p.rows > (a.prefix > kFewKeys ? kStreamRows : kFewRows)) {
         // With lengths that only the device knows, the caches are taken to be half full.
         const int64_t bytes = a.batch * a.kv_heads * a.cache * a.head_dim * 4 / (a.seq_lens ? 2 : 1);
         p.splits = tensor_splits(a.kv_heads, p.rows, a.prefix, bytes);
@@ -576,10 +557,7 @@ Plan plan_of(const nb200_prefix_attn_args& a) {
     auto places = [](int64_t keys) { return keys ? kEntry + (keys + kStepKeys - 1) / kStepKeys : 0; };
     const int64_t prefix_steps = p.prefix_tiles ? places(a.prefix) : 0, own_steps = places(a.cache);
     const int64_t steps = a.kv_heads * (p.prefix_tiles * prefix_steps + a.batch * p.own_tiles * own_steps);
-    // Beside the tensor cores' kernel, SMs become free at different times: shorter pieces, but of eight places at least.
-    p.ctas = kCtas * (int64_t)sm_count();
-    if (p.splits) p.ctas = std::max(p.ctas, std::min(kPieces * p.ctas, steps / (8 * kWarps)));
-    p.ctas = std::max<int64_t>(1, std::min<int64_t>((steps + kWarps - 1) / kWarps, p.ctas));
+    p.ctas = std::max<int64_t>(1, std::min<int64_t>((steps + kWarps - 1) / kWarps, kCtas * (int64_t)sm_count()));
     const int64_t share = std::max<int64_t>(1, steps / (p.ctas * kWarps));
     p.most_parts = p.splits + (prefix_steps + own_steps) / share + 2;
     auto take = [&](int64_t floats) {

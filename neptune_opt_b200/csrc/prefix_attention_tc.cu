@@ -463,18 +463,22 @@ int launch(const CUtensorMap& mk, const CUtensorMap& mv, const TensorPart& a, Sh
 
 }  // namespace
 
-// Ranges of keys. A CTA has an SM for itself, for about 8 us and 2 us a tile (1 us where its streams alternate); SMs
-// without one run the caches' workers beside it, which at the GPU's copy rate take 23 SM-us a MB. The number of ranges
-// for which both end first; the fewest of those, as every range is one more part to join.
+// Ranges of keys. A CTA has an SM for itself, for about 8 us and 2 us a tile (1 us where its streams alternate). The caches'
+// workers run beside it on the SMs that are left, at about 95 MB/ms each and 5800 together, and on all of them behind it.
+// The number of ranges for which both end first; the fewest of those, as every range is one more part to join.
 int tensor_splits(int64_t kv_heads, int64_t rows, int64_t keys, int64_t other_bytes) {
     const int64_t units = kv_heads * ((rows + 2 * kRows - 1) / (2 * kRows)), tiles = (keys + kKeys - 1) / kKeys;
-    const int64_t sms = sm_count(), per_tile = rows > kRows ? 2 : 1, other = other_bytes * 23 / 1000000;
-    int64_t best = 1, least = INT64_MAX;
+    const int64_t sms = sm_count();
+    const float per_tile = rows > kRows ? 2.f : 1.f, other = (float)other_bytes * 1e-3f;  // KB; KB a us below
+    int64_t best = 1;
+    float least = 1e30f;
     auto consider = [&](int64_t s) {
         if (s < 1 || s > tiles) return;
-        const int64_t each = 8 + per_tile * ((tiles + s - 1) / s);
-        const int64_t cost = std::max((units * s + sms - 1) / sms * each, (units * s * each + other) / sms);
-        if (cost < least) best = s, least = cost;
+        const int64_t waves = (units * s + sms - 1) / sms;
+        const float end = (float)waves * (8.f + per_tile * (float)((tiles + s - 1) / s));
+        const float beside = std::min(95.f * (float)(sms - units * s / waves), 5800.f);
+        const float cost = end + std::max(other - beside * end, 0.f) / 5800.f;
+        if (cost < 0.98f * least) best = s, least = cost;
     };
     const int64_t wave = std::max<int64_t>(1, sms / units);
     for (int64_t i = 1; i <= 8; ++i) consider(wave * i / 8);
