@@ -102,7 +102,8 @@ def check(s, got=None):
 
 @pytest.mark.parametrize("dtype", list(HALF_STEP))
 @pytest.mark.parametrize("vocab", [1, 7, 31, 32, 33, 1000, 4096, 5003, 16384, 16391, 50001])
-@pytest.mark.parametrize("history,biases,masked", [(0, 0, False), (0, 0, True), (60, 0, False), (0, 9, True), (200, 40, True)])
+@pytest.mark.parametrize("history,biases,masked", [(0, 0, False), (0, 0, True), (60, 0, False), (0, 9, True), (200, 40, True),
+                                                    (700, 200, True)])
 def test_against_the_formulas(dtype, vocab, history, biases, masked):
     check(make(5, vocab, dtype, history, biases, masked, seed=vocab))
 

@@ -257,8 +257,8 @@ def test_c_logits_refuses_before_any_launch():
     for bad in ({"rows": -1}, {"vocab": 0}, {"history": -1}, {"biases": -1}, {"dtype": 4}, {"history": 5}, {"biases": 5},
                 {"history": 5, "tokens": 1 << 20, "tdt": 2}, {"biases": 5, "bi": 1 << 20}, {"logits": None}, {"out": NULL},
                 {"biases": 5, "bi": 1 << 20, "bv": 1 << 20, "bdt": 9}, {"stride": -100},
-                {"history": 5, "tokens": 1 << 20, "work": NULL}, {"history": 5, "tokens": 1 << 20, "work": ODD},
-                {"history": 5, "tokens": 1 << 20, "nbytes": 64}):
+                {"history": 5000, "tokens": 1 << 20, "work": NULL}, {"history": 5000, "tokens": 1 << 20, "work": ODD},
+                {"history": 5000, "tokens": 1 << 20, "nbytes": 64}):
         assert call(**bad) == L.NB200_ERR_ARG, bad
     assert call(biases=1025, bi=1 << 20, bv=1 << 20) == L.NB200_ERR_CAPACITY
     assert call(vocab=(1 << 30) + 1) == L.NB200_ERR_CAPACITY
