@@ -40,8 +40,9 @@
 // The serving operators (the same, but without a gradient: one that is asked for is refused):
 //   prefix_attention(Tensor q, Tensor prefix_k, Tensor prefix_v, Tensor k, Tensor v, Tensor? seq_lens, float scale,
 //                    bool with_lse) -> (Tensor o, Tensor lse)
-//   norm8(Tensor x, Tensor weight, Tensor? residual, int group, ScalarType dtype, float eps)
-//              -> (Tensor q, Tensor scale, Tensor y)
+//   norm8(Tensor x, Tensor weight, Tensor? residual, int group, int kind, float eps)
+//              -> (Tensor q, Tensor scale, Tensor y)          kind 0 float8_e4m3fn, 1 float8_e5m2, 2 int8 (packages
+//                                                            hand a dtype on by another number)
 //   penalize_logits(Tensor logits, Tensor? tokens, Tensor? token_lens, Tensor? prompt_lens, Tensor? repetition,
 //                   Tensor? presence, Tensor? frequency, Tensor? bias_index, Tensor? bias_value, Tensor? allowed,
 //                   Tensor? temperature) -> Tensor
@@ -734,22 +735,21 @@ std::tuple<at::Tensor, at::Tensor> prefix_attention_cuda(const at::Tensor& q_, c
     return {o, lse};
 }
 
-int byte_kind(at::ScalarType t, const char* what) {
-    if (t == at::kFloat8_e4m3fn) return NB200_E4M3;
-    if (t == at::kFloat8_e5m2) return NB200_E5M2;
-    TORCH_CHECK_TYPE(t == at::kChar, what, ": dtype must be float8_e4m3fn, float8_e5m2 or int8, got ", t);
-    return NB200_I8;
+at::ScalarType byte_dtype(int64_t kind, const char* what) {
+    TORCH_CHECK_TYPE(kind >= NB200_E4M3 && kind <= NB200_I8, what, ": dtype must be float8_e4m3fn, float8_e5m2 or int8");
+    return kind == NB200_E4M3 ? at::kFloat8_e4m3fn : kind == NB200_E5M2 ? at::kFloat8_e5m2 : at::kChar;
 }
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor> norm8_cuda(const at::Tensor& x_, const at::Tensor& weight_,
-                                                          const OptTensor& residual_, int64_t group,
-                                                          at::ScalarType dtype, double eps) {
+                                                          const OptTensor& residual_, int64_t group, int64_t kind,
+                                                          double eps) {
     const char* what = "nb200.norm8";
+    const at::ScalarType dtype = byte_dtype(kind, what);
     check_strided(x_, what);
     check_cuda(x_, what);
     nb200_norm8_args a = {};
     a.dtype = dtype_code(x_);
-    a.kind = byte_kind(dtype, what);
+    a.kind = (int32_t)kind;
     TORCH_CHECK_VALUE(x_.dim() >= 1 && x_.size(-1) >= 1, what, ": x must be [..., width]");
     NormInputs::same_kind(weight_, x_, what);
     TORCH_CHECK_VALUE(weight_.dim() == 1 && weight_.size(0) == x_.size(-1), what,
@@ -955,11 +955,11 @@ std::tuple<at::Tensor, at::Tensor> prefix_attention_meta(const at::Tensor& q, co
             with_lse ? at::empty_symint(std::vector<c10::SymInt>(qs.begin(), qs.end() - 1), f32) : at::empty({0}, f32)};
 }
 std::tuple<at::Tensor, at::Tensor, at::Tensor> norm8_meta(const at::Tensor& x, const at::Tensor&,
-                                                          const OptTensor& residual, int64_t group,
-                                                          at::ScalarType dtype, double) {
+                                                          const OptTensor& residual, int64_t group, int64_t kind,
+                                                          double) {
     std::vector<c10::SymInt> shape = lead_sym_shape(x, false);
     shape.emplace_back(group > 0 ? x.sym_size(-1) / group : c10::SymInt(1));
-    return {at::empty_symint(x.sym_sizes(), x.options().dtype(dtype)),
+    return {at::empty_symint(x.sym_sizes(), x.options().dtype(byte_dtype(kind, "nb200.norm8"))),
             at::empty_symint(shape, x.options().dtype(at::kFloat)),
             present(residual) ? like_meta(x) : none_like(x)};
 }
@@ -1057,7 +1057,7 @@ TORCH_LIBRARY(nb200, m) {
           "-> Tensor");
     m.def("prefix_attention(Tensor q, Tensor prefix_k, Tensor prefix_v, Tensor k, Tensor v, Tensor? seq_lens, "
           "float scale, bool with_lse) -> (Tensor, Tensor)");
-    m.def("norm8(Tensor x, Tensor weight, Tensor? residual, int group, ScalarType dtype, float eps) "
+    m.def("norm8(Tensor x, Tensor weight, Tensor? residual, int group, int kind, float eps) "
           "-> (Tensor, Tensor, Tensor)");
     m.def("penalize_logits(Tensor logits, Tensor? tokens, Tensor? token_lens, Tensor? prompt_lens, "
           "Tensor? repetition, Tensor? presence, Tensor? frequency, Tensor? bias_index, Tensor? bias_value, "

@@ -23,6 +23,8 @@ import struct
 from neptune_opt_b200.torch_op import run_cxx
 
 GROUPS = (16, 32, 64, 128)
+KINDS = {"float8_e4m3fn": 0, "float8_e5m2": 1, "int8": 2}
+_KINDS = None
 MAX_WIDTH = 16384
 
 
@@ -48,7 +50,7 @@ def validate_quantized_norm_inputs(x, weight, residual, group, dtype, eps):
             raise TypeError(f"{what}: {name} must share x's float32/bfloat16/float16 dtype, got {t.dtype}")
         if t.device != x.device:
             raise ValueError(f"{what}: {name} must be on the device of x")
-    if dtype not in (torch.float8_e4m3fn, torch.float8_e5m2, torch.int8):
+    if dtype not in (None, torch.float8_e4m3fn, torch.float8_e5m2, torch.int8):
         raise TypeError(f"{what}: dtype must be float8_e4m3fn, float8_e5m2 or int8, got {dtype}")
     if x.device.type not in ("cuda", "meta"):
         raise ValueError(f"{what}: inputs must be CUDA tensors, got {x.device}")
@@ -70,9 +72,12 @@ def quantized_rms_norm(x, weight, residual=None, *, group=None, dtype=None, eps:
     """(q, scale, y): the normalised rows in 8 bits (dtype, float8_e4m3fn by default), their fp32 scales
     [..., 1] or [..., width / group], and the new residual stream in x's dtype (None without a residual).
     All fresh and contiguous."""
-    import torch
+    global _KINDS
+    if _KINDS is None:
+        import torch
 
-    dtype = torch.float8_e4m3fn if dtype is None else dtype
-    q, scale, y = run_cxx("norm8", x, (x, weight, residual, 0 if group is None else group if group else -1, dtype, eps),
-                          validate_quantized_norm_inputs, x, weight, residual, group, dtype, eps)
+        _KINDS = {getattr(torch, name): kind for name, kind in KINDS.items()}
+        _KINDS[None] = KINDS["float8_e4m3fn"]
+    q, scale, y = run_cxx("norm8", x, (x, weight, residual, 0 if group is None else group if group else -1,
+                                       _KINDS.get(dtype, -1), eps), validate_quantized_norm_inputs, x, weight, residual, group, dtype, eps)
     return q, scale, None if residual is None else y
