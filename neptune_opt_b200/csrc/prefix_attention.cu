@@ -25,10 +25,11 @@ namespace prefix {
 namespace {
 
 constexpr int kWarps = 4;      // warps of a stream kernel's CTA, each a worker of its own
-constexpr int kCtas = 2;       // its CTAs per SM
 constexpr int kStepKeys = 16;  // keys of a worker's step
 constexpr int kStages = 3;     // steps of a worker in shared memory: one in use, two in flight
 constexpr int kEntry = 2;      // what a unit costs beside its steps, in steps
+// CTAs that an SM can hold: half the head dimension leaves room for twice as many.
+template <int D, int NT> constexpr int kCtas = D == 64 && NT <= 2 ? 4 : 2;
 
 // A unit of the stream kernel is a tile of 8 NT query rows and the keys they share: units of the prefix
 // (key/value head, row tile; none when the prefix runs on the tensor cores), then units of the caches
@@ -176,7 +177,7 @@ __device__ __forceinline__ Cursor piece_of(const StreamArgs& a, int worker, int 
 // Every wait is bounded; one that runs out sets bit 1 of the fault word, and the worker waits (again with a limit) for
 // its copies and leaves its slots unwritten.
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kWarps * 32, kCtas)
+__global__ void __launch_bounds__(kWarps * 32, kCtas<D, NT>)
     stream_kernel(const __grid_constant__ CUtensorMap shared_k, const __grid_constant__ CUtensorMap shared_v,
                   const __grid_constant__ CUtensorMap own_k, const __grid_constant__ CUtensorMap own_v,
                   const StreamArgs a) {
@@ -237,13 +238,15 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas)
     int nrows = 0;
     auto load_rows = [&](const Cursor& c, uint32_t(*q)[D / 16][2]) {
         const bool shared = c.batch < 0;
-        const int own_rows = a.query.group * a.query.tokens;
-        const int row0 = (shared ? 0 : c.batch * own_rows) + c.tile * 8 * NT;
-        const int rows = (shared ? a.rows : own_rows) - c.tile * 8 * NT;
+        const int first = c.tile * 8 * NT, rows = (shared ? a.rows : a.query.group * a.query.tokens) - first;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             const int in = 8 * n + (lane >> 2);  // past the last row: the first one again, whose result is not stored
-            const T* p = query_row<T>(a.query, c.head, row0 + (in < rows ? in : 0)) + 2 * (lane & 3);
+            int seq = c.batch, g = first + (in < rows ? in : 0), tok = 0;
+            if (a.query.tokens > 1) tok = g % a.query.tokens, g /= a.query.tokens;
+            if (shared) seq = g / a.query.group, g %= a.query.group;
+            const T* p = static_cast<const T*>(a.query.q) + seq * a.query.qb +
+                         (int64_t)(c.head * a.query.group + g) * a.query.qh + tok * a.query.qt + 2 * (lane & 3);
 #pragma unroll
             for (int d = 0; d < D / 16; ++d)
 #pragma unroll
@@ -260,7 +263,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas)
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                limit[n][e] = shared ? use.keys - 1 : lowest + (in_unit + 8 * n + 2 * (lane & 3) + e) % a.query.tokens;
+                limit[n][e] = shared ? use.keys - 1
+                              : lowest + (a.query.tokens > 1 ? (in_unit + 8 * n + 2 * (lane & 3) + e) % a.query.tokens : 0);
                 m[n][e] = -NB200_INF, l[n][e] = 0.f;
             }
 #pragma unroll
@@ -554,10 +558,16 @@ Plan plan_of(const nb200_prefix_attn_args& a) {
     p.own_tiles = (own_rows + tile - 1) / tile;
     p.slot_rows = std::min(tile, most);
     p.units = a.kv_heads * (p.prefix_tiles + a.batch * p.own_tiles);
-    auto places = [](int64_t keys) { return keys ? kEntry + (keys + kStepKeys - 1) / kStepKeys : 0; };
-    const int64_t prefix_steps = p.prefix_tiles ? places(a.prefix) : 0, own_steps = places(a.cache);
+    auto line = [](int64_t keys) { return keys ? kEntry + (keys + kStepKeys - 1) / kStepKeys : 0; };
+    const int64_t prefix_steps = p.prefix_tiles ? line(a.prefix) : 0, own_steps = line(a.cache);
     const int64_t steps = a.kv_heads * (p.prefix_tiles * prefix_steps + a.batch * p.own_tiles * own_steps);
-    p.ctas = std::max<int64_t>(1, std::min<int64_t>((steps + kWarps - 1) / kWarps, kCtas * (int64_t)sm_count()));
+    // Two CTAs an SM. Four where each worker still has 16 places and the SM holds four (caches of 256 sequences, head
+    // dimension 64: 33.5 us, with two 37.4; with few places the more parts cost more than that gives, 12.8 us against 10.9).
+    // Four, two at a time, beside the tensor cores' kernel where pieces are short anyway, because SMs become free at
+    // different times (32 sequences: 25.9 us against 26.9; 256 sequences, with long pieces, 101 against 96).
+    const int64_t sms = sm_count(), places = steps / (2 * sms * kWarps);
+    const bool four = (a.head_dim == 64 && p.nt <= 2 && places >= 32) || (p.splits && places < 32);
+    p.ctas = std::max<int64_t>(1, std::min<int64_t>((steps + kWarps - 1) / kWarps, (four ? 4 : 2) * sms));
     const int64_t share = std::max<int64_t>(1, steps / (p.ctas * kWarps));
     p.most_parts = p.splits + (prefix_steps + own_steps) / share + 2;
     auto take = [&](int64_t floats) {

@@ -16,14 +16,7 @@ struct Query {
     const void* q;
     int64_t qb, qh, qt;  // strides in elements
     int group, tokens;   // query heads per key/value head, new tokens per sequence
-};
-
-// Query row r = (b group + g) tokens + t of key/value head `head`.
-template <typename T>
-__device__ __forceinline__ const T* query_row(const Query& a, int head, int r) {
-    const int t = r % a.tokens, g = r / a.tokens % a.group, b = r / a.tokens / a.group;
-    return static_cast<const T*>(a.q) + b * a.qb + (int64_t)(head * a.group + g) * a.qh + t * a.qt;
-}
+};  // row r = (b group + g) tokens + t of key/value head `head` is q[b, head group + g, t]
 
 // Probabilities are rounded to the inputs' type for the product with the values. They are at most 2^8 (the
 // running maximum may lag behind by that much), so fp16 has room for 2^6 more: that keeps the probabilities of very

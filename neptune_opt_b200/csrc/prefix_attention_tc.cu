@@ -380,9 +380,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     u.head = (int)(id / (unsigned)a.splits);
     u.nrows = min(2 * kRows, a.rows - u.row0);
     u.pair = u.nrows > kRows;
-    const int64_t tiles = (a.keys + kKeys - 1) / kKeys;
-    u.tile0 = (int)(tiles * split / a.splits);
-    u.n = (int)(tiles * (split + 1) / a.splits) - u.tile0;
+    // The first tiles % splits ranges have a tile more.
+    const int tiles = (a.keys + kKeys - 1) / kKeys, each = tiles / a.splits, more = tiles % a.splits;
+    u.tile0 = split * each + min(split, more);
+    u.n = each + (split < more);
 
     if (threadIdx.x == 0) {
         for (int t = 0; t < 2; ++t) {
@@ -413,15 +414,28 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp < 8) {
         // The query rows, into the 128-byte swizzled tiles that the products read, while the first K/V tiles come;
         // rows past the last are zero. All copies of a thread in flight together: one after another their latencies took 15 us.
-        const int rows = u.pair ? 2 * kRows : kRows;
-        for (int i = threadIdx.x; i < rows * (D / 8); i += 256) {
-            const int row = i / (D / 8), ch = i % (D / 8);
-            const T* src = query_row<T>(a.query, u.head, u.row0 + (row < u.nrows ? row : 0)) + 8 * ch;
+        constexpr int kPieces = D / 8, kStep = 256 / kPieces;  // 16-byte pieces of a row; rows of one round of the threads
+        const int ch = threadIdx.x % kPieces, tokens = a.query.tokens, group = a.query.group;
+        int row = threadIdx.x / kPieces;
+        // Row row0 + row as (sequence, head, token); a round adds kStep rows, without a division.
+        int tok = (u.row0 + row) % tokens, g = (u.row0 + row) / tokens, seq = g / group;
+        g %= group;
+        const int add_tok = kStep % tokens, add_g = kStep / tokens % group, add_seq = kStep / tokens / group;
+        for (const int rows = u.pair ? 2 * kRows : kRows; row < rows; row += kStep) {
+            const bool in = row < u.nrows;
+            const T* src = static_cast<const T*>(a.query.q) +
+                           (in ? seq * a.query.qb + (int64_t)(u.head * group + g) * a.query.qh + tok * a.query.qt + 8 * ch : 0);
             uint8_t* dst = smem + (row / kRows) * S::kTile + (ch >> 3) * S::kHalf + (row % kRows) * 128 +
                            (((ch & 7) ^ (row & 7)) << 4);
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src),
-                         "r"(row < u.nrows ? 16 : 0)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(in ? 16 : 0)
                          : "memory");
+            tok += add_tok;
+            const bool carry = tok >= tokens;
+            tok -= carry ? tokens : 0;
+            g += add_g + carry;
+            const bool next = g >= group;
+            g -= next ? group : 0;
+            seq += add_seq + next;
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
         fence_proxy_async();
