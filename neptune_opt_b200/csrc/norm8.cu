@@ -31,7 +31,7 @@ struct Norm8 {
     int width, group;  // group = columns that share a scale
     int group_bits;    // log2 of it, where there is more than one
     int kind;
-    float eps, per_most;  // 1 / the type's largest value
+    float eps, most, per_most;  // the type's largest value, and one over it
 };
 
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -265,17 +265,22 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) norm8_kernel(const Norm
                 for (int k = 0; k < NV; ++k) top[k] = max_nan(top[k], __shfl_xor_sync(0xffffffffu, top[k], o));
         }
         uint8_t* q = static_cast<uint8_t*>(a.q) + row * a.width;
-        // A group's scale, and what takes weight * y to its quotients. The two factors are one product unless that overflows,
-        // as for the smallest scale.
+        // A group's scale, and what takes weight * y to its quotients: most / max |weight * y|, in which rsqrt has cancelled (two
+        // roundings between the values and their quotients, so that few land on another byte than the exact ones do). The
+        // smallest scale, an infinite one, NaN and a maximum whose own reciprocal leaves fp32 take the long way, in two factors.
         float s = 0.f;
         uint64_t by = 0, then = 0;
         auto take = [&](float m) {
             s = m * rstd * a.per_most;
-            s = s < 1.17549435e-38f ? 1.17549435e-38f : s;  // NaN stays
-            const float inv = reciprocal(s), both = rstd * inv;
-            const bool one = !(both > 3.4e38f);
-            by = f2(one ? both : rstd, one ? both : rstd);
-            then = f2(one ? 1.f : inv, one ? 1.f : inv);
+            const bool one = m > 1e-30f && m < 1e30f && s > 1.17549435e-38f && s < NB200_INF;
+            if (one) {
+                const float r = reciprocal(m), f = fmaf(r, fmaf(-m, r, 1.f), r) * a.most;
+                by = f2(f, f);
+            } else {
+                s = s < 1.17549435e-38f ? 1.17549435e-38f : s;  // NaN stays
+                const float inv = reciprocal(s);
+                by = f2(rstd, rstd), then = f2(inv, inv);
+            }
             return one;
         };
         bool one = true;
@@ -366,7 +371,7 @@ int by_layout(const Norm8& a, cudaStream_t st) {
 int launch_norm8(const nb200_norm8_args& n, void* q, float* scale, void* y, cudaStream_t st) {
     const float most = n.kind == NB200_E4M3 ? 448.f : n.kind == NB200_E5M2 ? 57344.f : 127.f;
     Norm8 a = {n.x, n.residual, n.weight, q, n.residual ? y : nullptr, scale, n.rows, n.stride_x, n.stride_residual,
-                     (int)n.width, (int)(n.group ? n.group : n.width), 0, n.kind, (float)n.eps, 1.f / most};
+                     (int)n.width, (int)(n.group ? n.group : n.width), 0, n.kind, (float)n.eps, most, 1.f / most};
     while (n.group && (1 << a.group_bits) < n.group) ++a.group_bits;
     if (n.dtype == NB200_F32) return by_layout<float>(a, st);
     if (n.dtype == NB200_BF16) return by_layout<__nv_bfloat16>(a, st);

@@ -196,6 +196,33 @@ def test_rows_of_zeros_and_values_that_are_not_numbers(kind, group, width):
     assert bool(torch.isnan(scale[0, 0])) and bool(torch.isnan(scale).all()) == (group is None)
 
 
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("group", [None, 64])
+def test_values_take_the_byte_that_is_nearest(kind, group):
+    """Without a residual a quotient is weight x / max |weight x| times the type's largest value: both products, the
+    reciprocal, its factor and the last product round once, and once more the conversion of the 64-bit quotient here.
+    With d = 6 2^-24 between the two, a byte is at most 2 d of the quotient further off than the nearest one."""
+    import torch
+
+    import neptune_opt_b200 as NB
+
+    x, w, _ = make((501, 1024), "float32", 5, residual=False)
+    q, _, _ = NB.quantized_rms_norm(x, w, group=group, dtype=getattr(torch, kind))
+    h = (x.double() * w.double()).view(501, -1, group or 1024)
+    quotient = (h / h.abs().amax(-1, keepdim=True) * KINDS[kind][0]).view_as(q)
+    nearest = quotient.round() if kind == "int8" else quotient.to(q.dtype).double()
+    further = (q.double() - quotient).abs() - (nearest - quotient).abs()
+    assert bool((further <= 2 * 6 * 2.0 ** -24 * quotient.abs()).all())
+
+
+@pytest.mark.parametrize("by,weight", [(1e-17, 1e-20), (1e-16, 1e-21), (1e17, 1e18)])
+def test_products_whose_reciprocal_leaves_fp32(by, weight):
+    """Where weight x is about 1e-37 or 1e35, its reciprocal times the largest value is not fp32's."""
+    x, w, _ = make((33, 512), "float32", 6, residual=False)
+    check(x * by, w * weight, None, None, "float8_e4m3fn", eps=1e-40)
+    check(x * by, w * weight, None, 128, "int8", eps=1e-40)
+
+
 def test_the_largest_value_fills_the_type():
     import torch
 
