@@ -174,6 +174,15 @@ int check_prefix_attention(const char* what, const nb200_prefix_attn_args* a, co
                   (long long)a->cache);
         return NB200_ERR_CAPACITY;
     }
+    // The steps of 16 keys that the tiles of 8 query rows take, which the kernels count in 32 bits for a worker, and for
+    // one tile of every sequence. (Only tensors whose rows overlap get this far.)
+    const int64_t own_tiles = a->heads / a->kv_heads * a->tokens / 8 + 1, tiles = a->batch * own_tiles;
+    const int64_t own_steps = a->batch * (a->cache / 16 + 3), prefix_steps = a->prefix / 16 + 3;
+    if (own_steps > most || (double)a->kv_heads * ((double)own_tiles * own_steps + (double)tiles * prefix_steps) > 0x1p40) {
+        set_error("%s: batch=%lld, prefix=%lld, cache=%lld exceed the kernel's index range", what, (long long)a->batch,
+                  (long long)a->prefix, (long long)a->cache);
+        return NB200_ERR_CAPACITY;
+    }
     // The copies' limits: multiples of 16 bytes, below 2^40 bytes.
     auto bad = [](int64_t stride, int64_t size) { return size > 1 && (stride < 8 || stride % 8 || stride >= (int64_t)1 << 39); };
     for (int i = 0; i < 5; ++i) {

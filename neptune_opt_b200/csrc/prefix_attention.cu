@@ -34,9 +34,9 @@ template <int D, int NT> constexpr int kCtas = D == 64 && NT <= 2 ? 4 : 2;
 // A unit of the stream kernel is a tile of 8 NT query rows and the keys they share: units of the prefix
 // (key/value head, row tile; none when the prefix runs on the tensor cores), then units of the caches
 // (sequence, key/value head, row tile). All units' steps of 16 keys stand in one line, each unit's behind kEntry
-// places for its own start and end, and every worker takes an equal piece of the line, whatever the sequences' lengths are. A piece covers the end of one unit, whole units,
-// the beginning of another: worker w's result for unit u goes to slot w + u, which no other pair has, and
-// span[u] says which workers had a share in u.
+// places for its own start and end, and every worker takes an equal piece of the line, whatever the sequences'
+// lengths are. A piece covers the end of one unit, whole units, the beginning of another: worker w's result for
+// unit u goes to slot w + u, which no other pair has, and span[u] says which workers had a share in u.
 struct StreamArgs {
     Query query;
     const int* lens;  // tokens of each sequence (null: all of the cache)

@@ -214,7 +214,8 @@ def test_c_prefix_attention_refuses_before_any_launch():
                 {"work": ODD}, {"work": NULL}, {"nbytes": 64}):
         assert _c_attention(**bad) == L.NB200_ERR_ARG, bad
     assert _c_attention(dim=96) == L.NB200_ERR_UNSUPPORTED and _c_attention(dim=0) == L.NB200_ERR_UNSUPPORTED
-    for big in ({"prefix": (1 << 30) + 1}, {"cache": (1 << 30) + 1}, {"tokens": 1 << 28}, {"batch": 1 << 28}):
+    for big in ({"prefix": (1 << 30) + 1}, {"cache": (1 << 30) + 1}, {"tokens": 1 << 28}, {"batch": 1 << 28},
+                {"batch": 1 << 15, "cache": 1 << 20}, {"batch": 1 << 13, "cache": 1 << 20, "heads": 4096, "kv": 4096}):
         assert _c_attention(**big) == L.NB200_ERR_CAPACITY, big
     s = L.NB200AttnStrides(8 * 16 * 128, 16 * 128, 128)
     for bad in (L.NB200AttnStrides(16384, 2049, 128), L.NB200AttnStrides(16384, 0, 128), L.NB200AttnStrides(16384, 1 << 39, 128)):
