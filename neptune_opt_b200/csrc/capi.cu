@@ -240,7 +240,7 @@ int check_logits(const char* what, const nb200_logits_args* a) {
         return NB200_ERR_ARG;
     }
     const int64_t most = (int64_t)1 << 30;
-    if (a->rows > most || a->vocab > most || a->history > most || a->biases > 1024) {
+    if (a->rows > most || a->vocab > most || a->history >= most / 2 || a->biases > 1024) {
         set_error("%s: rows=%lld, vocab=%lld, history=%lld or biases=%lld (at most 1024) exceed the kernel's range", what,
                   (long long)a->rows, (long long)a->vocab, (long long)a->history, (long long)a->biases);
         return NB200_ERR_CAPACITY;

@@ -217,6 +217,34 @@ def test_layouts():
         check(one)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("vocab,rows,history", [(1, 9, 0), (5, 9, 4), (15, 9, 4), (17, 9, 0), (23, 9, 4), (1003, 9, 40),
+                                                (1003, 9, 600), (8199, 9, 600), (16401, 3, 0), (16401, 3, 40),
+                                                (16401, 3, 600)])
+def test_rows_cut_differently_than_the_output(dtype, vocab, rows, history):
+    """Every pair of places behind a 16-byte boundary, the first and the last row at the ends of their memory, NaN
+    between the rows: bit for bit what contiguous logits give."""
+    import torch
+
+    import neptune_opt_b200 as NB
+
+    gen = torch.Generator(device="cuda").manual_seed(vocab + history)
+    x = torch.randn(rows, vocab, device="cuda", generator=gen).to(getattr(torch, dtype))
+    given = {"temperature": torch.rand(rows, device="cuda", generator=gen) + 0.5,
+             "allowed": torch.randint(-2 ** 31, 2 ** 31, (rows, -(-vocab // 32)), device="cuda", generator=gen).int()}
+    if history:
+        given |= {"tokens": torch.randint(0, vocab, (rows, history), device="cuda", generator=gen),
+                  "presence": torch.rand(rows, device="cuda", generator=gen),
+                  "frequency": torch.rand(rows, device="cuda", generator=gen)}
+    want = NB.penalize_logits(x, **given)
+    for at in range(8):
+        for pad in range(8):
+            room = torch.full((at + (rows - 1) * (vocab + pad) + vocab,), float("nan"), device="cuda", dtype=x.dtype)
+            strided = room.as_strided((rows, vocab), (vocab + pad, 1), at)
+            strided.copy_(x)
+            assert torch.equal(NB.penalize_logits(strided, **given), want), (at, pad)
+
+
 def test_offsets_past_32_bits():
     """Logits of which the later rows lie more than 2^32 elements from the first."""
     import torch

@@ -263,5 +263,6 @@ def test_c_logits_refuses_before_any_launch():
         assert call(**bad) == L.NB200_ERR_ARG, bad
     assert call(biases=1025, bi=1 << 20, bv=1 << 20) == L.NB200_ERR_CAPACITY
     assert call(vocab=(1 << 30) + 1) == L.NB200_ERR_CAPACITY
+    assert call(history=1 << 29) == L.NB200_ERR_CAPACITY
     assert lib.nb200_penalize_logits(None, FAKE, FAKE, 1 << 30, NULL) == L.NB200_ERR_ARG
     assert lib.nb200_penalize_logits_work_bytes(None) == L.NB200_ERR_ARG
