@@ -11,7 +11,8 @@
 //
 // A row belongs to one warp (up to 512 columns) or to one CTA. The bound is HBM traffic, two reads and one write of the
 // row's type and one byte, with issue slots close behind: the arithmetic runs on packed pairs, and what depends on the
-// 8-bit type or the group is decided once per vector (28 instructions a value before, about 10 now).
+// 8-bit type or the group is decided once per vector (28 instructions a value before, about 10 now). bf16 [16384, 4096]
+// with a residual and groups of 128: 77 us, 6.1 TB/s; fp32 [3003, 1001] 8 us, 4.8 TB/s.
 #include <cuda_fp8.h>
 
 #include <algorithm>
@@ -83,9 +84,9 @@ __device__ __forceinline__ void unpack2(const uint4& u, uint64_t* p) {
 //   WHOLE    every row starts on a 16-byte boundary and is whole vectors
 //   SHIFTED  rows of a width that is no multiple of V, one behind the other: vectors start on 16-byte boundaries all the
 //            same, and the first and the last one of a row hold columns of its neighbours, too, which are left out of the
-//            sums and not stored (nor loaded, behind the last rows). The cut depends on the
-//            row's number modulo `period` alone; a worker takes rows of one residue, and its weights stay in registers.
-//            (bf16 [16384, 4001] took 203 us column by column.)
+//            sums and not stored (nor loaded, behind the last rows). The cut depends on the row's number modulo V alone; a
+//            worker takes rows of one residue, and its weights stay in registers. (bf16 [16384, 4001] 87 us, column by
+//            column 203.)
 //   SINGLE   any strides: columns are moved one by one, with a scale per row side by side over the threads
 enum Layout { WHOLE, SHIFTED, SINGLE };
 
@@ -341,8 +342,8 @@ int by_width(const Norm8& a, cudaStream_t st) {
     const int n = a.width + (L == SHIFTED ? V - 1 : 0);  // columns of a row's vectors, at most
     if (n <= 256) return launch<T, GROUPED, L, 32, 8 / V>(a, st);
     if (n <= 512) return launch<T, GROUPED, L, 32, 16 / V>(a, st);
-    // From here on a CTA a row: bf16 [65536, 1024] 75 us (a warp a row 80), fp32 [3003, 1001] 7.8 us (10.8); at 512 columns it is
-    // the other way round (137 us, 100).
+    // From here on a CTA a row: bf16 [65536, 1024] 75 us (a warp a row 80), fp32 [3003, 1001] 7.8 us (10.8); at 512 columns
+    // it is the other way round (137 us, 100).
     if (n <= 1024) return launch<T, GROUPED, L, 128, 8 / V>(a, st);
     if (n <= 2048) return launch<T, GROUPED, L, 128, 16 / V>(a, st);
     if (n <= 4096) return launch<T, GROUPED, L, 128, 32 / V>(a, st);

@@ -14,7 +14,9 @@
 // key/value head, T = new tokens): a sequence's rows are neighbours, and all B G T of them meet the prefix.
 //
 // Three kernels: tensor_part_kernel (prefix_attention_tc.cu) for a prefix with many query rows; stream_kernel
-// for the caches, and for a prefix with few rows, where the bound is the keys' bytes; join_kernel.
+// for the caches, and for a prefix with few rows, where the bound is the keys' bytes; join_kernel. bf16, 32 heads on 8 of
+// 128: 256 sequences behind 16384 keys with uneven caches up to 512 take 117 us a call (bytes 53, the prefix's products
+// 43), 4 behind 131072 keys 97 us, 5.6 TB/s.
 #include <algorithm>
 
 #include "attn.cuh"
@@ -429,7 +431,8 @@ struct JoinArgs {
 };
 
 // WIDE: a CTA per query row, its eight warps taking turns at the parts; else a warp per row. The parts are the
-// tensor cores' (or the prefix units' slots), then the own units' slots, weighed and added in a fixed order. A query before its
+// tensor cores' (or the prefix units' slots), then the own units' slots, weighed and added in a fixed order. The bound is
+// latency: 3 to 5 us behind the other kernels. A query before its
 // sequence's first token (a free slot of the batch) reads out as zero with a log-sum-exp of -inf.
 template <typename T, int D, bool WIDE>
 __global__ void __launch_bounds__(256) join_kernel(const JoinArgs a) {
@@ -528,8 +531,8 @@ __global__ void __launch_bounds__(256) join_kernel(const JoinArgs a) {
 
 // ------------------------------------------------------------------ host side
 // Up to kStreamRows query rows of a key/value head meet the prefix in the stream kernel, and up to kFewRows if it is no
-// longer than kFewKeys; otherwise it goes to the tensor cores. bf16, 8 heads of 128: 4 rows, 8192 keys 12.4 us against 16.2;
-// 16 rows, 131072 keys 99 us against 90; 16 rows, 1000 keys 12.4 against 10.6, 300 keys 8.3 against 10.3.
+// longer than kFewKeys; otherwise it goes to the tensor cores. bf16, 8 heads of 128: 4 rows, 8192 keys 12.4 us against
+// 16.2; 16 rows, 131072 keys 99 us against 90; 16 rows, 1000 keys 12.4 against 10.6, 300 keys 8.3 against 10.3.
 constexpr int kStreamRows = 8, kFewRows = 32, kFewKeys = 512;
 
 struct Plan {
@@ -562,7 +565,8 @@ Plan plan_of(const nb200_prefix_attn_args& a) {
     const int64_t prefix_steps = p.prefix_tiles ? line(a.prefix) : 0, own_steps = line(a.cache);
     const int64_t steps = a.kv_heads * (p.prefix_tiles * prefix_steps + a.batch * p.own_tiles * own_steps);
     // Two CTAs an SM. Four where each worker still has 16 places and the SM holds four (caches of 256 sequences, head
-    // dimension 64: 33.5 us, with two 37.4; with few places the more parts cost more than that gives, 12.8 us against 10.9).
+    // dimension 64: 33.5 us, with two 37.4; with few places the more parts cost more than that gives, 12.8 us against
+    // 10.9).
     // Four, two at a time, beside the tensor cores' kernel where pieces are short anyway, because SMs become free at
     // different times (32 sequences: 25.9 us against 26.9; 256 sequences, with long pieces, 101 against 96).
     const int64_t sms = sm_count(), places = steps / (2 * sms * kWarps);
