@@ -286,16 +286,20 @@ __device__ __forceinline__ uint32_t mask_bits(const int32_t* allowed, int64_t v,
     return shift + count <= 32 ? lo >> shift : __funnelshift_r(lo, (uint32_t)__ldg(allowed + (v >> 5) + 1), shift);
 }
 
-// Where a sweep has a row's named tokens from: there are none; from name_kernel's entries; or, if they are few, from the
-// history itself.
+// Where a sweep has a row's named tokens from: there are none; from name_kernel's entries; or, where that costs less, from
+// the history itself, which every tile counts in shared memory.
 enum Names { NONE, ENTRIES, SELF };
-constexpr int kSelfTokens = 512, kSelfBiases = 128;
+constexpr int kSelfTokens = 4096, kSelfBiases = kSweepThreads;
+// SELF's word for a token: mentions in the history from kMention on, those in the output below, and between them whether it
+// is biased, and whether only so.
+constexpr uint32_t kMention = 1u << 16, kWithBias = 1u << 14, kOnlyBias = 1u << 15;
+static_assert(kSelfTokens < (int)kWithBias, "a count's bits");
 
 // Temperature and mask of a tile, and all of it for its named tokens. JOINED: rows of input and output are cut by different
 // 16-byte boundaries (a vocabulary that is padded on the one side), and a vector of the output is joined from two. bf16
 // [1024, 131071] of rows 131072 apart: 157 us, token by token 336; [256, 32001] 7.6 and 16.3.
 template <typename T, Names NAMES, bool JOINED>
-__global__ void __launch_bounds__(kSweepThreads, NAMES == SELF ? 1 : JOINED ? 4 : kSweepCtas) sweep_kernel(const Logits a) {
+__global__ void __launch_bounds__(kSweepThreads, NAMES == SELF || JOINED ? 4 : kSweepCtas) sweep_kernel(const Logits a) {
     constexpr int V = Elem<T>::V;
     constexpr bool NAMED = NAMES == ENTRIES;
     if (!NAMED) {  // else the inputs are older than name_kernel, which had them before this one could start
@@ -336,28 +340,56 @@ __global__ void __launch_bounds__(kSweepThreads, NAMES == SELF ? 1 : JOINED ? 4 
         if (e0 + (int)threadIdx.x < e1) entry = entries[e0 + threadIdx.x];
     };
     if (later) look_up();
-    // SELF: the history, a prompt's token v as -2 - v and what is none as -1; the biases; bits for the tile's tokens that
-    // have been found, that were found again, and that are biased.
-    __shared__ __align__(16) int list[NAMES == SELF ? kSelfTokens : 4];
-    __shared__ int bias_token[NAMES == SELF ? kSelfBiases : 1];
+    // SELF: a word for each of the tile's tokens, those that are named, in any order, and the biases.
+    constexpr int kCounts = NAMES == SELF ? kTile<T> + 16 : 4;
+    __shared__ __align__(16) uint32_t counts[kCounts];
+    __shared__ uint16_t list[NAMES == SELF ? kSelfTokens + kSelfBiases : 1];
+    __shared__ int bias_token[NAMES == SELF ? kSelfBiases : 1], listed;
     __shared__ float bias_value[NAMES == SELF ? kSelfBiases : 1];
-    constexpr int kWords = NAMES == SELF ? kTile<T> / 32 + 1 : 1;
-    __shared__ uint32_t found[kWords], twice[kWords], with_bias[kWords];
     const int biases = (int)n.biases;
-    int len = 0;
     if constexpr (NAMES == SELF) {
-        len = (int)(n.token_lens ? min((int64_t)n.token_lens[row], n.history) : n.history);
-        const int64_t prompt = n.prompt_lens ? n.prompt_lens[row] : 0;
-        for (int i = threadIdx.x; i < kSelfTokens; i += kSweepThreads) {
-            const int64_t v = i < n.history ? index_at(n.tokens, row * n.stride_tokens + i, n.token_dtype) : -1;
-            list[i] = i >= len || v < 0 || v >= n.vocab ? -1 : i < prompt ? -2 - (int)v : (int)v;
-        }
+        constexpr int kAtOnce = 4;  // of a thread, on their way together
+        const int size = (int)(hi - lo);
+        auto here = [&](int64_t v) { return v >= lo && v < hi ? (int)(v - lo) : -1; };
+        auto put = [&](int v) { list[atomicAdd(&listed, 1)] = (uint16_t)v; };
+        int token[kAtOnce], bias = -1;
+        auto load = [&](int64_t i0) {
+#pragma unroll
+            for (int k = 0; k < kAtOnce; ++k) {
+                const int64_t i = i0 + k * kSweepThreads;
+                token[k] = i < n.history ? here(index_at(n.tokens, row * n.stride_tokens + i, n.token_dtype)) : -1;
+            }
+        };
+        load(threadIdx.x);
         if (threadIdx.x < biases) {
-            const int64_t v = index_at(n.bias_index, row * n.stride_bias_index + threadIdx.x, n.bias_dtype);
-            bias_token[threadIdx.x] = v < 0 || v >= n.vocab ? -1 : (int)v;
+            bias = here(index_at(n.bias_index, row * n.stride_bias_index + threadIdx.x, n.bias_dtype));
+            bias_token[threadIdx.x] = bias;
             bias_value[threadIdx.x] = __ldg(n.bias_value + row * n.stride_bias_value + threadIdx.x);
         }
-        for (int i = threadIdx.x; i < kWords; i += kSweepThreads) found[i] = twice[i] = with_bias[i] = 0u;
+        const int64_t len = n.token_lens ? min((int64_t)n.token_lens[row], n.history) : n.history;
+        const int64_t prompt = n.prompt_lens ? n.prompt_lens[row] : 0;
+        for (int i = threadIdx.x * 4; i < size; i += kSweepThreads * 4)
+            *reinterpret_cast<uint4*>(counts + i) = make_uint4(0u, 0u, 0u, 0u);
+        if (threadIdx.x == 0) listed = 0;
+        __syncthreads();
+        for (int64_t i0 = threadIdx.x; i0 < len;) {
+#pragma unroll
+            for (int k = 0; k < kAtOnce; ++k) {
+                const int64_t i = i0 + k * kSweepThreads;
+                if (i < len && token[k] >= 0 && atomicAdd(&counts[token[k]], kMention + (i >= prompt)) == 0u) put(token[k]);
+            }
+            if ((i0 += kAtOnce * kSweepThreads) < len) load(i0);
+        }
+        if (biases) {
+            __syncthreads();
+            if (bias >= 0) {
+                const uint32_t old = atomicOr(&counts[bias], kWithBias);
+                if (old < kMention && !(old & kWithBias)) {  // its first bias, and the history does not name it
+                    atomicOr(&counts[bias], kOnlyBias);
+                    put(bias);
+                }
+            }
+        }
     }
 #pragma unroll
     for (int k = 0; k < kVectors; ++k) {
@@ -405,45 +437,14 @@ __global__ void __launch_bounds__(kSweepThreads, NAMES == SELF ? 1 : JOINED ? 4 
                 if (e0 + (int)threadIdx.x < e1) entry = entries[e0 + threadIdx.x];
             }
         } else {
-            // Whoever first comes to a token redoes it, and counts it in the list if somebody came again.
-            auto here = [&](int v) { return v >= lo && v < hi; };
-            auto bit = [&](int v) { return 1u << ((uint32_t)(v - lo) & 31); };
-            auto word = [&](uint32_t* map, int v) -> uint32_t& { return map[(uint32_t)(v - lo) >> 5]; };
-            auto bias_of = [&](int v) {  // in the order in which they are given
-                float sum = 0.f;
-                if (word(with_bias, v) & bit(v))
+            for (int e = threadIdx.x; e < listed; e += kSweepThreads) {
+                const int v = list[e];
+                const uint32_t word = counts[v];
+                float bias = 0.f;
+                if (word & kWithBias)  // in the order in which they are given
                     for (int j = 0; j < biases; ++j)
-                        if (bias_token[j] == v) sum += bias_value[j];
-                return sum;
-            };
-            auto token = [&](int i) { return list[i] < -1 ? -2 - list[i] : list[i]; };
-            if (threadIdx.x < biases && here(bias_token[threadIdx.x]))
-                atomicOr(&word(with_bias, bias_token[threadIdx.x]), bit(bias_token[threadIdx.x]));
-            bool first[kSelfTokens / kSweepThreads];
-#pragma unroll
-            for (int k = 0; k < kSelfTokens / kSweepThreads; ++k) {
-                const int i = threadIdx.x + k * kSweepThreads, v = token(i);
-                first[k] = here(v) && !(atomicOr(&word(found, v), bit(v)) & bit(v));
-                if (here(v) && !first[k]) atomicOr(&word(twice, v), bit(v));
-            }
-            __syncthreads();
-#pragma unroll
-            for (int k = 0; k < kSelfTokens / kSweepThreads; ++k) {
-                const int i = threadIdx.x + k * kSweepThreads, v = token(i);
-                if (!first[k]) continue;
-                int count = list[i] >= 0;
-                if (word(twice, v) & bit(v)) {
-                    count = 0;
-                    for (int j = 0; j < len; j += 4) {
-                        const int4 o = *reinterpret_cast<const int4*>(list + j);
-                        count += (o.x == v) + (o.y == v) + (o.z == v) + (o.w == v);
-                    }
-                }
-                again(v, (uint32_t)count, bias_of(v), true);
-            }
-            if (threadIdx.x < biases) {  // what the history does not name
-                const int v = bias_token[threadIdx.x];
-                if (here(v) && !(atomicOr(&word(found, v), bit(v)) & bit(v))) again(v, 0u, bias_of(v), false);
+                        if (bias_token[j] == v) bias += bias_value[j];
+                again(lo + v, word & (kWithBias - 1u), bias, !(word & kOnlyBias));
             }
         }
     }
@@ -466,10 +467,11 @@ int64_t plan(Logits& a, int tile) {
     a.tiles = (int)((n.vocab + tile - 1) / tile);
     const int64_t entries = std::min(n.history + n.biases, n.vocab);
     if (!entries) return 0;
-    // Few names, and no more tiles than SMs: the sweep looks for them itself, without a second launch and its workspace.
-    // fp32, vocabulary of 32000: 8 rows with histories of 300 take 8 us a call, 11 with both kernels; 50 rows with
-    // histories of 512 11 us on the GPU alone, 5.5 with both.
-    a.self = n.history <= kSelfTokens && n.biases <= kSelfBiases && n.rows * a.tiles <= sm_count();
+    // A few tiles a row, or a few an SM: the sweep names the tokens itself, every tile for itself, without a second launch and
+    // its workspace. bf16 [8, 32000], histories of 300: 3.5 us on the GPU alone, 4.8 with both kernels; histories of 2048:
+    // 6.2, 9.3; 512 rows 27.9, 32.4. Of [n, 131072] 32 rows, 3.5 tiles an SM, with histories of 512 take 5.9, 5.3, and with
+    // 4096 13.0, 13.5; 128 rows, 14 tiles an SM, 13.8, 11.8 and 32.9, 24.3.
+    a.self = n.history <= kSelfTokens && n.biases <= kSelfBiases && (a.tiles <= 4 || n.rows * a.tiles <= 6 * sm_count());
     if (a.self) return 0;
     // The table stays three eighths empty at least. Where it, or the bit maps, would be too large, the vocabulary is dealt
     // out to as many CTAs as it takes for every token of a range to fit, whatever the history holds.
