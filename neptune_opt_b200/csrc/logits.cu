@@ -291,8 +291,8 @@ __device__ __forceinline__ uint32_t mask_bits(const int32_t* allowed, int64_t v,
 enum Names { NONE, ENTRIES, SELF };
 constexpr int kSelfTokens = 4096, kSelfBiases = kSweepThreads;
 // SELF's word for a token: mentions in the history from kMention on, those in the output below, and between them whether it
-// is biased, and whether only so.
-constexpr uint32_t kMention = 1u << 16, kWithBias = 1u << 14, kOnlyBias = 1u << 15;
+// is biased, and whether more than once.
+constexpr uint32_t kMention = 1u << 16, kWithBias = 1u << 14, kManyBiases = 1u << 15;
 static_assert(kSelfTokens < (int)kWithBias, "a count's bits");
 
 // Temperature and mask of a tile, and all of it for its named tokens. JOINED: rows of input and output are cut by different
@@ -340,19 +340,20 @@ __global__ void __launch_bounds__(kSweepThreads, NAMES == SELF || JOINED ? 4 : k
         if (e0 + (int)threadIdx.x < e1) entry = entries[e0 + threadIdx.x];
     };
     if (later) look_up();
-    // SELF: a word for each of the tile's tokens, those that are named, in any order, and the biases.
+    // SELF: a word for each of the tile's tokens, those that the history names, in any order, and the biases.
     constexpr int kCounts = NAMES == SELF ? kTile<T> + 16 : 4;
     __shared__ __align__(16) uint32_t counts[kCounts];
-    __shared__ uint16_t list[NAMES == SELF ? kSelfTokens + kSelfBiases : 1];
+    __shared__ uint16_t list[NAMES == SELF ? kSelfTokens : 1];
     __shared__ int bias_token[NAMES == SELF ? kSelfBiases : 1], listed;
     __shared__ float bias_value[NAMES == SELF ? kSelfBiases : 1];
     const int biases = (int)n.biases;
+    int bias = -1;  // the thread's biased token, if no thread before it has the same
     if constexpr (NAMES == SELF) {
         constexpr int kAtOnce = 4;  // of a thread, on their way together
         const int size = (int)(hi - lo);
         auto here = [&](int64_t v) { return v >= lo && v < hi ? (int)(v - lo) : -1; };
         auto put = [&](int v) { list[atomicAdd(&listed, 1)] = (uint16_t)v; };
-        int token[kAtOnce], bias = -1;
+        int token[kAtOnce];
         auto load = [&](int64_t i0) {
 #pragma unroll
             for (int k = 0; k < kAtOnce; ++k) {
@@ -376,19 +377,13 @@ __global__ void __launch_bounds__(kSweepThreads, NAMES == SELF || JOINED ? 4 : k
 #pragma unroll
             for (int k = 0; k < kAtOnce; ++k) {
                 const int64_t i = i0 + k * kSweepThreads;
-                if (i < len && token[k] >= 0 && atomicAdd(&counts[token[k]], kMention + (i >= prompt)) == 0u) put(token[k]);
+                if (i < len && token[k] >= 0 && atomicAdd(&counts[token[k]], kMention + (i >= prompt)) < kMention) put(token[k]);
             }
             if ((i0 += kAtOnce * kSweepThreads) < len) load(i0);
         }
-        if (biases) {
-            __syncthreads();
-            if (bias >= 0) {
-                const uint32_t old = atomicOr(&counts[bias], kWithBias);
-                if (old < kMention && !(old & kWithBias)) {  // its first bias, and the history does not name it
-                    atomicOr(&counts[bias], kOnlyBias);
-                    put(bias);
-                }
-            }
+        if (bias >= 0 && (atomicOr(&counts[bias], kWithBias) & kWithBias)) {
+            atomicOr(&counts[bias], kManyBiases);
+            bias = -1;
         }
     }
 #pragma unroll
@@ -439,12 +434,17 @@ __global__ void __launch_bounds__(kSweepThreads, NAMES == SELF || JOINED ? 4 : k
         } else {
             for (int e = threadIdx.x; e < listed; e += kSweepThreads) {
                 const int v = list[e];
-                const uint32_t word = counts[v];
-                float bias = 0.f;
-                if (word & kWithBias)  // in the order in which they are given
+                if (!(counts[v] & kWithBias)) again(lo + v, counts[v] & (kWithBias - 1u), 0.f, true);
+            }
+            if (bias >= 0) {
+                const uint32_t word = counts[bias];
+                float sum = bias_value[threadIdx.x];
+                if (word & kManyBiases) {  // in the order in which they are given
+                    sum = 0.f;
                     for (int j = 0; j < biases; ++j)
-                        if (bias_token[j] == v) bias += bias_value[j];
-                again(lo + v, word & (kWithBias - 1u), bias, !(word & kOnlyBias));
+                        if (bias_token[j] == bias) sum += bias_value[j];
+                }
+                again(lo + bias, word & (kWithBias - 1u), sum, word >= kMention);
             }
         }
     }
