@@ -467,10 +467,10 @@ int64_t plan(Logits& a, int tile) {
     a.tiles = (int)((n.vocab + tile - 1) / tile);
     const int64_t entries = std::min(n.history + n.biases, n.vocab);
     if (!entries) return 0;
-    // A few tiles a row, or a few an SM: the sweep names the tokens itself, every tile for itself, without a second launch and
-    // its workspace. bf16 [8, 32000], histories of 300: 3.5 us on the GPU alone, 4.8 with both kernels; histories of 2048:
-    // 6.2, 9.3; 512 rows 27.9, 32.4. Of [n, 131072] 32 rows, 3.5 tiles an SM, with histories of 512 take 5.9, 5.3, and with
-    // 4096 13.0, 13.5; 128 rows, 14 tiles an SM, 13.8, 11.8 and 32.9, 24.3.
+    // A few tiles a row, or a few an SM: every tile counts the history itself, without a second launch and its workspace.
+    // bf16 [8, 32000] on the GPU alone, histories of 512: 3.5 us, with both kernels 4.8; of 2048: 6.2 and 9.3, 512 rows 27.9
+    // and 32.4. [32, 131072], 3.5 tiles an SM: histories of 512 5.9 and 5.3, of 4096 13.0 and 13.5; 128 rows, 14 tiles an
+    // SM: 13.8 and 11.8, 32.9 and 24.3.
     a.self = n.history <= kSelfTokens && n.biases <= kSelfBiases && (a.tiles <= 4 || n.rows * a.tiles <= 6 * sm_count());
     if (a.self) return 0;
     // The table stays three eighths empty at least. Where it, or the bit maps, would be too large, the vocabulary is dealt

@@ -108,6 +108,32 @@ def test_against_the_formulas(dtype, vocab, history, biases, masked):
     check(make(5, vocab, dtype, history, biases, masked, seed=vocab))
 
 
+@pytest.mark.parametrize("dtype", list(HALF_STEP))
+@pytest.mark.parametrize("vocab", [1, 33, 1000, 5003, 16391, 50001])
+@pytest.mark.parametrize("history,biases", [(40, 257), (700, 300), (4096, 1024), (4097, 3), (9000, 600)])
+def test_histories_and_biases_that_the_sweep_does_not_count(dtype, vocab, history, biases):
+    check(make(3, vocab, dtype, history, biases, True, seed=vocab + history))
+
+
+@pytest.mark.parametrize("dtype", list(HALF_STEP))
+@pytest.mark.parametrize("history,biases", [(0, 7), (300, 0), (2049, 100), (4096, 256)])
+def test_few_and_many_rows_agree(dtype, history, biases):
+    """Few tiles count the history themselves, many take it from the names' kernel; rows of other boundaries, too."""
+    import torch
+
+    import neptune_opt_b200 as NB
+
+    s = make(220, 40009, dtype, history, biases, True, seed=history)
+    want = NB.penalize_logits(**s)
+    check({k: v[:5] for k, v in s.items()}, want[:5])
+    for lo, hi in ((0, 1), (1, 30), (30, 90)):
+        assert torch.equal(NB.penalize_logits(**{k: v[lo:hi] for k, v in s.items()}), want[lo:hi])
+    for at, width in ((0, 40064), (3, 40013), (8, 40017)):
+        room = torch.full((220, width), math.nan, device="cuda", dtype=s["logits"].dtype)
+        room[:, at:at + 40009] = s["logits"]
+        assert torch.equal(NB.penalize_logits(**{**s, "logits": room[:, at:at + 40009]}), want)
+
+
 @pytest.mark.parametrize("index", ["int32", "int64"])
 @pytest.mark.parametrize("rows", [1, 2, 97, 700])
 def test_row_counts_and_index_types(index, rows):
