@@ -776,6 +776,12 @@ int nb200_norm8(const nb200_norm8_args* args, void* q, float* scale, void* y, vo
         set_error("nb200_norm8: null pointer");
         return NB200_ERR_ARG;
     }
+    const uintptr_t values = (uintptr_t)args->x | (uintptr_t)args->residual | (uintptr_t)args->weight |
+                             (args->residual ? (uintptr_t)y : 0);
+    if (values & (args->dtype == NB200_F32 ? 3u : 1u) || (uintptr_t)scale & 3u) {
+        set_error("nb200_norm8: a tensor is not aligned to its elements");
+        return NB200_ERR_ARG;
+    }
     return launch_norm8(*args, q, scale, y, (cudaStream_t)stream);
 }
 
@@ -791,6 +797,16 @@ int nb200_penalize_logits(const nb200_logits_args* args, void* out, void* work, 
     if (!args->logits || !out || (args->history && !args->tokens) ||
         (args->biases && (!args->bias_index || !args->bias_value))) {
         set_error("nb200_penalize_logits: null pointer");
+        return NB200_ERR_ARG;
+    }
+    uintptr_t words = (uintptr_t)args->token_lens | (uintptr_t)args->prompt_lens | (uintptr_t)args->allowed |
+                      (uintptr_t)args->repetition | (uintptr_t)args->presence | (uintptr_t)args->frequency |
+                      (uintptr_t)args->temperature;
+    if (args->biases) words |= (uintptr_t)args->bias_value;
+    auto off = [](const void* p, int32_t index) { return ((uintptr_t)p & (index == NB200_I64 ? 7u : 3u)) != 0; };
+    if (((uintptr_t)args->logits | (uintptr_t)out) & (args->dtype == NB200_F32 ? 3u : 1u) || words & 3u ||
+        (args->history && off(args->tokens, args->token_dtype)) || (args->biases && off(args->bias_index, args->bias_dtype))) {
+        set_error("nb200_penalize_logits: a tensor is not aligned to its elements");
         return NB200_ERR_ARG;
     }
     const int64_t need = logits_work_bytes(*args);

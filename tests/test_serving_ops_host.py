@@ -266,3 +266,32 @@ def test_c_logits_refuses_before_any_launch():
     assert call(history=1 << 29) == L.NB200_ERR_CAPACITY
     assert lib.nb200_penalize_logits(None, FAKE, FAKE, 1 << 30, NULL) == L.NB200_ERR_ARG
     assert lib.nb200_penalize_logits_work_bytes(None) == L.NB200_ERR_ARG
+
+
+def test_c_entries_refuse_tensors_off_their_elements():
+    lib = L.load()
+    base = 1 << 20
+
+    def norm(dtype, x=base, w=base, r=base, scale=base, y=base):
+        a = L.NB200Norm8Args(x, r, w, 4, 64, 0, 64, 64, dtype, 0, 1e-6)
+        return lib.nb200_norm8(ctypes.byref(a), FAKE, ctypes.c_void_p(scale), ctypes.c_void_p(y), NULL)
+
+    for dtype, off in ((0, 2), (1, 1), (2, 1)):
+        for name in ("x", "w", "r", "y"):
+            assert norm(dtype, **{name: base + off}) == L.NB200_ERR_ARG, (dtype, name)
+    assert norm(1, scale=base + 2) == L.NB200_ERR_ARG
+
+    pointers = ("logits", "tokens", "bias_index", "bias_value", "token_lens", "prompt_lens", "allowed", "repetition",
+                "presence", "frequency", "temperature")
+
+    def logits(dtype=0, index=1, out=base, **changes):
+        a = L.NB200LogitsArgs(*(changes.get(name, base) for name in pointers), 4, 100, 8, 8, 100, 8, 8, 8, 4, dtype, index,
+                              index)
+        return lib.nb200_penalize_logits(ctypes.byref(a), ctypes.c_void_p(out), FAKE, 1 << 30, NULL)
+
+    for name in pointers:
+        assert logits(**{name: base + 2}) == L.NB200_ERR_ARG, name
+    for name in ("tokens", "bias_index"):
+        assert logits(**{name: base + 4}) == L.NB200_ERR_ARG, name
+    assert logits(out=base + 2) == L.NB200_ERR_ARG
+    assert logits(dtype=1, logits=base + 1) == L.NB200_ERR_ARG and logits(dtype=2, out=base + 1) == L.NB200_ERR_ARG
