@@ -14,9 +14,10 @@
 // key/value head, T = new tokens): a sequence's rows are neighbours, and all B G T of them meet the prefix.
 //
 // Three kernels: tensor_part_kernel (prefix_attention_tc.cu) for a prefix with many query rows; stream_kernel
-// for the caches, and for a prefix with few rows, where the bound is the keys' bytes; join_kernel. bf16, 32 heads on 8 of
-// 128: 256 sequences behind 16384 keys with uneven caches up to 512 take 117 us a call (bytes 53, the prefix's products
-// 43), 4 behind 131072 keys 97 us, 5.6 TB/s.
+// for the caches, and for a prefix with few rows, where the bound is the keys' bytes; join_kernel. Few keys for few
+// sequences take one, solo_kernel. bf16, 32 heads on 8 of
+// 128: 256 sequences behind 16384 keys with uneven caches up to 512 take 118 us a call (bytes 53, the prefix's products
+// 43), 4 behind 131072 keys 98 us, 5.5 TB/s.
 #include <algorithm>
 
 #include "attn.cuh"
@@ -168,6 +169,108 @@ __device__ __forceinline__ Cursor piece_of(const StreamArgs& a, int worker, int 
     return c;
 }
 
+// What a worker keeps of a unit's query rows, its running maximum (log2 domain), sum and output, and what a step of 16
+// keys does to it. Column tile n of a lane's accumulators: query rows 8 n + 2 (lane % 4) and the next one.
+template <typename T, int D, int NT>
+struct Rows {
+    float o[NT][D / 16][4], m[NT][2], l[NT][2];
+
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) m[n][e] = -NB200_INF, l[n][e] = 0.f;
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[n][d][e] = 0.f;
+        }
+    }
+    // Keys kb on, of a box at ks and vs in shared memory; `limit`: the last key a row sees, `lowest`: the least of them.
+    __device__ __forceinline__ void step(const uint32_t (*qf)[D / 16][2], uint32_t ks, uint32_t vs, int kb,
+                                         const int (*limit)[2], int lowest, float sl2, int lane) {
+        constexpr uint32_t kBox = kStepKeys * 128;
+        // This lane's address in a box: the row it loads for ldmatrix, and the swizzle of its 16-byte pieces.
+        const int k_row = lane & 15, k_piece = lane >> 4;                         // K: keys 0-15, then 8 columns on
+        const int v_row = (lane >> 4) * 8 + (lane & 7), v_piece = lane >> 3 & 1;  // V, transposed: columns, then keys
+        float s[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) {
+            uint32_t f[4];
+            ldmatrix4(f, ks + (d / 4) * kBox + k_row * 128 + (((2 * (d % 4) + k_piece) ^ (k_row & 7)) << 4));
+#pragma unroll
+            for (int n = 0; n < NT; ++n) Mma<T>::mul(s[n], f, qf[n][d]);
+        }
+        // s[n][e]: key lane / 4 + 8 (e / 2), query row e % 2 of the lane's two.
+        if (kb + kStepKeys - 1 > lowest) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (kb + (lane >> 2) + 8 * (e / 2) > limit[n][e % 2]) s[n][e] = -NB200_INF;
+        }
+        bool grow = false;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) grow |= fmaxf(s[n][e], s[n][e + 2]) * sl2 > m[n][e] + kSlack;
+        if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float top = fmaxf(s[n][e], s[n][e + 2]) * sl2;
+#pragma unroll
+                    for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+                    const float next = fmaxf(m[n][e], top);
+                    const float f = next == m[n][e] ? 1.f : ex2(m[n][e] - next);
+                    m[n][e] = next;
+                    l[n][e] *= f;
+#pragma unroll
+                    for (int d = 0; d < D / 16; ++d) o[n][d][e] *= f, o[n][d][e + 2] *= f;
+                }
+        }
+        uint32_t p[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            float x[4];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float ref = (m[n][e] == -NB200_INF ? 0.f : m[n][e]) - kLift<T>;
+                x[e] = ex2(fmaf(s[n][e], sl2, -ref));
+                x[e + 2] = ex2(fmaf(s[n][e + 2], sl2, -ref));
+                l[n][e] += x[e] + x[e + 2];
+            }
+            p[n][0] = transpose8(Elem<T>::pack_word(x[0], x[1]));
+            p[n][1] = transpose8(Elem<T>::pack_word(x[2], x[3]));
+        }
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) {
+            uint32_t f[4];
+            ldmatrix4_t(f, vs + (d / 4) * kBox + v_row * 128 + (((2 * (d % 4) + v_piece) ^ (v_row & 7)) << 4));
+#pragma unroll
+            for (int n = 0; n < NT; ++n) Mma<T>::mul(o[n][d], f, p[n]);
+        }
+    }
+};
+
+// Zeroes a staged V's keys from `keys` on.
+template <int D>
+__device__ __forceinline__ void zero_behind(uint32_t vs, int keys, int lane) {
+    if (keys >= kStepKeys) return;
+    for (int i = keys * 8 + lane; i < kStepKeys * 8; i += 32)
+#pragma unroll
+        for (int h = 0; h < D / 64; ++h)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(vs + h * kStepKeys * 128 + i * 16), "r"(0u)
+                         : "memory");
+    fence_proxy_async();
+    __syncwarp();
+}
+
 // Every warp is a worker: its lane 0 has the keys and values of the steps copied (TMA) into shared memory that no
 // other warp touches, two steps ahead and across the units' borders, and the warp keeps the running maximum, sum
 // and output of its unit in registers. No barrier, no atomics.
@@ -236,7 +339,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, NT>)
     // Column tile n of this lane's accumulators: query rows 8 n + 2 (lane % 4) and the next one.
     uint32_t qf[NT][D / 16][2], next_q[kAhead ? NT : 1][D / 16][2];
     int limit[NT][2], lowest = 0;  // last key a row sees; of the unit's rows, the least
-    float o[NT][D / 16][4], m[NT][2], l[NT][2];
+    Rows<T, D, NT> t;
     int nrows = 0;
     auto load_rows = [&](const Cursor& c, uint32_t(*q)[D / 16][2]) {
         const bool shared = c.batch < 0;
@@ -264,16 +367,11 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, NT>)
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
+            for (int e = 0; e < 2; ++e)
                 limit[n][e] = shared ? use.keys - 1
                               : lowest + (a.query.tokens > 1 ? (in_unit + 8 * n + 2 * (lane & 3) + e) % a.query.tokens : 0);
-                m[n][e] = -NB200_INF, l[n][e] = 0.f;
-            }
-#pragma unroll
-            for (int d = 0; d < D / 16; ++d)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[n][d][e] = 0.f;
         }
+        t.clear();
         if (kAhead && use.left > use.steps - use.step) {
             Cursor c = use;
             c.next_unit(a);
@@ -284,9 +382,6 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, NT>)
     begin();
     if (lane == 0 && use.step == 0) a.span[use.unit(a)].x = worker;
 
-    // This lane's address in a box: the row it loads for ldmatrix, and the swizzle of its 16-byte pieces.
-    const int k_row = lane & 15, k_piece = lane >> 4;                            // K: keys 0-15, then 8 columns on
-    const int v_row = (lane >> 4) * 8 + (lane & 7), v_piece = lane >> 3 & 1;     // V, transposed: columns, then keys
     bool ok = true;
     int stage = 0, done = 0;
     uint32_t phase = 0;
@@ -298,76 +393,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, NT>)
         const uint32_t ks = mine + stage * (2 * kTile), vs = ks + kTile;
         const int kb = use.step * kStepKeys;
         // What a cache holds behind a sequence must not reach the products: 0 times an infinity is none.
-        if (use.batch >= 0 && kb + kStepKeys > use.keys) {
-            for (int i = (use.keys - kb) * 8 + lane; i < kStepKeys * 8; i += 32)
-#pragma unroll
-                for (int h = 0; h < D / 64; ++h)
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(vs + h * kBox + i * 16), "r"(0u) : "memory");
-            fence_proxy_async();
-            __syncwarp();
-        }
-        float s[NT][4];
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
-#pragma unroll
-        for (int d = 0; d < D / 16; ++d) {
-            uint32_t f[4];
-            ldmatrix4(f, ks + (d / 4) * kBox + k_row * 128 + (((2 * (d % 4) + k_piece) ^ (k_row & 7)) << 4));
-#pragma unroll
-            for (int n = 0; n < NT; ++n) Mma<T>::mul(s[n], f, qf[n][d]);
-        }
-        // s[n][e]: key lane / 4 + 8 (e / 2), query row e % 2 of the lane's two.
-        if (kb + kStepKeys - 1 > lowest) {
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (kb + (lane >> 2) + 8 * (e / 2) > limit[n][e % 2]) s[n][e] = -NB200_INF;
-        }
-        bool grow = false;
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) grow |= fmaxf(s[n][e], s[n][e + 2]) * a.sl2 > m[n][e] + kSlack;
-        if (__any_sync(0xffffffffu, grow)) {
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    float top = fmaxf(s[n][e], s[n][e + 2]) * a.sl2;
-#pragma unroll
-                    for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-                    const float next = fmaxf(m[n][e], top);
-                    const float f = next == m[n][e] ? 1.f : ex2(m[n][e] - next);
-                    m[n][e] = next;
-                    l[n][e] *= f;
-#pragma unroll
-                    for (int d = 0; d < D / 16; ++d) o[n][d][e] *= f, o[n][d][e + 2] *= f;
-                }
-        }
-        uint32_t p[NT][2];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            float x[4];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const float ref = (m[n][e] == -NB200_INF ? 0.f : m[n][e]) - kLift<T>;
-                x[e] = ex2(fmaf(s[n][e], a.sl2, -ref));
-                x[e + 2] = ex2(fmaf(s[n][e + 2], a.sl2, -ref));
-                l[n][e] += x[e] + x[e + 2];
-            }
-            p[n][0] = transpose8(Elem<T>::pack_word(x[0], x[1]));
-            p[n][1] = transpose8(Elem<T>::pack_word(x[2], x[3]));
-        }
-#pragma unroll
-        for (int d = 0; d < D / 16; ++d) {
-            uint32_t f[4];
-            ldmatrix4_t(f, vs + (d / 4) * kBox + v_row * 128 + (((2 * (d % 4) + v_piece) ^ (v_row & 7)) << 4));
-#pragma unroll
-            for (int n = 0; n < NT; ++n) Mma<T>::mul(o[n][d], f, p[n]);
-        }
+        if (use.batch >= 0) zero_behind<D>(vs, use.keys - kb, lane);
+        t.step(qf, ks, vs, kb, limit, lowest, a.sl2, lane);
 
         ++done;
         if (++stage == kStages) stage = 0, phase ^= 1u;
@@ -385,17 +412,17 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, NT>)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
 #pragma unroll
-                for (int w = 4; w < 32; w <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], w);
+                for (int w = 4; w < 32; w <<= 1) t.l[n][e] += __shfl_xor_sync(0xffffffffu, t.l[n][e], w);
                 const int in = 8 * n + 2 * (lane & 3) + e;
                 if (in < nrows) {
-                    const float inv = l[n][e] == 0.f ? 0.f : 1.f / l[n][e];
+                    const float inv = t.l[n][e] == 0.f ? 0.f : 1.f / t.l[n][e];
                     float* dst = a.o + (slot + in) * D + (lane >> 2);
 #pragma unroll
                     for (int d = 0; d < D / 16; ++d) {
-                        dst[16 * d] = o[n][d][e] * inv;
-                        dst[16 * d + 8] = o[n][d][e + 2] * inv;
+                        dst[16 * d] = t.o[n][d][e] * inv;
+                        dst[16 * d + 8] = t.o[n][d][e + 2] * inv;
                     }
-                    if (lane < 4) a.lse[slot + in] = l[n][e] == 0.f ? -NB200_INF : m[n][e] + log2f(l[n][e]) - kLift<T>;
+                    if (lane < 4) a.lse[slot + in] = t.l[n][e] == 0.f ? -NB200_INF : t.m[n][e] + log2f(t.l[n][e]) - kLift<T>;
                 }
             }
         if (lane == 0 && ends) a.span[unit].y = worker;
@@ -416,6 +443,144 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, NT>)
     if (!ok)
         for (int i = done; i < sent; ++i) drain_bar(&full[warp][i % kStages], (i / kStages) & 1u);
     if (waits) pdl_wait();
+}
+
+// The same in one kernel without parts in memory, where a CTA a sequence and key/value head is enough: its warps share the
+// prefix and the cache, one list of keys for the same rows, and join in shared memory. (Rows as in stream_kernel; of a
+// unit's two tiles the prefix's rows are the sequence's own.) The bound is latency, a launch and a few steps.
+constexpr int kSoloWarps = 8;
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kSoloWarps * 32, 1)
+    solo_kernel(const __grid_constant__ CUtensorMap shared_k, const __grid_constant__ CUtensorMap shared_v,
+                const __grid_constant__ CUtensorMap own_k, const __grid_constant__ CUtensorMap own_v, const StreamArgs a,
+                void* out, float* out_lse) {
+    constexpr uint32_t kBox = kStepKeys * 128, kTile = kBox * (D / 64);
+    constexpr int kPitch = D + 4;  // floats of a row in shared memory: no two lanes of a store meet in a bank
+    static_assert(8 * NT * kPitch * 4 <= kStages * 2 * kTile, "a warp leaves its output in its stages");
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t full[kSoloWarps][kStages];
+    __shared__ int abort_flag[kSoloWarps];
+    __shared__ float sh_m[kSoloWarps][8 * NT], sh_l[kSoloWarps][8 * NT];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t all_stages = (smem_u32(smem_raw) + 1023u) & ~1023u, mine = all_stages + warp * (kStages * 2 * kTile);
+    if (lane == 0) {
+        for (int i = 0; i < kStages; ++i) mbar_init(&full[warp][i], 1);
+        abort_flag[warp] = 0;
+        fence_barrier_init();
+    }
+    pdl_wait();
+    pdl_trigger();
+    const int seq = (int)(blockIdx.x / (unsigned)a.kv_heads), head = (int)(blockIdx.x % (unsigned)a.kv_heads);
+    const int group = a.query.group, tokens = a.query.tokens, rows = group * tokens;
+    const int own = tokens_of(a.lens, seq, a.cache), shared_steps = steps_of(a.prefix), steps = shared_steps + steps_of(own);
+    const int share = (steps + kSoloWarps - 1) / kSoloWarps, begin = warp * share, end = min(begin + share, steps);
+    int get = begin;
+    auto copy = [&](int stage) {
+        if (get >= end) return;
+        if (lane == 0) {
+            const bool shared = get < shared_steps;
+            const CUtensorMap *mk = shared ? &shared_k : &own_k, *mv = shared ? &shared_v : &own_v;
+            const int b = shared ? 0 : seq, key = (shared ? get : get - shared_steps) * kStepKeys;
+            uint64_t* bar = &full[warp][stage];
+            mbar_expect_tx(bar, 2 * kTile);
+#pragma unroll
+            for (int h = 0; h < D / 64; ++h) {
+                tma_load(mine + stage * 2 * kTile + h * kBox, mk, 64 * h, key, head, b, bar);
+                tma_load(mine + stage * 2 * kTile + kTile + h * kBox, mv, 64 * h, key, head, b, bar);
+            }
+        }
+        ++get;
+    };
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) copy(i);
+
+    uint32_t qf[NT][D / 16][2];
+    int limit[NT][2];  // of the cache's keys
+    Rows<T, D, NT> t;
+    t.clear();
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int in = 8 * n + (lane >> 2), row = in < rows ? in : 0;
+        const T* p = static_cast<const T*>(a.query.q) + seq * a.query.qb +
+                     (int64_t)(head * group + row / tokens) * a.query.qh + row % tokens * a.query.qt + 2 * (lane & 3);
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) qf[n][d][h] = *reinterpret_cast<const uint32_t*>(p + 16 * d + 8 * h);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) limit[n][e] = own - tokens + (8 * n + 2 * (lane & 3) + e) % tokens;
+    }
+    int ok = 1, stage = 0;
+    uint32_t phase = 0;
+    for (int i = begin; i < end; ++i) {
+        ok = __all_sync(0xffffffffu, wait_bar(&full[warp][stage], phase, &abort_flag[warp]));
+        if (!ok) {
+            for (int c = i; c < get; ++c) drain_bar(&full[warp][(c - begin) % kStages], ((c - begin) / kStages) & 1u);
+            break;
+        }
+        // Everyone has left the stage that is filled next.
+        copy(stage == 0 ? kStages - 1 : stage - 1);
+        const uint32_t ks = mine + stage * (2 * kTile), vs = ks + kTile;
+        if (i < shared_steps) {
+            int last[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) last[n][0] = last[n][1] = a.prefix - 1;
+            t.step(qf, ks, vs, i * kStepKeys, last, a.prefix - 1, a.sl2, lane);
+        } else {
+            const int kb = (i - shared_steps) * kStepKeys;
+            zero_behind<D>(vs, own - kb, lane);
+            t.step(qf, ks, vs, kb, limit, own - tokens, a.sl2, lane);
+        }
+        if (++stage == kStages) stage = 0, phase ^= 1u;
+    }
+    // The warp's results, into its own stages, which no copy is under way to.
+    float* part = static_cast<float*>(__cvta_shared_to_generic(mine));
+    if (ok) {
+        __syncwarp();
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                for (int w = 4; w < 32; w <<= 1) t.l[n][e] += __shfl_xor_sync(0xffffffffu, t.l[n][e], w);
+                const int in = 8 * n + 2 * (lane & 3) + e;
+                if (lane < 4) sh_m[warp][in] = t.m[n][e], sh_l[warp][in] = t.l[n][e];
+#pragma unroll
+                for (int d = 0; d < D / 16; ++d) {
+                    part[in * kPitch + 16 * d + (lane >> 2)] = t.o[n][d][e];
+                    part[in * kPitch + 16 * d + 8 + (lane >> 2)] = t.o[n][d][e + 2];
+                }
+            }
+    }
+    if (!__syncthreads_and(ok)) return;
+    constexpr int E = D / 32;
+    for (int in = warp; in < rows; in += kSoloWarps) {
+        float top = -NB200_INF, sum = 0.f, v[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = 0.f;
+        if (own - tokens + in % tokens >= 0) {
+#pragma unroll
+            for (int w = 0; w < kSoloWarps; ++w) top = fmaxf(top, sh_m[w][in]);
+#pragma unroll
+            for (int w = 0; w < kSoloWarps; ++w) {
+                const float l = sh_l[w][in], m = sh_m[w][in];
+                const float f = m == -NB200_INF ? l : ex2(m - top);  // without a score but -inf the sum is 0, or NaN
+                sum += f * l;
+                const float* o = static_cast<const float*>(__cvta_shared_to_generic(all_stages + w * (kStages * 2 * kTile))) +
+                                 in * kPitch + lane * E;
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[e] = f == 0.f ? v[e] : fmaf(f, o[e], v[e]);
+            }
+        }
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const int64_t at = ((int64_t)seq * a.kv_heads + head) * rows + in;
+        uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<T*>(out) + at * D) + lane * (E / 2);
+#pragma unroll
+        for (int e = 0; e < E; e += 2) dst[e / 2] = Elem<T>::pack_word(v[e] * inv, v[e + 1] * inv);
+        if (out_lse && lane == 0)
+            out_lse[at] = sum == 0.f ? -NB200_INF : (top + log2f(sum) - kLift<T>) * 0.69314718055994531f;
+    }
 }
 
 struct JoinArgs {
@@ -538,6 +703,7 @@ constexpr int kStreamRows = 8, kFewRows = 32, kFewKeys = 512;
 struct Plan {
     int64_t rows;                  // query rows of a key/value head
     int nt;                        // 8-row tiles of a unit
+    bool solo;                     // solo_kernel does it all
     int splits;                    // of the prefix on the tensor cores (0: it is in the stream kernel, or empty)
     int64_t prefix_tiles, own_tiles, slot_rows, units, ctas;
     int64_t most_parts;            // parts of a row, at most
@@ -549,6 +715,18 @@ Plan plan_of(const nb200_prefix_attn_args& a) {
     Plan p = {};
     const int64_t own_rows = a.heads / a.kv_heads * a.tokens;
     p.rows = a.batch * own_rows;
+    // One kernel while what an SM reads, here in keys of head dimension 128, costs less than a second launch and the join.
+    // bf16 on the GPU alone, 128: 1 sequence, 4 heads on 1, prefix 200, cache 64 4.5 us (with parts in memory 5.7); 32 heads
+    // on 8, prefix 500, caches of 300, 1 sequence 7.4 (6.8), 16 sequences 7.7 (13.5), 32 14.5 (15.9); 4 sequences, 1000 and
+    // 1000 13.4 (15.3), 3000 and 200 19.0 (11.6); 1 sequence, 1000 and 1000 13.3 (8.8).
+    const int64_t units = a.batch * a.kv_heads, waves = (units + sm_count() - 1) / sm_count();
+    p.solo = own_rows <= 16 && units < 1 << 20 &&
+             waves * (a.prefix + a.cache) * a.head_dim / 128 <= std::min<int64_t>(500 + 40 * units, 2048);
+    if (p.solo) {
+        p.nt = own_rows <= 8 ? 1 : 2;
+        p.bytes = 16;
+        return p;
+    }
     if (a.prefix && p.rows > (a.prefix > kFewKeys ? kStreamRows : kFewRows)) {
         // With lengths that only the device knows, the caches are taken to be half full.
         const int64_t bytes = a.batch * a.kv_heads * a.cache * a.head_dim * 4 / (a.seq_lens ? 2 : 1);
@@ -588,7 +766,7 @@ Plan plan_of(const nb200_prefix_attn_args& a) {
     return p;
 }
 
-SharedLimit g_shared[12];
+SharedLimit g_shared[20];
 
 struct Maps {
     CUtensorMap shared_k, shared_v, own_k, own_v;
@@ -599,6 +777,16 @@ int launch_stream(const Maps& m, const StreamArgs& a, int64_t ctas, SharedLimit&
     constexpr uint32_t bytes = kWarps * kStages * 2 * kStepKeys * D * 2 + 1024;  // + alignment slack
     if (const int rc = limit.raise("nb200_prefix_attention", stream_kernel<T, D, NT>, bytes)) return rc;
     launch_pdl(stream_kernel<T, D, NT>, (unsigned)ctas, kWarps * 32, bytes, st, m.shared_k, m.shared_v, m.own_k, m.own_v, a);
+    count_launch();
+    return finish_launch("nb200_prefix_attention");
+}
+
+template <typename T, int D, int NT>
+int launch_solo(const Maps& m, const StreamArgs& a, void* o, float* lse, SharedLimit& limit, cudaStream_t st) {
+    constexpr uint32_t bytes = kSoloWarps * kStages * 2 * kStepKeys * D * 2 + 1024;  // + alignment slack
+    if (const int rc = limit.raise("nb200_prefix_attention", solo_kernel<T, D, NT>, bytes)) return rc;
+    launch_pdl(solo_kernel<T, D, NT>, (unsigned)(a.batch * a.kv_heads), kSoloWarps * 32, bytes, st, m.shared_k, m.shared_v,
+               m.own_k, m.own_v, a, o, lse);
     count_launch();
     return finish_launch("nb200_prefix_attention");
 }
@@ -624,7 +812,7 @@ int launch_all(const nb200_prefix_attn_args& n, const nb200_attn_strides* s, con
     StreamArgs a = {};
     a.query = query;
     Maps maps = {};
-    if (p.prefix_tiles &&
+    if ((p.prefix_tiles || (p.solo && n.prefix)) &&
         ((rc = encode_keys(&maps.shared_k, "prefix_k", pk, n.dtype, D, n.prefix, n.kv_heads, 1, s[1], kStepKeys)) ||
          (rc = encode_keys(&maps.shared_v, "prefix_v", pv, n.dtype, D, n.prefix, n.kv_heads, 1, s[2], kStepKeys))))
         return rc;
@@ -632,10 +820,14 @@ int launch_all(const nb200_prefix_attn_args& n, const nb200_attn_strides* s, con
                     (rc = encode_keys(&maps.own_v, "v", v, n.dtype, D, n.cache, n.kv_heads, n.batch, s[4], kStepKeys))))
         return rc;
     a.lens = n.seq_lens;
-    a.batch = (int)n.batch, a.kv_heads = (int)n.kv_heads, a.prefix = p.prefix_tiles ? (int)n.prefix : 0, a.cache = (int)n.cache;
+    a.batch = (int)n.batch, a.kv_heads = (int)n.kv_heads;
+    a.prefix = p.prefix_tiles || p.solo ? (int)n.prefix : 0, a.cache = (int)n.cache;
     a.rows = (int)p.rows, a.prefix_tiles = (int)p.prefix_tiles, a.own_tiles = (int)p.own_tiles;
     a.slot_rows = (int)p.slot_rows;
     a.sl2 = sl2;
+    if (p.solo)
+        return p.nt == 1 ? launch_solo<T, D, 1>(maps, a, o, lse, limits[3], st)
+                         : launch_solo<T, D, 2>(maps, a, o, lse, limits[4], st);
     a.o = at(p.o), a.lse = at(p.lse), a.span = reinterpret_cast<int2*>(at(p.span));
     a.beside = p.splits > 0;  // the tensor cores' kernel started after all that came before
     rc = p.nt == 1   ? launch_stream<T, D, 1>(maps, a, p.ctas, limits[0], st)
@@ -694,9 +886,9 @@ int launch_prefix_attention(const nb200_prefix_attn_args& n, const nb200_attn_st
     if (n.dtype == NB200_BF16)
         return n.head_dim == 128
                    ? launch_all<__nv_bfloat16, 128>(n, s, q, pk, pv, k, v, o, lse, w, g_shared, st)
-                   : launch_all<__nv_bfloat16, 64>(n, s, q, pk, pv, k, v, o, lse, w, g_shared + 3, st);
-    return n.head_dim == 128 ? launch_all<__half, 128>(n, s, q, pk, pv, k, v, o, lse, w, g_shared + 6, st)
-                             : launch_all<__half, 64>(n, s, q, pk, pv, k, v, o, lse, w, g_shared + 9, st);
+                   : launch_all<__nv_bfloat16, 64>(n, s, q, pk, pv, k, v, o, lse, w, g_shared + 5, st);
+    return n.head_dim == 128 ? launch_all<__half, 128>(n, s, q, pk, pv, k, v, o, lse, w, g_shared + 10, st)
+                             : launch_all<__half, 64>(n, s, q, pk, pv, k, v, o, lse, w, g_shared + 15, st);
 }
 
 }  // namespace nb200

@@ -263,6 +263,62 @@ def test_offsets_past_32_bits():
     check((q, pk, pv, room[:, :, -30:], v))
 
 
+# Calls of few keys and sequences run as one kernel; what follows does not: more than 16 query rows a key/value
+# head of a sequence, or more keys than few units take on.
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("batch,heads,kv_heads,tokens,prefix,cache", [
+    (1, 1, 1, 1, 333, 2100), (2, 8, 2, 2, 2000, 333), (3, 16, 1, 1, 100, 2500), (3, 24, 1, 1, 333, 150), (2, 6, 2, 7, 40, 90),
+    (2, 4, 2, 1, 0, 3001), (2, 4, 2, 1, 3001, 3), (2, 33, 1, 1, 17, 1), (9, 24, 1, 2, 0, 64)])
+def test_parts_in_memory(dtype, dim, batch, heads, kv_heads, tokens, prefix, cache):
+    args = make(batch, heads, kv_heads, tokens, dim, prefix, cache, dtype, seed=prefix)
+    check(args)
+    check(args, lens_of(*[(cache, 0, tokens, cache // 2, 1, 99999, -3, 16, 17)[i] for i in range(batch)]))
+
+
+def test_empty_rows_and_junk_with_parts_in_memory():
+    import torch
+
+    import neptune_opt_b200 as NB
+
+    q, pk, pv, k, v = make(5, 48, 2, 1, 128, 140, 90)
+    lens = lens_of(90, 33, 0, 1, 17)
+    want = check((q, pk, pv, k, v), lens)
+    assert not want[0][2].any()
+    for junk in (math.nan, math.inf, -math.inf):
+        k2, v2 = k.clone(), v.clone()
+        for i, n in enumerate(lens.tolist()):
+            k2[i, :, n:] = junk
+            v2[i, :, n:] = junk
+        got = NB.prefix_attention(q, pk, pv, k2, v2, lens, return_lse=True)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    q[..., 0] = q[..., 0].abs() + 0.5
+    pk[..., 0] = -math.inf
+    k[..., 0] = -math.inf
+    o, lse = NB.prefix_attention(q, pk, pv, k, v, return_lse=True)
+    assert not o.any() and bool((lse == -math.inf).all())
+    k[1, 0, 5] = math.nan
+    o, lse = NB.prefix_attention(q, pk, pv, k, v, return_lse=True)
+    assert bool(torch.isnan(o[1, :24]).all()) and not o[1, 24:].any() and not o[0].any()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_one_kernel_and_parts_in_memory_agree(dim):
+    """The first sequences alone and the whole batch, which has more units than SMs: both within the bounds, in layouts
+    of rows that lie apart."""
+    import torch
+
+    import neptune_opt_b200 as NB
+
+    q, pk, pv, k, v = make(200, 8, 4, 1, dim, 301, 1500)
+    q, k, v = q.transpose(0, 1).contiguous().transpose(0, 1), k.transpose(1, 2).contiguous().transpose(1, 2), v
+    lens = torch.randint(0, 1501, (200,), dtype=torch.int32, device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    for n in (1, 7, 40, 200):
+        o, lse = NB.prefix_attention(q[:n], pk, pv, k[:n], v[:n], lens[:n], return_lse=True)
+        some = slice(max(0, n - 3), n)
+        check((q[some], pk, pv, k[some], v[some]), lens[some], got=(o[some], lse[some]))
+
+
 def test_other_scales():
     check(make(2, 4, 2, 1, 128, 90, 20), scale=1.0)
     check(make(2, 4, 2, 1, 128, 90, 20, std=3.0), scale=1e-4)
