@@ -448,9 +448,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, NT>)
 // The same in one kernel without parts in memory, where a CTA a sequence and key/value head is enough: its warps share the
 // prefix and the cache, one list of keys for the same rows, and join in shared memory. (Rows as in stream_kernel; of a
 // unit's two tiles the prefix's rows are the sequence's own.) The bound is latency, a launch and a few steps.
-constexpr int kSoloWarps = 8;
-template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kSoloWarps * 32, 1)
+template <typename T, int D, int NT, int W>
+__global__ void __launch_bounds__(W * 32, D == 64 || W == 4 ? 2 : 1)
     solo_kernel(const __grid_constant__ CUtensorMap shared_k, const __grid_constant__ CUtensorMap shared_v,
                 const __grid_constant__ CUtensorMap own_k, const __grid_constant__ CUtensorMap own_v, const StreamArgs a,
                 void* out, float* out_lse) {
@@ -458,9 +457,9 @@ __global__ void __launch_bounds__(kSoloWarps * 32, 1)
     constexpr int kPitch = D + 4;  // floats of a row in shared memory: no two lanes of a store meet in a bank
     static_assert(8 * NT * kPitch * 4 <= kStages * 2 * kTile, "a warp leaves its output in its stages");
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t full[kSoloWarps][kStages];
-    __shared__ int abort_flag[kSoloWarps];
-    __shared__ float sh_m[kSoloWarps][8 * NT], sh_l[kSoloWarps][8 * NT];
+    __shared__ uint64_t full[W][kStages];
+    __shared__ int abort_flag[W];
+    __shared__ float sh_m[W][8 * NT], sh_l[W][8 * NT];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t all_stages = (smem_u32(smem_raw) + 1023u) & ~1023u, mine = all_stages + warp * (kStages * 2 * kTile);
     if (lane == 0) {
@@ -473,7 +472,7 @@ __global__ void __launch_bounds__(kSoloWarps * 32, 1)
     const int seq = (int)(blockIdx.x / (unsigned)a.kv_heads), head = (int)(blockIdx.x % (unsigned)a.kv_heads);
     const int group = a.query.group, tokens = a.query.tokens, rows = group * tokens;
     const int own = tokens_of(a.lens, seq, a.cache), shared_steps = steps_of(a.prefix), steps = shared_steps + steps_of(own);
-    const int share = (steps + kSoloWarps - 1) / kSoloWarps, begin = warp * share, end = min(begin + share, steps);
+    const int share = (steps + W - 1) / W, begin = warp * share, end = min(begin + share, steps);
     int get = begin;
     auto copy = [&](int stage) {
         if (get >= end) return;
@@ -555,15 +554,15 @@ __global__ void __launch_bounds__(kSoloWarps * 32, 1)
     }
     if (!__syncthreads_and(ok)) return;
     constexpr int E = D / 32;
-    for (int in = warp; in < rows; in += kSoloWarps) {
+    for (int in = warp; in < rows; in += W) {
         float top = -NB200_INF, sum = 0.f, v[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) v[e] = 0.f;
         if (own - tokens + in % tokens >= 0) {
 #pragma unroll
-            for (int w = 0; w < kSoloWarps; ++w) top = fmaxf(top, sh_m[w][in]);
+            for (int w = 0; w < W; ++w) top = fmaxf(top, sh_m[w][in]);
 #pragma unroll
-            for (int w = 0; w < kSoloWarps; ++w) {
+            for (int w = 0; w < W; ++w) {
                 const float l = sh_l[w][in], m = sh_m[w][in];
                 const float f = m == -NB200_INF ? l : ex2(m - top);  // without a score but -inf the sum is 0, or NaN
                 sum += f * l;
@@ -715,13 +714,16 @@ Plan plan_of(const nb200_prefix_attn_args& a) {
     Plan p = {};
     const int64_t own_rows = a.heads / a.kv_heads * a.tokens;
     p.rows = a.batch * own_rows;
-    // One kernel while what an SM reads, here in keys of head dimension 128, costs less than a second launch and the join.
-    // bf16 on the GPU alone, 128: 1 sequence, 4 heads on 1, prefix 200, cache 64 4.5 us (with parts in memory 5.7); 32 heads
-    // on 8, prefix 500, caches of 300, 1 sequence 7.4 (6.8), 16 sequences 7.7 (13.5), 32 14.5 (15.9); 4 sequences, 1000 and
-    // 1000 13.4 (15.3), 3000 and 200 19.0 (11.6); 1 sequence, 1000 and 1000 13.3 (8.8).
+    // One kernel while reading the prefix once a sequence, and a sequence's keys into one SM (about 190 keys of head
+    // dimension 128 a us, in which everything here is counted), costs less than a second launch, the parts and the join.
+    // bf16 on the GPU alone, 32 heads on 8 of 128, full caches, prefix and cache: 200 and 64, 1 sequence 4.5 us (with parts
+    // in memory 5.9), 32 5.8 (12.0), 256 35 (26); 500 and 1024, 4 sequences 10.8 (11.1), 32 24 (32); 1000 and 1000, 1 sequence
+    // 13.1 (8.8), 16 13.6 (17.4); 2000 and 100, 4 13.5 (10.5), 32 23.5 (19.0); 100 and 4096, 4 24 (16), 64 157 (171). The last
+    // limit is for one long sequence among short ones.
     const int64_t units = a.batch * a.kv_heads, waves = (units + sm_count() - 1) / sm_count();
-    p.solo = own_rows <= 16 && units < 1 << 20 &&
-             waves * (a.prefix + a.cache) * a.head_dim / 128 <= std::min<int64_t>(500 + 40 * units, 2048);
+    const int64_t prefix_keys = waves * a.prefix * a.head_dim / 128, own_keys = waves * a.cache * a.head_dim / 128;
+    p.solo = own_rows <= 16 && prefix_keys <= 1500 + own_keys / 7 &&
+             (waves == 1 ? prefix_keys + own_keys <= 500 + 40 * units : a.cache * a.head_dim <= 4096 * 128);
     if (p.solo) {
         p.nt = own_rows <= 8 ? 1 : 2;
         p.bytes = 16;
@@ -766,7 +768,7 @@ Plan plan_of(const nb200_prefix_attn_args& a) {
     return p;
 }
 
-SharedLimit g_shared[20];
+SharedLimit g_shared[28];
 
 struct Maps {
     CUtensorMap shared_k, shared_v, own_k, own_v;
@@ -781,12 +783,12 @@ int launch_stream(const Maps& m, const StreamArgs& a, int64_t ctas, SharedLimit&
     return finish_launch("nb200_prefix_attention");
 }
 
-template <typename T, int D, int NT>
+template <typename T, int D, int NT, int W>
 int launch_solo(const Maps& m, const StreamArgs& a, void* o, float* lse, SharedLimit& limit, cudaStream_t st) {
-    constexpr uint32_t bytes = kSoloWarps * kStages * 2 * kStepKeys * D * 2 + 1024;  // + alignment slack
-    if (const int rc = limit.raise("nb200_prefix_attention", solo_kernel<T, D, NT>, bytes)) return rc;
-    launch_pdl(solo_kernel<T, D, NT>, (unsigned)(a.batch * a.kv_heads), kSoloWarps * 32, bytes, st, m.shared_k, m.shared_v,
-               m.own_k, m.own_v, a, o, lse);
+    constexpr uint32_t bytes = W * kStages * 2 * kStepKeys * D * 2 + 1024;  // + alignment slack
+    if (const int rc = limit.raise("nb200_prefix_attention", solo_kernel<T, D, NT, W>, bytes)) return rc;
+    launch_pdl(solo_kernel<T, D, NT, W>, (unsigned)(a.batch * a.kv_heads), W * 32, bytes, st, m.shared_k, m.shared_v, m.own_k,
+               m.own_v, a, o, lse);
     count_launch();
     return finish_launch("nb200_prefix_attention");
 }
@@ -825,9 +827,15 @@ int launch_all(const nb200_prefix_attn_args& n, const nb200_attn_strides* s, con
     a.rows = (int)p.rows, a.prefix_tiles = (int)p.prefix_tiles, a.own_tiles = (int)p.own_tiles;
     a.slot_rows = (int)p.slot_rows;
     a.sl2 = sl2;
-    if (p.solo)
-        return p.nt == 1 ? launch_solo<T, D, 1>(maps, a, o, lse, limits[3], st)
-                         : launch_solo<T, D, 2>(maps, a, o, lse, limits[4], st);
+    if (p.solo) {
+        // Where there are more CTAs than SMs, two an SM: one starts while the other reads. Head dimension 128 has room for
+        // them with four warps each.
+        if (D == 128 && a.batch * (int64_t)a.kv_heads > sm_count())
+            return p.nt == 1 ? launch_solo<T, D, 1, 4>(maps, a, o, lse, limits[3], st)
+                             : launch_solo<T, D, 2, 4>(maps, a, o, lse, limits[4], st);
+        return p.nt == 1 ? launch_solo<T, D, 1, 8>(maps, a, o, lse, limits[5], st)
+                         : launch_solo<T, D, 2, 8>(maps, a, o, lse, limits[6], st);
+    }
     a.o = at(p.o), a.lse = at(p.lse), a.span = reinterpret_cast<int2*>(at(p.span));
     a.beside = p.splits > 0;  // the tensor cores' kernel started after all that came before
     rc = p.nt == 1   ? launch_stream<T, D, 1>(maps, a, p.ctas, limits[0], st)
@@ -886,9 +894,9 @@ int launch_prefix_attention(const nb200_prefix_attn_args& n, const nb200_attn_st
     if (n.dtype == NB200_BF16)
         return n.head_dim == 128
                    ? launch_all<__nv_bfloat16, 128>(n, s, q, pk, pv, k, v, o, lse, w, g_shared, st)
-                   : launch_all<__nv_bfloat16, 64>(n, s, q, pk, pv, k, v, o, lse, w, g_shared + 5, st);
-    return n.head_dim == 128 ? launch_all<__half, 128>(n, s, q, pk, pv, k, v, o, lse, w, g_shared + 10, st)
-                             : launch_all<__half, 64>(n, s, q, pk, pv, k, v, o, lse, w, g_shared + 15, st);
+                   : launch_all<__nv_bfloat16, 64>(n, s, q, pk, pv, k, v, o, lse, w, g_shared + 7, st);
+    return n.head_dim == 128 ? launch_all<__half, 128>(n, s, q, pk, pv, k, v, o, lse, w, g_shared + 14, st)
+                             : launch_all<__half, 64>(n, s, q, pk, pv, k, v, o, lse, w, g_shared + 21, st);
 }
 
 }  // namespace nb200
