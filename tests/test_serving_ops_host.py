@@ -211,7 +211,7 @@ def test_c_prefix_attention_refuses_before_any_launch():
         assert _c_attention(**empty, q=NULL, work=NULL) == L.NB200_OK
     for bad in ({"kv": 3}, {"kv": 0}, {"dtype": 0}, {"dtype": 7}, {"scale": 0.0}, {"scale": float("nan")}, {"batch": -1},
                 {"prefix": -1}, {"cache": -1}, {"tokens": -1}, {"q": NULL}, {"q": ODD}, {"pk": NULL}, {"k": ODD}, {"lse": ODD},
-                {"work": ODD}, {"work": NULL}, {"nbytes": 64}):
+                {"work": ODD}, {"work": NULL}, {"nbytes": 8}, {"nbytes": 4096, "prefix": 4000}):
         assert _c_attention(**bad) == L.NB200_ERR_ARG, bad
     assert _c_attention(dim=96) == L.NB200_ERR_UNSUPPORTED and _c_attention(dim=0) == L.NB200_ERR_UNSUPPORTED
     for big in ({"prefix": (1 << 30) + 1}, {"cache": (1 << 30) + 1}, {"tokens": 1 << 28}, {"batch": 1 << 28},
