@@ -434,7 +434,7 @@ int nb200_norm8(const nb200_norm8_args* args, void* q, float* scale, void* y, vo
  * bias index outside [0, vocab) is skipped. repetition, presence, frequency, temperature: fp32 [rows], each
  * nullable (no such step); the caller keeps repetition and temperature positive. allowed (nullable) is
  * [rows, ceil(vocab / 32)] int32, bit v % 32 of word v / 32. logits is [rows, vocab], out contiguous like it, of one
- * dtype; every tensor has unit column stride. biases <= 1024 (else NB200_ERR_CAPACITY). work: device memory, 16-byte
+ * dtype, and no memory of logits; every tensor has unit column stride. biases <= 1024 (else NB200_ERR_CAPACITY). work: device memory, 16-byte
  * aligned, of nb200_penalize_logits_work_bytes(args) bytes (0 without history and biases). No counterpart in the
  * reference. */
 typedef struct {

@@ -809,6 +809,13 @@ int nb200_penalize_logits(const nb200_logits_args* args, void* out, void* work, 
         set_error("nb200_penalize_logits: a tensor is not aligned to its elements");
         return NB200_ERR_ARG;
     }
+    // A named token's logit is read once more after its tile is written.
+    const uintptr_t size = args->dtype == NB200_F32 ? 4 : 2, in = (uintptr_t)args->logits, to = (uintptr_t)out;
+    if (in < to + (uintptr_t)(args->rows * args->vocab) * size &&
+        to < in + (uintptr_t)((args->rows - 1) * args->stride_logits + args->vocab) * size) {
+        set_error("nb200_penalize_logits: out must not overlap logits");
+        return NB200_ERR_ARG;
+    }
     const int64_t need = logits_work_bytes(*args);
     if (need && (!work || !aligned16(work) || work_bytes < need)) {
         set_error("nb200_penalize_logits: work must hold %lld bytes, 16-byte aligned", (long long)need);

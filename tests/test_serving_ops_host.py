@@ -284,14 +284,18 @@ def test_c_entries_refuse_tensors_off_their_elements():
     pointers = ("logits", "tokens", "bias_index", "bias_value", "token_lens", "prompt_lens", "allowed", "repetition",
                 "presence", "frequency", "temperature")
 
-    def logits(dtype=0, index=1, out=base, **changes):
-        a = L.NB200LogitsArgs(*(changes.get(name, base) for name in pointers), 4, 100, 8, 8, 100, 8, 8, 8, 4, dtype, index,
+    def logits(dtype=0, index=1, out=1 << 28, history=8, work=FAKE, nbytes=1 << 30, **changes):
+        a = L.NB200LogitsArgs(*(changes.get(name, base) for name in pointers), 4, 100, history, 8, 100, 8, 8, 8, 4, dtype, index,
                               index)
-        return lib.nb200_penalize_logits(ctypes.byref(a), ctypes.c_void_p(out), FAKE, 1 << 30, NULL)
+        return lib.nb200_penalize_logits(ctypes.byref(a), ctypes.c_void_p(out), work, nbytes, NULL)
 
     for name in pointers:
         assert logits(**{name: base + 2}) == L.NB200_ERR_ARG, name
     for name in ("tokens", "bias_index"):
         assert logits(**{name: base + 4}) == L.NB200_ERR_ARG, name
-    assert logits(out=base + 2) == L.NB200_ERR_ARG
-    assert logits(dtype=1, logits=base + 1) == L.NB200_ERR_ARG and logits(dtype=2, out=base + 1) == L.NB200_ERR_ARG
+    assert logits(out=(1 << 28) + 2) == L.NB200_ERR_ARG
+    for out in (base, base + 4 * 399, base - 4 * 399):  # in place, or over an end of the input
+        assert logits(out=out) == L.NB200_ERR_ARG
+    assert logits(dtype=1, logits=base + 1) == L.NB200_ERR_ARG and logits(dtype=2, out=(1 << 28) + 1) == L.NB200_ERR_ARG
+    for bad in ({"work": NULL}, {"work": ODD}, {"nbytes": 64}):
+        assert logits(history=5000, **bad) == L.NB200_ERR_ARG, bad
