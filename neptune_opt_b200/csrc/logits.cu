@@ -20,6 +20,7 @@
 
 #include "common.cuh"
 #include "launch.h"
+#include "logits_rows.h"
 
 namespace nb200 {
 namespace {
@@ -44,37 +45,26 @@ template <typename T> constexpr int kTileBits = 10 + (Elem<T>::V == 8 ? 3 : 2);
 template <typename T> constexpr int kTile = 1 << kTileBits<T>;
 static_assert(kTile<float> == kSweepThreads * kVectors * 4, "a tile is what a CTA's threads hold");
 
-// A row's pointers, and how many tokens lie before the first whole vector of its output; tile 0 holds those, too. The input
-// of a vector lies `shift` tokens behind a 16-byte boundary, and both blocks that hold it lie in the row.
+// A row's pointers, and how it is cut.
 template <typename T>
-struct Row {
+struct Row : RowCut<(int)sizeof(T)> {
     const T* x;
     T* out;
     const int32_t* allowed;
-    int head, shift;
-    __device__ __forceinline__ Row(const Logits& a, int64_t row) {
-        const nb200_logits_args& n = a.n;
-        x = static_cast<const T*>(n.logits) + row * n.stride_logits;
-        out = static_cast<T*>(a.out) + row * n.vocab;
-        allowed = n.allowed ? n.allowed + row * n.stride_allowed : nullptr;
-        constexpr int V = Elem<T>::V;
-        auto behind = [](const void* p) { return (int)(((uint32_t)reinterpret_cast<uintptr_t>(p) & 15u) / sizeof(T)); };
-        const int first = (V - behind(out)) % V;
-        shift = (behind(x) + first) % V;
-        head = (int)min((int64_t)(first < shift ? first + V : first), n.vocab);
-    }
-    // Whole vectors from token `from` to `to`.
-    __device__ __forceinline__ int vectors(int64_t from, int64_t to, int64_t vocab) const {
-        constexpr int V = Elem<T>::V;
-        if (shift) to = min(to, vocab - (V - shift));
-        return to > from ? (int)((to - from) / V) : 0;
-    }
-    // V tokens from v on, of two neighbouring blocks.
+    __device__ __forceinline__ Row(const Logits& a, int64_t row)
+        : Row(a, static_cast<const T*>(a.n.logits) + row * a.n.stride_logits, static_cast<T*>(a.out) + row * a.n.vocab,
+              a.n.allowed ? a.n.allowed + row * a.n.stride_allowed : nullptr) {}
+    __device__ __forceinline__ Row(const Logits& a, const T* x, T* out, const int32_t* allowed)
+        : RowCut<(int)sizeof(T)>(reinterpret_cast<uintptr_t>(x), reinterpret_cast<uintptr_t>(out), a.n.vocab), x(x), out(out),
+          allowed(allowed) {}
+    // V tokens from v on, of the blocks that hold them.
     __device__ __forceinline__ uint4 joined(int64_t v) const {
-        const T* p = x + v - shift;
-        const uint4 lo = ld_keep(p), hi = ld_keep(p + Elem<T>::V);
+        const T* p = x + v - this->shift;
+        const uint4 lo = ld_keep(p);
+        uint4 hi = lo;  // not looked at where there is one block
+        if (this->blocks() > 1) hi = ld_keep(p + Elem<T>::V);
         uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-        const int bytes = shift * (int)sizeof(T);
+        const int bytes = this->shift * (int)sizeof(T);
 #pragma unroll
         for (int i = 0; i < 6; ++i) w[i] = bytes & 8 ? w[i + 2] : w[i];
 #pragma unroll
@@ -310,9 +300,8 @@ __global__ void __launch_bounds__(kSweepThreads, NAMES == SELF || JOINED ? 4 : k
     const int64_t row = blockIdx.x / (unsigned)a.tiles;
     const int tile = (int)(blockIdx.x % (unsigned)a.tiles);
     const Row<T> r(a, row);
-    const int64_t lo = tile ? min(r.head + (int64_t)tile * kTile<T>, n.vocab) : 0;
-    const int64_t hi = min(r.head + (int64_t)(tile + 1) * kTile<T>, n.vocab);
-    const int64_t body = tile ? lo : r.head;
+    const int64_t lo = r.begin(tile, kTile<T>, n.vocab), hi = r.end(tile, kTile<T>, n.vocab);
+    const int64_t body = r.body(tile, kTile<T>, n.vocab);
     const int vectors = JOINED ? r.vectors(body, hi, n.vocab) : (int)((hi - body) / V);
     uint4 raw[kVectors];
     uint32_t ok[kVectors];
