@@ -3,11 +3,7 @@
 
 #include <stdint.h>
 
-#ifdef __CUDACC__
-#define NB200_PLAIN __host__ __device__ __forceinline__
-#else
-#define NB200_PLAIN inline
-#endif
+#include "plain.h"
 
 namespace nb200 {
 

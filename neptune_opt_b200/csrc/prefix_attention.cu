@@ -22,35 +22,26 @@
 
 #include "attn.cuh"
 #include "prefix_attention.cuh"
+#include "prefix_line.h"
 
 namespace nb200 {
 namespace prefix {
 namespace {
 
 constexpr int kWarps = 4;      // warps of a stream kernel's CTA, each a worker of its own
-constexpr int kStepKeys = 16;  // keys of a worker's step
 constexpr int kStages = 3;     // steps of a worker in shared memory: one in use, two in flight
-constexpr int kEntry = 2;      // what a unit costs beside its steps, in steps
 // CTAs that an SM can hold: half the head dimension leaves room for twice as many.
 template <int D, int NT> constexpr int kCtas = D == 64 && NT <= 2 ? 4 : 2;
 
-// A unit of the stream kernel is a tile of 8 NT query rows and the keys they share: units of the prefix
-// (key/value head, row tile; none when the prefix runs on the tensor cores), then units of the caches
-// (sequence, key/value head, row tile). All units' steps of 16 keys stand in one line, each unit's behind kEntry
-// places for its own start and end, and every worker takes an equal piece of the line, whatever the sequences'
-// lengths are. A piece covers the end of one unit, whole units, the beginning of another: worker w's result for
-// unit u goes to slot w + u, which no other pair has, and span[u] says which workers had a share in u.
-struct StreamArgs {
+// What the stream kernel's workers share out (prefix_line.h), row tiles of 8 NT query rows each, and where it goes.
+struct StreamArgs : Line {
     Query query;
-    const int* lens;  // tokens of each sequence (null: all of the cache)
-    int batch, kv_heads, prefix, cache;
-    int rows;                      // query rows of a key/value head over all sequences
-    int prefix_tiles, own_tiles;   // row tiles of a unit's rows
+    int rows;       // query rows of a key/value head over all sequences
     int slot_rows;
-    float sl2;                     // scale * log2(e)
-    float *o, *lse;                // [slots][slot_rows][D], [slots][slot_rows]
-    int2* span;                    // [units]: first and last worker
-    bool beside;                   // runs beside the kernel ahead of it, of which it needs nothing
+    float sl2;      // scale * log2(e)
+    float *o, *lse; // [slots][slot_rows][D], [slots][slot_rows]
+    int2* span;     // [units]: first and last worker
+    bool beside;    // runs beside the kernel ahead of it, of which it needs nothing
 };
 
 template <typename T> struct Mma;
@@ -82,54 +73,20 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {  // an 8 x 8 matrix
     return y;
 }
 
-__device__ __forceinline__ int steps_of(int keys) { return (keys + kStepKeys - 1) / kStepKeys; }
-// Places of a unit in the line.
-__device__ __forceinline__ int places_of(int keys) { return keys > 0 ? kEntry + steps_of(keys) : 0; }
-
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint64_t* bar) {
     tc::tma_load_4d(reinterpret_cast<void*>(__cvta_shared_to_generic(dst)), map, c0, c1, c2, c3, bar);
 }
-
-// A position in the line: a step of a unit, and how many places of the worker's piece are left from there on.
-struct Cursor {
-    int batch;  // -1: a unit of the prefix
-    int head, tile, step, steps, keys;
-    int left;   // <= 0: at the end
-
-    __device__ __forceinline__ void sequence(const StreamArgs& a, int b) {
-        batch = b, head = 0, tile = 0, keys = tokens_of(a.lens, b, a.cache), steps = steps_of(keys);
-    }
-    // The first step of the next unit; only while places are left.
-    __device__ __forceinline__ void next_unit(const StreamArgs& a) {
-        step = 0;
-        left -= kEntry;
-        if (++tile < (batch < 0 ? a.prefix_tiles : a.own_tiles)) return;
-        tile = 0;
-        if (++head < a.kv_heads) return;
-        int b = batch;
-        do sequence(a, ++b);
-        while (steps == 0 && b + 1 < a.batch);
-    }
-    __device__ __forceinline__ void next(const StreamArgs& a) {
-        --left;
-        if (++step == steps && left > 0) next_unit(a);
-    }
-    __device__ __forceinline__ int unit(const StreamArgs& a) const {
-        return batch < 0 ? head * a.prefix_tiles + tile
-                         : a.kv_heads * a.prefix_tiles + (batch * a.kv_heads + head) * a.own_tiles + tile;
-    }
-};
 
 // The piece of the line that a worker takes (a whole warp calls it). Each lane sums up the places of a run of sequences;
 // the run that holds the piece's first place is then walked by its lane.
 __device__ __forceinline__ Cursor piece_of(const StreamArgs& a, int worker, int workers) {
     const int lane = threadIdx.x & 31;
-    const int64_t each = (int64_t)a.kv_heads * a.own_tiles;  // units of a sequence
+    const int64_t each = a.units_of_a_sequence();
     const int run = (a.batch + 31) / 32, b0 = min(lane * run, a.batch), b1 = min(b0 + run, a.batch);
     int own = 0;  // places of the lane's sequences, for one unit of each
     if (a.lens) {
 #pragma unroll 8
-        for (int b = b0; b < b1; ++b) own += places_of(tokens_of(a.lens, b, a.cache));
+        for (int b = b0; b < b1; ++b) own += places_of(a.tokens(b));
     } else {
         own = (b1 - b0) * places_of(a.cache);
     }
@@ -139,33 +96,26 @@ __device__ __forceinline__ Cursor piece_of(const StreamArgs& a, int worker, int 
         const int x = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += x;
     }
-    const int64_t shared = (int64_t)a.kv_heads * a.prefix_tiles * places_of(a.prefix);
-    const int64_t all = shared + each * __shfl_sync(0xffffffffu, upto, 31);
+    const int64_t shared = a.shared_places(), all = shared + each * __shfl_sync(0xffffffffu, upto, 31);
     const int64_t share = (all + workers - 1) / workers;
     int64_t at = worker * share;
     Cursor c;
     c.left = 0;
     if (at >= all) return c;
     c.left = (int)min(share, all - at);
-    int tiles = a.prefix_tiles;
-    if (at < shared) {
-        c.batch = -1, c.keys = a.prefix, c.steps = steps_of(a.prefix);
-    } else {
+    int b = -1;
+    if (at >= shared) {
         at -= shared;
-        tiles = a.own_tiles;
         const int unit_at = (int)(at / each);  // the place, counted in one unit of each sequence
         const int holder = __ffs(__ballot_sync(0xffffffffu, upto > unit_at)) - 1;
-        int b = b0, before = upto - own;
+        int before = upto - own;
+        b = b0;
         if (lane == holder)
-            for (int p; before + (p = places_of(tokens_of(a.lens, b, a.cache))) <= unit_at; ++b) before += p;
+            for (int p; before + (p = places_of(a.tokens(b))) <= unit_at; ++b) before += p;
         b = __shfl_sync(0xffffffffu, b, holder);
         at -= each * __shfl_sync(0xffffffffu, before, holder);
-        c.sequence(a, b);
     }
-    const int places = kEntry + c.steps, unit = (int)(at / places), place = (int)(at - (int64_t)unit * places) - kEntry;
-    c.head = unit / tiles, c.tile = unit % tiles;
-    c.step = max(place, 0);
-    c.left -= max(-place, 0);
+    c.start(a, b, at);
     return c;
 }
 
@@ -280,7 +230,7 @@ __device__ __forceinline__ void zero_behind(uint32_t vs, int keys, int lane) {
 // fragments of K and V serve all NT column tiles.
 //
 // Every wait is bounded; one that runs out sets bit 1 of the fault word, and the worker waits (again with a limit) for
-// its copies and leaves its slots unwritten.
+// its copies and leaves NaN in the slots of its unfinished shares.
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kWarps * 32, kCtas<D, NT>)
     stream_kernel(const __grid_constant__ CUtensorMap shared_k, const __grid_constant__ CUtensorMap shared_v,
@@ -439,15 +389,24 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, NT>)
         }
         begin();
     }
-    // Every copy lands before the CTA may exit; `sent` were issued, of which `done` have been waited for.
-    if (!ok)
+    if (!ok) {
+        // Every copy lands before the CTA may exit; `sent` were issued, of which `done` have been waited for.
         for (int i = done; i < sent; ++i) drain_bar(&full[warp][i % kStages], (i / kStages) & 1u);
+        for (;;) {
+            const int unit = use.unit(a);
+            for (int in = lane; in < a.slot_rows; in += 32) a.lse[((int64_t)worker + unit) * a.slot_rows + in] = NB200_NAN;
+            if (lane == 0 && use.ends_unit()) a.span[unit].y = worker;
+            if (!use.skip_unit(a)) break;
+            if (lane == 0) a.span[use.unit(a)].x = worker;
+        }
+    }
     if (waits) pdl_wait();
 }
 
 // The same in one kernel without parts in memory, where a CTA a sequence and key/value head is enough: its warps share the
 // prefix and the cache, one list of keys for the same rows, and join in shared memory. (Rows as in stream_kernel; of a
-// unit's two tiles the prefix's rows are the sequence's own.) The bound is latency, a launch and a few steps.
+// unit's two tiles the prefix's rows are the sequence's own.) The bound is latency, a launch and a few steps. A wait that
+// runs out, as there: the CTA's rows read out as NaN.
 template <typename T, int D, int NT, int W>
 __global__ void __launch_bounds__(W * 32, D == 64 || W == 4 ? 2 : 1)
     solo_kernel(const __grid_constant__ CUtensorMap shared_k, const __grid_constant__ CUtensorMap shared_v,
@@ -552,13 +511,13 @@ __global__ void __launch_bounds__(W * 32, D == 64 || W == 4 ? 2 : 1)
                 }
             }
     }
-    if (!__syncthreads_and(ok)) return;
+    const bool complete = __syncthreads_and(ok);
     constexpr int E = D / 32;
     for (int in = warp; in < rows; in += W) {
-        float top = -NB200_INF, sum = 0.f, v[E];
+        float top = -NB200_INF, sum = complete ? 0.f : NB200_NAN, v[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) v[e] = 0.f;
-        if (own - tokens + in % tokens >= 0) {
+        if (complete && own - tokens + in % tokens >= 0) {
 #pragma unroll
             for (int w = 0; w < W; ++w) top = fmaxf(top, sh_m[w][in]);
 #pragma unroll
@@ -586,6 +545,7 @@ struct JoinArgs {
     const float *tensor_o, *tensor_lse;  // parts of the tensor cores: [splits][kv_heads][rows][D], and without D
     const float *o, *lse;                // slots of the stream kernel
     const int2* span;
+    int workers;                         // of the stream kernel
     void* out;                           // [batch, heads, tokens, D]
     float* out_lse;                      // nullable
     const int* lens;
@@ -597,7 +557,8 @@ struct JoinArgs {
 // WIDE: a CTA per query row, its eight warps taking turns at the parts; else a warp per row. The parts are the
 // tensor cores' (or the prefix units' slots), then the own units' slots, weighed and added in a fixed order. The bound is
 // latency: 3 to 5 us behind the other kernels. A query before its
-// sequence's first token (a free slot of the batch) reads out as zero with a log-sum-exp of -inf.
+// sequence's first token (a free slot of the batch) reads out as zero with a log-sum-exp of -inf; a row whose parts are
+// not all there as NaN.
 template <typename T, int D, bool WIDE>
 __global__ void __launch_bounds__(256) join_kernel(const JoinArgs a) {
     constexpr int E = D / 32, kTurns = WIDE ? 8 : 1;  // parts of a turn are kTurns apart
@@ -624,16 +585,21 @@ __global__ void __launch_bounds__(256) join_kernel(const JoinArgs a) {
         const int in = r - b * a.group * a.tokens;
         const int unit = a.kv_heads * a.prefix_tiles + (b * a.kv_heads + head) * a.own_tiles + in / a.tile_rows;
         const int2 w = a.span[unit];
+        bool known = are_workers(w.x, w.y, a.workers);
         if (a.splits) {
             far_o = a.tensor_o, far_lse = a.tensor_lse, far = id, far_step = all, nfar = a.splits;
         } else if (a.prefix_tiles) {
             const int shared = head * a.prefix_tiles + r / a.tile_rows;
             const int2 u = a.span[shared];
+            known &= are_workers(u.x, u.y, a.workers);
             far = (int64_t)(u.x + shared) * a.slot_rows + r % a.tile_rows;
             nfar = u.y - u.x + 1;
         }
         const int64_t near = (int64_t)(w.x + unit) * a.slot_rows + in % a.tile_rows;
-        const int parts = nfar + w.y - w.x + 1;
+        // Unless lengths change while a call runs, or a worker is lost, the spans are right; what they name is read only then.
+        if (!known) atomicOr(&g_attn_fault, 2u);
+        const int parts = known ? nfar + w.y - w.x + 1 : 0;
+        if (!known) sum = NB200_NAN;
         auto row_of = [&](int i) { return i < nfar ? far + i * far_step : near + (int64_t)(i - nfar) * a.slot_rows; };
         auto lse_of = [&](int i) { return i < parts ? (i < nfar ? far_lse : a.lse)[row_of(i)] : -NB200_INF; };
         // Four o's in flight at a time, the first four before their weights are known.
@@ -648,7 +614,7 @@ __global__ void __launch_bounds__(256) join_kernel(const JoinArgs a) {
             }
         };
         const int start = WIDE ? warp : 0;
-        load4(start);
+        if (known) load4(start);
         for (int i = lane; i < parts; i += 32) top = fmaxf(top, lse_of(i));
         top = warp_max(top);
         for (int i0 = start; i0 < parts; i0 += 32 * kTurns) {  // 32 parts, weighed by the 32 lanes
@@ -844,6 +810,7 @@ int launch_all(const nb200_prefix_attn_args& n, const nb200_attn_strides* s, con
     if (rc) return rc;
     JoinArgs j = {};
     j.tensor_o = at(p.tensor_o), j.tensor_lse = at(p.tensor_lse), j.o = a.o, j.lse = a.lse, j.span = a.span;
+    j.workers = (int)p.ctas * kWarps;
     j.out = o, j.out_lse = lse, j.lens = n.seq_lens;
     j.kv_heads = a.kv_heads, j.group = query.group, j.tokens = query.tokens, j.rows = a.rows, j.cache = a.cache;
     j.splits = p.splits, j.prefix_tiles = a.prefix_tiles, j.own_tiles = a.own_tiles, j.tile_rows = 8 * p.nt;

@@ -18,8 +18,8 @@
 // columns the last P_t was read from: one thread's MMAs execute in issue order.
 //
 // Every wait is bounded; one that runs out sets bit 1 of the fault word and the CTA's abort flag, the producer
-// waits for its copies, the MMA thread for its products, and the CTA frees its tensor memory and ends with its
-// part unwritten.
+// waits for its copies, the MMA thread for its products, and the CTA frees its tensor memory and ends with NaN in its
+// part's sums.
 #include <algorithm>
 
 #include "attn.cuh"
@@ -322,8 +322,14 @@ __device__ __forceinline__ void softmax_stream(uint8_t* smem, Bars* b, uint32_t 
         if (t == 1) b->m[r] = m, b->l[r] = l;
         asm volatile("bar.sync 1, 256;" ::: "memory");
         if (t == 1) return;
+        if (*abort) ok = false;  // either stream
     }
-    if (!ok) return;
+    const int row = (u.pair ? t * kRows : 0) + r;
+    const int64_t at = ((int64_t)split * a.kv_heads + u.head) * a.rows + u.row0 + row;
+    if (!ok) {
+        if (row < u.nrows) a.lse[at] = NB200_NAN;
+        return;
+    }
     float f0 = 1.f, f1 = 0.f;
     const bool merge = !u.pair && u.n > 1;
     if (merge) {
@@ -336,8 +342,6 @@ __device__ __forceinline__ void softmax_stream(uint8_t* smem, Bars* b, uint32_t 
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     f0 *= inv, f1 *= inv;
-    const int row = (u.pair ? t * kRows : 0) + r;
-    const int64_t at = ((int64_t)split * a.kv_heads + u.head) * a.rows + u.row0 + row;
     float4* out = reinterpret_cast<float4*>(a.o + at * D);
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) {
