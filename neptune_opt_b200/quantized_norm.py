@@ -68,16 +68,23 @@ def validate_quantized_norm_inputs(x, weight, residual, group, dtype, eps):
         raise NotImplementedError(f"{what}: width {x.shape[-1]} exceeds {MAX_WIDTH}")
 
 
-def quantized_rms_norm(x, weight, residual=None, *, group=None, dtype=None, eps: float = 1e-6):
-    """(q, scale, y): the normalised rows in 8 bits (dtype, float8_e4m3fn by default), their fp32 scales
-    [..., 1] or [..., width / group], and the new residual stream in x's dtype (None without a residual).
-    All fresh and contiguous."""
+def _kinds():
+    """The op's number of each dtype; None stands for the default. Threads may meet here: the table is shown whole."""
     global _KINDS
     if _KINDS is None:
         import torch
 
-        _KINDS = {getattr(torch, name): kind for name, kind in KINDS.items()}
-        _KINDS[None] = KINDS["float8_e4m3fn"]
+        kinds = {getattr(torch, name): kind for name, kind in KINDS.items()}
+        kinds[None] = KINDS["float8_e4m3fn"]
+        _KINDS = kinds
+    return _KINDS
+
+
+def quantized_rms_norm(x, weight, residual=None, *, group=None, dtype=None, eps: float = 1e-6):
+    """(q, scale, y): the normalised rows in 8 bits (dtype, float8_e4m3fn by default), their fp32 scales
+    [..., 1] or [..., width / group], and the new residual stream in x's dtype (None without a residual).
+    All fresh and contiguous."""
     q, scale, y = run_cxx("norm8", x, (x, weight, residual, 0 if group is None else group if group else -1,
-                                       _KINDS.get(dtype, -1), eps), validate_quantized_norm_inputs, x, weight, residual, group, dtype, eps)
+                                       _kinds().get(dtype, -1), eps), validate_quantized_norm_inputs, x, weight, residual,
+                          group, dtype, eps)
     return q, scale, None if residual is None else y
