@@ -493,8 +493,10 @@ int launch(const Logits& a, SharedLimit& shared, cudaStream_t st) {
         if (const int rc = shared.raise(what, name_kernel<T>, most)) return rc;
         launch_pdl(name_kernel<T>, (unsigned)(n.rows * a.parts), kNameThreads,
                    name_bytes(a.range, a.slots, a.buckets, (int)n.biases), st, a);
+        count_launch();
+        if (const int rc = finish_launch(what)) return rc;  // the sweep takes addresses from what the names' kernel leaves
         launch_pdl(alike ? sweep_kernel<T, ENTRIES, false> : sweep_kernel<T, ENTRIES, true>, grid, kSweepThreads, 0, st, a);
-        count_launch(2);
+        count_launch();
     } else {
         auto kernel = a.self ? alike ? sweep_kernel<T, SELF, false> : sweep_kernel<T, SELF, true>
                              : alike ? sweep_kernel<T, NONE, false> : sweep_kernel<T, NONE, true>;
