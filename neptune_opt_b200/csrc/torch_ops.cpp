@@ -59,7 +59,10 @@
 #include <torch/csrc/inductor/aoti_torch/utils.h>
 #include <torch/library.h>
 
+#include <algorithm>
+#include <cmath>
 #include <cstring>
+#include <initializer_list>
 #include <map>
 #include <mutex>
 #include <string>
@@ -683,7 +686,7 @@ at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType dtype, const at::Tensor& 
 
 // What prefix_attention asks of its tensors, symbolic sizes too.
 void check_prefix_attention(const at::Tensor& q, const at::Tensor& pk, const at::Tensor& pv, const at::Tensor& k,
-                            const at::Tensor& v, const OptTensor& seq_lens, const char* what) {
+                            const at::Tensor& v, const OptTensor& seq_lens, double scale, const char* what) {
     for (const at::Tensor* t : {&q, &pk, &pv, &k, &v}) {
         check_strided(*t, what);
         TORCH_CHECK_TYPE(t->scalar_type() == q.scalar_type() &&
@@ -700,6 +703,9 @@ void check_prefix_attention(const at::Tensor& q, const at::Tensor& pk, const at:
     TORCH_CHECK_VALUE(qs[1] == ks[1] || (ks[1] > 0 && qs[1] % ks[1] == 0), what, ": ", qs[1],
                       " query heads cannot share ", ks[1], " key/value heads");
     check_seq_lens(seq_lens, q, what);
+    TORCH_CHECK_VALUE(std::isfinite((float)scale) && (float)scale > 0.f, what, ": scale must be finite and positive");
+    TORCH_CHECK_NOT_IMPLEMENTED(qs[3] == 64 || qs[3] == 128, what, ": head_dim ", qs[3],
+                                " is not supported (the kernels are built for 64 and 128)");
 }
 
 // As attn_rows, for [kv_heads, prefix, head_dim].
@@ -715,7 +721,7 @@ std::tuple<at::Tensor, at::Tensor> prefix_attention_cuda(const at::Tensor& q_, c
                                                          bool with_lse) {
     const char* what = "nb200.prefix_attention";
     check_cuda(q_, what);
-    check_prefix_attention(q_, pk_, pv_, k_, v_, seq_lens, what);
+    check_prefix_attention(q_, pk_, pv_, k_, v_, seq_lens, scale, what);
     c10::cuda::CUDAGuard guard(q_.device());
     const at::Tensor q = attn_rows(q_), k = attn_rows(k_), v = attn_rows(v_), pk = prefix_rows(pk_), pv = prefix_rows(pv_);
     at::Tensor o = fresh(q.sizes(), q.scalar_type(), q);
@@ -740,20 +746,36 @@ at::ScalarType byte_dtype(int64_t kind, const char* what) {
     return kind == NB200_E4M3 ? at::kFloat8_e4m3fn : kind == NB200_E5M2 ? at::kFloat8_e5m2 : at::kChar;
 }
 
+// What norm8 asks of its arguments, symbolic sizes too.
+void check_norm8(const at::Tensor& x, const at::Tensor& weight, const OptTensor& residual, int64_t group, double eps,
+                 const char* what) {
+    check_strided(x, what);
+    dtype_code(x);
+    TORCH_CHECK_VALUE(x.dim() >= 1 && x.sym_size(-1) >= 1, what, ": x must be [..., width]");
+    const c10::SymInt width = x.sym_size(-1);
+    NormInputs::same_kind(weight, x, what);
+    TORCH_CHECK_VALUE(weight.dim() == 1 && weight.sym_size(0) == width, what, ": weight must be 1-D with x's last dimension");
+    if (present(residual)) {
+        NormInputs::same_kind(*residual, x, what);
+        TORCH_CHECK_VALUE(residual->sym_sizes() == x.sym_sizes(), what, ": residual must have x's shape");
+    }
+    TORCH_CHECK_VALUE(group == 0 || group == 16 || group == 32 || group == 64 || group == 128, what,
+                      ": group must be 0, 16, 32, 64 or 128, got ", group);
+    TORCH_CHECK_VALUE(group == 0 || width % group == 0, what, ": width ", width, " is not whole groups of ", group);
+    TORCH_CHECK_VALUE(std::isfinite((float)eps) && (float)eps > 0.f, what, ": eps must be finite and positive in fp32");
+    TORCH_CHECK_NOT_IMPLEMENTED(width <= 16384, what, ": width ", width, " exceeds 16384");
+}
+
 std::tuple<at::Tensor, at::Tensor, at::Tensor> norm8_cuda(const at::Tensor& x_, const at::Tensor& weight_,
                                                           const OptTensor& residual_, int64_t group, int64_t kind,
                                                           double eps) {
     const char* what = "nb200.norm8";
     const at::ScalarType dtype = byte_dtype(kind, what);
-    check_strided(x_, what);
     check_cuda(x_, what);
+    check_norm8(x_, weight_, residual_, group, eps, what);
     nb200_norm8_args a = {};
     a.dtype = dtype_code(x_);
     a.kind = (int32_t)kind;
-    TORCH_CHECK_VALUE(x_.dim() >= 1 && x_.size(-1) >= 1, what, ": x must be [..., width]");
-    NormInputs::same_kind(weight_, x_, what);
-    TORCH_CHECK_VALUE(weight_.dim() == 1 && weight_.size(0) == x_.size(-1), what,
-                      ": weight must be 1-D with x's last dimension");
     a.width = x_.size(-1);
     a.rows = x_.numel() / a.width;
     a.group = group;
@@ -765,8 +787,6 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> norm8_cuda(const at::Tensor& x_, 
     a.stride_x = x.stride(0);
     a.weight = weight.data_ptr();
     if (present(residual_)) {
-        NormInputs::same_kind(*residual_, x_, what);
-        TORCH_CHECK_VALUE(residual_->sizes() == x_.sizes(), what, ": residual must have x's shape");
         residual = unit_rows(*residual_, a.rows);
         a.residual = residual.data_ptr();
         a.stride_residual = residual.stride(0);
@@ -776,8 +796,6 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> norm8_cuda(const at::Tensor& x_, 
     }
     at::Tensor q = fresh(x_.sizes(), dtype, x_);
     std::vector<int64_t> shape = lead_shape(x_, false);
-    TORCH_CHECK_VALUE(group >= 0 && (group == 0 || a.width % group == 0), what, ": width ", a.width,
-                      " is not whole groups of ", group);
     shape.push_back(group ? a.width / group : 1);
     at::Tensor scale = fresh(shape, at::kFloat, x_);
     check(api().norm8(&a, q.data_ptr(), scale.data_ptr<float>(), a.residual ? y.data_ptr() : nullptr, stream_of(x_)),
@@ -785,39 +803,75 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> norm8_cuda(const at::Tensor& x_, 
     return {q, scale, y};
 }
 
+// A tensor beside the logits: of one of the types, with a row (dims 2) or a value (dims 1) for each of theirs.
+void check_beside(const OptTensor& t, const char* name, int64_t dims, std::initializer_list<at::ScalarType> dtypes,
+                  const at::Tensor& logits, const char* what) {
+    if (!present(t)) return;
+    check_strided(*t, what);
+    TORCH_CHECK_TYPE(std::find(dtypes.begin(), dtypes.end(), t->scalar_type()) != dtypes.end(), what, ": ", name, " must be ",
+                     *dtypes.begin(), dtypes.size() > 1 ? " or int64" : "", ", got ", t->scalar_type());
+    TORCH_CHECK_VALUE(t->device() == logits.device() && t->dim() == dims && t->sym_size(0) == logits.sym_size(0), what, ": ",
+                      name, dims == 1 ? " must be [rows]" : " must be [rows, ...]", " on the device of logits");
+}
+
+// What penalize_logits asks of its tensors, symbolic sizes too.
+void check_logits(const at::Tensor& logits, const OptTensor& tokens, const OptTensor& token_lens,
+                  const OptTensor& prompt_lens, const OptTensor& repetition, const OptTensor& presence,
+                  const OptTensor& frequency, const OptTensor& bias_index, const OptTensor& bias_value,
+                  const OptTensor& allowed, const OptTensor& temperature, const char* what) {
+    check_strided(logits, what);
+    dtype_code(logits);
+    TORCH_CHECK_VALUE(logits.dim() == 2 && logits.sym_size(1) >= 1, what, ": logits must be [rows, vocab]");
+    const auto beside = [&](const OptTensor& t, const char* name, int64_t dims, std::initializer_list<at::ScalarType> dtypes) {
+        check_beside(t, name, dims, dtypes, logits, what);
+    };
+    beside(tokens, "tokens", 2, {at::kInt, at::kLong});
+    beside(token_lens, "token_lens", 1, {at::kInt});
+    beside(prompt_lens, "prompt_lens", 1, {at::kInt});
+    beside(repetition, "repetition", 1, {at::kFloat});
+    beside(presence, "presence", 1, {at::kFloat});
+    beside(frequency, "frequency", 1, {at::kFloat});
+    beside(temperature, "temperature", 1, {at::kFloat});
+    beside(bias_index, "bias_index", 2, {at::kInt, at::kLong});
+    beside(bias_value, "bias_value", 2, {at::kFloat});
+    beside(allowed, "allowed", 2, {at::kInt});
+    TORCH_CHECK_VALUE(present(tokens) || !(present(token_lens) || present(prompt_lens) || present(repetition) ||
+                                           present(presence) || present(frequency)),
+                      what, ": lengths or penalties without tokens");
+    TORCH_CHECK_VALUE(present(bias_index) == present(bias_value), what, ": bias_index and bias_value go together");
+    if (present(bias_index)) {
+        TORCH_CHECK_VALUE(bias_index->sym_sizes() == bias_value->sym_sizes(), what, ": the shapes of the biases differ");
+        TORCH_CHECK_NOT_IMPLEMENTED(bias_index->sym_size(1) <= 1024, what, ": ", bias_index->sym_size(1),
+                                    " biases per row exceed 1024");
+    }
+    if (present(allowed)) {
+        const c10::SymInt words = (logits.sym_size(1) + 31) / 32;
+        TORCH_CHECK_VALUE(allowed->sym_size(1) == words, what, ": allowed must hold ", words, " words a row, got ",
+                          allowed->sym_size(1));
+    }
+}
+
 // The descriptor of the logits' inputs and the tensors whose memory it names.
 struct LogitsInputs {
     nb200_logits_args a = {};
     std::vector<at::Tensor> keep;
-    const at::Tensor& x;
-    const char* what;
-    // A tensor per row of the logits: [rows, columns] of the given type, or null.
-    const void* rows_of(const OptTensor& t, const char* name, int64_t* columns, int64_t* stride) {
+    // A tensor with a row for each of the logits', or null.
+    const void* rows_of(const OptTensor& t, int64_t* columns, int64_t* stride) {
         if (!present(t)) return nullptr;
-        check_strided(*t, what);
-        TORCH_CHECK_VALUE(t->device() == x.device() && t->dim() == 2 && t->size(0) == a.rows, what, ": ", name,
-                          " must be [rows, ...] on the device of logits");
         keep.push_back(unit_rows(*t, a.rows));
         *columns = t->size(1);
         *stride = keep.back().stride(0);
         return keep.back().data_ptr();
     }
     template <typename T>
-    const T* per_row(const OptTensor& t, const char* name, at::ScalarType dtype) {
+    const T* per_row(const OptTensor& t) {
         if (!present(t)) return nullptr;
-        check_strided(*t, what);
-        TORCH_CHECK_TYPE(t->scalar_type() == dtype, what, ": ", name, " must be ", dtype);
-        TORCH_CHECK_VALUE(t->device() == x.device() && t->dim() == 1 && t->size(0) == a.rows, what, ": ", name,
-                          " must be [rows] on the device of logits");
         if (t->is_contiguous()) return t->data_ptr<T>();
         keep.push_back(t->contiguous());
         return keep.back().data_ptr<T>();
     }
-    LogitsInputs(const at::Tensor& logits, const char* w) : x(logits), what(w) {
-        check_strided(x, what);
-        check_cuda(x, what);
+    explicit LogitsInputs(const at::Tensor& x) {
         a.dtype = dtype_code(x);
-        TORCH_CHECK_VALUE(x.dim() == 2 && x.size(1) >= 1, what, ": logits must be [rows, vocab]");
         a.rows = x.size(0);
         a.vocab = x.size(1);
         keep.reserve(16);
@@ -829,36 +883,26 @@ at::Tensor penalize_logits_cuda(const at::Tensor& logits, const OptTensor& token
                                 const OptTensor& frequency, const OptTensor& bias_index, const OptTensor& bias_value,
                                 const OptTensor& allowed, const OptTensor& temperature) {
     const char* what = "nb200.penalize_logits";
-    LogitsInputs in(logits, what);
+    check_cuda(logits, what);
+    check_logits(logits, tokens, token_lens, prompt_lens, repetition, presence, frequency, bias_index, bias_value, allowed,
+                 temperature, what);
+    LogitsInputs in(logits);
     nb200_logits_args& a = in.a;
     c10::cuda::CUDAGuard guard(logits.device());
     int64_t columns = 0;
-    a.logits = in.rows_of(logits, "logits", &columns, &a.stride_logits);
+    a.logits = in.rows_of(logits, &columns, &a.stride_logits);
     if (present(tokens)) a.token_dtype = index_code(*tokens);
-    a.tokens = in.rows_of(tokens, "tokens", &a.history, &a.stride_tokens);
-    a.token_lens = in.per_row<int32_t>(token_lens, "token_lens", at::kInt);
-    a.prompt_lens = in.per_row<int32_t>(prompt_lens, "prompt_lens", at::kInt);
-    a.repetition = in.per_row<float>(repetition, "repetition", at::kFloat);
-    a.presence = in.per_row<float>(presence, "presence", at::kFloat);
-    a.frequency = in.per_row<float>(frequency, "frequency", at::kFloat);
-    a.temperature = in.per_row<float>(temperature, "temperature", at::kFloat);
-    TORCH_CHECK_VALUE(present(tokens) || !(present(token_lens) || present(prompt_lens) || present(repetition) ||
-                                           present(presence) || present(frequency)),
-                      what, ": lengths or penalties without tokens");
-    TORCH_CHECK_VALUE(present(bias_index) == present(bias_value), what, ": bias_index and bias_value go together");
-    if (present(bias_index)) {
-        a.bias_dtype = index_code(*bias_index);
-        TORCH_CHECK_TYPE(bias_value->scalar_type() == at::kFloat, what, ": bias_value must be float32");
-        TORCH_CHECK_VALUE(bias_index->sizes() == bias_value->sizes(), what, ": the shapes of the biases differ");
-        a.bias_index = in.rows_of(bias_index, "bias_index", &a.biases, &a.stride_bias_index);
-        a.bias_value = static_cast<const float*>(in.rows_of(bias_value, "bias_value", &columns, &a.stride_bias_value));
-    }
-    if (present(allowed)) {
-        TORCH_CHECK_TYPE(allowed->scalar_type() == at::kInt, what, ": allowed must be int32");
-        a.allowed = static_cast<const int32_t*>(in.rows_of(allowed, "allowed", &columns, &a.stride_allowed));
-        TORCH_CHECK_VALUE(columns == (a.vocab + 31) / 32, what, ": allowed must hold ", (a.vocab + 31) / 32,
-                          " words a row, got ", columns);
-    }
+    a.tokens = in.rows_of(tokens, &a.history, &a.stride_tokens);
+    a.token_lens = in.per_row<int32_t>(token_lens);
+    a.prompt_lens = in.per_row<int32_t>(prompt_lens);
+    a.repetition = in.per_row<float>(repetition);
+    a.presence = in.per_row<float>(presence);
+    a.frequency = in.per_row<float>(frequency);
+    a.temperature = in.per_row<float>(temperature);
+    if (present(bias_index)) a.bias_dtype = index_code(*bias_index);
+    a.bias_index = in.rows_of(bias_index, &a.biases, &a.stride_bias_index);
+    a.bias_value = static_cast<const float*>(in.rows_of(bias_value, &columns, &a.stride_bias_value));
+    a.allowed = static_cast<const int32_t*>(in.rows_of(allowed, &columns, &a.stride_allowed));
     at::Tensor out = fresh(logits.sizes(), logits.scalar_type(), logits);
     const int64_t bytes = api().penalize_logits_work_bytes(&a);
     if (bytes < 0) check((int)bytes, what);
@@ -946,26 +990,30 @@ at::Tensor distill_loss_bwd_meta(const at::Tensor&, const at::Tensor& x, const a
 }
 std::tuple<at::Tensor, at::Tensor> prefix_attention_meta(const at::Tensor& q, const at::Tensor& pk,
                                                          const at::Tensor& pv, const at::Tensor& k,
-                                                         const at::Tensor& v, const OptTensor& seq_lens, double,
+                                                         const at::Tensor& v, const OptTensor& seq_lens, double scale,
                                                          bool with_lse) {
-    check_prefix_attention(q, pk, pv, k, v, seq_lens, "nb200.prefix_attention");
+    check_prefix_attention(q, pk, pv, k, v, seq_lens, scale, "nb200.prefix_attention");
     const auto qs = q.sym_sizes();
     const auto f32 = q.options().dtype(at::kFloat);
     return {at::empty_symint(qs, q.options()),
             with_lse ? at::empty_symint(std::vector<c10::SymInt>(qs.begin(), qs.end() - 1), f32) : at::empty({0}, f32)};
 }
-std::tuple<at::Tensor, at::Tensor, at::Tensor> norm8_meta(const at::Tensor& x, const at::Tensor&,
+std::tuple<at::Tensor, at::Tensor, at::Tensor> norm8_meta(const at::Tensor& x, const at::Tensor& weight,
                                                           const OptTensor& residual, int64_t group, int64_t kind,
-                                                          double) {
+                                                          double eps) {
+    check_norm8(x, weight, residual, group, eps, "nb200.norm8");
     std::vector<c10::SymInt> shape = lead_sym_shape(x, false);
     shape.emplace_back(group > 0 ? x.sym_size(-1) / group : c10::SymInt(1));
     return {at::empty_symint(x.sym_sizes(), x.options().dtype(byte_dtype(kind, "nb200.norm8"))),
             at::empty_symint(shape, x.options().dtype(at::kFloat)),
             present(residual) ? like_meta(x) : none_like(x)};
 }
-at::Tensor penalize_logits_meta(const at::Tensor& logits, const OptTensor&, const OptTensor&, const OptTensor&,
-                                const OptTensor&, const OptTensor&, const OptTensor&, const OptTensor&,
-                                const OptTensor&, const OptTensor&, const OptTensor&) {
+at::Tensor penalize_logits_meta(const at::Tensor& logits, const OptTensor& tokens, const OptTensor& token_lens,
+                                const OptTensor& prompt_lens, const OptTensor& repetition, const OptTensor& presence,
+                                const OptTensor& frequency, const OptTensor& bias_index, const OptTensor& bias_value,
+                                const OptTensor& allowed, const OptTensor& temperature) {
+    check_logits(logits, tokens, token_lens, prompt_lens, repetition, presence, frequency, bias_index, bias_value, allowed,
+                 temperature, "nb200.penalize_logits");
     return like_meta(logits);
 }
 
