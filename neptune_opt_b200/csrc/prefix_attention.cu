@@ -4,8 +4,9 @@
 //   o = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale q k_j),   j over the prefix and the sequence's own
 //                                                              tokens up to the query's own position
 //
-// The keys are cut into parts. A part's result for a query row is the pair (o, log2 sum) over its keys
-// alone, and pairs merge exactly: with w_i = 2^(l_i - max l), o = sum w_i o_i / sum w_i. So the prefix is
+// The keys are cut into parts. A part's result for a query row is its output o over its keys alone, their maximum score m
+// and the sum l behind it, and parts merge exactly: with w_i = l_i exp(scale (m_i - max m)), o = sum w_i o_i / sum w_i. (The
+// pair, not m + log l: beside a maximum far from 0 the logarithm would be rounded away.) So the prefix is
 // read once for the query rows of all sequences, whatever their number, each own cache once for its
 // sequence, and long key ranges are split until the GPU is full; one pass over the pairs joins them, in a
 // fixed order.
@@ -38,8 +39,9 @@ struct StreamArgs : Line {
     Query query;
     int rows;       // query rows of a key/value head over all sequences
     int slot_rows;
-    float sl2;      // scale * log2(e)
-    float *o, *lse; // [slots][slot_rows][D], [slots][slot_rows]
+    float scale, sl2, slack;  // sl2 = scale * log2(e); kSlack in scores
+    float* o;       // [slots][slot_rows][D]
+    float2* ml;     // [slots][slot_rows]
     int2* span;     // [units]: first and last worker
     bool beside;    // runs beside the kernel ahead of it, of which it needs nothing
 };
@@ -119,7 +121,7 @@ __device__ __forceinline__ Cursor piece_of(const StreamArgs& a, int worker, int 
     return c;
 }
 
-// What a worker keeps of a unit's query rows, its running maximum (log2 domain), sum and output, and what a step of 16
+// What a worker keeps of a unit's query rows, its running maximum, sum and output, and what a step of 16
 // keys does to it. Column tile n of a lane's accumulators: query rows 8 n + 2 (lane % 4) and the next one.
 template <typename T, int D, int NT>
 struct Rows {
@@ -138,7 +140,7 @@ struct Rows {
     }
     // Keys kb on, of a box at ks and vs in shared memory; `limit`: the last key a row sees, `lowest`: the least of them.
     __device__ __forceinline__ void step(const uint32_t (*qf)[D / 16][2], uint32_t ks, uint32_t vs, int kb,
-                                         const int (*limit)[2], int lowest, float sl2, int lane) {
+                                         const int (*limit)[2], int lowest, float sl2, float slack, int lane) {
         constexpr uint32_t kBox = kStepKeys * 128;
         // This lane's address in a box: the row it loads for ldmatrix, and the swizzle of its 16-byte pieces.
         const int k_row = lane & 15, k_piece = lane >> 4;                         // K: keys 0-15, then 8 columns on
@@ -167,17 +169,17 @@ struct Rows {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) grow |= fmaxf(s[n][e], s[n][e + 2]) * sl2 > m[n][e] + kSlack;
+            for (int e = 0; e < 2; ++e) grow |= fmaxf(s[n][e], s[n][e + 2]) > m[n][e] + slack;
         if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    float top = fmaxf(s[n][e], s[n][e + 2]) * sl2;
+                    float top = fmaxf(s[n][e], s[n][e + 2]);
 #pragma unroll
                     for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
                     const float next = fmaxf(m[n][e], top);
-                    const float f = next == m[n][e] ? 1.f : ex2(m[n][e] - next);
+                    const float f = next == m[n][e] ? 1.f : ex2((m[n][e] - next) * sl2);
                     m[n][e] = next;
                     l[n][e] *= f;
 #pragma unroll
@@ -190,9 +192,9 @@ struct Rows {
             float x[4];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const float ref = (m[n][e] == -NB200_INF ? 0.f : m[n][e]) - kLift<T>;
-                x[e] = ex2(fmaf(s[n][e], sl2, -ref));
-                x[e + 2] = ex2(fmaf(s[n][e + 2], sl2, -ref));
+                const float top = m[n][e] == -NB200_INF ? 0.f : m[n][e];
+                x[e] = ex2(fmaf(s[n][e] - top, sl2, kLift<T>));
+                x[e + 2] = ex2(fmaf(s[n][e + 2] - top, sl2, kLift<T>));
                 l[n][e] += x[e] + x[e + 2];
             }
             p[n][0] = transpose8(Elem<T>::pack_word(x[0], x[1]));
@@ -344,7 +346,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, NT>)
         const int kb = use.step * kStepKeys;
         // What a cache holds behind a sequence must not reach the products: 0 times an infinity is none.
         if (use.batch >= 0) zero_behind<D>(vs, use.keys - kb, lane);
-        t.step(qf, ks, vs, kb, limit, lowest, a.sl2, lane);
+        t.step(qf, ks, vs, kb, limit, lowest, a.sl2, a.slack, lane);
 
         ++done;
         if (++stage == kStages) stage = 0, phase ^= 1u;
@@ -372,7 +374,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, NT>)
                         dst[16 * d] = t.o[n][d][e] * inv;
                         dst[16 * d + 8] = t.o[n][d][e + 2] * inv;
                     }
-                    if (lane < 4) a.lse[slot + in] = t.l[n][e] == 0.f ? -NB200_INF : t.m[n][e] + log2f(t.l[n][e]) - kLift<T>;
+                    if (lane < 4) a.ml[slot + in] = make_float2(t.m[n][e], t.l[n][e]);
                 }
             }
         if (lane == 0 && ends) a.span[unit].y = worker;
@@ -394,7 +396,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, NT>)
         for (int i = done; i < sent; ++i) drain_bar(&full[warp][i % kStages], (i / kStages) & 1u);
         for (;;) {
             const int unit = use.unit(a);
-            for (int in = lane; in < a.slot_rows; in += 32) a.lse[((int64_t)worker + unit) * a.slot_rows + in] = NB200_NAN;
+            for (int in = lane; in < a.slot_rows; in += 32) a.ml[((int64_t)worker + unit) * a.slot_rows + in] = make_float2(NB200_NAN, NB200_NAN);
             if (lane == 0 && use.ends_unit()) a.span[unit].y = worker;
             if (!use.skip_unit(a)) break;
             if (lane == 0) a.span[use.unit(a)].x = worker;
@@ -484,11 +486,11 @@ __global__ void __launch_bounds__(W * 32, D == 64 || W == 4 ? 2 : 1)
             int last[NT][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n) last[n][0] = last[n][1] = a.prefix - 1;
-            t.step(qf, ks, vs, i * kStepKeys, last, a.prefix - 1, a.sl2, lane);
+            t.step(qf, ks, vs, i * kStepKeys, last, a.prefix - 1, a.sl2, a.slack, lane);
         } else {
             const int kb = (i - shared_steps) * kStepKeys;
             zero_behind<D>(vs, own - kb, lane);
-            t.step(qf, ks, vs, kb, limit, own - tokens, a.sl2, lane);
+            t.step(qf, ks, vs, kb, limit, own - tokens, a.sl2, a.slack, lane);
         }
         if (++stage == kStages) stage = 0, phase ^= 1u;
     }
@@ -523,7 +525,7 @@ __global__ void __launch_bounds__(W * 32, D == 64 || W == 4 ? 2 : 1)
 #pragma unroll
             for (int w = 0; w < W; ++w) {
                 const float l = sh_l[w][in], m = sh_m[w][in];
-                const float f = m == -NB200_INF ? l : ex2(m - top);  // without a score but -inf the sum is 0, or NaN
+                const float f = weight_of(m, l, top, a.sl2);
                 sum += f * l;
                 const float* o = static_cast<const float*>(__cvta_shared_to_generic(all_stages + w * (kStages * 2 * kTile))) +
                                  in * kPitch + lane * E;
@@ -537,13 +539,14 @@ __global__ void __launch_bounds__(W * 32, D == 64 || W == 4 ? 2 : 1)
 #pragma unroll
         for (int e = 0; e < E; e += 2) dst[e / 2] = Elem<T>::pack_word(v[e] * inv, v[e + 1] * inv);
         if (out_lse && lane == 0)
-            out_lse[at] = sum == 0.f ? -NB200_INF : (top + log2f(sum) - kLift<T>) * 0.69314718055994531f;
+            out_lse[at] = natural_lse<T>(top, sum, a.scale);
     }
 }
 
 struct JoinArgs {
-    const float *tensor_o, *tensor_lse;  // parts of the tensor cores: [splits][kv_heads][rows][D], and without D
-    const float *o, *lse;                // slots of the stream kernel
+    const float *tensor_o, *o;           // parts of the tensor cores, [splits][kv_heads][rows][D]; slots of the stream kernel
+    const float2 *tensor_ml, *ml;        // the same without D
+    float scale, sl2;
     const int2* span;
     int workers;                         // of the stream kernel
     void* out;                           // [batch, heads, tokens, D]
@@ -579,7 +582,8 @@ __global__ void __launch_bounds__(256) join_kernel(const JoinArgs a) {
     for (int e = 0; e < E; ++e) v[e] = 0.f;
     if (len - a.tokens + t >= 0) {
         // Two runs of parts: rows `far + i far_step` of one array, `near + i slot_rows` of another.
-        const float *far_o = a.o, *far_lse = a.lse;
+        const float* far_o = a.o;
+        const float2* far_ml = a.ml;
         int64_t far = 0, far_step = a.slot_rows;
         int nfar = 0;
         const int in = r - b * a.group * a.tokens;
@@ -587,7 +591,7 @@ __global__ void __launch_bounds__(256) join_kernel(const JoinArgs a) {
         const int2 w = a.span[unit];
         bool known = are_workers(w.x, w.y, a.workers);
         if (a.splits) {
-            far_o = a.tensor_o, far_lse = a.tensor_lse, far = id, far_step = all, nfar = a.splits;
+            far_o = a.tensor_o, far_ml = a.tensor_ml, far = id, far_step = all, nfar = a.splits;
         } else if (a.prefix_tiles) {
             const int shared = head * a.prefix_tiles + r / a.tile_rows;
             const int2 u = a.span[shared];
@@ -601,7 +605,7 @@ __global__ void __launch_bounds__(256) join_kernel(const JoinArgs a) {
         const int parts = known ? nfar + w.y - w.x + 1 : 0;
         if (!known) sum = NB200_NAN;
         auto row_of = [&](int i) { return i < nfar ? far + i * far_step : near + (int64_t)(i - nfar) * a.slot_rows; };
-        auto lse_of = [&](int i) { return i < parts ? (i < nfar ? far_lse : a.lse)[row_of(i)] : -NB200_INF; };
+        auto ml_of = [&](int i) { return i < parts ? (i < nfar ? far_ml : a.ml)[row_of(i)] : make_float2(-NB200_INF, 0.f); };
         // Four o's in flight at a time, the first four before their weights are known.
         float o[4][E];
         auto load4 = [&](int i) {
@@ -615,11 +619,11 @@ __global__ void __launch_bounds__(256) join_kernel(const JoinArgs a) {
         };
         const int start = WIDE ? warp : 0;
         if (known) load4(start);
-        for (int i = lane; i < parts; i += 32) top = fmaxf(top, lse_of(i));
+        for (int i = lane; i < parts; i += 32) top = fmaxf(top, ml_of(i).x);
         top = warp_max(top);
         for (int i0 = start; i0 < parts; i0 += 32 * kTurns) {  // 32 parts, weighed by the 32 lanes
-            const float x = lse_of(i0 + lane * kTurns);
-            const float mine = x == -NB200_INF ? 0.f : ex2(x - top);  // NaN stays
+            const float2 ml = ml_of(i0 + lane * kTurns);
+            const float mine = ml.y * weight_of(ml.x, ml.y, top, a.sl2);
             sum += mine;
             for (int i = 0; i < 32 && i0 + i * kTurns < parts; i += 4) {
                 if (i0 + i > start) load4(i0 + i * kTurns);
@@ -656,7 +660,7 @@ __global__ void __launch_bounds__(256) join_kernel(const JoinArgs a) {
     uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + at * D) + lane * (E / 2);
 #pragma unroll
     for (int e = 0; e < E / 2; ++e) out[e] = w[e];
-    if (a.out_lse && lane == 0) a.out_lse[at] = sum == 0.f ? -NB200_INF : (top + log2f(sum)) * 0.69314718055994531f;
+    if (a.out_lse && lane == 0) a.out_lse[at] = natural_lse<T>(top, sum, a.scale);
 }
 
 // ------------------------------------------------------------------ host side
@@ -673,7 +677,7 @@ struct Plan {
     int64_t prefix_tiles, own_tiles, slot_rows, units, ctas;
     int64_t most_parts;            // parts of a row, at most
     // Workspace, in bytes from its start.
-    int64_t tensor_o, tensor_lse, o, lse, span, bytes;
+    int64_t tensor_o, tensor_ml, o, ml, span, bytes;
 };
 
 Plan plan_of(const nb200_prefix_attn_args& a) {
@@ -728,8 +732,8 @@ Plan plan_of(const nb200_prefix_attn_args& a) {
     const int64_t slots = p.units + p.ctas * kWarps;
     p.tensor_o = take(p.splits * a.kv_heads * p.rows * a.head_dim);
     p.o = take(slots * p.slot_rows * a.head_dim);
-    p.tensor_lse = take(p.splits * a.kv_heads * p.rows);
-    p.lse = take(slots * p.slot_rows);
+    p.tensor_ml = take(2 * p.splits * a.kv_heads * p.rows);
+    p.ml = take(2 * slots * p.slot_rows);
     p.span = take(2 * p.units);
     return p;
 }
@@ -770,11 +774,13 @@ int launch_all(const nb200_prefix_attn_args& n, const nb200_attn_strides* s, con
         return NB200_ERR_CAPACITY;
     }
     auto at = [&](int64_t offset) { return reinterpret_cast<float*>(work + offset); };
+    auto pairs_at = [&](int64_t offset) { return reinterpret_cast<float2*>(work + offset); };
     const Query query = {q, s[0].batch, s[0].head, s[0].seq, (int)(n.heads / n.kv_heads), (int)n.tokens};
     const float sl2 = n.scale * 1.4426950408889634f;
     int rc;
     if (p.splits) {
-        const TensorPart t = {query, (int)n.kv_heads, (int)p.rows, (int)n.prefix, p.splits, sl2, at(p.tensor_o), at(p.tensor_lse)};
+        const TensorPart t = {query, (int)n.kv_heads, (int)p.rows, (int)n.prefix, p.splits, sl2, slack_of(sl2),
+                              at(p.tensor_o), pairs_at(p.tensor_ml)};
         if ((rc = launch_tensor_part(t, n.dtype, n.head_dim, pk, s[1], pv, s[2], st))) return rc;
     }
     StreamArgs a = {};
@@ -792,7 +798,7 @@ int launch_all(const nb200_prefix_attn_args& n, const nb200_attn_strides* s, con
     a.prefix = p.prefix_tiles || p.solo ? (int)n.prefix : 0, a.cache = (int)n.cache;
     a.rows = (int)p.rows, a.prefix_tiles = (int)p.prefix_tiles, a.own_tiles = (int)p.own_tiles;
     a.slot_rows = (int)p.slot_rows;
-    a.sl2 = sl2;
+    a.scale = n.scale, a.sl2 = sl2, a.slack = slack_of(sl2);
     if (p.solo) {
         // Where there are more CTAs than SMs, two an SM: one starts while the other reads. Head dimension 128 has room for
         // them with four warps each.
@@ -802,14 +808,15 @@ int launch_all(const nb200_prefix_attn_args& n, const nb200_attn_strides* s, con
         return p.nt == 1 ? launch_solo<T, D, 1, 8>(maps, a, o, lse, limits[5], st)
                          : launch_solo<T, D, 2, 8>(maps, a, o, lse, limits[6], st);
     }
-    a.o = at(p.o), a.lse = at(p.lse), a.span = reinterpret_cast<int2*>(at(p.span));
+    a.o = at(p.o), a.ml = pairs_at(p.ml), a.span = reinterpret_cast<int2*>(at(p.span));
     a.beside = p.splits > 0;  // the tensor cores' kernel started after all that came before
     rc = p.nt == 1   ? launch_stream<T, D, 1>(maps, a, p.ctas, limits[0], st)
          : p.nt == 2 ? launch_stream<T, D, 2>(maps, a, p.ctas, limits[1], st)
                      : launch_stream<T, D, 4>(maps, a, p.ctas, limits[2], st);
     if (rc) return rc;
     JoinArgs j = {};
-    j.tensor_o = at(p.tensor_o), j.tensor_lse = at(p.tensor_lse), j.o = a.o, j.lse = a.lse, j.span = a.span;
+    j.tensor_o = at(p.tensor_o), j.tensor_ml = pairs_at(p.tensor_ml), j.o = a.o, j.ml = a.ml, j.span = a.span;
+    j.scale = a.scale, j.sl2 = a.sl2;
     j.workers = (int)p.ctas * kWarps;
     j.out = o, j.out_lse = lse, j.lens = n.seq_lens;
     j.kv_heads = a.kv_heads, j.group = query.group, j.tokens = query.tokens, j.rows = a.rows, j.cache = a.cache;

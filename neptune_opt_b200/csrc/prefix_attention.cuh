@@ -4,9 +4,11 @@
 
 #include <cuda.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "common.cuh"
+#include "fastmath.cuh"
 #include "launch.h"
 
 namespace nb200 {
@@ -24,15 +26,32 @@ struct Query {
 constexpr float kSlack = 8.f;
 template <typename T> constexpr float kLift = std::is_same<T, __half>::value ? 6.f : 0.f;
 
+// A running maximum m is kept as the score it is, before scale and log2(e), and subtracted before they come in, 2^((s - m) sl2):
+// so no finite score leaves fp32 on the way, and scores that are all alike weigh alike however far from 0 they are. (As
+// 2^(s sl2 - m sl2) in one multiply-add, the rounding of m sl2 was left over: scores of -1e19 came out as NaN, or as no weight.)
+// 2^(m sl2 - top sl2): what a sum behind maximum m weighs beside one behind `top`. Without a score but -inf the sum l is 0, or
+// NaN, and weighs that.
+__device__ __forceinline__ float weight_of(float m, float l, float top, float sl2) {
+    return m == -NB200_INF ? l : ex2((m - top) * sl2);
+}
+// The natural log-sum-exp of a row.
+template <typename T>
+__device__ __forceinline__ float natural_lse(float m, float l, float scale) {
+    return l == 0.f ? -NB200_INF : fmaf(m, scale, (log2f(l) - kLift<T>) * 0.69314718055994531f);
+}
+
 // The prefix on the tensor cores (prefix_attention_tc.cu): query rows of a key/value head in blocks of 256, the
 // prefix's tiles of 128 keys in `splits` nearly equal ranges. Results as of any part: o [splits][kv_heads][rows][D],
-// lse [splits][kv_heads][rows].
+// ml [splits][kv_heads][rows].
 struct TensorPart {
     Query query;
     int kv_heads, rows, keys, splits;
-    float sl2;
-    float *o, *lse;
+    float sl2, slack;  // scale * log2(e), and kSlack in scores
+    float* o;
+    float2* ml;
 };
+// kSlack as a difference of scores; where scores count for next to nothing, still one that can be added to them.
+inline float slack_of(float sl2) { return std::min(kSlack / sl2, 1e30f); }
 // [batch, heads, keys, D] as a tensor map with a {64, box_keys} box and 128-byte swizzle. The stride of a dimension of one
 // element is never used and may be anything.
 int encode_keys(CUtensorMap* map, const char* what, const void* base, int dtype, int64_t d, int64_t keys, int64_t heads,

@@ -1,5 +1,5 @@
 // The shared prefix on the tensor cores: softmax(scale Q K^T) V of many query rows against a range of the
-// prefix's keys, with the range's log2 sum (one part of prefix_attention.cu).
+// prefix's keys, with the range's maximum and sum (one part of prefix_attention.cu).
 //
 // One CTA owns up to 256 query rows of one key/value head, gathered from all sequences, and a range of 128-key
 // tiles. Two softmax warpgroups each own a stream: a 128-row query tile with its scores and output in tensor
@@ -9,7 +9,7 @@
 //
 //   warp 9      producer: K and V tiles through a ring of stages (TMA), in the order in which they are used
 //   warp 8      MMA: S_t = Q K^T (shared x shared -> TMEM, fp32), O_t += P_t V (P from TMEM, V from shared)
-//   warps 0-7   softmax of stream t = warp / 4: scores, running maximum (log2 domain), rescale O_t when the
+//   warps 0-7   softmax of stream t = warp / 4: scores, running maximum, rescale O_t when the
 //               maximum grew by more than 2^8, P_t in the inputs' type into the upper half of S_t's columns
 //
 // TMEM (512 columns x 128 lanes): S_0 [0, 128), S_1 [128, 256), O_0 [256, 256 + D), O_1 [384, 384 + D).
@@ -215,15 +215,24 @@ __device__ __forceinline__ void mma_issuer(uint8_t* smem, Bars* b, uint32_t tmem
     drain_bar(&b->o_final, 0);
 }
 
-// Half qp of P for this row: p = 2^(s sl2 - m), rounded into TMEM, its fp32 value added to the row sums.
-template <typename T>
-__device__ __forceinline__ void p_half(const float* s, int qp, uint64_t sl2, uint64_t nm, uint64_t& acc0, uint64_t& acc1,
-                                       uint32_t tP) {
+// While |m sl2| is at most kFar the exponent takes one multiply-add here, 2^(s sl2 - m sl2), of which the rounding of m sl2 takes 2^-16 at
+// most; a warp with a row that is farther from 0 subtracts first. (Subtracting always spills, and takes 80 us for 77 over 16384
+// keys and 1024 rows a head.)
+constexpr float kFar = 256.f;
+__device__ __forceinline__ bool is_far(float m, float sl2) { return m != -NB200_INF && fabsf(m * sl2) > kFar; }
+
+// Half qp of P for this row: p = 2^(s sl2 + nm), FAR: 2^((s - m) sl2 + nm), rounded into TMEM, its fp32 value added to the
+// row sums.
+template <typename T, bool FAR>
+__device__ __forceinline__ void p_half(const float* s, int qp, uint64_t minus_m, uint64_t sl2, uint64_t nm, uint64_t& acc0,
+                                       uint64_t& acc1, uint32_t tP) {
     uint32_t pk[32];
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
         const int pi = 32 * qp + i;
-        const uint64_t x = fma2(f2(s[2 * pi], s[2 * pi + 1]), sl2, nm);
+        uint64_t x = f2(s[2 * pi], s[2 * pi + 1]);
+        if constexpr (FAR) x = add2(x, minus_m);
+        x = fma2(x, sl2, nm);
         const uint64_t p = f2(ex2_ftz(f2lo(x)), ex2_ftz(f2hi(x)));
         if (i & 1) acc1 = add2(acc1, p);
         else acc0 = add2(acc0, p);
@@ -244,8 +253,8 @@ __device__ __forceinline__ void softmax_stream(uint8_t* smem, Bars* b, uint32_t 
     const uint32_t tS = tmem + lanes + kColS + 128 * t, tP = tS + kColP, tO = tmem + lanes + kColO + 128 * t;
     const float sl2 = a.sl2;
     const int n = u.tiles_of(t);
-    float m = -NB200_INF, l = 0.f;
-    bool ok = true;
+    float m = -NB200_INF, l = 0.f, add = kLift<T>;  // add: what the exponent gets beside s sl2
+    bool ok = true, far = false;  // far: a maximum of the warp is
     for (int i = 0; i < n; ++i) {
         // All lanes take the same branch: the TMEM accesses below are warp-collective.
         if (!(ok = __all_sync(0xffffffffu, wait_bar(&b->s_full[t], i & 1u, abort)))) break;
@@ -271,10 +280,10 @@ __device__ __forceinline__ void softmax_stream(uint8_t* smem, Bars* b, uint32_t 
         }
         a0 = max3(a0, s[124], s[125]);
         a1 = max3(a1, s[126], s[127]);
-        const float mnew = fmaxf(m, fmaxf(max3(a0, a1, a2), a3) * sl2);
-        if (__any_sync(0xffffffffu, mnew > m + kSlack)) {
+        const float mnew = fmaxf(m, fmaxf(max3(a0, a1, a2), a3));
+        if (__any_sync(0xffffffffu, mnew > m + a.slack)) {
             // Move the whole warp to the new maxima; rows whose maximum did not move keep factor 1.
-            const float f = mnew == m ? 1.f : ex2(m - mnew);
+            const float f = mnew == m ? 1.f : ex2((m - mnew) * sl2);
             if (i > 0) {
 #pragma unroll
                 for (int c = 0; c < D / 32; ++c) {
@@ -287,18 +296,25 @@ __device__ __forceinline__ void softmax_stream(uint8_t* smem, Bars* b, uint32_t 
             }
             l *= f;
             m = mnew;
+            add = kLift<T> - (m == -NB200_INF ? 0.f : m * sl2);  // no score but -inf so far: all p are 0
+            far = __any_sync(0xffffffffu, is_far(m, sl2));
         }
-        const float ref = (m == -NB200_INF ? 0.f : m) - kLift<T>;  // no score but -inf so far: all p are 0
-        const uint64_t sl2x2 = f2(sl2, sl2), nm = f2(-ref, -ref);
+        const uint64_t sl2x2 = f2(sl2, sl2);
         uint64_t acc0 = 0, acc1 = 0;
+        auto probabilities = [&](auto is) {
+            constexpr bool FAR = decltype(is)::value;
+            const float top = m == -NB200_INF ? 0.f : m, x = FAR ? kLift<T> : add;
 #pragma unroll
-        for (int qp = 0; qp < 2; ++qp) {
-            p_half<T>(s, qp, sl2x2, nm, acc0, acc1, tP);
-            tc::tmem_wait_st();
-            tc::fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&b->p_full[t][qp]);
-        }
+            for (int qp = 0; qp < 2; ++qp) {
+                p_half<T, FAR>(s, qp, f2(-top, -top), sl2x2, f2(x, x), acc0, acc1, tP);
+                tc::tmem_wait_st();
+                tc::fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&b->p_full[t][qp]);
+            }
+        };
+        if (__builtin_expect(far, 0)) probabilities(std::true_type{});
+        else probabilities(std::false_type{});
         const uint64_t acc = add2(acc0, acc1);
         l += f2lo(acc) + f2hi(acc);
     }
@@ -327,16 +343,15 @@ __device__ __forceinline__ void softmax_stream(uint8_t* smem, Bars* b, uint32_t 
     const int row = (u.pair ? t * kRows : 0) + r;
     const int64_t at = ((int64_t)split * a.kv_heads + u.head) * a.rows + u.row0 + row;
     if (!ok) {
-        if (row < u.nrows) a.lse[at] = NB200_NAN;
+        if (row < u.nrows) a.ml[at] = make_float2(NB200_NAN, NB200_NAN);
         return;
     }
     float f0 = 1.f, f1 = 0.f;
     const bool merge = !u.pair && u.n > 1;
     if (merge) {
         const float m1 = b->m[r], top = fmaxf(m, m1);
-        // Without a finite score a stream's sum is 0, or NaN.
-        f0 = m == -NB200_INF ? l : ex2(m - top);
-        f1 = m1 == -NB200_INF ? b->l[r] : ex2(m1 - top);
+        f0 = weight_of(m, l, top, sl2);
+        f1 = weight_of(m1, b->l[r], top, sl2);
         l = l * f0 + b->l[r] * f1;
         m = top;
     }
@@ -362,7 +377,7 @@ __device__ __forceinline__ void softmax_stream(uint8_t* smem, Bars* b, uint32_t 
             }
         }
     }
-    if (row < u.nrows) a.lse[at] = l == 0.f ? -NB200_INF : m + log2f(l) - kLift<T>;
+    if (row < u.nrows) a.ml[at] = make_float2(m, l);
 }
 
 template <typename T, int D>
