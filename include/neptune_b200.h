@@ -432,10 +432,12 @@ int nb200_norm8(const nb200_norm8_args* args, void* q, float* scale, void* y, vo
  * tokens (nullable with history = 0) is [rows, history]: the first token_lens[row] (null: all) are the row's
  * history, of which the first prompt_lens[row] (null: none) are its prompt and the others its output. A token or
  * bias index outside [0, vocab) is skipped. repetition, presence, frequency, temperature: fp32 [rows], each
- * nullable (no such step); the caller keeps repetition and temperature positive. allowed (nullable) is
+ * nullable (no such step); the caller keeps repetition and temperature positive (of one below 2^-128 fp32 does not
+ * hold the reciprocal: its largest value stands in, so that 0 stays 0). allowed (nullable) is
  * [rows, ceil(vocab / 32)] int32, bit v % 32 of word v / 32. logits is [rows, vocab], out contiguous like it, of one
- * dtype, and no memory of logits; every tensor has unit column stride. biases <= 1024 (else NB200_ERR_CAPACITY). work: device memory, 16-byte
- * aligned, of nb200_penalize_logits_work_bytes(args) bytes (0 without history and biases). No counterpart in the
+ * dtype, and no memory of logits; every tensor has unit column stride. biases <= 1024 (else NB200_ERR_CAPACITY).
+ * work: device memory, 16-byte aligned, of nb200_penalize_logits_work_bytes(args) bytes (0 without history and
+ * biases). No counterpart in the
  * reference. */
 typedef struct {
     const void *logits, *tokens, *bias_index;

@@ -285,6 +285,21 @@ constexpr int kSelfTokens = 4096, kSelfBiases = kSweepThreads;
 constexpr uint32_t kMention = 1u << 16, kWithBias = 1u << 14, kManyBiases = 1u << 15;
 static_assert(kSelfTokens < (int)kWithBias, "a count's bits");
 
+// x / d, d positive, by d's reciprocal. An fp32 quotient is corrected once by its remainder (Markstein's method), which leaves it
+// rounded once; beside a 16-bit result's rounding of 2^-11 or 2^-8 the reciprocal's 2^-24 counts for nothing. Where fp32 does
+// not hold the reciprocal (d below 2^-128) its largest value stands in: 0 / d stays 0.
+template <typename T>
+struct Divisor {
+    float d, inv;
+    __device__ __forceinline__ explicit Divisor(const float* p) : d(p ? *p : 1.f), inv(fminf(1.f / d, 0x1.fffffep127f)) {}
+    __device__ __forceinline__ float operator()(float x) const {
+        const float q = x * inv;
+        if constexpr (sizeof(T) != 4) return q;
+        const float exact = fmaf(fmaf(-q, d, x), inv, q);
+        return fabsf(q) < NB200_INF ? exact : q;  // of an infinity the remainder is NaN
+    }
+};
+
 // Temperature and mask of a tile, and all of it for its named tokens. JOINED: rows of input and output are cut by different
 // 16-byte boundaries (a vocabulary that is padded on the one side), and a vector of the output is joined from two. bf16
 // [1024, 131071] of rows 131072 apart: 157 us, token by token 336; [256, 32001] 7.6 and 16.3.
@@ -314,7 +329,7 @@ __global__ void __launch_bounds__(kSweepThreads, NAMES == SELF || JOINED ? 4 : k
             ok[k] = r.allowed ? mask_bits(r.allowed, body + (int64_t)i * V, V) : ~0u;
         }
     }
-    const float inv = n.temperature ? 1.f / n.temperature[row] : 1.f;
+    const Divisor<T> cool(n.temperature ? n.temperature + row : nullptr);
     // A CTA of the first wave runs beside name_kernel and waits for it only behind its tile. Those that come later find
     // it done, and have their entries on the way with the logits.
     const bool later = NAMED && blockIdx.x >= a.first;
@@ -382,7 +397,7 @@ __global__ void __launch_bounds__(kSweepThreads, NAMES == SELF || JOINED ? 4 : k
             float f[V];
             Elem<T>::unpack(raw[k], f);
 #pragma unroll
-            for (int j = 0; j < V; ++j) f[j] = ok[k] >> j & 1u ? f[j] * inv : -NB200_INF;
+            for (int j = 0; j < V; ++j) f[j] = ok[k] >> j & 1u ? cool(f[j]) : -NB200_INF;
             const uint4 o = Elem<T>::pack(f);
             if (NAMES) *reinterpret_cast<uint4*>(r.out + body + (int64_t)i * V) = o;
             else st_stream(r.out + body + (int64_t)i * V, o);
@@ -390,17 +405,17 @@ __global__ void __launch_bounds__(kSweepThreads, NAMES == SELF || JOINED ? 4 : k
     }
     // What lies before the first vector and behind the last one, or all of it.
     auto allows = [&](int64_t v) { return !r.allowed || ((uint32_t)__ldg(r.allowed + (v >> 5)) >> (v & 31) & 1u); };
-    auto one = [&](int64_t v) { r.out[v] = Elem<T>::from_f(allows(v) ? Elem<T>::to_f(r.x[v]) * inv : -NB200_INF); };
+    auto one = [&](int64_t v) { r.out[v] = Elem<T>::from_f(allows(v) ? cool(Elem<T>::to_f(r.x[v])) : -NB200_INF); };
     for (int64_t v = lo + threadIdx.x; v < body; v += kSweepThreads) one(v);
     for (int64_t v = body + (int64_t)vectors * V + threadIdx.x; v < hi; v += kSweepThreads) one(v);
     if constexpr (NAMES != NONE) {
-        const float rep = n.repetition ? n.repetition[row] : 1.f, inv_rep = 1.f / rep;
+        const Divisor<T> rep(n.repetition ? n.repetition + row : nullptr);
         const float freq = n.frequency ? n.frequency[row] : 0.f, pres = n.presence ? n.presence[row] : 0.f;
         auto again = [&](int64_t v, uint32_t count, float bias, bool history) {
             float f = Elem<T>::to_f(r.x[v]);
-            if (history) f *= f > 0.f ? inv_rep : rep;
+            if (history) f = f > 0.f ? rep(f) : f * rep.d;
             if (count) f = f - freq * (float)count - pres;
-            f = (f + bias) * inv;
+            f = cool(f + bias);
             r.out[v] = Elem<T>::from_f(allows(v) ? f : -NB200_INF);
         };
         if (NAMED && !later) look_up();

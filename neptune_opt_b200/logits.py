@@ -11,7 +11,8 @@ Per row and token, in this order, in fp32 and rounded once:
 logits is [rows, vocab] in float32, bfloat16 or float16. tokens [rows, history] int32/int64 holds each row's
 tokens: the first token_lens (default: all), of which the first prompt_lens (default: none) are its prompt and
 the others its output. repetition, presence, frequency and temperature are float32 [rows], each optional; the
-caller keeps repetition and temperature positive. bias_index [rows, n] int32/int64 and bias_value [rows, n]
+caller keeps repetition and temperature positive (for one below 2^-128, whose reciprocal fp32 does not hold, its
+largest value stands in, so that 0 stays 0). bias_index [rows, n] int32/int64 and bias_value [rows, n]
 float32, n at most 1024. A token or index outside [0, vocab) is skipped. allowed [rows, ceil(vocab / 32)]
 int32 has bit v % 32 of word v // 32 for token v; a row may allow nothing. One mask, history or bias list for
 all rows may be passed expanded. The reference has no such operator; `softmax`, `log_softmax` and the folds take
