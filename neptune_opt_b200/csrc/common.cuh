@@ -33,6 +33,16 @@ int finish_launch(const char* what);  // checks cudaGetLastError, returns nb200_
 // kernel has completed and its writes are visible, so results are exactly those of plain stream
 // order. pdl_trigger() allows the next PDL kernel to be scheduled; it can start only after every
 // CTA of this grid has triggered or exited, so a grid never waits on a dependent for resources.
+//
+// The second kernel of one call may do more before it waits, where every CTA of the call's first kernel triggers behind its own
+// pdl_wait(): the second one then starts after all work ahead of the call has completed and its results have been flushed to
+// global memory, so only what the first kernel touches is still to be waited for. Until then the second one may write memory
+// that the first one neither reads nor writes, and read what was written before the call: by TMA or ld_early, past L1, which
+// no wait has made current, or behind fence_early, of device scope, which makes L1 drop what it holds. These are stream_kernel behind
+// tensor_part_kernel, and join_kernel's lengths (prefix_attention.cu; if stream_kernel waited first, 256 sequences behind 16384
+// keys would take 150 us for 96). Each still waits before it ends, or one CTA for all, so that a kernel behind it that waits
+// for it has waited for both. (attn_bwd_kernel, too, waits for its statistics alone; the kernel ahead of it is launched in
+// plain stream order, which begins with every cache current.)
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
@@ -62,6 +72,11 @@ __device__ __forceinline__ void cluster_arrive_started() {
 __device__ __forceinline__ void cluster_wait_started() {
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+
+// What a kernel reads before its pdl_wait(), and what makes plain reads do.
+__device__ __forceinline__ void fence_early() { asm volatile("fence.acq_rel.gpu;" ::: "memory"); }
+template <typename T>
+__device__ __forceinline__ T ld_early(const T* p) { return __ldcg(p); }
 
 inline size_t dtype_size(int dtype) { return dtype == NB200_F32 ? 4 : 2; }
 

@@ -34,7 +34,6 @@ struct Logits {
     int buckets, span;     // buckets of a row, each of 2^span tiles
     int64_t most;          // entries of a part, at most
     bool self;             // the sweep finds the named tokens by itself
-    unsigned first;        // CTAs of the sweep that begin before the names are known
     int* starts;           // [rows][parts][buckets + 1]: where a bucket's entries begin
     uint4* entries;        // [rows][parts][most]: token, count in the output, bias, whether the history has it
 };
@@ -307,10 +306,8 @@ template <typename T, Names NAMES, bool JOINED>
 __global__ void __launch_bounds__(kSweepThreads, NAMES == SELF || JOINED ? 4 : kSweepCtas) sweep_kernel(const Logits a) {
     constexpr int V = Elem<T>::V;
     constexpr bool NAMED = NAMES == ENTRIES;
-    if (!NAMED) {  // else the inputs are older than name_kernel, which had them before this one could start
-        pdl_wait();
-        pdl_trigger();
-    }
+    pdl_wait();
+    pdl_trigger();
     const nb200_logits_args& n = a.n;
     const int64_t row = blockIdx.x / (unsigned)a.tiles;
     const int tile = (int)(blockIdx.x % (unsigned)a.tiles);
@@ -330,20 +327,15 @@ __global__ void __launch_bounds__(kSweepThreads, NAMES == SELF || JOINED ? 4 : k
         }
     }
     const Divisor<T> cool(n.temperature ? n.temperature + row : nullptr);
-    // A CTA of the first wave runs beside name_kernel and waits for it only behind its tile. Those that come later find
-    // it done, and have their entries on the way with the logits.
-    const bool later = NAMED && blockIdx.x >= a.first;
+    // The entries are on their way with the logits.
     const int* starts = a.starts + row * a.parts * (a.buckets + 1) + (NAMED ? tile >> a.span : 0);
     const uint4* entries = a.entries + row * a.parts * a.most;
     int e0 = 0, e1 = 0;
     uint4 entry = make_uint4(0u, 0u, 0u, 0u);
-    auto look_up = [&] {
-        pdl_wait();
-        pdl_trigger();
+    if (NAMED) {
         e0 = starts[0], e1 = starts[1];
         if (e0 + (int)threadIdx.x < e1) entry = entries[e0 + threadIdx.x];
-    };
-    if (later) look_up();
+    }
     // SELF: a word for each of the tile's tokens, those that the history names, in any order, and the biases.
     constexpr int kCounts = NAMES == SELF ? kTile<T> + 16 : 4;
     __shared__ __align__(16) uint32_t counts[kCounts];
@@ -418,7 +410,6 @@ __global__ void __launch_bounds__(kSweepThreads, NAMES == SELF || JOINED ? 4 : k
             f = cool(f + bias);
             r.out[v] = Elem<T>::from_f(allows(v) ? f : -NB200_INF);
         };
-        if (NAMED && !later) look_up();
         __syncthreads();  // the tile is written
         if constexpr (NAMED) {
 #pragma unroll 1
@@ -486,7 +477,6 @@ int64_t plan(Logits& a, int tile) {
     a.most = std::min<int64_t>(entries, a.range);
     while (((a.tiles - 1) >> a.span) >= kMostBuckets) ++a.span;
     a.buckets = ((a.tiles - 1) >> a.span) + 1;
-    a.first = (unsigned)(kSweepCtas * sm_count());
     return n.rows * a.parts * (a.most * 16 + (a.buckets + 1) * 4);
 }
 

@@ -43,7 +43,7 @@ struct StreamArgs : Line {
     float* o;       // [slots][slot_rows][D]
     float2* ml;     // [slots][slot_rows]
     int2* span;     // [units]: first and last worker
-    bool beside;    // runs beside the kernel ahead of it, of which it needs nothing
+    bool beside;    // runs beside the kernel ahead of it, of which it needs nothing (common.cuh)
 };
 
 template <typename T> struct Mma;
@@ -253,7 +253,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, NT>)
         abort_flag[warp] = 0;
         fence_barrier_init();
     }
-    if (!a.beside) pdl_wait();
+    if (a.beside) fence_early();
+    else pdl_wait();
     pdl_trigger();
     const int worker = (int)blockIdx.x * kWarps + warp;
     // The kernel that joins the parts waits for this one alone, so this one ends after the kernel ahead of it: its last
@@ -432,7 +433,7 @@ __global__ void __launch_bounds__(W * 32, D == 64 || W == 4 ? 2 : 1)
     pdl_trigger();
     const int seq = (int)(blockIdx.x / (unsigned)a.kv_heads), head = (int)(blockIdx.x % (unsigned)a.kv_heads);
     const int group = a.query.group, tokens = a.query.tokens, rows = group * tokens;
-    const int own = tokens_of(a.lens, seq, a.cache), shared_steps = steps_of(a.prefix), steps = shared_steps + steps_of(own);
+    const int own = a.tokens(seq), shared_steps = steps_of(a.prefix), steps = shared_steps + steps_of(own);
     const int share = (steps + W - 1) / W, begin = warp * share, end = min(begin + share, steps);
     int get = begin;
     auto copy = [&](int stage) {
@@ -573,8 +574,7 @@ __global__ void __launch_bounds__(256) join_kernel(const JoinArgs a) {
     const int head = (int)(id / a.rows), r = (int)(id % a.rows);
     const int t = r % a.tokens, g = r / a.tokens % a.group, b = r / a.tokens / a.group;
     const int64_t at = ((int64_t)b * a.kv_heads * a.group + head * a.group + g) * a.tokens + t;
-    // The lengths are older than the kernels ahead, which had them before this one could start.
-    const int len = tokens_of(a.lens, b, a.cache);
+    const int len = a.lens ? max(0, min(ld_early(a.lens + b), a.cache)) : a.cache;
     pdl_wait();
     pdl_trigger();
     float top = -NB200_INF, sum = 0.f, v[E];
