@@ -555,7 +555,8 @@ struct JoinArgs {
     const int* lens;
     int kv_heads, group, tokens, rows, cache;
     int splits;                          // of the tensor cores (0: none)
-    int prefix_tiles, own_tiles, tile_rows, slot_rows;
+    bool shared;                         // units of the prefix come first
+    int own_tiles, tile_rows, slot_rows;
 };
 
 // WIDE: a CTA per query row, its eight warps taking turns at the parts; else a warp per row. The parts are the
@@ -587,16 +588,15 @@ __global__ void __launch_bounds__(256) join_kernel(const JoinArgs a) {
         int64_t far = 0, far_step = a.slot_rows;
         int nfar = 0;
         const int in = r - b * a.group * a.tokens;
-        const int unit = a.kv_heads * a.prefix_tiles + (b * a.kv_heads + head) * a.own_tiles + in / a.tile_rows;
+        const int unit = (a.shared ? a.kv_heads : 0) + (b * a.kv_heads + head) * a.own_tiles + in / a.tile_rows;
         const int2 w = a.span[unit];
         bool known = are_workers(w.x, w.y, a.workers);
         if (a.splits) {
             far_o = a.tensor_o, far_ml = a.tensor_ml, far = id, far_step = all, nfar = a.splits;
-        } else if (a.prefix_tiles) {
-            const int shared = head * a.prefix_tiles + r / a.tile_rows;
-            const int2 u = a.span[shared];
+        } else if (a.shared) {
+            const int2 u = a.span[head];
             known &= are_workers(u.x, u.y, a.workers);
-            far = (int64_t)(u.x + shared) * a.slot_rows + r % a.tile_rows;
+            far = (int64_t)(u.x + head) * a.slot_rows + r;
             nfar = u.y - u.x + 1;
         }
         const int64_t near = (int64_t)(w.x + unit) * a.slot_rows + in % a.tile_rows;
@@ -674,7 +674,8 @@ struct Plan {
     int nt;                        // 8-row tiles of a unit
     bool solo;                     // solo_kernel does it all
     int splits;                    // of the prefix on the tensor cores (0: it is in the stream kernel, or empty)
-    int64_t prefix_tiles, own_tiles, slot_rows, units, ctas;
+    bool shared;                   // the stream kernel's line has the prefix's units
+    int64_t own_tiles, slot_rows, units, ctas;
     int64_t most_parts;            // parts of a row, at most
     // Workspace, in bytes from its start.
     int64_t tensor_o, tensor_ml, o, ml, span, bytes;
@@ -704,16 +705,17 @@ Plan plan_of(const nb200_prefix_attn_args& a) {
         const int64_t bytes = a.batch * a.kv_heads * a.cache * a.head_dim * 4 / (a.seq_lens ? 2 : 1);
         p.splits = tensor_splits(a.kv_heads, p.rows, a.prefix, bytes);
     }
-    const int64_t most = a.prefix && !p.splits ? p.rows : own_rows;
-    p.nt = most <= 8 ? 1 : most <= 16 ? 2 : 4;
+    p.shared = a.prefix && !p.splits;
+    const int64_t most = p.shared ? p.rows : own_rows;
+    p.nt = most <= 8 ? 1 : most <= 16 ? 2 : 4;  // one tile holds all rows that meet the prefix
+    static_assert(kStreamRows <= 32 && kFewRows <= 32, "a tile's rows");
     const int64_t tile = 8 * p.nt;
-    p.prefix_tiles = a.prefix && !p.splits ? (p.rows + tile - 1) / tile : 0;
     p.own_tiles = (own_rows + tile - 1) / tile;
     p.slot_rows = std::min(tile, most);
-    p.units = a.kv_heads * (p.prefix_tiles + a.batch * p.own_tiles);
+    p.units = a.kv_heads * (p.shared + a.batch * p.own_tiles);
     auto line = [](int64_t keys) { return keys ? kEntry + (keys + kStepKeys - 1) / kStepKeys : 0; };
-    const int64_t prefix_steps = p.prefix_tiles ? line(a.prefix) : 0, own_steps = line(a.cache);
-    const int64_t steps = a.kv_heads * (p.prefix_tiles * prefix_steps + a.batch * p.own_tiles * own_steps);
+    const int64_t prefix_steps = p.shared ? line(a.prefix) : 0, own_steps = line(a.cache);
+    const int64_t steps = a.kv_heads * (prefix_steps + a.batch * p.own_tiles * own_steps);
     // Two CTAs an SM. Four where each worker still has 16 places and the SM holds four (caches of 256 sequences, head
     // dimension 64: 33.5 us, with two 37.4; with few places the more parts cost more than that gives, 12.8 us against
     // 10.9).
@@ -786,7 +788,7 @@ int launch_all(const nb200_prefix_attn_args& n, const nb200_attn_strides* s, con
     StreamArgs a = {};
     a.query = query;
     Maps maps = {};
-    if ((p.prefix_tiles || (p.solo && n.prefix)) &&
+    if ((p.shared || (p.solo && n.prefix)) &&
         ((rc = encode_keys(&maps.shared_k, "prefix_k", pk, n.dtype, D, n.prefix, n.kv_heads, 1, s[1], kStepKeys)) ||
          (rc = encode_keys(&maps.shared_v, "prefix_v", pv, n.dtype, D, n.prefix, n.kv_heads, 1, s[2], kStepKeys))))
         return rc;
@@ -795,8 +797,8 @@ int launch_all(const nb200_prefix_attn_args& n, const nb200_attn_strides* s, con
         return rc;
     a.lens = n.seq_lens;
     a.batch = (int)n.batch, a.kv_heads = (int)n.kv_heads;
-    a.prefix = p.prefix_tiles || p.solo ? (int)n.prefix : 0, a.cache = (int)n.cache;
-    a.rows = (int)p.rows, a.prefix_tiles = (int)p.prefix_tiles, a.own_tiles = (int)p.own_tiles;
+    a.prefix = p.shared || p.solo ? (int)n.prefix : 0, a.cache = (int)n.cache;
+    a.rows = (int)p.rows, a.own_tiles = (int)p.own_tiles;
     a.slot_rows = (int)p.slot_rows;
     a.scale = n.scale, a.sl2 = sl2, a.slack = slack_of(sl2);
     if (p.solo) {
@@ -820,7 +822,7 @@ int launch_all(const nb200_prefix_attn_args& n, const nb200_attn_strides* s, con
     j.workers = (int)p.ctas * kWarps;
     j.out = o, j.out_lse = lse, j.lens = n.seq_lens;
     j.kv_heads = a.kv_heads, j.group = query.group, j.tokens = query.tokens, j.rows = a.rows, j.cache = a.cache;
-    j.splits = p.splits, j.prefix_tiles = a.prefix_tiles, j.own_tiles = a.own_tiles, j.tile_rows = 8 * p.nt;
+    j.splits = p.splits, j.shared = p.shared, j.own_tiles = a.own_tiles, j.tile_rows = 8 * p.nt;
     j.slot_rows = a.slot_rows;
     const int64_t rows = n.kv_heads * p.rows;
     // A warp per row while the rows fill the GPU and their parts are few.

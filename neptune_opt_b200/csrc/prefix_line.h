@@ -1,8 +1,9 @@
 // The line of work that the stream kernel of attention behind a shared prefix deals out to its workers: plain arithmetic,
 // for kernels and host compilers alike.
 //
-// A unit is a tile of query rows and the keys they share: units of the prefix (key/value head, row tile; none when the
-// prefix runs on the tensor cores), then units of the caches (sequence, key/value head, row tile). All units' steps of 16
+// A unit is a tile of query rows and the keys they share: units of the prefix (a key/value head each, as few query rows as
+// one tile holds; none when the prefix runs on the tensor cores), then units of the caches (sequence, key/value head, row
+// tile). All units' steps of 16
 // keys stand in one line, each unit's behind kEntry places for its own start and end, and every worker takes an equal piece
 // of the line, whatever the sequences' lengths are. A piece covers the end of one unit, whole units, the beginning of
 // another: worker w's result for unit u goes to slot w + u, which no other pair has, and span[u] says which workers had a
@@ -25,14 +26,16 @@ NB200_PLAIN int places_of(int keys) { return keys > 0 ? kEntry + steps_of(keys) 
 
 struct Line {
     const int* lens;  // tokens of each sequence (null: all of the cache)
-    int batch, kv_heads, prefix, cache;
-    int prefix_tiles, own_tiles;  // row tiles of a unit's rows
+    int batch, kv_heads, cache;
+    int prefix;     // keys of the prefix's units (0: there are none)
+    int own_tiles;  // row tiles of a sequence's query rows
 
     NB200_PLAIN int tokens(int b) const {
         const int n = lens ? lens[b] : cache;
         return n < 0 ? 0 : n < cache ? n : cache;
     }
-    NB200_PLAIN int64_t shared_places() const { return (int64_t)kv_heads * prefix_tiles * places_of(prefix); }
+    NB200_PLAIN int64_t shared_places() const { return (int64_t)kv_heads * places_of(prefix); }
+    NB200_PLAIN int shared_units() const { return prefix ? kv_heads : 0; }
     NB200_PLAIN int64_t units_of_a_sequence() const { return (int64_t)kv_heads * own_tiles; }
 };
 
@@ -47,9 +50,9 @@ struct Cursor {
     }
     // The first place of a piece: place `at` of the prefix's units (b = -1) or of sequence b's.
     NB200_PLAIN void start(const Line& a, int b, int64_t at) {
-        sequence(a, b < 0 ? 0 : b);
-        int tiles = a.own_tiles;
-        if (b < 0) batch = -1, tiles = a.prefix_tiles, keys = a.prefix, steps = steps_of(keys);
+        if (b < 0) batch = -1, keys = a.prefix, steps = steps_of(keys);
+        else sequence(a, b);
+        const int tiles = b < 0 ? 1 : a.own_tiles;
         const int places = kEntry + steps, unit = (int)(at / places), place = (int)(at - (int64_t)unit * places) - kEntry;
         head = unit / tiles, tile = unit % tiles;
         step = place > 0 ? place : 0;
@@ -59,7 +62,7 @@ struct Cursor {
     NB200_PLAIN void next_unit(const Line& a) {
         step = 0;
         left -= kEntry;
-        if (++tile < (batch < 0 ? a.prefix_tiles : a.own_tiles)) return;
+        if (batch >= 0 && ++tile < a.own_tiles) return;
         tile = 0;
         if (++head < a.kv_heads) return;
         int b = batch;
@@ -78,8 +81,7 @@ struct Cursor {
         return left > 0;
     }
     NB200_PLAIN int unit(const Line& a) const {
-        return batch < 0 ? head * a.prefix_tiles + tile
-                         : a.kv_heads * a.prefix_tiles + (batch * a.kv_heads + head) * a.own_tiles + tile;
+        return batch < 0 ? head : a.shared_units() + (batch * a.kv_heads + head) * a.own_tiles + tile;
     }
 };
 

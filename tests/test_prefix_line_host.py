@@ -19,16 +19,16 @@ using namespace nb200::prefix;
 struct Span { int x = -7, y = -7; };
 
 // The workers of a call, one behind the other; worker w gives up before its stop[w]th step (< 0: never). 0: all is right.
-extern "C" int deal(const int* lens, int batch, int kv_heads, int prefix, int cache, int prefix_tiles, int own_tiles,
-                    int workers, const int* stop) {
+extern "C" int deal(const int* lens, int batch, int kv_heads, int prefix, int cache, int own_tiles, int workers,
+                    const int* stop) {
     Line a;
     a.lens = lens, a.batch = batch, a.kv_heads = kv_heads, a.prefix = prefix, a.cache = cache;
-    a.prefix_tiles = prefix_tiles, a.own_tiles = own_tiles;
+    a.own_tiles = own_tiles;
     const int64_t shared = a.shared_places(), each = a.units_of_a_sequence();
     int64_t all = shared;
     for (int b = 0; b < batch; ++b) all += each * places_of(a.tokens(b));
     const int64_t share = (all + workers - 1) / workers;
-    const int units = kv_heads * (prefix_tiles + batch * own_tiles);
+    const int units = a.shared_units() + kv_heads * batch * own_tiles;
     std::vector<Span> span(units);
     std::map<std::pair<int, int>, int> slot;             // (worker, unit): steps taken, -1 where it gave up
     std::vector<std::vector<int>> taken(units);
@@ -77,7 +77,7 @@ extern "C" int deal(const int* lens, int batch, int kv_heads, int prefix, int ca
         }
     }
     for (int u = 0; u < units; ++u) {
-        const int keys = u < kv_heads * prefix_tiles ? prefix : a.tokens((u - kv_heads * prefix_tiles) / (int)each);
+        const int keys = u < a.shared_units() ? prefix : a.tokens((u - a.shared_units()) / (int)each);
         if (!keys) {
             if (span[u].x != -7 || span[u].y != -7) return 3;
             continue;
@@ -109,14 +109,13 @@ def lib(tmp_path_factory):
 
 def _deal(lib, rng, gives_up):
     batch, kv_heads, own_tiles = rng.randint(1, 70), rng.choice([1, 2, 3, 8]), rng.choice([1, 1, 2, 5])
-    prefix_tiles = rng.choice([0, 1])
-    cache, prefix = rng.choice([0, 1, 16, 17, 300, 2000]), rng.choice([1, 15, 16, 333, 5000]) if prefix_tiles else 0
+    cache, prefix = rng.choice([0, 1, 16, 17, 300, 2000]), rng.choice([0, 0, 0, 1, 15, 16, 333, 5000])
     lens = [rng.choice([0, 0, 1, cache, cache + 9, -4, rng.randint(0, cache)]) for _ in range(batch)]
     workers = 4 * rng.choice([1, 2, 7, 148, 296, 592])
     stop = [rng.choice([0, 1, 2, 5, 20]) if rng.random() < gives_up else -1 for _ in range(workers)]
     as_ints = lambda v: (ctypes.c_int * len(v))(*v)  # noqa: E731
     with_lens = as_ints(lens) if rng.random() < 0.8 else None
-    return lib.deal(with_lens, batch, kv_heads, prefix, cache, prefix_tiles, own_tiles, workers, as_ints(stop))
+    return lib.deal(with_lens, batch, kv_heads, prefix, cache, own_tiles, workers, as_ints(stop))
 
 
 @pytest.mark.parametrize("gives_up", [0.0, 0.05, 0.6, 1.0])
