@@ -817,6 +817,7 @@ int nb200_penalize_logits(const nb200_logits_args* args, void* out, void* work, 
         return NB200_ERR_ARG;
     }
     const int64_t need = logits_work_bytes(*args);
+    if (need < 0) return (int)need;
     if (need && (!work || !aligned16(work) || work_bytes < need)) {
         set_error("nb200_penalize_logits: work must hold %lld bytes, 16-byte aligned", (long long)need);
         return NB200_ERR_ARG;

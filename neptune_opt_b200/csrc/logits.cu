@@ -456,10 +456,19 @@ static_assert(kMostBiases <= 2 * kNameThreads, "two biases a thread");
 static_assert(name_bytes(kMostRange, slots_of(kMostTable + kMostBiases), kMostBuckets, kMostBiases) <= 200 << 10, "shared memory");
 SharedLimit g_shared[3];
 
-// The shapes of a call, and the bytes of its workspace.
+// Whether a grid holds that many CTAs a row.
+int64_t held(const nb200_logits_args& n, int64_t ctas) {
+    if (n.rows * ctas <= 0x7fffffffLL) return NB200_OK;
+    set_error("nb200_penalize_logits: rows=%lld, vocab=%lld exceed the kernel's index range", (long long)n.rows,
+              (long long)n.vocab);
+    return NB200_ERR_CAPACITY;
+}
+
+// The shapes of a call, and the bytes of its workspace (negative: an error).
 int64_t plan(Logits& a, int tile) {
     const nb200_logits_args& n = a.n;
     a.tiles = (int)((n.vocab + tile - 1) / tile);
+    if (const int64_t rc = held(n, a.tiles)) return rc;
     const int64_t entries = std::min(n.history + n.biases, n.vocab);
     if (!entries) return 0;
     // A few tiles a row, or a few an SM: every tile counts the history itself, without a second launch and its workspace.
@@ -472,6 +481,7 @@ int64_t plan(Logits& a, int tile) {
     // out to as many CTAs as it takes for every token of a range to fit, whatever the history holds.
     const int64_t fits = n.history / 2 <= kMostTable ? kMostRange : kMostTable;
     a.parts = (int)((n.vocab + fits - 1) / fits);
+    if (const int64_t rc = held(n, a.parts)) return rc;
     a.range = (int)((n.vocab + a.parts - 1) / a.parts);
     a.slots = slots_of((int)std::min<int64_t>(n.history / 2, a.range) + (int)n.biases);
     a.most = std::min<int64_t>(entries, a.range);
@@ -486,10 +496,6 @@ template <typename T>
 int launch(const Logits& a, SharedLimit& shared, cudaStream_t st) {
     const char* what = "nb200_penalize_logits";
     const nb200_logits_args& n = a.n;
-    if (n.rows * std::max(a.tiles, a.parts) > 0x7fffffffLL) {
-        set_error("%s: rows=%lld, vocab=%lld exceed the kernel's index range", what, (long long)n.rows, (long long)n.vocab);
-        return NB200_ERR_CAPACITY;
-    }
     const unsigned grid = (unsigned)(n.rows * a.tiles);
     const bool alike = ((reinterpret_cast<uintptr_t>(n.logits) ^ reinterpret_cast<uintptr_t>(a.out)) & 15u) == 0 &&
                        (n.rows == 1 || (n.stride_logits - n.vocab) % Elem<T>::V == 0);
@@ -520,7 +526,7 @@ int64_t logits_work_bytes(const nb200_logits_args& n) {
 
 int launch_logits(const nb200_logits_args& n, void* out, void* work, cudaStream_t st) {
     Logits a = {n, out};
-    plan(a, tile_of(n.dtype));
+    if (const int64_t rc = plan(a, tile_of(n.dtype)); rc < 0) return (int)rc;
     a.entries = static_cast<uint4*>(work);
     a.starts = reinterpret_cast<int*>(a.entries + n.rows * a.parts * a.most);
     if (n.dtype == NB200_F32) return launch<float>(a, g_shared[0], st);

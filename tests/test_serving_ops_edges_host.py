@@ -121,3 +121,19 @@ def test_traced_ops_refuse_what_no_kernel_takes(op, error, bad):
 def _meta_ops():
     """The ops are registered by the first call of a function."""
     NB.penalize_logits(_meta(1, 1))
+
+
+def test_no_workspace_is_quoted_for_logits_that_no_grid_holds():
+    """Rows times tiles, or times the naming kernel's parts, past 2^31: refused before a size is worked out of them."""
+    import ctypes
+
+    lib = L.load()
+
+    def work(rows, vocab, history):
+        a = L.NB200LogitsArgs(*[1 << 20] * 2, *[None] * 9, rows, vocab, history, 0, vocab, history, 0, 0, 0, 0, 1, 0)
+        return lib.nb200_penalize_logits_work_bytes(ctypes.byref(a)), lib.nb200_penalize_logits(
+            ctypes.byref(a), ctypes.c_void_p(1 << 63), ctypes.c_void_p(1 << 40), 1 << 62, None)
+
+    for sizes in ((1 << 30, 1 << 30, 1 << 28), (1 << 30, 1 << 30, 5000), (1 << 30, 1 << 24, 0), (1 << 26, 1 << 18, 1 << 20)):
+        assert work(*sizes) == (L.NB200_ERR_CAPACITY,) * 2, sizes
+    assert work(1 << 20, 1 << 20, 9000)[0] > 0
