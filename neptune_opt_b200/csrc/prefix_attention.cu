@@ -48,6 +48,7 @@ struct StreamArgs : Line {
 
 template <typename T> struct Mma;
 template <> struct Mma<__nv_bfloat16> {
+    static constexpr uint32_t kExponents = 0x7f807f80u;  // of a pair, all ones: infinities and NaN
     __device__ __forceinline__ static void mul(float* d, const uint32_t* a, const uint32_t* b) {
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -55,6 +56,7 @@ template <> struct Mma<__nv_bfloat16> {
     }
 };
 template <> struct Mma<__half> {
+    static constexpr uint32_t kExponents = 0x7c007c00u;
     __device__ __forceinline__ static void mul(float* d, const uint32_t* a, const uint32_t* b) {
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -122,8 +124,9 @@ __device__ __forceinline__ Cursor piece_of(const StreamArgs& a, int worker, int 
 }
 
 // What a worker keeps of a unit's query rows, its running maximum, sum and output, and what a step of 16
-// keys does to it. Column tile n of a lane's accumulators: query rows 8 n + 2 (lane % 4) and the next one.
-template <typename T, int D, int NT>
+// keys does to it. Column tile n of a lane's accumulators: query rows 8 n + 2 (lane % 4) and the next one. SEVERAL: of new
+// tokens a sequence (what only several need would cost single ones 2 to 5%).
+template <typename T, int D, int NT, bool SEVERAL>
 struct Rows {
     float o[NT][D / 16][4], m[NT][2], l[NT][2];
 
@@ -138,9 +141,25 @@ struct Rows {
                 for (int e = 0; e < 4; ++e) o[n][d][e] = 0.f;
         }
     }
-    // Keys kb on, of a box at ks and vs in shared memory; `limit`: the last key a row sees, `lowest`: the least of them.
+    // Whether the lane's part of a staged V's keys from..to holds an infinity or NaN.
+    __device__ __forceinline__ static bool any_odd(uint32_t vs, int from, int to, int lane) {
+        bool odd = false;
+#pragma unroll 1
+        for (int i = from * 8 + lane; i < (to + 1) * 8; i += 32)
+#pragma unroll 1
+            for (int h = 0; h < D / 64; ++h) {
+                uint32_t w[4];
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(vs + h * kStepKeys * 128 + i * 16));
+#pragma unroll
+                for (int k = 0; k < 4; ++k) odd |= __vcmpeq2(w[k] & Mma<T>::kExponents, Mma<T>::kExponents) != 0u;
+            }
+        return odd;
+    }
+    // Keys kb on, of a box at ks and vs in shared memory; `limit`: the last key a row sees, `lowest` and `highest`: the least
+    // and the greatest of them.
     __device__ __forceinline__ void step(const uint32_t (*qf)[D / 16][2], uint32_t ks, uint32_t vs, int kb,
-                                         const int (*limit)[2], int lowest, float sl2, float slack, int lane) {
+                                         const int (*limit)[2], int lowest, int highest, float sl2, float slack, int lane) {
         constexpr uint32_t kBox = kStepKeys * 128;
         // This lane's address in a box: the row it loads for ldmatrix, and the swizzle of its 16-byte pieces.
         const int k_row = lane & 15, k_piece = lane >> 4;                         // K: keys 0-15, then 8 columns on
@@ -200,10 +219,47 @@ struct Rows {
             p[n][0] = transpose8(Elem<T>::pack_word(x[0], x[1]));
             p[n][1] = transpose8(Elem<T>::pack_word(x[2], x[3]));
         }
+        auto values = [&](int d, uint32_t* f) {
+            ldmatrix4_t(f, vs + (d / 4) * kBox + v_row * 128 + (((2 * (d % 4) + v_piece) ^ (v_row & 7)) << 4));
+        };
+        // Of several new tokens the earlier ones do not see the later ones' keys: their probabilities there are 0, which takes
+        // any value but an infinity or NaN out of the product. Where there is one, the rows of each limit take the product
+        // by themselves, the greatest limit first, and the values that no row is left to see are zeroed.
+        if (SEVERAL && min(highest, kb + kStepKeys - 1) > lowest) {
+            const int last = min(highest, kb + kStepKeys - 1);
+            if (__any_sync(0xffffffffu, any_odd(vs, max(lowest + 1 - kb, 0), last - kb, lane))) {
+#pragma unroll 1
+                for (int key = last; key >= max(lowest, kb); --key) {
+#pragma unroll
+                    for (int d = 0; d < D / 16; ++d) {
+                        uint32_t f[4];
+                        values(d, f);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            float x[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) x[e] = o[n][d][e];
+                            Mma<T>::mul(x, f, p[n]);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (min(limit[n][e % 2], last) == key) o[n][d][e] = x[e];
+                        }
+                    }
+                    __syncwarp();
+                    if (lane < 8 * (D / 64))
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(vs + lane / 8 * kBox + (key - kb) * 128 + lane % 8 * 16),
+                                     "r"(0u)
+                                     : "memory");
+                    fence_proxy_async();
+                    __syncwarp();
+                }
+                return;
+            }
+        }
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) {
             uint32_t f[4];
-            ldmatrix4_t(f, vs + (d / 4) * kBox + v_row * 128 + (((2 * (d % 4) + v_piece) ^ (v_row & 7)) << 4));
+            values(d, f);
 #pragma unroll
             for (int n = 0; n < NT; ++n) Mma<T>::mul(o[n][d], f, p[n]);
         }
@@ -233,7 +289,7 @@ __device__ __forceinline__ void zero_behind(uint32_t vs, int keys, int lane) {
 //
 // Every wait is bounded; one that runs out sets bit 1 of the fault word, and the worker waits (again with a limit) for
 // its copies and leaves NaN in the slots of its unfinished shares.
-template <typename T, int D, int NT>
+template <typename T, int D, int NT, bool SEVERAL>
 __global__ void __launch_bounds__(kWarps * 32, kCtas<D, NT>)
     stream_kernel(const __grid_constant__ CUtensorMap shared_k, const __grid_constant__ CUtensorMap shared_v,
                   const __grid_constant__ CUtensorMap own_k, const __grid_constant__ CUtensorMap own_v,
@@ -292,7 +348,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, NT>)
     // Column tile n of this lane's accumulators: query rows 8 n + 2 (lane % 4) and the next one.
     uint32_t qf[NT][D / 16][2], next_q[kAhead ? NT : 1][D / 16][2];
     int limit[NT][2], lowest = 0;  // last key a row sees; of the unit's rows, the least
-    Rows<T, D, NT> t;
+    Rows<T, D, NT, SEVERAL> t;
     int nrows = 0;
     auto load_rows = [&](const Cursor& c, uint32_t(*q)[D / 16][2]) {
         const bool shared = c.batch < 0;
@@ -301,7 +357,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, NT>)
         for (int n = 0; n < NT; ++n) {
             const int in = 8 * n + (lane >> 2);  // past the last row: the first one again, whose result is not stored
             int seq = c.batch, g = first + (in < rows ? in : 0), tok = 0;
-            if (a.query.tokens > 1) tok = g % a.query.tokens, g /= a.query.tokens;
+            if constexpr (SEVERAL) tok = g % a.query.tokens, g /= a.query.tokens;
             if (shared) seq = g / a.query.group, g %= a.query.group;
             const T* p = static_cast<const T*>(a.query.q) + seq * a.query.qb +
                          (int64_t)(c.head * a.query.group + g) * a.query.qh + tok * a.query.qt + 2 * (lane & 3);
@@ -322,7 +378,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, NT>)
 #pragma unroll
             for (int e = 0; e < 2; ++e)
                 limit[n][e] = shared ? use.keys - 1
-                              : lowest + (a.query.tokens > 1 ? (in_unit + 8 * n + 2 * (lane & 3) + e) % a.query.tokens : 0);
+                              : lowest + (SEVERAL ? (in_unit + 8 * n + 2 * (lane & 3) + e) % a.query.tokens : 0);
         }
         t.clear();
         if (kAhead && use.left > use.steps - use.step) {
@@ -347,7 +403,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, NT>)
         const int kb = use.step * kStepKeys;
         // What a cache holds behind a sequence must not reach the products: 0 times an infinity is none.
         if (use.batch >= 0) zero_behind<D>(vs, use.keys - kb, lane);
-        t.step(qf, ks, vs, kb, limit, lowest, a.sl2, a.slack, lane);
+        t.step(qf, ks, vs, kb, limit, lowest, use.keys - 1, a.sl2, a.slack, lane);
 
         ++done;
         if (++stage == kStages) stage = 0, phase ^= 1u;
@@ -410,7 +466,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, NT>)
 // prefix and the cache, one list of keys for the same rows, and join in shared memory. (Rows as in stream_kernel; of a
 // unit's two tiles the prefix's rows are the sequence's own.) The bound is latency, a launch and a few steps. A wait that
 // runs out, as there: the CTA's rows read out as NaN.
-template <typename T, int D, int NT, int W>
+template <typename T, int D, int NT, int W, bool SEVERAL>
 __global__ void __launch_bounds__(W * 32, D == 64 || W == 4 ? 2 : 1)
     solo_kernel(const __grid_constant__ CUtensorMap shared_k, const __grid_constant__ CUtensorMap shared_v,
                 const __grid_constant__ CUtensorMap own_k, const __grid_constant__ CUtensorMap own_v, const StreamArgs a,
@@ -432,7 +488,7 @@ __global__ void __launch_bounds__(W * 32, D == 64 || W == 4 ? 2 : 1)
     pdl_wait();
     pdl_trigger();
     const int seq = (int)(blockIdx.x / (unsigned)a.kv_heads), head = (int)(blockIdx.x % (unsigned)a.kv_heads);
-    const int group = a.query.group, tokens = a.query.tokens, rows = group * tokens;
+    const int group = a.query.group, tokens = SEVERAL ? a.query.tokens : 1, rows = group * tokens;
     const int own = a.tokens(seq), shared_steps = steps_of(a.prefix), steps = shared_steps + steps_of(own);
     const int share = (steps + W - 1) / W, begin = warp * share, end = min(begin + share, steps);
     int get = begin;
@@ -458,7 +514,7 @@ __global__ void __launch_bounds__(W * 32, D == 64 || W == 4 ? 2 : 1)
 
     uint32_t qf[NT][D / 16][2];
     int limit[NT][2];  // of the cache's keys
-    Rows<T, D, NT> t;
+    Rows<T, D, NT, SEVERAL> t;
     t.clear();
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -487,11 +543,11 @@ __global__ void __launch_bounds__(W * 32, D == 64 || W == 4 ? 2 : 1)
             int last[NT][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n) last[n][0] = last[n][1] = a.prefix - 1;
-            t.step(qf, ks, vs, i * kStepKeys, last, a.prefix - 1, a.sl2, a.slack, lane);
+            t.step(qf, ks, vs, i * kStepKeys, last, a.prefix - 1, a.prefix - 1, a.sl2, a.slack, lane);
         } else {
             const int kb = (i - shared_steps) * kStepKeys;
             zero_behind<D>(vs, own - kb, lane);
-            t.step(qf, ks, vs, kb, limit, own - tokens, a.sl2, a.slack, lane);
+            t.step(qf, ks, vs, kb, limit, own - tokens, own - 1, a.sl2, a.slack, lane);
         }
         if (++stage == kStages) stage = 0, phase ^= 1u;
     }
@@ -740,32 +796,34 @@ Plan plan_of(const nb200_prefix_attn_args& a) {
     return p;
 }
 
-SharedLimit g_shared[28];
+constexpr int kVariants = 7;  // of a type, a head dimension, and one or several new tokens
+SharedLimit g_shared[8 * kVariants];
 
 struct Maps {
     CUtensorMap shared_k, shared_v, own_k, own_v;
 };
 
-template <typename T, int D, int NT>
+template <typename T, int D, int NT, bool SEVERAL>
 int launch_stream(const Maps& m, const StreamArgs& a, int64_t ctas, SharedLimit& limit, cudaStream_t st) {
     constexpr uint32_t bytes = kWarps * kStages * 2 * kStepKeys * D * 2 + 1024;  // + alignment slack
-    if (const int rc = limit.raise("nb200_prefix_attention", stream_kernel<T, D, NT>, bytes)) return rc;
-    launch_pdl(stream_kernel<T, D, NT>, (unsigned)ctas, kWarps * 32, bytes, st, m.shared_k, m.shared_v, m.own_k, m.own_v, a);
+    if (const int rc = limit.raise("nb200_prefix_attention", stream_kernel<T, D, NT, SEVERAL>, bytes)) return rc;
+    launch_pdl(stream_kernel<T, D, NT, SEVERAL>, (unsigned)ctas, kWarps * 32, bytes, st, m.shared_k, m.shared_v, m.own_k,
+               m.own_v, a);
     count_launch();
     return finish_launch("nb200_prefix_attention");
 }
 
-template <typename T, int D, int NT, int W>
+template <typename T, int D, int NT, int W, bool SEVERAL>
 int launch_solo(const Maps& m, const StreamArgs& a, void* o, float* lse, SharedLimit& limit, cudaStream_t st) {
     constexpr uint32_t bytes = W * kStages * 2 * kStepKeys * D * 2 + 1024;  // + alignment slack
-    if (const int rc = limit.raise("nb200_prefix_attention", solo_kernel<T, D, NT, W>, bytes)) return rc;
-    launch_pdl(solo_kernel<T, D, NT, W>, (unsigned)(a.batch * a.kv_heads), W * 32, bytes, st, m.shared_k, m.shared_v, m.own_k,
-               m.own_v, a, o, lse);
+    if (const int rc = limit.raise("nb200_prefix_attention", solo_kernel<T, D, NT, W, SEVERAL>, bytes)) return rc;
+    launch_pdl(solo_kernel<T, D, NT, W, SEVERAL>, (unsigned)(a.batch * a.kv_heads), W * 32, bytes, st, m.shared_k, m.shared_v,
+               m.own_k, m.own_v, a, o, lse);
     count_launch();
     return finish_launch("nb200_prefix_attention");
 }
 
-template <typename T, int D>
+template <typename T, int D, bool SEVERAL>
 int launch_all(const nb200_prefix_attn_args& n, const nb200_attn_strides* s, const void* q, const void* pk,
                const void* pv, const void* k, const void* v, void* o, float* lse, char* work, SharedLimit* limits,
                cudaStream_t st) {
@@ -805,16 +863,16 @@ int launch_all(const nb200_prefix_attn_args& n, const nb200_attn_strides* s, con
         // Where there are more CTAs than SMs, two an SM: one starts while the other reads. Head dimension 128 has room for
         // them with four warps each.
         if (D == 128 && a.batch * (int64_t)a.kv_heads > sm_count())
-            return p.nt == 1 ? launch_solo<T, D, 1, 4>(maps, a, o, lse, limits[3], st)
-                             : launch_solo<T, D, 2, 4>(maps, a, o, lse, limits[4], st);
-        return p.nt == 1 ? launch_solo<T, D, 1, 8>(maps, a, o, lse, limits[5], st)
-                         : launch_solo<T, D, 2, 8>(maps, a, o, lse, limits[6], st);
+            return p.nt == 1 ? launch_solo<T, D, 1, 4, SEVERAL>(maps, a, o, lse, limits[3], st)
+                             : launch_solo<T, D, 2, 4, SEVERAL>(maps, a, o, lse, limits[4], st);
+        return p.nt == 1 ? launch_solo<T, D, 1, 8, SEVERAL>(maps, a, o, lse, limits[5], st)
+                         : launch_solo<T, D, 2, 8, SEVERAL>(maps, a, o, lse, limits[6], st);
     }
     a.o = at(p.o), a.ml = pairs_at(p.ml), a.span = reinterpret_cast<int2*>(at(p.span));
     a.beside = p.splits > 0;  // the tensor cores' kernel started after all that came before
-    rc = p.nt == 1   ? launch_stream<T, D, 1>(maps, a, p.ctas, limits[0], st)
-         : p.nt == 2 ? launch_stream<T, D, 2>(maps, a, p.ctas, limits[1], st)
-                     : launch_stream<T, D, 4>(maps, a, p.ctas, limits[2], st);
+    rc = p.nt == 1   ? launch_stream<T, D, 1, SEVERAL>(maps, a, p.ctas, limits[0], st)
+         : p.nt == 2 ? launch_stream<T, D, 2, SEVERAL>(maps, a, p.ctas, limits[1], st)
+                     : launch_stream<T, D, 4, SEVERAL>(maps, a, p.ctas, limits[2], st);
     if (rc) return rc;
     JoinArgs j = {};
     j.tensor_o = at(p.tensor_o), j.tensor_ml = pairs_at(p.tensor_ml), j.o = a.o, j.ml = a.ml, j.span = a.span;
@@ -867,12 +925,18 @@ int launch_prefix_attention(const nb200_prefix_attn_args& n, const nb200_attn_st
                             const void* pv, const void* k, const void* v, void* o, float* lse, void* work,
                             cudaStream_t st) {
     char* w = static_cast<char*>(work);
-    if (n.dtype == NB200_BF16)
-        return n.head_dim == 128
-                   ? launch_all<__nv_bfloat16, 128>(n, s, q, pk, pv, k, v, o, lse, w, g_shared, st)
-                   : launch_all<__nv_bfloat16, 64>(n, s, q, pk, pv, k, v, o, lse, w, g_shared + 7, st);
-    return n.head_dim == 128 ? launch_all<__half, 128>(n, s, q, pk, pv, k, v, o, lse, w, g_shared + 14, st)
-                             : launch_all<__half, 64>(n, s, q, pk, pv, k, v, o, lse, w, g_shared + 21, st);
+    const int variant = (n.dtype == NB200_BF16 ? 0 : 4) + (n.head_dim == 128 ? 0 : 2) + (n.tokens > 1);
+    auto launch = [&](auto kernels) { return kernels(n, s, q, pk, pv, k, v, o, lse, w, g_shared + variant * kVariants, st); };
+    switch (variant) {
+        case 0: return launch(launch_all<__nv_bfloat16, 128, false>);
+        case 1: return launch(launch_all<__nv_bfloat16, 128, true>);
+        case 2: return launch(launch_all<__nv_bfloat16, 64, false>);
+        case 3: return launch(launch_all<__nv_bfloat16, 64, true>);
+        case 4: return launch(launch_all<__half, 128, false>);
+        case 5: return launch(launch_all<__half, 128, true>);
+        case 6: return launch(launch_all<__half, 64, false>);
+        default: return launch(launch_all<__half, 64, true>);
+    }
 }
 
 }  // namespace nb200
