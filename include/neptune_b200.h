@@ -384,11 +384,12 @@ int nb200_distill_loss_bwd(const nb200_distill_args* args, const float* grad, in
  * seq_lens (nullable, device memory: every sequence fills its cache): own tokens of each sequence, the new
  * ones included, read as clamped to [0, cache]. Query t stands at own position seq_lens[b] - tokens + t;
  * one before its sequence's first token (a free slot) has a zero row of o and an lse of -inf, as has a row
- * whose every score is -inf. What the caches hold at or past seq_lens does not matter. dtype NB200_BF16 or
+ * whose every score is -inf. What the caches hold at or past seq_lens does not matter, nor
+ * what a later new token holds to an earlier one. dtype NB200_BF16 or
  * NB200_F16 for all tensors; probabilities are rounded to it for the product with V, all sums are fp32.
  * head_dim 64 or 128 (else NB200_ERR_UNSUPPORTED); heads a multiple of kv_heads; bases and strides as for
- * nb200_attention_fwd. prefix or cache may be 0. work: device memory, 16-byte aligned, of
- * nb200_prefix_attention_work_bytes(args) bytes. The result does not depend on scheduling. No counterpart in
+ * nb200_attention_fwd. prefix or cache may be 0. o, lse and work share no memory with the inputs. work: device memory,
+ * 16-byte aligned, of nb200_prefix_attention_work_bytes(args) bytes. The result does not depend on scheduling. No counterpart in
  * the reference; the merge of partial results is its split plan's (neptune_codegen/algebra.py:348-403). */
 typedef struct {
     int64_t batch, heads, kv_heads, tokens, head_dim, prefix, cache;
@@ -409,7 +410,7 @@ int nb200_prefix_attention(const nb200_prefix_attn_args* args, const nb200_attn_
  * rounded to dtype, h is taken from the unrounded y. A NaN in a row makes its scales NaN and its bytes NaN (0 in
  * int8). x and residual are [rows, width] with unit column stride, weight contiguous [width], all of one dtype; q, y
  * and scale ([rows] or [rows, width / group], fp32) are contiguous. Pointers need their elements' alignment only
- * (rows that all start on 16-byte boundaries move faster). group is 0, 16, 32, 64 or 128 and divides width;
+ * (rows that all start on 16-byte boundaries move faster); q, scale and y share no memory with the inputs. group is 0, 16, 32, 64 or 128 and divides width;
  * width <= 16384 (else NB200_ERR_CAPACITY). The norm is the reference's (neptune_codegen/emitters.py:549-627)
  * without its intermediate rounding; the reference has no 8-bit output. */
 typedef enum { NB200_E4M3 = 0, NB200_E5M2 = 1, NB200_I8 = 2 } nb200_byte_kind;

@@ -17,8 +17,8 @@
 // Three kernels: tensor_part_kernel (prefix_attention_tc.cu) for a prefix with many query rows; stream_kernel
 // for the caches, and for a prefix with few rows, where the bound is the keys' bytes; join_kernel. Few keys for few
 // sequences take one, solo_kernel. bf16, 32 heads on 8 of
-// 128: 256 sequences behind 16384 keys with uneven caches up to 512 take 118 us a call (bytes 53, the prefix's products
-// 43), 4 behind 131072 keys 98 us, 5.5 TB/s.
+// 128: 256 sequences behind 16384 keys with uneven caches up to 512 take 117 us a call (bytes 53, the prefix's products
+// 43), 4 behind 131072 keys 96 us, 5.6 TB/s.
 #include <algorithm>
 
 #include "attn.cuh"

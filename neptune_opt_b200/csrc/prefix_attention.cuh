@@ -20,7 +20,10 @@ struct Query {
     int group, tokens;   // query heads per key/value head, new tokens per sequence
 };  // row r = (b group + g) tokens + t of key/value head `head` is q[b, head group + g, t]
 
-// Probabilities are rounded to the inputs' type for the product with the values. They are at most 2^8 (the
+// Probabilities are rounded to the inputs' type for the product with the values, whose two operands are of one type: half a
+// step of it beside the same half step of the values and of the result (bf16 2-norms of 0.0022 for 0.0017 with probabilities of
+// 32 bits; the sums that divide take them unrounded). What the rounding leaves off could go into a second product; on the
+// tensor cores the softmax, which bounds a tile there, would convert and store twice. They are at most 2^8 (the
 // running maximum may lag behind by that much), so fp16 has room for 2^6 more: that keeps the probabilities of very
 // many unlikely keys above fp16's smallest value.
 constexpr float kSlack = 8.f;

@@ -12,9 +12,11 @@ h // (heads // kv_heads). seq_lens [batch] int32 counts each sequence's own toke
 in k and v) included; without it every sequence fills its cache. Query t stands at own position
 seq_lens[b] - tokens + t and sees the prefix and the own tokens up to there. A query before its
 sequence's first token (a free slot of the batch) reads out as zero with a log-sum-exp of -inf, and so
-does a row whose every score is -inf. What the caches hold behind a sequence does not matter. prefix or
-cache may be 0: without a prefix this is attention against a cache. Any number of new tokens is right, but
-the caches' side is laid out for few: every 32 query rows read a sequence's cache once more.
+does a row whose every score is -inf. What the caches hold behind a sequence does not matter, nor what a
+later new token holds to an earlier one. Tensors whose rows the kernels' copies cannot read (an expanded
+batch, a base off the 16-byte boundary) are copied first, in every call. prefix or cache may be 0: without a
+prefix this is attention against a cache. Any number of new tokens is right, but the caches' side is laid out
+for few: every 32 query rows read a sequence's cache once more.
 
 The prefix is read once for the queries of all sequences, and every key range is split as far as the GPU
 has room; the partial results are merged as the split plan merges its states (the reference's merge
