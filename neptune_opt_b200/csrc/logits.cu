@@ -295,7 +295,7 @@ struct Divisor {
         const float q = x * inv;
         if constexpr (sizeof(T) != 4) return q;
         const float exact = fmaf(fmaf(-q, d, x), inv, q);
-        return fabsf(q) < NB200_INF ? exact : q;  // of an infinity the remainder is NaN
+        return exact == exact ? exact : q;  // beside an infinite x, q or d the remainder is NaN
     }
 };
 

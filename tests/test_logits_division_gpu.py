@@ -98,3 +98,21 @@ def test_temperatures_at_the_ends_of_fp32(dtype, t):
     assert torch.equal(torch.sign(got[:, :1]), torch.zeros_like(got[:, :1])) and bool((got * x >= 0)[x.abs() < math.inf].all())
     if t > 2.0 ** -128:
         check(got, want, 2.0 ** -20)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+def test_an_infinite_divisor_leaves_nothing(dtype):
+    """x / inf is 0 for every number x, by temperature and by repetition penalty."""
+    import torch
+
+    import neptune_opt_b200 as NB
+
+    x, gen = logits(3, 5003, getattr(torch, dtype), 3)
+    endless = torch.full((3,), math.inf, device="cuda")
+    assert not bool(NB.penalize_logits(x, temperature=endless).any())
+    for history in (40, 9000):
+        tokens = torch.randint(0, 5003, (3, history), device="cuda", generator=gen)
+        seen = torch.zeros(3, 5003, dtype=torch.bool, device="cuda").scatter_(1, tokens, True)
+        got = NB.penalize_logits(x, tokens, repetition=endless)
+        want = torch.where(seen, torch.where(x > 0, 0.0, x.float() * math.inf), x.float()).to(x.dtype)
+        assert torch.equal(got.nan_to_num(nan=-7.0), want.nan_to_num(nan=-7.0))
