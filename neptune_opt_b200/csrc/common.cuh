@@ -34,15 +34,15 @@ int finish_launch(const char* what);  // checks cudaGetLastError, returns nb200_
 // order. pdl_trigger() allows the next PDL kernel to be scheduled; it can start only after every
 // CTA of this grid has triggered or exited, so a grid never waits on a dependent for resources.
 //
-// The second kernel of one call may do more before it waits, where every CTA of the call's first kernel triggers behind its own
-// pdl_wait(): the second one then starts after all work ahead of the call has completed and its results have been flushed to
-// global memory, so only what the first kernel touches is still to be waited for. Until then the second one may write memory
-// that the first one neither reads nor writes, and read what was written before the call: by TMA or ld_early, past L1, which
-// no wait has made current, or behind fence_early, of device scope, which makes L1 drop what it holds. These are stream_kernel behind
-// tensor_part_kernel, and join_kernel's lengths (prefix_attention.cu; if stream_kernel waited first, 256 sequences behind 16384
-// keys would take 150 us for 96). Each still waits before it ends, or one CTA for all, so that a kernel behind it that waits
-// for it has waited for both. (attn_bwd_kernel, too, waits for its statistics alone; the kernel ahead of it is launched in
-// plain stream order, which begins with every cache current.)
+// The second kernel of one call may do more before it waits, where every CTA of the call's first kernel triggers behind its
+// own pdl_wait(): the second one then starts after all work ahead of the call has completed and its results have been flushed
+// to global memory, so only what the first kernel touches is still to be waited for. Until then the second one may write
+// memory that the first one neither reads nor writes, and read what was written before the call: by TMA or ld_early, past L1,
+// which no wait has made current, or behind fence_early, of device scope, which makes L1 drop what it holds. These are
+// stream_kernel behind tensor_part_kernel, and join_kernel's lengths (prefix_attention.cu; if stream_kernel waited first, 256
+// sequences behind 16384 keys would take 150 us for 96). Each still waits before it ends, or one CTA for all, so that a kernel
+// behind it that waits for it has waited for both. (attn_bwd_kernel, too, waits for its statistics alone; the kernel ahead of
+// it is launched in plain stream order, which begins with every cache current.)
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

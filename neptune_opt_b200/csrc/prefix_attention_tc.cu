@@ -215,9 +215,9 @@ __device__ __forceinline__ void mma_issuer(uint8_t* smem, Bars* b, uint32_t tmem
     drain_bar(&b->o_final, 0);
 }
 
-// While |m sl2| is at most kFar the exponent takes one multiply-add here, 2^(s sl2 - m sl2), of which the rounding of m sl2 takes 2^-16 at
-// most; a warp with a row that is farther from 0 subtracts first. (Subtracting always spills, and takes 80 us for 77 over 16384
-// keys and 1024 rows a head.)
+// While |m sl2| is at most kFar the exponent takes one multiply-add here, 2^(s sl2 - m sl2), from which the rounding of m sl2
+// takes 2^-16 at most; a warp with a row that is farther from 0 subtracts first. (Subtracting always spills, and takes 80 us
+// for 77 over 16384 keys and 1024 rows a head.)
 constexpr float kFar = 256.f;
 __device__ __forceinline__ bool is_far(float m, float sl2) { return m != -NB200_INF && fabsf(m * sl2) > kFar; }
 
